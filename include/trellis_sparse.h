@@ -440,6 +440,64 @@ int tsp_c2s_part(const float* d_x, int64_t n, int cin, const int32_t* d_nbr, con
                  void* d_workspace, size_t workspace_bytes, int flags, int part, int64_t t0, int64_t nt,
                  void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Pieces of a transformer block over packed voxel rows (no counterpart in the reference's sparse
+ * path; for models that put attention over the same rows that the convs and linears here work on):
+ * group norm, rotary positions on several axes, attention. Samples are packed: rows of sample s are
+ * [offsets[s], offsets[s + 1]) of device int32 offsets [samples + 1], non-decreasing and within
+ * [0, n] (bounds that are not are cut to it). Rows outside every sample are left as they were. NULL
+ * offsets mean one sample of all rows. Nothing is allocated; everything runs in stream order and may
+ * be captured into a graph. Calls that may overlap need workspaces of their own.
+ * ------------------------------------------------------------------------------------- */
+
+/* Group norm, channels last: out[i][c] = act((x[i][c] - mean) / sqrt(var + eps) * gamma[c] + beta[c])
+ * with the mean and the biased variance of the c / groups channels of c's group over all rows of i's
+ * sample, in fp32; act is x * sigmoid(x) when silu != 0. gamma and beta f32 [c] or NULL. Any dtypes;
+ * d_out may equal d_x where they are the same. At most 4096 groups. The workspace, 8-byte aligned,
+ * holds tsp_group_norm_workspace_bytes bytes; the result does not depend on what it held, nor on the
+ * order in which workgroups run. */
+size_t tsp_group_norm_workspace_bytes(int64_t n, int c, int groups, int samples);
+int tsp_group_norm(const void* d_x, int x_dtype, int64_t n, int c, int groups, const int32_t* d_offsets,
+                   int samples, const float* d_gamma, const float* d_beta, float eps, int silu, void* d_out,
+                   int out_dtype, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* Rows of heads: element e of head h of row i is data[i * row_stride + h * head_stride + e] (a view into
+ * the output of one linear for q, k and v, for instance). */
+typedef struct {
+    void* data;
+    int64_t row_stride, head_stride;   /* in elements */
+} tsp_heads;
+
+/* Rotary positions on several axes. Row i stands at d_pos[i][0 .. axes-1] (int32, any value); pair j of
+ * axis a is turned by the angle pos[i][a] * theta^(-j / pairs[a]): (u, v) becomes
+ * (u cos - v sin, v cos + u sin). The d / 2 pairs of a head are elements (2p, 2p + 1), or with
+ * TSP_ROPE_HALVES (p, p + d/2); axis 0's pairs[0] pairs come first, then axis 1's, and pairs after the
+ * last axis's stay as they are. Angles are exact to 2^-23 at any position. q and k (hk heads; NULL and 0
+ * without) are turned in one launch. With gamma (f32 [heads][d], or NULL), a head's row is
+ * RMS-normalised first: x / sqrt(mean(x^2) + eps) * gamma. 1 to 4 axes; d a multiple of 8 up to 256.
+ * Any dtypes; an output may be its own input where they are the same dtype and strides, and must not
+ * overlap the inputs otherwise. */
+enum { TSP_ROPE_HALVES = 1 };
+int tsp_rope_axes(const tsp_heads* q, int hq, const tsp_heads* k, int hk, int dtype, int64_t n, int d,
+                  const int32_t* d_pos, int axes, const int* pairs, double theta, int flags,
+                  const float* d_q_gamma, const float* d_k_gamma, float eps, const tsp_heads* q_out,
+                  const tsp_heads* k_out, int out_dtype, void* stream);
+
+/* Softmax attention within packed samples: out[i][h] = sum_j p_j v[j][h'] with p = softmax_j(scale *
+ * q[i][h] . k[j][h']), h' = h / (hq / hkv), over the keys of i's sample: all Lk of them, or with causal
+ * != 0 those with j <= i + (Lk - Lq), i and j counted within the sample (the last query sees every key: a
+ * prompt, or new tokens after a cache). q_offsets and k_offsets give the samples' rows in q and in k and
+ * v. A row that sees no key gets zeros; a key that a row does not see has no effect on it, whatever it
+ * holds. f16 or bf16 (out of the same type), d a multiple of 8 up to 128, hq % hkv == 0, scale > 0; data
+ * 16-byte aligned, strides multiples of 8. out must not overlap the inputs. Where there are few queries
+ * the keys are split over the device and the parts joined in the workspace, 16-byte aligned, of
+ * tsp_attention_workspace_bytes bytes (0, and NULL will do, where they are not). */
+size_t tsp_attention_workspace_bytes(int64_t nq, int64_t nk, int samples, int hq, int hkv, int d);
+int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_heads* v, int dtype, int64_t nq, int64_t nk,
+                  int hq, int hkv, int d, const int32_t* d_q_offsets, const int32_t* d_k_offsets, int samples,
+                  float scale, int causal, const tsp_heads* out, void* d_workspace, size_t workspace_bytes,
+                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif

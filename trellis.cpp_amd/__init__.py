@@ -35,6 +35,7 @@ EXPORTS = (
     "tsp_mask_positive",
     "tsp_convnext_workspace_bytes", "tsp_convnext", "tsp_convnext_ex", "tsp_c2s_workspace_bytes", "tsp_c2s",
     "tsp_c2s_ex", "tsp_c2s_part",
+    "tsp_group_norm_workspace_bytes", "tsp_group_norm", "tsp_rope_axes", "tsp_attention_workspace_bytes", "tsp_attention",
 )
 
 BLOCK_CAST_F32 = 2
@@ -55,6 +56,11 @@ class C2SWeights(ctypes.Structure):
                 ("conv1_weight", ctypes.c_void_p), ("conv1_dtype", ctypes.c_int), ("conv1_bias", ctypes.c_void_p),
                 ("conv1_packed", ctypes.c_void_p), ("conv2_weight", ctypes.c_void_p), ("conv2_dtype", ctypes.c_int),
                 ("conv2_bias", ctypes.c_void_p), ("conv2_packed", ctypes.c_void_p)]
+
+
+class Heads(ctypes.Structure):
+    """tsp_heads: rows of heads, strides in elements."""
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
 
 
 class TspError(RuntimeError):
@@ -171,6 +177,20 @@ def lib() -> ctypes.CDLL:
     L.tsp_c2s_part.restype = c_int
     L.tsp_c2s_part.argtypes = [c_vp, c_i64, c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_int, c_vp, c_vp, c2w,
                                c_vp, c_vp, c_int, c_vp, c_sz, c_int, c_int, c_i64, c_i64, c_vp]
+    c_f, hp = ctypes.c_float, ctypes.POINTER(Heads)
+    L.tsp_group_norm_workspace_bytes.restype = c_sz
+    L.tsp_group_norm_workspace_bytes.argtypes = [c_i64, c_int, c_int, c_int]
+    L.tsp_group_norm.restype = c_int
+    L.tsp_group_norm.argtypes = [c_vp, c_int, c_i64, c_int, c_int, c_vp, c_int, c_vp, c_vp, c_f, c_int, c_vp, c_int, c_vp,
+                                 c_sz, c_vp]
+    L.tsp_rope_axes.restype = c_int
+    L.tsp_rope_axes.argtypes = [hp, c_int, hp, c_int, c_int, c_i64, c_int, c_vp, c_int, ctypes.POINTER(c_int),
+                                ctypes.c_double, c_int, c_vp, c_vp, c_f, hp, hp, c_int, c_vp]
+    L.tsp_attention_workspace_bytes.restype = c_sz
+    L.tsp_attention_workspace_bytes.argtypes = [c_i64, c_i64, c_int, c_int, c_int, c_int]
+    L.tsp_attention.restype = c_int
+    L.tsp_attention.argtypes = [hp, hp, hp, c_int, c_i64, c_i64, c_int, c_int, c_int, c_vp, c_vp, c_int, c_f, c_int, hp,
+                                c_vp, c_sz, c_vp]
     _lib = L
     return L
 
@@ -783,3 +803,228 @@ def c2s(x, nbr, mask, mstart, gidx, m: int, cout: int, child_nbr, p: dict, plan=
         for t0, nt in conv2_tiles:
             _check("tsp_c2s_part", lib().tsp_c2s_part(*args, 2, t0, nt, _stream(stream)))
     return out if out16 is None else (out, out16)
+
+
+# --------------------------------------------------------------------------------------------
+# transformer pieces over packed rows
+# --------------------------------------------------------------------------------------------
+class _On:
+    """Runs a call on its tensors' device and on the given stream: what it allocates there belongs to
+    that stream, and its tensors are kept from reuse until the stream is past the call."""
+
+    def __init__(self, device, stream):
+        torch = _torch()
+        self.device, self.current, self.guards = device, torch.cuda.current_stream(device), []
+        if stream is not None and stream.device != device:
+            raise ValueError(f"stream is on {stream.device}, the tensors on {device}")
+        self.stream = stream if stream is not None else self.current
+        self.other = self.stream != self.current
+
+    def __enter__(self):
+        torch = _torch()
+        if self.device.index != torch.cuda.current_device():
+            self.guards.append(torch.cuda.device(self.device))
+        if self.other:
+            self.guards.append(torch.cuda.stream(self.stream))
+        for g in self.guards:
+            g.__enter__()
+        return self
+
+    def __exit__(self, *exc):
+        for g in reversed(self.guards):
+            g.__exit__(*exc)
+
+    def keep(self, *tensors):
+        if self.other:
+            for t in tensors:
+                if t is not None:
+                    t.record_stream(self.stream)
+                    t.record_stream(self.current)
+
+    @property
+    def ptr(self):
+        return ctypes.c_void_p(self.stream.cuda_stream)
+
+
+def _same_device(device, **ts):
+    if device.type != "cuda":
+        raise ValueError("tensors must live on the GPU")
+    for name, t in ts.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} must live on {device}, got {t.device}")
+
+
+def _offsets(t, name: str):
+    """(offsets, samples) of packed rows; None: one sample."""
+    if t is None:
+        return None, 1
+    if t.dtype != _torch().int32 or t.dim() != 1 or t.numel() < 2 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 vector of samples + 1 entries")
+    return t, t.numel() - 1
+
+
+def _workspace_ok(ws, need: int, name: str):
+    if ws.dtype != _torch().uint8 or ws.numel() < need or not ws.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous uint8 buffer of {name} ({need}) bytes")
+
+
+def group_norm_workspace(n: int, c: int, groups: int, samples: int = 1, device="cuda"):
+    """The uint8 workspace group_norm needs for these sizes."""
+    return _torch().empty(max(lib().tsp_group_norm_workspace_bytes(n, c, groups, samples), 16), dtype=_torch().uint8,
+                          device=device)
+
+
+def group_norm(x, groups: int, gamma=None, beta=None, eps: float = 1e-6, silu: bool = False, offsets=None, out_dtype=None,
+               out=None, workspace=None, stream=None):
+    """Group norm over packed samples, channels last: x [N, C], each sample's rows and a group's
+    C / groups channels normalised together (biased variance) [* gamma + beta] [then SiLU]. offsets int32
+    [samples + 1] on the GPU: the samples' first rows and the last one's end (None: one sample); rows
+    outside every sample are left as they were in out. out [N, C] may be x; workspace
+    (group_norm_workspace) may be given to reuse it."""
+    torch = _torch()
+    if x.dim() != 2 or groups < 1 or x.shape[1] % groups:
+        raise ValueError(f"x must be [N, C] with C a multiple of groups={groups}, got {tuple(x.shape)}")
+    n, c = x.shape
+    dev = x.device
+    offsets, samples = _offsets(offsets, "offsets")
+    for name, t in (("gamma", gamma), ("beta", beta)):
+        if t is not None and (t.dtype != torch.float32 or t.numel() != c or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous float32 vector of {c}")
+    if out is not None:
+        _check_out(out, n, c, out_dtype or out.dtype, dev)
+    _same_device(dev, offsets=offsets, gamma=gamma, beta=beta, workspace=workspace)
+    xd = dtype_code(x.dtype)
+    need = lib().tsp_group_norm_workspace_bytes(n, c, groups, samples)
+    if workspace is not None:
+        _workspace_ok(workspace, need, "tsp_group_norm_workspace_bytes")
+    with _On(dev, stream) as on:
+        xc = x.contiguous()
+        if out is None:
+            out = torch.empty((n, c), dtype=out_dtype or x.dtype, device=dev)
+        ws = workspace if workspace is not None else torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        on.keep(x, xc, gamma, beta, offsets, out, ws)
+        _check("tsp_group_norm",
+               lib().tsp_group_norm(_ptr(xc), xd, n, c, groups, _ptr(offsets), samples, _ptr(gamma), _ptr(beta), eps,
+                                    1 if silu else 0, _ptr(out), dtype_code(out.dtype), _ptr(ws), ws.numel(), on.ptr))
+    return out
+
+
+def _heads_fit(t) -> bool:
+    """Whether the kernels can read t [N, H, D] where it lies."""
+    n, h, d = t.shape
+    return ((d == 1 or t.stride(2) == 1) and t.data_ptr() % 16 == 0 and (n <= 1 or (t.stride(0) % 8 == 0 and t.stride(0) <= 1 << 20))
+            and (h <= 1 or t.stride(1) % 8 == 0))
+
+
+def _fitted(t):
+    """t where it lies if the kernels can read it there, else a copy that they can."""
+    return t if _heads_fit(t) else t.clone(memory_format=_torch().contiguous_format)
+
+
+def _heads(t) -> Heads:
+    n, h, d = t.shape
+    head = t.stride(1) if h > 1 else d
+    return Heads(t.data_ptr(), t.stride(0) if n > 1 else h * d, head)
+
+
+def _check_heads_out(out, like, dtype, name: str):
+    if tuple(out.shape) != tuple(like.shape) or out.dtype != dtype or out.device != like.device:
+        raise ValueError(f"{name} must be {dtype} {list(like.shape)} on {like.device}")
+    if not _heads_fit(out):
+        raise ValueError(f"{name} must be 16-byte aligned with contiguous heads and strides that are multiples of 8")
+
+
+def rope_axes(q, pos, k=None, pairs=None, theta: float = 10000.0, interleaved: bool = True, q_gamma=None, k_gamma=None,
+              eps: float = 1e-6, out_dtype=None, q_out=None, k_out=None, stream=None):
+    """Rotary positions on several axes: q [N, Hq, D] (and k [N, Hk, D] in the same launch) turned by
+    pos int32 [N, axes]. Pair j of axis a turns by pos[:, a] * theta ** (-j / pairs[a]); pairs defaults to
+    D // 2 // axes on every axis, and a head's pairs after the last axis's stay as they are. Pairs are
+    neighbours (2p, 2p + 1), or with interleaved=False (p, p + D/2). q_gamma [Hq, D] and k_gamma [Hk, D]
+    (float32): every head is RMS-normalised first, x / sqrt(mean(x^2) + eps) * gamma. -> q's result, or the
+    pair with k. Heads may be strided views; q_out and k_out may be q and k themselves."""
+    torch = _torch()
+    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
+        raise ValueError("q must be [N, Hq, D] and k [N, Hk, D]")
+    n, hq, d = q.shape
+    dev = q.device
+    if k is not None and k.dtype != q.dtype:
+        raise ValueError("q and k must have one dtype")
+    if k is None and (k_gamma is not None or k_out is not None):
+        raise ValueError("k_gamma and k_out need k")
+    if pos.dtype != torch.int32 or pos.dim() != 2 or pos.shape[0] != n or not 1 <= pos.shape[1] <= 4:
+        raise ValueError("pos must be int32 [N, axes] with 1 to 4 axes")
+    axes = pos.shape[1]
+    pairs = [d // 2 // axes] * axes if pairs is None else [int(p) for p in pairs]
+    if len(pairs) != axes:
+        raise ValueError(f"pairs must name a count for each of {axes} axes")
+    for name, g, t in (("q_gamma", q_gamma, q), ("k_gamma", k_gamma, k)):
+        if g is not None and (g.dtype != torch.float32 or tuple(g.shape) != tuple(t.shape[1:]) or not g.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous float32 {list(t.shape[1:])}")
+    _same_device(dev, k=k, pos=pos, q_gamma=q_gamma, k_gamma=k_gamma)
+    odt = out_dtype or (q_out.dtype if q_out is not None else k_out.dtype if k_out is not None else q.dtype)
+    for name, o, t in (("q_out", q_out, q), ("k_out", k_out, k)):
+        if o is not None:
+            _check_heads_out(o, t, odt, name)
+    with _On(dev, stream) as on:
+        qc = _fitted(q)
+        kc = None if k is None else _fitted(k)
+        pc = pos.contiguous()
+        if q_out is None:
+            q_out = torch.empty((n, hq, d), dtype=odt, device=dev)
+        if k is not None and k_out is None:
+            k_out = torch.empty(tuple(k.shape), dtype=odt, device=dev)
+        on.keep(q, k, qc, kc, pos, pc, q_gamma, k_gamma, q_out, k_out)
+        kh = None if k is None else ctypes.byref(_heads(kc))
+        koh = None if k is None else ctypes.byref(_heads(k_out))
+        _check("tsp_rope_axes",
+               lib().tsp_rope_axes(ctypes.byref(_heads(qc)), hq, kh, 0 if k is None else k.shape[1], dtype_code(q.dtype), n, d,
+                                   _ptr(pc), axes, (ctypes.c_int * axes)(*pairs), theta, 0 if interleaved else 1, _ptr(q_gamma),
+                                   _ptr(k_gamma), eps, ctypes.byref(_heads(q_out)), koh, dtype_code(odt), on.ptr))
+    return q_out if k is None else (q_out, k_out)
+
+
+def attention_workspace(nq: int, nk: int, samples: int, hq: int, hkv: int, d: int, device="cuda"):
+    """The uint8 workspace attention needs for these sizes."""
+    return _torch().empty(max(lib().tsp_attention_workspace_bytes(nq, nk, samples, hq, hkv, d), 16), dtype=_torch().uint8,
+                          device=device)
+
+
+def attention(q, k, v, q_offsets=None, k_offsets=None, causal: bool = False, scale=None, out=None, workspace=None, stream=None):
+    """Softmax attention within packed samples: q [Nq, Hq, D], k and v [Nk, Hkv, D] (f16 or bf16, D a
+    multiple of 8 up to 128, Hq a multiple of Hkv: head h of q reads head h // (Hq // Hkv)) -> [Nq, Hq, D].
+    Row i of a sample sees all of the sample's keys, or with causal the keys j <= i + (Lk - Lq); a row that
+    sees none gets zeros. q_offsets and k_offsets int32 [samples + 1] on the GPU: the samples' rows in q
+    and in k and v (None, both: one sample); rows of out outside every sample are left as they were. scale
+    defaults to D ** -0.5. Heads may be strided views; workspace (attention_workspace) may be given to
+    reuse it."""
+    torch = _torch()
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[2] != q.shape[2]:
+        raise ValueError("q must be [Nq, Hq, D], k and v [Nk, Hkv, D]")
+    (nq, hq, d), (nk, hkv, _) = q.shape, k.shape
+    dev = q.device
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must have one dtype")
+    if (q_offsets is None) != (k_offsets is None):
+        raise ValueError("q_offsets and k_offsets come together")
+    q_offsets, samples = _offsets(q_offsets, "q_offsets")
+    k_offsets, k_samples = _offsets(k_offsets, "k_offsets")
+    if samples != k_samples:
+        raise ValueError("q_offsets and k_offsets must name the same samples")
+    _same_device(dev, k=k, v=v, q_offsets=q_offsets, k_offsets=k_offsets, workspace=workspace)
+    if out is not None:
+        _check_heads_out(out, q, q.dtype, "out")
+    need = lib().tsp_attention_workspace_bytes(nq, nk, samples, hq, hkv, d)
+    if workspace is not None:
+        _workspace_ok(workspace, need, "tsp_attention_workspace_bytes")
+    with _On(dev, stream) as on:
+        qc, kc, vc = _fitted(q), _fitted(k), _fitted(v)
+        if out is None:
+            out = torch.empty((nq, hq, d), dtype=q.dtype, device=dev)
+        ws = workspace if workspace is not None or need == 0 else torch.empty(need, dtype=torch.uint8, device=dev)
+        on.keep(q, k, v, qc, kc, vc, q_offsets, k_offsets, out, ws)
+        _check("tsp_attention",
+               lib().tsp_attention(ctypes.byref(_heads(qc)), ctypes.byref(_heads(kc)), ctypes.byref(_heads(vc)),
+                                   dtype_code(q.dtype), nq, nk, hq, hkv, d, _ptr(q_offsets), _ptr(k_offsets), samples,
+                                   d ** -0.5 if scale is None else scale, 1 if causal else 0, ctypes.byref(_heads(out)),
+                                   _ptr(ws), 0 if ws is None else ws.numel(), on.ptr))
+    return out

@@ -1,0 +1,327 @@
+// Softmax attention within packed samples: for query row i of sample s and head h (on key head
+// h / (hq / hkv)),
+//   out[i][h] = sum_j exp(scale q_i . k_j - max) v_j / sum_j exp(scale q_i . k_j - max)
+// over the keys j that the row sees: all of its sample's, or with `causal` the first Lk - Lq + i + 1 of
+// them. A row that sees no key gets zeros.
+//
+// One pass over the keys with the running maximum and sum of each row. Both products run on the matrix
+// cores (v_mfma_f32_32x32x16) with their roles turned: S^T = K Q^T and O^T = V^T P^T. A lane then holds
+// 16 of a tile's 32 scores of ONE query row (lane % 32; the other lane half holds the others), so a row's
+// maximum and sum need no more than one exchange between the halves, and the probabilities are, after
+// their rounding to 16 bits, the second product's operand where they stand: an operand lane wants eight
+// keys, which eight does not matter as long as V's operand has the same, and V's lie in the order 4 of
+// every 8 that S^T leaves.
+//
+// The rows of a workgroup are (query, head of the group) pairs: the heads that share a key head read its
+// tiles once.
+//
+// Statistics and accumulators are fp32. P is rounded to the inputs' 16-bit type, as the matrix cores take
+// it (half a step, 2^-9 of a probability in bf16: below the rounding of the output).
+#include <algorithm>
+#include <cmath>
+
+#include "common.hpp"
+#include "packed.hpp"
+
+namespace tsp {
+namespace {
+
+constexpr int AT_KEYS = 64;                   // keys of a tile
+constexpr int AT_MAX_D = 128;
+
+struct AttnArgs {
+    const uint16_t *q, *k, *v;
+    uint16_t* o;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;   // strides in elements
+    const int32_t *q_off, *k_off;
+    int64_t nq, nk;
+    int samples, hkv, share, d, causal, units;
+    float scale2;                             // scale * log2(e)
+};
+
+template <bool BF16>
+__device__ __forceinline__ f32x16_t mfma32(const u32x4_t& a, const u32x4_t& b, const f32x16_t& c) {
+    if constexpr (BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// Two values rounded to nearest even into a packed pair.
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (BF16) return f32x2_to_bf16x2_bits(lo, hi);
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{lo, hi}, f16x2_t));
+}
+
+// The value of the other lane half (lane ^ 32), for both halves: {lower half's, upper half's}.
+__device__ __forceinline__ float2 both_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return float2{__uint_as_float(r[0]), __uint_as_float(r[1])};
+}
+
+template <bool BF16>
+__device__ __forceinline__ bool nonfinite16(uint32_t b) {
+    constexpr uint32_t kExp = BF16 ? 0x7F80u : 0x7C00u;
+    return (b & kExp) == kExp;
+}
+
+// Byte offsets in a staged tile of AT_KEYS rows of DP values, as 16-byte pieces. K is read 16 bytes of
+// one d at 32 consecutive keys: the piece is xored with the key, so that 16 keys cover all banks. V is
+// read 64 bytes of 4 consecutive keys: the 64-byte quarter is xored with the key.
+template <int DP>
+__device__ __forceinline__ int k_piece(int key, int piece) {
+    constexpr int P = DP / 8;
+    return key * (DP * 2) + ((piece ^ (DP == 128 ? key & 15 : (key >> 1) & 7)) & (P - 1)) * 16;
+}
+template <int DP>
+__device__ __forceinline__ int v_piece(int key, int piece) {
+    return key * (DP * 2) + (piece ^ (DP == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2)) * 16;
+}
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4_ptr;
+
+// V^T operand (32 d x 16 keys) of keys 16 ks + {4h..4h+3, 8+4h..8+4h+3}: each of the two transposing
+// loads takes 4 keys x 16 d a group of 16 lanes.
+template <int DP>
+__device__ __forceinline__ u32x4_t v_operand(const char* sv, int ks, int db, int lane) {
+    const int key = ks * 16 + 4 * (lane >> 5) + ((lane >> 2) & 3);
+    const int piece = db * 4 + ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1), sub = (lane & 1) * 8;
+    const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(sv + v_piece<DP>(key, piece) + sub));
+    const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(sv + v_piece<DP>(key + 8, piece) + sub));
+    const uint2 ua = __builtin_bit_cast(uint2, a), ub = __builtin_bit_cast(uint2, b);
+    return u32x4_t{ua.x, ua.y, ub.x, ub.y};
+}
+
+// Keys of a tile that a row sees, for the rows of a wave's 32.
+struct RowLimits {
+    int lane, lo, hi;      // this lane's row, the wave's first and last
+};
+
+template <bool BF16, int DP, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
+    constexpr int KS = DP / 16, DB = DP / 32, P = DP / 8, NT = NW * 64, ROWS = NW * 32;
+    __shared__ __attribute__((aligned(16))) char sK[AT_KEYS * DP * 2];
+    __shared__ __attribute__((aligned(16))) char sV[AT_KEYS * DP * 2];
+    const int head = blockIdx.x / a.units, unit = blockIdx.x - head * a.units;
+    const PackedUnit u = packed_unit(a.q_off, a.samples, a.nq, a.share, ROWS, unit);
+    if (u.sample < 0) return;
+    int64_t krow0, krows;
+    packed_rows(a.k_off, u.sample, a.nk, krow0, krows);
+    const int lk = (int)krows;
+    const int64_t rows = u.rows * a.share;
+    const int64_t tile0 = (int64_t)(unit - u.first) * ROWS;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
+
+    // rows past the sample's last are copies of it that are not stored
+    auto limit = [&](int64_t r) -> int {
+        r = r < rows ? r : rows - 1;
+        if (!a.causal) return lk;
+        const int64_t n = krows - u.rows + r / a.share + 1;
+        return n < 0 ? 0 : n < krows ? (int)n : lk;
+    };
+    const int64_t r = tile0 + wave * 32 + r32, rc = r < rows ? r : rows - 1;
+    const RowLimits lim{limit(r), limit(tile0 + wave * 32), limit(tile0 + wave * 32 + 31)};
+    const int wg_end = limit(tile0 + ROWS - 1);
+    const int64_t qi = rc / a.share;
+    const int hq = head * a.share + (int)(rc - qi * a.share);
+
+    // Q^T operand: d = 16 ks + 8 h .. + 7 of the lane's row
+    u32x4_t qf[KS];
+    {
+        const uint16_t* qp = a.q + (u.row0 + qi) * a.q_row + hq * a.q_head;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+            qf[ks] = ks * 16 + h * 8 < a.d ? *reinterpret_cast<const u32x4_t*>(qp + ks * 16 + h * 8) : u32x4_t{0, 0, 0, 0};
+    }
+    const uint16_t* kp = a.k + krow0 * a.k_row + head * a.k_head;
+    const uint16_t* vp = a.v + krow0 * a.v_row + head * a.v_head;
+
+    f32x16_t o[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db) o[db] = f32x16_t{};
+    float m = -INFINITY, l = 0.f;
+
+    for (int base = 0; base < wg_end; base += AT_KEYS) {
+        __syncthreads();
+        for (int e = threadIdx.x; e < AT_KEYS * P; e += NT) {
+            const int key = e / P, piece = e % P;
+            u32x4_t x{0, 0, 0, 0}, y{0, 0, 0, 0};
+            if (base + key < lk && piece * 8 < a.d) {
+                x = *reinterpret_cast<const u32x4_t*>(kp + (int64_t)(base + key) * a.k_row + piece * 8);
+                y = *reinterpret_cast<const u32x4_t*>(vp + (int64_t)(base + key) * a.v_row + piece * 8);
+            }
+            *reinterpret_cast<u32x4_t*>(sK + k_piece<DP>(key, piece)) = x;
+            *reinterpret_cast<u32x4_t*>(sV + v_piece<DP>(key, piece)) = y;
+        }
+        __syncthreads();
+        if (base >= lim.hi) continue;
+
+        // scores: s[kb][i] is key kb * 32 + 8 (i / 4) + 4 h + i % 4 of the tile
+        f32x16_t s[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            s[kb] = f32x16_t{};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                s[kb] = mfma32<BF16>(*reinterpret_cast<const u32x4_t*>(sK + k_piece<DP>(kb * 32 + r32, ks * 2 + h)), qf[ks], s[kb]);
+        }
+        const bool masked = base + AT_KEYS > lim.lo;
+        if (masked) {
+            const int left = lim.lane - base - 4 * h;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[kb][i] = kb * 32 + 8 * (i / 4) + i % 4 < left ? s[kb][i] : -INFINITY;
+        }
+        float mt = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[kb][i]);
+        const float2 mh = both_halves(mt);
+        const float mn = fmaxf(m, fmaxf(mh.x, mh.y));
+        const float mz = mn == -INFINITY ? 0.f : mn;        // (no key seen yet, or scores of -inf alone)
+        const float corr = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mz) * a.scale2);
+        m = mn;
+        const float mc = mz * a.scale2;
+        float sum = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], a.scale2, -mc));
+                sum += s[kb][i];
+            }
+        l = l * corr + sum;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[db][i] *= corr;
+        u32x4_t pf[4];
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pf[ks][e] = pack2<BF16>(s[ks / 2][8 * (ks % 2) + 2 * e], s[ks / 2][8 * (ks % 2) + 2 * e + 1]);
+
+        // Rows of the tile that see different keys: a probability of zero must not meet an Inf or a NaN
+        // of a key that its row does not see. Zero times V shows whether there is one.
+        bool odd = false;
+        if (masked && a.causal) {
+            f32x16_t z = f32x16_t{};
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                for (int db = 0; db < DB; ++db) z = mfma32<BF16>(v_operand<DP>(sV, ks, db, lane), u32x4_t{0, 0, 0, 0}, z);
+            float t = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) t += z[i];
+            odd = __any(t != t);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int db = 0; db < DB; ++db) {
+                u32x4_t vf = v_operand<DP>(sV, ks, db, lane);
+                if (odd) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (nonfinite16<BF16>(vf[e])) vf[e] &= 0xffff0000u;
+                        if (nonfinite16<BF16>(vf[e] >> 16)) vf[e] &= 0xffffu;
+                    }
+                }
+                o[db] = mfma32<BF16>(vf, pf[ks], o[db]);
+            }
+        if (odd) {      // the values left out, key by key, for the rows that see them
+            for (int key = 0; key < AT_KEYS; ++key) {
+                float p = 0.f;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if ((kb * 32 + 8 * (i / 4) + i % 4) == (key & ~4)) p = s[kb][i];
+                const float2 ph = both_halves(p);
+                p = key & 4 ? ph.y : ph.x;
+                const bool sees = base + key < lim.lane;
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int e = db * 32 + 8 * (i / 4) + 4 * h + i % 4;
+                        const uint32_t b = *reinterpret_cast<const uint16_t*>(sV + v_piece<DP>(key, e >> 3) + (e & 7) * 2);
+                        if (sees && nonfinite16<BF16>(b)) o[db][i] += p * (BF16 ? bf16_bits_to_f32((uint16_t)b) : f16_bits_to_f32((uint16_t)b));
+                    }
+            }
+        }
+    }
+
+    const float2 lh = both_halves(l);
+    const float inv = 1.0f / (lh.x + lh.y);
+    if (r >= rows) return;
+    uint16_t* op = a.o + (u.row0 + qi) * a.o_row + hq * a.o_head;
+    const bool none = lim.lane == 0;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int e = db * 32 + 8 * g + 4 * h;
+            if (e < a.d)
+                *reinterpret_cast<uint2*>(op + e) = none ? uint2{0, 0} : uint2{pack2<BF16>(o[db][4 * g] * inv, o[db][4 * g + 1] * inv),
+                                                                              pack2<BF16>(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv)};
+        }
+}
+
+constexpr int AT_NW = 4;
+
+}  // namespace
+}  // namespace tsp
+
+using namespace tsp;
+
+extern "C" size_t tsp_attention_workspace_bytes(int64_t nq, int64_t nk, int samples, int hq, int hkv, int d) { return 0; }
+
+extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_heads* v, int dtype, int64_t nq, int64_t nk, int hq,
+                             int hkv, int d, const int32_t* d_q_offsets, const int32_t* d_k_offsets, int samples, float scale,
+                             int causal, const tsp_heads* out, void* d_workspace, size_t workspace_bytes, void* stream) {
+    clear_error();
+    TSP_REQUIRE(nq >= 0 && nq < (1ll << 31) && nk >= 0 && nk < (1ll << 31) - AT_KEYS, TSP_ERR_INVALID, "tsp_attention: nq=%lld nk=%lld out of range",
+                (long long)nq, (long long)nk);
+    TSP_REQUIRE(hq > 0 && hkv > 0 && hq % hkv == 0 && hq <= 4096, TSP_ERR_INVALID, "tsp_attention: %d heads on %d", hq, hkv);
+    TSP_REQUIRE(dtype_valid(dtype), TSP_ERR_INVALID, "tsp_attention: bad dtype");
+    TSP_REQUIRE(samples > 0 && (samples == 1 || (d_q_offsets && d_k_offsets)), TSP_ERR_INVALID,
+                "tsp_attention: samples=%d (without offsets: 1)", samples);
+    TSP_REQUIRE(std::isfinite(scale) && scale > 0.f, TSP_ERR_INVALID, "tsp_attention: scale=%g", scale);
+    TSP_REQUIRE(dtype != TSP_F32, TSP_ERR_UNSUPPORTED, "tsp_attention: f16 or bf16");
+    TSP_REQUIRE(d > 0 && d % 8 == 0 && d <= AT_MAX_D, TSP_ERR_UNSUPPORTED, "tsp_attention: heads of %d (need a multiple of 8 up to %d)",
+                d, AT_MAX_D);
+    if (nq == 0) return TSP_OK;
+    TSP_REQUIRE(q && out && q->data && out->data && (nk == 0 || (k && v && k->data && v->data)), TSP_ERR_INVALID,
+                "tsp_attention: null pointer");
+    const tsp_heads empty{nullptr, 0, 0};
+    const tsp_heads kk = nk ? *k : empty, vv = nk ? *v : empty;
+    TSP_REQUIRE(heads_aligned(*q) && heads_aligned(*out) && heads_aligned(kk) && heads_aligned(vv), TSP_ERR_INVALID,
+                "tsp_attention: data must be 16-byte aligned, strides multiples of 8 (a row's up to 2^20)");
+    TSP_REQUIRE(heads_apart(*out, nq, hq, d), TSP_ERR_INVALID, "tsp_attention: the output's heads overlap");
+    TSP_REQUIRE(out->data != kk.data && out->data != vv.data && out->data != q->data, TSP_ERR_INVALID, "tsp_attention: out must not alias q, k or v");
+    const int share = hq / hkv;
+    const int64_t units = ceil_div(nq * share, AT_NW * 32) + (samples > 1 ? samples : 0);
+    TSP_REQUIRE(units * hkv * AT_NW * 64 < (1ll << 32), TSP_ERR_INVALID, "tsp_attention: too many rows");
+    const AttnArgs a{static_cast<const uint16_t*>(q->data), static_cast<const uint16_t*>(kk.data), static_cast<const uint16_t*>(vv.data),
+                     static_cast<uint16_t*>(out->data), q->row_stride, q->head_stride, kk.row_stride, kk.head_stride, vv.row_stride,
+                     vv.head_stride, out->row_stride, out->head_stride, d_q_offsets, d_k_offsets, nq, nk, samples, hkv, share, d,
+                     causal ? 1 : 0, (int)units, scale * 1.44269504088896340736f};
+    const dim3 grid((unsigned)(units * hkv)), block(AT_NW * 64);
+    hipStream_t s = as_stream(stream);
+    if (dtype == TSP_BF16) {
+        if (d <= 64) hipLaunchKernelGGL((k_attention<true, 64, AT_NW>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((k_attention<true, 128, AT_NW>), grid, block, 0, s, a);
+    } else {
+        if (d <= 64) hipLaunchKernelGGL((k_attention<false, 64, AT_NW>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((k_attention<false, 128, AT_NW>), grid, block, 0, s, a);
+    }
+    TSP_CHECK_LAUNCH();
+    return TSP_OK;
+}

@@ -1,0 +1,87 @@
+// Packed samples: rows of several samples one after another, sample s on rows [offsets[s],
+// offsets[s + 1]) (device int32 [samples + 1], non-decreasing). Kernels cut every sample into units of
+// at most `per` rows; a launch has as many workgroups as there can be units (ceil(n / per) + samples:
+// the host does not know the lengths) and each finds its own unit here.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "common.hpp"
+
+namespace tsp {
+
+struct PackedUnit {
+    int sample;        // -1: there are fewer units
+    int first, count;  // the sample's first unit, how many it has
+    int64_t row0, rows;   // the sample's rows
+};
+
+// Rows of sample s; bounds outside [0, n] or out of order are cut to it, so that no row outside the
+// tensor is touched. offsets NULL: one sample of all n rows.
+__device__ __forceinline__ void packed_rows(const int32_t* offsets, int s, int64_t n, int64_t& row0, int64_t& rows) {
+    if (!offsets) {
+        row0 = 0;
+        rows = n;
+        return;
+    }
+    const int64_t a = offsets[s], b = offsets[s + 1];
+    row0 = a < 0 ? 0 : a > n ? n : a;
+    rows = (b > n ? n : b) - row0;
+    if (rows < 0) rows = 0;
+}
+
+// The unit-th unit of `per` rows (each row counted `mult` times), called by whole waves with a uniform
+// unit: 64 samples a step, their unit counts summed across the wave.
+__device__ __forceinline__ PackedUnit packed_unit(const int32_t* offsets, int samples, int64_t n, int mult, int per, int unit) {
+    PackedUnit u{-1, 0, 0, 0, 0};
+    if (samples == 1) {
+        packed_rows(offsets, 0, n, u.row0, u.rows);
+        u.count = (int)((u.rows * mult + per - 1) / per);
+        if (unit < u.count) u.sample = 0;
+        return u;
+    }
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int s0 = 0; s0 < samples; s0 += 64) {
+        const int s = s0 + lane;
+        int64_t row0 = 0, rows = 0;
+        if (s < samples) packed_rows(offsets, s, n, row0, rows);
+        const int cnt = (int)((rows * mult + per - 1) / per);
+        int end = cnt;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int v = __shfl_up(end, o, 64);
+            if (lane >= o) end += v;
+        }
+        const uint64_t past = __ballot(before + end > unit);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            u.sample = s0 + l;
+            u.count = __builtin_amdgcn_readlane(cnt, l);
+            u.first = before + __builtin_amdgcn_readlane(end, l) - u.count;
+            u.row0 = __builtin_amdgcn_readlane((int)row0, l);
+            u.rows = __builtin_amdgcn_readlane((int)rows, l);
+            return u;
+        }
+        before += __builtin_amdgcn_readlane(end, 63);
+    }
+    return u;
+}
+
+// Rows of heads as the transformer pieces take them: 16-byte aligned, strides multiples of 8 elements (a
+// row's below 2^20, so that a tile of rows spans less than 2^31 bytes).
+inline bool heads_aligned(const tsp_heads& t) {
+    return t.row_stride >= 0 && t.head_stride >= 0 && t.row_stride <= (1ll << 20) && t.head_stride <= (1ll << 40) &&
+           t.row_stride % 8 == 0 && t.head_stride % 8 == 0 && reinterpret_cast<uintptr_t>(t.data) % 16 == 0;
+}
+// ... that can be written: no two heads of d elements share one.
+inline bool heads_apart(const tsp_heads& t, int64_t n, int heads, int d) {
+    const int64_t r = t.row_stride, h = t.head_stride;
+    if (n <= 1 && heads <= 1) return true;
+    if (heads <= 1) return r >= d;
+    if (n <= 1) return h >= d;
+    return (h >= d && r >= (heads - 1) * h + d) || (r >= d && h >= (n - 1) * r + d);
+}
+
+}  // namespace tsp
