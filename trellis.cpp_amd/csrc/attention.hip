@@ -35,8 +35,10 @@ struct AttnArgs {
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;   // strides in elements
     const int32_t *q_off, *k_off;
     int64_t nq, nk;
-    int samples, hkv, share, d, causal, units;
+    int samples, hkv, share, d, causal, units, splits;
     float scale2;                             // scale * log2(e)
+    float* part;                              // splits > 1: [split][nq * hq][d] sums of p v, then
+    float2* stat;                             // [split][nq * hq] maximum and sum of p (-1: no key seen)
 };
 
 template <bool BF16>
@@ -105,7 +107,8 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
     constexpr int KS = DP / 16, DB = DP / 32, P = DP / 8, NT = NW * 64, ROWS = NW * 32;
     __shared__ __attribute__((aligned(16))) char sK[AT_KEYS * DP * 2];
     __shared__ __attribute__((aligned(16))) char sV[AT_KEYS * DP * 2];
-    const int head = blockIdx.x / a.units, unit = blockIdx.x - head * a.units;
+    const int split = blockIdx.x % a.splits, hu = blockIdx.x / a.splits;
+    const int head = hu / a.units, unit = hu - head * a.units;
     const PackedUnit u = packed_unit(a.q_off, a.samples, a.nq, a.share, ROWS, unit);
     if (u.sample < 0) return;
     int64_t krow0, krows;
@@ -144,7 +147,10 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
     for (int db = 0; db < DB; ++db) o[db] = f32x16_t{};
     float m = -INFINITY, l = 0.f;
 
-    for (int base = 0; base < wg_end; base += AT_KEYS) {
+    // this split's share of the workgroup's tiles
+    const int tiles = (wg_end + AT_KEYS - 1) / AT_KEYS, per = (tiles + a.splits - 1) / a.splits;
+    const int begin = split * per * AT_KEYS, end = min(wg_end, begin + per * AT_KEYS);
+    for (int base = begin; base < end; base += AT_KEYS) {
         __syncthreads();
         for (int e = threadIdx.x; e < AT_KEYS * P; e += NT) {
             const int key = e / P, piece = e % P;
@@ -259,8 +265,24 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
     }
 
     const float2 lh = both_halves(l);
-    const float inv = 1.0f / (lh.x + lh.y);
+    const float sum = lh.x + lh.y;
     if (r >= rows) return;
+    if (a.splits > 1) {
+        const int64_t item = ((int64_t)split * a.nq + u.row0 + qi) * (a.hkv * a.share) + hq;
+        const bool seen = lim.lane > begin && begin < end;
+        if (h == 0) a.stat[item] = float2{m, seen ? sum : -1.f};
+        if (!seen) return;
+        float* op = a.part + item * a.d;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int e = db * 32 + 8 * g + 4 * h;
+                if (e < a.d) *reinterpret_cast<f32x4_t*>(op + e) = f32x4_t{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+            }
+        return;
+    }
+    const float inv = 1.0f / sum;
     uint16_t* op = a.o + (u.row0 + qi) * a.o_row + hq * a.o_head;
     const bool none = lim.lane == 0;
 #pragma unroll
@@ -274,14 +296,87 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
         }
 }
 
-constexpr int AT_NW = 4;
+// The splits' sums joined: sum_s w_s (p v)_s / sum_s w_s (sum p)_s, w_s = exp(max_s - max). 16 lanes a
+// row and head, 8 elements each. A split whose scores were all -inf has sums of 0 (or NaN): its weight
+// does not matter.
+template <bool BF16>
+__global__ __launch_bounds__(256) void k_attention_join(AttnArgs a) {
+    const int heads = a.hkv * a.share, e = (threadIdx.x & 15) * 8;
+    const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4, row = item / heads;
+    int64_t first = 0, last = a.nq;
+    if (a.q_off) {
+        first = a.q_off[0];
+        last = a.q_off[a.samples];
+    }
+    if (row >= a.nq || row < first || row >= last || e >= a.d) return;
+    const int64_t step = a.nq * heads;
+    float m = -INFINITY;
+    bool seen = false;
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 t = a.stat[s * step + item];
+        if (t.y == -1.f) continue;
+        m = fmaxf(m, t.x);
+        seen = true;
+    }
+    float acc[8] = {}, sum = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 t = a.stat[s * step + item];
+        if (t.y == -1.f) continue;
+        const float w = t.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((t.x - m) * a.scale2);
+        const f32x4_t* p = reinterpret_cast<const f32x4_t*>(a.part + (s * step + item) * a.d + e);
+        const f32x4_t x = p[0], y = p[1];
+        sum += w * t.y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            acc[i] += w * x[i];
+            acc[4 + i] += w * y[i];
+        }
+    }
+    const float inv = 1.0f / sum;
+    u32x4_t y{0, 0, 0, 0};
+    if (seen)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+    *reinterpret_cast<u32x4_t*>(a.o + row * a.o_row + (item - row * heads) * a.o_head + e) = y;
+}
+
+// How a call is cut: waves of a workgroup (32 rows each), units of rows, splits of the keys.
+struct AttnCut {
+    int nw, splits;
+    int64_t units;
+};
+
+AttnCut attn_cut(int64_t nq, int64_t nk, int samples, int hkv, int share) {
+    AttnCut c;
+    // one wave where a sample has at most its 32 rows (by the mean: the host does not know the lengths)
+    c.nw = ceil_div(nq, samples) * share <= 32 ? 1 : 4;
+    c.units = ceil_div(nq * share, c.nw * 32) + (samples > 1 ? samples : 0);
+    // splits: the rounds that the workgroups take on the device's slots, each as long as a split's tiles
+    // and about three tiles' time of start and end
+    const int64_t busy = (ceil_div(nq * share, c.nw * 32) + (samples > 1 ? samples / 2 : 0)) * hkv, slots = c.nw == 1 ? 1024 : 512;
+    const int64_t tiles = ceil_div(ceil_div(nk, samples), AT_KEYS);
+    c.splits = 1;
+    int64_t best = ceil_div(busy, slots) * (tiles + 3);
+    for (int s = 2; s <= 128 && busy * s <= 4 * slots; ++s) {
+        const int64_t cost = ceil_div(busy * s, slots) * (ceil_div(tiles, s) + 3) + 3;
+        if (cost < best) {
+            best = cost;
+            c.splits = s;
+        }
+    }
+    return c;
+}
 
 }  // namespace
 }  // namespace tsp
 
 using namespace tsp;
 
-extern "C" size_t tsp_attention_workspace_bytes(int64_t nq, int64_t nk, int samples, int hq, int hkv, int d) { return 0; }
+extern "C" size_t tsp_attention_workspace_bytes(int64_t nq, int64_t nk, int samples, int hq, int hkv, int d) {
+    if (nq <= 0 || nq >= (1ll << 31) || nk < 0 || nk >= (1ll << 31) || samples <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || d <= 0) return 0;
+    const AttnCut c = attn_cut(nq, nk, samples, hkv, hq / hkv);
+    return c.splits == 1 ? 0 : (size_t)c.splits * nq * hq * ((size_t)d * sizeof(float) + sizeof(float2));
+}
 
 extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_heads* v, int dtype, int64_t nq, int64_t nk, int hq,
                              int hkv, int d, const int32_t* d_q_offsets, const int32_t* d_k_offsets, int samples, float scale,
@@ -307,21 +402,37 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
     TSP_REQUIRE(heads_apart(*out, nq, hq, d), TSP_ERR_INVALID, "tsp_attention: the output's heads overlap");
     TSP_REQUIRE(out->data != kk.data && out->data != vv.data && out->data != q->data, TSP_ERR_INVALID, "tsp_attention: out must not alias q, k or v");
     const int share = hq / hkv;
-    const int64_t units = ceil_div(nq * share, AT_NW * 32) + (samples > 1 ? samples : 0);
-    TSP_REQUIRE(units * hkv * AT_NW * 64 < (1ll << 32), TSP_ERR_INVALID, "tsp_attention: too many rows");
+    const AttnCut c = attn_cut(nq, nk, samples, hkv, share);
+    const int64_t blocks = c.units * hkv * c.splits;
+    TSP_REQUIRE(blocks * c.nw * 64 < (1ll << 32), TSP_ERR_INVALID, "tsp_attention: too many rows");
+    const size_t need = tsp_attention_workspace_bytes(nq, nk, samples, hq, hkv, d);
+    TSP_REQUIRE(need == 0 || d_workspace, TSP_ERR_INVALID, "tsp_attention: null workspace");
+    TSP_REQUIRE(workspace_bytes >= need, TSP_ERR_WORKSPACE, "tsp_attention: workspace of %zu bytes, needs %zu", workspace_bytes, need);
+    TSP_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0, TSP_ERR_INVALID, "tsp_attention: workspace not 16-byte aligned");
+    float* part = need ? static_cast<float*>(d_workspace) : nullptr;
+    float2* stat = need ? reinterpret_cast<float2*>(part + (int64_t)c.splits * nq * hq * d) : nullptr;
     const AttnArgs a{static_cast<const uint16_t*>(q->data), static_cast<const uint16_t*>(kk.data), static_cast<const uint16_t*>(vv.data),
                      static_cast<uint16_t*>(out->data), q->row_stride, q->head_stride, kk.row_stride, kk.head_stride, vv.row_stride,
                      vv.head_stride, out->row_stride, out->head_stride, d_q_offsets, d_k_offsets, nq, nk, samples, hkv, share, d,
-                     causal ? 1 : 0, (int)units, scale * 1.44269504088896340736f};
-    const dim3 grid((unsigned)(units * hkv)), block(AT_NW * 64);
+                     causal ? 1 : 0, (int)c.units, c.splits, scale * 1.44269504088896340736f, part, stat};
+    const dim3 grid((unsigned)blocks), block(c.nw * 64);
     hipStream_t s = as_stream(stream);
-    if (dtype == TSP_BF16) {
-        if (d <= 64) hipLaunchKernelGGL((k_attention<true, 64, AT_NW>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((k_attention<true, 128, AT_NW>), grid, block, 0, s, a);
-    } else {
-        if (d <= 64) hipLaunchKernelGGL((k_attention<false, 64, AT_NW>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((k_attention<false, 128, AT_NW>), grid, block, 0, s, a);
-    }
+    auto go = [&](auto bf, auto dp, auto nw) {
+        hipLaunchKernelGGL((k_attention<decltype(bf)::value, decltype(dp)::value, decltype(nw)::value>), grid, block, 0, s, a);
+        if (c.splits > 1)
+            hipLaunchKernelGGL((k_attention_join<decltype(bf)::value>), dim3((unsigned)ceil_div(nq * hq * 16, 256)), dim3(256), 0, s, a);
+    };
+    using std::integral_constant;
+    auto by_width = [&](auto bf) {
+        auto by_waves = [&](auto dp) {
+            if (c.nw == 1) go(bf, dp, integral_constant<int, 1>{});
+            else go(bf, dp, integral_constant<int, 4>{});
+        };
+        if (d <= 64) by_waves(integral_constant<int, 64>{});
+        else by_waves(integral_constant<int, 128>{});
+    };
+    if (dtype == TSP_BF16) by_width(integral_constant<bool, true>{});
+    else by_width(integral_constant<bool, false>{});
     TSP_CHECK_LAUNCH();
     return TSP_OK;
 }
