@@ -34,7 +34,7 @@ struct AttnArgs {
     uint16_t* o;
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;   // strides in elements
     const int32_t *q_off, *k_off;
-    int64_t nq, nk;
+    int64_t nq, nk;                           // below 2^31, nq * share too
     int samples, hkv, share, d, causal, units, splits;
     float scale2;                             // scale * log2(e)
     float* part;                              // splits > 1: [split][nq * hq][d] sums of p v, then
@@ -97,50 +97,66 @@ __device__ __forceinline__ u32x4_t v_operand(const char* sv, int ks, int db, int
     return u32x4_t{ua.x, ua.y, ub.x, ub.y};
 }
 
+// Waits for this wave's loads into LDS (which the compiler's own waits do not always cover).
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 // Keys of a tile that a row sees, for the rows of a wave's 32.
 struct RowLimits {
-    int lane, lo, hi;      // this lane's row, the wave's first and last
+    int lane, hi;      // this lane's row, the wave's last
 };
 
 template <bool BF16, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
     constexpr int KS = DP / 16, DB = DP / 32, P = DP / 8, NT = NW * 64, ROWS = NW * 32;
-    __shared__ __attribute__((aligned(16))) char sK[AT_KEYS * DP * 2];
-    __shared__ __attribute__((aligned(16))) char sV[AT_KEYS * DP * 2];
+    constexpr int TILE = AT_KEYS * DP * 2;
+    __shared__ __attribute__((aligned(16))) char sK0[TILE], sK1[TILE], sV0[TILE], sV1[TILE];
     const int split = blockIdx.x % a.splits, hu = blockIdx.x / a.splits;
     const int head = hu / a.units, unit = hu - head * a.units;
-    const PackedUnit u = packed_unit(a.q_off, a.samples, a.nq, a.share, ROWS, unit);
+    const PackedUnit u = packed_unit(a.q_off, a.samples, (int)a.nq, a.share, ROWS, unit);
     if (u.sample < 0) return;
-    int64_t krow0, krows;
-    packed_rows(a.k_off, u.sample, a.nk, krow0, krows);
-    const int lk = (int)krows;
-    const int64_t rows = u.rows * a.share;
-    const int64_t tile0 = (int64_t)(unit - u.first) * ROWS;
+    int krow0, lk;
+    packed_rows(a.k_off, u.sample, (int)a.nk, krow0, lk);
+    const int rows = u.rows * a.share, tile0 = (unit - u.first) * ROWS;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
 
     // rows past the sample's last are copies of it that are not stored
-    auto limit = [&](int64_t r) -> int {
-        r = r < rows ? r : rows - 1;
-        if (!a.causal) return lk;
-        const int64_t n = krows - u.rows + r / a.share + 1;
-        return n < 0 ? 0 : n < krows ? (int)n : lk;
-    };
-    const int64_t r = tile0 + wave * 32 + r32, rc = r < rows ? r : rows - 1;
-    const RowLimits lim{limit(r), limit(tile0 + wave * 32), limit(tile0 + wave * 32 + 31)};
-    const int wg_end = limit(tile0 + ROWS - 1);
-    const int64_t qi = rc / a.share;
-    const int hq = head * a.share + (int)(rc - qi * a.share);
+    auto limit = [&](int query) { return a.causal ? min(max(lk - u.rows + query + 1, 0), lk) : lk; };
+    auto query = [&](int r) { return (int)((unsigned)min(r, rows - 1) / (unsigned)a.share); };
+    const int r = tile0 + wave * 32 + r32, qi = query(r);
+    const RowLimits lim{limit(qi), limit(query(tile0 + wave * 32 + 31))};
+    const int wg_end = limit(query(tile0 + ROWS - 1));
+    const int hq = head * a.share + min(r, rows - 1) - qi * a.share;
 
     // Q^T operand: d = 16 ks + 8 h .. + 7 of the lane's row
     u32x4_t qf[KS];
     {
-        const uint16_t* qp = a.q + (u.row0 + qi) * a.q_row + hq * a.q_head;
+        const uint16_t* qp = a.q + (int64_t)(u.row0 + qi) * a.q_row + hq * a.q_head;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
             qf[ks] = ks * 16 + h * 8 < a.d ? *reinterpret_cast<const u32x4_t*>(qp + ks * 16 + h * 8) : u32x4_t{0, 0, 0, 0};
     }
-    const uint16_t* kp = a.k + krow0 * a.k_row + head * a.k_head;
-    const uint16_t* vp = a.v + krow0 * a.v_row + head * a.v_head;
+    const uint16_t* kp = a.k + (int64_t)krow0 * a.k_row + head * a.k_head;
+    const uint16_t* vp = a.v + (int64_t)krow0 * a.v_row + head * a.v_head;
+
+    // A tile goes straight from memory to LDS, 1 KiB a wave and load: 16 bytes a lane, each from the piece
+    // that belongs in its place. Rows past the sample's last key and pieces past d read as zeros (out of
+    // the buffer's range).
+    constexpr int LOADS = TILE / 1024 / NW;
+    auto stage = [&](const uint16_t* p, int64_t stride, int base, char* s, bool is_v) {
+        const int rows = min(AT_KEYS, lk - base);
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(p + base * stride), (short)0, (int)(rows * stride * 2), 0x00027000);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int at = (i * NW + wave) * 1024, key = at / (DP * 2) + lane / P, place = lane % P;
+            const int piece = is_v ? v_piece<DP>(key, place) / 16 % P : k_piece<DP>(key, place) / 16 % P;
+            const int off = piece * 8 < a.d ? (int)(key * stride + piece * 8) * 2 : -1;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(s + at), 16, off, 0, 0, 0);
+        }
+    };
+    auto stage_tile = [&](int base, char* sk, char* sv) {
+        stage(kp, a.k_row, base, sk, false);
+        stage(vp, a.v_row, base, sv, true);
+    };
 
     f32x16_t o[DB];
 #pragma unroll
@@ -150,21 +166,8 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
     // this split's share of the workgroup's tiles
     const int tiles = (wg_end + AT_KEYS - 1) / AT_KEYS, per = (tiles + a.splits - 1) / a.splits;
     const int begin = split * per * AT_KEYS, end = min(wg_end, begin + per * AT_KEYS);
-    for (int base = begin; base < end; base += AT_KEYS) {
-        __syncthreads();
-        for (int e = threadIdx.x; e < AT_KEYS * P; e += NT) {
-            const int key = e / P, piece = e % P;
-            u32x4_t x{0, 0, 0, 0}, y{0, 0, 0, 0};
-            if (base + key < lk && piece * 8 < a.d) {
-                x = *reinterpret_cast<const u32x4_t*>(kp + (int64_t)(base + key) * a.k_row + piece * 8);
-                y = *reinterpret_cast<const u32x4_t*>(vp + (int64_t)(base + key) * a.v_row + piece * 8);
-            }
-            *reinterpret_cast<u32x4_t*>(sK + k_piece<DP>(key, piece)) = x;
-            *reinterpret_cast<u32x4_t*>(sV + v_piece<DP>(key, piece)) = y;
-        }
-        __syncthreads();
-        if (base >= lim.hi) continue;
-
+    auto attend = [&](auto masked_tile, int base, const char* sK, const char* sV) {
+        constexpr bool MASKED = decltype(masked_tile)::value;
         // scores: s[kb][i] is key kb * 32 + 8 (i / 4) + 4 h + i % 4 of the tile
         f32x16_t s[2];
 #pragma unroll
@@ -174,8 +177,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
             for (int ks = 0; ks < KS; ++ks)
                 s[kb] = mfma32<BF16>(*reinterpret_cast<const u32x4_t*>(sK + k_piece<DP>(kb * 32 + r32, ks * 2 + h)), qf[ks], s[kb]);
         }
-        const bool masked = base + AT_KEYS > lim.lo;
-        if (masked) {
+        if constexpr (MASKED) {
             const int left = lim.lane - base - 4 * h;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
@@ -191,6 +193,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
         const float2 mh = both_halves(mt);
         const float mn = fmaxf(m, fmaxf(mh.x, mh.y));
         const float mz = mn == -INFINITY ? 0.f : mn;        // (no key seen yet, or scores of -inf alone)
+        // (nothing is summed yet where m is -inf: any finite factor will do)
         const float corr = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mz) * a.scale2);
         m = mn;
         const float mc = mz * a.scale2;
@@ -216,7 +219,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
         // Rows of the tile that see different keys: a probability of zero must not meet an Inf or a NaN
         // of a key that its row does not see. Zero times V shows whether there is one.
         bool odd = false;
-        if (masked && a.causal) {
+        if (MASKED && a.causal) {
             f32x16_t z = f32x16_t{};
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
@@ -232,7 +235,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
                 u32x4_t vf = v_operand<DP>(sV, ks, db, lane);
-                if (odd) {
+                if (MASKED && odd) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         if (nonfinite16<BF16>(vf[e])) vf[e] &= 0xffff0000u;
@@ -241,7 +244,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
                 }
                 o[db] = mfma32<BF16>(vf, pf[ks], o[db]);
             }
-        if (odd) {      // the values left out, key by key, for the rows that see them
+        if (MASKED && odd) {      // the values left out, key by key, for the rows that see them
             for (int key = 0; key < AT_KEYS; ++key) {
                 float p = 0.f;
 #pragma unroll
@@ -262,6 +265,34 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
                     }
             }
         }
+    };
+    // Two buffers: a tile is read while the next one is on its way. The wait is for this wave's own loads;
+    // the barrier then says that every wave's have landed, and that no wave reads the other buffer any more.
+    auto next = [&](int base, char* sk, char* sv) {
+        wait_loads();
+        __syncthreads();
+        if (base < end) stage_tile(base, sk, sv);
+    };
+    if (begin < end) stage_tile(begin, sK0, sV0);
+    // tiles that every row of the workgroup sees whole, then the others
+    const int whole = min(end, limit(query(tile0)));
+    int base = begin;
+    bool second = false;
+    while (base + AT_KEYS <= whole) {
+        next(base + AT_KEYS, sK1, sV1);
+        attend(std::false_type{}, base, sK0, sV0);
+        base += AT_KEYS;
+        if (base + AT_KEYS > whole) {
+            second = true;
+            break;
+        }
+        next(base + AT_KEYS, sK0, sV0);
+        attend(std::false_type{}, base, sK1, sV1);
+        base += AT_KEYS;
+    }
+    for (; base < end; base += AT_KEYS, second = !second) {
+        next(base + AT_KEYS, second ? sK0 : sK1, second ? sV0 : sV1);
+        if (base < lim.hi) attend(std::true_type{}, base, second ? sK1 : sK0, second ? sV1 : sV0);
     }
 
     const float2 lh = both_halves(l);
@@ -283,7 +314,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
         return;
     }
     const float inv = 1.0f / sum;
-    uint16_t* op = a.o + (u.row0 + qi) * a.o_row + hq * a.o_head;
+    uint16_t* op = a.o + (int64_t)(u.row0 + qi) * a.o_row + hq * a.o_head;
     const bool none = lim.lane == 0;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -373,7 +404,7 @@ AttnCut attn_cut(int64_t nq, int64_t nk, int samples, int hkv, int share) {
 using namespace tsp;
 
 extern "C" size_t tsp_attention_workspace_bytes(int64_t nq, int64_t nk, int samples, int hq, int hkv, int d) {
-    if (nq <= 0 || nq >= (1ll << 31) || nk < 0 || nk >= (1ll << 31) || samples <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || d <= 0) return 0;
+    if (nq <= 0 || nq >= (1ll << 31) || nk < 0 || nk >= (1ll << 31) - (1ll << 16) || samples <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || d <= 0) return 0;
     const AttnCut c = attn_cut(nq, nk, samples, hkv, hq / hkv);
     return c.splits == 1 ? 0 : (size_t)c.splits * nq * hq * ((size_t)d * sizeof(float) + sizeof(float2));
 }
@@ -382,7 +413,7 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
                              int hkv, int d, const int32_t* d_q_offsets, const int32_t* d_k_offsets, int samples, float scale,
                              int causal, const tsp_heads* out, void* d_workspace, size_t workspace_bytes, void* stream) {
     clear_error();
-    TSP_REQUIRE(nq >= 0 && nq < (1ll << 31) && nk >= 0 && nk < (1ll << 31) - AT_KEYS, TSP_ERR_INVALID, "tsp_attention: nq=%lld nk=%lld out of range",
+    TSP_REQUIRE(nq >= 0 && nq < (1ll << 31) && nk >= 0 && nk < (1ll << 31) - (1ll << 16), TSP_ERR_INVALID, "tsp_attention: nq=%lld nk=%lld out of range",
                 (long long)nq, (long long)nk);
     TSP_REQUIRE(hq > 0 && hkv > 0 && hq % hkv == 0 && hq <= 4096, TSP_ERR_INVALID, "tsp_attention: %d heads on %d", hq, hkv);
     TSP_REQUIRE(dtype_valid(dtype), TSP_ERR_INVALID, "tsp_attention: bad dtype");
@@ -404,7 +435,7 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
     const int share = hq / hkv;
     const AttnCut c = attn_cut(nq, nk, samples, hkv, share);
     const int64_t blocks = c.units * hkv * c.splits;
-    TSP_REQUIRE(blocks * c.nw * 64 < (1ll << 32), TSP_ERR_INVALID, "tsp_attention: too many rows");
+    TSP_REQUIRE(blocks * c.nw * 64 < (1ll << 32) && nq * share < (1ll << 31) - 1024, TSP_ERR_INVALID, "tsp_attention: too many rows");
     const size_t need = tsp_attention_workspace_bytes(nq, nk, samples, hq, hkv, d);
     TSP_REQUIRE(need == 0 || d_workspace, TSP_ERR_INVALID, "tsp_attention: null workspace");
     TSP_REQUIRE(workspace_bytes >= need, TSP_ERR_WORKSPACE, "tsp_attention: workspace of %zu bytes, needs %zu", workspace_bytes, need);

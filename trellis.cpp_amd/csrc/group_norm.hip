@@ -29,9 +29,9 @@ struct GnArgs {
 };
 
 __device__ __forceinline__ int unit_rows(const PackedUnit& u, int unit, int per, int64_t& row) {
-    const int64_t lo = (int64_t)(unit - u.first) * per;
+    const int lo = (unit - u.first) * per;
     row = u.row0 + lo;
-    return (int)(u.rows - lo < per ? u.rows - lo : per);
+    return min(u.rows - lo, per);
 }
 
 __device__ __forceinline__ float act(float y, int silu) { return silu ? y / (1.0f + expf(-y)) : y; }
@@ -41,7 +41,7 @@ __device__ __forceinline__ float act(float y, int silu) { return silu ? y / (1.0
 template <int XDT>
 __global__ __launch_bounds__(GN_NT) void k_gn_stats(GnArgs a) {
     __shared__ float2 sPart[GN_NT / 64];
-    const PackedUnit u = packed_unit(a.offsets, a.samples, a.n, 1, a.per, blockIdx.x);
+    const PackedUnit u = packed_unit(a.offsets, a.samples, (int)a.n, 1, a.per, blockIdx.x);
     if (u.sample < 0) return;
     int64_t row;
     const int rows = unit_rows(u, blockIdx.x, a.per, row);
@@ -74,20 +74,20 @@ __global__ __launch_bounds__(GN_NT) void k_gn_stats(GnArgs a) {
 // Mean and 1 / sqrt(var + eps) of every group of the unit's sample, into LDS.
 __device__ __forceinline__ void join_units(const GnArgs& a, const PackedUnit& u, float* sMean, float* sRstd) {
     const int cg = a.c / a.groups;
-    const float total = (float)(u.rows * cg);
+    const float total = (float)u.rows * (float)cg;
     for (int g = threadIdx.x; g < a.groups; g += GN_NT) {
         const float2* p = a.part + (int64_t)u.first * a.groups + g;
         // (the units' means less the first one's: of equal values the mean is that value)
         const float m0 = p->x;
         float m = 0.f;
         for (int i = 1; i < u.count; ++i)
-            m += (p[(int64_t)i * a.groups].x - m0) * ((float)(min<int64_t>(a.per, u.rows - (int64_t)i * a.per) * cg) / total);
+            m += (p[(int64_t)i * a.groups].x - m0) * ((float)min(a.per, u.rows - i * a.per) * (float)cg / total);
         m += m0;
         float q = 0.f;
         for (int i = 0; i < u.count; ++i) {
             const float2 t = p[(int64_t)i * a.groups];
             const float d = t.x - m;
-            q += t.y + d * d * (float)(min<int64_t>(a.per, u.rows - (int64_t)i * a.per) * cg);
+            q += t.y + d * d * (float)min(a.per, u.rows - i * a.per) * (float)cg;
         }
         sMean[g] = m;
         sRstd[g] = 1.0f / sqrtf(q / total + a.eps);
@@ -98,7 +98,7 @@ __device__ __forceinline__ void join_units(const GnArgs& a, const PackedUnit& u,
 template <int XDT, int ODT>
 __global__ __launch_bounds__(GN_NT) void k_gn_apply(GnArgs a) {
     __shared__ float sMean[GN_MAX_GROUPS], sRstd[GN_MAX_GROUPS];
-    const PackedUnit u = packed_unit(a.offsets, a.samples, a.n, 1, a.per, blockIdx.x);
+    const PackedUnit u = packed_unit(a.offsets, a.samples, (int)a.n, 1, a.per, blockIdx.x);
     if (u.sample < 0) return;
     join_units(a, u, sMean, sRstd);
     int64_t row;
@@ -134,7 +134,7 @@ void dt_switch(int dt, F&& f) {
 using namespace tsp;
 
 extern "C" size_t tsp_group_norm_workspace_bytes(int64_t n, int c, int groups, int samples) {
-    if (n <= 0 || n >= (1ll << 31) || c <= 0 || groups <= 0 || samples <= 0) return 0;
+    if (n <= 0 || n >= (1ll << 31) - (1ll << 24) || c <= 0 || groups <= 0 || samples <= 0) return 0;
     return (size_t)gn_units(n, samples) * groups * sizeof(float2);
 }
 
@@ -142,7 +142,7 @@ extern "C" int tsp_group_norm(const void* d_x, int x_dtype, int64_t n, int c, in
                               int samples, const float* d_gamma, const float* d_beta, float eps, int silu, void* d_out,
                               int out_dtype, void* d_workspace, size_t workspace_bytes, void* stream) {
     clear_error();
-    TSP_REQUIRE(n >= 0 && n < (1ll << 31) && c > 0, TSP_ERR_INVALID, "tsp_group_norm: n=%lld c=%d out of range", (long long)n, c);
+    TSP_REQUIRE(n >= 0 && n < (1ll << 31) - (1ll << 24) && c > 0, TSP_ERR_INVALID, "tsp_group_norm: n=%lld c=%d out of range", (long long)n, c);
     TSP_REQUIRE(groups > 0 && c % groups == 0, TSP_ERR_INVALID, "tsp_group_norm: %d channels in %d groups", c, groups);
     TSP_REQUIRE(samples > 0 && (d_offsets || samples == 1), TSP_ERR_INVALID,
                 "tsp_group_norm: samples=%d (without offsets: 1)", samples);

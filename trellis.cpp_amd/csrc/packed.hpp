@@ -14,30 +14,23 @@ namespace tsp {
 struct PackedUnit {
     int sample;        // -1: there are fewer units
     int first, count;  // the sample's first unit, how many it has
-    int64_t row0, rows;   // the sample's rows
+    int row0, rows;    // the sample's rows
 };
 
-// Rows of sample s; bounds outside [0, n] or out of order are cut to it, so that no row outside the
-// tensor is touched. offsets NULL: one sample of all n rows.
-__device__ __forceinline__ void packed_rows(const int32_t* offsets, int s, int64_t n, int64_t& row0, int64_t& rows) {
-    if (!offsets) {
-        row0 = 0;
-        rows = n;
-        return;
-    }
-    const int64_t a = offsets[s], b = offsets[s + 1];
-    row0 = a < 0 ? 0 : a > n ? n : a;
-    rows = (b > n ? n : b) - row0;
-    if (rows < 0) rows = 0;
+// Rows of sample s of n < 2^31; bounds outside [0, n] or out of order are cut to it, so that no row
+// outside the tensor is touched. offsets NULL: one sample of all n rows.
+__device__ __forceinline__ void packed_rows(const int32_t* offsets, int s, int n, int& row0, int& rows) {
+    row0 = offsets ? min(max(offsets[s], 0), n) : 0;
+    rows = offsets ? max(min(offsets[s + 1], n), row0) - row0 : n;
 }
 
-// The unit-th unit of `per` rows (each row counted `mult` times), called by whole waves with a uniform
-// unit: 64 samples a step, their unit counts summed across the wave.
-__device__ __forceinline__ PackedUnit packed_unit(const int32_t* offsets, int samples, int64_t n, int mult, int per, int unit) {
+// The unit-th unit of `per` rows (each row counted `mult` times; n * mult + per < 2^31), called by whole
+// waves with a uniform unit: 64 samples a step, their unit counts summed across the wave.
+__device__ __forceinline__ PackedUnit packed_unit(const int32_t* offsets, int samples, int n, int mult, int per, int unit) {
     PackedUnit u{-1, 0, 0, 0, 0};
     if (samples == 1) {
         packed_rows(offsets, 0, n, u.row0, u.rows);
-        u.count = (int)((u.rows * mult + per - 1) / per);
+        u.count = (int)((unsigned)(u.rows * mult + per - 1) / (unsigned)per);
         if (unit < u.count) u.sample = 0;
         return u;
     }
@@ -45,9 +38,9 @@ __device__ __forceinline__ PackedUnit packed_unit(const int32_t* offsets, int sa
     int before = 0;
     for (int s0 = 0; s0 < samples; s0 += 64) {
         const int s = s0 + lane;
-        int64_t row0 = 0, rows = 0;
+        int row0 = 0, rows = 0;
         if (s < samples) packed_rows(offsets, s, n, row0, rows);
-        const int cnt = (int)((rows * mult + per - 1) / per);
+        const int cnt = (int)((unsigned)(rows * mult + per - 1) / (unsigned)per);
         int end = cnt;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -60,8 +53,8 @@ __device__ __forceinline__ PackedUnit packed_unit(const int32_t* offsets, int sa
             u.sample = s0 + l;
             u.count = __builtin_amdgcn_readlane(cnt, l);
             u.first = before + __builtin_amdgcn_readlane(end, l) - u.count;
-            u.row0 = __builtin_amdgcn_readlane((int)row0, l);
-            u.rows = __builtin_amdgcn_readlane((int)rows, l);
+            u.row0 = __builtin_amdgcn_readlane(row0, l);
+            u.rows = __builtin_amdgcn_readlane(rows, l);
             return u;
         }
         before += __builtin_amdgcn_readlane(end, 63);
