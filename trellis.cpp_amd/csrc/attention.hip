@@ -57,6 +57,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{lo, hi}, f16x2_t));
 }
 
+// The sum of a packed pair and c, in fp32.
+template <bool BF16>
+__device__ __forceinline__ float add2(uint32_t p, float c) {
+    if constexpr (BF16) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, p), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), c, false);
+    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, p), __builtin_bit_cast(f16x2_t, 0x3c003c00u), c, false);
+}
+
 // The value of the other lane half (lane ^ 32), for both halves: {lower half's, upper half's}.
 __device__ __forceinline__ float2 both_halves(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -105,9 +112,28 @@ struct RowLimits {
     int lane, hi;      // this lane's row, the wave's last
 };
 
+#ifdef __HIP_DEVICE_COMPILE__       // (the host pass knows neither the register constraint nor the argument segment)
+// Keeps a value in scalar registers of its own from here on.
+template <class T>
+__device__ __forceinline__ void keep_scalar(T& x) {
+    asm volatile("" : "+s"(x));
+}
+
+// The kernel's arguments read anew: kept in scalar registers from the start on they would push the main
+// loop's own out of them.
+typedef const __attribute__((address_space(4))) AttnArgs* AttnArgsPtr;
+__device__ __forceinline__ AttnArgsPtr reread_args() {
+    AttnArgsPtr p = (AttnArgsPtr)__builtin_amdgcn_kernarg_segment_ptr();
+    keep_scalar(p);
+    return p;
+}
+#endif
+
 template <bool BF16, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
-    constexpr int KS = DP / 16, DB = DP / 32, P = DP / 8, NT = NW * 64, ROWS = NW * 32;
+__global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
+#ifdef __HIP_DEVICE_COMPILE__
+    const auto& a = *reread_args();
+    constexpr int KS = DP / 16, DB = DP / 32, P = DP / 8, ROWS = NW * 32;
     constexpr int TILE = AT_KEYS * DP * 2;
     __shared__ __attribute__((aligned(16))) char sK0[TILE], sK1[TILE], sV0[TILE], sV1[TILE];
     const int split = blockIdx.x % a.splits, hu = blockIdx.x / a.splits;
@@ -117,11 +143,11 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
     int krow0, lk;
     packed_rows(a.k_off, u.sample, (int)a.nk, krow0, lk);
     const int rows = u.rows * a.share, tile0 = (unit - u.first) * ROWS;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
 
     // rows past the sample's last are copies of it that are not stored
-    auto limit = [&](int query) { return a.causal ? min(max(lk - u.rows + query + 1, 0), lk) : lk; };
-    auto query = [&](int r) { return (int)((unsigned)min(r, rows - 1) / (unsigned)a.share); };
+    auto limit = [&](int query) __attribute__((always_inline)) { return a.causal ? min(max(lk - u.rows + query + 1, 0), lk) : lk; };
+    auto query = [&](int r) __attribute__((always_inline)) { return (int)((unsigned)min(r, rows - 1) / (unsigned)a.share); };
     const int r = tile0 + wave * 32 + r32, qi = query(r);
     const RowLimits lim{limit(qi), limit(query(tile0 + wave * 32 + 31))};
     const int wg_end = limit(query(tile0 + ROWS - 1));
@@ -135,27 +161,39 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
         for (int ks = 0; ks < KS; ++ks)
             qf[ks] = ks * 16 + h * 8 < a.d ? *reinterpret_cast<const u32x4_t*>(qp + ks * 16 + h * 8) : u32x4_t{0, 0, 0, 0};
     }
-    const uint16_t* kp = a.k + (int64_t)krow0 * a.k_row + head * a.k_head;
-    const uint16_t* vp = a.v + (int64_t)krow0 * a.v_row + head * a.v_head;
+    const char* kp = reinterpret_cast<const char*>(a.k + (int64_t)krow0 * a.k_row + head * a.k_head);
+    const char* vp = reinterpret_cast<const char*>(a.v + (int64_t)krow0 * a.v_row + head * a.v_head);
+    int k_bytes = (int)a.k_row * 2, v_bytes = (int)a.v_row * 2;      // of a row
+    float scale2 = a.scale2;
+    keep_scalar(kp);
+    keep_scalar(vp);
+    keep_scalar(k_bytes);
+    keep_scalar(v_bytes);
+    keep_scalar(scale2);
 
     // A tile goes straight from memory to LDS, 1 KiB a wave and load: 16 bytes a lane, each from the piece
     // that belongs in its place. Rows past the sample's last key and pieces past d read as zeros (out of
     // the buffer's range).
     constexpr int LOADS = TILE / 1024 / NW;
-    auto stage = [&](const uint16_t* p, int64_t stride, int base, char* s, bool is_v) {
-        const int rows = min(AT_KEYS, lk - base);
-        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(p + base * stride), (short)0, (int)(rows * stride * 2), 0x00027000);
+    int k_at[LOADS], v_at[LOADS];            // a lane's byte offsets within the tile's rows
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int at = (i * NW + wave) * 1024, key = at / (DP * 2) + lane / P, place = lane % P;
-            const int piece = is_v ? v_piece<DP>(key, place) / 16 % P : k_piece<DP>(key, place) / 16 % P;
-            const int off = piece * 8 < a.d ? (int)(key * stride + piece * 8) * 2 : -1;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(s + at), 16, off, 0, 0, 0);
-        }
+    for (int i = 0; i < LOADS; ++i) {
+        const int key = (i * NW + wave) * (1024 / (DP * 2)) + lane / P;
+        const int kp = k_piece<DP>(key, lane % P) / 16 % P, vp = v_piece<DP>(key, lane % P) / 16 % P;
+        k_at[i] = kp * 8 < a.d ? key * k_bytes + kp * 16 : -1;
+        v_at[i] = vp * 8 < a.d ? key * v_bytes + vp * 16 : -1;
+        asm volatile("" : "+v"(k_at[i]), "+v"(v_at[i]));       // (computed here, not in every tile)
+    }
+    auto stage = [&](const char* p, int bytes, int base, const int (&at)[LOADS], char* s) __attribute__((always_inline)) {
+        const int n = min(AT_KEYS, lk - base);
+        const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(p + (int64_t)base * bytes), (short)0, n * bytes, 0x00027000);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(s + (i * NW + wave) * 1024), 16, at[i], 0, 0, 0);
     };
-    auto stage_tile = [&](int base, char* sk, char* sv) {
-        stage(kp, a.k_row, base, sk, false);
-        stage(vp, a.v_row, base, sv, true);
+    auto stage_tile = [&](int base, char* sk, char* sv) __attribute__((always_inline)) {
+        stage(kp, k_bytes, base, k_at, sk);
+        stage(vp, v_bytes, base, v_at, sv);
     };
 
     f32x16_t o[DB];
@@ -166,7 +204,8 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
     // this split's share of the workgroup's tiles
     const int tiles = (wg_end + AT_KEYS - 1) / AT_KEYS, per = (tiles + a.splits - 1) / a.splits;
     const int begin = split * per * AT_KEYS, end = min(wg_end, begin + per * AT_KEYS);
-    auto attend = [&](auto masked_tile, int base, const char* sK, const char* sV) {
+    const bool causal = a.causal;
+    auto attend = [&](auto masked_tile, int base, const char* sK, const char* sV) __attribute__((always_inline)) {
         constexpr bool MASKED = decltype(masked_tile)::value;
         // scores: s[kb][i] is key kb * 32 + 8 (i / 4) + 4 h + i % 4 of the tile
         f32x16_t s[2];
@@ -191,35 +230,37 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[kb][i]);
         const float2 mh = both_halves(mt);
-        const float mn = fmaxf(m, fmaxf(mh.x, mh.y));
-        const float mz = mn == -INFINITY ? 0.f : mn;        // (no key seen yet, or scores of -inf alone)
-        // (nothing is summed yet where m is -inf: any finite factor will do)
-        const float corr = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mz) * a.scale2);
-        m = mn;
-        const float mc = mz * a.scale2;
-        float sum = 0.f;
+        mt = fmaxf(mh.x, mh.y);
+        // The maximum that the exponents are taken from moves only when a row's has grown by a factor of 2^8
+        // (p and its sums have room for that), so that most tiles leave the sums as they are.
+        if (__any((mt - m) * scale2 > 8.f)) {
+            const float mn = fmaxf(m, mt);
+            const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * scale2);
+            m = mn;
+            l *= corr;
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[db][i] *= corr;
+        }
+        const float mc = m == -INFINITY ? 0.f : m * scale2;      // (no key seen yet, or scores of -inf alone)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], a.scale2, -mc));
-                sum += s[kb][i];
-            }
-        l = l * corr + sum;
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[db][i] *= corr;
+            for (int i = 0; i < 16; ++i) s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], scale2, -mc));
         u32x4_t pf[4];
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) pf[ks][e] = pack2<BF16>(s[ks / 2][8 * (ks % 2) + 2 * e], s[ks / 2][8 * (ks % 2) + 2 * e + 1]);
+            for (int e = 0; e < 4; ++e) {
+                pf[ks][e] = pack2<BF16>(s[ks / 2][8 * (ks % 2) + 2 * e], s[ks / 2][8 * (ks % 2) + 2 * e + 1]);
+                l = add2<BF16>(pf[ks][e], l);
+            }
 
         // Rows of the tile that see different keys: a probability of zero must not meet an Inf or a NaN
         // of a key that its row does not see. Zero times V shows whether there is one.
         bool odd = false;
-        if (MASKED && a.causal) {
+        if (MASKED && causal) {
             f32x16_t z = f32x16_t{};
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
@@ -268,7 +309,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
     };
     // Two buffers: a tile is read while the next one is on its way. The wait is for this wave's own loads;
     // the barrier then says that every wave's have landed, and that no wave reads the other buffer any more.
-    auto next = [&](int base, char* sk, char* sv) {
+    auto next = [&](int base, char* sk, char* sv) __attribute__((always_inline)) {
         wait_loads();
         __syncthreads();
         if (base < end) stage_tile(base, sk, sv);
@@ -298,71 +339,109 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs a) {
     const float2 lh = both_halves(l);
     const float sum = lh.x + lh.y;
     if (r >= rows) return;
-    if (a.splits > 1) {
-        const int64_t item = ((int64_t)split * a.nq + u.row0 + qi) * (a.hkv * a.share) + hq;
+    const auto& b = *reread_args();
+    if (b.splits > 1) {
+        const int64_t item = ((int64_t)split * b.nq + u.row0 + qi) * (b.hkv * b.share) + hq;
         const bool seen = lim.lane > begin && begin < end;
-        if (h == 0) a.stat[item] = float2{m, seen ? sum : -1.f};
+        if (h == 0) b.stat[item] = float2{m, seen ? sum : -1.f};
         if (!seen) return;
-        float* op = a.part + item * a.d;
+        float* op = b.part + item * b.d;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int e = db * 32 + 8 * g + 4 * h;
-                if (e < a.d) *reinterpret_cast<f32x4_t*>(op + e) = f32x4_t{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+                if (e < b.d) *reinterpret_cast<f32x4_t*>(op + e) = f32x4_t{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
             }
         return;
     }
     const float inv = 1.0f / sum;
-    uint16_t* op = a.o + (int64_t)(u.row0 + qi) * a.o_row + hq * a.o_head;
+    uint16_t* op = b.o + (int64_t)(u.row0 + qi) * b.o_row + hq * b.o_head;
     const bool none = lim.lane == 0;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const int e = db * 32 + 8 * g + 4 * h;
-            if (e < a.d)
+            if (e < b.d)
                 *reinterpret_cast<uint2*>(op + e) = none ? uint2{0, 0} : uint2{pack2<BF16>(o[db][4 * g] * inv, o[db][4 * g + 1] * inv),
                                                                               pack2<BF16>(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv)};
         }
+#endif
 }
 
-// The splits' sums joined: sum_s w_s (p v)_s / sum_s w_s (sum p)_s, w_s = exp(max_s - max). 16 lanes a
-// row and head, 8 elements each. A split whose scores were all -inf has sums of 0 (or NaN): its weight
-// does not matter.
-template <bool BF16>
+// The splits' sums joined: sum_s w_s (p v)_s / sum_s w_s (sum p)_s, w_s = exp(max_s - max). A row and head
+// takes G groups of 16 lanes (8 elements each); the splits are dealt to the groups, whose sums are then
+// added in LDS in their order. A split whose scores were all -inf has sums of 0 (or NaN): its weight does
+// not matter. G = 1 for up to 16 splits, 16 beyond.
+constexpr int AT_MAX_SPLITS = 256, AT_FEW_SPLITS = 16;
+template <bool BF16, int G>
 __global__ __launch_bounds__(256) void k_attention_join(AttnArgs a) {
-    const int heads = a.hkv * a.share, e = (threadIdx.x & 15) * 8;
-    const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4, row = item / heads;
-    int64_t first = 0, last = a.nq;
-    if (a.q_off) {
-        first = a.q_off[0];
-        last = a.q_off[a.samples];
-    }
-    if (row >= a.nq || row < first || row >= last || e >= a.d) return;
-    const int64_t step = a.nq * heads;
-    float m = -INFINITY;
-    bool seen = false;
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 t = a.stat[s * step + item];
-        if (t.y == -1.f) continue;
-        m = fmaxf(m, t.x);
-        seen = true;
-    }
-    float acc[8] = {}, sum = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 t = a.stat[s * step + item];
-        if (t.y == -1.f) continue;
-        const float w = t.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((t.x - m) * a.scale2);
-        const f32x4_t* p = reinterpret_cast<const f32x4_t*>(a.part + (s * step + item) * a.d + e);
-        const f32x4_t x = p[0], y = p[1];
-        sum += w * t.y;
+    constexpr int ITEMS = 16 / G;
+    __shared__ float sW[ITEMS][G == 1 ? AT_FEW_SPLITS : AT_MAX_SPLITS];     // weights; -1: no key seen
+    __shared__ float sAcc[G][AT_MAX_D], sSum[G];
+    const int heads = a.hkv * a.share, lane = threadIdx.x & 15, group = threadIdx.x >> 4, e = lane * 8;
+    const int g = group % G, at = group / G, mine = threadIdx.x % (G * 16);
+    const int64_t item = (int64_t)blockIdx.x * ITEMS + at, row = item / heads, step = a.nq * heads;
+    const bool live = row < a.nq && !(a.q_off && (row < a.q_off[0] || row >= a.q_off[a.samples]));
+    float m = -INFINITY, sum = 0.f;
+    float2 t{-INFINITY, -1.f};
+    if (live && mine < a.splits) t = a.stat[mine * step + item];
+    m = t.x;
+    if constexpr (G == 1) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            acc[i] += w * x[i];
-            acc[4 + i] += w * y[i];
+        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 16));
+    } else {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        if ((threadIdx.x & 63) == 0) sSum[threadIdx.x >> 6] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(sSum[0], sSum[1]), fmaxf(sSum[2], sSum[3]));
+        __syncthreads();
+    }
+    const float w0 = t.y == -1.f ? -1.f : t.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((t.x - m) * a.scale2);
+    if (mine < (G == 1 ? AT_FEW_SPLITS : AT_MAX_SPLITS)) sW[at][mine] = w0;
+    // the sum of p over all splits, and whether any saw a key
+    sum = t.y == -1.f ? 0.f : w0 * t.y;
+    bool seen = t.y != -1.f;
+    if constexpr (G == 1) {
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 16);
+        seen = (__ballot(seen) >> (threadIdx.x & 48)) & 0xffff;
+        __syncthreads();
+    } else {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        if ((threadIdx.x & 63) == 0) sSum[threadIdx.x >> 6] = sum;
+        seen = __syncthreads_or(seen);
+        sum = (sSum[0] + sSum[1]) + (sSum[2] + sSum[3]);
+    }
+    float acc[8] = {};
+    if (live && e < a.d) {
+#pragma unroll 4
+        for (int s = g; s < a.splits; s += G) {
+            const float w = sW[at][s];
+            if (w == -1.f) continue;
+            const f32x4_t* p = reinterpret_cast<const f32x4_t*>(a.part + (s * step + item) * a.d + e);
+            const f32x4_t x = p[0], y = p[1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                acc[i] += w * x[i];
+                acc[4 + i] += w * y[i];
+            }
         }
     }
+    if constexpr (G > 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sAcc[g][e + i] = acc[i];
+        __syncthreads();
+        if (g != 0) return;
+#pragma unroll
+        for (int k = 1; k < G; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] += sAcc[k][e + i];
+    }
+    if (!live || e >= a.d) return;
     const float inv = 1.0f / sum;
     u32x4_t y{0, 0, 0, 0};
     if (seen)
@@ -384,11 +463,11 @@ AttnCut attn_cut(int64_t nq, int64_t nk, int samples, int hkv, int share) {
     c.units = ceil_div(nq * share, c.nw * 32) + (samples > 1 ? samples : 0);
     // splits: the rounds that the workgroups take on the device's slots, each as long as a split's tiles
     // and about three tiles' time of start and end
-    const int64_t busy = (ceil_div(nq * share, c.nw * 32) + (samples > 1 ? samples / 2 : 0)) * hkv, slots = c.nw == 1 ? 1024 : 512;
+    const int64_t busy = (ceil_div(nq * share, c.nw * 32) + (samples > 1 ? samples / 2 : 0)) * hkv, slots = 512;
     const int64_t tiles = ceil_div(ceil_div(nk, samples), AT_KEYS);
     c.splits = 1;
     int64_t best = ceil_div(busy, slots) * (tiles + 3);
-    for (int s = 2; s <= 128 && busy * s <= 4 * slots; ++s) {
+    for (int s = 2; s <= AT_MAX_SPLITS && busy * s <= 4 * slots; ++s) {
         const int64_t cost = ceil_div(busy * s, slots) * (ceil_div(tiles, s) + 3) + 3;
         if (cost < best) {
             best = cost;
@@ -450,8 +529,10 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
     hipStream_t s = as_stream(stream);
     auto go = [&](auto bf, auto dp, auto nw) {
         hipLaunchKernelGGL((k_attention<decltype(bf)::value, decltype(dp)::value, decltype(nw)::value>), grid, block, 0, s, a);
-        if (c.splits > 1)
-            hipLaunchKernelGGL((k_attention_join<decltype(bf)::value>), dim3((unsigned)ceil_div(nq * hq * 16, 256)), dim3(256), 0, s, a);
+        if (c.splits > AT_FEW_SPLITS)
+            hipLaunchKernelGGL((k_attention_join<decltype(bf)::value, 16>), dim3((unsigned)(nq * hq)), dim3(256), 0, s, a);
+        else if (c.splits > 1)
+            hipLaunchKernelGGL((k_attention_join<decltype(bf)::value, 1>), dim3((unsigned)ceil_div(nq * hq, 16)), dim3(256), 0, s, a);
     };
     using std::integral_constant;
     auto by_width = [&](auto bf) {
