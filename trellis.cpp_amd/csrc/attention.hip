@@ -175,26 +175,29 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
     // that belongs in its place. Rows past the sample's last key and pieces past d read as zeros (out of
     // the buffer's range).
     constexpr int LOADS = TILE / 1024 / NW;
-    int k_at[LOADS], v_at[LOADS];            // a lane's byte offsets within the tile's rows
+    // A lane's byte offsets within the tile's rows; those of loads PERIOD apart differ by whole rows alone.
+    constexpr int LOAD_ROWS = NW * (1024 / (DP * 2)), PERIOD = LOAD_ROWS >= 16 ? 1 : 16 / LOAD_ROWS;
+    constexpr int NOWHERE = 1 << 30;         // past every tile's rows
+    int k_at[PERIOD], v_at[PERIOD];
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
+    for (int i = 0; i < PERIOD; ++i) {
         const int key = (i * NW + wave) * (1024 / (DP * 2)) + lane / P;
         const int kp = k_piece<DP>(key, lane % P) / 16 % P, vp = v_piece<DP>(key, lane % P) / 16 % P;
-        k_at[i] = kp * 8 < a.d ? key * k_bytes + kp * 16 : -1;
-        v_at[i] = vp * 8 < a.d ? key * v_bytes + vp * 16 : -1;
+        k_at[i] = kp * 8 < a.d ? key * k_bytes + kp * 16 : NOWHERE;
+        v_at[i] = vp * 8 < a.d ? key * v_bytes + vp * 16 : NOWHERE;
         asm volatile("" : "+v"(k_at[i]), "+v"(v_at[i]));       // (computed here, not in every tile)
     }
-    auto stage = [&](const char* p, int bytes, int base, const int (&at)[LOADS], char* s) __attribute__((always_inline)) {
+    auto stage = [&](const char* p, int bytes, int base, const int (&at)[PERIOD], char* s) __attribute__((always_inline)) {
         const int n = min(AT_KEYS, lk - base);
         const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(p + (int64_t)base * bytes), (short)0, n * bytes, 0x00027000);
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(s + (i * NW + wave) * 1024), 16, at[i], 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(s + (i * NW + wave) * 1024), 16,
+                                                     at[i % PERIOD] + i / PERIOD * PERIOD * LOAD_ROWS * bytes, 0, 0, 0);
     };
-    auto stage_tile = [&](int base, char* sk, char* sv) __attribute__((always_inline)) {
-        stage(kp, k_bytes, base, k_at, sk);
-        stage(vp, v_bytes, base, v_at, sv);
-    };
+    // K or V of the tile at key base
+    auto stage_k = [&](int base, char* s) __attribute__((always_inline)) { stage(kp, k_bytes, base, k_at, s); };
+    auto stage_v = [&](int base, char* s) __attribute__((always_inline)) { stage(vp, v_bytes, base, v_at, s); };
 
     f32x16_t o[DB];
 #pragma unroll
@@ -205,10 +208,9 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
     const int tiles = (wg_end + AT_KEYS - 1) / AT_KEYS, per = (tiles + a.splits - 1) / a.splits;
     const int begin = split * per * AT_KEYS, end = min(wg_end, begin + per * AT_KEYS);
     const bool causal = a.causal;
-    auto attend = [&](auto masked_tile, int base, const char* sK, const char* sV) __attribute__((always_inline)) {
-        constexpr bool MASKED = decltype(masked_tile)::value;
-        // scores: s[kb][i] is key kb * 32 + 8 (i / 4) + 4 h + i % 4 of the tile
-        f32x16_t s[2];
+
+    // scores: s[kb][i] is key kb * 32 + 8 (i / 4) + 4 h + i % 4 of the tile
+    auto scores = [&](const char* sK, f32x16_t (&s)[2]) __attribute__((always_inline)) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             s[kb] = f32x16_t{};
@@ -216,23 +218,12 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
             for (int ks = 0; ks < KS; ++ks)
                 s[kb] = mfma32<BF16>(*reinterpret_cast<const u32x4_t*>(sK + k_piece<DP>(kb * 32 + r32, ks * 2 + h)), qf[ks], s[kb]);
         }
-        if constexpr (MASKED) {
-            const int left = lim.lane - base - 4 * h;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    s[kb][i] = kb * 32 + 8 * (i / 4) + i % 4 < left ? s[kb][i] : -INFINITY;
-        }
-        float mt = s[0][0];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[kb][i]);
+    };
+    // The maximum that the exponents are taken from moves only when a row's has grown by a factor of 2^8 (p
+    // and its sums have room for that), so that most tiles leave the sums as they are.
+    auto raise = [&](float mt) __attribute__((always_inline)) {
         const float2 mh = both_halves(mt);
         mt = fmaxf(mh.x, mh.y);
-        // The maximum that the exponents are taken from moves only when a row's has grown by a factor of 2^8
-        // (p and its sums have room for that), so that most tiles leave the sums as they are.
         if (__any((mt - m) * scale2 > 8.f)) {
             const float mn = fmaxf(m, mt);
             const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * scale2);
@@ -243,12 +234,22 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[db][i] *= corr;
         }
+    };
+    auto top = [&](const f32x16_t (&s)[2]) __attribute__((always_inline)) {
+        float mt = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[kb][i]);
+        return mt;
+    };
+    // s becomes p, pf the second product's operand
+    auto exponents = [&](f32x16_t (&s)[2], u32x4_t (&pf)[4]) __attribute__((always_inline)) {
         const float mc = m == -INFINITY ? 0.f : m * scale2;      // (no key seen yet, or scores of -inf alone)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], scale2, -mc));
-        u32x4_t pf[4];
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
@@ -256,11 +257,30 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
                 pf[ks][e] = pack2<BF16>(s[ks / 2][8 * (ks % 2) + 2 * e], s[ks / 2][8 * (ks % 2) + 2 * e + 1]);
                 l = add2<BF16>(pf[ks][e], l);
             }
-
+    };
+    auto weigh = [&](const char* sV, const u32x4_t (&pf)[4]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int db = 0; db < DB; ++db) o[db] = mfma32<BF16>(v_operand<DP>(sV, ks, db, lane), pf[ks], o[db]);
+    };
+    // A tile that not every row of the workgroup sees whole.
+    auto attend_masked = [&](int base, const char* sK, const char* sV) __attribute__((always_inline)) {
+        f32x16_t s[2];
+        u32x4_t pf[4];
+        scores(sK, s);
+        const int left = lim.lane - base - 4 * h;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                s[kb][i] = kb * 32 + 8 * (i / 4) + i % 4 < left ? s[kb][i] : -INFINITY;
+        raise(top(s));
+        exponents(s, pf);
         // Rows of the tile that see different keys: a probability of zero must not meet an Inf or a NaN
         // of a key that its row does not see. Zero times V shows whether there is one.
         bool odd = false;
-        if (MASKED && causal) {
+        if (causal) {
             f32x16_t z = f32x16_t{};
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
@@ -276,7 +296,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
                 u32x4_t vf = v_operand<DP>(sV, ks, db, lane);
-                if (MASKED && odd) {
+                if (odd) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         if (nonfinite16<BF16>(vf[e])) vf[e] &= 0xffff0000u;
@@ -285,7 +305,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
                 }
                 o[db] = mfma32<BF16>(vf, pf[ks], o[db]);
             }
-        if (MASKED && odd) {      // the values left out, key by key, for the rows that see them
+        if (odd) {      // the values left out, key by key, for the rows that see them
             for (int key = 0; key < AT_KEYS; ++key) {
                 float p = 0.f;
 #pragma unroll
@@ -307,33 +327,89 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
             }
         }
     };
-    // Two buffers: a tile is read while the next one is on its way. The wait is for this wave's own loads;
-    // the barrier then says that every wave's have landed, and that no wave reads the other buffer any more.
-    auto next = [&](int base, char* sk, char* sv) __attribute__((always_inline)) {
+    // The wait is for this wave's own loads; the barrier then says that every wave's have landed, and that
+    // no wave reads any more what was read before it.
+    auto landed = []() __attribute__((always_inline)) {
         wait_loads();
         __syncthreads();
-        if (base < end) stage_tile(base, sk, sv);
     };
-    if (begin < end) stage_tile(begin, sK0, sV0);
-    // tiles that every row of the workgroup sees whole, then the others
+    // Whole tiles: the scores of the next tile are formed while the exponents of this one are, and its
+    // maximum while this one's values are weighed, so that the matrix cores and the vector units both have
+    // work from one wave, in the order written here; operands are read four products ahead. Two buffers
+    // each for K and V; K is a tile ahead of V.
     const int whole = min(end, limit(query(tile0)));
+    auto k_operand = [&](const char* sK, int t) __attribute__((always_inline)) {
+        return *reinterpret_cast<const u32x4_t*>(sK + k_piece<DP>((t & 1) * 32 + r32, (t >> 1) * 2 + h));
+    };
+    auto step = [&](int base, char* k_this, const char* k_next, const char* v_this, char* v_next, f32x16_t (&s)[2],
+                    f32x16_t (&sn)[2]) __attribute__((always_inline)) {
+        constexpr int AHEAD = 4, NK = 2 * KS, PAIRS = 16 / NK, NV = 4 * DB;
+        u32x4_t pf[4], ring[AHEAD];
+        landed();
+        if (base + 2 * AT_KEYS < end) stage_k(base + 2 * AT_KEYS, k_this);
+        if (base + AT_KEYS < end) stage_v(base + AT_KEYS, v_next);
+        const float mc = m == -INFINITY ? 0.f : m * scale2;
+#pragma unroll
+        for (int t = 0; t < AHEAD; ++t) ring[t] = k_operand(k_next, t);
+#pragma unroll
+        for (int t = 0; t < NK; ++t) {
+            sn[t & 1] = mfma32<BF16>(ring[t % AHEAD], qf[t >> 1], t < 2 ? f32x16_t{} : sn[t & 1]);
+            if (t + AHEAD < NK) ring[t % AHEAD] = k_operand(k_next, t + AHEAD);
+            else ring[t % AHEAD] = v_operand<DP>(v_this, (t + AHEAD - NK) / DB, (t + AHEAD - NK) % DB, lane);
+#pragma unroll
+            for (int e = t * PAIRS; e < (t + 1) * PAIRS; ++e) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[e / 8][2 * (e % 8)], scale2, -mc));
+                const float y = __builtin_amdgcn_exp2f(fmaf(s[e / 8][2 * (e % 8) + 1], scale2, -mc));
+                pf[e / 4][e % 4] = pack2<BF16>(x, y);
+                l = add2<BF16>(pf[e / 4][e % 4], l);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        float mt = sn[0][0];
+#pragma unroll
+        for (int t = 0; t < NV; ++t) {
+            o[t % DB] = mfma32<BF16>(ring[t % AHEAD], pf[t / DB], o[t % DB]);
+            if (t + AHEAD < NV) ring[t % AHEAD] = v_operand<DP>(v_this, (t + AHEAD) / DB, (t + AHEAD) % DB, lane);
+#pragma unroll
+            for (int i = t * 32 / NV; i < (t + 1) * 32 / NV; ++i) mt = fmaxf(mt, sn[i / 16][i % 16]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        raise(mt);
+    };
     int base = begin;
     bool second = false;
-    while (base + AT_KEYS <= whole) {
-        next(base + AT_KEYS, sK1, sV1);
-        attend(std::false_type{}, base, sK0, sV0);
-        base += AT_KEYS;
-        if (base + AT_KEYS > whole) {
-            second = true;
-            break;
-        }
-        next(base + AT_KEYS, sK0, sV0);
-        attend(std::false_type{}, base, sK1, sV1);
-        base += AT_KEYS;
+    if (begin < end) {
+        stage_k(begin, sK0);
+        stage_v(begin, sV0);
+        if (begin + AT_KEYS < end) stage_k(begin + AT_KEYS, sK1);
     }
+    if (base + AT_KEYS <= whole) {
+        f32x16_t s0[2], s1[2];
+        landed();
+        scores(sK0, s0);
+        raise(top(s0));
+        for (; base + 3 * AT_KEYS <= whole; base += 2 * AT_KEYS) {
+            step(base, sK0, sK1, sV0, sV1, s0, s1);
+            step(base + AT_KEYS, sK1, sK0, sV1, sV0, s1, s0);
+        }
+        landed();
+        if (base + 2 * AT_KEYS < end) stage_k(base + 2 * AT_KEYS, sK0);
+        if (base + AT_KEYS < end) stage_v(base + AT_KEYS, sV1);
+        u32x4_t pf[4];
+        exponents(s0, pf);
+        weigh(sV0, pf);
+        base += AT_KEYS;
+        second = true;
+    }
+    // the others, a whole one among them at times (K and V of the first are on their way, K of the second too)
     for (; base < end; base += AT_KEYS, second = !second) {
-        next(base + AT_KEYS, second ? sK0 : sK1, second ? sV0 : sV1);
-        if (base < lim.hi) attend(std::true_type{}, base, second ? sK1 : sK0, second ? sV1 : sV0);
+        landed();
+        if (base < lim.hi) attend_masked(base, second ? sK1 : sK0, second ? sV1 : sV0);
+        if (base + AT_KEYS < end) stage_v(base + AT_KEYS, second ? sV0 : sV1);
+        if (base + 2 * AT_KEYS < end) {
+            __syncthreads();
+            stage_k(base + 2 * AT_KEYS, second ? sK1 : sK0);
+        }
     }
 
     const float2 lh = both_halves(l);
