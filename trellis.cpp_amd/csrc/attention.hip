@@ -35,11 +35,30 @@ struct AttnArgs {
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;   // strides in elements
     const int32_t *q_off, *k_off;
     int64_t nq, nk;                           // below 2^31, nq * share too
-    int samples, hkv, share, d, causal, units, splits;
+    int samples, hkv, share, d, causal;
+    int units;                                // of rows, a key head
+    int whole, splits;                        // the first `whole` of units * hkv see their keys at once, the others in splits
     float scale2;                             // scale * log2(e)
-    float* part;                              // splits > 1: [split][nq * hq][d] sums of p v, then
-    float2* stat;                             // [split][nq * hq] maximum and sum of p (-1: no key seen)
+    float* part;                              // [unit past whole][split][row][d] sums of p v, and
+    float2* stat;                             // [unit past whole][split][row] maximum and sum of p (-1: no key seen)
 };
+
+// A unit of `ROWS` rows (query, head of the group) of one key head.
+struct AttnUnit {
+    PackedUnit u;      // its sample (-1: none)
+    int head, row0, rows;   // the key head, its first row, the sample's rows
+};
+// Units go by head, then by row; with causal the last rows of a sample, which see most, come first.
+template <int ROWS, class Args>
+__device__ __forceinline__ AttnUnit attn_unit(const Args& a, int w) {
+    AttnUnit t;
+    t.head = (unsigned)w / (unsigned)a.units;
+    const int unit = w - t.head * a.units;
+    t.u = packed_unit(a.q_off, a.samples, (int)a.nq, a.share, ROWS, unit);
+    t.row0 = (a.causal ? t.u.count - 1 - (unit - t.u.first) : unit - t.u.first) * ROWS;
+    t.rows = t.u.rows * a.share;
+    return t;
+}
 
 template <bool BF16>
 __device__ __forceinline__ f32x16_t mfma32(const u32x4_t& a, const u32x4_t& b, const f32x16_t& c) {
@@ -136,13 +155,19 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
     constexpr int KS = DP / 16, DB = DP / 32, P = DP / 8, ROWS = NW * 32;
     constexpr int TILE = AT_KEYS * DP * 2;
     __shared__ __attribute__((aligned(16))) char sK0[TILE], sK1[TILE], sV0[TILE], sV1[TILE];
-    const int split = blockIdx.x % a.splits, hu = blockIdx.x / a.splits;
-    const int head = hu / a.units, unit = hu - head * a.units;
-    const PackedUnit u = packed_unit(a.q_off, a.samples, (int)a.nq, a.share, ROWS, unit);
+    int work = blockIdx.x, split = 0, splits = 1;
+    if (work >= a.whole) {
+        const int past = work - a.whole;
+        splits = a.splits;
+        work = a.whole + (unsigned)past / (unsigned)splits;
+        split = (unsigned)past % (unsigned)splits;
+    }
+    const AttnUnit t = attn_unit<ROWS>(a, work);
+    const PackedUnit& u = t.u;
+    const int head = t.head, rows = t.rows, tile0 = t.row0;
     if (u.sample < 0) return;
     int krow0, lk;
     packed_rows(a.k_off, u.sample, (int)a.nk, krow0, lk);
-    const int rows = u.rows * a.share, tile0 = (unit - u.first) * ROWS;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
 
     // rows past the sample's last are copies of it that are not stored
@@ -205,7 +230,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
     float m = -INFINITY, l = 0.f;
 
     // this split's share of the workgroup's tiles
-    const int tiles = (wg_end + AT_KEYS - 1) / AT_KEYS, per = (tiles + a.splits - 1) / a.splits;
+    const int tiles = (wg_end + AT_KEYS - 1) / AT_KEYS, per = (unsigned)(tiles + splits - 1) / (unsigned)splits;
     const int begin = split * per * AT_KEYS, end = min(wg_end, begin + per * AT_KEYS);
     const bool causal = a.causal;
 
@@ -416,8 +441,8 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
     const float sum = lh.x + lh.y;
     if (r >= rows) return;
     const auto& b = *reread_args();
-    if (b.splits > 1) {
-        const int64_t item = ((int64_t)split * b.nq + u.row0 + qi) * (b.hkv * b.share) + hq;
+    if (splits > 1) {
+        const int64_t item = ((int64_t)(work - b.whole) * splits + split) * ROWS + (r - tile0);
         const bool seen = lim.lane > begin && begin < end;
         if (h == 0) b.stat[item] = float2{m, seen ? sum : -1.f};
         if (!seen) return;
@@ -451,15 +476,20 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
 // added in LDS in their order. A split whose scores were all -inf has sums of 0 (or NaN): its weight does
 // not matter. G = 1 for up to 16 splits, 16 beyond.
 constexpr int AT_MAX_SPLITS = 256, AT_FEW_SPLITS = 16;
-template <bool BF16, int G>
+template <bool BF16, int G, int ROWS>
 __global__ __launch_bounds__(256) void k_attention_join(AttnArgs a) {
-    constexpr int ITEMS = 16 / G;
+    constexpr int ITEMS = 16 / G, BLOCKS = ROWS / ITEMS;
     __shared__ float sW[ITEMS][G == 1 ? AT_FEW_SPLITS : AT_MAX_SPLITS];     // weights; -1: no key seen
     __shared__ float sAcc[G][AT_MAX_D], sSum[G];
-    const int heads = a.hkv * a.share, lane = threadIdx.x & 15, group = threadIdx.x >> 4, e = lane * 8;
+    const int lane = threadIdx.x & 15, group = threadIdx.x >> 4, e = lane * 8;
     const int g = group % G, at = group / G, mine = threadIdx.x % (G * 16);
-    const int64_t item = (int64_t)blockIdx.x * ITEMS + at, row = item / heads, step = a.nq * heads;
-    const bool live = row < a.nq && !(a.q_off && (row < a.q_off[0] || row >= a.q_off[a.samples]));
+    const int past = blockIdx.x / BLOCKS, row = blockIdx.x % BLOCKS * ITEMS + at;
+    const AttnUnit w = attn_unit<ROWS>(a, a.whole + past);
+    const int r = w.row0 + row;
+    if (w.u.sample < 0 || w.row0 + row - at >= w.rows) return;
+    const bool live = r < w.rows;
+    const int64_t item = (int64_t)past * a.splits * ROWS + row;
+    constexpr int step = ROWS;
     float m = -INFINITY, sum = 0.f;
     float2 t{-INFINITY, -1.f};
     if (live && mine < a.splits) t = a.stat[mine * step + item];
@@ -523,34 +553,50 @@ __global__ __launch_bounds__(256) void k_attention_join(AttnArgs a) {
     if (seen)
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-    *reinterpret_cast<u32x4_t*>(a.o + row * a.o_row + (item - row * heads) * a.o_head + e) = y;
+    const int qi = (unsigned)r / (unsigned)a.share, hq = w.head * a.share + r - qi * a.share;
+    *reinterpret_cast<u32x4_t*>(a.o + (int64_t)(w.u.row0 + qi) * a.o_row + hq * a.o_head + e) = y;
 }
 
-// How a call is cut: waves of a workgroup (32 rows each), units of rows, splits of the keys.
+// How a call is cut: waves of a workgroup (32 rows each), units of rows a key head, how many of them see
+// their keys at once, splits of the others' keys.
 struct AttnCut {
     int nw, splits;
-    int64_t units;
+    int64_t units, whole;
 };
 
-AttnCut attn_cut(int64_t nq, int64_t nk, int samples, int hkv, int share) {
+AttnCut attn_cut(int64_t nq, int64_t nk, int samples, int hkv, int share, int d, bool causal) {
     AttnCut c;
     // one wave where a sample has at most its 32 rows (by the mean: the host does not know the lengths)
     c.nw = ceil_div(nq, samples) * share <= 32 ? 1 : 4;
-    c.units = ceil_div(nq * share, c.nw * 32) + (samples > 1 ? samples : 0);
-    // splits: the rounds that the workgroups take on the device's slots, each as long as a split's tiles
-    // and about three tiles' time of start and end
-    const int64_t busy = (ceil_div(nq * share, c.nw * 32) + (samples > 1 ? samples / 2 : 0)) * hkv, slots = 512;
+    const int64_t units = ceil_div(nq * share, c.nw * 32);
+    c.units = units + (samples > 1 ? samples : 0);
+    // The device holds `slots` workgroups at once (by registers and LDS); a round of fewer takes half of a full
+    // one's time and what its share of the slots adds. Where there are not `slots` units, their keys are
+    // split; where one sample's units leave a last round partly empty, that round's are. (Several samples,
+    // or causal ones, have units of unequal length, which fill each other's gaps.) Time is counted in
+    // tiles: about three for a workgroup's start and end, six for the join.
+    const int64_t busy = (units + (samples > 1 ? samples / 2 : 0)) * hkv;
+    const int64_t slots = 256 * (d > 64 ? 2 : c.nw == 1 ? 5 : 3);
     const int64_t tiles = ceil_div(ceil_div(nk, samples), AT_KEYS);
+    c.whole = c.units * hkv;
     c.splits = 1;
-    int64_t best = ceil_div(busy, slots) * (tiles + 3);
-    for (int s = 2; s <= AT_MAX_SPLITS && busy * s <= 4 * slots; ++s) {
-        const int64_t cost = ceil_div(busy * s, slots) * (ceil_div(tiles, s) + 3) + 3;
+    const int64_t full = busy / slots * slots;
+    if (busy == full || (full > 0 && (samples > 1 || causal))) return c;
+    auto rounds = [&](int64_t n, int64_t length) { return (n / slots + (n % slots ? 0.5 + 0.5 * (double)(n % slots) / slots : 0.)) * (length + 3); };
+    double best = rounds(busy - full, tiles);
+    for (int s = 2; s <= AT_MAX_SPLITS && (busy - full) * s <= 2 * slots; ++s) {
+        const double cost = rounds((busy - full) * s, ceil_div(tiles, s)) + 6;
         if (cost < best) {
             best = cost;
             c.splits = s;
+            c.whole = full;
         }
     }
     return c;
+}
+
+size_t attn_workspace(const AttnCut& c, int hkv, int d) {
+    return c.splits == 1 ? 0 : (size_t)(c.units * hkv - c.whole) * c.splits * c.nw * 32 * (d * sizeof(float) + sizeof(float2));
 }
 
 }  // namespace
@@ -560,8 +606,8 @@ using namespace tsp;
 
 extern "C" size_t tsp_attention_workspace_bytes(int64_t nq, int64_t nk, int samples, int hq, int hkv, int d) {
     if (nq <= 0 || nq >= (1ll << 31) || nk < 0 || nk >= (1ll << 31) - (1ll << 16) || samples <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || d <= 0) return 0;
-    const AttnCut c = attn_cut(nq, nk, samples, hkv, hq / hkv);
-    return c.splits == 1 ? 0 : (size_t)c.splits * nq * hq * ((size_t)d * sizeof(float) + sizeof(float2));
+    return std::max(attn_workspace(attn_cut(nq, nk, samples, hkv, hq / hkv, d, false), hkv, d),
+                    attn_workspace(attn_cut(nq, nk, samples, hkv, hq / hkv, d, true), hkv, d));
 }
 
 extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_heads* v, int dtype, int64_t nq, int64_t nk, int hq,
@@ -588,27 +634,28 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
     TSP_REQUIRE(heads_apart(*out, nq, hq, d), TSP_ERR_INVALID, "tsp_attention: the output's heads overlap");
     TSP_REQUIRE(out->data != kk.data && out->data != vv.data && out->data != q->data, TSP_ERR_INVALID, "tsp_attention: out must not alias q, k or v");
     const int share = hq / hkv;
-    const AttnCut c = attn_cut(nq, nk, samples, hkv, share);
-    const int64_t blocks = c.units * hkv * c.splits;
+    const AttnCut c = attn_cut(nq, nk, samples, hkv, share, d, causal != 0);
+    const int64_t past = c.units * hkv - c.whole, blocks = c.whole + past * c.splits;
     TSP_REQUIRE(blocks * c.nw * 64 < (1ll << 32) && nq * share < (1ll << 31) - 1024, TSP_ERR_INVALID, "tsp_attention: too many rows");
-    const size_t need = tsp_attention_workspace_bytes(nq, nk, samples, hq, hkv, d);
+    const size_t need = attn_workspace(c, hkv, d);
     TSP_REQUIRE(need == 0 || d_workspace, TSP_ERR_INVALID, "tsp_attention: null workspace");
     TSP_REQUIRE(workspace_bytes >= need, TSP_ERR_WORKSPACE, "tsp_attention: workspace of %zu bytes, needs %zu", workspace_bytes, need);
     TSP_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0, TSP_ERR_INVALID, "tsp_attention: workspace not 16-byte aligned");
     float* part = need ? static_cast<float*>(d_workspace) : nullptr;
-    float2* stat = need ? reinterpret_cast<float2*>(part + (int64_t)c.splits * nq * hq * d) : nullptr;
+    float2* stat = need ? reinterpret_cast<float2*>(part + past * c.splits * c.nw * 32 * d) : nullptr;
     const AttnArgs a{static_cast<const uint16_t*>(q->data), static_cast<const uint16_t*>(kk.data), static_cast<const uint16_t*>(vv.data),
                      static_cast<uint16_t*>(out->data), q->row_stride, q->head_stride, kk.row_stride, kk.head_stride, vv.row_stride,
                      vv.head_stride, out->row_stride, out->head_stride, d_q_offsets, d_k_offsets, nq, nk, samples, hkv, share, d,
-                     causal ? 1 : 0, (int)c.units, c.splits, scale * 1.44269504088896340736f, part, stat};
+                     causal ? 1 : 0, (int)c.units, (int)c.whole, c.splits, scale * 1.44269504088896340736f, part, stat};
     const dim3 grid((unsigned)blocks), block(c.nw * 64);
     hipStream_t s = as_stream(stream);
     auto go = [&](auto bf, auto dp, auto nw) {
         hipLaunchKernelGGL((k_attention<decltype(bf)::value, decltype(dp)::value, decltype(nw)::value>), grid, block, 0, s, a);
+        constexpr int ROWS = decltype(nw)::value * 32;
         if (c.splits > AT_FEW_SPLITS)
-            hipLaunchKernelGGL((k_attention_join<decltype(bf)::value, 16>), dim3((unsigned)(nq * hq)), dim3(256), 0, s, a);
+            hipLaunchKernelGGL((k_attention_join<decltype(bf)::value, 16, ROWS>), dim3((unsigned)(past * ROWS)), dim3(256), 0, s, a);
         else if (c.splits > 1)
-            hipLaunchKernelGGL((k_attention_join<decltype(bf)::value, 1>), dim3((unsigned)ceil_div(nq * hq, 16)), dim3(256), 0, s, a);
+            hipLaunchKernelGGL((k_attention_join<decltype(bf)::value, 1, ROWS>), dim3((unsigned)(past * ROWS / 16)), dim3(256), 0, s, a);
     };
     using std::integral_constant;
     auto by_width = [&](auto bf) {
