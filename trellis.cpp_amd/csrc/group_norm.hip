@@ -36,8 +36,59 @@ __device__ __forceinline__ int unit_rows(const PackedUnit& u, int unit, int per,
 
 __device__ __forceinline__ float act(float y, int silu) { return silu ? y / (1.0f + expf(-y)) : y; }
 
-// One group of one unit a workgroup. Sums are of x minus the group's first value, so that a mean far
-// from zero does not swallow the variance.
+// Eight consecutive values (16-byte accesses; the address is aligned).
+template <int DT>
+__device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8]) {
+    if constexpr (DT == TSP_F32) {
+        const f32x4_t* x = reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + i);
+        const f32x4_t a = x[0], b = x[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
+    } else {
+        const u32x4_t a = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint16_t lo = (uint16_t)(a[e] & 0xffffu), hi = (uint16_t)(a[e] >> 16);
+            v[2 * e] = DT == TSP_BF16 ? bf16_bits_to_f32(lo) : f16_bits_to_f32(lo);
+            v[2 * e + 1] = DT == TSP_BF16 ? bf16_bits_to_f32(hi) : f16_bits_to_f32(hi);
+        }
+    }
+}
+template <int DT>
+__device__ __forceinline__ void store8(void* p, int64_t i, const float (&v)[8]) {
+    if constexpr (DT == TSP_F32) {
+        f32x4_t* y = reinterpret_cast<f32x4_t*>(static_cast<float*>(p) + i);
+        y[0] = f32x4_t{v[0], v[1], v[2], v[3]};
+        y[1] = f32x4_t{v[4], v[5], v[6], v[7]};
+    } else {
+        u32x4_t a;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            a[e] = DT == TSP_BF16 ? f32x2_to_bf16x2_bits(v[2 * e], v[2 * e + 1])
+                                  : f32_to_f16_bits(v[2 * e]) | ((uint32_t)f32_to_f16_bits(v[2 * e + 1]) << 16);
+        *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(p) + i) = a;
+    }
+}
+
+// Lanes that share a group's sums, a power of two: all threads where there are few groups.
+__device__ __forceinline__ int lanes_a_group(int groups) {
+    int l = 64;
+    while (l > 1 && l * groups > GN_NT) l >>= 1;
+    return l;
+}
+__device__ __forceinline__ float sum_over(float v, int lanes) {
+    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// Sums are of x minus the group's first value in the unit, so that a mean far from zero does not swallow
+// the variance.
+__device__ __forceinline__ float2 unit_stat(float s, float q, float shift, float count) {
+    const float m = s / count;
+    return float2{shift + m, fmaxf(q - s * m, 0.f)};
+}
+
+// One group of one unit a workgroup, element by element: any width and alignment.
 template <int XDT>
 __global__ __launch_bounds__(GN_NT) void k_gn_stats(GnArgs a) {
     __shared__ float2 sPart[GN_NT / 64];
@@ -66,31 +117,102 @@ __global__ __launch_bounds__(GN_NT) void k_gn_stats(GnArgs a) {
             S += sPart[w].x;
             Q += sPart[w].y;
         }
-        const float m = S / (float)cnt;
-        a.part[(int64_t)blockIdx.x * a.groups + g] = float2{shift + m, fmaxf(Q - S * m, 0.f)};
+        a.part[(int64_t)blockIdx.x * a.groups + g] = unit_stat(S, Q, shift, (float)cnt);
     }
 }
 
-// Mean and 1 / sqrt(var + eps) of every group of the unit's sample, into LDS.
-__device__ __forceinline__ void join_units(const GnArgs& a, const PackedUnit& u, float* sMean, float* sRstd) {
-    const int cg = a.c / a.groups;
-    const float total = (float)u.rows * (float)cg;
-    for (int g = threadIdx.x; g < a.groups; g += GN_NT) {
-        const float2* p = a.part + (int64_t)u.first * a.groups + g;
-        // (the units' means less the first one's: of equal values the mean is that value)
-        const float m0 = p->x;
-        float m = 0.f;
-        for (int i = 1; i < u.count; ++i)
-            m += (p[(int64_t)i * a.groups].x - m0) * ((float)min(a.per, u.rows - i * a.per) * (float)cg / total);
-        m += m0;
-        float q = 0.f;
-        for (int i = 0; i < u.count; ++i) {
-            const float2 t = p[(int64_t)i * a.groups];
-            const float d = t.x - m;
-            q += t.y + d * d * (float)min(a.per, u.rows - i * a.per) * (float)cg;
+// All groups of one unit a workgroup: a thread keeps the sums of eight channels (of one value, PER = 1,
+// where they lie in one group, else of each) over every lanes-th row; they meet in LDS.
+template <int XDT, int PER>
+__global__ __launch_bounds__(GN_NT) void k_gn_stats_vec(GnArgs a) {
+    __shared__ float2 sSum[GN_NT * PER];
+    const PackedUnit u = packed_unit(a.offsets, a.samples, (int)a.n, 1, a.per, blockIdx.x);
+    if (u.sample < 0) return;
+    int64_t row;
+    const int rows = unit_rows(u, blockIdx.x, a.per, row);
+    const int cols = a.c / 8, lanes = GN_NT / cols, cg = a.c / a.groups;
+    const int lane = threadIdx.x / cols, col = threadIdx.x - lane * cols;
+    const bool live = lane < lanes;
+    float s[PER] = {}, q[PER] = {}, shift[PER];
+    if (live) {
+#pragma unroll
+        for (int k = 0; k < PER; ++k)
+            shift[k] = Elem<XDT>::load(reinterpret_cast<const typename Elem<XDT>::storage*>(a.x), row * a.c + (col * 8 + k) / cg * cg);
+        int r = lane;
+        constexpr int DEEP = 4;       // rows in flight
+        for (; r + (DEEP - 1) * lanes < rows; r += DEEP * lanes) {
+            float x[DEEP][8];
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i) load8<XDT>(a.x, (row + r + i * lanes) * a.c + col * 8, x[i]);
+#pragma unroll
+            for (int i = 0; i < DEEP; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int k = PER == 1 ? 0 : e;
+                    const float d = x[i][e] - shift[k];
+                    s[k] += d;
+                    q[k] += d * d;
+                }
         }
-        sMean[g] = m;
-        sRstd[g] = 1.0f / sqrtf(q / total + a.eps);
+        for (; r < rows; r += lanes) {
+            float x[8];
+            load8<XDT>(a.x, (row + r) * a.c + col * 8, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int k = PER == 1 ? 0 : e;
+                const float d = x[e] - shift[k];
+                s[k] += d;
+                q[k] += d * d;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < PER; ++k) sSum[(lane * cols + col) * PER + k] = float2{s[k], q[k]};
+    }
+    __syncthreads();
+    const int lg = lanes_a_group(a.groups), sub = threadIdx.x & (lg - 1), slots = cg * PER / 8;
+    for (int g0 = 0; g0 < a.groups; g0 += GN_NT / lg) {
+        const int g = g0 + threadIdx.x / lg;
+        float S = 0.f, Q = 0.f;
+        if (g < a.groups)
+            for (int e = sub; e < lanes * slots; e += lg) {
+                const int l = e / slots;
+                const float2 t = sSum[l * cols * PER + g * slots + (e - l * slots)];
+                S += t.x;
+                Q += t.y;
+            }
+        S = sum_over(S, lg);
+        Q = sum_over(Q, lg);
+        if (g < a.groups && sub == 0)
+            a.part[(int64_t)blockIdx.x * a.groups + g] =
+                unit_stat(S, Q, Elem<XDT>::load(reinterpret_cast<const typename Elem<XDT>::storage*>(a.x), row * a.c + g * cg),
+                          (float)rows * (float)cg);
+    }
+}
+
+// Mean and 1 / sqrt(var + eps) of every group of the unit's sample, into LDS: the units' means and squared
+// deviations joined about the first unit's mean.
+__device__ __forceinline__ void join_units(const GnArgs& a, const PackedUnit& u, float* sMean, float* sRstd) {
+    const float cg = (float)(a.c / a.groups), total = (float)u.rows * cg;
+    const int lg = lanes_a_group(a.groups), sub = threadIdx.x & (lg - 1);
+    for (int g0 = 0; g0 < a.groups; g0 += GN_NT / lg) {
+        const int g = g0 + threadIdx.x / lg;
+        const float2* p = a.part + (int64_t)u.first * a.groups + min(g, a.groups - 1);
+        const float m0 = p->x;
+        float s = 0.f, q = 0.f;
+#pragma unroll 8
+        for (int i = sub; i < u.count; i += lg) {
+            const float2 t = p[(int64_t)i * a.groups];
+            const float d = t.x - m0, n = (float)min(a.per, u.rows - i * a.per) * cg;
+            s += n * d;
+            q += t.y + n * d * d;
+        }
+        s = sum_over(s, lg);
+        q = sum_over(q, lg);
+        const float m = s / total;
+        if (g < a.groups && sub == 0) {
+            sMean[g] = m0 + m;
+            sRstd[g] = 1.0f / sqrtf(fmaxf(q - s * m, 0.f) / total + a.eps);
+        }
     }
     __syncthreads();
 }
@@ -115,9 +237,54 @@ __global__ __launch_bounds__(GN_NT) void k_gn_apply(GnArgs a) {
     }
 }
 
-// Rows of a unit: about 512 units, of 16 rows at least.
-int gn_per(int64_t n) { return (int)std::max<int64_t>(16, ceil_div(n, 512)); }
-int64_t gn_units(int64_t n, int samples) { return ceil_div(n, gn_per(n)) + samples; }
+// ... eight channels a thread, their factors in registers for all its rows. The units go in the reverse of
+// the first launch's order: what it read last is still in the caches.
+template <int XDT, int ODT>
+__global__ __launch_bounds__(GN_NT) void k_gn_apply_vec(GnArgs a) {
+    __shared__ float sMean[GN_MAX_GROUPS], sRstd[GN_MAX_GROUPS];
+    const int unit = gridDim.x - 1 - blockIdx.x;
+    const PackedUnit u = packed_unit(a.offsets, a.samples, (int)a.n, 1, a.per, unit);
+    if (u.sample < 0) return;
+    join_units(a, u, sMean, sRstd);
+    int64_t row;
+    const int rows = unit_rows(u, unit, a.per, row);
+    const int cols = a.c / 8, lanes = GN_NT / cols, cg = a.c / a.groups;
+    const int lane = threadIdx.x / cols, col = threadIdx.x - lane * cols;
+    if (lane >= lanes) return;
+    float mean[8], f[8], b[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int ch = col * 8 + e, g = ch / cg;
+        mean[e] = sMean[g];
+        f[e] = sRstd[g] * (a.gamma ? a.gamma[ch] : 1.f);
+        b[e] = a.beta ? a.beta[ch] : 0.f;
+    }
+    const int silu = a.silu;
+    auto norm = [&](int r, const float (&x)[8]) {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = act((x[e] - mean[e]) * f[e] + b[e], silu);
+        store8<ODT>(a.out, (row + r) * a.c + col * 8, y);
+    };
+    int r = lane;
+    constexpr int DEEP = 4;
+    for (; r + (DEEP - 1) * lanes < rows; r += DEEP * lanes) {
+        float x[DEEP][8];
+#pragma unroll
+        for (int i = 0; i < DEEP; ++i) load8<XDT>(a.x, (row + r + i * lanes) * a.c + col * 8, x[i]);
+#pragma unroll
+        for (int i = 0; i < DEEP; ++i) norm(r + i * lanes, x[i]);
+    }
+    for (; r < rows; r += lanes) {
+        float x[8];
+        load8<XDT>(a.x, (row + r) * a.c + col * 8, x);
+        norm(r, x);
+    }
+}
+
+// Rows of a unit: about 512 units, of two rows a thread at least (by eight channels a thread).
+int gn_per(int64_t n, int c) { return (int)std::max<int64_t>(2 * std::max(1, GN_NT * 8 / c), ceil_div(n, 512)); }
+int64_t gn_units(int64_t n, int c, int samples) { return ceil_div(n, gn_per(n, c)) + (samples > 1 ? samples : 0); }
 
 template <class F>
 void dt_switch(int dt, F&& f) {
@@ -135,7 +302,7 @@ using namespace tsp;
 
 extern "C" size_t tsp_group_norm_workspace_bytes(int64_t n, int c, int groups, int samples) {
     if (n <= 0 || n >= (1ll << 31) - (1ll << 24) || c <= 0 || groups <= 0 || samples <= 0) return 0;
-    return (size_t)gn_units(n, samples) * groups * sizeof(float2);
+    return (size_t)gn_units(n, c, samples) * groups * sizeof(float2);
 }
 
 extern "C" int tsp_group_norm(const void* d_x, int x_dtype, int64_t n, int c, int groups, const int32_t* d_offsets,
@@ -156,15 +323,21 @@ extern "C" int tsp_group_norm(const void* d_x, int x_dtype, int64_t n, int c, in
     TSP_REQUIRE(workspace_bytes >= tsp_group_norm_workspace_bytes(n, c, groups, samples), TSP_ERR_WORKSPACE,
                 "tsp_group_norm: workspace of %zu bytes, needs %zu", workspace_bytes,
                 tsp_group_norm_workspace_bytes(n, c, groups, samples));
-    const int64_t units = gn_units(n, samples);
+    const int64_t units = gn_units(n, c, samples);
     TSP_REQUIRE(units * GN_NT < (1ll << 32), TSP_ERR_INVALID, "tsp_group_norm: too many samples");
     hipStream_t s = as_stream(stream);
-    const GnArgs a{d_x, d_out, d_offsets, d_gamma, d_beta, static_cast<float2*>(d_workspace), n, c, groups, samples, gn_per(n), eps, silu};
+    const GnArgs a{d_x, d_out, d_offsets, d_gamma, d_beta, static_cast<float2*>(d_workspace), n, c, groups, samples, gn_per(n, c), eps, silu};
+    // rows of whole 16-byte pieces, eight channels a thread; element by element otherwise
+    const bool vec = c % 8 == 0 && c <= 8 * GN_NT && reinterpret_cast<uintptr_t>(d_x) % 16 == 0 && reinterpret_cast<uintptr_t>(d_out) % 16 == 0;
+    const dim3 grid((unsigned)units), block(GN_NT);
     dt_switch(x_dtype, [&](auto xd) {
         constexpr int XD = decltype(xd)::value;
-        hipLaunchKernelGGL((k_gn_stats<XD>), dim3((unsigned)units, (unsigned)groups), dim3(GN_NT), 0, s, a);
+        if (!vec) hipLaunchKernelGGL((k_gn_stats<XD>), dim3((unsigned)units, (unsigned)groups), block, 0, s, a);
+        else if (c / groups % 8 == 0) hipLaunchKernelGGL((k_gn_stats_vec<XD, 1>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((k_gn_stats_vec<XD, 8>), grid, block, 0, s, a);
         dt_switch(out_dtype, [&](auto od) {
-            hipLaunchKernelGGL((k_gn_apply<XD, decltype(od)::value>), dim3((unsigned)units), dim3(GN_NT), 0, s, a);
+            if (vec) hipLaunchKernelGGL((k_gn_apply_vec<XD, decltype(od)::value>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((k_gn_apply<XD, decltype(od)::value>), grid, block, 0, s, a);
         });
     });
     TSP_CHECK_LAUNCH();

@@ -27,53 +27,131 @@ struct RopeArgs {
     RopeSide side[2];
     const int32_t* pos;
     int64_t n;
-    int hq, heads, d, axes, halves;
+    int hq, heads, d, axes, halves, parts;
     float eps;
     double turns[RP_MAX_PAIRS];             // theta^(-j/P) / (2 pi) of each pair
     int8_t axis[RP_MAX_PAIRS];              // its axis, -1: not turned
 };
 
-// One (row, head) a group of L lanes; each lane takes whole pairs.
+// Four pairs of a head, as the lane that turns them holds them: elements 8 u .. 8 u + 7, or with halves 4 u
+// .. 4 u + 3 of each half.
+template <int DT>
+__device__ __forceinline__ void load_pairs(const void* p, int unit, int d, bool halves, float (&u)[4], float (&v)[4]) {
+    if constexpr (DT == TSP_F32) {
+        const float* x = static_cast<const float*>(p);
+        const f32x4_t a = *reinterpret_cast<const f32x4_t*>(x + (halves ? 4 * unit : 8 * unit));
+        const f32x4_t b = *reinterpret_cast<const f32x4_t*>(x + (halves ? 4 * unit + d / 2 : 8 * unit + 4));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            u[i] = halves ? a[i] : i < 2 ? a[2 * i] : b[2 * i - 4];
+            v[i] = halves ? b[i] : i < 2 ? a[2 * i + 1] : b[2 * i - 3];
+        }
+    } else {
+        const uint16_t* x = static_cast<const uint16_t*>(p);
+        auto f = [](uint32_t b) { return DT == TSP_BF16 ? bf16_bits_to_f32((uint16_t)b) : f16_bits_to_f32((uint16_t)b); };
+        if (halves) {
+            const uint2 a = *reinterpret_cast<const uint2*>(x + 4 * unit), b = *reinterpret_cast<const uint2*>(x + 4 * unit + d / 2);
+            u[0] = f(a.x & 0xffff), u[1] = f(a.x >> 16), u[2] = f(a.y & 0xffff), u[3] = f(a.y >> 16);
+            v[0] = f(b.x & 0xffff), v[1] = f(b.x >> 16), v[2] = f(b.y & 0xffff), v[3] = f(b.y >> 16);
+        } else {
+            const u32x4_t a = *reinterpret_cast<const u32x4_t*>(x + 8 * unit);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = f(a[i] & 0xffff), v[i] = f(a[i] >> 16);
+        }
+    }
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+    return DT == TSP_BF16 ? f32x2_to_bf16x2_bits(lo, hi) : f32_to_f16_bits(lo) | ((uint32_t)f32_to_f16_bits(hi) << 16);
+}
+template <int DT>
+__device__ __forceinline__ void store_pairs(void* p, int unit, int d, bool halves, const float (&u)[4], const float (&v)[4]) {
+    if constexpr (DT == TSP_F32) {
+        float* y = static_cast<float*>(p);
+        *reinterpret_cast<f32x4_t*>(y + (halves ? 4 * unit : 8 * unit)) =
+            halves ? f32x4_t{u[0], u[1], u[2], u[3]} : f32x4_t{u[0], v[0], u[1], v[1]};
+        *reinterpret_cast<f32x4_t*>(y + (halves ? 4 * unit + d / 2 : 8 * unit + 4)) =
+            halves ? f32x4_t{v[0], v[1], v[2], v[3]} : f32x4_t{u[2], v[2], u[3], v[3]};
+    } else {
+        uint16_t* y = static_cast<uint16_t*>(p);
+        if (halves) {
+            *reinterpret_cast<uint2*>(y + 4 * unit) = uint2{pack16<DT>(u[0], u[1]), pack16<DT>(u[2], u[3])};
+            *reinterpret_cast<uint2*>(y + 4 * unit + d / 2) = uint2{pack16<DT>(v[0], v[1]), pack16<DT>(v[2], v[3])};
+        } else {
+            *reinterpret_cast<u32x4_t*>(y + 8 * unit) =
+                u32x4_t{pack16<DT>(u[0], v[0]), pack16<DT>(u[1], v[1]), pack16<DT>(u[2], v[2]), pack16<DT>(u[3], v[3])};
+        }
+    }
+}
+
+// A group of L lanes takes one row and every `part`-th of its heads, four pairs a lane: the row's sines
+// and cosines are formed once for all of them. The heads' loads go out BATCH at a time.
 template <int XDT, int ODT, int L>
 __global__ __launch_bounds__(RP_NT) void k_rope(RopeArgs a) {
-    const int lane = threadIdx.x % L;
-    const int64_t item = ((int64_t)blockIdx.x * RP_NT + threadIdx.x) / L;
-    const bool live = item < a.n * a.heads;
-    const int64_t row = live ? item / a.heads : 0;
-    const int head = live ? (int)(item - row * a.heads) : 0;
-    const RopeSide& s = a.side[head >= a.hq];
-    const int h = head >= a.hq ? head - a.hq : head;
-    const auto* x = reinterpret_cast<const typename Elem<XDT>::storage*>(s.x) + row * s.x_row + h * s.x_head;
-    auto* y = reinterpret_cast<typename Elem<ODT>::storage*>(s.y) + row * s.y_row + h * s.y_head;
-    const float* gamma = s.gamma ? s.gamma + h * a.d : nullptr;
-    float scale = 1.f;
-    if (gamma) {
-        float q = 0.f;
-        for (int e = lane; e < a.d; e += L) {
-            const float v = Elem<XDT>::load(x, e);
-            q += v * v;
-        }
-        scale = 1.0f / sqrtf(group_sum<L>(q) / (float)a.d + a.eps);
+    constexpr int BATCH = 4, XS = XDT == TSP_F32 ? 4 : 2, OS = ODT == TSP_F32 ? 4 : 2;
+    const int unit = threadIdx.x % L;
+    const bool live = unit * 8 < a.d, halves = a.halves;
+    double turns[4];
+    int axis[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        axis[i] = live ? a.axis[4 * unit + i] : -1;
+        turns[i] = axis[i] < 0 ? 0. : a.turns[4 * unit + i];
     }
-    if (!live) return;
-    for (int p = lane; p < a.d / 2; p += L) {
-        const int i = a.halves ? p : 2 * p, j = a.halves ? p + a.d / 2 : 2 * p + 1;
-        float u = Elem<XDT>::load(x, i) * scale, v = Elem<XDT>::load(x, j) * scale;
-        if (gamma) {
-            u *= gamma[i];
-            v *= gamma[j];
+    const unsigned items = (unsigned)(a.n * a.parts);      // (below 2^31)
+    // (whole groups of lanes leave together)
+    for (unsigned item = (blockIdx.x * RP_NT + threadIdx.x) / L; item < items; item += gridDim.x * (RP_NT / L)) {
+        const int row = (int)(item / (unsigned)a.parts), part = (int)(item - (unsigned)row * a.parts);
+        float cs[4], sn[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            cs[i] = 1.f, sn[i] = 0.f;
+            if (axis[i] >= 0) {
+                const double t = (double)a.pos[(int64_t)row * a.axes + axis[i]] * turns[i];
+                sincospif(2.f * (float)(t - rint(t)), &sn[i], &cs[i]);
+            }
         }
-        const int ax = a.axis[p];
-        if (ax >= 0) {
-            const double t = (double)a.pos[row * a.axes + ax] * a.turns[p];
-            float sn, cs;
-            sincospif(2.f * (float)(t - rint(t)), &sn, &cs);
-            const float w = u * cs - v * sn;
-            v = v * cs + u * sn;
-            u = w;
+        for (int h0 = part; h0 < a.heads; h0 += BATCH * a.parts) {
+            float u[BATCH][4] = {}, v[BATCH][4] = {};
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                const int h = h0 + b * a.parts;
+                if (!live || h >= a.heads) continue;
+                const RopeSide& s = a.side[h >= a.hq];
+                load_pairs<XDT>(static_cast<const char*>(s.x) + ((int64_t)row * s.x_row + (h >= a.hq ? h - a.hq : h) * s.x_head) * XS,
+                                unit, a.d, halves, u[b], v[b]);
+            }
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                const int h = h0 + b * a.parts;
+                if (h >= a.heads) break;
+                const RopeSide& s = a.side[h >= a.hq];
+                const int hh = h >= a.hq ? h - a.hq : h;
+                if (s.gamma) {
+                    float q = 0.f, gu[4] = {}, gv[4] = {};
+                    if (live) {
+                        load_pairs<TSP_F32>(s.gamma + hh * a.d, unit, a.d, halves, gu, gv);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) q += u[b][i] * u[b][i] + v[b][i] * v[b][i];
+                    }
+                    const float scale = 1.0f / sqrtf(group_sum<L>(q) / (float)a.d + a.eps);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        u[b][i] *= scale * gu[i];
+                        v[b][i] *= scale * gv[i];
+                    }
+                }
+                if (!live) continue;
+                float x[4], y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[i] = u[b][i] * cs[i] - v[b][i] * sn[i];
+                    y[i] = v[b][i] * cs[i] + u[b][i] * sn[i];
+                    if (axis[i] < 0) x[i] = u[b][i], y[i] = v[b][i];     // (not 0 * Inf)
+                }
+                store_pairs<ODT>(static_cast<char*>(s.y) + ((int64_t)row * s.y_row + hh * s.y_head) * OS, unit, a.d, halves, x, y);
+            }
         }
-        Elem<ODT>::store(y, i, u);
-        Elem<ODT>::store(y, j, v);
     }
 }
 
@@ -139,13 +217,19 @@ extern "C" int tsp_rope_axes(const tsp_heads* q, int hq, const tsp_heads* k, int
             a.axis[p] = (int8_t)ax;
             a.turns[p] = std::pow(theta, -(double)j / pairs[ax]) / (2 * M_PI);
         }
-    constexpr int L = 16;
-    const int64_t blocks = ceil_div(n * a.heads * L, RP_NT);
-    TSP_REQUIRE(blocks * RP_NT < (1ll << 32), TSP_ERR_INVALID, "tsp_rope_axes: too many rows");
+    // Lanes of a group: a head's units of 8 elements and, where they are no power of two, some that idle. A row
+    // is shared by as many groups as it takes to give the device some 2048 workgroups, at most one a head.
+    const int lanes = d <= 64 ? 8 : d <= 128 ? 16 : 32, groups = RP_NT / lanes;
+    a.parts = (int)std::min<int64_t>(a.heads, std::max<int64_t>(1, 2048ll * groups / n));
+    const int64_t blocks = std::min<int64_t>(ceil_div(n * a.parts, groups), 8192);
     dt_switch(dtype, [&](auto xd) {
         dt_switch(out_dtype, [&](auto od) {
-            hipLaunchKernelGGL((k_rope<decltype(xd)::value, decltype(od)::value, L>), dim3((unsigned)blocks), dim3(RP_NT), 0,
-                               as_stream(stream), a);
+            constexpr int XD = decltype(xd)::value, OD = decltype(od)::value;
+            const dim3 grid((unsigned)blocks), block(RP_NT);
+            hipStream_t s = as_stream(stream);
+            if (lanes == 8) hipLaunchKernelGGL((k_rope<XD, OD, 8>), grid, block, 0, s, a);
+            else if (lanes == 16) hipLaunchKernelGGL((k_rope<XD, OD, 16>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((k_rope<XD, OD, 32>), grid, block, 0, s, a);
         });
     });
     TSP_CHECK_LAUNCH();
