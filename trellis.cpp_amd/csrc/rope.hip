@@ -21,42 +21,53 @@ struct RopeSide {
     void* y;
     int64_t x_row, x_head, y_row, y_head;   // strides in elements
     const float* gamma;                     // [heads][d], or NULL
+    int heads;
 };
 
 struct RopeArgs {
     RopeSide side[2];
     const int32_t* pos;
     int64_t n;
-    int hq, heads, d, axes, halves, parts;
-    float eps;
+    int d, axes, parts;
+    float eps, inv_d;
     double turns[RP_MAX_PAIRS];             // theta^(-j/P) / (2 pi) of each pair
     int8_t axis[RP_MAX_PAIRS];              // its axis, -1: not turned
 };
 
 // Four pairs of a head, as the lane that turns them holds them: elements 8 u .. 8 u + 7, or with halves 4 u
 // .. 4 u + 3 of each half.
-template <int DT>
-__device__ __forceinline__ void load_pairs(const void* p, int unit, int d, bool halves, float (&u)[4], float (&v)[4]) {
+template <int DT> struct Raw { u32x4_t a; };
+template <> struct Raw<TSP_F32> { f32x4_t a, b; };
+template <int DT, bool HALVES>
+__device__ __forceinline__ Raw<DT> load_raw(const void* p, int unit, int d) {
+    Raw<DT> r;
     if constexpr (DT == TSP_F32) {
         const float* x = static_cast<const float*>(p);
-        const f32x4_t a = *reinterpret_cast<const f32x4_t*>(x + (halves ? 4 * unit : 8 * unit));
-        const f32x4_t b = *reinterpret_cast<const f32x4_t*>(x + (halves ? 4 * unit + d / 2 : 8 * unit + 4));
+        r.a = *reinterpret_cast<const f32x4_t*>(x + (HALVES ? 4 * unit : 8 * unit));
+        r.b = *reinterpret_cast<const f32x4_t*>(x + (HALVES ? 4 * unit + d / 2 : 8 * unit + 4));
+    } else if constexpr (HALVES) {
+        const uint16_t* x = static_cast<const uint16_t*>(p);
+        const uint2 a = *reinterpret_cast<const uint2*>(x + 4 * unit), b = *reinterpret_cast<const uint2*>(x + 4 * unit + d / 2);
+        r.a = u32x4_t{a.x, a.y, b.x, b.y};
+    } else {
+        r.a = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(p) + 8 * unit);
+    }
+    return r;
+}
+template <int DT, bool HALVES>
+__device__ __forceinline__ void pairs_of(const Raw<DT>& r, float (&u)[4], float (&v)[4]) {
+    if constexpr (DT == TSP_F32) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            u[i] = halves ? a[i] : i < 2 ? a[2 * i] : b[2 * i - 4];
-            v[i] = halves ? b[i] : i < 2 ? a[2 * i + 1] : b[2 * i - 3];
+            u[i] = HALVES ? r.a[i] : i < 2 ? r.a[2 * i] : r.b[2 * i - 4];
+            v[i] = HALVES ? r.b[i] : i < 2 ? r.a[2 * i + 1] : r.b[2 * i - 3];
         }
     } else {
-        const uint16_t* x = static_cast<const uint16_t*>(p);
         auto f = [](uint32_t b) { return DT == TSP_BF16 ? bf16_bits_to_f32((uint16_t)b) : f16_bits_to_f32((uint16_t)b); };
-        if (halves) {
-            const uint2 a = *reinterpret_cast<const uint2*>(x + 4 * unit), b = *reinterpret_cast<const uint2*>(x + 4 * unit + d / 2);
-            u[0] = f(a.x & 0xffff), u[1] = f(a.x >> 16), u[2] = f(a.y & 0xffff), u[3] = f(a.y >> 16);
-            v[0] = f(b.x & 0xffff), v[1] = f(b.x >> 16), v[2] = f(b.y & 0xffff), v[3] = f(b.y >> 16);
-        } else {
-            const u32x4_t a = *reinterpret_cast<const u32x4_t*>(x + 8 * unit);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) u[i] = f(a[i] & 0xffff), v[i] = f(a[i] >> 16);
+        for (int i = 0; i < 4; ++i) {
+            u[i] = HALVES ? f(i & 1 ? r.a[i / 2] >> 16 : r.a[i / 2] & 0xffff) : f(r.a[i] & 0xffff);
+            v[i] = HALVES ? f(i & 1 ? r.a[2 + i / 2] >> 16 : r.a[2 + i / 2] & 0xffff) : f(r.a[i] >> 16);
         }
     }
 }
@@ -64,8 +75,8 @@ template <int DT>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     return DT == TSP_BF16 ? f32x2_to_bf16x2_bits(lo, hi) : f32_to_f16_bits(lo) | ((uint32_t)f32_to_f16_bits(hi) << 16);
 }
-template <int DT>
-__device__ __forceinline__ void store_pairs(void* p, int unit, int d, bool halves, const float (&u)[4], const float (&v)[4]) {
+template <int DT, bool halves>
+__device__ __forceinline__ void store_pairs(void* p, int unit, int d, const float (&u)[4], const float (&v)[4]) {
     if constexpr (DT == TSP_F32) {
         float* y = static_cast<float*>(p);
         *reinterpret_cast<f32x4_t*>(y + (halves ? 4 * unit : 8 * unit)) =
@@ -86,11 +97,11 @@ __device__ __forceinline__ void store_pairs(void* p, int unit, int d, bool halve
 
 // A group of L lanes takes one row and every `part`-th of its heads, four pairs a lane: the row's sines
 // and cosines are formed once for all of them. The heads' loads go out BATCH at a time.
-template <int XDT, int ODT, int L>
-__global__ __launch_bounds__(RP_NT) void k_rope(RopeArgs a) {
+template <int XDT, int ODT, int L, bool HALVES>
+__global__ __launch_bounds__(RP_NT, 4) void k_rope(RopeArgs a) {
     constexpr int BATCH = 4, XS = XDT == TSP_F32 ? 4 : 2, OS = ODT == TSP_F32 ? 4 : 2;
     const int unit = threadIdx.x % L;
-    const bool live = unit * 8 < a.d, halves = a.halves;
+    const bool live = unit * 8 < a.d;
     double turns[4];
     int axis[4];
 #pragma unroll
@@ -111,45 +122,51 @@ __global__ __launch_bounds__(RP_NT) void k_rope(RopeArgs a) {
                 sincospif(2.f * (float)(t - rint(t)), &sn[i], &cs[i]);
             }
         }
-        for (int h0 = part; h0 < a.heads; h0 += BATCH * a.parts) {
-            float u[BATCH][4] = {}, v[BATCH][4] = {};
+#pragma unroll 1
+        for (int side = 0; side < 2; ++side) {
+            const RopeSide& s = a.side[side];
+            const char* x = static_cast<const char*>(s.x) + ((int64_t)row * s.x_row + part * s.x_head) * XS;
+            char* y = static_cast<char*>(s.y) + ((int64_t)row * s.y_row + part * s.y_head) * OS;
+            const int64_t x_step = a.parts * s.x_head * XS, y_step = a.parts * s.y_head * OS;
+            const float* gamma = s.gamma + part * a.d;
+            for (int h0 = part; h0 < s.heads; h0 += BATCH * a.parts) {
+                Raw<XDT> raw[BATCH] = {};
 #pragma unroll
-            for (int b = 0; b < BATCH; ++b) {
-                const int h = h0 + b * a.parts;
-                if (!live || h >= a.heads) continue;
-                const RopeSide& s = a.side[h >= a.hq];
-                load_pairs<XDT>(static_cast<const char*>(s.x) + ((int64_t)row * s.x_row + (h >= a.hq ? h - a.hq : h) * s.x_head) * XS,
-                                unit, a.d, halves, u[b], v[b]);
-            }
+                for (int b = 0; b < BATCH; ++b)
+                    if (live && h0 + b * a.parts < s.heads) raw[b] = load_raw<XDT, HALVES>(x + b * x_step, unit, a.d);
+                x += BATCH * x_step;
 #pragma unroll
-            for (int b = 0; b < BATCH; ++b) {
-                const int h = h0 + b * a.parts;
-                if (h >= a.heads) break;
-                const RopeSide& s = a.side[h >= a.hq];
-                const int hh = h >= a.hq ? h - a.hq : h;
-                if (s.gamma) {
-                    float q = 0.f, gu[4] = {}, gv[4] = {};
+                for (int b = 0; b < BATCH; ++b) {
+                    if (h0 + b * a.parts >= s.heads) break;
+                    float u[4], v[4];
+                    pairs_of<XDT, HALVES>(raw[b], u, v);
+                    if (s.gamma) {
+                        float q = 0.f, gu[4], gv[4];
+                        Raw<TSP_F32> g{};
+                        if (live) g = load_raw<TSP_F32, HALVES>(gamma, unit, a.d);
+                        pairs_of<TSP_F32, HALVES>(g, gu, gv);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) q += u[i] * u[i] + v[i] * v[i];
+                        const float scale = __builtin_amdgcn_rsqf(fmaf(group_sum<L>(q), a.inv_d, a.eps));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            u[i] *= scale * gu[i];
+                            v[i] *= scale * gv[i];
+                        }
+                        gamma += a.parts * a.d;
+                    }
                     if (live) {
-                        load_pairs<TSP_F32>(s.gamma + hh * a.d, unit, a.d, halves, gu, gv);
+                        float p[4], r[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) q += u[b][i] * u[b][i] + v[b][i] * v[b][i];
+                        for (int i = 0; i < 4; ++i) {
+                            p[i] = u[i] * cs[i] - v[i] * sn[i];
+                            r[i] = v[i] * cs[i] + u[i] * sn[i];
+                            if (axis[i] < 0) p[i] = u[i], r[i] = v[i];     // (not 0 * Inf)
+                        }
+                        store_pairs<ODT, HALVES>(y, unit, a.d, p, r);
                     }
-                    const float scale = 1.0f / sqrtf(group_sum<L>(q) / (float)a.d + a.eps);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        u[b][i] *= scale * gu[i];
-                        v[b][i] *= scale * gv[i];
-                    }
+                    y += y_step;
                 }
-                if (!live) continue;
-                float x[4], y[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[i] = u[b][i] * cs[i] - v[b][i] * sn[i];
-                    y[i] = v[b][i] * cs[i] + u[b][i] * sn[i];
-                    if (axis[i] < 0) x[i] = u[b][i], y[i] = v[b][i];     // (not 0 * Inf)
-                }
-                store_pairs<ODT>(static_cast<char*>(s.y) + ((int64_t)row * s.y_row + hh * s.y_head) * OS, unit, a.d, halves, x, y);
             }
         }
     }
@@ -197,19 +214,17 @@ extern "C" int tsp_rope_axes(const tsp_heads* q, int hq, const tsp_heads* k, int
     TSP_REQUIRE(heads_apart(*q_out, n, hq, d) && (hk == 0 || heads_apart(*k_out, n, hk, d)), TSP_ERR_INVALID,
                 "tsp_rope_axes: the output's heads overlap");
     RopeArgs a{};
-    auto side = [](const tsp_heads& x, const tsp_heads& y, const float* g) {
-        return RopeSide{x.data, y.data, x.row_stride, x.head_stride, y.row_stride, y.head_stride, g};
+    auto side = [](const tsp_heads& x, const tsp_heads& y, const float* g, int heads) {
+        return RopeSide{x.data, y.data, x.row_stride, x.head_stride, y.row_stride, y.head_stride, g, heads};
     };
-    a.side[0] = side(*q, *q_out, d_q_gamma);
-    if (hk) a.side[1] = side(*k, *k_out, d_k_gamma);
+    a.side[0] = side(*q, *q_out, d_q_gamma, hq);
+    if (hk) a.side[1] = side(*k, *k_out, d_k_gamma, hk);
     a.pos = d_pos;
     a.n = n;
-    a.hq = hq;
-    a.heads = hq + hk;
     a.d = d;
     a.axes = axes;
-    a.halves = flags & TSP_ROPE_HALVES ? 1 : 0;
     a.eps = eps;
+    a.inv_d = 1.f / (float)d;
     for (int p = 0; p < d / 2; ++p) a.axis[p] = -1;
     int p = 0;
     for (int ax = 0; ax < axes; ++ax)
@@ -220,16 +235,23 @@ extern "C" int tsp_rope_axes(const tsp_heads* q, int hq, const tsp_heads* k, int
     // Lanes of a group: a head's units of 8 elements and, where they are no power of two, some that idle. A row
     // is shared by as many groups as it takes to give the device some 2048 workgroups, at most one a head.
     const int lanes = d <= 64 ? 8 : d <= 128 ? 16 : 32, groups = RP_NT / lanes;
-    a.parts = (int)std::min<int64_t>(a.heads, std::max<int64_t>(1, 2048ll * groups / n));
+    a.parts = (int)std::min<int64_t>(std::max(hq, hk), std::max<int64_t>(1, 2048ll * groups / n));
     const int64_t blocks = std::min<int64_t>(ceil_div(n * a.parts, groups), 8192);
     dt_switch(dtype, [&](auto xd) {
         dt_switch(out_dtype, [&](auto od) {
             constexpr int XD = decltype(xd)::value, OD = decltype(od)::value;
             const dim3 grid((unsigned)blocks), block(RP_NT);
             hipStream_t s = as_stream(stream);
-            if (lanes == 8) hipLaunchKernelGGL((k_rope<XD, OD, 8>), grid, block, 0, s, a);
-            else if (lanes == 16) hipLaunchKernelGGL((k_rope<XD, OD, 16>), grid, block, 0, s, a);
-            else hipLaunchKernelGGL((k_rope<XD, OD, 32>), grid, block, 0, s, a);
+            auto go = [&](auto l, auto halves) {
+                hipLaunchKernelGGL((k_rope<XD, OD, decltype(l)::value, decltype(halves)::value>), grid, block, 0, s, a);
+            };
+            auto by_pairing = [&](auto l) {
+                if (flags & TSP_ROPE_HALVES) go(l, std::true_type{});
+                else go(l, std::false_type{});
+            };
+            if (lanes == 8) by_pairing(std::integral_constant<int, 8>{});
+            else if (lanes == 16) by_pairing(std::integral_constant<int, 16>{});
+            else by_pairing(std::integral_constant<int, 32>{});
         });
     });
     TSP_CHECK_LAUNCH();
