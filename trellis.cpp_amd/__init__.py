@@ -812,20 +812,15 @@ class _On:
     """Runs a call on its tensors' device and on the given stream: what it allocates there belongs to
     that stream, and its tensors are kept from reuse until the stream is past the call."""
 
-    def __init__(self, device, stream):
-        torch = _torch()
-        self.device, self.current, self.guards = device, torch.cuda.current_stream(device), []
+    def __init__(self, device, stream, current):
         if stream is not None and stream.device != device:
             raise ValueError(f"stream is on {stream.device}, the tensors on {device}")
-        self.stream = stream if stream is not None else self.current
-        self.other = self.stream != self.current
+        self.device, self.current, self.guards = device, current, []
+        self.stream = stream if stream is not None else current
 
     def __enter__(self):
         torch = _torch()
-        if self.device.index != torch.cuda.current_device():
-            self.guards.append(torch.cuda.device(self.device))
-        if self.other:
-            self.guards.append(torch.cuda.stream(self.stream))
+        self.guards = [torch.cuda.device(self.device), torch.cuda.stream(self.stream)]
         for g in self.guards:
             g.__enter__()
         return self
@@ -835,15 +830,22 @@ class _On:
             g.__exit__(*exc)
 
     def keep(self, *tensors):
-        if self.other:
+        if self.stream != self.current:
             for t in tensors:
                 if t is not None:
                     t.record_stream(self.stream)
                     t.record_stream(self.current)
 
-    @property
-    def ptr(self):
-        return ctypes.c_void_p(self.stream.cuda_stream)
+
+def _launch(device, stream, call):
+    """call(stream pointer, keep) on the device and stream; keep(*tensors) is told every tensor the call
+    uses."""
+    torch = _torch()
+    current = torch.cuda.current_stream(device)
+    if stream is None and device.index == torch.cuda.current_device():
+        return call(current.cuda_stream, lambda *tensors: None)
+    with _On(device, stream, current) as on:
+        return call(on.stream.cuda_stream, on.keep)
 
 
 def _same_device(device, **ts):
@@ -863,9 +865,10 @@ def _offsets(t, name: str):
     return t, t.numel() - 1
 
 
-def _workspace_ok(ws, need: int, name: str):
-    if ws.dtype != _torch().uint8 or ws.numel() < need or not ws.is_contiguous():
-        raise ValueError(f"workspace must be a contiguous uint8 buffer of {name} ({need}) bytes")
+def _check_workspace(ws):
+    # (its size is the library's to check)
+    if ws.dtype != _torch().uint8 or not ws.is_contiguous():
+        raise ValueError("workspace must be a contiguous uint8 buffer")
 
 
 def group_norm_workspace(n: int, c: int, groups: int, samples: int = 1, device="cuda"):
@@ -894,43 +897,46 @@ def group_norm(x, groups: int, gamma=None, beta=None, eps: float = 1e-6, silu: b
         _check_out(out, n, c, out_dtype or out.dtype, dev)
     _same_device(dev, offsets=offsets, gamma=gamma, beta=beta, workspace=workspace)
     xd = dtype_code(x.dtype)
-    need = lib().tsp_group_norm_workspace_bytes(n, c, groups, samples)
     if workspace is not None:
-        _workspace_ok(workspace, need, "tsp_group_norm_workspace_bytes")
-    with _On(dev, stream) as on:
+        _check_workspace(workspace)
+
+    def call(s, keep):
         xc = x.contiguous()
-        if out is None:
-            out = torch.empty((n, c), dtype=out_dtype or x.dtype, device=dev)
-        ws = workspace if workspace is not None else torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-        on.keep(x, xc, gamma, beta, offsets, out, ws)
+        o = out if out is not None else torch.empty((n, c), dtype=out_dtype or x.dtype, device=dev)
+        ws = workspace
+        if ws is None:
+            ws = torch.empty(max(lib().tsp_group_norm_workspace_bytes(n, c, groups, samples), 16), dtype=torch.uint8, device=dev)
+        keep(x, xc, gamma, beta, offsets, o, ws)
         _check("tsp_group_norm",
                lib().tsp_group_norm(_ptr(xc), xd, n, c, groups, _ptr(offsets), samples, _ptr(gamma), _ptr(beta), eps,
-                                    1 if silu else 0, _ptr(out), dtype_code(out.dtype), _ptr(ws), ws.numel(), on.ptr))
-    return out
+                                    1 if silu else 0, _ptr(o), dtype_code(o.dtype), _ptr(ws), ws.numel(), s))
+        return o
+    return _launch(dev, stream, call)
 
 
-def _heads_fit(t) -> bool:
-    """Whether the kernels can read t [N, H, D] where it lies."""
+def _heads(t):
+    """t [N, H, D] as tsp_heads, or None where the kernels cannot read it as it lies."""
     n, h, d = t.shape
-    return ((d == 1 or t.stride(2) == 1) and t.data_ptr() % 16 == 0 and (n <= 1 or (t.stride(0) % 8 == 0 and t.stride(0) <= 1 << 20))
-            and (h <= 1 or t.stride(1) % 8 == 0))
+    row, head, one = t.stride()
+    p = t.data_ptr()
+    if p % 16 or (one != 1 and d != 1) or (n > 1 and (row % 8 or row > 1 << 20)) or (h > 1 and head % 8):
+        return None
+    return Heads(p, row if n > 1 else h * d, head if h > 1 else d)
 
 
 def _fitted(t):
-    """t where it lies if the kernels can read it there, else a copy that they can."""
-    return t if _heads_fit(t) else t.clone(memory_format=_torch().contiguous_format)
-
-
-def _heads(t) -> Heads:
-    n, h, d = t.shape
-    head = t.stride(1) if h > 1 else d
-    return Heads(t.data_ptr(), t.stride(0) if n > 1 else h * d, head)
+    """(t, its tsp_heads), t copied where the kernels could not read it as it lies."""
+    hd = _heads(t)
+    if hd is None:
+        t = t.clone(memory_format=_torch().contiguous_format)
+        hd = _heads(t) or Heads(t.data_ptr(), t.shape[1] * t.shape[2], t.shape[2])   # (D not of whole pieces: the library refuses it)
+    return t, hd
 
 
 def _check_heads_out(out, like, dtype, name: str):
-    if tuple(out.shape) != tuple(like.shape) or out.dtype != dtype or out.device != like.device:
+    if out.shape != like.shape or out.dtype != dtype or out.device != like.device:
         raise ValueError(f"{name} must be {dtype} {list(like.shape)} on {like.device}")
-    if not _heads_fit(out):
+    if _heads(out) is None:
         raise ValueError(f"{name} must be 16-byte aligned with contiguous heads and strides that are multiples of 8")
 
 
@@ -965,22 +971,23 @@ def rope_axes(q, pos, k=None, pairs=None, theta: float = 10000.0, interleaved: b
     for name, o, t in (("q_out", q_out, q), ("k_out", k_out, k)):
         if o is not None:
             _check_heads_out(o, t, odt, name)
-    with _On(dev, stream) as on:
-        qc = _fitted(q)
-        kc = None if k is None else _fitted(k)
+
+    def call(s, keep):
+        qc, qh = _fitted(q)
+        qo = q_out if q_out is not None else torch.empty((n, hq, d), dtype=odt, device=dev)
+        kc = ko = kh = koh = None
+        if k is not None:
+            kc, kh = _fitted(k)
+            ko = k_out if k_out is not None else torch.empty(k.shape, dtype=odt, device=dev)
+            koh = _fitted(ko)[1]
         pc = pos.contiguous()
-        if q_out is None:
-            q_out = torch.empty((n, hq, d), dtype=odt, device=dev)
-        if k is not None and k_out is None:
-            k_out = torch.empty(tuple(k.shape), dtype=odt, device=dev)
-        on.keep(q, k, qc, kc, pos, pc, q_gamma, k_gamma, q_out, k_out)
-        kh = None if k is None else ctypes.byref(_heads(kc))
-        koh = None if k is None else ctypes.byref(_heads(k_out))
+        keep(q, k, qc, kc, pos, pc, q_gamma, k_gamma, qo, ko)
         _check("tsp_rope_axes",
-               lib().tsp_rope_axes(ctypes.byref(_heads(qc)), hq, kh, 0 if k is None else k.shape[1], dtype_code(q.dtype), n, d,
-                                   _ptr(pc), axes, (ctypes.c_int * axes)(*pairs), theta, 0 if interleaved else 1, _ptr(q_gamma),
-                                   _ptr(k_gamma), eps, ctypes.byref(_heads(q_out)), koh, dtype_code(odt), on.ptr))
-    return q_out if k is None else (q_out, k_out)
+               lib().tsp_rope_axes(qh, hq, kh, 0 if k is None else k.shape[1], dtype_code(q.dtype), n, d, _ptr(pc), axes,
+                                   (ctypes.c_int * axes)(*pairs), theta, 0 if interleaved else 1, _ptr(q_gamma), _ptr(k_gamma), eps,
+                                   _fitted(qo)[1], koh, dtype_code(odt), s))
+        return qo if k is None else (qo, ko)
+    return _launch(dev, stream, call)
 
 
 def attention_workspace(nq: int, nk: int, samples: int, hq: int, hkv: int, d: int, device="cuda"):
@@ -1013,18 +1020,20 @@ def attention(q, k, v, q_offsets=None, k_offsets=None, causal: bool = False, sca
     _same_device(dev, k=k, v=v, q_offsets=q_offsets, k_offsets=k_offsets, workspace=workspace)
     if out is not None:
         _check_heads_out(out, q, q.dtype, "out")
-    need = lib().tsp_attention_workspace_bytes(nq, nk, samples, hq, hkv, d)
     if workspace is not None:
-        _workspace_ok(workspace, need, "tsp_attention_workspace_bytes")
-    with _On(dev, stream) as on:
-        qc, kc, vc = _fitted(q), _fitted(k), _fitted(v)
-        if out is None:
-            out = torch.empty((nq, hq, d), dtype=q.dtype, device=dev)
-        ws = workspace if workspace is not None or need == 0 else torch.empty(need, dtype=torch.uint8, device=dev)
-        on.keep(q, k, v, qc, kc, vc, q_offsets, k_offsets, out, ws)
+        _check_workspace(workspace)
+
+    def call(s, keep):
+        (qc, qh), (kc, kh), (vc, vh) = _fitted(q), _fitted(k), _fitted(v)
+        o = out if out is not None else torch.empty((nq, hq, d), dtype=q.dtype, device=dev)
+        ws = workspace
+        if ws is None:
+            need = lib().tsp_attention_workspace_bytes(nq, nk, samples, hq, hkv, d)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        keep(q, k, v, qc, kc, vc, q_offsets, k_offsets, o, ws)
         _check("tsp_attention",
-               lib().tsp_attention(ctypes.byref(_heads(qc)), ctypes.byref(_heads(kc)), ctypes.byref(_heads(vc)),
-                                   dtype_code(q.dtype), nq, nk, hq, hkv, d, _ptr(q_offsets), _ptr(k_offsets), samples,
-                                   d ** -0.5 if scale is None else scale, 1 if causal else 0, ctypes.byref(_heads(out)),
-                                   _ptr(ws), 0 if ws is None else ws.numel(), on.ptr))
-    return out
+               lib().tsp_attention(qh, kh, vh, dtype_code(q.dtype), nq, nk, hq, hkv, d, _ptr(q_offsets), _ptr(k_offsets), samples,
+                                   d ** -0.5 if scale is None else scale, 1 if causal else 0, _fitted(o)[1], _ptr(ws),
+                                   0 if ws is None else ws.numel(), s))
+        return o
+    return _launch(dev, stream, call)
