@@ -208,9 +208,14 @@ def _torch():
     return torch
 
 
+_codes = {}
+
+
 def dtype_code(dt) -> int:
-    torch = _torch()
-    return {torch.float32: TSP_F32, torch.float16: TSP_F16, torch.bfloat16: TSP_BF16}[dt]
+    if not _codes:
+        torch = _torch()
+        _codes.update({torch.float32: TSP_F32, torch.float16: TSP_F16, torch.bfloat16: TSP_BF16})
+    return _codes[dt]
 
 
 def _stream(stream=None):
@@ -837,23 +842,33 @@ class _On:
                     t.record_stream(self.current)
 
 
-def _launch(device, stream, call):
-    """call(stream pointer, keep) on the device and stream; keep(*tensors) is told every tensor the call
-    uses."""
-    torch = _torch()
-    current = torch.cuda.current_stream(device)
-    if stream is None and device.index == torch.cuda.current_device():
-        return call(current.cuda_stream, lambda *tensors: None)
+def _nothing(*tensors):
+    pass
+
+
+def _launch(device, stream, call, *args):
+    """call(stream pointer, keep, *args) on the device and stream; keep(*tensors) is told every tensor the
+    call uses."""
+    cuda = _torch().cuda
+    index = device.index
+    current = cuda.current_stream(index)
+    if stream is None and index == cuda.current_device():
+        return call(current.cuda_stream, _nothing, *args)
     with _On(device, stream, current) as on:
-        return call(on.stream.cuda_stream, on.keep)
+        return call(on.stream.cuda_stream, on.keep, *args)
 
 
-def _same_device(device, **ts):
+def _same_device(device, *named):
+    """named: name, tensor, name, tensor, ..."""
     if device.type != "cuda":
         raise ValueError("tensors must live on the GPU")
-    for name, t in ts.items():
+    for name, t in zip(named[::2], named[1::2]):
         if t is not None and t.device != device:
             raise ValueError(f"{name} must live on {device}, got {t.device}")
+
+
+def _p(t) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _offsets(t, name: str):
@@ -895,7 +910,7 @@ def group_norm(x, groups: int, gamma=None, beta=None, eps: float = 1e-6, silu: b
             raise ValueError(f"{name} must be a contiguous float32 vector of {c}")
     if out is not None:
         _check_out(out, n, c, out_dtype or out.dtype, dev)
-    _same_device(dev, offsets=offsets, gamma=gamma, beta=beta, workspace=workspace)
+    _same_device(dev, "offsets", offsets, "gamma", gamma, "beta", beta, "workspace", workspace)
     xd = dtype_code(x.dtype)
     if workspace is not None:
         _check_workspace(workspace)
@@ -908,8 +923,8 @@ def group_norm(x, groups: int, gamma=None, beta=None, eps: float = 1e-6, silu: b
             ws = torch.empty(max(lib().tsp_group_norm_workspace_bytes(n, c, groups, samples), 16), dtype=torch.uint8, device=dev)
         keep(x, xc, gamma, beta, offsets, o, ws)
         _check("tsp_group_norm",
-               lib().tsp_group_norm(_ptr(xc), xd, n, c, groups, _ptr(offsets), samples, _ptr(gamma), _ptr(beta), eps,
-                                    1 if silu else 0, _ptr(o), dtype_code(o.dtype), _ptr(ws), ws.numel(), s))
+               lib().tsp_group_norm(_p(xc), xd, n, c, groups, _p(offsets), samples, _p(gamma), _p(beta), eps,
+                                    1 if silu else 0, _p(o), dtype_code(o.dtype), _p(ws), ws.numel(), s))
         return o
     return _launch(dev, stream, call)
 
@@ -966,7 +981,7 @@ def rope_axes(q, pos, k=None, pairs=None, theta: float = 10000.0, interleaved: b
     for name, g, t in (("q_gamma", q_gamma, q), ("k_gamma", k_gamma, k)):
         if g is not None and (g.dtype != torch.float32 or tuple(g.shape) != tuple(t.shape[1:]) or not g.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous float32 {list(t.shape[1:])}")
-    _same_device(dev, k=k, pos=pos, q_gamma=q_gamma, k_gamma=k_gamma)
+    _same_device(dev, "k", k, "pos", pos, "q_gamma", q_gamma, "k_gamma", k_gamma)
     odt = out_dtype or (q_out.dtype if q_out is not None else k_out.dtype if k_out is not None else q.dtype)
     for name, o, t in (("q_out", q_out, q), ("k_out", k_out, k)):
         if o is not None:
@@ -983,8 +998,8 @@ def rope_axes(q, pos, k=None, pairs=None, theta: float = 10000.0, interleaved: b
         pc = pos.contiguous()
         keep(q, k, qc, kc, pos, pc, q_gamma, k_gamma, qo, ko)
         _check("tsp_rope_axes",
-               lib().tsp_rope_axes(qh, hq, kh, 0 if k is None else k.shape[1], dtype_code(q.dtype), n, d, _ptr(pc), axes,
-                                   (ctypes.c_int * axes)(*pairs), theta, 0 if interleaved else 1, _ptr(q_gamma), _ptr(k_gamma), eps,
+               lib().tsp_rope_axes(qh, hq, kh, 0 if k is None else k.shape[1], dtype_code(q.dtype), n, d, _p(pc), axes,
+                                   (ctypes.c_int * axes)(*pairs), theta, 0 if interleaved else 1, _p(q_gamma), _p(k_gamma), eps,
                                    _fitted(qo)[1], koh, dtype_code(odt), s))
         return qo if k is None else (qo, ko)
     return _launch(dev, stream, call)
@@ -1017,7 +1032,7 @@ def attention(q, k, v, q_offsets=None, k_offsets=None, causal: bool = False, sca
     k_offsets, k_samples = _offsets(k_offsets, "k_offsets")
     if samples != k_samples:
         raise ValueError("q_offsets and k_offsets must name the same samples")
-    _same_device(dev, k=k, v=v, q_offsets=q_offsets, k_offsets=k_offsets, workspace=workspace)
+    _same_device(dev, "k", k, "v", v, "q_offsets", q_offsets, "k_offsets", k_offsets, "workspace", workspace)
     if out is not None:
         _check_heads_out(out, q, q.dtype, "out")
     if workspace is not None:
@@ -1032,8 +1047,8 @@ def attention(q, k, v, q_offsets=None, k_offsets=None, causal: bool = False, sca
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         keep(q, k, v, qc, kc, vc, q_offsets, k_offsets, o, ws)
         _check("tsp_attention",
-               lib().tsp_attention(qh, kh, vh, dtype_code(q.dtype), nq, nk, hq, hkv, d, _ptr(q_offsets), _ptr(k_offsets), samples,
-                                   d ** -0.5 if scale is None else scale, 1 if causal else 0, _fitted(o)[1], _ptr(ws),
+               lib().tsp_attention(qh, kh, vh, dtype_code(q.dtype), nq, nk, hq, hkv, d, _p(q_offsets), _p(k_offsets), samples,
+                                   d ** -0.5 if scale is None else scale, 1 if causal else 0, _fitted(o)[1], _p(ws),
                                    0 if ws is None else ws.numel(), s))
         return o
     return _launch(dev, stream, call)

@@ -524,16 +524,28 @@ __global__ __launch_bounds__(256) void k_attention_join(AttnArgs a) {
     }
     float acc[8] = {};
     if (live && e < a.d) {
-#pragma unroll 4
-        for (int s = g; s < a.splits; s += G) {
-            const float w = sW[at][s];
-            if (w == -1.f) continue;
-            const f32x4_t* p = reinterpret_cast<const f32x4_t*>(a.part + (s * step + item) * a.d + e);
-            const f32x4_t x = p[0], y = p[1];
+        constexpr int BATCH = 8;      // splits on their way at a time
+        for (int s0 = g; s0 < a.splits; s0 += BATCH * G) {
+            f32x4_t x[BATCH], y[BATCH];
+            float w[BATCH];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                acc[i] += w * x[i];
-                acc[4 + i] += w * y[i];
+            for (int b = 0; b < BATCH; ++b) {
+                const int s = s0 + b * G;
+                w[b] = s < a.splits ? sW[at][s] : -1.f;
+                x[b] = y[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                if (w[b] == -1.f) continue;
+                const f32x4_t* p = reinterpret_cast<const f32x4_t*>(a.part + (s * step + item) * a.d + e);
+                x[b] = p[0];
+                y[b] = p[1];
+            }
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                if (w[b] == -1.f) continue;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    acc[i] += w[b] * x[b][i];
+                    acc[4 + i] += w[b] * y[b][i];
+                }
             }
         }
     }
@@ -584,7 +596,7 @@ AttnCut attn_cut(int64_t nq, int64_t nk, int samples, int hkv, int share, int d,
     if (busy == full || (full > 0 && (samples > 1 || causal))) return c;
     auto rounds = [&](int64_t n, int64_t length) { return (n / slots + (n % slots ? 0.5 + 0.5 * (double)(n % slots) / slots : 0.)) * (length + 3); };
     double best = rounds(busy - full, tiles);
-    for (int s = 2; s <= AT_MAX_SPLITS && (busy - full) * s <= 2 * slots; ++s) {
+    for (int s = 2; s <= AT_MAX_SPLITS && (busy - full) * s <= 2 * slots; s += 1 + s / 32) {
         const double cost = rounds((busy - full) * s, ceil_div(tiles, s)) + 6;
         if (cost < best) {
             best = cost;

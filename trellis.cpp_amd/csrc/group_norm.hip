@@ -2,9 +2,10 @@
 //   y = (x - mean) / sqrt(var + eps) * gamma[c] + beta[c], then y * sigmoid(y) where asked,
 // mean and (biased) var over the sample's rows and the group's channels.
 //
-// Two launches over the same units of rows. The first leaves each unit's mean and sum of squared
-// deviations per group in the workspace, the second joins a sample's units (in the order of the units,
-// whatever the order in which they ran) and normalises its rows.
+// Launches over the same units of rows: the first leaves each unit's mean and sum of squared deviations
+// per group in the workspace, the last normalises the rows; between them a sample's units are joined (in
+// the order of the units, whatever the order in which they ran), by a launch of its own where they are many.
+// Small samples take one launch.
 #include <algorithm>
 
 #include "common.hpp"
@@ -22,6 +23,7 @@ struct GnArgs {
     const int32_t* offsets;
     const float *gamma, *beta;
     float2* part;          // [unit][group]: mean, sum of squared deviations
+    float2* stat;          // [sample][group]: mean, 1 / sqrt(var + eps); NULL: the last launch joins the units
     int64_t n;
     int c, groups, samples, per;
     float eps;
@@ -183,29 +185,55 @@ __global__ __launch_bounds__(GN_NT) void k_gn_stats_vec(GnArgs a) {
     }
 }
 
-// Mean and 1 / sqrt(var + eps) of every group of the unit's sample, into LDS: the units' means and squared
-// deviations joined about the first unit's mean.
-__device__ __forceinline__ void join_units(const GnArgs& a, const PackedUnit& u, float* sMean, float* sRstd) {
+// Mean and 1 / sqrt(var + eps) of group g: the units' means and squared deviations joined about the first
+// unit's mean, by `lanes` lanes of which this is `sub`; all get the result.
+__device__ __forceinline__ float2 join_units(const GnArgs& a, const PackedUnit& u, int g, int lanes, int sub) {
     const float cg = (float)(a.c / a.groups), total = (float)u.rows * cg;
-    const int lg = lanes_a_group(a.groups), sub = threadIdx.x & (lg - 1);
-    for (int g0 = 0; g0 < a.groups; g0 += GN_NT / lg) {
-        const int g = g0 + threadIdx.x / lg;
-        const float2* p = a.part + (int64_t)u.first * a.groups + min(g, a.groups - 1);
-        const float m0 = p->x;
-        float s = 0.f, q = 0.f;
+    const float2* p = a.part + (int64_t)u.first * a.groups + g;
+    const float m0 = p->x;
+    float s = 0.f, q = 0.f;
 #pragma unroll 8
-        for (int i = sub; i < u.count; i += lg) {
-            const float2 t = p[(int64_t)i * a.groups];
-            const float d = t.x - m0, n = (float)min(a.per, u.rows - i * a.per) * cg;
-            s += n * d;
-            q += t.y + n * d * d;
+    for (int i = sub; i < u.count; i += lanes) {
+        const float2 t = p[(int64_t)i * a.groups];
+        const float d = t.x - m0, n = (float)min(a.per, u.rows - i * a.per) * cg;
+        s += n * d;
+        q += t.y + n * d * d;
+    }
+    s = sum_over(s, lanes);
+    q = sum_over(q, lanes);
+    const float m = s / total;
+    return float2{m0 + m, 1.0f / sqrtf(fmaxf(q - s * m, 0.f) / total + a.eps)};
+}
+
+// A wave a sample and group: where there are more than GN_FEW units, every workgroup of the last launch
+// joining them for itself would read them all some hundred times over (512 units of 32 groups: 15 us).
+constexpr int GN_FEW = 64;
+__global__ __launch_bounds__(256) void k_gn_join(GnArgs a) {
+    const int g = blockIdx.y * 4 + (threadIdx.x >> 6), sample = blockIdx.x;
+    if (g >= a.groups) return;
+    const PackedUnit u = packed_sample(a.offsets, (int)a.n, 1, a.per, sample);
+    if (u.rows == 0) return;
+    const float2 t = join_units(a, u, g, 64, threadIdx.x & 63);
+    if ((threadIdx.x & 63) == 0) a.stat[(int64_t)sample * a.groups + g] = t;
+}
+
+// The statistics of the unit's sample, into LDS.
+__device__ __forceinline__ void sample_stats(const GnArgs& a, const PackedUnit& u, float* sMean, float* sRstd) {
+    if (a.stat) {
+        for (int g = threadIdx.x; g < a.groups; g += GN_NT) {
+            const float2 t = a.stat[(int64_t)u.sample * a.groups + g];
+            sMean[g] = t.x;
+            sRstd[g] = t.y;
         }
-        s = sum_over(s, lg);
-        q = sum_over(q, lg);
-        const float m = s / total;
-        if (g < a.groups && sub == 0) {
-            sMean[g] = m0 + m;
-            sRstd[g] = 1.0f / sqrtf(fmaxf(q - s * m, 0.f) / total + a.eps);
+    } else {
+        const int lg = lanes_a_group(a.groups), sub = threadIdx.x & (lg - 1);
+        for (int g0 = 0; g0 < a.groups; g0 += GN_NT / lg) {
+            const int g = g0 + threadIdx.x / lg;
+            const float2 t = join_units(a, u, min(g, a.groups - 1), lg, sub);
+            if (g < a.groups && sub == 0) {
+                sMean[g] = t.x;
+                sRstd[g] = t.y;
+            }
         }
     }
     __syncthreads();
@@ -216,7 +244,7 @@ __global__ __launch_bounds__(GN_NT) void k_gn_apply(GnArgs a) {
     __shared__ float sMean[GN_MAX_GROUPS], sRstd[GN_MAX_GROUPS];
     const PackedUnit u = packed_unit(a.offsets, a.samples, (int)a.n, 1, a.per, blockIdx.x);
     if (u.sample < 0) return;
-    join_units(a, u, sMean, sRstd);
+    sample_stats(a, u, sMean, sRstd);
     int64_t row;
     const int rows = unit_rows(u, blockIdx.x, a.per, row);
     const int cg = a.c / a.groups;
@@ -255,7 +283,7 @@ __global__ __launch_bounds__(GN_NT) void k_gn_apply_vec(GnArgs a) {
     for (int e = 0; e < 8; ++e) f[e] = 1.f, b[e] = 0.f;
     if (a.gamma) load8<TSP_F32>(a.gamma, col * 8, f);
     if (a.beta) load8<TSP_F32>(a.beta, col * 8, b);
-    join_units(a, u, sMean, sRstd);
+    sample_stats(a, u, sMean, sRstd);
     if (lane >= lanes) return;
     float mean[8];
 #pragma unroll
@@ -278,8 +306,88 @@ __global__ __launch_bounds__(GN_NT) void k_gn_apply_vec(GnArgs a) {
     }
 }
 
-// Rows of a unit: about 512 units, of two rows a thread at least (by eight channels a thread).
-int gn_per(int64_t n, int c) { return (int)std::max<int64_t>(2 * std::max(1, GN_NT * 8 / c), ceil_div(n, 512)); }
+// Small samples in one launch: a workgroup takes one group of whole 16-byte pieces (or the groups of one
+// piece, `PER` of them) of a whole sample, held in registers, so that x is read once and mean and deviations
+// are formed one after the other.
+constexpr int GS_NT = 1024, GS_ROWS = 4;          // threads, rows a thread holds at most
+template <int XDT, int ODT, int PER>
+__global__ __launch_bounds__(GS_NT) void k_gn_small(GnArgs a) {
+    __shared__ float sSum[2][PER][GS_NT / 64];
+    int row0, rows;
+    packed_rows(a.offsets, blockIdx.y, (int)a.n, row0, rows);
+    if (rows == 0) return;
+    const int cg = a.c / a.groups, slab = cg < 8 ? 8 : cg, cols = slab / 8, lanes = GS_NT / cols;
+    const int lane = threadIdx.x / cols, col = threadIdx.x - lane * cols;
+    const int ch = blockIdx.x * slab + col * 8;
+    const int mine = lane < lanes ? (rows - lane + lanes - 1) / lanes : 0;       // rows of this thread
+    const auto* first = reinterpret_cast<const typename Elem<XDT>::storage*>(a.x) + (int64_t)row0 * a.c + blockIdx.x * slab;
+    float x[GS_ROWS][8], gamma[8], beta[8], shift[PER];
+#pragma unroll
+    for (int i = 0; i < GS_ROWS; ++i)
+        if (i < mine) load8<XDT>(a.x, (int64_t)(row0 + lane + i * lanes) * a.c + ch, x[i]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) gamma[e] = 1.f, beta[e] = 0.f;
+    if (a.gamma) load8<TSP_F32>(a.gamma, ch, gamma);
+    if (a.beta) load8<TSP_F32>(a.beta, ch, beta);
+    // sums go about the group's first value, so that equal values have their mean exactly
+#pragma unroll
+    for (int k = 0; k < PER; ++k) shift[k] = Elem<XDT>::load(first, k * (8 / PER));
+    auto workgroup_sums = [&](float (&v)[PER], int buffer) {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            v[k] = group_sum<64>(v[k]);
+            if ((threadIdx.x & 63) == 0) sSum[buffer][k][threadIdx.x >> 6] = v[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < PER; ++k) v[k] = group_sum<16>(sSum[buffer][k][threadIdx.x & 15]);
+    };
+    const float count = (float)rows * (float)cg;
+    float mean[PER] = {}, var[PER] = {};
+#pragma unroll
+    for (int i = 0; i < GS_ROWS; ++i)
+        if (i < mine)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mean[e * PER / 8] += x[i][e] - shift[e * PER / 8];
+    workgroup_sums(mean, 0);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) mean[k] = shift[k] + mean[k] / count;
+#pragma unroll
+    for (int i = 0; i < GS_ROWS; ++i)
+        if (i < mine)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float d = x[i][e] - mean[e * PER / 8];
+                var[e * PER / 8] += d * d;
+            }
+    workgroup_sums(var, 1);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) var[k] = 1.0f / sqrtf(var[k] / count + a.eps);
+#pragma unroll
+    for (int i = 0; i < GS_ROWS; ++i) {
+        if (i >= mine) break;
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = act((x[i][e] - mean[e * PER / 8]) * (var[e * PER / 8] * gamma[e]) + beta[e], a.silu);
+        store8<ODT>(a.out, (int64_t)(row0 + lane + i * lanes) * a.c + ch, y);
+    }
+}
+
+// Whether samples of up to n rows fit it. Eight rows a thread would still hold them, but lose to three
+// launches (bf16: 8,192 x 64 in 32 groups 14.9 us and 10.5; four rows: 2,606 x 64 8.1 and 9.6).
+bool gn_small(int64_t n, int c, int groups, int samples) {
+    const int cg = c / groups;
+    if ((cg % 8 && 8 % cg) || samples > 65535 || cg > 8 * GS_NT) return false;
+    return n <= (int64_t)GS_ROWS * (GS_NT / (cg < 8 ? 1 : cg / 8));
+}
+
+// Rows of a unit. Four rows a thread at least (one batch of loads; eight channels a thread): 60,013 x 64 in
+// bf16 takes 14.6 us so, 18.0 with two. About 512 units, which the device holds at once; 1024 where that is
+// far more than the caches hold and only the loads in flight count (bf16 with SiLU: 300,000 x 512 takes
+// 199 us with 512, 183 with 1024; 60,013 x 256 26 and 30).
+int gn_per(int64_t n, int c) {
+    return (int)std::max<int64_t>(4 * std::max(1, GN_NT * 8 / c), ceil_div(n, n * c > (1ll << 27) ? 1024 : 512));
+}
 int64_t gn_units(int64_t n, int c, int samples) { return ceil_div(n, gn_per(n, c)) + (samples > 1 ? samples : 0); }
 
 template <class F>
@@ -298,7 +406,7 @@ using namespace tsp;
 
 extern "C" size_t tsp_group_norm_workspace_bytes(int64_t n, int c, int groups, int samples) {
     if (n <= 0 || n >= (1ll << 31) - (1ll << 24) || c <= 0 || groups <= 0 || samples <= 0) return 0;
-    return (size_t)gn_units(n, c, samples) * groups * sizeof(float2);
+    return (size_t)(gn_units(n, c, samples) + samples) * groups * sizeof(float2);
 }
 
 extern "C" int tsp_group_norm(const void* d_x, int x_dtype, int64_t n, int c, int groups, const int32_t* d_offsets,
@@ -322,16 +430,33 @@ extern "C" int tsp_group_norm(const void* d_x, int x_dtype, int64_t n, int c, in
     const int64_t units = gn_units(n, c, samples);
     TSP_REQUIRE(units * GN_NT < (1ll << 32), TSP_ERR_INVALID, "tsp_group_norm: too many samples");
     hipStream_t s = as_stream(stream);
-    const GnArgs a{d_x, d_out, d_offsets, d_gamma, d_beta, static_cast<float2*>(d_workspace), n, c, groups, samples, gn_per(n, c), eps, silu};
+    float2* part = static_cast<float2*>(d_workspace);
+    const GnArgs a{d_x, d_out, d_offsets, d_gamma, d_beta, part, units > GN_FEW ? part + units * groups : nullptr, n, c, groups, samples, gn_per(n, c), eps, silu};
     // rows of whole 16-byte pieces, eight channels a thread; element by element otherwise
     const bool vec = c % 8 == 0 && c <= 8 * GN_NT && !(reinterpret_cast<uintptr_t>(d_x) % 16 || reinterpret_cast<uintptr_t>(d_out) % 16 ||
                        reinterpret_cast<uintptr_t>(d_gamma) % 16 || reinterpret_cast<uintptr_t>(d_beta) % 16);
+    if (vec && gn_small(n, c, groups, samples)) {
+        const int cg = c / groups;
+        const dim3 grid((unsigned)(c / (cg < 8 ? 8 : cg)), (unsigned)samples), block(GS_NT);
+        dt_switch(x_dtype, [&](auto xd) {
+            dt_switch(out_dtype, [&](auto od) {
+                constexpr int XD = decltype(xd)::value, OD = decltype(od)::value;
+                if (cg >= 8) hipLaunchKernelGGL((k_gn_small<XD, OD, 1>), grid, block, 0, s, a);
+                else if (cg == 4) hipLaunchKernelGGL((k_gn_small<XD, OD, 2>), grid, block, 0, s, a);
+                else if (cg == 2) hipLaunchKernelGGL((k_gn_small<XD, OD, 4>), grid, block, 0, s, a);
+                else hipLaunchKernelGGL((k_gn_small<XD, OD, 8>), grid, block, 0, s, a);
+            });
+        });
+        TSP_CHECK_LAUNCH();
+        return TSP_OK;
+    }
     const dim3 grid((unsigned)units), block(GN_NT);
     dt_switch(x_dtype, [&](auto xd) {
         constexpr int XD = decltype(xd)::value;
         if (!vec) hipLaunchKernelGGL((k_gn_stats<XD>), dim3((unsigned)units, (unsigned)groups), block, 0, s, a);
         else if (c / groups % 8 == 0) hipLaunchKernelGGL((k_gn_stats_vec<XD, 1>), grid, block, 0, s, a);
         else hipLaunchKernelGGL((k_gn_stats_vec<XD, 8>), grid, block, 0, s, a);
+        if (a.stat) hipLaunchKernelGGL(k_gn_join, dim3((unsigned)samples, (unsigned)ceil_div(groups, 4)), dim3(256), 0, s, a);
         dt_switch(out_dtype, [&](auto od) {
             if (vec) hipLaunchKernelGGL((k_gn_apply_vec<XD, decltype(od)::value>), grid, block, 0, s, a);
             else hipLaunchKernelGGL((k_gn_apply<XD, decltype(od)::value>), grid, block, 0, s, a);

@@ -62,6 +62,24 @@ __device__ __forceinline__ PackedUnit packed_unit(const int32_t* offsets, int sa
     return u;
 }
 
+// Sample `sample` and its units (uniform, by whole waves).
+__device__ __forceinline__ PackedUnit packed_sample(const int32_t* offsets, int n, int mult, int per, int sample) {
+    PackedUnit u{sample, 0, 0, 0, 0};
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int s = lane; s < sample; s += 64) {
+        int row0, rows;
+        packed_rows(offsets, s, n, row0, rows);
+        before += (int)((unsigned)(rows * mult + per - 1) / (unsigned)per);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o, 64);
+    u.first = __builtin_amdgcn_readfirstlane(before);
+    packed_rows(offsets, sample, n, u.row0, u.rows);
+    u.count = (int)((unsigned)(u.rows * mult + per - 1) / (unsigned)per);
+    return u;
+}
+
 // Rows of heads as the transformer pieces take them: 16-byte aligned, strides multiples of 8 elements (a
 // row's below 2^20, so that a tile of rows spans less than 2^31 bytes).
 inline bool heads_aligned(const tsp_heads& t) {
