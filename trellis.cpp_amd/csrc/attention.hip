@@ -38,6 +38,7 @@ struct AttnArgs {
     int samples, hkv, share, d, causal;
     int units;                                // of rows, a key head
     int whole, splits;                        // the first `whole` of units * hkv see their keys at once, the others in splits
+    FastDiv by_share, by_units, by_splits;
     float scale2;                             // scale * log2(e)
     float* part;                              // [unit past whole][split][row][d] sums of p v, and
     float2* stat;                             // [unit past whole][split][row] maximum and sum of p (-1: no key seen)
@@ -52,9 +53,9 @@ struct AttnUnit {
 template <int ROWS, class Args>
 __device__ __forceinline__ AttnUnit attn_unit(const Args& a, int w) {
     AttnUnit t;
-    t.head = (unsigned)w / (unsigned)a.units;
+    t.head = w / FastDiv{a.by_units.mul, a.by_units.shift};
     const int unit = w - t.head * a.units;
-    t.u = packed_unit(a.q_off, a.samples, (int)a.nq, a.share, ROWS, unit);
+    t.u = packed_unit<true>(a.q_off, a.samples, (int)a.nq, a.share, ROWS, unit, a.k_off, (int)a.nk);
     t.row0 = (a.causal ? t.u.count - 1 - (unit - t.u.first) : unit - t.u.first) * ROWS;
     t.rows = t.u.rows * a.share;
     return t;
@@ -159,20 +160,21 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
     if (work >= a.whole) {
         const int past = work - a.whole;
         splits = a.splits;
-        work = a.whole + (unsigned)past / (unsigned)splits;
-        split = (unsigned)past % (unsigned)splits;
+        const int at = past / FastDiv{a.by_splits.mul, a.by_splits.shift};
+        work = a.whole + at;
+        split = past - at * splits;
     }
     const AttnUnit t = attn_unit<ROWS>(a, work);
     const PackedUnit& u = t.u;
     const int head = t.head, rows = t.rows, tile0 = t.row0;
     if (u.sample < 0) return;
-    int krow0, lk;
-    packed_rows(a.k_off, u.sample, (int)a.nk, krow0, lk);
+    const int krow0 = u.other0, lk = u.others;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
 
     // rows past the sample's last are copies of it that are not stored
     auto limit = [&](int query) __attribute__((always_inline)) { return a.causal ? min(max(lk - u.rows + query + 1, 0), lk) : lk; };
-    auto query = [&](int r) __attribute__((always_inline)) { return (int)((unsigned)min(r, rows - 1) / (unsigned)a.share); };
+    const FastDiv by_share{a.by_share.mul, a.by_share.shift};
+    auto query = [&](int r) __attribute__((always_inline)) { return min(r, rows - 1) / by_share; };
     const int r = tile0 + wave * 32 + r32, qi = query(r);
     const RowLimits lim{limit(qi), limit(query(tile0 + wave * 32 + 31))};
     const int wg_end = limit(query(tile0 + ROWS - 1));
@@ -230,7 +232,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
     float m = -INFINITY, l = 0.f;
 
     // this split's share of the workgroup's tiles
-    const int tiles = (wg_end + AT_KEYS - 1) / AT_KEYS, per = (unsigned)(tiles + splits - 1) / (unsigned)splits;
+    const int tiles = (wg_end + AT_KEYS - 1) / AT_KEYS, per = splits == 1 ? tiles : (tiles + splits - 1) / FastDiv{a.by_splits.mul, a.by_splits.shift};
     const int begin = split * per * AT_KEYS, end = min(wg_end, begin + per * AT_KEYS);
     const bool causal = a.causal;
 
@@ -439,9 +441,9 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
 
     const float2 lh = both_halves(l);
     const float sum = lh.x + lh.y;
-    if (r >= rows) return;
     const auto& b = *reread_args();
     if (splits > 1) {
+        if (r >= rows) return;
         const int64_t item = ((int64_t)(work - b.whole) * splits + split) * ROWS + (r - tile0);
         const bool seen = lim.lane > begin && begin < end;
         if (h == 0) b.stat[item] = float2{m, seen ? sum : -1.f};
@@ -456,18 +458,27 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
             }
         return;
     }
-    const float inv = 1.0f / sum;
-    uint16_t* op = b.o + (int64_t)(u.row0 + qi) * b.o_row + hq * b.o_head;
-    const bool none = lim.lane == 0;
+    // Rows of out leave in 16-byte pieces, whole rows at a time: the wave's part of the tile goes through its own
+    // piece of the K buffers (swizzled as K is), since a lane holds 8 bytes of every 16 of its row.
+    const float inv = lim.lane == 0 ? 0.f : 1.0f / sum;      // (no key seen: zeros)
+    char* sO = NW == 1 || wave < NW / 2 ? sK0 + wave * (32 * DP * 2) : sK1 + (wave - NW / 2) * (32 * DP * 2);
+    static_assert(NW <= 4, "two waves' rows a buffer");
+    __syncthreads();
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int e = db * 32 + 8 * g + 4 * h;
-            if (e < b.d)
-                *reinterpret_cast<uint2*>(op + e) = none ? uint2{0, 0} : uint2{pack2<BF16>(o[db][4 * g] * inv, o[db][4 * g + 1] * inv),
-                                                                              pack2<BF16>(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv)};
-        }
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<uint2*>(sO + k_piece<DP>(r32, db * 4 + g) + h * 8) =
+                uint2{pack2<BF16>(o[db][4 * g] * inv, o[db][4 * g + 1] * inv), pack2<BF16>(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv)};
+    const int piece = lane % P;
+#pragma unroll
+    for (int i = 0; i < 32 / (64 / P); ++i) {
+        const int row = i * (64 / P) + lane / P, rr = tile0 + wave * 32 + row;
+        const u32x4_t x = *reinterpret_cast<const u32x4_t*>(sO + k_piece<DP>(row, piece));
+        if (rr >= rows || piece * 8 >= b.d) continue;
+        const int qr = rr / FastDiv{b.by_share.mul, b.by_share.shift}, hr = head * b.share + rr - qr * b.share;
+        *reinterpret_cast<u32x4_t*>(b.o + (int64_t)(u.row0 + qr) * b.o_row + hr * b.o_head + piece * 8) = x;
+    }
 #endif
 }
 
@@ -565,7 +576,7 @@ __global__ __launch_bounds__(256) void k_attention_join(AttnArgs a) {
     if (seen)
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-    const int qi = (unsigned)r / (unsigned)a.share, hq = w.head * a.share + r - qi * a.share;
+    const int qi = r / a.by_share, hq = w.head * a.share + r - qi * a.share;
     *reinterpret_cast<u32x4_t*>(a.o + (int64_t)(w.u.row0 + qi) * a.o_row + hq * a.o_head + e) = y;
 }
 
@@ -658,7 +669,8 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
     const AttnArgs a{static_cast<const uint16_t*>(q->data), static_cast<const uint16_t*>(kk.data), static_cast<const uint16_t*>(vv.data),
                      static_cast<uint16_t*>(out->data), q->row_stride, q->head_stride, kk.row_stride, kk.head_stride, vv.row_stride,
                      vv.head_stride, out->row_stride, out->head_stride, d_q_offsets, d_k_offsets, nq, nk, samples, hkv, share, d,
-                     causal ? 1 : 0, (int)c.units, (int)c.whole, c.splits, scale * 1.44269504088896340736f, part, stat};
+                     causal ? 1 : 0, (int)c.units, (int)c.whole, c.splits,
+                     fast_div((uint32_t)share), fast_div((uint32_t)c.units), fast_div((uint32_t)c.splits), scale * 1.44269504088896340736f, part, stat};
     const dim3 grid((unsigned)blocks), block(c.nw * 64);
     hipStream_t s = as_stream(stream);
     auto go = [&](auto bf, auto dp, auto nw) {

@@ -15,7 +15,22 @@ struct PackedUnit {
     int sample;        // -1: there are fewer units
     int first, count;  // the sample's first unit, how many it has
     int row0, rows;    // the sample's rows
+    int other0, others;   // the sample's rows in a second packed tensor, where one is asked for
 };
+
+// x / d for 0 <= x < 2^31 by a multiplication: with s = ceil(log2 d) and mul = floor(2^(31 + s) / d) + 1,
+// mul * d exceeds 2^(31 + s) by at most d <= 2^s, so that (x * mul) >> (31 + s) is exact. (The compiler's
+// own division is some thirty instructions.)
+struct FastDiv {
+    uint32_t mul;
+    int shift;
+};
+inline FastDiv fast_div(uint32_t d) {
+    int s = 0;
+    while ((1ull << s) < d) ++s;
+    return FastDiv{(uint32_t)((1ull << (31 + s)) / d + 1), s};
+}
+__device__ __forceinline__ int operator/(int x, FastDiv d) { return (int)(((uint64_t)(uint32_t)x * d.mul) >> (31 + d.shift)); }
 
 // Rows of sample s of n < 2^31; bounds outside [0, n] or out of order are cut to it, so that no row
 // outside the tensor is touched. offsets NULL: one sample of all n rows.
@@ -25,11 +40,15 @@ __device__ __forceinline__ void packed_rows(const int32_t* offsets, int s, int n
 }
 
 // The unit-th unit of `per` rows (each row counted `mult` times; n * mult + per < 2^31), called by whole
-// waves with a uniform unit: 64 samples a step, their unit counts summed across the wave.
-__device__ __forceinline__ PackedUnit packed_unit(const int32_t* offsets, int samples, int n, int mult, int per, int unit) {
-    PackedUnit u{-1, 0, 0, 0, 0};
+// waves with a uniform unit: 64 samples a step, their unit counts summed across the wave. With SECOND also
+// the sample's rows in a second tensor of n2 rows.
+template <bool SECOND = false>
+__device__ __forceinline__ PackedUnit packed_unit(const int32_t* offsets, int samples, int n, int mult, int per, int unit,
+                                                  const int32_t* offsets2 = nullptr, int n2 = 0) {
+    PackedUnit u{-1, 0, 0, 0, 0, 0, 0};
     if (samples == 1) {
         packed_rows(offsets, 0, n, u.row0, u.rows);
+        if constexpr (SECOND) packed_rows(offsets2, 0, n2, u.other0, u.others);
         u.count = (int)((unsigned)(u.rows * mult + per - 1) / (unsigned)per);
         if (unit < u.count) u.sample = 0;
         return u;
@@ -38,8 +57,11 @@ __device__ __forceinline__ PackedUnit packed_unit(const int32_t* offsets, int sa
     int before = 0;
     for (int s0 = 0; s0 < samples; s0 += 64) {
         const int s = s0 + lane;
-        int row0 = 0, rows = 0;
-        if (s < samples) packed_rows(offsets, s, n, row0, rows);
+        int row0 = 0, rows = 0, other0 = 0, others = 0;
+        if (s < samples) {
+            packed_rows(offsets, s, n, row0, rows);
+            if constexpr (SECOND) packed_rows(offsets2, s, n2, other0, others);
+        }
         const int cnt = (int)((unsigned)(rows * mult + per - 1) / (unsigned)per);
         int end = cnt;
 #pragma unroll
@@ -55,6 +77,10 @@ __device__ __forceinline__ PackedUnit packed_unit(const int32_t* offsets, int sa
             u.first = before + __builtin_amdgcn_readlane(end, l) - u.count;
             u.row0 = __builtin_amdgcn_readlane(row0, l);
             u.rows = __builtin_amdgcn_readlane(rows, l);
+            if constexpr (SECOND) {
+                u.other0 = __builtin_amdgcn_readlane(other0, l);
+                u.others = __builtin_amdgcn_readlane(others, l);
+            }
             return u;
         }
         before += __builtin_amdgcn_readlane(end, 63);
@@ -64,7 +90,7 @@ __device__ __forceinline__ PackedUnit packed_unit(const int32_t* offsets, int sa
 
 // Sample `sample` and its units (uniform, by whole waves).
 __device__ __forceinline__ PackedUnit packed_sample(const int32_t* offsets, int n, int mult, int per, int sample) {
-    PackedUnit u{sample, 0, 0, 0, 0};
+    PackedUnit u{sample, 0, 0, 0, 0, 0, 0};
     const int lane = threadIdx.x & 63;
     int before = 0;
     for (int s = lane; s < sample; s += 64) {
