@@ -38,7 +38,7 @@ struct AttnArgs {
     int samples, hkv, share, d, causal;
     int units;                                // of rows, a key head
     int whole, splits;                        // the first `whole` of units * hkv see their keys at once, the others in splits
-    FastDiv by_share, by_units, by_splits;
+    FastDiv by_share, by_heads, by_splits;
     float scale2;                             // scale * log2(e)
     float* part;                              // [unit past whole][split][row][d] sums of p v, and
     float2* stat;                             // [unit past whole][split][row] maximum and sum of p (-1: no key seen)
@@ -49,12 +49,14 @@ struct AttnUnit {
     PackedUnit u;      // its sample (-1: none)
     int head, row0, rows;   // the key head, its first row, the sample's rows
 };
-// Units go by head, then by row; with causal the last rows of a sample, which see most, come first.
+// The key heads of one unit of rows follow each other (with 8 of them each XCD, which takes every eighth
+// workgroup, has one head's keys in its L2), the longest samples come first, and with causal a sample's last
+// rows, which see most.
 template <int ROWS, class Args>
 __device__ __forceinline__ AttnUnit attn_unit(const Args& a, int w) {
     AttnUnit t;
-    t.head = w / FastDiv{a.by_units.mul, a.by_units.shift};
-    const int unit = w - t.head * a.units;
+    const int unit = w / FastDiv{a.by_heads.mul, a.by_heads.shift};
+    t.head = w - unit * a.hkv;
     t.u = packed_unit<true>(a.q_off, a.samples, (int)a.nq, a.share, ROWS, unit, a.k_off, (int)a.nk);
     t.row0 = (a.causal ? t.u.count - 1 - (unit - t.u.first) : unit - t.u.first) * ROWS;
     t.rows = t.u.rows * a.share;
@@ -670,7 +672,7 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
                      static_cast<uint16_t*>(out->data), q->row_stride, q->head_stride, kk.row_stride, kk.head_stride, vv.row_stride,
                      vv.head_stride, out->row_stride, out->head_stride, d_q_offsets, d_k_offsets, nq, nk, samples, hkv, share, d,
                      causal ? 1 : 0, (int)c.units, (int)c.whole, c.splits,
-                     fast_div((uint32_t)share), fast_div((uint32_t)c.units), fast_div((uint32_t)c.splits), scale * 1.44269504088896340736f, part, stat};
+                     fast_div((uint32_t)share), fast_div((uint32_t)hkv), fast_div((uint32_t)c.splits), scale * 1.44269504088896340736f, part, stat};
     const dim3 grid((unsigned)blocks), block(c.nw * 64);
     hipStream_t s = as_stream(stream);
     auto go = [&](auto bf, auto dp, auto nw) {
