@@ -595,11 +595,14 @@ AttnCut attn_cut(int64_t nq, int64_t nk, int samples, int hkv, int share, int d,
     c.nw = ceil_div(nq, samples) * share <= 32 ? 1 : 4;
     const int64_t units = ceil_div(nq * share, c.nw * 32);
     c.units = units + (samples > 1 ? samples : 0);
-    // The device holds `slots` workgroups at once (by registers and LDS); a round of fewer takes half of a full
-    // one's time and what its share of the slots adds. Where there are not `slots` units, their keys are
-    // split; where one sample's units leave a last round partly empty, that round's are. (Several samples,
-    // or causal ones, have units of unequal length, which fill each other's gaps.) Time is counted in
-    // tiles: about three for a workgroup's start and end, six for the join.
+    // The device holds `slots` workgroups at once (by registers and LDS), some on each of 256 CUs, and a round
+    // of them on few slots a CU is shorter: alone on its CU a workgroup of width 64 takes 0.37 of the time
+    // that it takes as one of three, of width 128 0.62 of that as one of two (measured: 0.75 and 2.0 us a
+    // tile, 1.2 and 1.9); one-wave workgroups wait for memory, and half a round's take half and half a
+    // round's time. Where there are not `slots` units, their keys are split; where one sample's units
+    // leave a last round partly empty, that round's are. (Several samples, or causal ones, have units of
+    // unequal length, which fill each other's gaps.) Time is counted in tiles: about three for a workgroup's
+    // start and end, five or six for the join.
     const int64_t busy = (units + (samples > 1 ? samples / 2 : 0)) * hkv;
     const int64_t slots = 256 * (d > 64 ? 2 : c.nw == 1 ? 5 : 3);
     const int64_t tiles = ceil_div(ceil_div(nk, samples), AT_KEYS);
@@ -607,10 +610,19 @@ AttnCut attn_cut(int64_t nq, int64_t nk, int samples, int hkv, int share, int d,
     c.splits = 1;
     const int64_t full = busy / slots * slots;
     if (busy == full || (full > 0 && (samples > 1 || causal))) return c;
-    auto rounds = [&](int64_t n, int64_t length) { return (n / slots + (n % slots ? 0.5 + 0.5 * (double)(n % slots) / slots : 0.)) * (length + 3); };
+    auto rounds = [&](int64_t n, int64_t length) {
+        const int64_t left = n % slots, used = ceil_div(left, 256);
+        const double part = left == 0     ? 0.
+                            : c.nw == 1   ? 0.5 + 0.5 * (double)left / (double)slots
+                            : used == 1   ? (d > 64 ? 0.62 : 0.37)
+                            : d > 64      ? 1.
+                            : used == 2   ? 0.68
+                                          : 1.;
+        return ((double)(n / slots) + part) * (double)(length + 3);
+    };
     double best = rounds(busy - full, tiles);
     for (int s = 2; s <= AT_MAX_SPLITS && (busy - full) * s <= 2 * slots; s += 1 + s / 32) {
-        const double cost = rounds((busy - full) * s, ceil_div(tiles, s)) + 6;
+        const double cost = rounds((busy - full) * s, ceil_div(tiles, s)) + (c.nw == 1 ? 6 : 5);
         if (cost < best) {
             best = cost;
             c.splits = s;
