@@ -472,10 +472,11 @@ typedef struct {
  * axis a is turned by the angle pos[i][a] * theta^(-j / pairs[a]): (u, v) becomes
  * (u cos - v sin, v cos + u sin). The d / 2 pairs of a head are elements (2p, 2p + 1), or with
  * TSP_ROPE_HALVES (p, p + d/2); axis 0's pairs[0] pairs come first, then axis 1's, and pairs after the
- * last axis's stay as they are. Angles are exact to 2^-23 at any position. q and k (hk heads; NULL and 0
- * without) are turned in one launch. With gamma (f32 [heads][d], or NULL), a head's row is
- * RMS-normalised first: x / sqrt(mean(x^2) + eps) * gamma. 1 to 4 axes; d a multiple of 8 up to 256.
- * Any dtypes; an output may be its own input where they are the same dtype and strides, and must not
+ * last axis's stay as they are. Angles are formed in 64 bits and are exact to 2^-22 for positions up to
+ * 2^28. q and k (hk heads; NULL and 0 without) are turned in one launch. With gamma (f32 [heads][d], or
+ * NULL), a head's row is RMS-normalised first: x / sqrt(mean(x^2) + eps) * gamma. 1 to 4 axes; d a
+ * multiple of 8 up to 256; data and gamma 16-byte aligned, strides multiples of 8 (rows' up to 2^20). Any
+ * dtypes; an output may be its own input where they have one dtype and the same strides, and must not
  * overlap the inputs otherwise. */
 enum { TSP_ROPE_HALVES = 1 };
 int tsp_rope_axes(const tsp_heads* q, int hq, const tsp_heads* k, int hk, int dtype, int64_t n, int d,
@@ -489,7 +490,8 @@ int tsp_rope_axes(const tsp_heads* q, int hq, const tsp_heads* k, int hk, int dt
  * prompt, or new tokens after a cache). q_offsets and k_offsets give the samples' rows in q and in k and
  * v. A row that sees no key gets zeros; a key that a row does not see has no effect on it, whatever it
  * holds. f16 or bf16 (out of the same type), d a multiple of 8 up to 128, hq % hkv == 0, scale > 0; data
- * 16-byte aligned, strides multiples of 8. out must not overlap the inputs. Where there are few queries
+ * 16-byte aligned, strides multiples of 8 (rows' up to 2^20; of k and v at least d; a head stride of 0 shares
+ * one head's data). nq, nk and nq * hq / hkv below 2^31 - 2^16. out must not overlap the inputs. Where there are few queries
  * the keys are split over the device and the parts joined in the workspace, 16-byte aligned, of
  * tsp_attention_workspace_bytes bytes (0, and NULL will do, where they are not). */
 size_t tsp_attention_workspace_bytes(int64_t nq, int64_t nk, int samples, int hq, int hkv, int d);

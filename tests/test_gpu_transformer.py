@@ -116,6 +116,14 @@ def test_group_norm_unaligned(gpu_lib):
     assert gpu_lib.group_norm(x[:0], 8).shape == (0, 64)
 
 
+def test_group_norm_unaligned_factors(gpu_lib):
+    randn = gen(18)
+    x, f = randn(700, 64), randn(129)
+    for gamma, beta in ((f[1:65], None), (None, f[65:]), (f[1:65], f[65:])):
+        y, slack = ref.group_norm(x, 8, [0, 700], gamma, beta, 1e-6, True)
+        ref.check(gpu_lib.group_norm(x, 8, gamma, beta, silu=True), y, slack, "factors")
+
+
 def test_group_norm_bad_offsets_stay_inside(gpu_lib):
     """Offsets out of order or outside [0, n]: no row outside the tensor is read or written."""
     import torch
@@ -180,6 +188,17 @@ def test_rope_views_in_place(gpu_lib):
     gpu_lib.rope_axes(odd, pos, q_out=dst[:, :, :64].transpose(0, 1))
     ref.check(dst[:, :, :64].transpose(0, 1), y, slack, "out heads first")
     assert (dst[:, :, 64:] == -7).all()
+
+
+def test_rope_unaligned_gamma(gpu_lib):
+    import torch
+    randn = gen(7)
+    x, pos = randn(50, 2, 64), torch.randint(0, 64, (50, 3), device="cuda", dtype=torch.int32)
+    g = randn(2 * 64 + 1)[1:].view(2, 64)
+    y, slack = ref.rope(x, pos, [10, 10, 10], 10000.0, True, g, 1e-6)
+    ref.check(gpu_lib.rope_axes(x, pos, q_gamma=g), y, slack, "gamma")
+    y, slack = ref.rope(x[:1].expand(50, 2, 64), pos, [10, 10, 10], 10000.0, True, None, 1e-6)
+    ref.check(gpu_lib.rope_axes(x[:1].expand(50, 2, 64), pos), y, slack, "broadcast row")
 
 
 def test_rope_values(gpu_lib):
@@ -267,6 +286,9 @@ def test_attention_views(gpu_lib):
     one = k[:, :1].expand(333, 4, 64)
     o, slack = ref.attention(q, one, v, [0, 333], [0, 333], False, 0.125)
     ref.check(gpu_lib.attention(q, one, v), o, slack, "broadcast head")
+    same = v[:1].expand(333, 4, 64)
+    out = gpu_lib.attention(q, k, same)
+    assert ((out - same).abs() <= 2.0 ** -9 * same.abs()).all()      # a mean of equal rows, p rounded to half steps
 
 
 @pytest.mark.parametrize("d", [64, 128, 40])
@@ -291,6 +313,36 @@ def test_attention_values_behind_the_mask(gpu_lib, d, key):
     out = gpu_lib.attention(q, k, v, ints(qb), ints(kb), causal=True)
     o, slack = ref.attention(q[3:73], k[10:90], v[10:90], [0, 70], [0, 80], True, d ** -0.5)
     ref.check(out[3:73], o, slack, "later keys")
+
+
+@pytest.mark.parametrize("hkv,lq,lk", [(1, 4, 300), (2, 7, 20_000), (4, 3, 61), (1, 8, 7), (2, 40, 5000)])
+def test_attention_few_rows_behind_the_mask(gpu_lib, hkv, lq, lk):
+    """The same for a few new tokens against a cache, split or not: the last keys hold an Inf and a NaN that
+    the earlier tokens do not see."""
+    import torch
+    randn = gen(lk)
+    q, k, v = randn(lq, 4, 64).bfloat16(), randn(lk, hkv, 64).bfloat16(), randn(lk, hkv, 64).bfloat16()
+    k[-1, 0, 5], v[-2, hkv - 1, 63], v[-1, 0, 0] = math.inf, math.nan, -math.inf
+    out = gpu_lib.attention(q, k, v, causal=True)
+    o, slack = ref.attention(q, k, v, [0, lq], [0, lk], True, 0.125)
+    ref.check(out, o, slack, "few rows")
+    seen = max(0, lk - 2 - (lk - lq))
+    assert torch.isfinite(out[:seen]).all()
+
+
+def test_attention_many_samples(gpu_lib):
+    """More samples than a wave has lanes, unequal and some empty, few and many rows each; the longest samples
+    first or last."""
+    import torch
+    for lens in ([(1 + i % 5, 3 + 7 * i % 50) for i in range(150)], [(100, 300 - 18 * i) for i in range(16)], [(64, 20 * i) for i in range(17)],
+                 [(i % 3 * 90, 200 + 40 * i) for i in range(9)]):
+        randn = gen(len(lens))
+        qb, kb = ref.offsets_of([a for a, _ in lens]), ref.offsets_of([b for _, b in lens])
+        q, k, v = randn(qb[-1], 4, 64).half(), randn(kb[-1], 2, 64).half(), randn(kb[-1], 2, 64).half()
+        for causal in (False, True):
+            out = gpu_lib.attention(q, k, v, ints(qb), ints(kb), causal=causal)
+            o, slack = ref.attention(q, k, v, qb, kb, causal, 0.125)
+            ref.check(out, o, slack, f"{len(lens)} samples")
 
 
 def test_attention_minus_infinity(gpu_lib):

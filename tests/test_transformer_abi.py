@@ -51,7 +51,7 @@ def test_rope_refusals(pkg):
         ref = lambda h: None if h is None else ctypes.byref(h)
         return L.tsp_rope_axes(ref(q), kw.get("hq", 8), ref(k), kw.get("hk", 8), kw.get("dt", 2), kw.get("n", 100), kw.get("d", 64),
                                kw.get("pos", FAKE), kw.get("axes", 3), (ctypes.c_int * len(pairs))(*pairs), kw.get("theta", 1e4),
-                               kw.get("flags", 0), NULL, NULL, kw.get("eps", 1e-6), ref(qo), ref(ko), kw.get("odt", 2), NULL)
+                               kw.get("flags", 0), kw.get("gq", NULL), kw.get("gk", NULL), kw.get("eps", 1e-6), ref(qo), ref(ko), kw.get("odt", 2), NULL)
     assert f(n=-1) == 1 and f(n=1 << 31) == 1 and f(dt=5) == 1 and f(odt=3) == 1 and f(flags=2) == 1
     assert f(hq=0) == 1 and f(hk=-1) == 1 and f(hk=0) == 1 and f(k=None) == 1 and f(hq=4096) == 1
     assert f(d=60) == 4 and f(d=264) == 4 and f(d=0) == 4 and "multiple of 8" in _err(pkg)
@@ -61,6 +61,7 @@ def test_rope_refusals(pkg):
     assert f(q=None) == 1 and f(qo=None) == 1 and f(pos=NULL) == 1 and f(ko=None) == 1 and f(q=_heads(pkg, 0)) == 1
     assert f(q=_heads(pkg, 0x10008)) == 1 and f(q=_heads(pkg, row=516)) == 1 and f(k=_heads(pkg, row=1 << 21)) == 1
     assert f(qo=_heads(pkg, 0x30000, 256, 64)) == 1 and f(ko=_heads(pkg, 0x30000, 512, 32)) == 1 and "overlap" in _err(pkg)
+    assert f(gq=ctypes.c_void_p(0x1004)) == 1 and f(gk=ctypes.c_void_p(0x1008)) == 1 and "gamma" in _err(pkg)
     assert f(n=0, q=None, pos=NULL) == 0
     assert f(n=0, q=None, pos=NULL, k=None, hk=0) == 0
 
@@ -83,6 +84,7 @@ def test_attention_refusals(pkg):
     assert f(q=None) == 1 and f(o=None) == 1 and f(k=None) == 1 and f(v=_heads(pkg, 0)) == 1
     assert f(q=_heads(pkg, 0x10008)) == 1 and f(k=_heads(pkg, 0x20000, 514)) == 1 and f(v=_heads(pkg, 0x30000, 1 << 21)) == 1
     assert f(o=_heads(pkg, 0x40000, 256)) == 1 and "overlap" in _err(pkg)
+    assert f(k=_heads(pkg, 0x20000, 0)) == 1 and f(v=_heads(pkg, 0x30000, 56), nk=1) == 1 and "rows overlap" in _err(pkg)
     assert f(o=_heads(pkg, 0x10000)) == 1 and "alias" in _err(pkg)
     assert f(nq=0, q=None, o=None) == 0
     need = L.tsp_attention_workspace_bytes(1, 100_000, 1, 16, 2, 128)

@@ -934,7 +934,7 @@ def _heads(t):
     n, h, d = t.shape
     row, head, one = t.stride()
     p = t.data_ptr()
-    if p % 16 or (one != 1 and d != 1) or (n > 1 and (row % 8 or row > 1 << 20)) or (h > 1 and head % 8):
+    if p % 16 or (one != 1 and d != 1) or (n > 1 and (row % 8 or not d <= row <= 1 << 20)) or (h > 1 and head % 8):
         return None
     return Heads(p, row if n > 1 else h * d, head if h > 1 else d)
 
@@ -996,10 +996,11 @@ def rope_axes(q, pos, k=None, pairs=None, theta: float = 10000.0, interleaved: b
             ko = k_out if k_out is not None else torch.empty(k.shape, dtype=odt, device=dev)
             koh = _fitted(ko)[1]
         pc = pos.contiguous()
-        keep(q, k, qc, kc, pos, pc, q_gamma, k_gamma, qo, ko)
+        gq, gk = (g if g is None or g.data_ptr() % 16 == 0 else g.clone() for g in (q_gamma, k_gamma))
+        keep(q, k, qc, kc, pos, pc, q_gamma, k_gamma, gq, gk, qo, ko)
         _check("tsp_rope_axes",
                lib().tsp_rope_axes(qh, hq, kh, 0 if k is None else k.shape[1], dtype_code(q.dtype), n, d, _p(pc), axes,
-                                   (ctypes.c_int * axes)(*pairs), theta, 0 if interleaved else 1, _p(q_gamma), _p(k_gamma), eps,
+                                   (ctypes.c_int * axes)(*pairs), theta, 0 if interleaved else 1, _p(gq), _p(gk), eps,
                                    _fitted(qo)[1], koh, dtype_code(odt), s))
         return qo if k is None else (qo, ko)
     return _launch(dev, stream, call)

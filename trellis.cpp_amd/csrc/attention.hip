@@ -668,6 +668,7 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
     const tsp_heads kk = nk ? *k : empty, vv = nk ? *v : empty;
     TSP_REQUIRE(heads_aligned(*q) && heads_aligned(*out) && heads_aligned(kk) && heads_aligned(vv), TSP_ERR_INVALID,
                 "tsp_attention: data must be 16-byte aligned, strides multiples of 8 (a row's up to 2^20)");
+    TSP_REQUIRE(nk == 0 || (kk.row_stride >= d && vv.row_stride >= d), TSP_ERR_INVALID, "tsp_attention: k's and v's rows overlap");
     TSP_REQUIRE(heads_apart(*out, nq, hq, d), TSP_ERR_INVALID, "tsp_attention: the output's heads overlap");
     TSP_REQUIRE(out->data != kk.data && out->data != vv.data && out->data != q->data, TSP_ERR_INVALID, "tsp_attention: out must not alias q, k or v");
     const int share = hq / hkv;

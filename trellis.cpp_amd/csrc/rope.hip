@@ -211,6 +211,8 @@ extern "C" int tsp_rope_axes(const tsp_heads* q, int hq, const tsp_heads* k, int
                 "tsp_rope_axes: null pointer");
     TSP_REQUIRE(heads_aligned(*q) && heads_aligned(*q_out) && (hk == 0 || (heads_aligned(*k) && heads_aligned(*k_out))), TSP_ERR_INVALID,
                 "tsp_rope_axes: data must be 16-byte aligned, strides multiples of 8 (a row's up to 2^20)");
+    TSP_REQUIRE(!(reinterpret_cast<uintptr_t>(d_q_gamma) % 16 || reinterpret_cast<uintptr_t>(d_k_gamma) % 16), TSP_ERR_INVALID,
+                "tsp_rope_axes: gamma must be 16-byte aligned");
     TSP_REQUIRE(heads_apart(*q_out, n, hq, d) && (hk == 0 || heads_apart(*k_out, n, hk, d)), TSP_ERR_INVALID,
                 "tsp_rope_axes: the output's heads overlap");
     RopeArgs a{};
