@@ -489,11 +489,13 @@ int tsp_rope_axes(const tsp_heads* q, int hq, const tsp_heads* k, int hk, int dt
  * != 0 those with j <= i + (Lk - Lq), i and j counted within the sample (the last query sees every key: a
  * prompt, or new tokens after a cache). q_offsets and k_offsets give the samples' rows in q and in k and
  * v. A row that sees no key gets zeros; a key that a row does not see has no effect on it, whatever it
- * holds. f16 or bf16 (out of the same type), d a multiple of 8 up to 128, hq % hkv == 0, scale > 0; data
- * 16-byte aligned, strides multiples of 8 (rows' up to 2^20; of k and v at least d; a head stride of 0 shares
- * one head's data). nq, nk and nq * hq / hkv below 2^31 - 2^16. out must not overlap the inputs. Where there are few queries
- * the keys are split over the device and the parts joined in the workspace, 16-byte aligned, of
- * tsp_attention_workspace_bytes bytes (0, and NULL will do, where they are not). */
+ * holds. q, k, v and out have one dtype: with f16 and bf16 the probabilities are rounded to it, f32 runs on
+ * the fp32 matrix cores (a sixteenth of the rate). d a multiple of 8 up to 128, hq % hkv == 0, scale > 0;
+ * data 16-byte aligned, strides multiples of 8 (rows' up to 2^20; of k and v at least d; a head stride of 0
+ * shares one head's data); nq, nk and nq * hq / hkv below 2^31 - 2^16; out must not overlap the inputs.
+ * Where there are few queries the keys are split over the device and the parts joined in the workspace,
+ * 16-byte aligned, of tsp_attention_workspace_bytes bytes (enough for every type and mask; 0, and NULL
+ * will do, where they are not). */
 size_t tsp_attention_workspace_bytes(int64_t nq, int64_t nk, int samples, int hq, int hkv, int d);
 int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_heads* v, int dtype, int64_t nq, int64_t nk,
                   int hq, int hkv, int d, const int32_t* d_q_offsets, const int32_t* d_k_offsets, int samples,

@@ -232,7 +232,7 @@ AT_CASES = [
 
 @pytest.mark.parametrize("case", range(len(AT_CASES)))
 @pytest.mark.parametrize("causal", [False, True])
-@pytest.mark.parametrize("key", ["f16", "bf16"])
+@pytest.mark.parametrize("key", ["f16", "bf16", "f32"])
 def test_attention(gpu_lib, case, causal, key):
     lens, hq, hkv, d = AT_CASES[case]
     print(f"[attention] {lens[:6]} heads {hq}/{hkv} d={d} causal={causal} {key}", flush=True)
@@ -292,7 +292,7 @@ def test_attention_views(gpu_lib):
 
 
 @pytest.mark.parametrize("d", [64, 128, 40])
-@pytest.mark.parametrize("key", ["f16", "bf16"])
+@pytest.mark.parametrize("key", ["f16", "bf16", "f32"])
 def test_attention_values_behind_the_mask(gpu_lib, d, key):
     """Infinities and NaN in keys and values that a row does not see: the next sample's, the rows between
     the samples, later keys of a causal sample. Rows that do see them get what the formula gives."""
@@ -316,12 +316,13 @@ def test_attention_values_behind_the_mask(gpu_lib, d, key):
 
 
 @pytest.mark.parametrize("hkv,lq,lk", [(1, 4, 300), (2, 7, 20_000), (4, 3, 61), (1, 8, 7), (2, 40, 5000)])
-def test_attention_few_rows_behind_the_mask(gpu_lib, hkv, lq, lk):
+@pytest.mark.parametrize("key", ["bf16", "f32"])
+def test_attention_few_rows_behind_the_mask(gpu_lib, hkv, lq, lk, key):
     """The same for a few new tokens against a cache, split or not: the last keys hold an Inf and a NaN that
     the earlier tokens do not see."""
     import torch
     randn = gen(lk)
-    q, k, v = randn(lq, 4, 64).bfloat16(), randn(lk, hkv, 64).bfloat16(), randn(lk, hkv, 64).bfloat16()
+    q, k, v = (randn(m, h, 64).to(dtype(key)) for m, h in ((lq, 4), (lk, hkv), (lk, hkv)))
     k[-1, 0, 5], v[-2, hkv - 1, 63], v[-1, 0, 0] = math.inf, math.nan, -math.inf
     out = gpu_lib.attention(q, k, v, causal=True)
     o, slack = ref.attention(q, k, v, [0, lq], [0, lk], True, 0.125)
@@ -392,6 +393,19 @@ def test_attention_cache_past_32_bits(gpu_lib):
         out = gpu_lib.attention(q, kv[:, :1], kv[:, 1:], causal=True)
         o, slack = ref.attention(q, data[:, :1], data[:, 1:], [0, nq], [0, rows], True, 0.125)
         ref.check(out, o, slack, f"{nq} rows")
+
+
+def test_attention_f32_views(gpu_lib):
+    """fp32 heads as views into one linear's output, and more rows than one workgroup's."""
+    import torch
+    randn = gen(41)
+    qkv = randn(333, 3, 4, 72)
+    q, k, v = qkv.unbind(1)
+    out = torch.full((333, 4, 80), -7.0, device="cuda")
+    gpu_lib.attention(q, k, v, causal=True, out=out[:, :, 8:])
+    o, slack = ref.attention(q, k, v, [0, 333], [0, 333], True, 72 ** -0.5)
+    ref.check(out[:, :, 8:], o, slack, "f32 views")
+    assert (out[:, :, :8] == -7).all()
 
 
 def test_attention_empty(gpu_lib):

@@ -77,7 +77,7 @@ def test_attention_refusals(pkg):
                                kw.get("scale", 0.125), 0, ref(o), kw.get("ws", FAKE), kw.get("wsb", 1 << 62), NULL)
     assert f(nq=-1) == 1 and f(nk=-1) == 1 and f(nq=1 << 31) == 1 and f(nk=(1 << 31) - 1) == 1
     assert f(hq=0) == 1 and f(hkv=0) == 1 and f(hkv=3) == 1 and f(hq=4, hkv=8) == 1 and "heads" in _err(pkg)
-    assert f(dt=3) == 1 and f(dt=0) == 4 and f(d=60) == 4 and f(d=136) == 4 and f(d=-8) == 4
+    assert f(dt=3) == 1 and f(dt=-1) == 1 and f(d=60) == 4 and f(d=136) == 4 and f(d=-8) == 4
     assert f(samples=0) == 1 and f(qoff=NULL) == 1 and f(koff=NULL) == 1
     for scale in (0.0, -1.0, math.nan, math.inf):
         assert f(scale=scale) == 1
@@ -87,11 +87,14 @@ def test_attention_refusals(pkg):
     assert f(k=_heads(pkg, 0x20000, 0)) == 1 and f(v=_heads(pkg, 0x30000, 56), nk=1) == 1 and "rows overlap" in _err(pkg)
     assert f(o=_heads(pkg, 0x10000)) == 1 and "alias" in _err(pkg)
     assert f(nq=0, q=None, o=None) == 0
-    need = L.tsp_attention_workspace_bytes(1, 100_000, 1, 16, 2, 128)
-    if need:
-        assert f(nq=1, nk=100_000, hq=16, hkv=2, d=128, samples=1, q=_heads(pkg, 0x10000, 2048, 128), k=_heads(pkg, 0x20000, 256, 128),
-                 v=_heads(pkg, 0x30000, 256, 128), o=_heads(pkg, 0x40000, 2048, 128), wsb=need - 1) == 5
-        assert "workspace" in _err(pkg)
+    # one token against a long cache: its keys are split, whatever the mask and type
+    assert L.tsp_attention_workspace_bytes(1, 100_000, 1, 16, 2, 128) > 1 << 16
+    few = dict(nq=1, nk=100_000, hq=16, hkv=2, d=128, samples=1, q=_heads(pkg, 0x10000, 2048, 128), k=_heads(pkg, 0x20000, 256, 128),
+               v=_heads(pkg, 0x30000, 256, 128), o=_heads(pkg, 0x40000, 2048, 128))
+    for dt in (0, 1, 2):
+        assert f(dt=dt, wsb=1024, **few) == 5 and "workspace" in _err(pkg)
+        assert f(dt=dt, ws=NULL, **few) == 1 and "null workspace" in _err(pkg)
+        assert f(dt=dt, ws=ctypes.c_void_p(0x1008), **few) == 1 and "aligned" in _err(pkg)
     assert L.tsp_attention_workspace_bytes(0, 5, 1, 8, 8, 64) == 0 and L.tsp_attention_workspace_bytes(5, 5, 1, 8, 3, 64) == 0
 
 

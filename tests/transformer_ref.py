@@ -67,12 +67,15 @@ def rope(x, pos, pairs, theta, interleaved, gamma, eps):
 def attention(q, k, v, q_bounds, k_bounds, causal, scale):
     """-> (o, slack), NaN outside the samples. slack: every probability is rounded to the 16-bit type (half a
     step of it, and 2^-25 of the largest below f16's normal range) and comes from a score with fp32 rounding
-    (2^-12 together), so what the sum of p |v| / sum p allows. Keys that a row does not see are left out."""
+    (2^-12 together), so what the sum of p |v| / sum p allows. fp32 heads: probabilities are not rounded; a
+    score of standard normal rows is off by at most d 2^-24 scale sum |q k| < 2^-14 for d <= 128, and a sum over
+    lk keys, two an addition, by lk 2^-25. Keys that a row does not see are left out."""
     nq, hq, d = q.shape
     hkv = k.shape[1]
     o = torch.full((nq, hq, d), math.nan, dtype=torch.float64, device=q.device)
     slack = torch.zeros_like(o)
-    part = half_step(q.dtype) + 2.0 ** -12
+    longest = max([b - a for a, b in zip(k_bounds, k_bounds[1:])], default=0)
+    part = 2.0 ** -14 + longest * 2.0 ** -25 if q.dtype == torch.float32 else half_step(q.dtype) + 2.0 ** -12
     for qa, qe, ka, ke in zip(q_bounds, q_bounds[1:], k_bounds, k_bounds[1:]):
         lq, lk = qe - qa, ke - ka
         if lq == 0:
@@ -104,7 +107,7 @@ def attention(q, k, v, q_bounds, k_bounds, causal, scale):
                     o[qa + i, h] = 0
                     continue
                 p = torch.softmax(ks[:m] @ qs[i] * scale, dim=0)
-                o[qa + i, h], slack[qa + i, h] = p @ vs[:m], part * (p @ vs[:m].abs()) + 2.0 ** -24 * vs[:m].abs().sum(0)
+                o[qa + i, h], slack[qa + i, h] = p @ vs[:m], part * (p @ vs[:m].abs()) + (2.0 ** -24 * vs[:m].abs().sum(0) if q.dtype == torch.float16 else 0.0)
     return o, slack
 
 

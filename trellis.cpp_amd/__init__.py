@@ -1013,7 +1013,7 @@ def attention_workspace(nq: int, nk: int, samples: int, hq: int, hkv: int, d: in
 
 
 def attention(q, k, v, q_offsets=None, k_offsets=None, causal: bool = False, scale=None, out=None, workspace=None, stream=None):
-    """Softmax attention within packed samples: q [Nq, Hq, D], k and v [Nk, Hkv, D] (f16 or bf16, D a
+    """Softmax attention within packed samples: q [Nq, Hq, D], k and v [Nk, Hkv, D] (one dtype, D a
     multiple of 8 up to 128, Hq a multiple of Hkv: head h of q reads head h // (Hq // Hkv)) -> [Nq, Hq, D].
     Row i of a sample sees all of the sample's keys, or with causal the keys j <= i + (Lk - Lq); a row that
     sees none gets zeros. q_offsets and k_offsets int32 [samples + 1] on the GPU: the samples' rows in q

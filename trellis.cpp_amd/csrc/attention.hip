@@ -20,48 +20,10 @@
 #include <algorithm>
 #include <cmath>
 
-#include "common.hpp"
-#include "packed.hpp"
+#include "attention_internal.hpp"
 
 namespace tsp {
 namespace {
-
-constexpr int AT_KEYS = 64;                   // keys of a tile
-constexpr int AT_MAX_D = 128;
-
-struct AttnArgs {
-    const uint16_t *q, *k, *v;
-    uint16_t* o;
-    int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;   // strides in elements
-    const int32_t *q_off, *k_off;
-    int64_t nq, nk;                           // below 2^31, nq * share too
-    int samples, hkv, share, d, causal;
-    int units;                                // of rows, a key head
-    int whole, splits;                        // the first `whole` of units * hkv see their keys at once, the others in splits
-    FastDiv by_share, by_heads, by_splits;
-    float scale2;                             // scale * log2(e)
-    float* part;                              // [unit past whole][split][row][d] sums of p v, and
-    float2* stat;                             // [unit past whole][split][row] maximum and sum of p (-1: no key seen)
-};
-
-// A unit of `ROWS` rows (query, head of the group) of one key head.
-struct AttnUnit {
-    PackedUnit u;      // its sample (-1: none)
-    int head, row0, rows;   // the key head, its first row, the sample's rows
-};
-// The key heads of one unit of rows follow each other (with 8 of them each XCD, which takes every eighth
-// workgroup, has one head's keys in its L2), the longest samples come first, and with causal a sample's last
-// rows, which see most.
-template <int ROWS, class Args>
-__device__ __forceinline__ AttnUnit attn_unit(const Args& a, int w) {
-    AttnUnit t;
-    const int unit = w / FastDiv{a.by_heads.mul, a.by_heads.shift};
-    t.head = w - unit * a.hkv;
-    t.u = packed_unit<true>(a.q_off, a.samples, (int)a.nq, a.share, ROWS, unit, a.k_off, (int)a.nk);
-    t.row0 = (a.causal ? t.u.count - 1 - (unit - t.u.first) : unit - t.u.first) * ROWS;
-    t.rows = t.u.rows * a.share;
-    return t;
-}
 
 template <bool BF16>
 __device__ __forceinline__ f32x16_t mfma32(const u32x4_t& a, const u32x4_t& b, const f32x16_t& c) {
@@ -84,12 +46,6 @@ template <bool BF16>
 __device__ __forceinline__ float add2(uint32_t p, float c) {
     if constexpr (BF16) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, p), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), c, false);
     else return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, p), __builtin_bit_cast(f16x2_t, 0x3c003c00u), c, false);
-}
-
-// The value of the other lane half (lane ^ 32), for both halves: {lower half's, upper half's}.
-__device__ __forceinline__ float2 both_halves(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return float2{__uint_as_float(r[0]), __uint_as_float(r[1])};
 }
 
 template <bool BF16>
@@ -125,14 +81,6 @@ __device__ __forceinline__ u32x4_t v_operand(const char* sv, int ks, int db, int
     const uint2 ua = __builtin_bit_cast(uint2, a), ub = __builtin_bit_cast(uint2, b);
     return u32x4_t{ua.x, ua.y, ub.x, ub.y};
 }
-
-// Waits for this wave's loads into LDS (which the compiler's own waits do not always cover).
-__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
-
-// Keys of a tile that a row sees, for the rows of a wave's 32.
-struct RowLimits {
-    int lane, hi;      // this lane's row, the wave's last
-};
 
 #ifdef __HIP_DEVICE_COMPILE__       // (the host pass knows neither the register constraint nor the argument segment)
 // Keeps a value in scalar registers of its own from here on.
@@ -185,13 +133,13 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
     // Q^T operand: d = 16 ks + 8 h .. + 7 of the lane's row
     u32x4_t qf[KS];
     {
-        const uint16_t* qp = a.q + (int64_t)(u.row0 + qi) * a.q_row + hq * a.q_head;
+        const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (int64_t)(u.row0 + qi) * a.q_row + hq * a.q_head;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
             qf[ks] = ks * 16 + h * 8 < a.d ? *reinterpret_cast<const u32x4_t*>(qp + ks * 16 + h * 8) : u32x4_t{0, 0, 0, 0};
     }
-    const char* kp = reinterpret_cast<const char*>(a.k + (int64_t)krow0 * a.k_row + head * a.k_head);
-    const char* vp = reinterpret_cast<const char*>(a.v + (int64_t)krow0 * a.v_row + head * a.v_head);
+    const char* kp = static_cast<const char*>(a.k) + 2 * ((int64_t)krow0 * a.k_row + head * a.k_head);
+    const char* vp = static_cast<const char*>(a.v) + 2 * ((int64_t)krow0 * a.v_row + head * a.v_head);
     int k_bytes = (int)a.k_row * 2, v_bytes = (int)a.v_row * 2;      // of a row
     float scale2 = a.scale2;
     keep_scalar(kp);
@@ -479,7 +427,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
         const u32x4_t x = *reinterpret_cast<const u32x4_t*>(sO + k_piece<DP>(row, piece));
         if (rr >= rows || piece * 8 >= b.d) continue;
         const int qr = rr / FastDiv{b.by_share.mul, b.by_share.shift}, hr = head * b.share + rr - qr * b.share;
-        *reinterpret_cast<u32x4_t*>(b.o + (int64_t)(u.row0 + qr) * b.o_row + hr * b.o_head + piece * 8) = x;
+        *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(b.o) + (int64_t)(u.row0 + qr) * b.o_row + hr * b.o_head + piece * 8) = x;
     }
 #endif
 }
@@ -489,7 +437,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
 // added in LDS in their order. A split whose scores were all -inf has sums of 0 (or NaN): its weight does
 // not matter. G = 1 for up to 16 splits, 16 beyond.
 constexpr int AT_MAX_SPLITS = 256, AT_FEW_SPLITS = 16;
-template <bool BF16, int G, int ROWS>
+template <int DT, int G, int ROWS>
 __global__ __launch_bounds__(256) void k_attention_join(AttnArgs a) {
     constexpr int ITEMS = 16 / G, BLOCKS = ROWS / ITEMS;
     __shared__ float sW[ITEMS][G == 1 ? AT_FEW_SPLITS : AT_MAX_SPLITS];     // weights; -1: no key seen
@@ -574,12 +522,20 @@ __global__ __launch_bounds__(256) void k_attention_join(AttnArgs a) {
     }
     if (!live || e >= a.d) return;
     const float inv = 1.0f / sum;
-    u32x4_t y{0, 0, 0, 0};
-    if (seen)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = pack2<BF16>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
     const int qi = r / a.by_share, hq = w.head * a.share + r - qi * a.share;
-    *reinterpret_cast<u32x4_t*>(a.o + (int64_t)(w.u.row0 + qi) * a.o_row + hq * a.o_head + e) = y;
+    const int64_t to = (int64_t)(w.u.row0 + qi) * a.o_row + hq * a.o_head + e;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = seen ? acc[i] * inv : 0.f;
+    if constexpr (DT == TSP_F32) {
+        f32x4_t* y = reinterpret_cast<f32x4_t*>(static_cast<float*>(a.o) + to);
+        y[0] = f32x4_t{acc[0], acc[1], acc[2], acc[3]};
+        y[1] = f32x4_t{acc[4], acc[5], acc[6], acc[7]};
+    } else {
+        u32x4_t y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = pack2<DT == TSP_BF16>(acc[2 * i], acc[2 * i + 1]);
+        *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.o) + to) = y;
+    }
 }
 
 // How a call is cut: waves of a workgroup (32 rows each), units of rows a key head, how many of them see
@@ -589,7 +545,7 @@ struct AttnCut {
     int64_t units, whole;
 };
 
-AttnCut attn_cut(int64_t nq, int64_t nk, int samples, int hkv, int share, int d, bool causal) {
+AttnCut attn_cut(int64_t nq, int64_t nk, int samples, int hkv, int share, int d, bool causal, bool f32) {
     AttnCut c;
     // one wave where a sample has at most its 32 rows (by the mean: the host does not know the lengths)
     c.nw = ceil_div(nq, samples) * share <= 32 ? 1 : 4;
@@ -605,7 +561,7 @@ AttnCut attn_cut(int64_t nq, int64_t nk, int samples, int hkv, int share, int d,
     // start and end, five or six for the join.
     const int64_t busy = (units + (samples > 1 ? samples / 2 : 0)) * hkv;
     const int64_t slots = 256 * (d > 64 ? 2 : c.nw == 1 ? 5 : 3);
-    const int64_t tiles = ceil_div(ceil_div(nk, samples), AT_KEYS);
+    const int64_t tiles = ceil_div(ceil_div(nk, samples), f32 ? AT_KEYS_F32 : AT_KEYS);
     c.whole = c.units * hkv;
     c.splits = 1;
     const int64_t full = busy / slots * slots;
@@ -643,8 +599,10 @@ using namespace tsp;
 
 extern "C" size_t tsp_attention_workspace_bytes(int64_t nq, int64_t nk, int samples, int hq, int hkv, int d) {
     if (nq <= 0 || nq >= (1ll << 31) || nk < 0 || nk >= (1ll << 31) - (1ll << 16) || samples <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || d <= 0) return 0;
-    return std::max(attn_workspace(attn_cut(nq, nk, samples, hkv, hq / hkv, d, false), hkv, d),
-                    attn_workspace(attn_cut(nq, nk, samples, hkv, hq / hkv, d, true), hkv, d));
+    size_t most = 0;      // (of either mask and type)
+    for (int i = 0; i < 4; ++i)
+        most = std::max(most, attn_workspace(attn_cut(nq, nk, samples, hkv, hq / hkv, d, i & 1, i & 2), hkv, d));
+    return most;
 }
 
 extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_heads* v, int dtype, int64_t nq, int64_t nk, int hq,
@@ -658,7 +616,6 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
     TSP_REQUIRE(samples > 0 && (samples == 1 || (d_q_offsets && d_k_offsets)), TSP_ERR_INVALID,
                 "tsp_attention: samples=%d (without offsets: 1)", samples);
     TSP_REQUIRE(std::isfinite(scale) && scale > 0.f, TSP_ERR_INVALID, "tsp_attention: scale=%g", scale);
-    TSP_REQUIRE(dtype != TSP_F32, TSP_ERR_UNSUPPORTED, "tsp_attention: f16 or bf16");
     TSP_REQUIRE(d > 0 && d % 8 == 0 && d <= AT_MAX_D, TSP_ERR_UNSUPPORTED, "tsp_attention: heads of %d (need a multiple of 8 up to %d)",
                 d, AT_MAX_D);
     if (nq == 0) return TSP_OK;
@@ -672,7 +629,7 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
     TSP_REQUIRE(heads_apart(*out, nq, hq, d), TSP_ERR_INVALID, "tsp_attention: the output's heads overlap");
     TSP_REQUIRE(out->data != kk.data && out->data != vv.data && out->data != q->data, TSP_ERR_INVALID, "tsp_attention: out must not alias q, k or v");
     const int share = hq / hkv;
-    const AttnCut c = attn_cut(nq, nk, samples, hkv, share, d, causal != 0);
+    const AttnCut c = attn_cut(nq, nk, samples, hkv, share, d, causal != 0, dtype == TSP_F32);
     const int64_t past = c.units * hkv - c.whole, blocks = c.whole + past * c.splits;
     TSP_REQUIRE(blocks * c.nw * 64 < (1ll << 32) && nq * share < (1ll << 31) - 1024, TSP_ERR_INVALID, "tsp_attention: too many rows");
     const size_t need = attn_workspace(c, hkv, d);
@@ -681,32 +638,41 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
     TSP_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0, TSP_ERR_INVALID, "tsp_attention: workspace not 16-byte aligned");
     float* part = need ? static_cast<float*>(d_workspace) : nullptr;
     float2* stat = need ? reinterpret_cast<float2*>(part + past * c.splits * c.nw * 32 * d) : nullptr;
-    const AttnArgs a{static_cast<const uint16_t*>(q->data), static_cast<const uint16_t*>(kk.data), static_cast<const uint16_t*>(vv.data),
-                     static_cast<uint16_t*>(out->data), q->row_stride, q->head_stride, kk.row_stride, kk.head_stride, vv.row_stride,
+    const AttnArgs a{q->data, kk.data, vv.data, out->data, q->row_stride, q->head_stride, kk.row_stride, kk.head_stride, vv.row_stride,
                      vv.head_stride, out->row_stride, out->head_stride, d_q_offsets, d_k_offsets, nq, nk, samples, hkv, share, d,
                      causal ? 1 : 0, (int)c.units, (int)c.whole, c.splits,
                      fast_div((uint32_t)share), fast_div((uint32_t)hkv), fast_div((uint32_t)c.splits), scale * 1.44269504088896340736f, part, stat};
     const dim3 grid((unsigned)blocks), block(c.nw * 64);
     hipStream_t s = as_stream(stream);
-    auto go = [&](auto bf, auto dp, auto nw) {
-        hipLaunchKernelGGL((k_attention<decltype(bf)::value, decltype(dp)::value, decltype(nw)::value>), grid, block, 0, s, a);
-        constexpr int ROWS = decltype(nw)::value * 32;
-        if (c.splits > AT_FEW_SPLITS)
-            hipLaunchKernelGGL((k_attention_join<decltype(bf)::value, 16, ROWS>), dim3((unsigned)(past * ROWS)), dim3(256), 0, s, a);
-        else if (c.splits > 1)
-            hipLaunchKernelGGL((k_attention_join<decltype(bf)::value, 1, ROWS>), dim3((unsigned)(past * ROWS / 16)), dim3(256), 0, s, a);
-    };
     using std::integral_constant;
-    auto by_width = [&](auto bf) {
-        auto by_waves = [&](auto dp) {
-            if (c.nw == 1) go(bf, dp, integral_constant<int, 1>{});
-            else go(bf, dp, integral_constant<int, 4>{});
-        };
-        if (d <= 64) by_waves(integral_constant<int, 64>{});
-        else by_waves(integral_constant<int, 128>{});
+    auto attend = [&](auto bf, auto dp, auto nw) {
+        hipLaunchKernelGGL((k_attention<decltype(bf)::value, decltype(dp)::value, decltype(nw)::value>), grid, block, 0, s, a);
     };
-    if (dtype == TSP_BF16) by_width(integral_constant<bool, true>{});
-    else by_width(integral_constant<bool, false>{});
+    auto by_width = [&](auto bf, auto nw) {
+        if (d <= 64) attend(bf, integral_constant<int, 64>{}, nw);
+        else attend(bf, integral_constant<int, 128>{}, nw);
+    };
+    auto join = [&](auto dt, auto nw) {
+        constexpr int DT = decltype(dt)::value, ROWS = decltype(nw)::value * 32;
+        if (c.splits > AT_FEW_SPLITS)
+            hipLaunchKernelGGL((k_attention_join<DT, 16, ROWS>), dim3((unsigned)(past * ROWS)), dim3(256), 0, s, a);
+        else if (c.splits > 1)
+            hipLaunchKernelGGL((k_attention_join<DT, 1, ROWS>), dim3((unsigned)(past * ROWS / 16)), dim3(256), 0, s, a);
+    };
+    auto by_type = [&](auto nw) {
+        if (dtype == TSP_BF16) {
+            by_width(std::true_type{}, nw);
+            join(integral_constant<int, TSP_BF16>{}, nw);
+        } else if (dtype == TSP_F16) {
+            by_width(std::false_type{}, nw);
+            join(integral_constant<int, TSP_F16>{}, nw);
+        } else {
+            launch_attention_f32(a, c.nw, (unsigned)blocks, s);
+            join(integral_constant<int, TSP_F32>{}, nw);
+        }
+    };
+    if (c.nw == 1) by_type(integral_constant<int, 1>{});
+    else by_type(integral_constant<int, 4>{});
     TSP_CHECK_LAUNCH();
     return TSP_OK;
 }
