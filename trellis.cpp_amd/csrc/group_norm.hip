@@ -6,6 +6,11 @@
 // per group in the workspace, the last normalises the rows; between them a sample's units are joined (in
 // the order of the units, whatever the order in which they ran), by a launch of its own where they are many.
 // Small samples take one launch.
+//
+// Bound by memory: x is read twice and out written once. Eight channels a thread (16 bytes of a 16-bit row),
+// four rows in flight; the last launch's first rows are on their way before its statistics. 599,577 x 128, f32 to
+// bf16, 2 samples: 72 us (4.3 TB/s), 5 and 74 us (6.2 TB/s: the second read comes from the memory-side cache in
+// part); 60,013 x 256, bf16, 6 samples: 9, 4 and 12.5 us.
 #include <algorithm>
 
 #include "common.hpp"

@@ -3,7 +3,12 @@
 // they are. With gamma, each head's row is RMS-normalised before: x / sqrt(mean(x^2) + eps) * gamma.
 //
 // An angle is formed in turns (pos * theta^(-j/P) / 2 pi) in 64 bits and only its fraction is rounded to
-// 32, so that a position of 10^9 turns as exactly as one of 10.
+// 32, so that a far position turns as exactly as a near one (to 2^-22 up to 2^28).
+//
+// Bound by memory: one read and one write. A row's sines and cosines (some 400 instructions for four pairs)
+// are formed once for all its heads; the heads' rows are loaded four at a time and kept packed until they
+// are turned. q and k of 35,001 rows x 8 heads of 128 with norms, bf16: 56 us, 5.1 TB/s; 117,343 x (16 + 4) heads
+// of 64, f16: 120 us, 5.0 TB/s (a copy of 4 GiB: 4.7).
 #include <algorithm>
 #include <cmath>
 
