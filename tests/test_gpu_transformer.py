@@ -140,7 +140,7 @@ ROPE_CASES = [
     # n, hq, hk, d, pairs, interleaved
     (1, 1, 0, 8, [4], True), (1, 1, 1, 8, [1, 1, 1, 1], False), (97, 16, 16, 64, [16, 16], False), (33, 3, 1, 128, [21, 21, 21], True),
     (40, 5, 2, 80, [13, 13, 13], False), (257, 8, 8, 96, [16, 0, 30], True), (19, 2, 2, 256, [128], False), (21, 4, 4, 40, [5], True),
-    (1000, 12, 12, 32, [8, 8], True), (3, 40, 8, 24, [0, 12], False), (5, 1, 7, 104, [30, 20], True), (2048, 16, 4, 64, [10, 10, 10], True),
+    (1000, 12, 12, 32, [8, 8], True), (37, 2, 1, 256, [40, 40, 40], True), (65, 1, 2, 200, [33, 33, 33], False), (3, 40, 8, 24, [0, 12], False), (5, 1, 7, 104, [30, 20], True), (2048, 16, 4, 64, [10, 10, 10], True),
 ]
 
 
@@ -377,6 +377,46 @@ def test_attention_leaves_other_rows(gpu_lib):
         guard = torch.full((400, 2, 64), -7.0, device="cuda", dtype=torch.float16)
         gpu_lib.attention(q, k, v, ints(qo), ints(ko), out=guard[100:300], causal=True)
         assert (guard[:100] == -7).all() and (guard[300:] == -7).all()
+
+
+@pytest.mark.parametrize("lo,hi,lk", [(2, 4, 9000), (1, 2, 30), (3, 300, 700), (5, 5, 100)])
+def test_attention_one_sample_inside(gpu_lib, lo, hi, lk):
+    """One sample that begins behind the first row and ends before the last, its keys split or not."""
+    import torch
+    randn = gen(lo)
+    q, k, v = randn(hi + 4, 4, 128).bfloat16(), randn(lk + 20, 2, 128).bfloat16(), randn(lk + 20, 2, 128).bfloat16()
+    k[:7], v[:7], k[7 + lk:], v[7 + lk:] = math.nan, math.inf, math.nan, math.nan
+    for causal in (False, True):
+        out = torch.full_like(q, -7.0)
+        gpu_lib.attention(q, k, v, ints([lo, hi]), ints([7, 7 + lk]), causal=causal, out=out)
+        assert (out[:lo] == -7).all() and (out[hi:] == -7).all()
+        o, slack = ref.attention(q[lo:hi], k[7:7 + lk], v[7:7 + lk], [0, hi - lo], [0, lk], causal, 128 ** -0.5)
+        ref.check(out[lo:hi], o, slack, "inside")
+
+
+def test_attention_many_rows(gpu_lib):
+    """More units than the device's rounds by far, and a last one of a single row."""
+    randn = gen(16)
+    q, k, v = randn(200_001, 2, 64).half(), randn(70, 1, 64).half(), randn(70, 1, 64).half()
+    o, slack = ref.attention(q, k, v, [0, 200_001], [0, 70], False, 0.125)
+    ref.check(gpu_lib.attention(q, k, v), o, slack, "many rows")
+
+
+def test_many_tiny_samples(gpu_lib):
+    """Two thousand samples of 0 to 2 rows."""
+    import torch
+    lens = [i % 3 for i in range(2000)]
+    bounds = ref.offsets_of(lens)
+    randn = gen(17)
+    x = randn(bounds[-1], 64)
+    y, slack = ref.group_norm(x, 8, bounds, None, None, 1e-5, False)
+    ref.check(gpu_lib.group_norm(x, 8, eps=1e-5, offsets=ints(bounds)), y, slack, "norm")
+    q = x.view(-1, 1, 64).half()
+    out = gpu_lib.attention(q, q, q, ints(bounds), ints(bounds), causal=True)
+    first = torch.tensor([a for a, m in zip(bounds, lens) if m], device="cuda")
+    assert torch.equal(out[first], q[first])       # a sample's first row sees itself alone
+    o, slack = ref.attention(q, q, q, bounds[:302], bounds[:302], True, 0.125)
+    ref.check(out[:bounds[301]], o[:bounds[301]], slack[:bounds[301]], "attention")
 
 
 def test_attention_cache_past_32_bits(gpu_lib):

@@ -948,11 +948,14 @@ def _fitted(t):
     return t, hd
 
 
-def _check_heads_out(out, like, dtype, name: str):
+def _heads_out(out, like, dtype, name: str):
+    """The tsp_heads of a caller's output."""
     if out.shape != like.shape or out.dtype != dtype or out.device != like.device:
         raise ValueError(f"{name} must be {dtype} {list(like.shape)} on {like.device}")
-    if _heads(out) is None:
+    hd = _heads(out)
+    if hd is None:
         raise ValueError(f"{name} must be 16-byte aligned with contiguous heads and strides that are multiples of 8")
+    return hd
 
 
 def rope_axes(q, pos, k=None, pairs=None, theta: float = 10000.0, interleaved: bool = True, q_gamma=None, k_gamma=None,
@@ -983,25 +986,24 @@ def rope_axes(q, pos, k=None, pairs=None, theta: float = 10000.0, interleaved: b
             raise ValueError(f"{name} must be a contiguous float32 {list(t.shape[1:])}")
     _same_device(dev, "k", k, "pos", pos, "q_gamma", q_gamma, "k_gamma", k_gamma)
     odt = out_dtype or (q_out.dtype if q_out is not None else k_out.dtype if k_out is not None else q.dtype)
-    for name, o, t in (("q_out", q_out, q), ("k_out", k_out, k)):
-        if o is not None:
-            _check_heads_out(o, t, odt, name)
+    qoh = None if q_out is None else _heads_out(q_out, q, odt, "q_out")
+    koh = None if k_out is None else _heads_out(k_out, k, odt, "k_out")
 
     def call(s, keep):
         qc, qh = _fitted(q)
-        qo = q_out if q_out is not None else torch.empty((n, hq, d), dtype=odt, device=dev)
-        kc = ko = kh = koh = None
-        if k is not None:
-            kc, kh = _fitted(k)
-            ko = k_out if k_out is not None else torch.empty(k.shape, dtype=odt, device=dev)
-            koh = _fitted(ko)[1]
+        kc, kh = (None, None) if k is None else _fitted(k)
+        qo, ko, qoh_, koh_ = q_out, k_out, qoh, koh
+        if qo is None:
+            qo, qoh_ = _fitted(torch.empty((n, hq, d), dtype=odt, device=dev))
+        if k is not None and ko is None:
+            ko, koh_ = _fitted(torch.empty(k.shape, dtype=odt, device=dev))
         pc = pos.contiguous()
         gq, gk = (g if g is None or g.data_ptr() % 16 == 0 else g.clone() for g in (q_gamma, k_gamma))
         keep(q, k, qc, kc, pos, pc, q_gamma, k_gamma, gq, gk, qo, ko)
         _check("tsp_rope_axes",
                lib().tsp_rope_axes(qh, hq, kh, 0 if k is None else k.shape[1], dtype_code(q.dtype), n, d, _p(pc), axes,
                                    (ctypes.c_int * axes)(*pairs), theta, 0 if interleaved else 1, _p(gq), _p(gk), eps,
-                                   _fitted(qo)[1], koh, dtype_code(odt), s))
+                                   qoh_, koh_, dtype_code(odt), s))
         return qo if k is None else (qo, ko)
     return _launch(dev, stream, call)
 
@@ -1034,14 +1036,13 @@ def attention(q, k, v, q_offsets=None, k_offsets=None, causal: bool = False, sca
     if samples != k_samples:
         raise ValueError("q_offsets and k_offsets must name the same samples")
     _same_device(dev, "k", k, "v", v, "q_offsets", q_offsets, "k_offsets", k_offsets, "workspace", workspace)
-    if out is not None:
-        _check_heads_out(out, q, q.dtype, "out")
+    given = None if out is None else _heads_out(out, q, q.dtype, "out")
     if workspace is not None:
         _check_workspace(workspace)
 
     def call(s, keep):
         (qc, qh), (kc, kh), (vc, vh) = _fitted(q), _fitted(k), _fitted(v)
-        o = out if out is not None else torch.empty((nq, hq, d), dtype=q.dtype, device=dev)
+        o, oh = (out, given) if out is not None else _fitted(torch.empty((nq, hq, d), dtype=q.dtype, device=dev))
         ws = workspace
         if ws is None:
             need = lib().tsp_attention_workspace_bytes(nq, nk, samples, hq, hkv, d)
@@ -1049,7 +1050,7 @@ def attention(q, k, v, q_offsets=None, k_offsets=None, causal: bool = False, sca
         keep(q, k, v, qc, kc, vc, q_offsets, k_offsets, o, ws)
         _check("tsp_attention",
                lib().tsp_attention(qh, kh, vh, dtype_code(q.dtype), nq, nk, hq, hkv, d, _p(q_offsets), _p(k_offsets), samples,
-                                   d ** -0.5 if scale is None else scale, 1 if causal else 0, _fitted(o)[1], _p(ws),
+                                   d ** -0.5 if scale is None else scale, 1 if causal else 0, oh, _p(ws),
                                    0 if ws is None else ws.numel(), s))
         return o
     return _launch(dev, stream, call)
