@@ -266,6 +266,30 @@ def test_attention_spread_and_growing_maximum(gpu_lib, spread, key):
     assert torch.isfinite(out).all()
 
 
+@pytest.mark.parametrize("key", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("rows,lk", [(200, 20_000), (1, 20_000), (64, 130)])
+@pytest.mark.parametrize("gap", [9.0, 10.5, 15.0])
+def test_attention_many_small_probabilities(gpu_lib, key, rows, lk, gap):
+    """One key far above thousands of equal ones, whose probabilities are below f16's normal range and together
+    weigh as much as its: they count in the sums as in the products."""
+    import torch
+    d = 64
+    q = torch.zeros(rows, 1, d, device="cuda")
+    q[:, 0, 0] = 4.0
+    k = torch.zeros(lk, 1, d, device="cuda")
+    k[lk // 2, 0, 0] = gap / 4.0
+    randn = gen(lk)
+    q, k, v = q.to(dtype(key)), k.to(dtype(key)), (randn(lk, 1, d) * 0.1 + 1.0).to(dtype(key))
+    out = gpu_lib.attention(q, k, v, scale=1.0)
+    s = (q.double()[:, 0] @ k.double()[:, 0].t())
+    p = torch.softmax(s, dim=1)
+    want = (p @ v.double()[:, 0])[:, None]
+    # f16: a probability of 2^-24 units is off by half a unit, in the sum and in the product alike
+    rel = {"f16": 2.0 ** -11 + 2.0 ** -25 * math.exp(gap), "bf16": 2.0 ** -8, "f32": 2.0 ** -20 + lk * 2.0 ** -25}[key]
+    slack = torch.full_like(want, 2 * rel + 2.0 ** -12 + lk * 2.0 ** -25) * v.double().abs().max()
+    ref.check(out, want, slack, "small probabilities")
+
+
 def test_attention_views(gpu_lib):
     """Views into one linear's output, heads first, unaligned, a head shared by broadcasting, and an output
     that is a view with other columns in it."""
