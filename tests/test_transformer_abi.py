@@ -62,6 +62,10 @@ def test_rope_refusals(pkg):
     assert f(q=_heads(pkg, 0x10008)) == 1 and f(q=_heads(pkg, row=516)) == 1 and f(k=_heads(pkg, row=1 << 21)) == 1
     assert f(qo=_heads(pkg, 0x30000, 256, 64)) == 1 and f(ko=_heads(pkg, 0x30000, 512, 32)) == 1 and "overlap" in _err(pkg)
     assert f(gq=ctypes.c_void_p(0x1004)) == 1 and f(gk=ctypes.c_void_p(0x1008)) == 1 and "gamma" in _err(pkg)
+    # an output that is another tensor of the call, or its own input seen differently
+    assert f(qo=_heads(pkg, 0x20000)) == 1 and f(ko=_heads(pkg, 0x10000)) == 1 and f(ko=_heads(pkg, 0x30000)) == 1
+    assert f(qo=_heads(pkg, 0x10000), odt=0) == 1 and f(ko=_heads(pkg, 0x20000, 1024, 64)) == 1
+    assert f(qo=_heads(pkg, 0x10000, 64, 6400)) == 1 and "its own input" in _err(pkg)
     assert f(n=0, q=None, pos=NULL) == 0
     assert f(n=0, q=None, pos=NULL, k=None, hk=0) == 0
 

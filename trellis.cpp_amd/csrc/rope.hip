@@ -220,6 +220,13 @@ extern "C" int tsp_rope_axes(const tsp_heads* q, int hq, const tsp_heads* k, int
                 "tsp_rope_axes: gamma must be 16-byte aligned");
     TSP_REQUIRE(heads_apart(*q_out, n, hq, d) && (hk == 0 || heads_apart(*k_out, n, hk, d)), TSP_ERR_INVALID,
                 "tsp_rope_axes: the output's heads overlap");
+    // in place a group of lanes has read its heads before it writes them: they must be the same ones
+    auto other = [&](const tsp_heads& x, const tsp_heads& y, int heads) {
+        return x.data == y.data && (dtype != out_dtype || (n > 1 && x.row_stride != y.row_stride) || (heads > 1 && x.head_stride != y.head_stride));
+    };
+    TSP_REQUIRE(!other(*q, *q_out, hq) && (hk == 0 || (!other(*k, *k_out, hk) && q->data != k_out->data && k->data != q_out->data &&
+                                                       q_out->data != k_out->data)),
+                TSP_ERR_INVALID, "tsp_rope_axes: an output may be its own input, with one dtype and the same strides, and no other");
     RopeArgs a{};
     auto side = [](const tsp_heads& x, const tsp_heads& y, const float* g, int heads) {
         return RopeSide{x.data, y.data, x.row_stride, x.head_stride, y.row_stride, y.head_stride, g, heads};
