@@ -72,6 +72,18 @@ def test_group_norm_far_mean_and_constant(gpu_lib, c, groups):
     assert (out[:, : c // groups] == 0).all()
 
 
+@pytest.mark.parametrize("n,c,groups", [(900, 64, 8), (900, 64, 32), (30_000, 64, 8), (30_000, 8, 1), (9000, 64, 32), (9000, 128, 64), (60_000, 36, 4), (40, 4104, 8)])
+@pytest.mark.parametrize("rows", [1, 40, 400])
+def test_group_norm_outliers_first(gpu_lib, n, c, groups, rows):
+    """The first row, or the first few, far from all others: the sums must not go about its values (a variance of
+    n values is then one n-th of what is summed)."""
+    randn = gen(rows)
+    x = randn(n, c)
+    x[:min(rows, n // 2)] += 3.0e4
+    y, slack = ref.group_norm(x, groups, [0, n], None, None, 1e-6, False)
+    ref.check(gpu_lib.group_norm(x, groups), y, slack, "outliers first")
+
+
 @pytest.mark.parametrize("c,groups", [(64, 8), (36, 4)])
 def test_group_norm_leaves_other_rows(gpu_lib, c, groups):
     """Rows before the first and behind the last sample keep what out held; a NaN stays in its sample and
@@ -133,6 +145,20 @@ def test_group_norm_bad_offsets_stay_inside(gpu_lib):
         guard = torch.full((600, 64), -7.0, device="cuda")
         gpu_lib.group_norm(x, 8, offsets=ints(bounds), out=guard[100:500])
         assert (guard[:100] == -7).all() and (guard[500:] == -7).all()
+
+
+@pytest.mark.parametrize("n,c", [(6000, 64), (20_000, 64), (6000, 60), (20_000, 60)])
+def test_group_norm_bad_offsets_in_the_workspace(gpu_lib, n, c):
+    """Offsets that name the same rows again and again have more units than the workspace holds: nothing behind
+    it is read (there are NaN there) or written."""
+    import torch
+    x = gen(19)(n, c)
+    need = gpu_lib.group_norm_workspace(n, c, 4, 5).numel()
+    ws = torch.full((16 * need,), 255, dtype=torch.uint8, device="cuda")
+    guard = torch.full((n + 200, c), -7.0, device="cuda")
+    gpu_lib.group_norm(x, 4, offsets=ints([0, n, 0, n, 0, n]), out=guard[100:100 + n], workspace=ws[:need])
+    assert (guard[:100] == -7).all() and (guard[100 + n:] == -7).all() and (ws[need:] == 255).all()
+    assert torch.isfinite(guard).all() and (guard[100:100 + n] != -7).all()
 
 
 # ---- rotary positions ---------------------------------------------------------------------------

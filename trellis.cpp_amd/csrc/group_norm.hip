@@ -9,8 +9,8 @@
 //
 // Bound by memory: x is read twice and out written once. Eight channels a thread (16 bytes of a 16-bit row),
 // four rows in flight; the last launch's first rows are on their way before its statistics. 599,577 x 128, f32 to
-// bf16, 2 samples: 72 us (4.3 TB/s), 5 and 74 us (6.2 TB/s: the second read comes from the memory-side cache in
-// part); 60,013 x 256, bf16, 6 samples: 9, 4 and 12.5 us.
+// bf16, 2 samples: 63 us (4.9 TB/s), 6 and 75 us (6.1 TB/s: the second read comes from the memory-side cache in
+// part); 60,013 x 256, bf16, 6 samples: 10, 4 and 12 us.
 #include <algorithm>
 
 #include "common.hpp"
@@ -33,6 +33,7 @@ struct GnArgs {
     int c, groups, samples, per;
     float eps;
     int silu;
+    int units;             // workgroups of the first and the last launch, units in part
 };
 
 __device__ __forceinline__ int unit_rows(const PackedUnit& u, int unit, int per, int64_t& row) {
@@ -92,17 +93,38 @@ __device__ __forceinline__ float sum_over(float v, int lanes) {
     return v;
 }
 
-// Sums are of x minus the group's first value in the unit, so that a mean far from zero does not swallow
-// the variance.
-__device__ __forceinline__ float2 unit_stat(float s, float q, float shift, float count) {
-    const float m = s / count;
+// Mean, sum of squared deviations and count of some values.
+struct Stat {
+    float mean, dev, n;
+};
+// ... from sums of x - shift and of its square. A shift among the values keeps a mean far from zero from
+// swallowing the variance; of n values, one that is far from all others swallows log2 n bits of it.
+__device__ __forceinline__ float2 stat_of(float s, float q, float shift, float n) {
+    const float m = s / n;
     return float2{shift + m, fmaxf(q - s * m, 0.f)};
+}
+// `count` parts of `total` values joined by `lanes` lanes of which this is `sub`; all get the result. The sums go
+// about the mean of the first parts' means, one a lane, so that a first part far from the others does no harm
+// (parts that are all equal have their mean exactly).
+template <class Part>
+__device__ __forceinline__ float2 join_parts(int count, float total, int lanes, int sub, Part part) {
+    const float first = part(0).mean;
+    const float m0 = first + sum_over(part(min(sub, count - 1)).mean - first, lanes) / (float)lanes;
+    float s = 0.f, q = 0.f;
+#pragma unroll 8
+    for (int i = sub; i < count; i += lanes) {
+        const Stat t = part(i);
+        const float d = t.mean - m0;
+        s += t.n * d;
+        q += t.dev + t.n * d * d;
+    }
+    return stat_of(sum_over(s, lanes), sum_over(q, lanes), m0, total);
 }
 
 // One group of one unit a workgroup, element by element: any width and alignment.
 template <int XDT>
 __global__ __launch_bounds__(GN_NT) void k_gn_stats(GnArgs a) {
-    __shared__ float2 sPart[GN_NT / 64];
+    __shared__ float2 sPart[GN_NT];
     const PackedUnit u = packed_unit(a.offsets, a.samples, (int)a.n, 1, a.per, blockIdx.x);
     if (u.sample < 0) return;
     int64_t row;
@@ -110,30 +132,26 @@ __global__ __launch_bounds__(GN_NT) void k_gn_stats(GnArgs a) {
     const int cg = a.c / a.groups, g = blockIdx.y;
     const auto* x = reinterpret_cast<const typename Elem<XDT>::storage*>(a.x) + row * a.c + g * cg;
     const int64_t cnt = (int64_t)rows * cg;
-    const float shift = Elem<XDT>::load(x, 0);
-    float s = 0.f, q = 0.f;
+    float s = 0.f, q = 0.f, shift = 0.f;
     for (int64_t e = threadIdx.x; e < cnt; e += GN_NT) {
         const int64_t r = e / cg;
-        const float d = Elem<XDT>::load(x, r * a.c + (e - r * cg)) - shift;
-        s += d;
-        q += d * d;
+        const float v = Elem<XDT>::load(x, r * a.c + (e - r * cg));
+        if (e == threadIdx.x) shift = v;
+        s += v - shift;
+        q += (v - shift) * (v - shift);
     }
-    s = group_sum<64>(s);
-    q = group_sum<64>(q);
-    if ((threadIdx.x & 63) == 0) sPart[threadIdx.x >> 6] = float2{s, q};
+    auto held = [&](int t) { return (float)((cnt - t + GN_NT - 1) / GN_NT); };      // values of thread t
+    if (threadIdx.x < cnt) sPart[threadIdx.x] = stat_of(s, q, shift, held(threadIdx.x));
     __syncthreads();
-    if (threadIdx.x == 0) {
-        float S = 0.f, Q = 0.f;
-        for (int w = 0; w < GN_NT / 64; ++w) {
-            S += sPart[w].x;
-            Q += sPart[w].y;
-        }
-        a.part[(int64_t)blockIdx.x * a.groups + g] = unit_stat(S, Q, shift, (float)cnt);
-    }
+    if (threadIdx.x >= 64) return;
+    const float2 t = join_parts((int)min(cnt, (int64_t)GN_NT), (float)cnt, 64, threadIdx.x,
+                                [&](int i) { return Stat{sPart[i].x, sPart[i].y, held(i)}; });
+    if (threadIdx.x == 0) a.part[(int64_t)blockIdx.x * a.groups + g] = t;
 }
 
 // All groups of one unit a workgroup: a thread keeps the sums of eight channels (of one value, PER = 1,
-// where they lie in one group, else of each) over every lanes-th row; they meet in LDS.
+// where they lie in one group, else of each) over every lanes-th row, about the mean of the first of them;
+// they meet in LDS.
 template <int XDT, int PER>
 __global__ __launch_bounds__(GN_NT) void k_gn_stats_vec(GnArgs a) {
     __shared__ float2 sSum[GN_NT * PER];
@@ -144,16 +162,26 @@ __global__ __launch_bounds__(GN_NT) void k_gn_stats_vec(GnArgs a) {
     const int cols = a.c / 8, lanes = GN_NT / cols, cg = a.c / a.groups;
     const int lane = threadIdx.x / cols, col = threadIdx.x - lane * cols;
     const bool live = lane < lanes;
-    float s[PER] = {}, q[PER] = {}, shift[PER];
-    if (live) {
-#pragma unroll
-        for (int k = 0; k < PER; ++k)
-            shift[k] = Elem<XDT>::load(reinterpret_cast<const typename Elem<XDT>::storage*>(a.x), row * a.c + (col * 8 + k) / cg * cg);
-        constexpr int DEEP = 4;       // rows in flight (past the last: the last again, not counted)
+    constexpr int DEEP = 4, EACH = 8 / PER;      // rows in flight (past the last: the last again, not counted)
+    const int whole = rows / lanes, more = rows - whole * lanes;
+    auto held = [&](int l) { return (float)((whole + (l < more ? 1 : 0)) * EACH); };      // values of a sum of lane l
+    if (live && lane < rows) {
+        float s[PER] = {}, q[PER] = {}, shift[PER] = {};
         for (int r = lane; r < rows; r += DEEP * lanes) {
             float x[DEEP][8];
 #pragma unroll
             for (int i = 0; i < DEEP; ++i) load8<XDT>(a.x, (row + min(r + i * lanes, rows - 1)) * a.c + col * 8, x[i]);
+            if (r == lane) {
+#pragma unroll
+                for (int k = 0; k < PER; ++k) {
+                    float d = 0.f;
+#pragma unroll
+                    for (int i = 0; i < DEEP; ++i)
+#pragma unroll
+                        for (int e = 0; e < EACH; ++e) d += x[i][k + e] - x[0][k];
+                    shift[k] = x[0][k] + d * (1.f / (DEEP * EACH));
+                }
+            }
 #pragma unroll
             for (int i = 0; i < DEEP; ++i) {
                 if (r + i * lanes >= rows) break;
@@ -167,47 +195,33 @@ __global__ __launch_bounds__(GN_NT) void k_gn_stats_vec(GnArgs a) {
             }
         }
 #pragma unroll
-        for (int k = 0; k < PER; ++k) sSum[(lane * cols + col) * PER + k] = float2{s[k], q[k]};
+        for (int k = 0; k < PER; ++k) sSum[(lane * cols + col) * PER + k] = stat_of(s[k], q[k], shift[k], held(lane));
     }
     __syncthreads();
     const int lg = lanes_a_group(a.groups), sub = threadIdx.x & (lg - 1), slots = cg * PER / 8;
+    const float total = (float)rows * (float)cg;
     for (int g0 = 0; g0 < a.groups; g0 += GN_NT / lg) {
-        const int g = g0 + threadIdx.x / lg;
-        float S = 0.f, Q = 0.f;
-        if (g < a.groups)
-            for (int e = sub; e < lanes * slots; e += lg) {
-                const int l = e / slots;
-                const float2 t = sSum[l * cols * PER + g * slots + (e - l * slots)];
-                S += t.x;
-                Q += t.y;
-            }
-        S = sum_over(S, lg);
-        Q = sum_over(Q, lg);
-        if (g < a.groups && sub == 0)
-            a.part[(int64_t)blockIdx.x * a.groups + g] =
-                unit_stat(S, Q, Elem<XDT>::load(reinterpret_cast<const typename Elem<XDT>::storage*>(a.x), row * a.c + g * cg),
-                          (float)rows * (float)cg);
+        const int g = g0 + threadIdx.x / lg, at = min(g, a.groups - 1) * slots;
+        const float2 t = join_parts(min(lanes, rows) * slots, total, lg, sub, [&](int e) {
+            const int l = e / slots;
+            const float2 v = sSum[l * cols * PER + at + (e - l * slots)];
+            return Stat{v.x, v.y, held(l)};
+        });
+        if (g < a.groups && sub == 0) a.part[(int64_t)blockIdx.x * a.groups + g] = t;
     }
 }
 
-// Mean and 1 / sqrt(var + eps) of group g: the units' means and squared deviations joined about the first
-// unit's mean, by `lanes` lanes of which this is `sub`; all get the result.
+// Mean and 1 / sqrt(var + eps) of group g from the sample's units. (Offsets out of order can name more units
+// than there are: those are not read.)
 __device__ __forceinline__ float2 join_units(const GnArgs& a, const PackedUnit& u, int g, int lanes, int sub) {
     const float cg = (float)(a.c / a.groups), total = (float)u.rows * cg;
-    const float2* p = a.part + (int64_t)u.first * a.groups + g;
-    const float m0 = p->x;
-    float s = 0.f, q = 0.f;
-#pragma unroll 8
-    for (int i = sub; i < u.count; i += lanes) {
-        const float2 t = p[(int64_t)i * a.groups];
-        const float d = t.x - m0, n = (float)min(a.per, u.rows - i * a.per) * cg;
-        s += n * d;
-        q += t.y + n * d * d;
-    }
-    s = sum_over(s, lanes);
-    q = sum_over(q, lanes);
-    const float m = s / total;
-    return float2{m0 + m, 1.0f / sqrtf(fmaxf(q - s * m, 0.f) / total + a.eps)};
+    const int first = max(u.first, 0), count = min(u.count, a.units - first);
+    const float2* p = a.part + (int64_t)first * a.groups + g;
+    const float2 t = join_parts(count, total, lanes, sub, [&](int i) {
+        const float2 v = p[(int64_t)i * a.groups];
+        return Stat{v.x, v.y, (float)min(a.per, u.rows - i * a.per) * cg};
+    });
+    return float2{t.x, 1.0f / sqrtf(t.y / total + a.eps)};
 }
 
 // A wave a sample and group: where there are more than GN_FEW units, every workgroup of the last launch
@@ -217,7 +231,7 @@ __global__ __launch_bounds__(256) void k_gn_join(GnArgs a) {
     const int g = blockIdx.y * 4 + (threadIdx.x >> 6), sample = blockIdx.x;
     if (g >= a.groups) return;
     const PackedUnit u = packed_sample(a.offsets, (int)a.n, 1, a.per, sample);
-    if (u.rows == 0) return;
+    if (u.rows == 0 || u.first >= a.units) return;
     const float2 t = join_units(a, u, g, 64, threadIdx.x & 63);
     if ((threadIdx.x & 63) == 0) a.stat[(int64_t)sample * a.groups + g] = t;
 }
@@ -334,9 +348,13 @@ __global__ __launch_bounds__(GS_NT) void k_gn_small(GnArgs a) {
     for (int e = 0; e < 8; ++e) gamma[e] = 1.f, beta[e] = 0.f;
     if (a.gamma) load8<TSP_F32>(a.gamma, ch, gamma);
     if (a.beta) load8<TSP_F32>(a.beta, ch, beta);
-    // sums go about the group's first value, so that equal values have their mean exactly
+    // the first sums go about one of the group's values, so that equal ones have their mean exactly: about the
+    // median of three, as one far from all others would round the mean to its own precision
 #pragma unroll
-    for (int k = 0; k < PER; ++k) shift[k] = Elem<XDT>::load(first, k * (8 / PER));
+    for (int k = 0; k < PER; ++k) {
+        auto value = [&](int r) { return Elem<XDT>::load(first, (int64_t)r * a.c + k * (8 / PER)); };
+        shift[k] = __builtin_amdgcn_fmed3f(value(0), value(rows / 2), value(rows - 1));
+    }
     auto workgroup_sums = [&](float (&v)[PER], int buffer) {
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
@@ -436,7 +454,8 @@ extern "C" int tsp_group_norm(const void* d_x, int x_dtype, int64_t n, int c, in
     TSP_REQUIRE(units * GN_NT < (1ll << 32), TSP_ERR_INVALID, "tsp_group_norm: too many samples");
     hipStream_t s = as_stream(stream);
     float2* part = static_cast<float2*>(d_workspace);
-    const GnArgs a{d_x, d_out, d_offsets, d_gamma, d_beta, part, units > GN_FEW ? part + units * groups : nullptr, n, c, groups, samples, gn_per(n, c), eps, silu};
+    const GnArgs a{d_x, d_out, d_offsets, d_gamma, d_beta, part, units > GN_FEW ? part + units * groups : nullptr, n, c, groups, samples, gn_per(n, c), eps, silu,
+                   (int)units};
     // rows of whole 16-byte pieces, eight channels a thread; element by element otherwise
     const bool vec = c % 8 == 0 && c <= 8 * GN_NT && !(reinterpret_cast<uintptr_t>(d_x) % 16 || reinterpret_cast<uintptr_t>(d_out) % 16 ||
                        reinterpret_cast<uintptr_t>(d_gamma) % 16 || reinterpret_cast<uintptr_t>(d_beta) % 16);
