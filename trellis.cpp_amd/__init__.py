@@ -849,12 +849,12 @@ def _nothing(*tensors):
 def _launch(device, stream, call, *args):
     """call(stream pointer, keep, *args) on the device and stream; keep(*tensors) is told every tensor the
     call uses."""
-    cuda = _torch().cuda
+    torch = _torch()
     index = device.index
-    current = cuda.current_stream(index)
-    if stream is None and index == cuda.current_device():
-        return call(current.cuda_stream, _nothing, *args)
-    with _On(device, stream, current) as on:
+    if stream is None and index == torch.cuda.current_device():
+        # (the stream's pointer alone: a Stream object is 1 us, a tenth of the host's side of a call)
+        return call(torch._C._cuda_getCurrentRawStream(index), _nothing, *args)
+    with _On(device, stream, torch.cuda.current_stream(index)) as on:
         return call(on.stream.cuda_stream, on.keep, *args)
 
 
@@ -862,9 +862,11 @@ def _same_device(device, *named):
     """named: name, tensor, name, tensor, ..."""
     if device.type != "cuda":
         raise ValueError("tensors must live on the GPU")
-    for name, t in zip(named[::2], named[1::2]):
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} must live on {device}, got {t.device}")
+    index = device.index
+    for i in range(1, len(named), 2):
+        t = named[i]
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{named[i - 1]} must live on {device}, got {t.device}")
 
 
 def _p(t) -> int:
@@ -929,33 +931,39 @@ def group_norm(x, groups: int, gamma=None, beta=None, eps: float = 1e-6, silu: b
     return _launch(dev, stream, call)
 
 
-def _heads(t):
-    """t [N, H, D] as tsp_heads, or None where the kernels cannot read it as it lies."""
-    n, h, d = t.shape
+def _heads(t, n: int, h: int, d: int):
+    """t [n, h, d] as tsp_heads, or None where the kernels cannot read it as it lies."""
     row, head, one = t.stride()
     p = t.data_ptr()
+    if one == 1 and d <= row <= 1 << 20 and not (p & 15 or (row | head) & 7):
+        return Heads(p, row, head)
+    # (the stride of an axis of one may be anything)
     if p % 16 or (one != 1 and d != 1) or (n > 1 and (row % 8 or not d <= row <= 1 << 20)) or (h > 1 and head % 8):
         return None
     return Heads(p, row if n > 1 else h * d, head if h > 1 else d)
 
 
-def _fitted(t):
-    """(t, its tsp_heads), t copied where the kernels could not read it as it lies."""
-    hd = _heads(t)
+def _fitted(t, n: int, h: int, d: int):
+    """(t [n, h, d], its tsp_heads), t copied where the kernels could not read it as it lies."""
+    hd = _heads(t, n, h, d)
     if hd is None:
         t = t.clone(memory_format=_torch().contiguous_format)
-        hd = _heads(t) or Heads(t.data_ptr(), t.shape[1] * t.shape[2], t.shape[2])   # (D not of whole pieces: the library refuses it)
+        hd = _heads(t, n, h, d) or Heads(t.data_ptr(), h * d, d)   # (D not of whole pieces: the library refuses it)
     return t, hd
 
 
-def _heads_out(out, like, dtype, name: str):
+def _heads_out(out, n: int, h: int, d: int, dtype, device, name: str):
     """The tsp_heads of a caller's output."""
-    if out.shape != like.shape or out.dtype != dtype or out.device != like.device:
-        raise ValueError(f"{name} must be {dtype} {list(like.shape)} on {like.device}")
-    hd = _heads(out)
+    if out.shape != (n, h, d) or out.dtype != dtype or out.device != device:
+        raise ValueError(f"{name} must be {dtype} {[n, h, d]} on {device}")
+    hd = _heads(out, n, h, d)
     if hd is None:
         raise ValueError(f"{name} must be 16-byte aligned with contiguous heads and strides that are multiples of 8")
     return hd
+
+
+def _aligned(t):
+    return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
 
 
 def rope_axes(q, pos, k=None, pairs=None, theta: float = 10000.0, interleaved: bool = True, q_gamma=None, k_gamma=None,
@@ -970,6 +978,7 @@ def rope_axes(q, pos, k=None, pairs=None, theta: float = 10000.0, interleaved: b
     if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
         raise ValueError("q must be [N, Hq, D] and k [N, Hk, D]")
     n, hq, d = q.shape
+    hk = 0 if k is None else k.shape[1]
     dev = q.device
     if k is not None and k.dtype != q.dtype:
         raise ValueError("q and k must have one dtype")
@@ -978,32 +987,31 @@ def rope_axes(q, pos, k=None, pairs=None, theta: float = 10000.0, interleaved: b
     if pos.dtype != torch.int32 or pos.dim() != 2 or pos.shape[0] != n or not 1 <= pos.shape[1] <= 4:
         raise ValueError("pos must be int32 [N, axes] with 1 to 4 axes")
     axes = pos.shape[1]
-    pairs = [d // 2 // axes] * axes if pairs is None else [int(p) for p in pairs]
+    pairs = (d // 2 // axes,) * axes if pairs is None else tuple(map(int, pairs))
     if len(pairs) != axes:
         raise ValueError(f"pairs must name a count for each of {axes} axes")
-    for name, g, t in (("q_gamma", q_gamma, q), ("k_gamma", k_gamma, k)):
-        if g is not None and (g.dtype != torch.float32 or tuple(g.shape) != tuple(t.shape[1:]) or not g.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous float32 {list(t.shape[1:])}")
+    for name, g, h in (("q_gamma", q_gamma, hq), ("k_gamma", k_gamma, hk)):
+        if g is not None and (g.dtype != torch.float32 or g.shape != (h, d) or not g.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous float32 {[h, d]}")
     _same_device(dev, "k", k, "pos", pos, "q_gamma", q_gamma, "k_gamma", k_gamma)
     odt = out_dtype or (q_out.dtype if q_out is not None else k_out.dtype if k_out is not None else q.dtype)
-    qoh = None if q_out is None else _heads_out(q_out, q, odt, "q_out")
-    koh = None if k_out is None else _heads_out(k_out, k, odt, "k_out")
+    qoh = None if q_out is None else _heads_out(q_out, n, hq, d, odt, dev, "q_out")
+    koh = None if k_out is None else _heads_out(k_out, n, hk, d, odt, dev, "k_out")
 
     def call(s, keep):
-        qc, qh = _fitted(q)
-        kc, kh = (None, None) if k is None else _fitted(k)
+        qc, qh = _fitted(q, n, hq, d)
+        kc, kh = (None, None) if k is None else _fitted(k, n, hk, d)
         qo, ko, qoh_, koh_ = q_out, k_out, qoh, koh
         if qo is None:
-            qo, qoh_ = _fitted(torch.empty((n, hq, d), dtype=odt, device=dev))
+            qo, qoh_ = _fitted(torch.empty((n, hq, d), dtype=odt, device=dev), n, hq, d)
         if k is not None and ko is None:
-            ko, koh_ = _fitted(torch.empty(k.shape, dtype=odt, device=dev))
+            ko, koh_ = _fitted(torch.empty((n, hk, d), dtype=odt, device=dev), n, hk, d)
         pc = pos.contiguous()
-        gq, gk = (g if g is None or g.data_ptr() % 16 == 0 else g.clone() for g in (q_gamma, k_gamma))
+        gq, gk = _aligned(q_gamma), _aligned(k_gamma)
         keep(q, k, qc, kc, pos, pc, q_gamma, k_gamma, gq, gk, qo, ko)
         _check("tsp_rope_axes",
-               lib().tsp_rope_axes(qh, hq, kh, 0 if k is None else k.shape[1], dtype_code(q.dtype), n, d, _p(pc), axes,
-                                   (ctypes.c_int * axes)(*pairs), theta, 0 if interleaved else 1, _p(gq), _p(gk), eps,
-                                   qoh_, koh_, dtype_code(odt), s))
+               lib().tsp_rope_axes(qh, hq, kh, hk, dtype_code(q.dtype), n, d, _p(pc), axes, (ctypes.c_int * axes)(*pairs), theta,
+                                   0 if interleaved else 1, _p(gq), _p(gk), eps, qoh_, koh_, dtype_code(odt), s))
         return qo if k is None else (qo, ko)
     return _launch(dev, stream, call)
 
@@ -1036,13 +1044,13 @@ def attention(q, k, v, q_offsets=None, k_offsets=None, causal: bool = False, sca
     if samples != k_samples:
         raise ValueError("q_offsets and k_offsets must name the same samples")
     _same_device(dev, "k", k, "v", v, "q_offsets", q_offsets, "k_offsets", k_offsets, "workspace", workspace)
-    given = None if out is None else _heads_out(out, q, q.dtype, "out")
+    given = None if out is None else _heads_out(out, nq, hq, d, q.dtype, dev, "out")
     if workspace is not None:
         _check_workspace(workspace)
 
     def call(s, keep):
-        (qc, qh), (kc, kh), (vc, vh) = _fitted(q), _fitted(k), _fitted(v)
-        o, oh = (out, given) if out is not None else _fitted(torch.empty((nq, hq, d), dtype=q.dtype, device=dev))
+        (qc, qh), (kc, kh), (vc, vh) = _fitted(q, nq, hq, d), _fitted(k, nk, hkv, d), _fitted(v, nk, hkv, d)
+        o, oh = (out, given) if out is not None else _fitted(torch.empty((nq, hq, d), dtype=q.dtype, device=dev), nq, hq, d)
         ws = workspace
         if ws is None:
             need = lib().tsp_attention_workspace_bytes(nq, nk, samples, hq, hkv, d)
