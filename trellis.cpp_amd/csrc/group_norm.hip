@@ -34,6 +34,7 @@ struct GnArgs {
     float eps;
     int silu;
     int units;             // workgroups of the first and the last launch, units in part
+    FastDiv by_cols, by_group, by_slots;      // 16-byte pieces of a row (or of a small sample's slab), channels of a group, its sums of a lane
 };
 
 __device__ __forceinline__ int unit_rows(const PackedUnit& u, int unit, int per, int64_t& row) {
@@ -160,7 +161,7 @@ __global__ __launch_bounds__(GN_NT) void k_gn_stats_vec(GnArgs a) {
     int64_t row;
     const int rows = unit_rows(u, blockIdx.x, a.per, row);
     const int cols = a.c / 8, lanes = GN_NT / cols, cg = a.c / a.groups;
-    const int lane = threadIdx.x / cols, col = threadIdx.x - lane * cols;
+    const int lane = (int)threadIdx.x / a.by_cols, col = threadIdx.x - lane * cols;
     const bool live = lane < lanes;
     constexpr int DEEP = 4, EACH = 8 / PER;      // rows in flight (past the last: the last again, not counted)
     const int whole = rows / lanes, more = rows - whole * lanes;
@@ -203,7 +204,7 @@ __global__ __launch_bounds__(GN_NT) void k_gn_stats_vec(GnArgs a) {
     for (int g0 = 0; g0 < a.groups; g0 += GN_NT / lg) {
         const int g = g0 + threadIdx.x / lg, at = min(g, a.groups - 1) * slots;
         const float2 t = join_parts(min(lanes, rows) * slots, total, lg, sub, [&](int e) {
-            const int l = e / slots;
+            const int l = e / a.by_slots;
             const float2 v = sSum[l * cols * PER + at + (e - l * slots)];
             return Stat{v.x, v.y, held(l)};
         });
@@ -226,7 +227,7 @@ __device__ __forceinline__ float2 join_units(const GnArgs& a, const PackedUnit& 
 
 // A wave a sample and group: where there are more than GN_FEW units, every workgroup of the last launch
 // joining them for itself would read them all some hundred times over (512 units of 32 groups: 15 us).
-constexpr int GN_FEW = 64;
+constexpr int GN_FEW = 256;
 __global__ __launch_bounds__(256) void k_gn_join(GnArgs a) {
     const int g = blockIdx.y * 4 + (threadIdx.x >> 6), sample = blockIdx.x;
     if (g >= a.groups) return;
@@ -288,8 +289,8 @@ __global__ __launch_bounds__(GN_NT) void k_gn_apply_vec(GnArgs a) {
     if (u.sample < 0) return;
     int64_t row;
     const int rows = unit_rows(u, unit, a.per, row);
-    const int cols = a.c / 8, lanes = GN_NT / cols, cg = a.c / a.groups;
-    const int lane = threadIdx.x / cols, col = threadIdx.x - lane * cols;
+    const int cols = a.c / 8, lanes = GN_NT / cols;
+    const int lane = (int)threadIdx.x / a.by_cols, col = threadIdx.x - lane * cols;
     constexpr int DEEP = 4;
     float x[DEEP][8], f[8], b[8];
     auto load = [&](int r) {      // (past the last row: the last again, not stored)
@@ -307,7 +308,7 @@ __global__ __launch_bounds__(GN_NT) void k_gn_apply_vec(GnArgs a) {
     float mean[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const int g = (col * 8 + e) / cg;
+        const int g = (col * 8 + e) / a.by_group;
         mean[e] = sMean[g];
         f[e] *= sRstd[g];
     }
@@ -336,7 +337,7 @@ __global__ __launch_bounds__(GS_NT) void k_gn_small(GnArgs a) {
     packed_rows(a.offsets, blockIdx.y, (int)a.n, row0, rows);
     if (rows == 0) return;
     const int cg = a.c / a.groups, slab = cg < 8 ? 8 : cg, cols = slab / 8, lanes = GS_NT / cols;
-    const int lane = threadIdx.x / cols, col = threadIdx.x - lane * cols;
+    const int lane = (int)threadIdx.x / a.by_cols, col = threadIdx.x - lane * cols;
     const int ch = blockIdx.x * slab + col * 8;
     const int mine = lane < lanes ? (rows - lane + lanes - 1) / lanes : 0;       // rows of this thread
     const auto* first = reinterpret_cast<const typename Elem<XDT>::storage*>(a.x) + (int64_t)row0 * a.c + blockIdx.x * slab;
@@ -454,13 +455,14 @@ extern "C" int tsp_group_norm(const void* d_x, int x_dtype, int64_t n, int c, in
     TSP_REQUIRE(units * GN_NT < (1ll << 32), TSP_ERR_INVALID, "tsp_group_norm: too many samples");
     hipStream_t s = as_stream(stream);
     float2* part = static_cast<float2*>(d_workspace);
-    const GnArgs a{d_x, d_out, d_offsets, d_gamma, d_beta, part, units > GN_FEW ? part + units * groups : nullptr, n, c, groups, samples, gn_per(n, c), eps, silu,
-                   (int)units};
+    GnArgs a{d_x, d_out, d_offsets, d_gamma, d_beta, part, units > GN_FEW ? part + units * groups : nullptr, n, c, groups, samples, gn_per(n, c), eps, silu,
+             (int)units, fast_div(std::max(1, c / 8)), fast_div(c / groups), fast_div(c / groups % 8 == 0 ? c / groups / 8 : c / groups)};
     // rows of whole 16-byte pieces, eight channels a thread; element by element otherwise
     const bool vec = c % 8 == 0 && c <= 8 * GN_NT && !(reinterpret_cast<uintptr_t>(d_x) % 16 || reinterpret_cast<uintptr_t>(d_out) % 16 ||
                        reinterpret_cast<uintptr_t>(d_gamma) % 16 || reinterpret_cast<uintptr_t>(d_beta) % 16);
     if (vec && gn_small(n, c, groups, samples)) {
         const int cg = c / groups;
+        a.by_cols = fast_div(cg < 8 ? 1 : cg / 8);
         const dim3 grid((unsigned)(c / (cg < 8 ? 8 : cg)), (unsigned)samples), block(GS_NT);
         dt_switch(x_dtype, [&](auto xd) {
             dt_switch(out_dtype, [&](auto od) {
