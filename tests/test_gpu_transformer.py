@@ -72,6 +72,21 @@ def test_group_norm_far_mean_and_constant(gpu_lib, c, groups):
     assert (out[:, : c // groups] == 0).all()
 
 
+@pytest.mark.parametrize("n,c,groups,bounds", [(4096, 64, 32, None), (2049, 64, 8, [0, 1024, 1025, 1025, 2049]), (3001, 24, 24, [5, 3000]),
+                                               (1100, 64, 4, None), (9000, 64, 32, None), (500, 60, 4, None)])
+def test_group_norm_in_place(gpu_lib, n, c, groups, bounds):
+    """In place and apart, the same values."""
+    import torch
+    randn = gen(n)
+    x, gamma = randn(n, c), randn(c)
+    off = None if bounds is None else ints(bounds)
+    y, slack = ref.group_norm(x, groups, bounds or [0, n], gamma, None, 1e-6, True)
+    lo, hi = (0, n) if bounds is None else (bounds[0], bounds[-1])
+    out = gpu_lib.group_norm(x, groups, gamma, silu=True, offsets=off)
+    ref.check(out[lo:hi], y[lo:hi], slack[lo:hi], "apart")
+    assert gpu_lib.group_norm(x, groups, gamma, silu=True, offsets=off, out=x) is x and torch.equal(x[lo:hi], out[lo:hi])
+
+
 @pytest.mark.parametrize("n,c,groups", [(900, 64, 8), (900, 64, 32), (30_000, 64, 8), (30_000, 8, 1), (9000, 64, 32), (9000, 128, 64), (60_000, 36, 4), (40, 4104, 8)])
 @pytest.mark.parametrize("rows", [1, 40, 400])
 def test_group_norm_outliers_first(gpu_lib, n, c, groups, rows):
