@@ -356,7 +356,26 @@ def test_attention_views(gpu_lib):
     assert ((out - same).abs() <= 2.0 ** -9 * same.abs()).all()      # a mean of equal rows, p rounded to half steps
 
 
-@pytest.mark.parametrize("d", [64, 128, 40])
+@pytest.mark.parametrize("d", [8, 24, 32, 40, 56, 72, 80, 88, 96, 104, 120])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("key", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("lq,lk,hq,hkv", [(300, 1000, 2, 1), (5, 3001, 4, 2), (129, 64, 1, 1)])
+def test_attention_widths(gpu_lib, d, causal, key, lq, lk, hq, hkv):
+    """Heads of widths that are none of the kernels' own, as views beside other values and into an output whose
+    other columns stay."""
+    import torch
+    randn = gen(d)
+    q, kv = randn(lq, hq, d + 8).to(dtype(key)), randn(lk, 2, hkv, d + 16).to(dtype(key))
+    q[:, :, d:], kv[..., d:] = math.nan, math.inf
+    q, k, v = q[:, :, :d], kv[:, 0, :, :d], kv[:, 1, :, :d]
+    out = torch.full((lq, hq, d + 8), -7.0, device="cuda", dtype=dtype(key))
+    gpu_lib.attention(q, k, v, causal=causal, out=out[:, :, 8:])
+    o, slack = ref.attention(q, k, v, [0, lq], [0, lk], causal, d ** -0.5)
+    ref.check(out[:, :, 8:], o, slack, f"width {d}")
+    assert (out[:, :, :8] == -7).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 40, 96, 32, 80])
 @pytest.mark.parametrize("key", ["f16", "bf16", "f32"])
 def test_attention_values_behind_the_mask(gpu_lib, d, key):
     """Infinities and NaN in keys and values that a row does not see: the next sample's, the rows between

@@ -69,15 +69,15 @@ __device__ __forceinline__ bool nonfinite16(uint32_t b) {
 
 // Byte offsets in a staged tile of AT_KEYS rows of DP values, as 16-byte pieces. K is read 16 bytes of
 // one d at 32 consecutive keys: the piece is xored with the key, so that 16 keys cover all banks. V is
-// read 64 bytes of 4 consecutive keys: the 64-byte quarter is xored with the key.
+// read 64 bytes of 4 consecutive keys: the 64-byte quarter is xored with the key. (Rows of 32 and 96 values
+// begin in another quarter of the banks each by themselves.)
 template <int DP>
 __device__ __forceinline__ int k_piece(int key, int piece) {
-    constexpr int P = DP / 8;
-    return key * (DP * 2) + ((piece ^ (DP == 128 ? key & 15 : (key >> 1) & 7)) & (P - 1)) * 16;
+    return key * (DP * 2) + (piece ^ (DP == 128 ? key & 15 : DP == 96 || DP == 32 ? (key >> 2) & 3 : (key >> 1) & 7)) * 16;
 }
 template <int DP>
 __device__ __forceinline__ int v_piece(int key, int piece) {
-    return key * (DP * 2) + (piece ^ (DP == 128 ? (key & 3) << 2 : ((key >> 1) & 1) << 2)) * 16;
+    return key * (DP * 2) + (piece ^ (DP == 128 ? (key & 3) << 2 : DP == 96 || DP == 32 ? 0 : ((key >> 1) & 1) << 2)) * 16;
 }
 
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
@@ -166,13 +166,15 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
     // the buffer's range).
     constexpr int LOADS = TILE / 1024 / NW;
     // A lane's byte offsets within the tile's rows; those of loads PERIOD apart differ by whole rows alone.
-    constexpr int LOAD_ROWS = NW * (1024 / (DP * 2)), PERIOD = LOAD_ROWS >= 16 ? 1 : 16 / LOAD_ROWS;
+    constexpr int LOAD_PIECES = NW * 64, PERIOD = DP == 96 ? 3 : LOAD_PIECES / P >= 16 ? 1 : 16 * P / LOAD_PIECES;
+    constexpr int PERIOD_ROWS = PERIOD * LOAD_PIECES / P;
+    static_assert(PERIOD_ROWS % 16 == 0 && LOADS % PERIOD == 0, "the swizzles repeat every 16 keys");
     constexpr int NOWHERE = 1 << 30;         // past every tile's rows
     int k_at[PERIOD], v_at[PERIOD];
 #pragma unroll
     for (int i = 0; i < PERIOD; ++i) {
-        const int key = (i * NW + wave) * (1024 / (DP * 2)) + lane / P;
-        const int kp = k_piece<DP>(key, lane % P) / 16 % P, vp = v_piece<DP>(key, lane % P) / 16 % P;
+        const int at = (i * NW + wave) * 64 + lane, key = at / P, slot = at % P;
+        const int kp = k_piece<DP>(key, slot) / 16 % P, vp = v_piece<DP>(key, slot) / 16 % P;
         k_at[i] = kp * 8 < a.d ? key * k_bytes + kp * 16 : NOWHERE;
         v_at[i] = vp * 8 < a.d ? key * v_bytes + vp * 16 : NOWHERE;
         asm volatile("" : "+v"(k_at[i]), "+v"(v_at[i]));       // (computed here, not in every tile)
@@ -183,7 +185,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(s + (i * NW + wave) * 1024), 16,
-                                                     at[i % PERIOD] + i / PERIOD * PERIOD * LOAD_ROWS * bytes, 0, 0, 0);
+                                                     at[i % PERIOD] + i / PERIOD * PERIOD_ROWS * bytes, 0, 0, 0);
     };
     // K or V of the tile at key base
     auto stage_k = [&](int base, char* s) __attribute__((always_inline)) { stage(kp, k_bytes, base, k_at, s); };
@@ -333,7 +335,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
     };
     auto step = [&](int base, char* k_this, const char* k_next, const char* v_this, char* v_next, f32x16_t (&s)[2],
                     f32x16_t (&sn)[2]) __attribute__((always_inline)) {
-        constexpr int AHEAD = 4, NK = 2 * KS, PAIRS = 16 / NK, NV = 4 * DB;
+        constexpr int AHEAD = 4, NK = 2 * KS, NV = 4 * DB;
         u32x4_t pf[4], ring[AHEAD];
         landed();
         if (base + 2 * AT_KEYS < end) stage_k(base + 2 * AT_KEYS, k_this);
@@ -347,7 +349,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
             if (t + AHEAD < NK) ring[t % AHEAD] = k_operand(k_next, t + AHEAD);
             else ring[t % AHEAD] = v_operand<DP>(v_this, (t + AHEAD - NK) / DB, (t + AHEAD - NK) % DB, lane);
 #pragma unroll
-            for (int e = t * PAIRS; e < (t + 1) * PAIRS; ++e) {
+            for (int e = t * 16 / NK; e < (t + 1) * 16 / NK; ++e) {
                 const float x = __builtin_amdgcn_exp2f(fmaf(s[e / 8][2 * (e % 8)], scale2, -mc));
                 const float y = __builtin_amdgcn_exp2f(fmaf(s[e / 8][2 * (e % 8) + 1], scale2, -mc));
                 pf[e / 4][e % 4] = pack2<BF16>(x, y);
@@ -433,10 +435,9 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
         for (int g = 0; g < 4; ++g)
             *reinterpret_cast<uint2*>(sO + k_piece<DP>(r32, db * 4 + g) + h * 8) =
                 uint2{pack2<BF16>(o[db][4 * g] * inv, o[db][4 * g + 1] * inv), pack2<BF16>(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv)};
-    const int piece = lane % P;
 #pragma unroll
-    for (int i = 0; i < 32 / (64 / P); ++i) {
-        const int row = i * (64 / P) + lane / P, rr = tile0 + wave * 32 + row;
+    for (int i = 0; i < P / 2; ++i) {
+        const int row = (i * 64 + lane) / P, piece = (i * 64 + lane) % P, rr = tile0 + wave * 32 + row;
         const u32x4_t x = *reinterpret_cast<const u32x4_t*>(sO + k_piece<DP>(row, piece));
         if (rr >= rows || piece * 8 >= b.d) continue;
         const int qr = rr / FastDiv{b.by_share.mul, b.by_share.shift}, hr = head * b.share + rr - qr * b.share;
@@ -573,7 +574,7 @@ AttnCut attn_cut(int64_t nq, int64_t nk, int samples, int hkv, int share, int d,
     // unequal length, which fill each other's gaps.) Time is counted in tiles: about three for a workgroup's
     // start and end, five or six for the join.
     const int64_t busy = (units + (samples > 1 ? samples / 2 : 0)) * hkv;
-    const int64_t slots = 256 * (d > 64 ? 2 : c.nw == 1 ? 5 : 3);
+    const int64_t slots = 256 * (c.nw == 4 ? (d > 64 ? 2 : 3) : d > 96 || (f32 && d > 64) ? 2 : d > 64 ? 3 : 5);
     const int64_t tiles = ceil_div(ceil_div(nk, samples), f32 ? AT_KEYS_F32 : AT_KEYS);
     c.whole = c.units * hkv;
     c.splits = 1;
@@ -661,8 +662,12 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
     auto attend = [&](auto bf, auto dp, auto nw) {
         hipLaunchKernelGGL((k_attention<decltype(bf)::value, decltype(dp)::value, decltype(nw)::value>), grid, block, 0, s, a);
     };
+    // Heads are widened to the next of four widths (zeros that cost products and LDS): 10,000 rows and keys, 8 heads
+    // of 32 take 182 us at their own width and 238 at 64; of 80, 300 at 96 and 345 at 128.
     auto by_width = [&](auto bf, auto nw) {
-        if (d <= 64) attend(bf, integral_constant<int, 64>{}, nw);
+        if (d <= 32) attend(bf, integral_constant<int, 32>{}, nw);
+        else if (d <= 64) attend(bf, integral_constant<int, 64>{}, nw);
+        else if (d <= 96) attend(bf, integral_constant<int, 96>{}, nw);
         else attend(bf, integral_constant<int, 128>{}, nw);
     };
     auto join = [&](auto dt, auto nw) {
