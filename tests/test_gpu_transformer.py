@@ -415,6 +415,54 @@ def test_attention_few_rows_behind_the_mask(gpu_lib, hkv, lq, lk, key):
     assert torch.isfinite(out[:seen]).all()
 
 
+SKEWED = [
+    # query and key lengths: one long sample among short ones, few rows each or not
+    ([1] * 16, [100] * 9 + [30_000] + [7] * 6), ([1] * 64, [20_000] + [65] * 63), ([3, 0, 8, 1, 2], [9000, 50, 0, 1, 3]),
+    ([1, 1], [12_000, 1]), ([2] * 20, [64 * (i % 5) for i in range(19)] + [15_000]), ([300, 10, 1], [300, 6000, 40_000]),
+    ([1] * 5, [5000] * 5), ([8] * 16, [5000 + 300 * i for i in range(16)]), ([33, 40, 5, 1], [33, 20_000, 70, 1]),
+    ([0] * 7 + [1], [100] * 7 + [25_000]), ([1] * 65, [40_000] + [10] * 64),
+]
+
+
+@pytest.mark.parametrize("case", range(len(SKEWED)))
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 64), (2, 2, 128), (12, 3, 96)])
+@pytest.mark.parametrize("causal,key", [(True, "bf16"), (False, "f16"), (True, "f32")])
+def test_attention_skewed_lengths(gpu_lib, case, hq, hkv, d, causal, key):
+    """Splits by the samples' lengths: every row once, the same values again, rows behind the samples left."""
+    import torch
+    lq, lk = SKEWED[case]
+    qb, kb = ref.offsets_of(lq), ref.offsets_of(lk)
+    randn = gen(case)
+    q, k, v = randn(qb[-1] + 2, hq, d).to(dtype(key)), randn(kb[-1] + 3, hkv, d).to(dtype(key)), randn(kb[-1] + 3, hkv, d).to(dtype(key))
+    k[kb[-1]:], v[kb[-1]:] = math.nan, math.inf
+    out = torch.full_like(q, -7.0)
+    gpu_lib.attention(q, k, v, ints(qb), ints(kb), causal=causal, out=out)
+    assert (out[qb[-1]:] == -7).all()
+    o, slack = ref.attention(q, k, v, qb, kb, causal, d ** -0.5)
+    ref.check(out[:qb[-1]], o[:qb[-1]], slack[:qb[-1]], "skewed")
+    ws = gpu_lib.attention_workspace(q.shape[0], k.shape[0], len(lq), hq, hkv, d)
+    ws.fill_(255)
+    again = torch.full_like(q, -7.0)
+    gpu_lib.attention(q, k, v, ints(qb), ints(kb), causal=causal, out=again, workspace=ws)
+    assert torch.equal(again, out)
+
+
+def test_attention_bad_offsets_by_length(gpu_lib):
+    """Offsets that name the same rows again and again, in calls that split by length: nothing outside the tensor
+    or behind the workspace is written."""
+    import torch
+    randn = gen(43)
+    q, k, v = randn(20, 4, 64).half(), randn(9000, 2, 64).half(), randn(9000, 2, 64).half()
+    need = gpu_lib.attention_workspace(20, 9000, 6, 4, 2, 64).numel()
+    for qo, ko in (([0, 20, 0, 20, 0, 20, 0], [0, 9000, 0, 9000, 0, 9000, 0]), ([0, 20, 0, 20, 0, 20, 0], [0, 9000, 10, 20, 5, 9000, 1]),
+                   ([-5, 30, 2, 2**31 - 1, -2**31, 20, 20], [9000, 0, 9000, 0, 2**31 - 1, -2**31, 9000])):
+        for causal in (False, True):
+            guard = torch.full((60, 4, 64), -7.0, device="cuda", dtype=torch.float16)
+            ws = torch.full((4 * need,), 255, dtype=torch.uint8, device="cuda")
+            gpu_lib.attention(q, k, v, ints(qo), ints(ko), out=guard[20:40], causal=causal, workspace=ws[:need])
+            assert (guard[:20] == -7).all() and (guard[40:] == -7).all() and (ws[need:] == 255).all()
+
+
 def test_attention_many_samples(gpu_lib):
     """More samples than a wave has lanes, unequal and some empty, few and many rows each; the longest samples
     first or last."""

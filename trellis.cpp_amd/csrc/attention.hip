@@ -119,15 +119,23 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
     constexpr int KS = DP / 16, DB = DP / 32, P = DP / 8, ROWS = NW * 32;
     constexpr int TILE = AT_KEYS * DP * 2;
     __shared__ __attribute__((aligned(16))) char sK0[TILE], sK1[TILE], sV0[TILE], sV1[TILE];
-    int work = blockIdx.x, split = 0, splits = 1;
-    if (work >= a.whole) {
-        const int past = work - a.whole;
-        splits = a.splits;
-        const int at = past / FastDiv{a.by_splits.mul, a.by_splits.shift};
-        work = a.whole + at;
-        split = past - at * splits;
+    int split = 0, splits = 1;
+    AttnUnit t;
+    if (a.extra) {
+        const AttnItem item = attn_item<ROWS, AT_KEYS, true>(a, blockIdx.x);
+        t = item;
+        split = item.split;
+        splits = item.splits;
+    } else {
+        int work = blockIdx.x;
+        if (work >= a.whole) {
+            const int past = work - a.whole, at = past / FastDiv{a.by_splits.mul, a.by_splits.shift};
+            splits = a.splits;
+            work = a.whole + at;
+            split = past - at * splits;
+        }
+        t = attn_unit<ROWS>(a, work);
     }
-    const AttnUnit t = attn_unit<ROWS>(a, work);
     const PackedUnit& u = t.u;
     const int head = t.head, rows = t.rows, tile0 = t.row0;
     if (u.sample < 0) return;
@@ -197,7 +205,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
     float m = -INFINITY, l = 0.f;
 
     // this split's share of the workgroup's tiles
-    const int tiles = (wg_end + AT_KEYS - 1) / AT_KEYS, per = splits == 1 ? tiles : (tiles + splits - 1) / FastDiv{a.by_splits.mul, a.by_splits.shift};
+    const int tiles = (wg_end + AT_KEYS - 1) / AT_KEYS, per = (int)((unsigned)(tiles + splits - 1) / (unsigned)splits);
     const int begin = split * per * AT_KEYS, end = min(wg_end, begin + per * AT_KEYS);
     const bool causal = a.causal;
 
@@ -409,7 +417,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
     const auto& b = *reread_args();
     if (splits > 1) {
         if (r >= rows) return;
-        const int64_t item = ((int64_t)(work - b.whole) * splits + split) * ROWS + (r - tile0);
+        const int64_t item = (int64_t)((int)blockIdx.x - b.whole) * ROWS + (r - tile0);
         const bool seen = lim.lane > begin && begin < end;
         if (h == 0) b.stat[item] = float2{m, seen ? sum : -1.f};
         if (!seen) return;
@@ -448,115 +456,148 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
 
 // The splits' sums joined: sum_s w_s (p v)_s / sum_s w_s (sum p)_s, w_s = exp(max_s - max). A row and head
 // takes G groups of 16 lanes (8 elements each); the splits are dealt to the groups, whose sums are then
-// added in LDS in their order. A split whose scores were all -inf has sums of 0 (or NaN): its weight does
-// not matter. G = 1 for up to 16 splits, 16 beyond.
-constexpr int AT_MAX_SPLITS = 256, AT_FEW_SPLITS = 16;
-template <int DT, int G, int ROWS>
+// added in a fixed order. A split whose scores were all -inf has sums of 0 (or NaN): its weight does
+// not matter. G = 1 for up to 16 splits, 16 beyond; 4, a wave, for samples that are split by their lengths, where
+// some have few (128 rows of 16 samples, 11 splits each: 15 us with 16 groups a row, 7 with 4), 16 beyond 32.
+constexpr int AT_FEW_SPLITS = 16;
+template <int DT, int G, int ROWS, bool BY_LENGTH>
 __global__ __launch_bounds__(256) void k_attention_join(AttnArgs a) {
-    constexpr int ITEMS = 16 / G, BLOCKS = ROWS / ITEMS;
+    constexpr int ITEMS = 16 / G, EACH = G == 4 ? AT_MAX_SPLITS / 64 : 1;      // rows a workgroup, splits a lane
     __shared__ float sW[ITEMS][G == 1 ? AT_FEW_SPLITS : AT_MAX_SPLITS];     // weights; -1: no key seen
-    __shared__ float sAcc[G][AT_MAX_D], sSum[G];
+    __shared__ float sAcc[G == 16 ? G : 1][AT_MAX_D], sSum[16];
     const int lane = threadIdx.x & 15, group = threadIdx.x >> 4, e = lane * 8;
     const int g = group % G, at = group / G, mine = threadIdx.x % (G * 16);
-    const int past = blockIdx.x / BLOCKS, row = blockIdx.x % BLOCKS * ITEMS + at;
-    const AttnUnit w = attn_unit<ROWS>(a, a.whole + past);
-    const int r = w.row0 + row;
-    if (w.u.sample < 0 || w.row0 + row - at >= w.rows) return;
-    const bool live = r < w.rows;
-    const int64_t item = (int64_t)past * a.splits * ROWS + row;
-    constexpr int step = ROWS;
-    float m = -INFINITY, sum = 0.f;
-    float2 t{-INFINITY, -1.f};
-    if (live && mine < a.splits) t = a.stat[mine * step + item];
-    m = t.x;
-    if constexpr (G == 1) {
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 16));
+    const int spread = G == 1 ? ROWS / ITEMS : a.spread;      // workgroups of a unit
+    const int past = (int)(blockIdx.x / (unsigned)spread), first = (int)(blockIdx.x - (unsigned)past * spread) * ITEMS;
+    AttnUnit w;
+    int splits = a.splits;
+    int64_t slot = (int64_t)past * a.splits;      // of the first of them in part
+    if constexpr (BY_LENGTH) {
+        const AttnItem t = attn_item<ROWS, DT == TSP_F32 ? AT_KEYS_F32 : AT_KEYS, false>(a, past);
+        splits = t.splits;
+        // (a unit of one split has been written; splits past the last are of offsets out of order)
+        if (splits == 1 || t.part + splits > a.items) return;
+        w = t;
+        slot = t.part;
     } else {
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-        if ((threadIdx.x & 63) == 0) sSum[threadIdx.x >> 6] = m;
-        __syncthreads();
-        m = fmaxf(fmaxf(sSum[0], sSum[1]), fmaxf(sSum[2], sSum[3]));
-        __syncthreads();
+        w = attn_unit<ROWS>(a, a.whole + past);
     }
-    const float w0 = t.y == -1.f ? -1.f : t.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((t.x - m) * a.scale2);
-    if (mine < (G == 1 ? AT_FEW_SPLITS : AT_MAX_SPLITS)) sW[at][mine] = w0;
-    // the sum of p over all splits, and whether any saw a key
-    sum = t.y == -1.f ? 0.f : w0 * t.y;
-    bool seen = t.y != -1.f;
-    if constexpr (G == 1) {
+    if (w.u.sample < 0) return;
+    for (int row0 = first; row0 < ROWS && w.row0 + row0 < w.rows; row0 += spread * ITEMS) {
+        const int row = row0 + at, r = w.row0 + row;
+        const bool live = r < w.rows;
+        const int64_t item = slot * ROWS + row;
+        float2 t[EACH];
+        float m = -INFINITY;
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 16);
-        seen = (__ballot(seen) >> (threadIdx.x & 48)) & 0xffff;
-        __syncthreads();
-    } else {
+        for (int i = 0; i < EACH; ++i) {
+            t[i] = float2{-INFINITY, -1.f};
+            if (live && mine + i * 64 < splits) t[i] = a.stat[(int64_t)(mine + i * 64) * ROWS + item];
+            m = fmaxf(m, t[i].x);
+        }
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-        if ((threadIdx.x & 63) == 0) sSum[threadIdx.x >> 6] = sum;
-        seen = __syncthreads_or(seen);
-        sum = (sSum[0] + sSum[1]) + (sSum[2] + sSum[3]);
-    }
-    float acc[8] = {};
-    if (live && e < a.d) {
-        constexpr int BATCH = 8;      // splits on their way at a time
-        for (int s0 = g; s0 < a.splits; s0 += BATCH * G) {
-            f32x4_t x[BATCH], y[BATCH];
-            float w[BATCH];
+        for (int o = G == 1 ? 8 : 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+        if constexpr (G == 16) {
+            if ((threadIdx.x & 63) == 0) sSum[threadIdx.x >> 6] = m;
+            __syncthreads();
+            m = fmaxf(fmaxf(sSum[0], sSum[1]), fmaxf(sSum[2], sSum[3]));
+            __syncthreads();
+        }
+        // the sum of p over all splits, and whether any saw a key
+        float sum = 0.f;
+        bool seen = false;
 #pragma unroll
-            for (int b = 0; b < BATCH; ++b) {
-                const int s = s0 + b * G;
-                w[b] = s < a.splits ? sW[at][s] : -1.f;
-                x[b] = y[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-                if (w[b] == -1.f) continue;
-                const f32x4_t* p = reinterpret_cast<const f32x4_t*>(a.part + (s * step + item) * a.d + e);
-                x[b] = p[0];
-                y[b] = p[1];
+        for (int i = 0; i < EACH; ++i) {
+            const float w0 = t[i].y == -1.f ? -1.f : t[i].x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((t[i].x - m) * a.scale2);
+            if (mine + i * 64 < (G == 1 ? AT_FEW_SPLITS : AT_MAX_SPLITS)) sW[at][mine + i * 64] = w0;
+            if (t[i].y != -1.f) {
+                sum += w0 * t[i].y;
+                seen = true;
             }
+        }
 #pragma unroll
-            for (int b = 0; b < BATCH; ++b) {
-                if (w[b] == -1.f) continue;
+        for (int o = G == 1 ? 8 : 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        if constexpr (G == 16) {
+            if ((threadIdx.x & 63) == 0) sSum[threadIdx.x >> 6] = sum;
+            seen = __syncthreads_or(seen);
+            sum = (sSum[0] + sSum[1]) + (sSum[2] + sSum[3]);
+        } else {
+            const uint64_t any = __ballot(seen);
+            seen = G == 4 ? any != 0 : (any >> (threadIdx.x & 48) & 0xffff) != 0;
+            __syncthreads();
+        }
+        float acc[8] = {};
+        if (live && e < a.d) {
+            constexpr int BATCH = 8;      // splits on their way at a time
+            for (int s0 = g; s0 < splits; s0 += BATCH * G) {
+                f32x4_t x[BATCH], y[BATCH];
+                float c[BATCH];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    acc[i] += w[b] * x[b][i];
-                    acc[4 + i] += w[b] * y[b][i];
+                for (int b = 0; b < BATCH; ++b) {
+                    const int s = s0 + b * G;
+                    c[b] = s < splits ? sW[at][s] : -1.f;
+                    x[b] = y[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                    if (c[b] == -1.f) continue;
+                    const f32x4_t* p = reinterpret_cast<const f32x4_t*>(a.part + ((int64_t)s * ROWS + item) * a.d + e);
+                    x[b] = p[0];
+                    y[b] = p[1];
+                }
+#pragma unroll
+                for (int b = 0; b < BATCH; ++b) {
+                    if (c[b] == -1.f) continue;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        acc[i] += c[b] * x[b][i];
+                        acc[4 + i] += c[b] * y[b][i];
+                    }
                 }
             }
         }
-    }
-    if constexpr (G > 1) {
+        if constexpr (G == 4) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sAcc[g][e + i] = acc[i];
-        __syncthreads();
-        if (g != 0) return;
+            for (int i = 0; i < 8; ++i) {
+                acc[i] += __shfl_xor(acc[i], 16, 64);
+                acc[i] += __shfl_xor(acc[i], 32, 64);
+            }
+        } else if constexpr (G == 16) {
 #pragma unroll
-        for (int k = 1; k < G; ++k)
+            for (int i = 0; i < 8; ++i) sAcc[g][e + i] = acc[i];
+            __syncthreads();
+            if (g == 0) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] += sAcc[k][e + i];
-    }
-    if (!live || e >= a.d) return;
-    const float inv = 1.0f / sum;
-    const int qi = r / a.by_share, hq = w.head * a.share + r - qi * a.share;
-    const int64_t to = (int64_t)(w.u.row0 + qi) * a.o_row + hq * a.o_head + e;
+                for (int k = 1; k < G; ++k)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = seen ? acc[i] * inv : 0.f;
-    if constexpr (DT == TSP_F32) {
-        f32x4_t* y = reinterpret_cast<f32x4_t*>(static_cast<float*>(a.o) + to);
-        y[0] = f32x4_t{acc[0], acc[1], acc[2], acc[3]};
-        y[1] = f32x4_t{acc[4], acc[5], acc[6], acc[7]};
-    } else {
-        u32x4_t y;
+                    for (int i = 0; i < 8; ++i) acc[i] += sAcc[k][e + i];
+            }
+        }
+        if (live && e < a.d && g == 0) {
+            const float inv = 1.0f / sum;
+            const int qi = r / a.by_share, hq = w.head * a.share + r - qi * a.share;
+            const int64_t to = (int64_t)(w.u.row0 + qi) * a.o_row + hq * a.o_head + e;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = pack2<DT == TSP_BF16>(acc[2 * i], acc[2 * i + 1]);
-        *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.o) + to) = y;
+            for (int i = 0; i < 8; ++i) acc[i] = seen ? acc[i] * inv : 0.f;
+            if constexpr (DT == TSP_F32) {
+                f32x4_t* y = reinterpret_cast<f32x4_t*>(static_cast<float*>(a.o) + to);
+                y[0] = f32x4_t{acc[0], acc[1], acc[2], acc[3]};
+                y[1] = f32x4_t{acc[4], acc[5], acc[6], acc[7]};
+            } else {
+                u32x4_t y;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = pack2<DT == TSP_BF16>(acc[2 * i], acc[2 * i + 1]);
+                *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.o) + to) = y;
+            }
+        }
+        if constexpr (G > 1) __syncthreads();      // (the next rows' weights and sums go where these are read)
     }
 }
 
 // How a call is cut: waves of a workgroup (32 rows each), units of rows a key head, how many of them see
 // their keys at once, splits of the others' keys.
 struct AttnCut {
-    int nw, splits;
+    int nw, splits, even;      // (even: of samples of nearly one length)
     int64_t units, whole;
+    int64_t extra;        // or by the samples' lengths (attn_item), into this many items a key head beside one a unit
+    int64_t blocks(int hkv) const { return extra ? (units * splits + 2) * hkv : whole + (units * hkv - whole) * splits; }      // (2: work's rounding)
 };
 
 AttnCut attn_cut(int64_t nq, int64_t nk, int samples, int hkv, int share, int d, bool causal, bool f32) {
@@ -577,7 +618,8 @@ AttnCut attn_cut(int64_t nq, int64_t nk, int samples, int hkv, int share, int d,
     const int64_t slots = 256 * (c.nw == 4 ? (d > 64 ? 2 : 3) : d > 96 || (f32 && d > 64) ? 2 : d > 64 ? 3 : 5);
     const int64_t tiles = ceil_div(ceil_div(nk, samples), f32 ? AT_KEYS_F32 : AT_KEYS);
     c.whole = c.units * hkv;
-    c.splits = 1;
+    c.splits = c.even = 1;
+    c.extra = 0;
     const int64_t full = busy / slots * slots;
     if (busy == full || (full > 0 && (samples > 1 || causal))) return c;
     auto rounds = [&](int64_t n, int64_t length) {
@@ -599,11 +641,22 @@ AttnCut attn_cut(int64_t nq, int64_t nk, int samples, int hkv, int share, int d,
             c.whole = full;
         }
     }
+    // Several samples may differ in length, which only the device knows. Those of few rows get a part in the join
+    // even where their mean asks for none, if one of them can be long: a row each of 64 samples, 16 heads on 2 of
+    // 128, 50,000 keys in all, takes 27 us, not 721, where one has nearly all of them (and 26, not 23, where all have 781).
+    c.even = c.splits;
+    if (samples > 1 && samples <= 64 && (c.splits > 1 || (c.nw == 1 && tiles * samples >= 256))) {
+        c.splits = std::max(c.splits, 2);
+        c.whole = 0;
+        // whole rounds of equal splits, where there are as many
+        const int64_t items = busy * c.splits, n = items * 10 < slots * 7 ? items : std::max<int64_t>(1, (2 * items + slots) / (2 * slots)) * slots;
+        c.extra = std::min(std::max(n / hkv - c.units, c.units), c.units * (c.splits - 1));
+    }
     return c;
 }
 
 size_t attn_workspace(const AttnCut& c, int hkv, int d) {
-    return c.splits == 1 ? 0 : (size_t)(c.units * hkv - c.whole) * c.splits * c.nw * 32 * (d * sizeof(float) + sizeof(float2));
+    return c.splits == 1 ? 0 : (size_t)(c.blocks(hkv) - c.whole) * c.nw * 32 * (d * sizeof(float) + sizeof(float2));
 }
 
 }  // namespace
@@ -644,17 +697,20 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
     TSP_REQUIRE(out->data != kk.data && out->data != vv.data && out->data != q->data, TSP_ERR_INVALID, "tsp_attention: out must not alias q, k or v");
     const int share = hq / hkv;
     const AttnCut c = attn_cut(nq, nk, samples, hkv, share, d, causal != 0, dtype == TSP_F32);
-    const int64_t past = c.units * hkv - c.whole, blocks = c.whole + past * c.splits;
+    const int64_t past = c.units * hkv - c.whole, blocks = c.blocks(hkv);
     TSP_REQUIRE(blocks * c.nw * 64 < (1ll << 32) && nq * share < (1ll << 31) - 1024, TSP_ERR_INVALID, "tsp_attention: too many rows");
     const size_t need = attn_workspace(c, hkv, d);
     TSP_REQUIRE(need == 0 || d_workspace, TSP_ERR_INVALID, "tsp_attention: null workspace");
     TSP_REQUIRE(workspace_bytes >= need, TSP_ERR_WORKSPACE, "tsp_attention: workspace of %zu bytes, needs %zu", workspace_bytes, need);
     TSP_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0, TSP_ERR_INVALID, "tsp_attention: workspace not 16-byte aligned");
     float* part = need ? static_cast<float*>(d_workspace) : nullptr;
-    float2* stat = need ? reinterpret_cast<float2*>(part + past * c.splits * c.nw * 32 * d) : nullptr;
+    float2* stat = need ? reinterpret_cast<float2*>(part + (blocks - c.whole) * c.nw * 32 * d) : nullptr;
+    // workgroups of a unit's join, by the mean rows of a unit
+    const bool many = c.splits > (c.extra ? 2 * AT_FEW_SPLITS : AT_FEW_SPLITS);
+    const int rows = (int)std::min<int64_t>(ceil_div(nq * share, samples), c.nw * 32), spread = many ? rows : c.extra ? (rows + 3) / 4 : c.nw * 2;
     const AttnArgs a{q->data, kk.data, vv.data, out->data, q->row_stride, q->head_stride, kk.row_stride, kk.head_stride, vv.row_stride,
                      vv.head_stride, out->row_stride, out->head_stride, d_q_offsets, d_k_offsets, nq, nk, samples, hkv, share, d,
-                     causal ? 1 : 0, (int)c.units, (int)c.whole, c.splits,
+                     causal ? 1 : 0, (int)c.whole, c.extra ? c.even : c.splits, (int)c.extra, (int)blocks, spread,
                      fast_div((uint32_t)share), fast_div((uint32_t)hkv), fast_div((uint32_t)c.splits), scale * 1.44269504088896340736f, part, stat};
     const dim3 grid((unsigned)blocks), block(c.nw * 64);
     hipStream_t s = as_stream(stream);
@@ -672,10 +728,12 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
     };
     auto join = [&](auto dt, auto nw) {
         constexpr int DT = decltype(dt)::value, ROWS = decltype(nw)::value * 32;
-        if (c.splits > AT_FEW_SPLITS)
-            hipLaunchKernelGGL((k_attention_join<DT, 16, ROWS>), dim3((unsigned)(past * ROWS)), dim3(256), 0, s, a);
-        else if (c.splits > 1)
-            hipLaunchKernelGGL((k_attention_join<DT, 1, ROWS>), dim3((unsigned)(past * ROWS / 16)), dim3(256), 0, s, a);
+        if (c.splits == 1) return;
+        const dim3 joins((unsigned)(past * a.spread));
+        if (c.extra && many) hipLaunchKernelGGL((k_attention_join<DT, 16, ROWS, true>), joins, dim3(256), 0, s, a);
+        else if (c.extra) hipLaunchKernelGGL((k_attention_join<DT, 4, ROWS, true>), joins, dim3(256), 0, s, a);
+        else if (many) hipLaunchKernelGGL((k_attention_join<DT, 16, ROWS, false>), joins, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((k_attention_join<DT, 1, ROWS, false>), joins, dim3(256), 0, s, a);
     };
     auto by_type = [&](auto nw) {
         if (dtype == TSP_BF16) {

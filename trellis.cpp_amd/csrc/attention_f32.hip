@@ -31,14 +31,23 @@ template <int DP, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void k_attention_f32(AttnArgs a) {
     constexpr int C = DP / 8, DB = DP / 32, P = DP / 4, ROWS = NW * 32, TILE = KEYS * DP * 4;
     __shared__ __attribute__((aligned(16))) char sK[2][TILE], sV[2][TILE];
-    int work = blockIdx.x, split = 0, splits = 1;
-    if (work >= a.whole) {
-        const int past = work - a.whole, at = past / a.by_splits;
-        splits = a.splits;
-        work = a.whole + at;
-        split = past - at * splits;
+    int split = 0, splits = 1;
+    AttnUnit t;
+    if (a.extra) {
+        const AttnItem item = attn_item<ROWS, KEYS, true>(a, blockIdx.x);
+        t = item;
+        split = item.split;
+        splits = item.splits;
+    } else {
+        int work = blockIdx.x;
+        if (work >= a.whole) {
+            const int past = work - a.whole, at = past / a.by_splits;
+            splits = a.splits;
+            work = a.whole + at;
+            split = past - at * splits;
+        }
+        t = attn_unit<ROWS>(a, work);
     }
-    const AttnUnit t = attn_unit<ROWS>(a, work);
     const PackedUnit& u = t.u;
     if (u.sample < 0) return;
     const int krow0 = u.other0, lk = u.others, rows = t.rows, tile0 = t.row0;
@@ -81,7 +90,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention_f32(AttnArgs a) {
 #pragma unroll
     for (int db = 0; db < DB; ++db) o[db] = f32x16_t{};
     float m = -INFINITY, l = 0.f;
-    const int tiles = (wg_end + KEYS - 1) / KEYS, per = splits == 1 ? tiles : (tiles + splits - 1) / a.by_splits;
+    const int tiles = (wg_end + KEYS - 1) / KEYS, per = (int)((unsigned)(tiles + splits - 1) / (unsigned)splits);
     const int begin = split * per * KEYS, end = min(wg_end, begin + per * KEYS);
     if (begin < end) {
         stage(kp, k_bytes, begin, sK[0], false);
@@ -179,7 +188,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention_f32(AttnArgs a) {
     const float sum = lh.x + lh.y;
     if (r >= rows) return;
     const bool parts = splits > 1, seen = lim.lane > begin && begin < end;
-    const int64_t item = ((int64_t)(work - a.whole) * splits + split) * ROWS + (r - tile0);
+    const int64_t item = (int64_t)((int)blockIdx.x - a.whole) * ROWS + (r - tile0);
     if (parts && h == 0) a.stat[item] = float2{m, seen ? sum : -1.f};
     if (parts && !seen) return;
     float* op = parts ? a.part + item * a.d : static_cast<float*>(a.o) + (int64_t)(u.row0 + qi) * a.o_row + hq * a.o_head;
