@@ -121,7 +121,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
     __shared__ __attribute__((aligned(16))) char sK0[TILE], sK1[TILE], sV0[TILE], sV1[TILE];
     int split = 0, splits = 1;
     AttnUnit t;
-    if (a.extra) {
+    if (__builtin_expect(a.extra != 0, 0)) {      // (its code out of the way of the others')
         const AttnItem item = attn_item<ROWS, AT_KEYS, true>(a, blockIdx.x);
         t = item;
         split = item.split;
@@ -467,8 +467,7 @@ __global__ __launch_bounds__(256) void k_attention_join(AttnArgs a) {
     __shared__ float sAcc[G == 16 ? G : 1][AT_MAX_D], sSum[16];
     const int lane = threadIdx.x & 15, group = threadIdx.x >> 4, e = lane * 8;
     const int g = group % G, at = group / G, mine = threadIdx.x % (G * 16);
-    const int spread = G == 1 ? ROWS / ITEMS : a.spread;      // workgroups of a unit
-    const int past = (int)(blockIdx.x / (unsigned)spread), first = (int)(blockIdx.x - (unsigned)past * spread) * ITEMS;
+    const int past = blockIdx.y, first = blockIdx.x * ITEMS;
     AttnUnit w;
     int splits = a.splits;
     int64_t slot = (int64_t)past * a.splits;      // of the first of them in part
@@ -483,7 +482,7 @@ __global__ __launch_bounds__(256) void k_attention_join(AttnArgs a) {
         w = attn_unit<ROWS>(a, a.whole + past);
     }
     if (w.u.sample < 0) return;
-    for (int row0 = first; row0 < ROWS && w.row0 + row0 < w.rows; row0 += spread * ITEMS) {
+    for (int row0 = first; row0 < ROWS && w.row0 + row0 < w.rows; row0 += gridDim.x * ITEMS) {
         const int row = row0 + at, r = w.row0 + row;
         const bool live = r < w.rows;
         const int64_t item = slot * ROWS + row;
@@ -710,7 +709,7 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
     const int rows = (int)std::min<int64_t>(ceil_div(nq * share, samples), c.nw * 32), spread = many ? rows : c.extra ? (rows + 3) / 4 : c.nw * 2;
     const AttnArgs a{q->data, kk.data, vv.data, out->data, q->row_stride, q->head_stride, kk.row_stride, kk.head_stride, vv.row_stride,
                      vv.head_stride, out->row_stride, out->head_stride, d_q_offsets, d_k_offsets, nq, nk, samples, hkv, share, d,
-                     causal ? 1 : 0, (int)c.whole, c.extra ? c.even : c.splits, (int)c.extra, (int)blocks, spread,
+                     causal ? 1 : 0, (int)c.whole, c.extra ? c.even : c.splits, (int)c.extra, (int)blocks,
                      fast_div((uint32_t)share), fast_div((uint32_t)hkv), fast_div((uint32_t)c.splits), scale * 1.44269504088896340736f, part, stat};
     const dim3 grid((unsigned)blocks), block(c.nw * 64);
     hipStream_t s = as_stream(stream);
@@ -729,7 +728,7 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
     auto join = [&](auto dt, auto nw) {
         constexpr int DT = decltype(dt)::value, ROWS = decltype(nw)::value * 32;
         if (c.splits == 1) return;
-        const dim3 joins((unsigned)(past * a.spread));
+        const dim3 joins((unsigned)spread, (unsigned)past);      // (a unit; there are few of them)
         if (c.extra && many) hipLaunchKernelGGL((k_attention_join<DT, 16, ROWS, true>), joins, dim3(256), 0, s, a);
         else if (c.extra) hipLaunchKernelGGL((k_attention_join<DT, 4, ROWS, true>), joins, dim3(256), 0, s, a);
         else if (many) hipLaunchKernelGGL((k_attention_join<DT, 16, ROWS, false>), joins, dim3(256), 0, s, a);

@@ -33,7 +33,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention_f32(AttnArgs a) {
     __shared__ __attribute__((aligned(16))) char sK[2][TILE], sV[2][TILE];
     int split = 0, splits = 1;
     AttnUnit t;
-    if (a.extra) {
+    if (__builtin_expect(a.extra != 0, 0)) {
         const AttnItem item = attn_item<ROWS, KEYS, true>(a, blockIdx.x);
         t = item;
         split = item.split;

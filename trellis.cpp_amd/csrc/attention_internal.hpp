@@ -23,7 +23,6 @@ struct AttnArgs {
     int whole, splits;                        // the first `whole` of units * hkv see their keys at once, the others in splits
     int extra;                                // several samples: as attn_item says (0: not), the share of its splits a key head
     int items;                                // workgroups there are for them
-    int spread;                               // workgroups of a unit's join
     FastDiv by_share, by_heads, by_splits;
     float scale2;                             // scale * log2(e)
     float* part;                              // [workgroup past whole][row][d] sums of p v, and
