@@ -1,0 +1,49 @@
+"""GPU tests of attention at the ends of its number range: keys that weigh little each and something together,
+against their 64-bit forms. Every bound is below what the fault that its test is for would cost, which the test
+checks."""
+from __future__ import annotations
+
+import math
+
+import pytest
+
+import transformer_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def dtype(key):
+    import torch
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[key]
+
+
+@pytest.mark.parametrize("key,gap,lk,d,at", [("bf16", 17.4, 2_400_000, 64, 0), ("bf16", 17.4, 2_400_001, 128, 70), ("f32", 17.4, 30_000, 64, 0)])
+@pytest.mark.parametrize("rows", [100_000, 3])
+def test_attention_keys_far_below_the_largest(gpu_lib, key, gap, lk, d, at, rows):
+    """One key `gap` nats above all others, its value 0 and theirs 1: the output is the others' weight, which
+    rounding must not take or add. Enough rows for the keys not to be split, and few."""
+    import torch
+    if key == "f32" and rows > 3:
+        rows = 40_000
+    print(f"[far below] {key} gap={gap} lk={lk} d={d} rows={rows}", flush=True)
+    q, k = torch.zeros(1, 1, d, device="cuda"), torch.zeros(lk, 1, d, device="cuda")
+    q[..., 0] = 4.0
+    k[at, 0, 0] = gap / 4.0
+    v = torch.ones(lk, 1, d, device="cuda", dtype=dtype(key))
+    v[at] = 0
+    q, k = q.to(dtype(key)), k.to(dtype(key))
+    out = gpu_lib.attention(q.expand(rows, 1, d).contiguous(), k, v, scale=1.0)
+    s = (k.double()[:, 0] @ q.double()[0, 0])
+    p = torch.softmax(s, dim=0)
+    small = 1 - p[at].item()
+    # Of the others' weight: half a step of p in the 16-bit type, 2^-12 for the score and the exponent, and their
+    # sum, a matrix core's over 16 keys (fp32: 2) at a time, by half a step of what is summed so far an addition, so of
+    # half the sum in the mean. Of all weight, which is divided by: the tiles of 64 (fp32: 32) keys added and a tile's 16
+    # additions.
+    half, keys, tile = (0.0, 2, 32) if key == "f32" else (ref.half_step(dtype(key)), 16, 64)
+    bound = small * (half + 2.0 ** -12 + (lk / keys / 2 + lk / tile + 16) * 2.0 ** -24)
+    bound += ref.half_step(dtype(key)) * (small + bound)
+    assert small > 2 * bound       # all of it lost would show
+    worst = (out.double() - small).abs().max().item()
+    print(f"  others weigh {small:.6f}, off by {worst:.3g}, bound {bound:.3g}", flush=True)
+    assert worst <= bound

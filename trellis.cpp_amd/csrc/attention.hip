@@ -250,13 +250,15 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], scale2, -mc));
+        float sum = 0.f;      // (of the tile first: a sixteenth as many additions meet the row's whole sum)
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 pf[ks][e] = pack2<BF16>(s[ks / 2][8 * (ks % 2) + 2 * e], s[ks / 2][8 * (ks % 2) + 2 * e + 1]);
-                l = add2<BF16>(pf[ks][e], l);
+                sum = add2<BF16>(pf[ks][e], sum);
             }
+        l += sum;
     };
     auto weigh = [&](const char* sV, const u32x4_t (&pf)[4]) __attribute__((always_inline)) {
 #pragma unroll
@@ -345,6 +347,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
                     f32x16_t (&sn)[2]) __attribute__((always_inline)) {
         constexpr int AHEAD = 4, NK = 2 * KS, NV = 4 * DB;
         u32x4_t pf[4], ring[AHEAD];
+        float sum = 0.f;
         landed();
         if (base + 2 * AT_KEYS < end) stage_k(base + 2 * AT_KEYS, k_this);
         if (base + AT_KEYS < end) stage_v(base + AT_KEYS, v_next);
@@ -361,10 +364,11 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
                 const float x = __builtin_amdgcn_exp2f(fmaf(s[e / 8][2 * (e % 8)], scale2, -mc));
                 const float y = __builtin_amdgcn_exp2f(fmaf(s[e / 8][2 * (e % 8) + 1], scale2, -mc));
                 pf[e / 4][e % 4] = pack2<BF16>(x, y);
-                l = add2<BF16>(pf[e / 4][e % 4], l);
+                sum = add2<BF16>(pf[e / 4][e % 4], sum);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        l += sum;
         float mt = sn[0][0];
 #pragma unroll
         for (int t = 0; t < NV; ++t) {
