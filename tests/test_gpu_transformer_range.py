@@ -17,7 +17,9 @@ def dtype(key):
     return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[key]
 
 
-@pytest.mark.parametrize("key,gap,lk,d,at", [("bf16", 17.4, 2_400_000, 64, 0), ("bf16", 17.4, 2_400_001, 128, 70), ("f32", 17.4, 30_000, 64, 0)])
+@pytest.mark.parametrize("key,gap,lk,d,at", [("f16", 17.0, 200_000, 64, 0), ("f16", 17.4, 200_000, 128, 0), ("f16", 17.4, 200_000, 64, 70),
+                                             ("f16", 15.0, 600_000, 64, 0), ("f16", 17.4, 100_001, 32, 33), ("f16", 20.0, 600_000, 64, 1),
+                                             ("bf16", 17.4, 2_400_000, 64, 0), ("bf16", 17.4, 2_400_001, 128, 70), ("f32", 17.4, 30_000, 64, 0)])
 @pytest.mark.parametrize("rows", [100_000, 3])
 def test_attention_keys_far_below_the_largest(gpu_lib, key, gap, lk, d, at, rows):
     """One key `gap` nats above all others, its value 0 and theirs 1: the output is the others' weight, which
@@ -39,10 +41,12 @@ def test_attention_keys_far_below_the_largest(gpu_lib, key, gap, lk, d, at, rows
     # Of the others' weight: half a step of p in the 16-bit type, 2^-12 for the score and the exponent, and their
     # sum, a matrix core's over 16 keys (fp32: 2) at a time, by half a step of what is summed so far an addition, so of
     # half the sum in the mean. Of all weight, which is divided by: the tiles of 64 (fp32: 32) keys added and a tile's 16
-    # additions.
+    # additions. f16 below its normal range, 2^-25 of the largest and kept 2^-11 lower: 2^-36 a key.
     half, keys, tile = (0.0, 2, 32) if key == "f32" else (ref.half_step(dtype(key)), 16, 64)
     bound = small * (half + 2.0 ** -12 + (lk / keys / 2 + lk / tile + 16) * 2.0 ** -24)
-    bound += ref.half_step(dtype(key)) * (small + bound)
+    if key == "f16":
+        bound += lk * 2.0 ** -36
+    bound += ref.half_step(dtype(key)) * (small + bound) + (2.0 ** -25 if key == "f16" else 0.0)
     assert small > 2 * bound       # all of it lost would show
     worst = (out.double() - small).abs().max().item()
     print(f"  others weigh {small:.6f}, off by {worst:.3g}, bound {bound:.3g}", flush=True)

@@ -16,8 +16,9 @@
 // tiles once.
 //
 // Statistics and accumulators are fp32. P is rounded to the inputs' 16-bit type, as the matrix cores take
-// it (half a step, 2^-8 of a probability in bf16 and 2^-11 in f16; a row's sum is of the rounded ones, so
-// that rows of equal values have their mean exactly).
+// it: half a step, 2^-8 of a probability in bf16 and 2^-11 in f16, there for those of 2^-25 of the row's largest and
+// more; smaller ones are off by up to 2^-36 of the largest. A row's sum is of the rounded ones, so that rows of equal
+// values have their mean exactly.
 //
 // Bound by the matrix cores and, at d <= 64, by the exponents beside them (a wave's tile of 64 keys is 16
 // products of 32 cycles, and 33 exponents of 10 with some 140 other instructions of 2.7). A wave holds 32 rows'
@@ -202,7 +203,8 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
     f32x16_t o[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db) o[db] = f32x16_t{};
-    float m = -INFINITY, l = 0.f;
+    constexpr float LAG = BF16 ? 8.f : 4.f, LIFT = BF16 ? 0.f : 11.f;
+    float m = -INFINITY, l = 0.f, mc = -LIFT;      // maximum, sum, what the exponents are less by
 
     // this split's share of the workgroup's tiles
     const int tiles = (wg_end + AT_KEYS - 1) / AT_KEYS, per = (int)((unsigned)(tiles + splits - 1) / (unsigned)splits);
@@ -219,15 +221,18 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
                 s[kb] = mfma32<BF16>(*reinterpret_cast<const u32x4_t*>(sK + k_piece<DP>(kb * 32 + r32, ks * 2 + h)), qf[ks], s[kb]);
         }
     };
-    // The maximum that the exponents are taken from moves only when a row's has grown by a factor of 2^8 (p
-    // and its sums have room for that), so that most tiles leave the sums as they are.
+    // The maximum that the exponents are taken from moves only when a row's has grown by a factor of 2^LAG (p
+    // and its sums have room for that), so that most tiles leave the sums as they are. In f16 p is 2^LIFT times
+    // its value, in l and in o alike, so that it fills the type's range from the top, 2^15: a key of 2^-(14 + LIFT)
+    // of the largest has all its bits, and one of up to 2^-(25 + LIFT) still counts.
     auto raise = [&](float mt) __attribute__((always_inline)) {
         const float2 mh = both_halves(mt);
         mt = fmaxf(mh.x, mh.y);
-        if (__any((mt - m) * scale2 > 8.f)) {
+        if (__any((mt - m) * scale2 > LAG)) {
             const float mn = fmaxf(m, mt);
             const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * scale2);
             m = mn;
+            mc = (mn == -INFINITY ? 0.f : mn * scale2) - LIFT;       // (no key seen yet, or scores of -inf alone)
             l *= corr;
 #pragma unroll
             for (int db = 0; db < DB; ++db)
@@ -245,7 +250,6 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
     };
     // s becomes p, pf the second product's operand
     auto exponents = [&](f32x16_t (&s)[2], u32x4_t (&pf)[4]) __attribute__((always_inline)) {
-        const float mc = m == -INFINITY ? 0.f : m * scale2;      // (no key seen yet, or scores of -inf alone)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -351,7 +355,6 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
         landed();
         if (base + 2 * AT_KEYS < end) stage_k(base + 2 * AT_KEYS, k_this);
         if (base + AT_KEYS < end) stage_v(base + AT_KEYS, v_next);
-        const float mc = m == -INFINITY ? 0.f : m * scale2;
 #pragma unroll
         for (int t = 0; t < AHEAD; ++t) ring[t] = k_operand(k_next, t);
 #pragma unroll
