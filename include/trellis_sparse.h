@@ -491,9 +491,10 @@ int tsp_rope_axes(const tsp_heads* q, int hq, const tsp_heads* k, int hk, int dt
  * v. A row that sees no key gets zeros; a key that a row does not see has no effect on it, whatever it
  * holds. q, k, v and out have one dtype: with f16 and bf16 the probabilities are rounded to it (in f16 those
  * below 2^-25 of a row's largest are off by up to 2^-36 of it), f32 runs on the fp32 matrix cores (a
- * sixteenth of the rate). d a multiple of 8 up to 128, hq % hkv == 0, scale > 0;
- * data 16-byte aligned, strides multiples of 8 (rows' up to 2^20; of k and v at least d; a head stride of 0
- * shares one head's data); nq, nk and nq * hq / hkv below 2^31 - 2^16; out must not overlap the inputs.
+ * sixteenth of the rate). Scores, and 2^8 times the sum of |v| over a row's keys, have to fit fp32; scale > 0,
+ * and scale * log2(e) finite. d a multiple of 8 up to 128, hq % hkv == 0; data 16-byte aligned, strides
+ * multiples of 8 (rows' up to 2^20; of k and v at least d; a head stride of 0 shares one head's data); nq, nk
+ * and nq * hq / hkv below 2^31 - 2^16; out must not overlap the inputs.
  * Where there are few queries the keys are split over the device and the parts joined in the workspace,
  * 16-byte aligned, of tsp_attention_workspace_bytes bytes (enough for every type and mask; 0, and NULL
  * will do, where they are not). */

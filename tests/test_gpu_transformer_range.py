@@ -1,6 +1,5 @@
 """GPU tests of attention at the ends of its number range: keys that weigh little each and something together,
-against their 64-bit forms. Every bound is below what the fault that its test is for would cost, which the test
-checks."""
+scores far from zero, against their 64-bit forms."""
 from __future__ import annotations
 
 import math
@@ -51,3 +50,33 @@ def test_attention_keys_far_below_the_largest(gpu_lib, key, gap, lk, d, at, rows
     worst = (out.double() - small).abs().max().item()
     print(f"  others weigh {small:.6f}, off by {worst:.3g}, bound {bound:.3g}", flush=True)
     assert worst <= bound
+
+
+@pytest.mark.parametrize("e", [12, 18, 24, 28, 33])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("order", ["rising", "falling", "mixed"])
+@pytest.mark.parametrize("key", ["f16", "bf16", "f32"])
+def test_attention_scores_far_from_zero(gpu_lib, e, sign, order, key):
+    """Scores of +-2^e with a few units between them, all of them exact in fp32: only differences count, whatever the
+    units are worth. (The largest score by itself, times scale * log2(e) in fp32, is up to 2^10 off.)"""
+    import torch
+    print(f"[far scores] 2^{e} {sign} {order} {key}", flush=True)
+    unit = 1 << max(0, e - 22)       # of a score: 24 bits below 2^(e + 1)
+    a = (e - 2) // 2
+    g = torch.Generator(device="cuda")
+    g.manual_seed(e)
+    for rows, lk, d, causal in ((1, 20_000, 128, False), (200, 1000, 64, True), (300, 700, 32, False)):
+        j = torch.arange(lk, device="cuda") * 255 // (lk - 1)
+        if order == "falling":
+            j = j.flip(0)
+        elif order == "mixed":
+            j = j[torch.randperm(lk, device="cuda", generator=g)]
+        q, k = torch.zeros(rows, 1, d, device="cuda"), torch.zeros(lk, 1, d, device="cuda")
+        q[..., :8], k[..., :8] = 2.0 ** a, sign * 2.0 ** (e - 3 - a)
+        q[..., 8], k[:, 0, 8] = float(unit), j.float()
+        v = torch.randn(lk, 1, d, device="cuda", generator=g)
+        q, k, v = q.to(dtype(key)), k.to(dtype(key)), v.to(dtype(key))
+        for scale in (1.0, 0.375 / unit):
+            out = gpu_lib.attention(q, k, v, causal=causal, scale=scale)
+            o, slack = ref.attention(q, k, v, [0, rows], [0, lk], causal, scale)
+            ref.check(out, o, slack, f"{rows} rows, scale {scale:.3g}")

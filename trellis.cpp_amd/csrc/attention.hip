@@ -204,7 +204,9 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
 #pragma unroll
     for (int db = 0; db < DB; ++db) o[db] = f32x16_t{};
     constexpr float LAG = BF16 ? 8.f : 4.f, LIFT = BF16 ? 0.f : 11.f;
+    constexpr float FAR = 1024.f;
     float m = -INFINITY, l = 0.f, mc = -LIFT;      // maximum, sum, what the exponents are less by
+    bool far = false;
 
     // this split's share of the workgroup's tiles
     const int tiles = (wg_end + AT_KEYS - 1) / AT_KEYS, per = (int)((unsigned)(tiles + splits - 1) / (unsigned)splits);
@@ -232,13 +234,25 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
             const float mn = fmaxf(m, mt);
             const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * scale2);
             m = mn;
-            mc = (mn == -INFINITY ? 0.f : mn * scale2) - LIFT;       // (no key seen yet, or scores of -inf alone)
+            far = __any(fabsf(mn) * scale2 > FAR && mn != -INFINITY);
+            mc = (far || mn == -INFINITY ? 0.f : mn * scale2) - LIFT;       // (-inf: no key seen yet, or scores of -inf alone)
             l *= corr;
 #pragma unroll
             for (int db = 0; db < DB; ++db)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[db][i] *= corr;
         }
+    };
+    // m * scale2 is rounded, and half a step of it is off in every exponent: that does not cancel where the maximum
+    // moves, and from 2^27 on takes p out of its type's range. So a wave with a maximum past FAR, where it is 2^-14,
+    // takes the maximum from the scores themselves, after raise.
+    auto near_top = [&](f32x16_t (&s)[2]) __attribute__((always_inline)) {
+        if (__builtin_expect(!far, 1)) return;
+        const float from = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[kb][i] -= from;
     };
     auto top = [&](const f32x16_t (&s)[2]) __attribute__((always_inline)) {
         float mt = s[0][0];
@@ -282,6 +296,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
             for (int i = 0; i < 16; ++i)
                 s[kb][i] = kb * 32 + 8 * (i / 4) + i % 4 < left ? s[kb][i] : -INFINITY;
         raise(top(s));
+        near_top(s);
         exponents(s, pf);
         // Rows of the tile that see different keys: a probability of zero must not meet an Inf or a NaN
         // of a key that its row does not see. Zero times V shows whether there is one.
@@ -382,6 +397,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
             __builtin_amdgcn_sched_barrier(0);
         }
         raise(mt);
+        near_top(sn);
     };
     int base = begin;
     bool second = false;
@@ -395,6 +411,7 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
         landed();
         scores(sK0, s0);
         raise(top(s0));
+        near_top(s0);
         for (; base + 3 * AT_KEYS <= whole; base += 2 * AT_KEYS) {
             step(base, sK0, sK1, sV0, sV1, s0, s1);
             step(base + AT_KEYS, sK1, sK0, sV1, sV0, s1, s0);
@@ -597,6 +614,8 @@ __global__ __launch_bounds__(256) void k_attention_join(AttnArgs a) {
     }
 }
 
+constexpr float kLog2e = 1.44269504088896340736f;
+
 // How a call is cut: waves of a workgroup (32 rows each), units of rows a key head, how many of them see
 // their keys at once, splits of the others' keys.
 struct AttnCut {
@@ -688,7 +707,7 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
     TSP_REQUIRE(dtype_valid(dtype), TSP_ERR_INVALID, "tsp_attention: bad dtype");
     TSP_REQUIRE(samples > 0 && (samples == 1 || (d_q_offsets && d_k_offsets)), TSP_ERR_INVALID,
                 "tsp_attention: samples=%d (without offsets: 1)", samples);
-    TSP_REQUIRE(std::isfinite(scale) && scale > 0.f, TSP_ERR_INVALID, "tsp_attention: scale=%g", scale);
+    TSP_REQUIRE(std::isfinite(scale * kLog2e) && scale > 0.f, TSP_ERR_INVALID, "tsp_attention: scale=%g", scale);
     TSP_REQUIRE(d > 0 && d % 8 == 0 && d <= AT_MAX_D, TSP_ERR_UNSUPPORTED, "tsp_attention: heads of %d (need a multiple of 8 up to %d)",
                 d, AT_MAX_D);
     if (nq == 0) return TSP_OK;
@@ -717,7 +736,7 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
     const AttnArgs a{q->data, kk.data, vv.data, out->data, q->row_stride, q->head_stride, kk.row_stride, kk.head_stride, vv.row_stride,
                      vv.head_stride, out->row_stride, out->head_stride, d_q_offsets, d_k_offsets, nq, nk, samples, hkv, share, d,
                      causal ? 1 : 0, (int)c.whole, c.extra ? c.even : c.splits, (int)c.extra, (int)blocks,
-                     fast_div((uint32_t)share), fast_div((uint32_t)hkv), fast_div((uint32_t)c.splits), scale * 1.44269504088896340736f, part, stat};
+                     fast_div((uint32_t)share), fast_div((uint32_t)hkv), fast_div((uint32_t)c.splits), scale * kLog2e, part, stat};
     const dim3 grid((unsigned)blocks), block(c.nw * 64);
     hipStream_t s = as_stream(stream);
     using std::integral_constant;

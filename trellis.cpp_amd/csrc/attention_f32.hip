@@ -134,11 +134,11 @@ __global__ __launch_bounds__(NW * 64, 2) void k_attention_f32(AttnArgs a) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[db][i] *= corr;
         }
-        const float mc = m == -INFINITY ? 0.f : m * a.scale2;
+        const float top = m == -INFINITY ? 0.f : m;      // (taken from the scores: m * scale2 would be rounded)
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.scale2, -mc));
+            s[i] = __builtin_amdgcn_exp2f((s[i] - top) * a.scale2);
             sum += s[i];
         }
         l += sum;
