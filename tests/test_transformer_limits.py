@@ -15,3 +15,16 @@ def test_attention_scale(pkg):
     for scale in (3.0e38, math.inf, math.nan, 0.0, -1.0):
         assert L.tsp_attention(q, k, v, 2, 100, 100, 8, 8, 64, FAKE, FAKE, 2, scale, 0, o, None, 0, None) == 1
         assert "scale" in L.tsp_last_error().decode()
+
+
+def test_group_norm_partial_overlap(pkg):
+    """An output that shares some of x's bytes but does not begin with them would be read after it is written."""
+    L = pkg.lib()
+    n, c = 100, 64
+    for xd, od in ((0, 0), (0, 2), (1, 0), (2, 2)):
+        size = {0: 4, 1: 2, 2: 2}
+        xb, ob = n * c * size[xd], n * c * size[od]
+        for x, out in ((0x100000, 0x100000 + xb - 16), (0x100000, 0x100000 + 16), (0x100000 + ob - 16, 0x100000), (0x100000 + c * 2, 0x100000)):
+            rc = L.tsp_group_norm(ctypes.c_void_p(x), xd, n, c, 8, None, 1, None, None, 1e-6, 0, ctypes.c_void_p(out), od,
+                                  ctypes.c_void_p(0x900000), 1 << 20, None)
+            assert rc == 1 and "overlaps" in L.tsp_last_error().decode()

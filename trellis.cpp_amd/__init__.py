@@ -899,7 +899,7 @@ def group_norm(x, groups: int, gamma=None, beta=None, eps: float = 1e-6, silu: b
     """Group norm over packed samples, channels last: x [N, C], each sample's rows and a group's
     C / groups channels normalised together (biased variance) [* gamma + beta] [then SiLU]. offsets int32
     [samples + 1] on the GPU: the samples' first rows and the last one's end (None: one sample); rows
-    outside every sample are left as they were in out. out [N, C] may be x; workspace
+    outside every sample are left as they were in out. out [N, C] may be x (and must not overlap it otherwise); workspace
     (group_norm_workspace) may be given to reuse it."""
     torch = _torch()
     if x.dim() != 2 or groups < 1 or x.shape[1] % groups:

@@ -456,6 +456,11 @@ extern "C" int tsp_group_norm(const void* d_x, int x_dtype, int64_t n, int c, in
     TSP_REQUIRE(workspace_bytes >= tsp_group_norm_workspace_bytes(n, c, groups, samples), TSP_ERR_WORKSPACE,
                 "tsp_group_norm: workspace of %zu bytes, needs %zu", workspace_bytes,
                 tsp_group_norm_workspace_bytes(n, c, groups, samples));
+    // (in place a workgroup reads what it writes and no other's rows: only where both are the same values)
+    const uintptr_t x0 = reinterpret_cast<uintptr_t>(d_x), o0 = reinterpret_cast<uintptr_t>(d_out);
+    auto bytes = [&](int dt) { return (uintptr_t)n * c * (dt == TSP_F32 ? 4 : 2); };
+    TSP_REQUIRE(x0 == o0 || x0 + bytes(x_dtype) <= o0 || o0 + bytes(out_dtype) <= x0, TSP_ERR_INVALID,
+                "tsp_group_norm: out overlaps x in part (it may be x, or apart)");
     const int64_t units = gn_units(n, c, samples);
     TSP_REQUIRE(units * GN_NT < (1ll << 32), TSP_ERR_INVALID, "tsp_group_norm: too many samples");
     hipStream_t s = as_stream(stream);
