@@ -4,6 +4,9 @@ from __future__ import annotations
 
 import ctypes
 import math
+import types
+
+import pytest
 
 FAKE = ctypes.c_void_p(0x1000)   # never dereferenced
 
@@ -28,3 +31,18 @@ def test_group_norm_partial_overlap(pkg):
             rc = L.tsp_group_norm(ctypes.c_void_p(x), xd, n, c, 8, None, 1, None, None, 1e-6, 0, ctypes.c_void_p(out), od,
                                   ctypes.c_void_p(0x900000), 1 << 20, None)
             assert rc == 1 and "overlaps" in L.tsp_last_error().decode()
+
+
+@pytest.mark.parametrize("private", [True, False])
+def test_current_stream_without_the_private_call(pkg, monkeypatch, private):
+    """The pieces' calls go to the current stream, by torch's public interface where the other one is not there."""
+    import torch
+    streams = []
+    if private:
+        monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 100 + i, raising=False)
+    else:
+        monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream", raising=False)
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda i: types.SimpleNamespace(cuda_stream=100 + i))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    pkg._launch(torch.device("cuda", 3), None, lambda s, keep: streams.append(s))
+    assert streams == [103]

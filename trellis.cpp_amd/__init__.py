@@ -846,14 +846,21 @@ def _nothing(*tensors):
     pass
 
 
+def _current_stream(index: int) -> int:
+    """The pointer of the device's current stream. torch's own call for it, which is not public, where there is
+    one: a Stream object is 1 us, a tenth of the host's side of a call."""
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(index) if raw else torch.cuda.current_stream(index).cuda_stream
+
+
 def _launch(device, stream, call, *args):
     """call(stream pointer, keep, *args) on the device and stream; keep(*tensors) is told every tensor the
     call uses."""
     torch = _torch()
     index = device.index
     if stream is None and index == torch.cuda.current_device():
-        # (the stream's pointer alone: a Stream object is 1 us, a tenth of the host's side of a call)
-        return call(torch._C._cuda_getCurrentRawStream(index), _nothing, *args)
+        return call(_current_stream(index), _nothing, *args)
     with _On(device, stream, torch.cuda.current_stream(index)) as on:
         return call(on.stream.cuda_stream, on.keep, *args)
 
