@@ -453,9 +453,11 @@ int tsp_c2s_part(const float* d_x, int64_t n, int cin, const int32_t* d_nbr, con
 /* Group norm, channels last: out[i][c] = act((x[i][c] - mean) / sqrt(var + eps) * gamma[c] + beta[c])
  * with the mean and the biased variance of the c / groups channels of c's group over all rows of i's
  * sample, in fp32; act is x * sigmoid(x) when silu != 0. gamma and beta f32 [c] or NULL. Any dtypes;
- * d_out may be d_x where they are the same, and must not overlap it otherwise. At most 4096 groups. The
- * workspace, 8-byte aligned, holds tsp_group_norm_workspace_bytes bytes; the result does not depend on what
- * it held, nor on the order in which workgroups run. */
+ * d_out may be d_x where they are the same, and must not overlap it otherwise. At most 4096 groups. Rows of
+ * whole 16-byte pieces (c a multiple of 8 up to 4096, x, out, gamma and beta 16-byte aligned) are read piece by
+ * piece, others value by value (60,013 x 256 bf16: 25 us and 115). The workspace, 8-byte aligned, holds
+ * tsp_group_norm_workspace_bytes bytes; the result does not depend on what it held, nor on the order in which
+ * workgroups run. */
 size_t tsp_group_norm_workspace_bytes(int64_t n, int c, int groups, int samples);
 int tsp_group_norm(const void* d_x, int x_dtype, int64_t n, int c, int groups, const int32_t* d_offsets,
                    int samples, const float* d_gamma, const float* d_beta, float eps, int silu, void* d_out,

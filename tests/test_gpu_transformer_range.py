@@ -1,5 +1,5 @@
 """GPU tests of attention at the ends of its number range: keys that weigh little each and something together,
-scores far from zero, against their 64-bit forms."""
+scores far from zero, against their 64-bit forms; and of group norm's factors off a 16-byte boundary."""
 from __future__ import annotations
 
 import math
@@ -80,3 +80,17 @@ def test_attention_scores_far_from_zero(gpu_lib, e, sign, order, key):
             out = gpu_lib.attention(q, k, v, causal=causal, scale=scale)
             o, slack = ref.attention(q, k, v, [0, rows], [0, lk], causal, scale)
             ref.check(out, o, slack, f"{rows} rows, scale {scale:.3g}")
+
+
+@pytest.mark.parametrize("n,c,groups", [(700, 64, 8), (60_000, 256, 32)])
+def test_group_norm_factors_inside_a_buffer(gpu_lib, n, c, groups):
+    """gamma and beta as slices of one parameter buffer, off a 16-byte boundary: the same kernels, so the same bits."""
+    import torch
+    g = torch.Generator(device="cuda")
+    g.manual_seed(n)
+    x, f = torch.randn(n, c, device="cuda", generator=g), torch.randn(2 * c + 1, device="cuda", generator=g)
+    gamma, beta = f[1:c + 1], f[c + 1:]
+    assert gamma.data_ptr() % 16 and beta.data_ptr() % 16
+    want = gpu_lib.group_norm(x, groups, gamma.clone(), beta.clone(), silu=True)
+    for a, b in ((gamma, beta), (gamma.clone(), beta), (gamma, beta.clone())):
+        assert torch.equal(gpu_lib.group_norm(x, groups, a, b, silu=True), want)

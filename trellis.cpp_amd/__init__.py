@@ -930,9 +930,10 @@ def group_norm(x, groups: int, gamma=None, beta=None, eps: float = 1e-6, silu: b
         ws = workspace
         if ws is None:
             ws = torch.empty(max(lib().tsp_group_norm_workspace_bytes(n, c, groups, samples), 16), dtype=torch.uint8, device=dev)
-        keep(x, xc, gamma, beta, offsets, o, ws)
+        g, b = _aligned(gamma), _aligned(beta)      # (the kernels would read all of x value by value otherwise)
+        keep(x, xc, gamma, beta, g, b, offsets, o, ws)
         _check("tsp_group_norm",
-               lib().tsp_group_norm(_p(xc), xd, n, c, groups, _p(offsets), samples, _p(gamma), _p(beta), eps,
+               lib().tsp_group_norm(_p(xc), xd, n, c, groups, _p(offsets), samples, _p(g), _p(b), eps,
                                     1 if silu else 0, _p(o), dtype_code(o.dtype), _p(ws), ws.numel(), s))
         return o
     return _launch(dev, stream, call)
