@@ -497,7 +497,9 @@ int tsp_rope_axes(const tsp_heads* q, int hq, const tsp_heads* k, int hk, int dt
  * and scale * log2(e) finite. d a multiple of 8 up to 128, hq % hkv == 0; data 16-byte aligned, strides
  * multiples of 8 (rows' up to 2^20; of k and v at least d; a head stride of 0 shares one head's data); nq, nk
  * and nq * hq / hkv below 2^31 - 2^16; out must not overlap the inputs.
- * Where there are few queries the keys are split over the device and the parts joined in the workspace,
+ * Where there are few queries the keys are split over the device, by the samples' lengths where up to 64 of
+ * them differ (a batch of more, or one that fills the device at its mean length, is not: a sample whose keys are
+ * many times the others' is better a call of its own), and the parts joined in the workspace,
  * 16-byte aligned, of tsp_attention_workspace_bytes bytes (enough for every type and mask; 0, and NULL
  * will do, where they are not). */
 size_t tsp_attention_workspace_bytes(int64_t nq, int64_t nk, int samples, int hq, int hkv, int d);

@@ -22,8 +22,11 @@
 //
 // Bound by the matrix cores and, at d <= 64, by the exponents beside them (a wave's tile of 64 keys is 16
 // products of 32 cycles, and 33 exponents of 10 with some 140 other instructions of 2.7). A wave holds 32 rows'
-// accumulators, its Q operands and two tiles' scores in at most 256 registers, two waves a SIMD (three at d <= 64);
-// the workgroups, two or three a CU, keep each other's barriers and loads covered. 35,001 rows, 8 heads of 128,
+// accumulators, its Q operands and two tiles' scores: where four share a workgroup in at most 256 registers, two waves a
+// SIMD (three at d <= 64), so that the workgroups, two or three a CU, keep each other's barriers and loads covered;
+// alone, at widths 96 and 128, in some 270 and 320 to 340, one a SIMD (at 64 KB of LDS each no more than two
+// fit the four SIMDs of a CU). The scalar registers of bf16 at width 128 do not all fit: of its loop's instructions, two tiles
+// long, 21 move them to and from a vector register (f16: none). 35,001 rows, 8 heads of 128,
 // bf16: 4.1-4.4 ms, 1,140-1,220 TFLOP/s, 67 % of the matrix cores' cycles at the 1.6 GHz that power leaves (a
 // library GEMM of 16,384^3: 1,391). 8 heads of 64, 12,288 to 16,384 keys: 840. One row against 40,009 keys, 16
 // heads on 2 of 128: 12 us and 6 for the join, 3.4 TB/s of keys and values.
@@ -114,7 +117,7 @@ __device__ __forceinline__ AttnArgsPtr reread_args() {
 #endif
 
 template <bool BF16, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void k_attention(AttnArgs) {
+__global__ __launch_bounds__(NW * 64, NW == 1 && DP > 64 ? 1 : 2) void k_attention(AttnArgs) {
 #ifdef __HIP_DEVICE_COMPILE__
     const auto& a = *reread_args();
     constexpr int KS = DP / 16, DB = DP / 32, P = DP / 8, ROWS = NW * 32;
@@ -639,6 +642,9 @@ AttnCut attn_cut(int64_t nq, int64_t nk, int samples, int hkv, int share, int d,
     // leave a last round partly empty, that round's are. (Several samples, or causal ones, have units of
     // unequal length, which fill each other's gaps.) Time is counted in tiles: about three for a workgroup's
     // start and end, five or six for the join.
+    // A sample leaves a partly filled unit, in the mean half of one. (A row each of 16, 65,536 keys, 32 heads on 8 of
+    // 128: 55 us so, 89 with none counted, 52 with whole ones; with those, 64 samples of which one has nearly
+    // all of 65,536 keys would fill the device by count and take 1,094 us, 66 so.)
     const int64_t busy = (units + (samples > 1 ? samples / 2 : 0)) * hkv;
     const int64_t slots = 256 * (c.nw == 4 ? (d > 64 ? 2 : 3) : d > 96 || (f32 && d > 64) ? 2 : d > 64 ? 3 : 5);
     const int64_t tiles = ceil_div(ceil_div(nk, samples), f32 ? AT_KEYS_F32 : AT_KEYS);
@@ -669,11 +675,19 @@ AttnCut attn_cut(int64_t nq, int64_t nk, int samples, int hkv, int share, int d,
     // Several samples may differ in length, which only the device knows. Those of few rows get a part in the join
     // even where their mean asks for none, if one of them can be long: a row each of 64 samples, 16 heads on 2 of
     // 128, 50,000 keys in all, takes 27 us, not 721, where one has nearly all of them (and 26, not 23, where all have 781).
+    // From 16,384 keys on: 18.6 us and 271 where one has them, 15.4 and 12.2 where all have as many; of 8,192 keys 16
+    // and 134, 15 and 12.
+    // Two kinds of batch are not split by length: more than 64 samples (a wave holds them, one a lane) and those that
+    // fill the device at their mean length, above. There a sample far longer than the mean is one workgroup's a unit
+    // and key head: 827 us for 65 samples where 64 take 27, and 1,500 for one row on 100,000 keys beside
+    // 4,000 causal rows (93 on 1,000 keys).
     c.even = c.splits;
     if (samples > 1 && samples <= 64 && (c.splits > 1 || (c.nw == 1 && tiles * samples >= 256))) {
         c.splits = std::max(c.splits, 2);
         c.whole = 0;
-        // whole rounds of equal splits, where there are as many
+        // Whole rounds of equal splits, from 0.7 of one on: with the next whole number always, 4 samples of which one
+        // has nearly all of 8,192 keys, 8 heads of 64, take 20 us (15 so); never, 5 of 100 rows and 100,000 keys, 16
+        // heads on 2 of 128, 109 (103), though others gain up to 10 %.
         const int64_t items = busy * c.splits, n = items * 10 < slots * 7 ? items : std::max<int64_t>(1, (2 * items + slots) / (2 * slots)) * slots;
         c.extra = std::min(std::max(n / hkv - c.units, c.units), c.units * (c.splits - 1));
     }

@@ -5,10 +5,11 @@
 // h, are the second product's operand one by one, unrounded, beside V's values of those same two keys; in
 // the first product a lane half takes d = 8 c + 4 h .. + 3 of K and Q as one 16-byte piece, four steps long.
 //
-// Bound by the matrix cores: 32x32x2 takes 64 cycles for a sixteenth of what 32x32x16 does in 32, so that
-// a tile of 32 keys is (D / 2 + D / 2) * 64 cycles a wave and the exponents a hundredth of it: nothing else
-// is worth overlapping beyond the next tile's loads. 8,192 rows and keys, 8 heads of 128: 2.46 ms, 112 of the
-// 157 TFLOP/s that the instruction has; of 64: 115.
+// Bound by the matrix cores: 32x32x2 takes 64 cycles for an eighth of what 32x32x16 does in 32 (a sixteenth of the
+// rate), so that a tile of 32 keys is (D / 2 + D / 2) * 64 cycles a wave and its 16 exponents, of 10 cycles, 2 to
+// 4 % of that: nothing else is worth overlapping beyond the next tile's loads. 8,192 rows and keys, 8 heads of 128:
+// 2.27 ms, 121 of the 157 TFLOP/s that the instruction has; of 64: 1.20 ms, 114. Heads of 32 and of 80 are widened to
+// those and take as long. One row on 40,009 keys, 16 heads on 2 of 128: 44 us on a floor of 12.
 #include "attention_internal.hpp"
 
 namespace tsp {
@@ -28,7 +29,7 @@ __device__ __forceinline__ int v_piece(int key, int piece) {
 }
 
 template <int DP, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void k_attention_f32(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, NW == 1 && DP > 64 ? 1 : 2) void k_attention_f32(AttnArgs a) {
     constexpr int C = DP / 8, DB = DP / 32, P = DP / 4, ROWS = NW * 32, TILE = KEYS * DP * 4;
     __shared__ __attribute__((aligned(16))) char sK[2][TILE], sV[2][TILE];
     int split = 0, splits = 1;
