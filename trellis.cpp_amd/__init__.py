@@ -1036,7 +1036,8 @@ def attention(q, k, v, q_offsets=None, k_offsets=None, causal: bool = False, sca
     Row i of a sample sees all of the sample's keys, or with causal the keys j <= i + (Lk - Lq); a row that
     sees none gets zeros. q_offsets and k_offsets int32 [samples + 1] on the GPU: the samples' rows in q
     and in k and v (None, both: one sample); rows of out outside every sample are left as they were. scale
-    defaults to D ** -0.5. Heads may be strided views; workspace (attention_workspace) may be given to
+    defaults to D ** -0.5. 16-bit heads' probabilities are rounded to their type, float32 heads' are not (and take
+    some ten times as long). Heads may be strided views; workspace (attention_workspace) may be given to
     reuse it."""
     torch = _torch()
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or k.shape[2] != q.shape[2]:
