@@ -476,7 +476,7 @@ typedef struct {
  * TSP_ROPE_HALVES (p, p + d/2); axis 0's pairs[0] pairs come first, then axis 1's, and pairs after the
  * last axis's stay as they are. Angles are formed in 64 bits and are exact to 2^-22 for positions up to
  * 2^28. q and k (hk heads; NULL and 0 without) are turned in one launch. With gamma (f32 [heads][d], or
- * NULL), a head's row is RMS-normalised first: x / sqrt(mean(x^2) + eps) * gamma. 1 to 4 axes; d a
+ * NULL), a head's row is RMS-normalised first: x / sqrt(mean(x^2) + eps) * gamma, in fp32. 1 to 4 axes; d a
  * multiple of 8 up to 256; data and gamma 16-byte aligned, strides multiples of 8 (rows' up to 2^20). Any
  * dtypes; an output may be its own input where they have one dtype and the same strides, and must not
  * overlap the inputs otherwise. */

@@ -1,5 +1,6 @@
 """GPU tests of attention at the ends of its number range: keys that weigh little each and something together,
-scores far from zero, against their 64-bit forms; and of group norm's factors off a 16-byte boundary."""
+scores far from zero, against their 64-bit forms; of group norm's factors off a 16-byte boundary; and of captured
+calls replayed with other lengths."""
 from __future__ import annotations
 
 import math
@@ -94,3 +95,42 @@ def test_group_norm_factors_inside_a_buffer(gpu_lib, n, c, groups):
     want = gpu_lib.group_norm(x, groups, gamma.clone(), beta.clone(), silu=True)
     for a, b in ((gamma, beta), (gamma.clone(), beta), (gamma, beta.clone())):
         assert torch.equal(gpu_lib.group_norm(x, groups, a, b, silu=True), want)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_replayed_with_other_lengths(gpu_lib, rows):
+    """A captured step replayed with other offsets in the same buffers, even and skewed: lengths are read on the
+    device, so each replay gives what an eager call does, and rows outside the samples stay."""
+    import torch
+    g = torch.Generator(device="cuda")
+    g.manual_seed(rows)
+    samples, n = 16, 30_000
+    nq = rows * samples
+    q, k, v = (torch.randn(m, h, 64, device="cuda", generator=g).bfloat16() for m, h in ((nq, 4), (n, 2), (n, 2)))
+    x = torch.randn(n, 64, device="cuda", generator=g)
+    qo = torch.arange(0, nq + 1, rows, device="cuda", dtype=torch.int32)
+    ko = torch.arange(0, n + 1, n // samples, device="cuda", dtype=torch.int32)[:samples + 1].contiguous()
+    o, y = torch.empty_like(q), torch.empty_like(x)
+    ws, wn = gpu_lib.attention_workspace(nq, n, samples, 4, 2, 64), gpu_lib.group_norm_workspace(n, 64, 8, samples)
+
+    def call():
+        gpu_lib.attention(q, k, v, qo, ko, causal=True, out=o, workspace=ws)
+        gpu_lib.group_norm(x, 8, silu=True, offsets=ko, out=y, workspace=wn)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for lengths in ([1800] * 16, [10] * 5 + [29_000] + [0] * 10, [100 * i for i in range(16)], [n // 16] * 16):
+        bounds = ref.offsets_of(lengths)
+        ko.copy_(torch.tensor(bounds, dtype=torch.int32))
+        o.fill_(-7), y.fill_(-7)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = o.clone(), y.clone()
+        o.fill_(-7), y.fill_(-7)
+        call()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], o) and torch.equal(got[1], y) and (y[bounds[-1]:] == -7).all()
+        want, slack = ref.attention(q, k, v, ref.offsets_of([rows] * samples), bounds, True, 0.125)
+        ref.check(o, want, slack, "replay")
