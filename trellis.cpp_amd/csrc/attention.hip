@@ -25,10 +25,10 @@
 // accumulators, its Q operands and two tiles' scores: where four share a workgroup in at most 256 registers, two waves a
 // SIMD (three at d <= 64), so that the workgroups, two or three a CU, keep each other's barriers and loads covered;
 // alone, at widths 96 and 128, in some 270 and 320 to 340, one a SIMD (at 64 KB of LDS each no more than two
-// fit the four SIMDs of a CU). The scalar registers of bf16 at width 128 do not all fit: of its loop's instructions, two tiles
-// long, 21 move them to and from a vector register (f16: none). 35,001 rows, 8 heads of 128,
-// bf16: 4.1-4.4 ms, 1,140-1,220 TFLOP/s, 67 % of the matrix cores' cycles at the 1.6 GHz that power leaves (a
-// library GEMM of 16,384^3: 1,391). 8 heads of 64, 12,288 to 16,384 keys: 840. One row against 40,009 keys, 16
+// fit the four SIMDs of a CU). The scalar registers of bf16 at width 128 do not all fit: of its loop's
+// instructions, two tiles long, 21 move them to and from a vector register (f16: none). 35,001 rows, 8 heads of
+// 128, bf16: 4.25-4.4 ms, 1,140-1,180 TFLOP/s, 65 % of the matrix cores' cycles at the 1.6 GHz that power leaves (a
+// library GEMM of 16,384^3: 1,391). 8 heads of 64, 10,000 rows and keys: 870. One row against 40,009 keys, 16
 // heads on 2 of 128: 12 us and 6 for the join, 3.4 TB/s of keys and values.
 // Tried and taken back: eight waves a workgroup (one a CU: as fast at 35,001 rows, 8-15 % slower at 1,029 to
 // 12,345 keys); the loads spread between the products (7 % slower: a wave stops at each); values a tile later
@@ -758,7 +758,7 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
         hipLaunchKernelGGL((k_attention<decltype(bf)::value, decltype(dp)::value, decltype(nw)::value>), grid, block, 0, s, a);
     };
     // Heads are widened to the next of four widths (zeros that cost products and LDS): 10,000 rows and keys, 8 heads
-    // of 32 take 182 us at their own width and 238 at 64; of 80, 300 at 96 and 345 at 128.
+    // of 32 take 170-182 us at their own width and 238 at 64; of 80, 297-300 at 96 and 345 at 128.
     auto by_width = [&](auto bf, auto nw) {
         if (d <= 32) attend(bf, integral_constant<int, 32>{}, nw);
         else if (d <= 64) attend(bf, integral_constant<int, 64>{}, nw);
