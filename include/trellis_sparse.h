@@ -508,6 +508,97 @@ int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_heads* v, in
                   float scale, int causal, const tsp_heads* out, void* d_workspace, size_t workspace_bytes,
                   void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * A served transformer block's step (no counterpart in the reference's sparse path): RMS norm with the
+ * residual's addition, linears on operands of 8 bits, a paged cache of keys and values in 4 or 16 bits
+ * and attention to it. Forward only, as everything here. Rows are packed and offsets mean what they mean
+ * above; nothing is allocated, everything runs in stream order and may be captured into a graph; calls that
+ * may overlap need workspaces of their own.
+ *
+ * Numbers of few bits: a block of 32 channels shares a power of two, a byte p that stands for 2^(p - 127)
+ * (255: NaN), the least one with which the block's largest value is at most the codes' largest: 448 for 8-bit
+ * codes (e4m3: 1 sign, 4 exponent, 3 mantissa bits, no infinity), 6 for 4-bit ones (e2m1: 0, 0.5, 1, 1.5, 2, 3, 4,
+ * 6 in codes 0 to 7, their negatives in 8 to 15). Values are rounded to the nearest code, halfway to the
+ * even one. A block with an Inf or a NaN in it has power 255 and stands for NaN as a whole.
+ * ------------------------------------------------------------------------------------- */
+
+/* 8-bit codes with powers, as an output dtype of tsp_rms_norm. */
+enum { TSP_MX8 = 3 };
+
+/* h = x + residual, out[i][c] = h[i][c] / sqrt(mean_c(h[i]^2) + eps) * gamma[c], residual_out = h, in fp32 (the norm is
+ * of the sum before residual_out rounds it; h^2 summed has to fit fp32). residual and residual_out share a dtype;
+ * both may be NULL, and residual_out alone; gamma f32 [c] or NULL. out_dtype TSP_MX8: codes to out, [n][c / 32] power
+ * bytes to d_powers (c a multiple of 32); else d_powers is not used. out and residual_out may be x or residual where
+ * the dtypes agree and must not overlap them or each other otherwise. c up to 2^20; rows of up to 8,192 channels
+ * in whole 16-byte pieces (c a multiple of 8, tensors and gamma 16-byte aligned) are read once, piece by piece, others twice,
+ * value by value. */
+int tsp_rms_norm(const void* d_x, int x_dtype, int64_t n, int c, const void* d_residual, int residual_dtype,
+                 const float* d_gamma, float eps, void* d_out, int out_dtype, uint8_t* d_powers, void* d_residual_out,
+                 void* stream);
+
+/* x [n][c] (c a multiple of 32) as 8-bit codes [n][c] and powers [n][c / 32]. x and codes 16-byte aligned. */
+int tsp_mx_quantize(const void* d_x, int x_dtype, int64_t n, int c, void* d_codes, uint8_t* d_powers, void* stream);
+
+/* out[n][co] = act(x W^T + bias) + residual on 8-bit operands x [n][ci] and W [co][ci] (codes 16-byte, powers 4-byte
+ * aligned; ci a multiple of 32); act 1 is y * sigmoid(y); bias f32 [co] and residual f32 [n][co] or NULL, out any dtype.
+ * out may be the residual where it is f32, and must not overlap the inputs otherwise. With 16-bit outputs products are
+ * added at the matrix cores' 8-bit precision (off by some 1.5e-5 of the result in the 2-norm, a small part of the
+ * output's rounding); with f32 outputs in fp32, at half the rate. The result does not depend on what the workspace,
+ * 16-byte aligned, of tsp_linear_mx_workspace_bytes bytes held (0, and NULL will do, where it needs none). */
+size_t tsp_linear_mx_workspace_bytes(int64_t n, int ci, int co);
+int tsp_linear_mx(const void* d_x, const uint8_t* d_x_powers, int64_t n, int ci, const void* d_w, const uint8_t* d_w_powers,
+                  const float* d_bias, int co, int act, const float* d_residual, void* d_out, int out_dtype,
+                  void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* A paged cache: `pages` pages of tsp_kv_page_bytes bytes, each of `page` tokens (16, 32, 64, 128 or 256) of `heads` heads
+ * of d elements (a multiple of 8 up to 128) of keys and of values. For each head in turn a page holds, with
+ * format TSP_KV_MX4, K codes [page][16 B], V codes [page][16 B], K powers [page][B] and V powers [page][B], where
+ * B = ceil(d / 32) and element 2i of a row is the low half of its byte i (elements past d are zero); with TSP_F16 or
+ * TSP_BF16, K [page][d] and V [page][d]. data 16-byte aligned.
+ *
+ * Sample s has d_lengths[s] keys; key j lies in page d_table[s][j / page], slot j % page, of the int32 table
+ * [samples][max_pages] (samples may share pages). Lengths are cut to [0, max_pages * page]. A page that is not
+ * one of the pool's holds nothing: its keys are not written, are seen by no row, and read as zeros. */
+enum { TSP_KV_MX4 = 4 };
+typedef struct {
+    void* data;
+    int64_t pages;
+    int page, heads, d, format;
+} tsp_kv_cache;
+size_t tsp_kv_page_bytes(int page, int heads, int d, int format);
+
+/* New keys and values into the cache, their positions on the way: of sample s with m rows of k and v (offsets as
+ * above), row i becomes key d_lengths[s] - m + i (d_lengths: the lengths after the call; keys below 0 or past the
+ * table are not written). Keys are turned, and RMS-normalised before that where k_gamma is given, as by
+ * tsp_rope_axes; so is q [n][hq][d] (NULL and 0 without), which goes to q_out. axes 0: no turning, d_pos and pairs
+ * not used. Keys for 4 bits are turned in 64 bits, so that each code is that of the exact value; their values
+ * have to fit fp32. One dtype for q, k, v and q_out; strides and alignment as for tsp_rope_axes; q_out may be q with
+ * the same strides. Two rows of a call must not go to one place in the cache. */
+int tsp_kv_append(const tsp_kv_cache* cache, const tsp_heads* k, const tsp_heads* v, int dtype, int64_t n,
+                  const int32_t* d_offsets, int samples, const int32_t* d_table, int max_pages, const int32_t* d_lengths,
+                  const tsp_heads* q, int hq, const int32_t* d_pos, int axes, const int* pairs, double theta, int flags,
+                  const float* d_q_gamma, const float* d_k_gamma, double eps, const tsp_heads* q_out, void* stream);
+
+/* Keys and values out of the cache, packed: of sample s with m rows of the outputs, row i is key d_lengths[s] - m + i
+ * (zeros where the cache does not hold it). Outputs [n][heads][d] of any dtype. */
+int tsp_kv_gather(const tsp_kv_cache* cache, int64_t n, const int32_t* d_offsets, int samples, const int32_t* d_table,
+                  int max_pages, const int32_t* d_lengths, const tsp_heads* k_out, const tsp_heads* v_out, int out_dtype,
+                  void* stream);
+
+/* Softmax attention of q's rows to their samples' cached keys, as tsp_attention computes it: of sample s with m rows,
+ * row i sees all of its d_lengths[s] keys, or with causal != 0 those with j <= i + (d_lengths[s] - m). A row that sees
+ * no key gets zeros; a key that a row does not see has no effect on it, whatever it holds. q and out f16 or bf16, of the cache's
+ * dtype where that holds 16 bits; hq a multiple of the cache's heads; scale > 0; with f16 heads a 4-bit cache's values have
+ * to fit f16. nq * hq / heads and max_pages * page below 2^31 - 2^16. The line of all work is cut evenly over the device
+ * whatever the samples' lengths, and joined in the workspace, 16-byte aligned, of
+ * tsp_attention_cached_workspace_bytes bytes; the result does not depend on what that held, nor on the order in
+ * which workgroups run. out must not overlap the inputs. */
+size_t tsp_attention_cached_workspace_bytes(int64_t nq, int samples, int hq, const tsp_kv_cache* cache, int max_pages);
+int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, int hq, const tsp_kv_cache* cache,
+                         const int32_t* d_offsets, int samples, const int32_t* d_table, int max_pages,
+                         const int32_t* d_lengths, float scale, int causal, const tsp_heads* out, void* d_workspace,
+                         size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,11 +12,12 @@ from __future__ import annotations
 import ctypes
 import os
 import subprocess
+from typing import Any, NamedTuple
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libtrellis_sparse.so")
 
-TSP_F32, TSP_F16, TSP_BF16 = 0, 1, 2
+TSP_F32, TSP_F16, TSP_BF16, TSP_MX8, TSP_KV_MX4 = 0, 1, 2, 3, 4
 ALGO = {"auto": 0, "mfma": 1, "narrow": 2, "mfma_gather": 3, "thin": 4, "thin_mfma": 5, "f32_mfma": 6}
 STATUS = {0: "OK", 1: "INVALID", 2: "HIP", 3: "RANGE", 4: "UNSUPPORTED", 5: "WORKSPACE"}
 
@@ -36,6 +37,8 @@ EXPORTS = (
     "tsp_convnext_workspace_bytes", "tsp_convnext", "tsp_convnext_ex", "tsp_c2s_workspace_bytes", "tsp_c2s",
     "tsp_c2s_ex", "tsp_c2s_part",
     "tsp_group_norm_workspace_bytes", "tsp_group_norm", "tsp_rope_axes", "tsp_attention_workspace_bytes", "tsp_attention",
+    "tsp_rms_norm", "tsp_mx_quantize", "tsp_linear_mx_workspace_bytes", "tsp_linear_mx",
+    "tsp_kv_page_bytes", "tsp_kv_append", "tsp_kv_gather", "tsp_attention_cached_workspace_bytes", "tsp_attention_cached",
 )
 
 BLOCK_CAST_F32 = 2
@@ -61,6 +64,12 @@ class C2SWeights(ctypes.Structure):
 class Heads(ctypes.Structure):
     """tsp_heads: rows of heads, strides in elements."""
     _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class KvCacheArg(ctypes.Structure):
+    """tsp_kv_cache."""
+    _fields_ = [("data", ctypes.c_void_p), ("pages", ctypes.c_int64), ("page", ctypes.c_int), ("heads", ctypes.c_int),
+                ("d", ctypes.c_int), ("format", ctypes.c_int)]
 
 
 class TspError(RuntimeError):
@@ -191,6 +200,27 @@ def lib() -> ctypes.CDLL:
     L.tsp_attention.restype = c_int
     L.tsp_attention.argtypes = [hp, hp, hp, c_int, c_i64, c_i64, c_int, c_int, c_int, c_vp, c_vp, c_int, c_f, c_int, hp,
                                 c_vp, c_sz, c_vp]
+    L.tsp_rms_norm.restype = c_int
+    L.tsp_rms_norm.argtypes = [c_vp, c_int, c_i64, c_int, c_vp, c_int, c_vp, c_f, c_vp, c_int, c_vp, c_vp, c_vp]
+    L.tsp_mx_quantize.restype = c_int
+    L.tsp_mx_quantize.argtypes = [c_vp, c_int, c_i64, c_int, c_vp, c_vp, c_vp]
+    L.tsp_linear_mx_workspace_bytes.restype = c_sz
+    L.tsp_linear_mx_workspace_bytes.argtypes = [c_i64, c_int, c_int]
+    L.tsp_linear_mx.restype = c_int
+    L.tsp_linear_mx.argtypes = [c_vp, c_vp, c_i64, c_int, c_vp, c_vp, c_vp, c_int, c_int, c_vp, c_vp, c_int, c_vp, c_sz, c_vp]
+    kvp = ctypes.POINTER(KvCacheArg)
+    L.tsp_kv_page_bytes.restype = c_sz
+    L.tsp_kv_page_bytes.argtypes = [c_int, c_int, c_int, c_int]
+    L.tsp_kv_append.restype = c_int
+    L.tsp_kv_append.argtypes = [kvp, hp, hp, c_int, c_i64, c_vp, c_int, c_vp, c_int, c_vp, hp, c_int, c_vp, c_int,
+                                ctypes.POINTER(c_int), ctypes.c_double, c_int, c_vp, c_vp, ctypes.c_double, hp, c_vp]
+    L.tsp_kv_gather.restype = c_int
+    L.tsp_kv_gather.argtypes = [kvp, c_i64, c_vp, c_int, c_vp, c_int, c_vp, hp, hp, c_int, c_vp]
+    L.tsp_attention_cached_workspace_bytes.restype = c_sz
+    L.tsp_attention_cached_workspace_bytes.argtypes = [c_i64, c_int, c_int, kvp, c_int]
+    L.tsp_attention_cached.restype = c_int
+    L.tsp_attention_cached.argtypes = [hp, c_int, c_i64, c_int, kvp, c_vp, c_int, c_vp, c_int, c_vp, c_f, c_int, hp, c_vp, c_sz,
+                                       c_vp]
     _lib = L
     return L
 
@@ -1069,5 +1099,314 @@ def attention(q, k, v, q_offsets=None, k_offsets=None, causal: bool = False, sca
                lib().tsp_attention(qh, kh, vh, dtype_code(q.dtype), nq, nk, hq, hkv, d, _p(q_offsets), _p(k_offsets), samples,
                                    d ** -0.5 if scale is None else scale, 1 if causal else 0, oh, _p(ws),
                                    0 if ws is None else ws.numel(), s))
+        return o
+    return _launch(dev, stream, call)
+
+
+# --------------------------------------------------------------------------------------------
+# a served transformer block's step: RMS norm, linears on 8 bits, a paged cache and attention to it
+# --------------------------------------------------------------------------------------------
+class Mx(NamedTuple):
+    """Rows in 8 bits: codes float8_e4m3fn [N, C], times a power of two for every 32 channels, float8_e8m0fnu
+    [N, C / 32]."""
+    codes: Any
+    powers: Any
+
+
+def mx_empty(n: int, c: int, device="cuda") -> Mx:
+    """Buffers for [N, C] rows in 8 bits."""
+    torch = _torch()
+    if c % 32:
+        raise ValueError(f"rows in 8 bits need a multiple of 32 channels, got {c}")
+    return Mx(torch.empty((n, c), dtype=torch.float8_e4m3fn, device=device),
+              torch.empty((n, c // 32), dtype=torch.float8_e8m0fnu, device=device))
+
+
+def _check_mx(m, n, c, device, name: str):
+    """n and c may be None: any. -> (n, c)"""
+    torch = _torch()
+    codes, powers = m
+    if codes.dtype != torch.float8_e4m3fn or powers.dtype not in (torch.float8_e8m0fnu, torch.uint8) or codes.dim() != 2 or powers.dim() != 2:
+        raise ValueError(f"{name} must be Mx(codes float8_e4m3fn [N, C], powers float8_e8m0fnu [N, C / 32])")
+    rows, ch = codes.shape
+    if (n is not None and rows != n) or (c is not None and ch != c) or ch % 32 or tuple(powers.shape) != (rows, ch // 32):
+        raise ValueError(f"{name} has codes {list(codes.shape)} and powers {list(powers.shape)}, expected {[n, c]} and one for 32 channels")
+    if not codes.is_contiguous() or not powers.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    _same_device(device, f"{name}'s codes", codes, f"{name}'s powers", powers)
+    return rows, ch
+
+
+def rms_norm(x, gamma=None, eps: float = 1e-6, residual=None, residual_out=None, out_dtype=None, out=None, stream=None):
+    """RMS norm of rows with the residual's addition: h = x [N, C] + residual, y = h / sqrt(mean(h^2) + eps) * gamma in
+    fp32 -> y, or with a residual (y, h in the residual's dtype). out_dtype torch.float8_e4m3fn (or out an Mx): y in 8
+    bits, as Mx, for linear_mx (C a multiple of 32). out and residual_out may be given; they may be x or residual where
+    the dtypes agree."""
+    torch = _torch()
+    if x.dim() != 2:
+        raise ValueError(f"x must be [N, C], got {tuple(x.shape)}")
+    n, c = x.shape
+    dev = x.device
+    if gamma is not None and (gamma.dtype != torch.float32 or gamma.numel() != c or not gamma.is_contiguous()):
+        raise ValueError(f"gamma must be a contiguous float32 vector of {c}")
+    if residual is not None and tuple(residual.shape) != (n, c):
+        raise ValueError(f"residual must be {[n, c]}, got {list(residual.shape)}")
+    if residual_out is not None:
+        if residual is None:
+            raise ValueError("residual_out needs a residual")
+        _check_out(residual_out, n, c, residual.dtype, dev)
+    _same_device(dev, "gamma", gamma, "residual", residual)
+    mx = isinstance(out, tuple) if out is not None else out_dtype == torch.float8_e4m3fn
+    if mx:
+        if out_dtype not in (None, torch.float8_e4m3fn):
+            raise ValueError(f"out is in 8 bits, out_dtype {out_dtype}")
+        if c % 32:
+            raise ValueError(f"rows in 8 bits need a multiple of 32 channels, got {c}")
+        if out is not None:
+            _check_mx(out, n, c, dev, "out")
+    elif out is not None:
+        _check_out(out, n, c, out_dtype or out.dtype, dev)
+    xd, rd = dtype_code(x.dtype), 0 if residual is None else dtype_code(residual.dtype)
+    odt = None if mx else (out.dtype if out is not None else out_dtype or x.dtype)
+    od = TSP_MX8 if mx else dtype_code(odt)
+
+    def call(s, keep):
+        xc, rc = x.contiguous(), None if residual is None else residual.contiguous()
+        o = out
+        if o is None:
+            o = mx_empty(n, c, dev) if mx else torch.empty((n, c), dtype=odt, device=dev)
+        codes, powers = o if mx else (o, None)
+        ro = residual_out
+        if ro is None and residual is not None:
+            ro = torch.empty((n, c), dtype=residual.dtype, device=dev)
+        g = _aligned(gamma)
+        keep(x, xc, residual, rc, gamma, g, codes, powers, ro)
+        _check("tsp_rms_norm", lib().tsp_rms_norm(_p(xc), xd, n, c, _p(rc), rd, _p(g), eps, _p(codes), od, _p(powers), _p(ro), s))
+        return o if residual is None else (o, ro)
+    return _launch(dev, stream, call)
+
+
+def mx_quantize(x, out=None, stream=None) -> Mx:
+    """x [N, C] rounded to 8 bits (C a multiple of 32): a layer's weight once, or rows that no norm precedes."""
+    if x.dim() != 2 or x.shape[1] % 32:
+        raise ValueError(f"x must be [N, C] with C a multiple of 32, got {tuple(x.shape)}")
+    n, c = x.shape
+    dev = x.device
+    _same_device(dev)
+    xd = dtype_code(x.dtype)
+    if out is not None:
+        _check_mx(out, n, c, dev, "out")
+
+    def call(s, keep):
+        xc = _aligned(x.contiguous())
+        o = out if out is not None else mx_empty(n, c, dev)
+        keep(x, xc, *o)
+        _check("tsp_mx_quantize", lib().tsp_mx_quantize(_p(xc), xd, n, c, _p(o[0]), _p(o[1]), s))
+        return o
+    return _launch(dev, stream, call)
+
+
+def linear_mx_workspace(n: int, ci: int, co: int, device="cuda"):
+    """The uint8 workspace linear_mx needs for these sizes."""
+    return _torch().empty(max(lib().tsp_linear_mx_workspace_bytes(n, ci, co), 16), dtype=_torch().uint8, device=device)
+
+
+def linear_mx(x, weight, bias=None, act: str = "none", residual=None, out_dtype=None, out=None, workspace=None, stream=None):
+    """act(x W^T + bias) + residual on operands in 8 bits: x Mx of [N, Ci], weight Mx of [Co, Ci], bias float32 [Co],
+    residual float32 [N, Co] -> [N, Co] in out_dtype (bfloat16 by default; float32 is added in fp32 throughout, at half
+    the rate). out may be given, and be a float32 residual itself; workspace (linear_mx_workspace) may be given to
+    reuse it."""
+    torch = _torch()
+    dev = x[0].device
+    n, ci = _check_mx(x, None, None, dev, "x")
+    co, _ = _check_mx(weight, None, ci, dev, "weight")
+    if bias is not None and (bias.dtype != torch.float32 or bias.numel() != co or not bias.is_contiguous()):
+        raise ValueError(f"bias must be a contiguous float32 vector of {co}")
+    if residual is not None and (residual.dtype != torch.float32 or tuple(residual.shape) != (n, co)):
+        raise ValueError(f"residual must be float32 {[n, co]}")
+    if out is not None:
+        _check_out(out, n, co, out_dtype or out.dtype, dev)
+    _same_device(dev, "bias", bias, "residual", residual, "workspace", workspace)
+    if workspace is not None:
+        _check_workspace(workspace)
+    odt = out.dtype if out is not None else out_dtype or torch.bfloat16
+    od, ac = dtype_code(odt), ACT[act]
+
+    def call(s, keep):
+        rc = None if residual is None else residual.contiguous()
+        o = out if out is not None else torch.empty((n, co), dtype=odt, device=dev)
+        ws = workspace
+        if ws is None:
+            need = lib().tsp_linear_mx_workspace_bytes(n, ci, co)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        xc, xp, wc, wp = _aligned(x[0]), _aligned(x[1]), _aligned(weight[0]), _aligned(weight[1])
+        keep(*x, *weight, xc, xp, wc, wp, bias, residual, rc, o, ws)
+        _check("tsp_linear_mx",
+               lib().tsp_linear_mx(_p(xc), _p(xp), n, ci, _p(wc), _p(wp), _p(bias), co, ac, _p(rc), _p(o), od, _p(ws),
+                                   0 if ws is None else ws.numel(), s))
+        return o
+    return _launch(dev, stream, call)
+
+
+class KVCache:
+    """A paged cache of keys and values: data uint8 [pages, bytes of a page], each page of `page` tokens (16, 32, 64, 128 or
+    256) of `heads` heads of d elements (a multiple of 8 up to 128), held as `dtype`: "mx4" (4 bits with a power of two for
+    every 32 elements), torch.float16 or torch.bfloat16. Made by kv_cache."""
+
+    def __init__(self, data, page: int, heads: int, d: int, dtype):
+        torch = _torch()
+        self.format = TSP_KV_MX4 if dtype == "mx4" else dtype_code(dtype) if dtype in (torch.float16, torch.bfloat16) else None
+        if self.format is None:
+            raise ValueError(f'a cache holds "mx4", float16 or bfloat16, not {dtype}')
+        size = lib().tsp_kv_page_bytes(page, heads, d, self.format)
+        if not size:
+            raise ValueError(f"no cache of pages of {page} tokens (16, 32, 64, 128 or 256), {heads} heads of {d} (a multiple of 8 up to 128)")
+        if data.dtype != torch.uint8 or data.dim() != 2 or data.shape[1] != size or not data.is_contiguous() or data.data_ptr() % 16:
+            raise ValueError(f"data must be a contiguous uint8 [pages, {size}], 16-byte aligned")
+        self.data, self.page, self.heads, self.d, self.dtype = data, page, heads, d, dtype
+        self.pages = data.shape[0]
+        self.arg = KvCacheArg(data.data_ptr(), self.pages, page, heads, d, self.format)
+
+
+def kv_cache(pages: int, page: int, heads: int, d: int, dtype="mx4", device="cuda") -> KVCache:
+    """A cache of that many pages, all zeros."""
+    torch = _torch()
+    code = TSP_KV_MX4 if dtype == "mx4" else dtype_code(dtype) if dtype in (torch.float16, torch.bfloat16) else -1
+    size = lib().tsp_kv_page_bytes(page, heads, d, code)
+    return KVCache(torch.zeros((pages, size), dtype=torch.uint8, device=device), page, heads, d, dtype)
+
+
+def _cache_places(cache, table, lengths, offsets, n: int, dev):
+    """Checks of a cache's table, lengths and rows' offsets -> (offsets, samples)."""
+    torch = _torch()
+    offsets, samples = _offsets(offsets, "offsets")
+    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != samples or table.shape[1] < 1 or not table.is_contiguous():
+        raise ValueError(f"table must be a contiguous int32 [{samples}, max_pages]")
+    if lengths.dtype != torch.int32 or lengths.dim() != 1 or lengths.shape[0] != samples or not lengths.is_contiguous():
+        raise ValueError(f"lengths must be a contiguous int32 [{samples}]")
+    _same_device(dev, "cache", cache.data, "table", table, "lengths", lengths, "offsets", offsets)
+    return offsets, samples
+
+
+def kv_append(cache: KVCache, k, v, table, lengths, offsets=None, q=None, pos=None, pairs=None, theta: float = 10000.0,
+              interleaved: bool = True, q_gamma=None, k_gamma=None, eps: float = 1e-6, q_out=None, stream=None):
+    """New keys and values k, v [N, Hkv, D] of packed samples into the cache, turned to their positions on the way. Of sample
+    s with m rows (offsets int32 [samples + 1]; None: one sample), row i becomes key lengths[s] - m + i (lengths int32
+    [samples]: the samples' keys after the call), in page table[s, key // page] of the int32 table [samples, max_pages].
+    pos int32 [N, axes], pairs, theta, interleaved and the gammas are rope_axes'; pos None: no turning. q [N, Hq, D] is
+    normalised and turned in the same launch -> q's result (None without q); rows that are no sample's are left as
+    they were in q_out, and in none. Keys whose place is not one of the cache's are not written; two rows must not have
+    one place. q_out may be q itself."""
+    torch = _torch()
+    if k.dim() != 3 or v.shape != k.shape or k.shape[1:] != (cache.heads, cache.d):
+        raise ValueError(f"k and v must be [N, {cache.heads}, {cache.d}]")
+    n, hkv, d = k.shape
+    dev = k.device
+    if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
+        raise ValueError("q, k and v must have one dtype")
+    if q is None and (q_gamma is not None or q_out is not None):
+        raise ValueError("q_gamma and q_out need q")
+    if q is not None and (q.dim() != 3 or q.shape[0] != n or q.shape[2] != d):
+        raise ValueError(f"q must be [{n}, Hq, {d}]")
+    hq = 0 if q is None else q.shape[1]
+    offsets, samples = _cache_places(cache, table, lengths, offsets, n, dev)
+    axes = 0
+    if pos is not None:
+        if pos.dtype != torch.int32 or pos.dim() != 2 or pos.shape[0] != n or not 1 <= pos.shape[1] <= 4:
+            raise ValueError("pos must be int32 [N, axes] with 1 to 4 axes")
+        axes = pos.shape[1]
+        pairs = (d // 2 // axes,) * axes if pairs is None else tuple(map(int, pairs))
+        if len(pairs) != axes:
+            raise ValueError(f"pairs must name a count for each of {axes} axes")
+    for name, g, h in (("q_gamma", q_gamma, hq), ("k_gamma", k_gamma, hkv)):
+        if g is not None and (g.dtype != torch.float32 or g.shape != (h, d) or not g.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous float32 {[h, d]}")
+    _same_device(dev, "q", q, "v", v, "pos", pos, "q_gamma", q_gamma, "k_gamma", k_gamma)
+    given = None if q_out is None else _heads_out(q_out, n, hq, d, k.dtype, dev, "q_out")
+    code = dtype_code(k.dtype)
+
+    def call(s, keep):
+        (kc, kh), (vc, vh) = _fitted(k, n, hkv, d), _fitted(v, n, hkv, d)
+        qc = qh = qo = qoh = None
+        if q is not None:
+            qc, qh = _fitted(q, n, hq, d)
+            qo, qoh = (q_out, given) if q_out is not None else _fitted(torch.empty((n, hq, d), dtype=q.dtype, device=dev), n, hq, d)
+        pc = None if pos is None else pos.contiguous()
+        gq, gk = _aligned(q_gamma), _aligned(k_gamma)
+        keep(k, v, q, kc, vc, qc, qo, pos, pc, q_gamma, k_gamma, gq, gk, table, lengths, offsets, cache.data)
+        _check("tsp_kv_append",
+               lib().tsp_kv_append(cache.arg, kh, vh, code, n, _p(offsets), samples, _p(table), table.shape[1], _p(lengths), qh, hq,
+                                   _p(pc), axes, (ctypes.c_int * axes)(*pairs) if axes else None, theta, 0 if interleaved else 1,
+                                   _p(gq), _p(gk), eps, qoh, s))
+        return qo
+    return _launch(dev, stream, call)
+
+
+def kv_gather(cache: KVCache, table, lengths, offsets=None, n=None, out_dtype=None, k_out=None, v_out=None, stream=None):
+    """Keys and values out of the cache -> packed (k, v) [N, Hkv, D] in out_dtype (bfloat16 by default, a 16-bit cache's own):
+    of sample s with m rows (offsets; None: one sample of n), row i is key lengths[s] - m + i, zeros where the cache does
+    not hold it; rows that are no sample's are left as they were. N is k_out's and v_out's, or n."""
+    torch = _torch()
+    dev = cache.data.device
+    for name, o in (("k_out", k_out), ("v_out", v_out)):
+        if o is not None and o.dim() == 3 and n is None:
+            n = o.shape[0]
+    if n is None:
+        raise ValueError("the number of rows: k_out, v_out or n")
+    offsets, samples = _cache_places(cache, table, lengths, offsets, n, dev)
+    odt = out_dtype or (k_out.dtype if k_out is not None else v_out.dtype if v_out is not None
+                        else torch.bfloat16 if cache.dtype == "mx4" else cache.dtype)
+    h, d = cache.heads, cache.d
+    kg = None if k_out is None else _heads_out(k_out, n, h, d, odt, dev, "k_out")
+    vg = None if v_out is None else _heads_out(v_out, n, h, d, odt, dev, "v_out")
+    code = dtype_code(odt)
+
+    def call(s, keep):
+        ko, kh = (k_out, kg) if k_out is not None else _fitted(torch.empty((n, h, d), dtype=odt, device=dev), n, h, d)
+        vo, vh = (v_out, vg) if v_out is not None else _fitted(torch.empty((n, h, d), dtype=odt, device=dev), n, h, d)
+        keep(ko, vo, table, lengths, offsets, cache.data)
+        _check("tsp_kv_gather", lib().tsp_kv_gather(cache.arg, n, _p(offsets), samples, _p(table), table.shape[1], _p(lengths), kh, vh, code, s))
+        return ko, vo
+    return _launch(dev, stream, call)
+
+
+def attention_cached_workspace(nq: int, samples: int, hq: int, cache: KVCache, max_pages: int):
+    """The uint8 workspace attention_cached needs for these sizes."""
+    return _torch().empty(max(lib().tsp_attention_cached_workspace_bytes(nq, samples, hq, cache.arg, max_pages), 16),
+                          dtype=_torch().uint8, device=cache.data.device)
+
+
+def attention_cached(q, cache: KVCache, table, lengths, offsets=None, causal: bool = True, scale=None, out=None, workspace=None,
+                     stream=None):
+    """Softmax attention of q [Nq, Hq, D] (float16 or bfloat16; a 16-bit cache's dtype) to its samples' cached keys ->
+    [Nq, Hq, D]. Of sample s with m rows (offsets int32 [samples + 1]; None: one sample), row i sees all lengths[s] keys, or
+    with causal those with j <= i + (lengths[s] - m): after kv_append with the same lengths, its own key and those before. A
+    row that sees none gets zeros; rows of out outside every sample are left as they were. Hq is a multiple of the
+    cache's heads, scale defaults to D ** -0.5; workspace (attention_cached_workspace) may be given to reuse it."""
+    torch = _torch()
+    if q.dim() != 3 or q.shape[2] != cache.d or q.shape[1] % cache.heads:
+        raise ValueError(f"q must be [Nq, Hq, {cache.d}] with Hq a multiple of {cache.heads}, got {list(q.shape)}")
+    nq, hq, d = q.shape
+    dev = q.device
+    if q.dtype not in (torch.float16, torch.bfloat16) or (cache.dtype != "mx4" and cache.dtype != q.dtype):
+        raise ValueError(f"q must be float16 or bfloat16, and a 16-bit cache's dtype; got {q.dtype} on {cache.dtype}")
+    offsets, samples = _cache_places(cache, table, lengths, offsets, nq, dev)
+    _same_device(dev, "workspace", workspace)
+    given = None if out is None else _heads_out(out, nq, hq, d, q.dtype, dev, "out")
+    if workspace is not None:
+        _check_workspace(workspace)
+    code = dtype_code(q.dtype)
+
+    def call(s, keep):
+        qc, qh = _fitted(q, nq, hq, d)
+        o, oh = (out, given) if out is not None else _fitted(torch.empty((nq, hq, d), dtype=q.dtype, device=dev), nq, hq, d)
+        ws = workspace
+        if ws is None:
+            need = lib().tsp_attention_cached_workspace_bytes(nq, samples, hq, cache.arg, table.shape[1])
+            ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        keep(q, qc, o, ws, table, lengths, offsets, cache.data)
+        _check("tsp_attention_cached",
+               lib().tsp_attention_cached(qh, code, nq, hq, cache.arg, _p(offsets), samples, _p(table), table.shape[1], _p(lengths),
+                                          d ** -0.5 if scale is None else scale, 1 if causal else 0, oh, _p(ws), ws.numel(), s))
         return o
     return _launch(dev, stream, call)

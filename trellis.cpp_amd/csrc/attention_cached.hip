@@ -1,0 +1,626 @@
+// Softmax attention of new queries to the keys and values of a paged cache (kv_cache.hpp), in 4 or 16 bits:
+//   out[i][h] = sum_j exp(scale q_i . k_j - max) v_j / sum_j exp(scale q_i . k_j - max)
+// over the keys j of i's sample that the row sees: all lengths[s] of them, or with `causal` those with
+// j <= i + (lengths[s] - Lq). A row that sees none gets zeros.
+//
+// A row is a (query, head of the group) pair, a unit is up to ROWS rows of a sample and key head, its work the tiles of
+// keys that they see. All units' tiles stand in one line, which is cut into as many equal parts as there are workgroups,
+// whatever the samples' lengths: only the device knows those. A workgroup goes through its part unit by unit; a
+// unit that a cut goes through leaves its rows' maxima, sums and sums of p v in the workspace, at most two a workgroup,
+// and a second launch joins them, in their order. (The line's weights are a linear estimate of a unit's tiles,
+// so that its sums have a closed form; where in a unit a cut falls goes by its true tiles.)
+//
+// 4-bit codes become 16-bit values with their power as they are read, two a conversion, exactly (in f16: for powers
+// that fit it). Both products run on the matrix cores with their roles turned, S^T = K Q^T and O^T = V^T P^T, so that
+// a lane holds scores of one row and P is the second product's operand where it stands. Statistics and accumulators are
+// fp32; P is rounded to the heads' type, as the packed attention's (attention.hip) is, and formed as there.
+//
+// Waves of their own, each with every fourth tile of 32 keys: K goes from memory to its operand, V through a piece of LDS
+// that is the wave's alone, where it is turned.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "attention_internal.hpp"
+#include "kv_cache.hpp"
+#include "mx.hpp"
+
+namespace tsp {
+namespace {
+
+constexpr int CF_KEYS = 32, CF_NW = 4;       // few rows: keys of a tile, waves
+
+struct CachedArgs {
+    const void* q;
+    void* o;
+    int64_t q_row, q_head, o_row, o_head;      // strides in elements
+    KvArgs cache;
+    const int32_t* q_off;
+    int64_t nq;                                // below 2^31, nq * share too
+    int samples, share, causal;
+    int groups, least;                         // workgroups, tiles that one has at least
+    FastDiv by_share;
+    float scale2;                              // scale * log2(e)
+    float* part;                               // [2 * groups][row][d] sums of p v, and
+    float2* stat;                              // [2 * groups][row] maximum and sum of p (-1: no key seen)
+};
+
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
+}
+__device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
+    return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)x, lane));
+}
+
+// A sample's units (one key head) and their weights, first + slope * j of the j-th.
+struct SampleWork {
+    int row0, lq, lk, count, first, slope;
+    __device__ __forceinline__ int64_t before(int64_t j) const { return first * j + slope * (j * (j - 1) / 2); }
+};
+// Keys that a row sees, by its query.
+__device__ __forceinline__ int cached_limit(int causal, int lq, int lk, int query) { return causal ? min(max(lk - lq + query + 1, 0), lk) : lk; }
+template <int ROWS, int TILE>
+__device__ __forceinline__ int unit_tiles(const CachedArgs& a, int lq, int lk, int j) {
+    const int last = min((j + 1) * ROWS, lq * a.share) - 1;
+    return (cached_limit(a.causal, lq, lk, last / a.by_share) + TILE - 1) / TILE;
+}
+template <int ROWS, int TILE>
+__device__ __forceinline__ SampleWork sample_work(const CachedArgs& a, int s) {
+    SampleWork w{0, 0, 0, 0, 1, 0};
+    if (s >= a.samples) return w;
+    packed_rows(a.q_off, s, (int)a.nq, w.row0, w.lq);
+    w.lk = kv_length(a.cache, s);
+    w.count = (int)((unsigned)(w.lq * a.share + ROWS - 1) / (unsigned)ROWS);
+    if (w.count == 0) return w;
+    w.first = max(1, unit_tiles<ROWS, TILE>(a, w.lq, w.lk, 0));
+    if (w.count > 1) w.slope = max(0, (unit_tiles<ROWS, TILE>(a, w.lq, w.lk, w.count - 1) - w.first) / (w.count - 1));
+    return w;
+}
+
+// The length of the line (by whole waves).
+template <int ROWS, int TILE>
+__device__ __forceinline__ int64_t line_length(const CachedArgs& a) {
+    int64_t sum = 0;
+    for (int s0 = 0; s0 < a.samples; s0 += 64) {
+        const SampleWork w = sample_work<ROWS, TILE>(a, s0 + (threadIdx.x & 63));
+        sum += w.before(w.count) * a.cache.heads;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    return uniform(sum);
+}
+
+// A unit and where it stands in the line.
+struct CachedUnit {
+    int sample, head, row0, lq, lk;      // (sample -1: none)
+    int first_row;                       // of its rows among the sample's
+    int tiles;
+    int64_t begin, end;
+};
+// The unit at a place in the line (by whole waves, all with one `at`).
+template <int ROWS, int TILE>
+__device__ __forceinline__ CachedUnit find_unit(const CachedArgs& a, int64_t at) {
+    CachedUnit u{-1, 0, 0, 0, 0, 0, 0, 0, 0};
+    const int lane = threadIdx.x & 63;
+    int64_t base = 0;
+    for (int s0 = 0; s0 < a.samples; s0 += 64) {
+        const SampleWork w = sample_work<ROWS, TILE>(a, s0 + lane);
+        const int64_t mine = w.before(w.count) * a.cache.heads;
+        int64_t end = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t v = __shfl_up(end, o, 64);
+            if (lane >= o) end += v;
+        }
+        end += base;
+        const uint64_t found = __ballot(at >= end - mine && at < end);
+        if (found) {
+            const int l = __builtin_ctzll(found);
+            u.sample = s0 + l;
+            u.row0 = __builtin_amdgcn_readlane(w.row0, l);
+            u.lq = __builtin_amdgcn_readlane(w.lq, l);
+            u.lk = __builtin_amdgcn_readlane(w.lk, l);
+            const SampleWork k{0, 0, 0, __builtin_amdgcn_readlane(w.count, l), __builtin_amdgcn_readlane(w.first, l), __builtin_amdgcn_readlane(w.slope, l)};
+            const int64_t start = lane_value(end - mine, l), per_head = k.before(k.count);
+            const int64_t in = at - start;
+            u.head = (int)(in / per_head);
+            const int64_t x = in - u.head * per_head;
+            int64_t j;
+            if (k.slope == 0) {
+                j = x / k.first;
+            } else {      // first j + slope j (j - 1) / 2 <= x
+                const double b = k.first - 0.5 * k.slope;
+                j = (int64_t)((sqrt(b * b + 2. * k.slope * (double)x) - b) / k.slope);
+                j = min(max(j, (int64_t)0), (int64_t)k.count - 1);
+                while (j > 0 && k.before(j) > x) --j;
+                while (j + 1 < k.count && k.before(j + 1) <= x) ++j;
+            }
+            j = uniform(j);
+            u.first_row = (int)j * ROWS;
+            u.begin = start + u.head * per_head + k.before(j);
+            u.end = u.begin + k.first + k.slope * j;
+            u.tiles = unit_tiles<ROWS, TILE>(a, u.lq, u.lk, (int)j);
+            return u;
+        }
+        base = lane_value(end, 63);
+    }
+    return u;
+}
+
+// Workgroups that share the line, and where the w-th begins.
+__device__ __forceinline__ int64_t line_groups(const CachedArgs& a, int64_t length) { return min((int64_t)a.groups, max((int64_t)1, length / a.least)); }
+__device__ __forceinline__ int64_t line_cut(int64_t length, int64_t groups, int64_t w) { return length * w / groups; }
+// The workgroup that holds a place.
+__device__ __forceinline__ int64_t line_group(int64_t length, int64_t groups, int64_t at) { return ((at + 1) * groups - 1) / length; }
+
+// One workgroup's piece of a unit: tiles [t0, t1) of it, and its place in the workspace (-1: it has all of the unit).
+struct CachedPiece {
+    int t0, t1, slot;
+};
+__device__ __forceinline__ CachedPiece cut_unit(const CachedUnit& u, int64_t from, int64_t to, int w) {
+    const int64_t lo = max(from, u.begin) - u.begin, hi = min(to, u.end) - u.begin, weight = u.end - u.begin;
+    CachedPiece p;
+    p.t0 = (int)(u.tiles * lo / weight);
+    p.t1 = (int)(u.tiles * hi / weight);
+    p.slot = lo == 0 && hi == weight ? -1 : 2 * w + (lo == 0);
+    return p;
+}
+
+// Four bytes of codes as eight 16-bit values.
+template <bool BF16>
+__device__ __forceinline__ u32x4_t widen4(uint32_t c, float s) {
+    if constexpr (BF16)
+        return u32x4_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0)),
+                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1)),
+                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2)),
+                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3))};
+    else
+        return u32x4_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 0)),
+                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 1)),
+                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 2)),
+                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, 3))};
+}
+
+template <bool BF16>
+__device__ __forceinline__ f32x4_t mfma16(const u32x4_t& a, const u32x4_t& b, const f32x4_t& c) {
+    if constexpr (BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// Byte offset of a 16-byte piece of V in a staged tile: as v_piece, and the piece's lowest bit xored with the key's, so
+// that the 16 pieces that two keys' lanes write at once (every fourth of each) lie in other banks.
+template <int DP>
+__device__ __forceinline__ int cv_piece(int key, int piece) { return v_piece<DP>(key, piece ^ (DP >= 64 ? key & 1 : 0)); }
+
+template <bool BF16>
+__device__ __forceinline__ bool any_nonfinite(const u32x4_t& v) {
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) odd |= nonfinite16<BF16>(v[i]) || nonfinite16<BF16>(v[i] >> 16);
+    return odd;
+}
+template <bool BF16>
+__device__ __forceinline__ u32x4_t finite_only(u32x4_t v) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (nonfinite16<BF16>(v[e])) v[e] &= 0xffff0000u;
+        if (nonfinite16<BF16>(v[e] >> 16)) v[e] &= 0xffffu;
+    }
+    return v;
+}
+template <bool BF16>
+__device__ __forceinline__ float value16(uint32_t b) { return BF16 ? bf16_bits_to_f32((uint16_t)b) : f16_bits_to_f32((uint16_t)b); }
+
+// ---- few rows ------------------------------------------------------------------------------------------------------
+// NB: blocks of 32 channels a head; MX4: 4-bit pages; RT: tiles of 16 rows.
+template <bool BF16, int NB, bool MX4, int RT>
+__global__ __launch_bounds__(CF_NW * 64) void k_cached_few(CachedArgs a) {
+    constexpr int DP = NB * 32, ROWS = RT * 16, DB = NB * 2;
+    constexpr int VP = MX4 ? NB : NB * 4;                        // 16-byte pieces of a key's V in the page
+    constexpr int VL = (CF_KEYS * VP + 63) / 64;                 // loads of them a lane
+    constexpr int V_BYTES = CF_KEYS * DP * 2, O_BYTES = ROWS * DP * 4;
+    __shared__ __attribute__((aligned(16))) char sBuf[CF_NW][V_BYTES > O_BYTES ? V_BYTES : O_BYTES];
+    __shared__ float2 sStat[CF_NW][ROWS];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
+    char* sV = sBuf[wave];
+    const KvArgs& kv = a.cache;
+    const int64_t length = line_length<ROWS, CF_KEYS>(a);
+    if (length == 0) return;
+    const int64_t groups = line_groups(a, length);
+    if ((int)blockIdx.x >= groups) return;
+    const int64_t to = line_cut(length, groups, blockIdx.x + 1);
+    const int page_mask = (1 << kv.page_bits) - 1;
+    constexpr float LAG = BF16 ? 8.f : 4.f, LIFT = BF16 ? 0.f : 11.f;
+
+    for (int64_t from = line_cut(length, groups, blockIdx.x); from < to;) {
+        const CachedUnit u = find_unit<ROWS, CF_KEYS>(a, from);
+        const CachedPiece piece = cut_unit(u, from, to, blockIdx.x);
+        from = u.end;
+        const int rows = u.lq * a.share;
+        // rows past the sample's last are copies of it that are not stored
+        int limit[RT];
+        u32x4_t qf[RT][NB];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int r = min(u.first_row + rt * 16 + r16, rows - 1), qi = r / a.by_share, hq = u.head * a.share + r - qi * a.share;
+            limit[rt] = cached_limit(a.causal, u.lq, u.lk, qi);
+            const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (int64_t)(u.row0 + qi) * a.q_row + hq * a.q_head;
+            // chunk c = NB g + i of eight channels
+#pragma unroll
+            for (int i = 0; i < NB; ++i) qf[rt][i] = (NB * g + i) * 8 < kv.d ? *reinterpret_cast<const u32x4_t*>(qp + (NB * g + i) * 8) : u32x4_t{0, 0, 0, 0};
+        }
+        const int all_see = cached_limit(a.causal, u.lq, u.lk, u.first_row / a.by_share);      // (the first row sees least)
+        f32x4_t o[RT][DB];
+        float m[RT], l[RT];
+        bool seen[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            m[rt] = -INFINITY, l[rt] = 0.f, seen[rt] = false;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) o[rt][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
+        // What a tile's keys are loaded into: K's chunks as they are read, V's pieces.
+        struct Raw {
+            u32x4_t k[2][MX4 ? 1 : NB], v[VL];
+            uint32_t kp[2][MX4 && NB == 3 ? 2 : 1], vp[MX4 ? VL : 1];
+            bool held[2];
+        };
+        auto load = [&](int tile, Raw& w) __attribute__((always_inline)) {
+            const uint8_t* head[2];
+            int slot[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const int key = tile * CF_KEYS + kb * 16;
+                head[kb] = key < u.lk ? kv_head(kv, u.sample, key, u.head) : nullptr;
+                w.held[kb] = head[kb] != nullptr;
+                slot[kb] = key & page_mask;
+                const int at = slot[kb] + r16;
+                if constexpr (MX4) {
+                    u32x4_t c{0, 0, 0, 0};
+                    w.kp[kb][0] = 0;
+                    if constexpr (NB == 3) w.kp[kb][1] = 0;
+                    if (head[kb]) {
+                        const uint8_t *p = head[kb] + kv_codes_at(kv, 0, at) + 4 * NB * g, *pw = head[kb] + kv_powers_at(kv, 0, at);
+                        if constexpr (NB == 4) c = *reinterpret_cast<const u32x4_t*>(p);
+                        else
+#pragma unroll
+                            for (int i = 0; i < NB; ++i) c[i] = *reinterpret_cast<const uint32_t*>(p + 4 * i);
+                        w.kp[kb][0] = pw[NB * g / 4];
+                        if constexpr (NB == 3) w.kp[kb][1] = pw[(NB * g + 2) / 4];
+                    }
+                    w.k[kb][0] = c;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) {
+                        w.k[kb][i] = u32x4_t{0, 0, 0, 0};
+                        if (head[kb] && (NB * g + i) * 8 < kv.d)
+                            w.k[kb][i] = *reinterpret_cast<const u32x4_t*>(head[kb] + ((int64_t)at * kv.d + (NB * g + i) * 8) * 2);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < VL; ++i) {
+                const int idx = i * 64 + lane, key = idx / VP, p = idx % VP;
+                const uint8_t* from_head = key < 16 ? head[0] : head[1];
+                const int at = (key < 16 ? slot[0] : slot[1]) + (key & 15);
+                w.v[i] = u32x4_t{0, 0, 0, 0};
+                if constexpr (MX4) w.vp[i] = 0;
+                // (keys past the sample's last: zeros, whatever the page holds)
+                if (key < CF_KEYS && from_head && tile * CF_KEYS + key < u.lk && (MX4 || p * 8 < kv.d)) {
+                    if constexpr (MX4) {
+                        w.v[i] = *reinterpret_cast<const u32x4_t*>(from_head + kv_codes_at(kv, 1, at) + p * 16);
+                        w.vp[i] = from_head[kv_powers_at(kv, 1, at) + p];
+                    } else {
+                        w.v[i] = *reinterpret_cast<const u32x4_t*>(from_head + ((int64_t)((1 << kv.page_bits) + at) * kv.d + p * 8) * 2);
+                    }
+                }
+            }
+        };
+        auto attend = [&](int tile, const Raw& w) __attribute__((always_inline)) {
+            const int base = tile * CF_KEYS;
+            // V to LDS, as 16-bit values
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < VL; ++i) {
+                const int idx = i * 64 + lane, key = idx / VP, p = idx % VP;
+                if (CF_KEYS * VP % 64 && key >= CF_KEYS) continue;
+                if constexpr (MX4) {
+                    const float s = mx_scale(w.vp[i]);
+                    odd |= w.vp[i] == 255;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const u32x4_t x = widen4<BF16>(w.v[i][j], s);
+                        if constexpr (!BF16) odd |= any_nonfinite<BF16>(x);
+                        *reinterpret_cast<u32x4_t*>(sV + cv_piece<DP>(key, p * 4 + j)) = x;
+                    }
+                } else {
+                    odd |= any_nonfinite<BF16>(w.v[i]);
+                    *reinterpret_cast<u32x4_t*>(sV + cv_piece<DP>(key, p)) = w.v[i];
+                }
+            }
+            // scores: s[rt][kb][i] is key 16 kb + 4 g + i
+            f32x4_t s[RT][2];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) s[rt][kb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    u32x4_t k;
+                    if constexpr (MX4) k = widen4<BF16>(w.k[kb][0][i], mx_scale(NB == 3 && (NB * g + i) / 4 != NB * g / 4 ? w.kp[kb][NB == 3 ? 1 : 0] : w.kp[kb][0]));
+                    else k = w.k[kb][i];
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) s[rt][kb] = mfma16<BF16>(k, qf[rt][i], s[rt][kb]);
+                }
+            }
+            const bool whole = base + CF_KEYS <= all_see && w.held[0] && w.held[1];
+            u32x4_t pf[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                if (whole) {
+                    seen[rt] = true;
+                } else {
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool sees = w.held[kb] && base + kb * 16 + 4 * g + i < limit[rt];
+                            seen[rt] |= sees;
+                            s[rt][kb][i] = sees ? s[rt][kb][i] : -INFINITY;
+                        }
+                }
+                float mt = fmaxf(fmaxf(fmaxf(s[rt][0][0], s[rt][0][1]), fmaxf(s[rt][0][2], s[rt][0][3])),
+                                 fmaxf(fmaxf(s[rt][1][0], s[rt][1][1]), fmaxf(s[rt][1][2], s[rt][1][3])));
+                mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+                mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+                // (the maximum moves where a row's has grown by a factor of 2^LAG alone; p has room for that)
+                if (__any((mt - m[rt]) * a.scale2 > LAG)) {
+                    const float mn = fmaxf(m[rt], mt), corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[rt] - mn) * a.scale2);
+                    m[rt] = mn;
+                    l[rt] *= corr;
+#pragma unroll
+                    for (int db = 0; db < DB; ++db)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[rt][db][i] *= corr;
+                }
+                const float top = m[rt] == -INFINITY ? 0.f : m[rt];
+                float sum = 0.f;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[rt][kb][i] = __builtin_amdgcn_exp2f(fmaf(s[rt][kb][i] - top, a.scale2, LIFT));
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        pf[rt][2 * kb + i] = pack2<BF16>(s[rt][kb][2 * i], s[rt][kb][2 * i + 1]);
+                        sum = add2<BF16>(pf[rt][2 * kb + i], sum);
+                    }
+                }
+                l[rt] += sum;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            // A probability of zero must not meet an Inf or a NaN of a key that its row does not see.
+            odd = !whole && __any(odd);
+#pragma unroll
+            for (int db = 0; db < DB; ++db) {
+                const int key = 4 * g + ((lane >> 2) & 3), p = db * 2 + ((lane >> 1) & 1), sub = (lane & 1) * 8;
+                const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(sV + cv_piece<DP>(key, p) + sub));
+                const s16x4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(sV + cv_piece<DP>(key + 16, p) + sub));
+                const uint2 ux = __builtin_bit_cast(uint2, x), uy = __builtin_bit_cast(uint2, y);
+                u32x4_t v{ux.x, ux.y, uy.x, uy.y};
+                if (odd) v = finite_only<BF16>(v);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) o[rt][db] = mfma16<BF16>(v, pf[rt], o[rt][db]);
+            }
+            if (odd) {      // the values left out, key by key, for the rows that see them
+                for (int key = 0; key < CF_KEYS; ++key) {
+                    const bool held = key < 16 ? w.held[0] : w.held[1];
+                    if (!held) continue;
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        float p = 0.f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if ((key & 19) == i) p = s[rt][0][i];
+                            if ((key & 19) == 16 + i) p = s[rt][1][i];
+                        }
+                        p = __shfl(p, (key & 12) * 4 + r16, 64);
+                        const bool sees = base + key < limit[rt];
+#pragma unroll
+                        for (int db = 0; db < DB; ++db)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const int e = db * 16 + 4 * g + i;
+                                const uint32_t b = *reinterpret_cast<const uint16_t*>(sV + cv_piece<DP>(key, e >> 3) + (e & 7) * 2);
+                                if (sees && nonfinite16<BF16>(b)) o[rt][db][i] += p * value16<BF16>(b);
+                            }
+                    }
+                }
+            }
+        };
+        int tile = piece.t0 + wave;
+        if (tile < piece.t1) {
+            Raw next;
+            load(tile, next);
+            for (; tile < piece.t1; tile += CF_NW) {
+                const Raw now = next;
+                if (tile + CF_NW < piece.t1) load(tile + CF_NW, next);
+                attend(tile, now);
+            }
+        }
+        // the waves' rows joined
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            l[rt] += __shfl_xor(l[rt], 16, 64);
+            l[rt] += __shfl_xor(l[rt], 32, 64);
+            int any = seen[rt];
+            any |= __shfl_xor(any, 16, 64);
+            any |= __shfl_xor(any, 32, 64);
+            if (g == 0) sStat[wave][rt * 16 + r16] = float2{m[rt], any ? l[rt] : -1.f};
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+                *reinterpret_cast<f32x4_t*>(sV + ((rt * 16 + r16) * DP + ((db * 16 + 4 * g) ^ ((r16 & 7) * 4))) * 4) = o[rt][db];
+        }
+        __syncthreads();
+        for (int item = threadIdx.x; item < ROWS * (DP / 4); item += CF_NW * 64) {
+            const int row = item / (DP / 4), e = item % (DP / 4) * 4, r = u.first_row + row;
+            if (r >= rows || e >= kv.d) continue;
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < CF_NW; ++w) top = fmaxf(top, sStat[w][row].y == -1.f ? -INFINITY : sStat[w][row].x);
+            float sum = 0.f;
+            bool any = false;
+            f32x4_t acc{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < CF_NW; ++w) {
+                const float2 st = sStat[w][row];
+                if (st.y == -1.f) continue;
+                any = true;
+                const float c = st.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st.x - top) * a.scale2);
+                sum += c * st.y;
+                const f32x4_t x = *reinterpret_cast<const f32x4_t*>(sBuf[w] + (row * DP + (e ^ ((row & 7) * 4))) * 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i] += c * x[i];
+            }
+            if (piece.slot >= 0) {
+                const int64_t at = (int64_t)piece.slot * ROWS + row;
+                if (e == 0) a.stat[at] = float2{top, any ? sum : -1.f};
+                *reinterpret_cast<f32x4_t*>(a.part + at * kv.d + e) = acc;
+            } else {
+                const float inv = any ? 1.f / sum : 0.f;
+                const int qi = r / a.by_share, hq = u.head * a.share + r - qi * a.share;
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + (int64_t)(u.row0 + qi) * a.o_row + hq * a.o_head + e) =
+                    uint2{pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv)};
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- the pieces of units that were cut, joined -----------------------------------------------------------------------
+// sum_s w_s (p v)_s / sum_s w_s (sum p)_s, w_s = exp(max_s - max), in the pieces' order. The workgroups of a unit are
+// those of the first cut through it, 16 rows each, 16 lanes a row, eight channels a lane.
+template <bool BF16, int ROWS, int TILE>
+__global__ __launch_bounds__(256) void k_cached_join(CachedArgs a) {
+    const int64_t length = line_length<ROWS, TILE>(a);
+    if (length == 0) return;
+    const int64_t groups = line_groups(a, length), cut = (int64_t)blockIdx.x + 1;
+    if (cut >= groups) return;
+    const int64_t place = line_cut(length, groups, cut);
+    const CachedUnit u = find_unit<ROWS, TILE>(a, place);
+    if (u.begin == place) return;
+    const int64_t g0 = line_group(length, groups, u.begin), g1 = line_group(length, groups, u.end - 1);
+    if (g0 != cut - 1) return;
+    const int row = blockIdx.y * 16 + (threadIdx.x >> 4), e = (threadIdx.x & 15) * 8, r = u.first_row + row;
+    if (r >= u.lq * a.share || e >= a.cache.d) return;
+    auto at = [&](int64_t w) { return (2 * w + (w == g0)) * ROWS + row; };
+    float top = -INFINITY;
+    for (int64_t w = g0; w <= g1; ++w) {
+        const float2 st = a.stat[at(w)];
+        if (st.y != -1.f) top = fmaxf(top, st.x);
+    }
+    float sum = 0.f, acc[8] = {};
+    bool any = false;
+    for (int64_t w = g0; w <= g1; ++w) {
+        const float2 st = a.stat[at(w)];
+        if (st.y == -1.f) continue;
+        any = true;
+        const float c = st.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st.x - top) * a.scale2);
+        sum += c * st.y;
+        float x[8];
+        load8<TSP_F32>(a.part, at(w) * a.cache.d + e, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] += c * x[i];
+    }
+    const float inv = any ? 1.f / sum : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = any ? acc[i] * inv : 0.f;
+    const int qi = r / a.by_share, hq = u.head * a.share + r - qi * a.share;
+    store8<BF16 ? TSP_BF16 : TSP_F16>(a.o, (int64_t)(u.row0 + qi) * a.o_row + hq * a.o_head + e, acc);
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// How a call is cut: the rows of a unit, the workgroups.
+struct CachedCut {
+    int rows, groups;
+};
+CachedCut cached_cut(int64_t nq, int samples, int hkv, int share) {
+    CachedCut c;
+    c.rows = 16;
+    c.groups = 1024;
+    (void)nq, (void)samples, (void)hkv, (void)share;
+    return c;
+}
+size_t cached_workspace(const CachedCut& c, int d) { return (size_t)c.groups * 2 * c.rows * (d * sizeof(float) + sizeof(float2)); }
+
+}  // namespace
+}  // namespace tsp
+
+using namespace tsp;
+
+extern "C" size_t tsp_attention_cached_workspace_bytes(int64_t nq, int samples, int hq, const tsp_kv_cache* cache, int max_pages) {
+    if (!cache || !kv_valid(*cache) || nq <= 0 || nq >= (1ll << 31) || samples <= 0 || hq <= 0 || hq % cache->heads || max_pages <= 0) return 0;
+    return cached_workspace(cached_cut(nq, samples, cache->heads, hq / cache->heads), cache->d);
+}
+
+extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, int hq, const tsp_kv_cache* cache, const int32_t* d_offsets,
+                                    int samples, const int32_t* d_table, int max_pages, const int32_t* d_lengths, float scale, int causal,
+                                    const tsp_heads* out, void* d_workspace, size_t workspace_bytes, void* stream) {
+    clear_error();
+    TSP_REQUIRE(cache, TSP_ERR_INVALID, "tsp_attention_cached: null cache");
+    const tsp_kv_cache& c = *cache;
+    TSP_REQUIRE(kv_valid(c), TSP_ERR_UNSUPPORTED, "tsp_attention_cached: a cache of %lld pages of %d tokens, %d heads of %d, format %d",
+                (long long)c.pages, c.page, c.heads, c.d, c.format);
+    TSP_REQUIRE(dtype == TSP_F16 || dtype == TSP_BF16, dtype == TSP_F32 ? TSP_ERR_UNSUPPORTED : TSP_ERR_INVALID,
+                "tsp_attention_cached: heads must be f16 or bf16");
+    TSP_REQUIRE(c.format == TSP_KV_MX4 || c.format == dtype, TSP_ERR_UNSUPPORTED, "tsp_attention_cached: a 16-bit cache has the heads' dtype");
+    TSP_REQUIRE(nq >= 0 && nq < (1ll << 31), TSP_ERR_INVALID, "tsp_attention_cached: nq=%lld out of range", (long long)nq);
+    TSP_REQUIRE(hq > 0 && hq % c.heads == 0 && hq <= 4096, TSP_ERR_INVALID, "tsp_attention_cached: %d heads on %d", hq, c.heads);
+    TSP_REQUIRE(samples > 0 && (samples == 1 || d_offsets), TSP_ERR_INVALID, "tsp_attention_cached: samples=%d (without offsets: 1)", samples);
+    TSP_REQUIRE(max_pages > 0 && (int64_t)max_pages * c.page < (1ll << 31) - (1ll << 16), TSP_ERR_INVALID, "tsp_attention_cached: max_pages=%d", max_pages);
+    TSP_REQUIRE(std::isfinite(scale * kLog2e) && scale > 0.f, TSP_ERR_INVALID, "tsp_attention_cached: scale=%g", scale);
+    if (nq == 0) return TSP_OK;
+    TSP_REQUIRE(q && out && q->data && out->data && d_table && d_lengths && (c.data || c.pages == 0), TSP_ERR_INVALID,
+                "tsp_attention_cached: null pointer");
+    TSP_REQUIRE(heads_aligned(*q) && heads_aligned(*out) && reinterpret_cast<uintptr_t>(c.data) % 16 == 0, TSP_ERR_INVALID,
+                "tsp_attention_cached: data must be 16-byte aligned, strides multiples of 8 (a row's up to 2^20)");
+    TSP_REQUIRE(heads_apart(*out, nq, hq, c.d), TSP_ERR_INVALID, "tsp_attention_cached: the output's heads overlap");
+    const size_t span = (size_t)((nq - 1) * out->row_stride + (hq - 1) * out->head_stride + c.d) * 2;
+    TSP_REQUIRE(out->data != q->data && !overlap(c.data, (size_t)(kv_head_bytes(c) * c.heads) * c.pages, out->data, span), TSP_ERR_INVALID,
+                "tsp_attention_cached: out must not alias q or the cache");
+    const int share = hq / c.heads;
+    TSP_REQUIRE(nq * share < (1ll << 31) - 1024, TSP_ERR_INVALID, "tsp_attention_cached: too many rows");
+    const CachedCut cut = cached_cut(nq, samples, c.heads, share);
+    const size_t need = cached_workspace(cut, c.d);
+    TSP_REQUIRE(d_workspace, TSP_ERR_INVALID, "tsp_attention_cached: null workspace");
+    TSP_REQUIRE(workspace_bytes >= need, TSP_ERR_WORKSPACE, "tsp_attention_cached: workspace of %zu bytes, needs %zu", workspace_bytes, need);
+    TSP_REQUIRE(reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0, TSP_ERR_INVALID, "tsp_attention_cached: workspace not 16-byte aligned");
+    float* part = static_cast<float*>(d_workspace);
+    const CachedArgs a{q->data, out->data, q->row_stride, q->head_stride, out->row_stride, out->head_stride, kv_args(c, d_table, max_pages, d_lengths),
+                       d_offsets, nq, samples, share, causal ? 1 : 0, cut.groups, CF_NW, fast_div((uint32_t)share), scale * kLog2e, part,
+                       reinterpret_cast<float2*>(part + (size_t)cut.groups * 2 * cut.rows * c.d)};
+    hipStream_t s = as_stream(stream);
+    auto go = [&](auto bf, auto nb, auto mx) {
+        constexpr bool BF16 = decltype(bf)::value;
+        hipLaunchKernelGGL((k_cached_few<BF16, decltype(nb)::value, decltype(mx)::value, 1>), dim3((unsigned)cut.groups), dim3(CF_NW * 64), 0, s, a);
+    };
+    auto by_width = [&](auto bf, auto mx) {
+        if (c.d <= 32) go(bf, std::integral_constant<int, 1>{}, mx);
+        else if (c.d <= 64) go(bf, std::integral_constant<int, 2>{}, mx);
+        else if (c.d <= 96) go(bf, std::integral_constant<int, 3>{}, mx);
+        else go(bf, std::integral_constant<int, 4>{}, mx);
+    };
+    auto by_type = [&](auto bf) {
+        if (c.format == TSP_KV_MX4) by_width(bf, std::true_type{});
+        else by_width(bf, std::false_type{});
+        constexpr bool BF16 = decltype(bf)::value;
+        hipLaunchKernelGGL((k_cached_join<BF16, 16, CF_KEYS>), dim3((unsigned)cut.groups - 1), dim3(256), 0, s, a);
+    };
+    if (dtype == TSP_BF16) by_type(std::true_type{});
+    else by_type(std::false_type{});
+    TSP_CHECK_LAUNCH();
+    return TSP_OK;
+}

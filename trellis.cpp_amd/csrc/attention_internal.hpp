@@ -1,4 +1,5 @@
-// What the 16-bit and the fp32 attention kernels share: the call's arguments, how a workgroup finds its rows.
+// What the attention kernels share: the call's arguments, how a workgroup finds its rows, the 16-bit products'
+// operands.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -114,6 +115,63 @@ __device__ __forceinline__ AttnItem attn_item(const Args& a, int w) {
     t.row0 = (a.causal ? t.u.count - 1 - unit : unit) * ROWS;
     t.rows = t.u.rows * a.share;
     return t;
+}
+
+template <bool BF16>
+__device__ __forceinline__ f32x16_t mfma32(const u32x4_t& a, const u32x4_t& b, const f32x16_t& c) {
+    if constexpr (BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// Two values rounded to nearest even into a packed pair.
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    if constexpr (BF16) return f32x2_to_bf16x2_bits(lo, hi);
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{lo, hi}, f16x2_t));
+}
+
+// The sum of a packed pair and c, in fp32.
+template <bool BF16>
+__device__ __forceinline__ float add2(uint32_t p, float c) {
+    if constexpr (BF16) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, p), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), c, false);
+    else return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, p), __builtin_bit_cast(f16x2_t, 0x3c003c00u), c, false);
+}
+
+template <bool BF16>
+__device__ __forceinline__ bool nonfinite16(uint32_t b) {
+    constexpr uint32_t kExp = BF16 ? 0x7F80u : 0x7C00u;
+    return (b & kExp) == kExp;
+}
+
+// Byte offsets in a staged tile of AT_KEYS rows of DP values, as 16-byte pieces. K is read 16 bytes of
+// one d at 32 consecutive keys: the piece is xored with the key, so that 16 keys cover all banks. V is
+// read 64 bytes of 4 consecutive keys: the 64-byte quarter is xored with the key. (Rows of 32 and 96 values
+// begin in another quarter of the banks each by themselves.)
+template <int DP>
+__device__ __forceinline__ int k_piece(int key, int piece) {
+    return key * (DP * 2) + (piece ^ (DP == 128 ? key & 15 : DP == 96 || DP == 32 ? (key >> 2) & 3 : (key >> 1) & 7)) * 16;
+}
+template <int DP>
+__device__ __forceinline__ int v_piece(int key, int piece) {
+    return key * (DP * 2) + (piece ^ (DP == 128 ? (key & 3) << 2 : DP == 96 || DP == 32 ? 0 : ((key >> 1) & 1) << 2)) * 16;
+}
+
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4_ptr;
+
+// V^T operand (32 d x 16 keys) of keys 16 ks + {4h..4h+3, 8+4h..8+4h+3}: each of the two transposing
+// loads takes 4 keys x 16 d a group of 16 lanes.
+template <int DP>
+__device__ __forceinline__ u32x4_t v_operand(const char* sv, int ks, int db, int lane) {
+    const int key = ks * 16 + 4 * (lane >> 5) + ((lane >> 2) & 3);
+    const int piece = db * 4 + ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1), sub = (lane & 1) * 8;
+    const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(sv + v_piece<DP>(key, piece) + sub));
+    const s16x4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(sv + v_piece<DP>(key + 8, piece) + sub));
+    const uint2 ua = __builtin_bit_cast(uint2, a), ub = __builtin_bit_cast(uint2, b);
+    return u32x4_t{ua.x, ua.y, ub.x, ub.y};
 }
 
 // The value of the other lane half (lane ^ 32), for both halves: {lower half's, upper half's}.

@@ -1,0 +1,257 @@
+// Root-mean-square norm of rows with the residual's addition before it and, where asked, an 8-bit output:
+//   h = x + residual,  y = h / sqrt(mean(h^2) + eps) * gamma,  residual_out = h
+// in fp32; the norm is of the sum before residual_out rounds it. In 8 bits y leaves as e4m3 codes and a power of two
+// for every 32 channels (mx.hpp), the operands of tsp_linear_mx. tsp_mx_quantize rounds rows without a norm.
+//
+// Bound by memory: one read, one write. A wave holds a row of up to 2,048 channels in registers, eight consecutive
+// ones a lane and piece, four waves one of up to 8,192; gamma stays in registers while the wave goes over its
+// rows. Four neighbouring lanes hold a block of 32, so that its largest value is two lane moves. Other rows (not of
+// whole 16-byte pieces, or longer) are read twice, value by value, by a workgroup each.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "common.hpp"
+#include "mx.hpp"
+
+namespace tsp {
+namespace {
+
+constexpr int RN_NT = 256;
+constexpr int RN_NONE = -1;      // no residual
+
+struct RmsArgs {
+    const void *x, *residual;
+    const float* gamma;
+    void *out, *residual_out;
+    uint8_t* powers;
+    int64_t n;
+    int c, out_dtype;
+    float eps, inv_c;
+};
+
+template <int DT>
+__device__ __forceinline__ void store_if(void* p, int64_t i, const float (&v)[8]) {
+    if constexpr (DT != RN_NONE) store8<DT>(p, i, v);
+}
+
+// A row by NW waves (1: four rows a workgroup), CHUNKS pieces of 8 channels a lane.
+template <int XDT, int RDT, int NW, int CHUNKS>
+__global__ __launch_bounds__(RN_NT) void k_rms_norm(RmsArgs a) {
+    __shared__ float sum_of[2][4];
+    const int lane = threadIdx.x % (NW * 64), wave = threadIdx.x / 64, pieces = a.c / 8;
+    float gamma[CHUNKS][8];
+#pragma unroll
+    for (int k = 0; k < CHUNKS; ++k) {
+        const int piece = k * NW * 64 + lane;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) gamma[k][e] = 1.f;
+        if (a.gamma && piece < pieces) load8<TSP_F32>(a.gamma, piece * 8, gamma[k]);
+    }
+    int turn = 0;
+    // (with NW = 4 the whole workgroup has one row, and leaves together)
+    for (int64_t row = NW == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x; row < a.n; row += (int64_t)gridDim.x * (NW == 1 ? 4 : 1), turn ^= 1) {
+        const int64_t base = row * a.c;
+        float h[CHUNKS][8], q = 0.f;
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+            const int piece = k * NW * 64 + lane;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[k][e] = 0.f;
+            if (piece < pieces) {
+                load8<XDT>(a.x, base + piece * 8, h[k]);
+                if constexpr (RDT != RN_NONE) {
+                    float r[8];
+                    load8<RDT>(a.residual, base + piece * 8, r);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) h[k][e] += r[e];
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q += h[k][e] * h[k][e];
+        }
+        q = group_sum<64>(q);
+        if constexpr (NW > 1) {     // (two places taken in turn: one barrier a row)
+            if ((threadIdx.x & 63) == 0) sum_of[turn][wave] = q;
+            __syncthreads();
+            q = (sum_of[turn][0] + sum_of[turn][1]) + (sum_of[turn][2] + sum_of[turn][3]);
+        }
+        const float scale = __builtin_amdgcn_rsqf(fmaf(q, a.inv_c, a.eps));
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+            const int piece = k * NW * 64 + lane;
+            if (piece >= pieces) break;      // (whole quads of lanes, where blocks of 32 are asked for)
+            const int64_t at = base + piece * 8;
+            if constexpr (RDT != RN_NONE) {
+                if (a.residual_out) store_if<RDT>(a.residual_out, at, h[k]);
+            }
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = h[k][e] * scale * gamma[k][e];
+            if (a.out_dtype == TSP_MX8) {
+                const uint32_t power = mx_power_of<MX_E4M3>(y);
+                *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.out) + at) = mx_codes8(y, power);
+                if ((lane & 3) == 0) a.powers[at / MX_BLOCK] = (uint8_t)power;
+            } else if (a.out_dtype == TSP_BF16) {
+                store8<TSP_BF16>(a.out, at, y);
+            } else if (a.out_dtype == TSP_F16) {
+                store8<TSP_F16>(a.out, at, y);
+            } else {
+                store8<TSP_F32>(a.out, at, y);
+            }
+        }
+    }
+}
+
+// Any row, value by value; a block of 32 channels is 32 neighbouring threads'.
+__device__ __forceinline__ float load1(const void* p, int dt, int64_t i) {
+    return dt == TSP_F32 ? static_cast<const float*>(p)[i]
+           : dt == TSP_BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]) : f16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
+}
+__device__ __forceinline__ void store1(void* p, int dt, int64_t i, float v) {
+    if (dt == TSP_F32) static_cast<float*>(p)[i] = v;
+    else static_cast<uint16_t*>(p)[i] = dt == TSP_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
+}
+__device__ __forceinline__ void store_mx8(void* codes, uint8_t* powers, int64_t i, float v) {
+    uint32_t m = abs_bits(v);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 32));
+    const uint32_t power = mx_power<MX_E4M3>(m);
+    s16x2_t c{0, 0};
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, v, 0.f, mx_scale(power), false);
+    static_cast<uint8_t*>(codes)[i] = (uint8_t)__builtin_bit_cast(uint32_t, c);
+    if ((threadIdx.x & 31) == 0) powers[i / MX_BLOCK] = (uint8_t)power;
+}
+__global__ __launch_bounds__(RN_NT) void k_rms_norm_any(RmsArgs a, int x_dtype, int residual_dtype) {
+    __shared__ float sum_of[RN_NT / 64];
+    for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
+        const int64_t base = row * a.c;
+        float q = 0.f;
+        for (int i = threadIdx.x; i < a.c; i += RN_NT) {
+            float h = load1(a.x, x_dtype, base + i);
+            if (a.residual) h += load1(a.residual, residual_dtype, base + i);
+            q += h * h;
+        }
+        q = group_sum<64>(q);
+        if ((threadIdx.x & 63) == 0) sum_of[threadIdx.x / 64] = q;
+        __syncthreads();
+        q = (sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3]);
+        __syncthreads();
+        const float scale = __builtin_amdgcn_rsqf(fmaf(q, a.inv_c, a.eps));
+        for (int i = threadIdx.x; i < a.c; i += RN_NT) {
+            float h = load1(a.x, x_dtype, base + i);
+            if (a.residual) h += load1(a.residual, residual_dtype, base + i);
+            if (a.residual_out) store1(a.residual_out, residual_dtype, base + i, h);
+            const float y = h * scale * (a.gamma ? a.gamma[i] : 1.f);
+            if (a.out_dtype == TSP_MX8) store_mx8(a.out, a.powers, base + i, y);
+            else store1(a.out, a.out_dtype, base + i, y);
+        }
+    }
+}
+
+// Rows' values as they follow each other in memory; a block of 32 never spans two rows.
+template <int XDT>
+__global__ __launch_bounds__(RN_NT) void k_mx_quantize(const void* x, int64_t pieces, uint8_t* codes, uint8_t* powers) {
+    for (int64_t p = (int64_t)blockIdx.x * RN_NT + threadIdx.x; p < pieces; p += (int64_t)gridDim.x * RN_NT) {
+        float v[8];
+        load8<XDT>(x, p * 8, v);
+        const uint32_t power = mx_power_of<MX_E4M3>(v);
+        *reinterpret_cast<uint2*>(codes + p * 8) = mx_codes8(v, power);
+        if ((threadIdx.x & 3) == 0) powers[p / 4] = (uint8_t)power;
+    }
+}
+
+template <class F>
+void dt_switch(int dt, F&& f) {
+    switch (dt) {
+        case TSP_F32: f(std::integral_constant<int, TSP_F32>{}); break;
+        case TSP_F16: f(std::integral_constant<int, TSP_F16>{}); break;
+        default: f(std::integral_constant<int, TSP_BF16>{}); break;
+    }
+}
+
+}  // namespace
+}  // namespace tsp
+
+using namespace tsp;
+
+extern "C" int tsp_rms_norm(const void* d_x, int x_dtype, int64_t n, int c, const void* d_residual, int residual_dtype,
+                            const float* d_gamma, float eps, void* d_out, int out_dtype, uint8_t* d_powers, void* d_residual_out,
+                            void* stream) {
+    clear_error();
+    TSP_REQUIRE(n >= 0 && n < (1ll << 31) && c > 0 && c <= (1 << 20), TSP_ERR_INVALID, "tsp_rms_norm: n=%lld c=%d out of range", (long long)n, c);
+    TSP_REQUIRE(dtype_valid(x_dtype) && (dtype_valid(out_dtype) || out_dtype == TSP_MX8) && (!d_residual || dtype_valid(residual_dtype)),
+                TSP_ERR_INVALID, "tsp_rms_norm: bad dtype");
+    TSP_REQUIRE(eps >= 0.f && std::isfinite(eps), TSP_ERR_INVALID, "tsp_rms_norm: eps=%g", eps);
+    TSP_REQUIRE(out_dtype != TSP_MX8 || c % MX_BLOCK == 0, TSP_ERR_UNSUPPORTED, "tsp_rms_norm: 8-bit rows of %d channels (need a multiple of %d)",
+                c, MX_BLOCK);
+    TSP_REQUIRE(d_residual || !d_residual_out, TSP_ERR_INVALID, "tsp_rms_norm: residual_out without a residual");
+    if (n == 0) return TSP_OK;
+    TSP_REQUIRE(d_x && d_out && (out_dtype != TSP_MX8 || d_powers), TSP_ERR_INVALID, "tsp_rms_norm: null pointer");
+    const size_t elems = (size_t)n * c;
+    auto bytes = [&](int dt) { return dt == TSP_MX8 ? elems : elems * dtype_size(dt); };
+    // a value is read by the thread that writes it, and before: an output may be an input where both are the same values
+    struct Part { const void* p; size_t bytes; int dt; };
+    const Part in[2] = {{d_x, bytes(x_dtype), x_dtype}, {d_residual, d_residual ? bytes(residual_dtype) : 0, residual_dtype}};
+    const Part out[3] = {{d_out, bytes(out_dtype), out_dtype},
+                         {d_residual_out, d_residual_out ? bytes(residual_dtype) : 0, residual_dtype},
+                         {out_dtype == TSP_MX8 ? d_powers : nullptr, elems / MX_BLOCK, -1}};
+    for (const Part& o : out)
+        for (const Part& i : in)
+            TSP_REQUIRE(!overlap(o.p, o.bytes, i.p, i.bytes) || (o.p == i.p && o.dt == i.dt), TSP_ERR_INVALID,
+                        "tsp_rms_norm: an output overlaps an input (it may be one of the same dtype, or apart)");
+    TSP_REQUIRE(!overlap(out[0].p, out[0].bytes, out[1].p, out[1].bytes) && !overlap(out[0].p, out[0].bytes, out[2].p, out[2].bytes) &&
+                    !overlap(out[1].p, out[1].bytes, out[2].p, out[2].bytes) &&
+                    !(d_gamma && (overlap(out[0].p, out[0].bytes, d_gamma, (size_t)c * 4) || overlap(out[1].p, out[1].bytes, d_gamma, (size_t)c * 4) ||
+                                  overlap(out[2].p, out[2].bytes, d_gamma, (size_t)c * 4))),
+                TSP_ERR_INVALID, "tsp_rms_norm: the outputs overlap each other or gamma");
+    const RmsArgs a{d_x, d_residual, d_gamma, d_out, d_residual_out, d_powers, n, c, out_dtype, eps, 1.f / (float)c};
+    auto off16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; };
+    hipStream_t s = as_stream(stream);
+    const dim3 block(RN_NT);
+    if (c % 8 || c > 8192 || off16(d_x) || off16(d_residual) || off16(d_gamma) || off16(d_out) || off16(d_residual_out)) {
+        hipLaunchKernelGGL(k_rms_norm_any, dim3((unsigned)std::min<int64_t>(n, 16384)), block, 0, s, a, x_dtype, residual_dtype);
+        TSP_CHECK_LAUNCH();
+        return TSP_OK;
+    }
+    dt_switch(x_dtype, [&](auto xd) {
+        auto go = [&](auto rd) {
+            constexpr int XD = decltype(xd)::value, RD = decltype(rd)::value;
+            const dim3 by_wave((unsigned)std::min<int64_t>(ceil_div(n, 4), 2048)), by_group((unsigned)std::min<int64_t>(n, 4096));
+            if (c <= 512) hipLaunchKernelGGL((k_rms_norm<XD, RD, 1, 1>), by_wave, block, 0, s, a);
+            else if (c <= 1024) hipLaunchKernelGGL((k_rms_norm<XD, RD, 1, 2>), by_wave, block, 0, s, a);
+            else if (c <= 2048) hipLaunchKernelGGL((k_rms_norm<XD, RD, 1, 4>), by_wave, block, 0, s, a);
+            else if (c <= 4096) hipLaunchKernelGGL((k_rms_norm<XD, RD, 4, 2>), by_group, block, 0, s, a);
+            else hipLaunchKernelGGL((k_rms_norm<XD, RD, 4, 4>), by_group, block, 0, s, a);
+        };
+        if (d_residual) dt_switch(residual_dtype, go);
+        else go(std::integral_constant<int, RN_NONE>{});
+    });
+    TSP_CHECK_LAUNCH();
+    return TSP_OK;
+}
+
+extern "C" int tsp_mx_quantize(const void* d_x, int x_dtype, int64_t n, int c, void* d_codes, uint8_t* d_powers, void* stream) {
+    clear_error();
+    TSP_REQUIRE(n >= 0 && n < (1ll << 31) && c > 0 && c <= (1 << 20), TSP_ERR_INVALID, "tsp_mx_quantize: n=%lld c=%d out of range", (long long)n, c);
+    TSP_REQUIRE(dtype_valid(x_dtype), TSP_ERR_INVALID, "tsp_mx_quantize: bad dtype");
+    TSP_REQUIRE(c % MX_BLOCK == 0, TSP_ERR_UNSUPPORTED, "tsp_mx_quantize: rows of %d channels (need a multiple of %d)", c, MX_BLOCK);
+    if (n == 0) return TSP_OK;
+    TSP_REQUIRE(d_x && d_codes && d_powers, TSP_ERR_INVALID, "tsp_mx_quantize: null pointer");
+    TSP_REQUIRE(reinterpret_cast<uintptr_t>(d_x) % 16 == 0 && reinterpret_cast<uintptr_t>(d_codes) % 16 == 0, TSP_ERR_INVALID,
+                "tsp_mx_quantize: x and codes must be 16-byte aligned");
+    const size_t elems = (size_t)n * c;
+    TSP_REQUIRE(!overlap(d_x, elems * dtype_size(x_dtype), d_codes, elems) && !overlap(d_x, elems * dtype_size(x_dtype), d_powers, elems / MX_BLOCK) &&
+                    !overlap(d_codes, elems, d_powers, elems / MX_BLOCK),
+                TSP_ERR_INVALID, "tsp_mx_quantize: x, codes and powers must not overlap");
+    const int64_t pieces = (int64_t)(elems / 8);
+    dt_switch(x_dtype, [&](auto xd) {
+        hipLaunchKernelGGL((k_mx_quantize<decltype(xd)::value>), dim3((unsigned)std::min<int64_t>(ceil_div(pieces, RN_NT), 8192)), dim3(RN_NT), 0,
+                           as_stream(stream), d_x, pieces, static_cast<uint8_t*>(d_codes), d_powers);
+    });
+    TSP_CHECK_LAUNCH();
+    return TSP_OK;
+}
