@@ -15,8 +15,9 @@
 // a lane holds scores of one row and P is the second product's operand where it stands. Statistics and accumulators are
 // fp32; P is rounded to the heads' type, as the packed attention's (attention.hip) is, and formed as there.
 //
-// Waves of their own, each with every fourth tile of 32 keys: K goes from memory to its operand, V through a piece of LDS
-// that is the wave's alone, where it is turned.
+// Two kernels. Few rows (k_cached_few): waves of their own, each with every eighth tile of 32 keys: K goes from memory to its
+// operand, V through a piece of LDS that is the wave's alone, where it is turned. Many rows (k_cached_many): four waves of 32
+// rows share a tile of 64 keys, widened into LDS by all of them.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -28,7 +29,8 @@
 namespace tsp {
 namespace {
 
-constexpr int CF_KEYS = 32, CF_NW = 4;       // few rows: keys of a tile, waves
+constexpr int CF_KEYS = 32, CF_NW = 8;                               // few rows: keys of a tile, waves
+constexpr int CM_KEYS = 64, CM_NW = 4, CM_ROWS = CM_NW * 32;         // many
 
 struct CachedArgs {
     const void* q;
@@ -42,7 +44,13 @@ struct CachedArgs {
     FastDiv by_share;
     float scale2;                              // scale * log2(e)
     float* part;                               // [2 * groups][row][d] sums of p v, and
-    float2* stat;                              // [2 * groups][row] maximum and sum of p (-1: no key seen)
+    float2* stat;                              // [2 * groups][row] maximum and sum of p (-1: no key seen), and
+    struct JoinItem* join;                     // [groups] the unit that is cut at the workgroup's end and began in it
+};
+
+// rows left in the unit from its first (0: none), the first, the sample's first row, the key head, the last workgroup.
+struct JoinItem {
+    int rows, first_row, row0, head, last, pad[3];
 };
 
 __device__ __forceinline__ int64_t uniform(int64_t x) {
@@ -165,6 +173,12 @@ __device__ __forceinline__ CachedPiece cut_unit(const CachedUnit& u, int64_t fro
     p.slot = lo == 0 && hi == weight ? -1 : 2 * w + (lo == 0);
     return p;
 }
+// What the join has to know of a workgroup's last unit (one thread).
+__device__ __forceinline__ void tell_join(const CachedArgs& a, const CachedUnit& u, int64_t to, int64_t length, int64_t groups, int w, bool begins) {
+    JoinItem j{};
+    if (begins && u.end > to) j = JoinItem{u.lq * a.share - u.first_row, u.first_row, u.row0, u.head, (int)line_group(length, groups, u.end - 1), {}};
+    a.join[w] = j;
+}
 
 // Four bytes of codes as eight 16-bit values.
 template <bool BF16>
@@ -226,10 +240,11 @@ __global__ __launch_bounds__(CF_NW * 64) void k_cached_few(CachedArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
     char* sV = sBuf[wave];
     const KvArgs& kv = a.cache;
-    const int64_t length = line_length<ROWS, CF_KEYS>(a);
-    if (length == 0) return;
-    const int64_t groups = line_groups(a, length);
-    if ((int)blockIdx.x >= groups) return;
+    const int64_t length = line_length<ROWS, CF_KEYS>(a), groups = line_groups(a, length);
+    if (length == 0 || (int)blockIdx.x >= groups) {
+        if (threadIdx.x == 0) a.join[blockIdx.x].rows = 0;
+        return;
+    }
     const int64_t to = line_cut(length, groups, blockIdx.x + 1);
     const int page_mask = (1 << kv.page_bits) - 1;
     constexpr float LAG = BF16 ? 8.f : 4.f, LIFT = BF16 ? 0.f : 11.f;
@@ -237,6 +252,7 @@ __global__ __launch_bounds__(CF_NW * 64) void k_cached_few(CachedArgs a) {
     for (int64_t from = line_cut(length, groups, blockIdx.x); from < to;) {
         const CachedUnit u = find_unit<ROWS, CF_KEYS>(a, from);
         const CachedPiece piece = cut_unit(u, from, to, blockIdx.x);
+        if (threadIdx.x == 0 && u.end >= to) tell_join(a, u, to, length, groups, blockIdx.x, from <= u.begin);
         from = u.end;
         const int rows = u.lq * a.share;
         // rows past the sample's last are copies of it that are not stored
@@ -499,62 +515,465 @@ __global__ __launch_bounds__(CF_NW * 64) void k_cached_few(CachedArgs a) {
     }
 }
 
+// ---- many rows -----------------------------------------------------------------------------------------------------
+template <bool BF16, int NB, bool MX4>
+__global__ __launch_bounds__(CM_NW * 64, MX4 ? 2 : 1) void k_cached_many(CachedArgs a) {
+    constexpr int DP = NB * 32, KS = DP / 16, DB = NB, TILE = CM_KEYS * DP * 2, NT = CM_NW * 64;
+    constexpr int PIECES = MX4 ? NB : NB * 4;                              // 16-byte pieces of a key in the page
+    constexpr int LOADS = (CM_KEYS * PIECES + NT - 1) / NT;                // of them a thread, of K and of V
+    __shared__ __attribute__((aligned(16))) char sK0[TILE], sK1[TILE], sV0[TILE], sV1[TILE];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
+    const KvArgs& kv = a.cache;
+    const int64_t length = line_length<CM_ROWS, CM_KEYS>(a), groups = line_groups(a, length);
+    if (length == 0 || (int)blockIdx.x >= groups) {
+        if (threadIdx.x == 0) a.join[blockIdx.x].rows = 0;
+        return;
+    }
+    const int64_t to = line_cut(length, groups, blockIdx.x + 1);
+    const int page_mask = (1 << kv.page_bits) - 1;
+    constexpr float LAG = BF16 ? 8.f : 4.f, LIFT = BF16 ? 0.f : 11.f, FAR = 1024.f;
+    const float scale2 = a.scale2;
+
+    for (int64_t from = line_cut(length, groups, blockIdx.x); from < to;) {
+        const CachedUnit u = find_unit<CM_ROWS, CM_KEYS>(a, from);
+        const CachedPiece piece = cut_unit(u, from, to, blockIdx.x);
+        if (threadIdx.x == 0 && u.end >= to) tell_join(a, u, to, length, groups, blockIdx.x, from <= u.begin);
+        from = u.end;
+        const int rows = u.lq * a.share;
+        // rows past the sample's last are copies of it that are not stored
+        auto query = [&](int r) __attribute__((always_inline)) { return min(r, rows - 1) / a.by_share; };
+        auto limit = [&](int r) __attribute__((always_inline)) { return cached_limit(a.causal, u.lq, u.lk, query(r)); };
+        const int r = u.first_row + wave * 32 + r32, lim = limit(r), wave_end = limit(u.first_row + wave * 32 + 31);
+        const int t0 = piece.t0, t1 = piece.t1;
+        // Q^T operand: d = 16 ks + 8 h .. + 7 of the lane's row
+        u32x4_t qf[KS];
+        {
+            const int qi = query(r), hq = u.head * a.share + min(r, rows - 1) - qi * a.share;
+            const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (int64_t)(u.row0 + qi) * a.q_row + hq * a.q_head;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                qf[ks] = ks * 16 + h * 8 < kv.d ? *reinterpret_cast<const u32x4_t*>(qp + ks * 16 + h * 8) : u32x4_t{0, 0, 0, 0};
+        }
+        // Whether all of the piece's pages are the pool's (else every tile is looked at key by key).
+        bool sound = true;
+        const int32_t* pages = kv.table + (int64_t)u.sample * kv.max_pages;
+        const int end_key = min(t1 * CM_KEYS, u.lk);
+        for (int p = ((t0 * CM_KEYS) >> kv.page_bits) + threadIdx.x; (int64_t)p << kv.page_bits < end_key; p += NT) sound &= (unsigned)pages[p] < (unsigned)kv.pages;
+        sound = __syncthreads_and(sound);
+
+        // A thread's pieces of a tile: 16 bytes at keys idx / PIECES. Keys past the sample's last, and those of no page, are zeros.
+        struct Raw {
+            u32x4_t x[LOADS];
+            uint32_t p[MX4 ? LOADS : 1];
+        };
+        auto load = [&](int tile, int side, Raw& w) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int idx = i * NT + threadIdx.x, in = idx / PIECES, p = idx % PIECES, key = tile * CM_KEYS + in;
+                w.x[i] = u32x4_t{0, 0, 0, 0};
+                if constexpr (MX4) w.p[i] = 0;
+                if (in >= CM_KEYS || key >= u.lk || tile >= t1 || (!MX4 && p * 8 >= kv.d)) continue;
+                const int page = pages[key >> kv.page_bits], slot = key & page_mask;
+                if ((unsigned)page >= (unsigned)kv.pages) continue;
+                const uint8_t* head = kv.data + page * kv.page_bytes + u.head * kv.head_bytes;
+                if constexpr (MX4) {
+                    w.x[i] = *reinterpret_cast<const u32x4_t*>(head + kv_codes_at(kv, side, slot) + p * 16);
+                    w.p[i] = head[kv_powers_at(kv, side, slot) + p];
+                } else {
+                    w.x[i] = *reinterpret_cast<const u32x4_t*>(head + ((int64_t)((side << kv.page_bits) + slot) * kv.d + p * 8) * 2);
+                }
+            }
+        };
+        auto put = [&](const Raw& w, int side, char* s) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int idx = i * NT + threadIdx.x, key = idx / PIECES, p = idx % PIECES;
+                if (CM_KEYS * PIECES % NT && key >= CM_KEYS) continue;
+                if constexpr (MX4) {
+                    const float scale = mx_scale(w.p[i]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        *reinterpret_cast<u32x4_t*>(s + (side ? cv_piece<DP>(key, p * 4 + j) : k_piece<DP>(key, p * 4 + j))) = widen4<BF16>(w.x[i][j], scale);
+                } else {
+                    *reinterpret_cast<u32x4_t*>(s + (side ? cv_piece<DP>(key, p) : k_piece<DP>(key, p))) = w.x[i];
+                }
+            }
+        };
+        f32x16_t o[DB];
+#pragma unroll
+        for (int db = 0; db < DB; ++db) o[db] = f32x16_t{};
+        float m = -INFINITY, l = 0.f, mc = -LIFT;      // maximum, sum, what the exponents are less by
+        bool far = false, seen = false;
+
+        // scores: s[kb][i] is key kb * 32 + 8 (i / 4) + 4 h + i % 4 of the tile
+        auto k_operand = [&](const char* sK, int t) __attribute__((always_inline)) {
+            return *reinterpret_cast<const u32x4_t*>(sK + k_piece<DP>((t & 1) * 32 + r32, (t >> 1) * 2 + h));
+        };
+        auto scores = [&](const char* sK, f32x16_t (&s)[2]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < 2 * KS; ++t) s[t & 1] = mfma32<BF16>(k_operand(sK, t), qf[t >> 1], t < 2 ? f32x16_t{} : s[t & 1]);
+        };
+        // (raise, near_top: as in the packed attention)
+        auto raise = [&](float mt) __attribute__((always_inline)) {
+            const float2 mh = both_halves(mt);
+            mt = fmaxf(mh.x, mh.y);
+            if (__any((mt - m) * scale2 > LAG)) {
+                const float mn = fmaxf(m, mt);
+                const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * scale2);
+                m = mn;
+                far = __any(fabsf(mn) * scale2 > FAR && mn != -INFINITY);
+                mc = (far || mn == -INFINITY ? 0.f : mn * scale2) - LIFT;
+                l *= corr;
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[db][i] *= corr;
+            }
+        };
+        auto near_top = [&](f32x16_t (&s)[2]) __attribute__((always_inline)) {
+            if (__builtin_expect(!far, 1)) return;
+            const float top = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[kb][i] -= top;
+        };
+        auto top_of = [&](const f32x16_t (&s)[2]) __attribute__((always_inline)) {
+            float mt = s[0][0];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[kb][i]);
+            return mt;
+        };
+        auto exponents = [&](f32x16_t (&s)[2], u32x4_t (&pf)[4]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], scale2, -mc));
+            float sum = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    pf[ks][e] = pack2<BF16>(s[ks / 2][8 * (ks % 2) + 2 * e], s[ks / 2][8 * (ks % 2) + 2 * e + 1]);
+                    sum = add2<BF16>(pf[ks][e], sum);
+                }
+            l += sum;
+        };
+        // V^T operand, as v_operand with this kernel's places
+        auto values = [&](const char* sV, int ks, int db) __attribute__((always_inline)) {
+            const int key = ks * 16 + 4 * h + ((lane >> 2) & 3), p = db * 4 + ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1), sub = (lane & 1) * 8;
+            const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(sV + cv_piece<DP>(key, p) + sub));
+            const s16x4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(sV + cv_piece<DP>(key + 8, p) + sub));
+            const uint2 ux = __builtin_bit_cast(uint2, x), uy = __builtin_bit_cast(uint2, y);
+            return u32x4_t{ux.x, ux.y, uy.x, uy.y};
+        };
+        // A tile that not every row of the workgroup sees whole.
+        auto attend_masked = [&](int base, const char* sK, const char* sV) __attribute__((always_inline)) {
+            f32x16_t s[2];
+            u32x4_t pf[4];
+            scores(sK, s);
+            int held = 15;      // a bit for 16 keys
+            if (!sound) {
+                held = 0;
+                for (int k = 0; k < 4; ++k) {
+                    const int key = base + k * 16;
+                    if (key < u.lk && (unsigned)pages[key >> kv.page_bits] < (unsigned)kv.pages) held |= 1 << k;
+                }
+            }
+            const int left = lim - base - 4 * h;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const bool sees = kb * 32 + 8 * (i / 4) + i % 4 < left && (held >> (kb * 2 + i / 8) & 1);
+                    seen |= sees;
+                    s[kb][i] = sees ? s[kb][i] : -INFINITY;
+                }
+            raise(top_of(s));
+            near_top(s);
+            exponents(s, pf);
+            // A probability of zero must not meet an Inf or a NaN of a key that its row does not see. Zero times V
+            // shows whether there is one.
+            bool odd = false;
+            if (a.causal) {
+                f32x16_t z = f32x16_t{};
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) z = mfma32<BF16>(values(sV, ks, db), u32x4_t{0, 0, 0, 0}, z);
+                float t = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) t += z[i];
+                odd = __any(t != t);
+            }
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                for (int db = 0; db < DB; ++db) {
+                    u32x4_t vf = values(sV, ks, db);
+                    if (odd) vf = finite_only<BF16>(vf);
+                    o[db] = mfma32<BF16>(vf, pf[ks], o[db]);
+                }
+            if (odd) {      // the values left out, key by key, for the rows that see them
+                for (int key = 0; key < CM_KEYS; ++key) {
+                    float p = 0.f;
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if ((kb * 32 + 8 * (i / 4) + i % 4) == (key & ~4)) p = s[kb][i];
+                    const float2 ph = both_halves(p);
+                    p = key & 4 ? ph.y : ph.x;
+                    const bool sees = base + key < lim;      // (a key of no page is zeros)
+#pragma unroll
+                    for (int db = 0; db < DB; ++db)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int e = db * 32 + 8 * (i / 4) + 4 * h + i % 4;
+                            const uint32_t b = *reinterpret_cast<const uint16_t*>(sV + cv_piece<DP>(key, e >> 3) + (e & 7) * 2);
+                            if (sees && nonfinite16<BF16>(b)) o[db][i] += p * value16<BF16>(b);
+                        }
+                }
+            }
+        };
+        // Whole tiles: the scores of the next tile are formed while the exponents of this one are, and its maximum while this one's
+        // values are weighed; operands are read four products ahead. Two buffers each for K and V, K a tile ahead of V; in
+        // registers both a tile further.
+        const int all_see = sound ? limit(u.first_row) / CM_KEYS : 0;      // tiles that every row sees whole
+        const int whole = min(t1, all_see);
+        Raw wk, wv;
+        auto step = [&](int tile, char* k_this, const char* k_next, const char* v_this, char* v_next, f32x16_t (&s)[2],
+                        f32x16_t (&sn)[2]) __attribute__((always_inline)) {
+            constexpr int AHEAD = 4, NK = 2 * KS, NV = 4 * DB;
+            u32x4_t pf[4], ring[AHEAD];
+            float sum = 0.f;
+            __syncthreads();
+            put(wk, 0, k_this);
+            put(wv, 1, v_next);
+            load(tile + 3, 0, wk);
+            load(tile + 2, 1, wv);
+#pragma unroll
+            for (int t = 0; t < AHEAD; ++t) ring[t] = k_operand(k_next, t);
+#pragma unroll
+            for (int t = 0; t < NK; ++t) {
+                sn[t & 1] = mfma32<BF16>(ring[t % AHEAD], qf[t >> 1], t < 2 ? f32x16_t{} : sn[t & 1]);
+                if (t + AHEAD < NK) ring[t % AHEAD] = k_operand(k_next, t + AHEAD);
+                else ring[t % AHEAD] = values(v_this, (t + AHEAD - NK) / DB, (t + AHEAD - NK) % DB);
+#pragma unroll
+                for (int e = t * 16 / NK; e < (t + 1) * 16 / NK; ++e) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[e / 8][2 * (e % 8)], scale2, -mc));
+                    const float y = __builtin_amdgcn_exp2f(fmaf(s[e / 8][2 * (e % 8) + 1], scale2, -mc));
+                    pf[e / 4][e % 4] = pack2<BF16>(x, y);
+                    sum = add2<BF16>(pf[e / 4][e % 4], sum);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            l += sum;
+            float mt = sn[0][0];
+#pragma unroll
+            for (int t = 0; t < NV; ++t) {
+                o[t % DB] = mfma32<BF16>(ring[t % AHEAD], pf[t / DB], o[t % DB]);
+                if (t + AHEAD < NV) ring[t % AHEAD] = values(v_this, (t + AHEAD) / DB, (t + AHEAD) % DB);
+#pragma unroll
+                for (int i = t * 32 / NV; i < (t + 1) * 32 / NV; ++i) mt = fmaxf(mt, sn[i / 16][i % 16]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            raise(mt);
+            near_top(sn);
+        };
+        // on the way: K of the first two tiles and V of the first in LDS, K of the third and V of the second in registers
+        if (t0 < t1) {
+            load(t0, 0, wk);
+            load(t0, 1, wv);
+            __syncthreads();        // (the last piece's rows have left LDS)
+            put(wk, 0, sK0);
+            put(wv, 1, sV0);
+            load(t0 + 1, 0, wk);
+            put(wk, 0, sK1);
+            load(t0 + 2, 0, wk);
+            load(t0 + 1, 1, wv);
+        }
+        int tile = t0;
+        bool second = false;
+        if (tile < whole) {
+            seen = true;
+            f32x16_t s0[2], s1[2];
+            __syncthreads();
+            scores(sK0, s0);
+            raise(top_of(s0));
+            near_top(s0);
+            for (; tile + 3 <= whole; tile += 2) {
+                step(tile, sK0, sK1, sV0, sV1, s0, s1);
+                step(tile + 1, sK1, sK0, sV1, sV0, s1, s0);
+            }
+            __syncthreads();
+            put(wk, 0, sK0);
+            put(wv, 1, sV1);
+            load(tile + 3, 0, wk);
+            load(tile + 2, 1, wv);
+            u32x4_t pf[4];
+            exponents(s0, pf);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                for (int db = 0; db < DB; ++db) o[db] = mfma32<BF16>(values(sV0, ks, db), pf[ks], o[db]);
+            ++tile;
+            second = true;
+        }
+        // the others, a whole one among them at times
+        for (; tile < t1; ++tile, second = !second) {
+            __syncthreads();
+            if (tile * CM_KEYS < wave_end) attend_masked(tile * CM_KEYS, second ? sK1 : sK0, second ? sV1 : sV0);
+            __syncthreads();
+            put(wk, 0, second ? sK1 : sK0);
+            put(wv, 1, second ? sV0 : sV1);
+            load(tile + 3, 0, wk);
+            load(tile + 2, 1, wv);
+        }
+
+        const float2 lh = both_halves(l);
+        const float sum = lh.x + lh.y;
+        const uint64_t some = __ballot(seen);
+        const bool any = (some >> r32 & 1) || (some >> (r32 + 32) & 1);
+        if (piece.slot >= 0) {
+            if (r < rows) {
+                const int64_t item = (int64_t)piece.slot * CM_ROWS + (r - u.first_row);
+                if (h == 0) a.stat[item] = float2{m, any ? sum : -1.f};
+                float* op = a.part + item * kv.d;
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int e = db * 32 + 8 * g + 4 * h;
+                        if (any && e < kv.d) *reinterpret_cast<f32x4_t*>(op + e) = f32x4_t{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+                    }
+            }
+            continue;
+        }
+        // Rows of out leave in 16-byte pieces, through the wave's piece of the K buffers.
+        constexpr int P = DP / 8;
+        const float inv = any ? 1.0f / sum : 0.f;
+        char* sO = (wave < CM_NW / 2 ? sK0 : sK1) + wave % (CM_NW / 2) * (32 * DP * 2);
+        __syncthreads();
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<uint2*>(sO + k_piece<DP>(r32, db * 4 + g) + h * 8) =
+                    any ? uint2{pack2<BF16>(o[db][4 * g] * inv, o[db][4 * g + 1] * inv), pack2<BF16>(o[db][4 * g + 2] * inv, o[db][4 * g + 3] * inv)} : uint2{0, 0};
+#pragma unroll
+        for (int i = 0; i < P / 2; ++i) {
+            const int row = (i * 64 + lane) / P, p = (i * 64 + lane) % P, rr = u.first_row + wave * 32 + row;
+            const u32x4_t x = *reinterpret_cast<const u32x4_t*>(sO + k_piece<DP>(row, p));
+            if (rr >= rows || p * 8 >= kv.d) continue;
+            const int qr = rr / a.by_share, hr = u.head * a.share + rr - qr * a.share;
+            *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.o) + (int64_t)(u.row0 + qr) * a.o_row + hr * a.o_head + p * 8) = x;
+        }
+    }
+}
+
 // ---- the pieces of units that were cut, joined -----------------------------------------------------------------------
-// sum_s w_s (p v)_s / sum_s w_s (sum p)_s, w_s = exp(max_s - max), in the pieces' order. The workgroups of a unit are
-// those of the first cut through it, 16 rows each, 16 lanes a row, eight channels a lane.
-template <bool BF16, int ROWS, int TILE>
+// sum_s w_s (p v)_s / sum_s w_s (sum p)_s, w_s = exp(max_s - max), in an order that the pieces' number alone sets. G groups of 16
+// lanes a row, eight channels a lane: 4 (a wave), or 16 where units have many pieces.
+template <bool BF16, int ROWS, int G>
 __global__ __launch_bounds__(256) void k_cached_join(CachedArgs a) {
-    const int64_t length = line_length<ROWS, TILE>(a);
-    if (length == 0) return;
-    const int64_t groups = line_groups(a, length), cut = (int64_t)blockIdx.x + 1;
-    if (cut >= groups) return;
-    const int64_t place = line_cut(length, groups, cut);
-    const CachedUnit u = find_unit<ROWS, TILE>(a, place);
-    if (u.begin == place) return;
-    const int64_t g0 = line_group(length, groups, u.begin), g1 = line_group(length, groups, u.end - 1);
-    if (g0 != cut - 1) return;
-    const int row = blockIdx.y * 16 + (threadIdx.x >> 4), e = (threadIdx.x & 15) * 8, r = u.first_row + row;
-    if (r >= u.lq * a.share || e >= a.cache.d) return;
-    auto at = [&](int64_t w) { return (2 * w + (w == g0)) * ROWS + row; };
+    constexpr int ITEMS = 16 / G, BATCH = 8;
+    __shared__ float sAcc[G == 16 ? 16 : 1][KV_MAX_D], sMax[4], sSum[4];
+    const JoinItem j = a.join[blockIdx.x];
+    const int group = threadIdx.x >> 4, g = group % G, e = (threadIdx.x & 15) * 8, mine = threadIdx.x % (G * 16);
+    const int row = blockIdx.y * ITEMS + group / G;
+    if ((int)(blockIdx.y * ITEMS) >= j.rows) return;
+    const bool live = row < j.rows;
+    const int g0 = blockIdx.x, pieces = j.last - g0 + 1;
+    auto at = [&](int i) { return (int64_t)(2 * (g0 + i) + (i == 0)) * ROWS + (live ? row : 0); };
     float top = -INFINITY;
-    for (int64_t w = g0; w <= g1; ++w) {
-        const float2 st = a.stat[at(w)];
+    for (int i = mine; i < pieces; i += G * 16) {
+        const float2 st = a.stat[at(i)];
         if (st.y != -1.f) top = fmaxf(top, st.x);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    if constexpr (G == 16) {
+        if ((threadIdx.x & 63) == 0) sMax[threadIdx.x >> 6] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(sMax[0], sMax[1]), fmaxf(sMax[2], sMax[3]));
     }
     float sum = 0.f, acc[8] = {};
     bool any = false;
-    for (int64_t w = g0; w <= g1; ++w) {
-        const float2 st = a.stat[at(w)];
-        if (st.y == -1.f) continue;
-        any = true;
-        const float c = st.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st.x - top) * a.scale2);
-        sum += c * st.y;
-        float x[8];
-        load8<TSP_F32>(a.part, at(w) * a.cache.d + e, x);
+    for (int i0 = g; i0 < pieces; i0 += BATCH * G) {
+        float c[BATCH], x[BATCH][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] += c * x[i];
+        for (int b = 0; b < BATCH; ++b) {
+            const int i = i0 + b * G;
+            c[b] = -1.f;
+            if (i >= pieces) continue;
+            const float2 st = a.stat[at(i)];
+            if (e < a.cache.d) load8<TSP_F32>(a.part, at(i) * a.cache.d + e, x[b]);
+            if (st.y == -1.f) continue;
+            any = true;
+            c[b] = st.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st.x - top) * a.scale2);
+            sum += c[b] * st.y;
+        }
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+            if (c[b] == -1.f) continue;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[k] += c[b] * x[b][k];
+        }
     }
-    const float inv = any ? 1.f / sum : 0.f;
+    // over the groups
+    int seen = any;
+    sum += __shfl_xor(sum, 16, 64), seen |= __shfl_xor(seen, 16, 64);
+    sum += __shfl_xor(sum, 32, 64), seen |= __shfl_xor(seen, 32, 64);
+    if constexpr (G == 16) {
+        if ((threadIdx.x & 63) == 0) sSum[threadIdx.x >> 6] = sum;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = any ? acc[i] * inv : 0.f;
-    const int qi = r / a.by_share, hq = u.head * a.share + r - qi * a.share;
-    store8<BF16 ? TSP_BF16 : TSP_F16>(a.o, (int64_t)(u.row0 + qi) * a.o_row + hq * a.o_head + e, acc);
+        for (int k = 0; k < 8; ++k) sAcc[g][e + k] = acc[k];
+        seen = __syncthreads_or(seen);
+        sum = (sSum[0] + sSum[1]) + (sSum[2] + sSum[3]);
+        if (g == 0) {
+#pragma unroll
+            for (int o = 1; o < 16; ++o)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) acc[k] += sAcc[o][e + k];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            acc[k] += __shfl_xor(acc[k], 16, 64);
+            acc[k] += __shfl_xor(acc[k], 32, 64);
+        }
+    }
+    if (!live || g != 0 || e >= a.cache.d) return;
+    const float inv = 1.f / sum;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[k] = seen ? acc[k] * inv : 0.f;
+    const int r = j.first_row + row, qi = r / a.by_share, hq = j.head * a.share + r - qi * a.share;
+    store8<BF16 ? TSP_BF16 : TSP_F16>(a.o, (int64_t)(j.row0 + qi) * a.o_row + hq * a.o_head + e, acc);
 }
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// How a call is cut: the rows of a unit, the workgroups.
+// How a call is cut: the rows of a unit, the workgroups. Few rows are those that fit a unit of 32 in the mean (the host
+// does not know the lengths).
 struct CachedCut {
-    int rows, groups;
+    int rows, groups, least;
+    bool many_pieces;      // of a unit
 };
 CachedCut cached_cut(int64_t nq, int samples, int hkv, int share) {
     CachedCut c;
-    c.rows = 16;
-    c.groups = 1024;
-    (void)nq, (void)samples, (void)hkv, (void)share;
+    const int64_t each = ceil_div(nq, samples) * share;
+    c.rows = each <= 16 ? 16 : each <= 32 ? 32 : CM_ROWS;
+    c.groups = 512;      // two a CU
+    c.least = c.rows == CM_ROWS ? 4 : CF_NW;
+    c.many_pieces = c.groups > 32 * ceil_div(nq * share, c.rows) * hkv;
     return c;
 }
-size_t cached_workspace(const CachedCut& c, int d) { return (size_t)c.groups * 2 * c.rows * (d * sizeof(float) + sizeof(float2)); }
+size_t cached_workspace(const CachedCut& c, int d) {
+    return (size_t)c.groups * (2 * c.rows * (d * sizeof(float) + sizeof(float2)) + sizeof(JoinItem));
+}
 
 }  // namespace
 }  // namespace tsp
@@ -599,13 +1018,18 @@ extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, i
     TSP_REQUIRE(workspace_bytes >= need, TSP_ERR_WORKSPACE, "tsp_attention_cached: workspace of %zu bytes, needs %zu", workspace_bytes, need);
     TSP_REQUIRE(reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0, TSP_ERR_INVALID, "tsp_attention_cached: workspace not 16-byte aligned");
     float* part = static_cast<float*>(d_workspace);
+    float2* stat = reinterpret_cast<float2*>(part + (size_t)cut.groups * 2 * cut.rows * c.d);
     const CachedArgs a{q->data, out->data, q->row_stride, q->head_stride, out->row_stride, out->head_stride, kv_args(c, d_table, max_pages, d_lengths),
-                       d_offsets, nq, samples, share, causal ? 1 : 0, cut.groups, CF_NW, fast_div((uint32_t)share), scale * kLog2e, part,
-                       reinterpret_cast<float2*>(part + (size_t)cut.groups * 2 * cut.rows * c.d)};
+                       d_offsets, nq, samples, share, causal ? 1 : 0, cut.groups, cut.least, fast_div((uint32_t)share), scale * kLog2e, part, stat,
+                       reinterpret_cast<JoinItem*>(stat + (size_t)cut.groups * 2 * cut.rows)};
     hipStream_t s = as_stream(stream);
     auto go = [&](auto bf, auto nb, auto mx) {
-        constexpr bool BF16 = decltype(bf)::value;
-        hipLaunchKernelGGL((k_cached_few<BF16, decltype(nb)::value, decltype(mx)::value, 1>), dim3((unsigned)cut.groups), dim3(CF_NW * 64), 0, s, a);
+        constexpr bool BF16 = decltype(bf)::value, MX4 = decltype(mx)::value;
+        constexpr int NB = decltype(nb)::value;
+        const dim3 grid((unsigned)cut.groups);
+        if (cut.rows == 16) hipLaunchKernelGGL((k_cached_few<BF16, NB, MX4, 1>), grid, dim3(CF_NW * 64), 0, s, a);
+        else if (cut.rows == 32) hipLaunchKernelGGL((k_cached_few<BF16, NB, MX4, 2>), grid, dim3(CF_NW * 64), 0, s, a);
+        else hipLaunchKernelGGL((k_cached_many<BF16, NB, MX4>), grid, dim3(CM_NW * 64), 0, s, a);
     };
     auto by_width = [&](auto bf, auto mx) {
         if (c.d <= 32) go(bf, std::integral_constant<int, 1>{}, mx);
@@ -613,11 +1037,19 @@ extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, i
         else if (c.d <= 96) go(bf, std::integral_constant<int, 3>{}, mx);
         else go(bf, std::integral_constant<int, 4>{}, mx);
     };
+    auto join = [&](auto bf, auto rows) {
+        constexpr bool BF16 = decltype(bf)::value;
+        constexpr int ROWS = decltype(rows)::value;
+        const unsigned cuts = (unsigned)cut.groups - 1;
+        if (cut.many_pieces) hipLaunchKernelGGL((k_cached_join<BF16, ROWS, 16>), dim3(cuts, ROWS), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((k_cached_join<BF16, ROWS, 4>), dim3(cuts, ROWS / 4), dim3(256), 0, s, a);
+    };
     auto by_type = [&](auto bf) {
         if (c.format == TSP_KV_MX4) by_width(bf, std::true_type{});
         else by_width(bf, std::false_type{});
-        constexpr bool BF16 = decltype(bf)::value;
-        hipLaunchKernelGGL((k_cached_join<BF16, 16, CF_KEYS>), dim3((unsigned)cut.groups - 1), dim3(256), 0, s, a);
+        if (cut.rows == 16) join(bf, std::integral_constant<int, 16>{});
+        else if (cut.rows == 32) join(bf, std::integral_constant<int, 32>{});
+        else join(bf, std::integral_constant<int, CM_ROWS>{});
     };
     if (dtype == TSP_BF16) by_type(std::true_type{});
     else by_type(std::false_type{});
