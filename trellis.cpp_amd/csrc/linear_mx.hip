@@ -28,7 +28,8 @@ struct LinearArgs {
     void* out;
     int64_t n;
     int ci, co, act, out_dtype;
-    int vec;       // rows of out and residual in whole pieces of four
+    int vec;       // outputs of a row in whole aligned pieces of 8 (co a multiple of it), of 4, or 0
+    int tiles;
 };
 
 __device__ __forceinline__ f32x4_t scaled_product(u32x4_t a0, u32x4_t a1, uint32_t ap, u32x4_t b0, u32x4_t b1, uint32_t bp, f32x4_t c) {
@@ -57,95 +58,106 @@ __device__ __forceinline__ f32x4_t exact_product(u32x4_t a, u32x4_t b, f32x4_t c
 // wants channels 16 g and 64 + 16 g, and applies the power of block g of four; in the other form a lane takes its own
 // block, 32 g and 32 g + 16.
 template <bool EXACT>
-__device__ __forceinline__ int operand_piece(int g, int half) { return EXACT ? 2 * g + half : g + 4 * half; }
+__device__ __forceinline__ constexpr int operand_piece(int g, int half) { return EXACT ? 2 * g + half : g + 4 * half; }
 
-// Four consecutive outputs of a row.
-__device__ __forceinline__ void finish(const LinearArgs& a, int64_t row, int o, f32x4_t y) {
-    if (row >= a.n || o >= a.co) return;
-    const int64_t at = row * a.co + o;
-    const int count = min(4, a.co - o);
-    if (a.bias) {
+__device__ __forceinline__ f32x4_t silu4(f32x4_t y) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < count) y[i] += a.bias[o + i];
-    }
-    if (a.act) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = y[i] / (1.f + __expf(-y[i]));
-    }
-    if (a.vec) {
-        if (a.residual) y += *reinterpret_cast<const f32x4_t*>(a.residual + at);
-        if (a.out_dtype == TSP_F32) {
-            *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.out) + at) = y;
-        } else {
-            uint2 p;
-            if (a.out_dtype == TSP_BF16) p = uint2{f32x2_to_bf16x2_bits(y[0], y[1]), f32x2_to_bf16x2_bits(y[2], y[3])};
-            else p = uint2{f32_to_f16_bits(y[0]) | ((uint32_t)f32_to_f16_bits(y[1]) << 16), f32_to_f16_bits(y[2]) | ((uint32_t)f32_to_f16_bits(y[3]) << 16)};
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = p;
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (i >= count) break;
-        const float v = y[i] + (a.residual ? a.residual[at + i] : 0.f);
-        if (a.out_dtype == TSP_F32) static_cast<float*>(a.out)[at + i] = v;
-        else static_cast<uint16_t*>(a.out)[at + i] = a.out_dtype == TSP_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
-    }
+    for (int i = 0; i < 4; ++i) y[i] = y[i] / (1.f + __expf(-y[i]));
+    return y;
 }
 
-// A tile of TX rows x TW outputs by WX x WW waves. Codes go straight from memory to LDS, 16 bytes a lane, each from the
-// piece that belongs in its place: piece p of row r lies in slot p ^ (r % 8), so that eight rows cover all banks.
-// Rows and channels past the ends read as zeros (out of the buffer's range).
-template <int TX, int TW, int WX, int WW, bool EXACT>
+// An output, its bias and activation applied.
+__device__ __forceinline__ void finish1(const LinearArgs& a, int64_t row, int o, float y) {
+    const int64_t at = row * a.co + o;
+    if (a.residual) y += a.residual[at];
+    if (a.out_dtype == TSP_F32) static_cast<float*>(a.out)[at] = y;
+    else static_cast<uint16_t*>(a.out)[at] = a.out_dtype == TSP_BF16 ? f32_to_bf16_bits(y) : f32_to_f16_bits(y);
+}
+// EACH pieces of four consecutive outputs of a row, which begin on a boundary of their size (co is a multiple of four).
+template <int EACH>
+__device__ __forceinline__ void finish4(const LinearArgs& a, int64_t row, int o, f32x4_t (&y)[EACH]) {
+    if (o >= a.co) return;
+    const int64_t at = row * a.co + o;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k)
+        if (a.residual && o + 4 * k < a.co) y[k] += *reinterpret_cast<const f32x4_t*>(a.residual + at + 4 * k);
+    if (a.out_dtype == TSP_F32) {
+#pragma unroll
+        for (int k = 0; k < EACH; ++k)
+            if (o + 4 * k < a.co) *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.out) + at + 4 * k) = y[k];
+        return;
+    }
+    uint2 p[EACH];
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+        if (a.out_dtype == TSP_BF16) p[k] = uint2{f32x2_to_bf16x2_bits(y[k][0], y[k][1]), f32x2_to_bf16x2_bits(y[k][2], y[k][3])};
+        else p[k] = uint2{f32_to_f16_bits(y[k][0]) | ((uint32_t)f32_to_f16_bits(y[k][1]) << 16), f32_to_f16_bits(y[k][2]) | ((uint32_t)f32_to_f16_bits(y[k][3]) << 16)};
+    }
+    uint16_t* out = static_cast<uint16_t*>(a.out) + at;
+    if constexpr (EACH == 2) {
+        if (a.vec == 8) {       // (rows of whole 16-byte pieces)
+            *reinterpret_cast<u32x4_t*>(out) = u32x4_t{p[0].x, p[0].y, p[1].x, p[1].y};
+            return;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < EACH; ++k)
+        if (o + 4 * k < a.co) *reinterpret_cast<uint2*>(out + 4 * k) = p[k];
+}
+
+// Waits for all but the last N of this wave's loads and for its LDS reads, and then for the workgroup. (A plain barrier
+// waits for every load.)
+template <int N>
+__device__ __forceinline__ void loads_and_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// A tile of TX rows x TW outputs by WX x WW waves, in steps of 128 channels that STAGES buffers hold, so that STAGES - 1 of them
+// are on their way. Codes go straight from memory to LDS, 16 bytes a lane, each from the piece that belongs in its place:
+// piece p of row r lies in slot p ^ (r % 8), so that eight rows cover all banks. Powers go there too, a row's four of a step
+// at once, or with ANY (channels that are no whole steps) one a load. Rows and channels past the ends read as zeros (out of the
+// buffer's range), and so do steps past the last, which keep the count of loads that are on their way. Each buffer is
+// an array of its own: of one array the compiler would have every load land before any of it is read.
+template <int TX, int TW, int WX, int WW, int STAGES, bool EXACT, bool ANY>
 __global__ __launch_bounds__(WX * WW * 64) void k_linear_mx(LinearArgs a) {
-    constexpr int NW = WX * WW, NT = NW * 64, RX = TX / WX / 16, RW = TW / WW / 16;
-    constexpr int LOADS_X = TX * LM_K / 1024 / NW, LOADS_W = TW * LM_K / 1024 / NW;
-    static_assert((TX + TW) % NT == 0 && LOADS_X > 0 && LOADS_W > 0, "whole loads a wave");
-    __shared__ __attribute__((aligned(16))) uint8_t sX[2][TX * LM_K], sW[2][TW * LM_K];
-    __shared__ uint32_t sP[2][TX + TW];      // the rows' four powers of a step, x's first
+#ifdef __HIP_DEVICE_COMPILE__       // (the host pass does not know the loads)
+    constexpr int NW = WX * WW, NT = NW * 64, RX = TX / WX / 16, RW = TW / WW / 16, ROWS = TX + TW;
+    constexpr int LOADS_X = TX * LM_K / 1024 / NW, LOADS_W = TW * LM_K / 1024 / NW, PARTS = ANY ? 4 : 1;
+    constexpr int PROWS = (ROWS + NT - 1) / NT * NT, LOADS = LOADS_X + LOADS_W + PARTS * PROWS / NT;      // (every wave has as many)
+    static_assert(TX % 64 == 0 && LOADS_X > 0 && LOADS_W > 0 && STAGES >= 2 && STAGES <= 4, "whole loads a wave");
+    static_assert(TX * LM_K % (1024 * NW) == 0 && TW * LM_K % (1024 * NW) == 0, "whole loads a wave");
+    __shared__ __attribute__((aligned(16))) uint8_t sC0[ROWS * LM_K], sC1[ROWS * LM_K], sC2[STAGES > 2 ? ROWS * LM_K : 16], sC3[STAGES > 3 ? ROWS * LM_K : 16];
+    __shared__ uint32_t sP0[PARTS * PROWS], sP1[PARTS * PROWS], sP2[STAGES > 2 ? PARTS * PROWS : 1], sP3[STAGES > 3 ? PARTS * PROWS : 1];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
-    const int tiles_w = (a.co + TW - 1) / TW;
-    const int64_t x0 = (int64_t)(blockIdx.x / tiles_w) * TX;
-    const int w0 = (int)(blockIdx.x % tiles_w) * TW;
+    // An eighth of the tiles each XCD (which takes every eighth workgroup), outputs of one tile of rows next to each other.
+    const int tiles_w = (a.co + TW - 1) / TW, tile = (int)(blockIdx.x % 8) * (int)(gridDim.x / 8) + (int)(blockIdx.x / 8);
+    if (tile >= a.tiles) return;
+    const int64_t x0 = (int64_t)(tile / tiles_w) * TX;
+    const int w0 = tile % tiles_w * TW, blocks = a.ci / MX_BLOCK;
     const int rows_x = (int)min((int64_t)TX, a.n - x0), rows_w = min(TW, a.co - w0);
-    const auto rx = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x + x0 * a.ci), (short)0, rows_x * a.ci, 0x00027000);
-    const auto rw = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (int64_t)w0 * a.ci), (short)0, rows_w * a.ci, 0x00027000);
+    auto buffer = [](const uint8_t* p, int bytes) __attribute__((always_inline)) { return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, bytes, 0x00027000); };
+    const auto rx = buffer(a.x + x0 * a.ci, rows_x * a.ci), rw = buffer(a.w + (int64_t)w0 * a.ci, rows_w * a.ci);
+    const auto rxp = buffer(a.xp + x0 * blocks, rows_x * blocks), rwp = buffer(a.wp + (int64_t)w0 * blocks, rows_w * blocks);
     constexpr int NOWHERE = 1 << 30;      // past every tile's bytes
-    auto stage = [&](int k0, int buf) __attribute__((always_inline)) {
-        const int row = lane >> 3, k = k0 + ((lane & 7) ^ (row & 7)) * 16;
-        const int at = k < a.ci ? row * a.ci + k : NOWHERE;
+    const int row8 = lane >> 3, piece8 = ((lane & 7) ^ (row8 & 7)) * 16;
+    using lds = __attribute__((address_space(3))) void*;
+    auto stage = [&](int k0, uint8_t* sC, uint32_t* sP) __attribute__((always_inline)) {
+        const int at = k0 + piece8 < a.ci ? row8 * a.ci + k0 + piece8 : NOWHERE;
 #pragma unroll
         for (int i = 0; i < LOADS_X; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (__attribute__((address_space(3))) void*)(sX[buf] + (i * NW + wave) * 1024), 16,
-                                                     at + (i * NW + wave) * 8 * a.ci, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rx, (lds)(sC + (i * NW + wave) * 1024), 16, at + (i * NW + wave) * 8 * a.ci, 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < LOADS_W; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (__attribute__((address_space(3))) void*)(sW[buf] + (i * NW + wave) * 1024), 16,
-                                                     at + (i * NW + wave) * 8 * a.ci, 0, 0, 0);
-    };
-    const int blocks = a.ci / MX_BLOCK;
-    constexpr int EACH = (TX + TW) / NT;      // rows of powers a thread
-    auto powers = [&](int k0, uint32_t (&p)[EACH]) __attribute__((always_inline)) {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rw, (lds)(sC + TX * LM_K + (i * NW + wave) * 1024), 16, at + (i * NW + wave) * 8 * a.ci, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            const int r = i * NT + threadIdx.x, row = r < TX ? r : r - TX, b = k0 / MX_BLOCK;
-            const bool there = row < (r < TX ? rows_x : rows_w);
-            const uint8_t* from = (r < TX ? a.xp + (x0 + row) * blocks : a.wp + (int64_t)(w0 + row) * blocks) + b;
-            p[i] = 0;
-            if (!there) continue;
-            if (blocks % 4 == 0) {
-                p[i] = *reinterpret_cast<const uint32_t*>(from);
-            } else {
+        for (int i = 0; i < PROWS / NT; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (b + j < blocks) p[i] |= (uint32_t)from[j] << (8 * j);
+            for (int j = 0; j < PARTS; ++j) {
+                const int r0 = (i * NW + wave) * 64, b = k0 / MX_BLOCK + j;      // 64 rows of x, or of W
+                const int from = b < blocks && r0 < ROWS ? ((r0 < TX ? r0 : r0 - TX) + lane) * blocks + b : NOWHERE;
+                if (r0 < TX) __builtin_amdgcn_raw_ptr_buffer_load_lds(rxp, (lds)(sP + j * PROWS + r0), ANY ? 1 : 4, from, 0, 0, 0);
+                else __builtin_amdgcn_raw_ptr_buffer_load_lds(rwp, (lds)(sP + j * PROWS + r0), ANY ? 1 : 4, from, 0, 0, 0);
             }
-        }
-    };
-    auto put_powers = [&](int buf, const uint32_t (&p)[EACH]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) sP[buf][i * NT + threadIdx.x] = p[i];
     };
     const int wx = wave / WW * RX * 16, ww = wave % WW * RW * 16;      // the wave's first rows of the tile
     f32x4_t acc[RW][RX];
@@ -153,69 +165,217 @@ __global__ __launch_bounds__(WX * WW * 64) void k_linear_mx(LinearArgs a) {
     for (int i = 0; i < RW; ++i)
 #pragma unroll
         for (int j = 0; j < RX; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    auto piece = [&](const uint8_t* s, int row, int half) __attribute__((always_inline)) {
-        return *reinterpret_cast<const u32x4_t*>(s + row * LM_K + ((operand_piece<EXACT>(g, half) ^ (row & 7)) * 16));
-    };
-    uint32_t p[EACH];
-    stage(0, 0);
-    powers(0, p);
-    put_powers(0, p);
-    int buf = 0;
-    for (int k0 = 0; k0 < a.ci; k0 += LM_K, buf ^= 1) {
-        __builtin_amdgcn_s_waitcnt(0x0f70);      // this wave's own loads; the barrier says that every wave's have landed
-        __syncthreads();
-        const bool more = k0 + LM_K < a.ci;
-        if (more) {
-            stage(k0 + LM_K, buf ^ 1);
-            powers(k0 + LM_K, p);
-        }
-        const uint8_t *px = reinterpret_cast<const uint8_t*>(sP[buf]) + g, *pw = px + TX * 4;
+    // Rows of W follow x's. The second half of an operand is the piece whose number differs in one bit.
+    constexpr int flip = (operand_piece<EXACT>(0, 0) ^ operand_piece<EXACT>(0, 1)) * 16;
+    const int swizzled = (operand_piece<EXACT>(g, 0) ^ (r16 & 7)) * 16;
+    const int x_at = (wx + r16) * LM_K + swizzled, w_at = (TX + ww + r16) * LM_K + swizzled;
+    const int xp_at = (wx + r16) * 4 + (ANY ? g * PROWS * 4 : g), wp_at = xp_at + (TX + ww - wx) * 4;
+    auto multiply = [&](const uint8_t* sC, const uint32_t* sP) __attribute__((always_inline)) {
+        // (rows 16 apart have one swizzle, and places that differ by a constant)
+        auto piece = [&](bool of_w, int i, int half) __attribute__((always_inline)) {
+            return *reinterpret_cast<const u32x4_t*>(sC + ((of_w ? w_at : x_at) ^ (half ? flip : 0)) + i * 16 * LM_K);
+        };
+        auto power = [&](bool of_w, int i) __attribute__((always_inline)) {
+            return (uint32_t) reinterpret_cast<const uint8_t*>(sP)[(of_w ? wp_at : xp_at) + i * 64];
+        };
+        // (the smaller side is held, the other comes by)
         if constexpr (EXACT) {
-            u32x4_t x[RX][4];
 #pragma unroll
-            for (int j = 0; j < RX; ++j) {
-                const int row = wx + j * 16 + r16;
-                const uint32_t power = px[row * 4];
-                widen(piece(sX[buf], row, 0), power, x[j][0], x[j][1]);
-                widen(piece(sX[buf], row, 1), power, x[j][2], x[j][3]);
-            }
+            for (int half = 0; half < 2; ++half) {
+                u32x4_t w[RW][2];
 #pragma unroll
-            for (int i = 0; i < RW; ++i) {
-                const int row = ww + i * 16 + r16;
-                const uint32_t power = pw[row * 4];
-                u32x4_t w[4];
-                widen(piece(sW[buf], row, 0), power, w[0], w[1]);
-                widen(piece(sW[buf], row, 1), power, w[2], w[3]);
+                for (int i = 0; i < RW; ++i) widen(piece(true, i, half), power(true, i), w[i][0], w[i][1]);
 #pragma unroll
-                for (int s = 0; s < 4; ++s)
+                for (int j = 0; j < RX; ++j) {
+                    u32x4_t x[2];
+                    widen(piece(false, j, half), power(false, j), x[0], x[1]);
 #pragma unroll
-                    for (int j = 0; j < RX; ++j) acc[i][j] = exact_product(w[s], x[j][s], acc[i][j]);
+                    for (int s = 0; s < 2; ++s)
+#pragma unroll
+                        for (int i = 0; i < RW; ++i) acc[i][j] = exact_product(w[i][s], x[s], acc[i][j]);
+                }
             }
         } else {
-            u32x4_t x[RX][2];
-            uint32_t xp[RX];
-#pragma unroll
-            for (int j = 0; j < RX; ++j) {
-                const int row = wx + j * 16 + r16;
-                xp[j] = px[row * 4];
-                x[j][0] = piece(sX[buf], row, 0);
-                x[j][1] = piece(sX[buf], row, 1);
-            }
+            u32x4_t w[RW][2];
+            uint32_t wp[RW];
 #pragma unroll
             for (int i = 0; i < RW; ++i) {
-                const int row = ww + i * 16 + r16;
-                const uint32_t wp = pw[row * 4];
-                const u32x4_t w0 = piece(sW[buf], row, 0), w1 = piece(sW[buf], row, 1);
+                wp[i] = power(true, i);
+                w[i][0] = piece(true, i, 0);
+                w[i][1] = piece(true, i, 1);
+            }
 #pragma unroll
-                for (int j = 0; j < RX; ++j) acc[i][j] = scaled_product(w0, w1, wp, x[j][0], x[j][1], xp[j], acc[i][j]);
+            for (int j = 0; j < RX; ++j) {
+                const uint32_t xp = power(false, j);
+                const u32x4_t x0 = piece(false, j, 0), x1 = piece(false, j, 1);
+#pragma unroll
+                for (int i = 0; i < RW; ++i) acc[i][j] = scaled_product(w[i][0], w[i][1], wp[i], x0, x1, xp, acc[i][j]);
             }
         }
-        if (more) put_powers(buf ^ 1, p);
+    };
+    auto codes = [&](auto i) __attribute__((always_inline)) -> uint8_t* {
+        constexpr int I = decltype(i)::value;
+        if constexpr (I == 0) return sC0;
+        else if constexpr (I == 1) return sC1;
+        else if constexpr (I == 2) return sC2;
+        else return sC3;
+    };
+    auto powers = [&](auto i) __attribute__((always_inline)) -> uint32_t* {
+        constexpr int I = decltype(i)::value;
+        if constexpr (I == 0) return sP0;
+        else if constexpr (I == 1) return sP1;
+        else if constexpr (I == 2) return sP2;
+        else return sP3;
+    };
+    // The step at k0 in buffer I; the one STAGES - 1 later takes the place of the step before.
+    auto step = [&](int k0, auto i) __attribute__((always_inline)) {
+        constexpr int I = decltype(i)::value, LAST = (I + STAGES - 1) % STAGES;
+        using Last = std::integral_constant<int, LAST>;
+        if (k0 >= a.ci) return;
+        loads_and_barrier<LOADS * (STAGES - 2)>();
+        stage(k0 + (STAGES - 1) * LM_K, codes(Last{}), powers(Last{}));
+        multiply(codes(i), powers(i));
+    };
+    using std::integral_constant;
+    stage(0, sC0, sP0);
+    if constexpr (STAGES > 2) stage(LM_K, sC1, sP1);
+    if constexpr (STAGES > 3) stage(2 * LM_K, sC2, sP2);
+    for (int k0 = 0; k0 < a.ci; k0 += STAGES * LM_K) {
+        step(k0, integral_constant<int, 0>{});
+        step(k0 + LM_K, integral_constant<int, 1>{});
+        if constexpr (STAGES > 2) step(k0 + 2 * LM_K, integral_constant<int, 2>{});
+        if constexpr (STAGES > 3) step(k0 + 3 * LM_K, integral_constant<int, 3>{});
     }
+    loads_and_barrier<0>();      // (no load is on its way to LDS any more, and none of it is read)
+    // Rows leave in whole pieces: 16 of them at a time go through the wave's own part of LDS, 16-byte piece p of row r in
+    // place p ^ r.
+    constexpr int PIECES = RW * 4;
+    static_assert(NW * 16 * PIECES * 16 <= ROWS * LM_K && (PIECES == 16 || PIECES == 8), "the waves' parts fit a buffer");
+    char* s = reinterpret_cast<char*>(sC0) + wave * (16 * PIECES * 16);
+    f32x4_t bias[RW];
 #pragma unroll
     for (int i = 0; i < RW; ++i)
 #pragma unroll
-        for (int j = 0; j < RX; ++j) finish(a, x0 + wx + j * 16 + r16, w0 + ww + i * 16 + 4 * g, acc[i][j]);
+        for (int e = 0; e < 4; ++e) {
+            const int o = w0 + ww + i * 16 + 4 * g + e;
+            bias[i][e] = a.bias && o < a.co ? a.bias[o] : 0.f;
+        }
+#pragma unroll
+    for (int j = 0; j < RX; ++j) {
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+            f32x4_t y = acc[i][j] + bias[i];
+            if (a.act) y = silu4(y);
+            *reinterpret_cast<f32x4_t*>(s + (r16 * PIECES + ((i * 4 + g) ^ (r16 & (PIECES - 1)))) * 16) = y;
+        }
+        asm volatile("" ::: "memory");      // (the wave's own writes; LDS takes them in order)
+        const int64_t row0 = x0 + wx + j * 16;
+        if (a.vec == 0) {
+            for (int at = lane; at < 16 * PIECES * 4; at += 64) {
+                const int r = at / (PIECES * 4), e = at % (PIECES * 4);
+                const float y = *reinterpret_cast<const float*>(s + (r * PIECES + ((e / 4) ^ (r & (PIECES - 1)))) * 16 + e % 4 * 4);
+                if (row0 + r < a.n && w0 + ww + e < a.co) finish1(a, row0 + r, w0 + ww + e, y);
+            }
+        } else {
+            // two pieces of four outputs a lane where they leave in 16 bits, one in 32
+            auto leave = [&](auto each) __attribute__((always_inline)) {
+                constexpr int EACH = decltype(each)::value, LANES = PIECES / EACH;
+#pragma unroll
+                for (int q = 0; q < 16 * LANES / 64; ++q) {
+                    const int r = (q * 64 + lane) / LANES, p = (q * 64 + lane) % LANES * EACH;
+                    f32x4_t y[EACH];
+#pragma unroll
+                    for (int k = 0; k < EACH; ++k) y[k] = *reinterpret_cast<const f32x4_t*>(s + (r * PIECES + ((p + k) ^ (r & (PIECES - 1)))) * 16);
+                    if (row0 + r < a.n) finish4<EACH>(a, row0 + r, w0 + ww + p * 4, y);
+                }
+            };
+            if constexpr (EXACT) leave(std::integral_constant<int, 1>{});
+            else leave(std::integral_constant<int, 2>{});
+        }
+        asm volatile("" ::: "memory");
+    }
+#endif
+}
+
+// Up to RT * 16 rows: W is all there is to read. Eight waves take 16 outputs, every eighth step of 128 channels each, straight
+// from memory to the operands; their sums meet in LDS, in the waves' order.
+constexpr int LF_NW = 8;
+template <int RT, bool EXACT>
+__global__ __launch_bounds__(LF_NW * 64) void k_linear_mx_few(LinearArgs a) {
+    __shared__ f32x4_t sAcc[LF_NW][RT][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
+    const int o0 = blockIdx.x * 16, blocks = a.ci / MX_BLOCK;
+    f32x4_t acc[RT];
+#pragma unroll
+    for (int j = 0; j < RT; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    struct Operand {
+        u32x4_t c[2];
+        uint32_t p;
+    };
+    auto load = [&](const uint8_t* codes, const uint8_t* powers, int row, bool there, int k0) __attribute__((always_inline)) {
+        Operand x{{{0, 0, 0, 0}, {0, 0, 0, 0}}, 0};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int k = k0 + operand_piece<EXACT>(g, half) * 16;
+            if (there && k < a.ci) x.c[half] = *reinterpret_cast<const u32x4_t*>(codes + (int64_t)row * a.ci + k);
+        }
+        if (there && k0 / MX_BLOCK + g < blocks) x.p = powers[(int64_t)row * blocks + k0 / MX_BLOCK + g];
+        return x;
+    };
+    auto multiply = [&](const Operand& w, const Operand (&x)[RT]) __attribute__((always_inline)) {
+        if constexpr (EXACT) {
+            u32x4_t wf[4];
+            widen(w.c[0], w.p, wf[0], wf[1]);
+            widen(w.c[1], w.p, wf[2], wf[3]);
+#pragma unroll
+            for (int j = 0; j < RT; ++j) {
+                u32x4_t xf[4];
+                widen(x[j].c[0], x[j].p, xf[0], xf[1]);
+                widen(x[j].c[1], x[j].p, xf[2], xf[3]);
+#pragma unroll
+                for (int s = 0; s < 4; ++s) acc[j] = exact_product(wf[s], xf[s], acc[j]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < RT; ++j) acc[j] = scaled_product(w.c[0], w.c[1], w.p, x[j].c[0], x[j].c[1], x[j].p, acc[j]);
+        }
+    };
+    constexpr int AHEAD = RT == 1 ? 4 : 2, STEP = LF_NW * LM_K;      // steps on their way
+    for (int k0 = wave * LM_K; k0 < a.ci; k0 += AHEAD * STEP) {
+        Operand w[AHEAD], x[AHEAD][RT];
+#pragma unroll
+        for (int s = 0; s < AHEAD; ++s) {
+            const int k = k0 + s * STEP;
+            w[s] = load(a.w, a.wp, o0 + r16, o0 + r16 < a.co && k < a.ci, k);
+#pragma unroll
+            for (int j = 0; j < RT; ++j) x[s][j] = load(a.x, a.xp, j * 16 + r16, j * 16 + r16 < a.n && k < a.ci, k);
+        }
+#pragma unroll
+        for (int s = 0; s < AHEAD; ++s)
+            if (k0 + s * STEP < a.ci) multiply(w[s], x[s]);
+    }
+#pragma unroll
+    for (int j = 0; j < RT; ++j) sAcc[wave][j][lane] = acc[j];
+    __syncthreads();
+    if (wave >= RT) return;
+    f32x4_t y = sAcc[0][wave][lane];
+#pragma unroll
+    for (int w = 1; w < LF_NW; ++w) y += sAcc[w][wave][lane];
+    const int64_t row = wave * 16 + r16;
+    const int o = o0 + 4 * g;
+    if (row >= a.n) return;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (a.bias && o + e < a.co) y[e] += a.bias[o + e];
+    if (a.act) y = silu4(y);
+    if (a.vec) {
+        f32x4_t one[1] = {y};
+        finish4<1>(a, row, o, one);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (o + e < a.co) finish1(a, row, o + e, y[e]);
+    }
 }
 
 }  // namespace
@@ -250,14 +410,52 @@ extern "C" int tsp_linear_mx(const void* d_x, const uint8_t* d_x_powers, int64_t
                     !overlap(d_out, out_bytes, d_bias, (size_t)co * 4) &&
                     (!overlap(d_out, out_bytes, d_residual, (size_t)n * co * 4) || (d_out == d_residual && out_dtype == TSP_F32)),
                 TSP_ERR_INVALID, "tsp_linear_mx: out overlaps an input (it may be an f32 residual, or apart)");
-    const bool vec = co % 4 == 0 && !(reinterpret_cast<uintptr_t>(d_out) % 16 || reinterpret_cast<uintptr_t>(d_residual) % 16);
-    const LinearArgs a{static_cast<const uint8_t*>(d_x), d_x_powers, static_cast<const uint8_t*>(d_w), d_w_powers, d_bias, d_residual,
-                       d_out, n, ci, co, act, out_dtype, vec};
+    const int vec = co % 4 || reinterpret_cast<uintptr_t>(d_out) % 16 || reinterpret_cast<uintptr_t>(d_residual) % 16 ? 0 : co % 8 ? 4 : 8;
+    LinearArgs a{static_cast<const uint8_t*>(d_x), d_x_powers, static_cast<const uint8_t*>(d_w), d_w_powers, d_bias, d_residual,
+                       d_out, n, ci, co, act, out_dtype, vec, 0};
     hipStream_t s = as_stream(stream);
-    const int64_t tiles = ceil_div(n, 128) * ceil_div(co, 128);
-    TSP_REQUIRE(tiles < (1ll << 24), TSP_ERR_INVALID, "tsp_linear_mx: too many rows and outputs");
-    if (out_dtype == TSP_F32) hipLaunchKernelGGL((k_linear_mx<128, 128, 2, 2, true>), dim3((unsigned)tiles), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_linear_mx<128, 128, 2, 2, false>), dim3((unsigned)tiles), dim3(256), 0, s, a);
+    using std::integral_constant;
+    auto by_form = [&](auto&& go) {
+        if (out_dtype == TSP_F32) go(std::true_type{});
+        else go(std::false_type{});
+    };
+    if (n <= 64) {
+        by_form([&](auto exact) {
+            constexpr bool EXACT = decltype(exact)::value;
+            const dim3 grid((unsigned)ceil_div(co, 16)), block(LF_NW * 64);
+            if (n <= 16) hipLaunchKernelGGL((k_linear_mx_few<1, EXACT>), grid, block, 0, s, a);
+            else if (n <= 32) hipLaunchKernelGGL((k_linear_mx_few<2, EXACT>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((k_linear_mx_few<4, EXACT>), grid, block, 0, s, a);
+        });
+        TSP_CHECK_LAUNCH();
+        return TSP_OK;
+    }
+    auto go = [&](auto tx, auto tw, auto wx, auto ww, auto stages) -> int {
+        constexpr int TX = decltype(tx)::value, TW = decltype(tw)::value, WX = decltype(wx)::value, WW = decltype(ww)::value, ST = decltype(stages)::value;
+        const int64_t tiles = ceil_div(n, TX) * ceil_div(co, TW);
+        TSP_REQUIRE(tiles * WX * WW * 64 < (1ll << 31), TSP_ERR_INVALID, "tsp_linear_mx: too many rows and outputs");
+        a.tiles = (int)tiles;
+        by_form([&](auto exact) {
+            constexpr bool EXACT = decltype(exact)::value;
+            const dim3 grid((unsigned)ceil_div(tiles, 8) * 8), block(WX * WW * 64);
+            if (ci % LM_K == 0) hipLaunchKernelGGL((k_linear_mx<TX, TW, WX, WW, ST, EXACT, false>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((k_linear_mx<TX, TW, WX, WW, ST, EXACT, true>), grid, block, 0, s, a);
+        });
+        return TSP_OK;
+    };
+    auto I = [](auto v) { return v; };
+    (void)I;
+    int rc;
+    const int64_t big = ceil_div(n, 256) * ceil_div(co, 256);
+    const char* e = getenv("LM_CFG");
+    const int cfg = e ? atoi(e) : big >= 256 ? 0 : 1;
+    if (cfg == 0) rc = go(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{});
+    else if (cfg == 1) rc = go(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
+    else if (cfg == 2) rc = go(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 4>{});
+    else if (cfg == 3) rc = go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
+    else if (cfg == 4) rc = go(integral_constant<int, 256>{}, integral_constant<int, 128>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
+    else rc = go(integral_constant<int, 128>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 3>{});
+    if (rc != TSP_OK) return rc;
     TSP_CHECK_LAUNCH();
     return TSP_OK;
 }
