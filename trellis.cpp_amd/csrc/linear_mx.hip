@@ -129,11 +129,15 @@ __global__ __launch_bounds__(WX * WW * 64) void k_linear_mx(LinearArgs a) {
     __shared__ __attribute__((aligned(16))) uint8_t sC0[ROWS * LM_K], sC1[ROWS * LM_K], sC2[STAGES > 2 ? ROWS * LM_K : 16], sC3[STAGES > 3 ? ROWS * LM_K : 16];
     __shared__ uint32_t sP0[PARTS * PROWS], sP1[PARTS * PROWS], sP2[STAGES > 2 ? PARTS * PROWS : 1], sP3[STAGES > 3 ? PARTS * PROWS : 1];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
-    // An eighth of the tiles each XCD (which takes every eighth workgroup), outputs of one tile of rows next to each other.
-    const int tiles_w = (a.co + TW - 1) / TW, tile = (int)(blockIdx.x % 8) * (int)(gridDim.x / 8) + (int)(blockIdx.x / 8);
+    // An eighth of the tiles each XCD, which takes every eighth workgroup and has an L2 of its own: bands of BAND tiles of
+    // rows, column by column, so that what runs on it at once is a patch of about as many rows as outputs.
+    constexpr int BAND = 8;
+    const int tiles_w = (a.co + TW - 1) / TW, tiles_x = a.tiles / tiles_w;
+    const int tile = (int)(blockIdx.x % 8) * (int)(gridDim.x / 8) + (int)(blockIdx.x / 8);
     if (tile >= a.tiles) return;
-    const int64_t x0 = (int64_t)(tile / tiles_w) * TX;
-    const int w0 = tile % tiles_w * TW, blocks = a.ci / MX_BLOCK;
+    const int band = tile / (BAND * tiles_w), in = tile - band * BAND * tiles_w, high = min(BAND, tiles_x - band * BAND);
+    const int64_t x0 = (int64_t)(band * BAND + in % high) * TX;
+    const int w0 = in / high * TW, blocks = a.ci / MX_BLOCK;
     const int rows_x = (int)min((int64_t)TX, a.n - x0), rows_w = min(TW, a.co - w0);
     auto buffer = [](const uint8_t* p, int bytes) __attribute__((always_inline)) { return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, bytes, 0x00027000); };
     const auto rx = buffer(a.x + x0 * a.ci, rows_x * a.ci), rw = buffer(a.w + (int64_t)w0 * a.ci, rows_w * a.ci);
@@ -297,17 +301,19 @@ __global__ __launch_bounds__(WX * WW * 64) void k_linear_mx(LinearArgs a) {
 #endif
 }
 
-// Up to RT * 16 rows: W is all there is to read. Eight waves take 16 outputs, every eighth step of 128 channels each, straight
-// from memory to the operands; their sums meet in LDS, in the waves' order.
+// Up to RT * 16 rows: W is all there is to read. Eight waves take WT * 16 outputs, every eighth step of 128 channels each,
+// straight from memory to the operands; their sums meet in LDS, in the waves' order.
 constexpr int LF_NW = 8;
-template <int RT, bool EXACT>
+template <int RT, int WT, bool EXACT>
 __global__ __launch_bounds__(LF_NW * 64) void k_linear_mx_few(LinearArgs a) {
-    __shared__ f32x4_t sAcc[LF_NW][RT][64];
+    __shared__ f32x4_t sAcc[LF_NW][WT * RT][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
-    const int o0 = blockIdx.x * 16, blocks = a.ci / MX_BLOCK;
-    f32x4_t acc[RT];
+    const int o0 = blockIdx.x * (WT * 16), blocks = a.ci / MX_BLOCK;
+    f32x4_t acc[WT][RT];
 #pragma unroll
-    for (int j = 0; j < RT; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < WT; ++i)
+#pragma unroll
+        for (int j = 0; j < RT; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     struct Operand {
         u32x4_t c[2];
         uint32_t p;
@@ -322,31 +328,39 @@ __global__ __launch_bounds__(LF_NW * 64) void k_linear_mx_few(LinearArgs a) {
         if (there && k0 / MX_BLOCK + g < blocks) x.p = powers[(int64_t)row * blocks + k0 / MX_BLOCK + g];
         return x;
     };
-    auto multiply = [&](const Operand& w, const Operand (&x)[RT]) __attribute__((always_inline)) {
+    auto multiply = [&](const Operand (&w)[WT], const Operand (&x)[RT]) __attribute__((always_inline)) {
         if constexpr (EXACT) {
-            u32x4_t wf[4];
-            widen(w.c[0], w.p, wf[0], wf[1]);
-            widen(w.c[1], w.p, wf[2], wf[3]);
+            u32x4_t wf[WT][4];
+#pragma unroll
+            for (int i = 0; i < WT; ++i) {
+                widen(w[i].c[0], w[i].p, wf[i][0], wf[i][1]);
+                widen(w[i].c[1], w[i].p, wf[i][2], wf[i][3]);
+            }
 #pragma unroll
             for (int j = 0; j < RT; ++j) {
                 u32x4_t xf[4];
                 widen(x[j].c[0], x[j].p, xf[0], xf[1]);
                 widen(x[j].c[1], x[j].p, xf[2], xf[3]);
 #pragma unroll
-                for (int s = 0; s < 4; ++s) acc[j] = exact_product(wf[s], xf[s], acc[j]);
+                for (int s = 0; s < 4; ++s)
+#pragma unroll
+                    for (int i = 0; i < WT; ++i) acc[i][j] = exact_product(wf[i][s], xf[s], acc[i][j]);
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < RT; ++j) acc[j] = scaled_product(w.c[0], w.c[1], w.p, x[j].c[0], x[j].c[1], x[j].p, acc[j]);
+            for (int j = 0; j < RT; ++j)
+#pragma unroll
+                for (int i = 0; i < WT; ++i) acc[i][j] = scaled_product(w[i].c[0], w[i].c[1], w[i].p, x[j].c[0], x[j].c[1], x[j].p, acc[i][j]);
         }
     };
-    constexpr int AHEAD = RT == 1 ? 4 : 2, STEP = LF_NW * LM_K;      // steps on their way
+    constexpr int AHEAD = RT * WT <= 2 ? 4 : 2, STEP = LF_NW * LM_K;      // steps on their way
     for (int k0 = wave * LM_K; k0 < a.ci; k0 += AHEAD * STEP) {
-        Operand w[AHEAD], x[AHEAD][RT];
+        Operand w[AHEAD][WT], x[AHEAD][RT];
 #pragma unroll
         for (int s = 0; s < AHEAD; ++s) {
             const int k = k0 + s * STEP;
-            w[s] = load(a.w, a.wp, o0 + r16, o0 + r16 < a.co && k < a.ci, k);
+#pragma unroll
+            for (int i = 0; i < WT; ++i) w[s][i] = load(a.w, a.wp, o0 + i * 16 + r16, o0 + i * 16 + r16 < a.co && k < a.ci, k);
 #pragma unroll
             for (int j = 0; j < RT; ++j) x[s][j] = load(a.x, a.xp, j * 16 + r16, j * 16 + r16 < a.n && k < a.ci, k);
         }
@@ -355,14 +369,16 @@ __global__ __launch_bounds__(LF_NW * 64) void k_linear_mx_few(LinearArgs a) {
             if (k0 + s * STEP < a.ci) multiply(w[s], x[s]);
     }
 #pragma unroll
-    for (int j = 0; j < RT; ++j) sAcc[wave][j][lane] = acc[j];
+    for (int i = 0; i < WT; ++i)
+#pragma unroll
+        for (int j = 0; j < RT; ++j) sAcc[wave][i * RT + j][lane] = acc[i][j];
     __syncthreads();
-    if (wave >= RT) return;
+    if (wave >= WT * RT) return;
     f32x4_t y = sAcc[0][wave][lane];
 #pragma unroll
     for (int w = 1; w < LF_NW; ++w) y += sAcc[w][wave][lane];
-    const int64_t row = wave * 16 + r16;
-    const int o = o0 + 4 * g;
+    const int64_t row = wave % RT * 16 + r16;
+    const int o = o0 + wave / RT * 16 + 4 * g;
     if (row >= a.n) return;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -376,6 +392,27 @@ __global__ __launch_bounds__(LF_NW * 64) void k_linear_mx_few(LinearArgs a) {
         for (int e = 0; e < 4; ++e)
             if (o + e < a.co) finish1(a, row, o + e, y[e]);
     }
+}
+
+// The tile with the least time of its rounds. A step of 128 channels takes a workgroup so many us where the device is full
+// (8,192 rows and outputs of 8,192 channels) and where it has a CU to itself (1,000 rows, 4,096 -> 1,024); a tile's first loads
+// and its rows' way out some more. (35,001 rows, 4,096 -> 1,024, fp32 out: 323 us by tiles of 256 x 256, 299 by 128 x 128;
+// 1,024 -> 4,096 in bf16: 190 and 205; 1,000 rows, 4,096 -> 1,024 in bf16: 53, 33, 22 and 18 by the four.)
+int linear_shape(int64_t n, int ci, int co, bool exact) {
+    struct Shape { int x, w, slots; double full, alone, full_exact, alone_exact, rest; };
+    static const Shape shapes[4] = {{256, 256, 256, 2.08, 1.4, 3.4, 2.7, 6.}, {128, 128, 512, 1.2, 0.8, 1.84, 1.4, 3.},
+                                    {128, 64, 512, 0.98, 0.55, 1.17, 0.72, 2.5}, {64, 64, 512, 0.7, 0.4, 0.83, 0.7, 2.}};
+    int best = 0;
+    double least = 1e30;
+    for (int i = 0; i < 4; ++i) {
+        const Shape& s = shapes[i];
+        const int64_t tiles = ceil_div(n, s.x) * ceil_div(co, s.w), rest = tiles % s.slots, steps = ceil_div(ci, LM_K);
+        const double full = steps * (exact ? s.full_exact : s.full) + s.rest, alone = steps * (exact ? s.alone_exact : s.alone) + s.rest;
+        // (a round of at most a workgroup a CU is as long as one alone; one of nearly 256 large ones is not)
+        const double time = (double)(tiles / s.slots) * full + (rest == 0 ? 0. : rest <= (s.slots == 256 ? 128 : 256) ? alone : full);
+        if (time < least) least = time, best = i;
+    }
+    return best;
 }
 
 }  // namespace
@@ -419,13 +456,24 @@ extern "C" int tsp_linear_mx(const void* d_x, const uint8_t* d_x_powers, int64_t
         if (out_dtype == TSP_F32) go(std::true_type{});
         else go(std::false_type{});
     };
-    if (n <= 64) {
+    // Few rows by the other kernel, with two tiles of outputs a workgroup where there are many: us, by it (one tile, two) and by
+    // tiles, in bf16 / fp32. 5 rows, 1,024 -> 4,096: 3.6 (3.8) and 5.4 / 3.9 (4.8) and 8.2. 32 rows, 4,096 -> 1,024: 10.1 (12.8)
+    // and 12.1 / 10.6 (13.0) and 22.8; 48: 12.9 and 12.1 / 13.3 and 22.9. 32 rows, 8,192 -> 8,192: 36 (24.9) and 27.3 / 37 (25.9)
+    // and 47; 4,096 -> 16,384: 37 (25) and 16.9 / 39 (27) and 27; 5 rows of it 17.8 (17.5) and 16.8 / 21.3 (19.9) and 26.4.
+    if (n <= 16 || (co <= 8192 && n <= (out_dtype == TSP_F32 ? 64 : 32))) {
         by_form([&](auto exact) {
             constexpr bool EXACT = decltype(exact)::value;
-            const dim3 grid((unsigned)ceil_div(co, 16)), block(LF_NW * 64);
-            if (n <= 16) hipLaunchKernelGGL((k_linear_mx_few<1, EXACT>), grid, block, 0, s, a);
-            else if (n <= 32) hipLaunchKernelGGL((k_linear_mx_few<2, EXACT>), grid, block, 0, s, a);
-            else hipLaunchKernelGGL((k_linear_mx_few<4, EXACT>), grid, block, 0, s, a);
+            auto few = [&](auto rt, auto wt) {
+                constexpr int RT = decltype(rt)::value, WT = decltype(wt)::value;
+                hipLaunchKernelGGL((k_linear_mx_few<RT, WT, EXACT>), dim3((unsigned)ceil_div(co, 16 * WT)), dim3(LF_NW * 64), 0, s, a);
+            };
+            auto by_rows = [&](auto wt) {
+                if (n <= 16) few(integral_constant<int, 1>{}, wt);
+                else if (n <= 32) few(integral_constant<int, 2>{}, wt);
+                else few(integral_constant<int, 4>{}, wt);
+            };
+            if (co >= 8192) by_rows(integral_constant<int, 2>{});
+            else by_rows(integral_constant<int, 1>{});
         });
         TSP_CHECK_LAUNCH();
         return TSP_OK;
@@ -443,18 +491,12 @@ extern "C" int tsp_linear_mx(const void* d_x, const uint8_t* d_x_powers, int64_t
         });
         return TSP_OK;
     };
-    auto I = [](auto v) { return v; };
-    (void)I;
+    const int shape = linear_shape(n, ci, co, out_dtype == TSP_F32);
     int rc;
-    const int64_t big = ceil_div(n, 256) * ceil_div(co, 256);
-    const char* e = getenv("LM_CFG");
-    const int cfg = e ? atoi(e) : big >= 256 ? 0 : 1;
-    if (cfg == 0) rc = go(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{});
-    else if (cfg == 1) rc = go(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
-    else if (cfg == 2) rc = go(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 4>{});
-    else if (cfg == 3) rc = go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
-    else if (cfg == 4) rc = go(integral_constant<int, 256>{}, integral_constant<int, 128>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
-    else rc = go(integral_constant<int, 128>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 3>{});
+    if (shape == 0) rc = go(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{});
+    else if (shape == 1) rc = go(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
+    else if (shape == 2) rc = go(integral_constant<int, 128>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 3>{});
+    else rc = go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
     if (rc != TSP_OK) return rc;
     TSP_CHECK_LAUNCH();
     return TSP_OK;
