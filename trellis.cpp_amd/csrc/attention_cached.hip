@@ -40,144 +40,167 @@ struct CachedArgs {
     const int32_t* q_off;
     int64_t nq;                                // below 2^31, nq * share too
     int samples, share, causal;
-    int groups, least;                         // workgroups, tiles that one has at least
+    int least, shift;                          // tiles that a workgroup has at least; weights are in 2^shift of them
     FastDiv by_share;
     float scale2;                              // scale * log2(e)
     float* part;                               // [2 * groups][row][d] sums of p v, and
-    float2* stat;                              // [2 * groups][row] maximum and sum of p (-1: no key seen), and
-    struct JoinItem* join;                     // [groups] the unit that is cut at the workgroup's end and began in it
+    float2* stat;                              // [2 * kGroups][row] maximum and sum of p (-1: no key seen), and
+    struct JoinItem* join;                     // [kGroups] the unit that is cut at the workgroup's end and began in it
 };
+
+constexpr int kGroups = 512;      // workgroups, two a CU
 
 // rows left in the unit from its first (0: none), the first, the sample's first row, the key head, the last workgroup.
 struct JoinItem {
     int rows, first_row, row0, head, last, pad[3];
 };
 
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-    return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
+#ifdef __HIP_DEVICE_COMPILE__       // (the host pass knows neither the register constraint nor the argument segment)
+// The kernel's arguments read anew: kept in scalar registers from the start on they would push the loops' own out of them.
+typedef const __attribute__((address_space(4))) CachedArgs* CachedArgsPtr;
+__device__ __forceinline__ CachedArgsPtr reread_args() {
+    CachedArgsPtr p = (CachedArgsPtr)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
 }
-__device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
-    return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)x, lane));
-}
+#endif
 
-// A sample's units (one key head) and their weights, first + slope * j of the j-th.
+// A sample's units (one key head) and their weights, first + slope * j of the j-th. (All sums of weights are below 2^30.)
 struct SampleWork {
-    int row0, lq, lk, count, first, slope;
-    __device__ __forceinline__ int64_t before(int64_t j) const { return first * j + slope * (j * (j - 1) / 2); }
+    int row0, lq, lk, count;
+    uint32_t first, slope;
+    __device__ __forceinline__ uint32_t before(uint32_t j) const { return first * j + slope * j * (j - 1) / 2; }
 };
 // Keys that a row sees, by its query.
 __device__ __forceinline__ int cached_limit(int causal, int lq, int lk, int query) { return causal ? min(max(lk - lq + query + 1, 0), lk) : lk; }
-template <int ROWS, int TILE>
-__device__ __forceinline__ int unit_tiles(const CachedArgs& a, int lq, int lk, int j) {
+template <int ROWS, int TILE, class Args>
+__device__ __forceinline__ int unit_tiles(const Args& a, int lq, int lk, int j) {
     const int last = min((j + 1) * ROWS, lq * a.share) - 1;
-    return (cached_limit(a.causal, lq, lk, last / a.by_share) + TILE - 1) / TILE;
+    return (cached_limit(a.causal, lq, lk, last / FastDiv{a.by_share.mul, a.by_share.shift}) + TILE - 1) / TILE;
 }
-template <int ROWS, int TILE>
-__device__ __forceinline__ SampleWork sample_work(const CachedArgs& a, int s) {
+template <int ROWS, int TILE, class Args>
+__device__ __forceinline__ SampleWork sample_work(const Args& a, int s) {
     SampleWork w{0, 0, 0, 0, 1, 0};
     if (s >= a.samples) return w;
     packed_rows(a.q_off, s, (int)a.nq, w.row0, w.lq);
-    w.lk = kv_length(a.cache, s);
+    w.lk = (int)min((int64_t)max(a.cache.lengths[s], 0), (int64_t)a.cache.max_pages << a.cache.page_bits);
     w.count = (int)((unsigned)(w.lq * a.share + ROWS - 1) / (unsigned)ROWS);
     if (w.count == 0) return w;
-    w.first = max(1, unit_tiles<ROWS, TILE>(a, w.lq, w.lk, 0));
-    if (w.count > 1) w.slope = max(0, (unit_tiles<ROWS, TILE>(a, w.lq, w.lk, w.count - 1) - w.first) / (w.count - 1));
+    w.first = max(1, unit_tiles<ROWS, TILE>(a, w.lq, w.lk, 0) >> a.shift);
+    if (w.count > 1) w.slope = (uint32_t)max(0, (unit_tiles<ROWS, TILE>(a, w.lq, w.lk, w.count - 1) >> a.shift) - (int)w.first) / (uint32_t)(w.count - 1);
     return w;
 }
 
-// The length of the line (by whole waves).
-template <int ROWS, int TILE>
-__device__ __forceinline__ int64_t line_length(const CachedArgs& a) {
-    int64_t sum = 0;
-    for (int s0 = 0; s0 < a.samples; s0 += 64) {
-        const SampleWork w = sample_work<ROWS, TILE>(a, s0 + (threadIdx.x & 63));
-        sum += w.before(w.count) * a.cache.heads;
-    }
+// The line: its length, each workgroup's part, and where there are up to 64 samples, what a lane knows of its own (by whole waves).
+struct Line {
+    uint32_t length, per;
+    SampleWork w;
+    uint32_t end;      // of the sample's units
+    __device__ __forceinline__ uint32_t cut(int group) const { return min(per * (uint32_t)group, length); }
+    __device__ __forceinline__ int group(uint32_t at) const { return (int)(at / per); }
+};
+__device__ __forceinline__ uint32_t scan64(uint32_t v) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    return uniform(sum);
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t x = __shfl_up(v, o, 64);
+        if (lane >= o) v += x;
+    }
+    return v;
+}
+template <int ROWS, int TILE, class Args>
+__device__ __forceinline__ Line make_line(const Args& a) {
+    Line l;
+    l.length = 0;
+    if (a.samples == 1) {
+        l.w = sample_work<ROWS, TILE>(a, 0);
+        l.length = l.end = __builtin_amdgcn_readfirstlane(l.w.before(l.w.count) * a.cache.heads);
+    } else {
+        for (int s0 = 0; s0 < a.samples; s0 += 64) {
+            l.w = sample_work<ROWS, TILE>(a, s0 + (threadIdx.x & 63));
+            l.end = l.length + scan64(l.w.before(l.w.count) * a.cache.heads);
+            l.length = __builtin_amdgcn_readlane(l.end, 63);
+        }
+    }
+    l.per = max((uint32_t)a.least, (l.length + kGroups - 1) / kGroups);
+    return l;
 }
 
 // A unit and where it stands in the line.
 struct CachedUnit {
-    int sample, head, row0, lq, lk;      // (sample -1: none)
+    int sample, head, row0, lq, lk;
     int first_row;                       // of its rows among the sample's
     int tiles;
-    int64_t begin, end;
+    uint32_t begin, end;
 };
 // The unit at a place in the line (by whole waves, all with one `at`).
-template <int ROWS, int TILE>
-__device__ __forceinline__ CachedUnit find_unit(const CachedArgs& a, int64_t at) {
-    CachedUnit u{-1, 0, 0, 0, 0, 0, 0, 0, 0};
-    const int lane = threadIdx.x & 63;
-    int64_t base = 0;
-    for (int s0 = 0; s0 < a.samples; s0 += 64) {
-        const SampleWork w = sample_work<ROWS, TILE>(a, s0 + lane);
-        const int64_t mine = w.before(w.count) * a.cache.heads;
-        int64_t end = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int64_t v = __shfl_up(end, o, 64);
-            if (lane >= o) end += v;
-        }
-        end += base;
-        const uint64_t found = __ballot(at >= end - mine && at < end);
-        if (found) {
-            const int l = __builtin_ctzll(found);
-            u.sample = s0 + l;
-            u.row0 = __builtin_amdgcn_readlane(w.row0, l);
-            u.lq = __builtin_amdgcn_readlane(w.lq, l);
-            u.lk = __builtin_amdgcn_readlane(w.lk, l);
-            const SampleWork k{0, 0, 0, __builtin_amdgcn_readlane(w.count, l), __builtin_amdgcn_readlane(w.first, l), __builtin_amdgcn_readlane(w.slope, l)};
-            const int64_t start = lane_value(end - mine, l), per_head = k.before(k.count);
-            const int64_t in = at - start;
-            u.head = (int)(in / per_head);
-            const int64_t x = in - u.head * per_head;
-            int64_t j;
-            if (k.slope == 0) {
-                j = x / k.first;
-            } else {      // first j + slope j (j - 1) / 2 <= x
-                const double b = k.first - 0.5 * k.slope;
-                j = (int64_t)((sqrt(b * b + 2. * k.slope * (double)x) - b) / k.slope);
-                j = min(max(j, (int64_t)0), (int64_t)k.count - 1);
-                while (j > 0 && k.before(j) > x) --j;
-                while (j + 1 < k.count && k.before(j + 1) <= x) ++j;
+template <int ROWS, int TILE, class Args>
+__device__ __forceinline__ CachedUnit find_unit(const Args& a, const Line& line, uint32_t at) {
+    CachedUnit u{0, 0, 0, 0, 0, 0, 0, 0, 0};
+    SampleWork k = line.w;
+    uint32_t base = 0;
+    if (a.samples > 1) {
+        SampleWork w = line.w;
+        uint32_t end = line.end, mine = 0;
+        uint64_t found = 0;
+        for (int s0 = 0; s0 < a.samples; s0 += 64) {
+            if (a.samples > 64) {
+                w = sample_work<ROWS, TILE>(a, s0 + (threadIdx.x & 63));
+                end = base + scan64(w.before(w.count) * a.cache.heads);
             }
-            j = uniform(j);
-            u.first_row = (int)j * ROWS;
-            u.begin = start + u.head * per_head + k.before(j);
-            u.end = u.begin + k.first + k.slope * j;
-            u.tiles = unit_tiles<ROWS, TILE>(a, u.lq, u.lk, (int)j);
-            return u;
+            mine = w.before(w.count) * a.cache.heads;
+            found = __ballot(at >= end - mine && at < end);
+            u.sample = s0;
+            if (found) break;
+            base = __builtin_amdgcn_readlane(end, 63);
         }
-        base = lane_value(end, 63);
+        const int l = found ? __builtin_ctzll(found) : 0;      // (there is one: `at` is below the line's length)
+        auto of = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane(x, l); };
+        k = SampleWork{(int)of(w.row0), (int)of(w.lq), (int)of(w.lk), (int)of(w.count), of(w.first), of(w.slope)};
+        base = of(end - mine);
+        u.sample += l;
     }
+    u.row0 = k.row0, u.lq = k.lq, u.lk = k.lk;
+    const uint32_t per_head = k.before(k.count), in = at - base;
+    const uint32_t head = in / per_head, x = in - head * per_head;
+    u.head = (int)head;
+    uint32_t j = 0;
+    if (k.count > 1) {
+        if (k.slope == 0) {
+            j = x / k.first;
+        } else {      // first j + slope j (j - 1) / 2 <= x
+            const float b = (float)k.first - 0.5f * (float)k.slope;
+            j = (uint32_t)max((int)((sqrtf(b * b + 2.f * (float)k.slope * (float)x) - b) / (float)k.slope), 0);
+            j = min(j, (uint32_t)k.count - 1);
+            while (j > 0 && k.before(j) > x) --j;
+            while (j + 1 < (uint32_t)k.count && k.before(j + 1) <= x) ++j;
+        }
+        j = __builtin_amdgcn_readfirstlane(j);
+    }
+    u.first_row = (int)j * ROWS;
+    u.begin = base + head * per_head + k.before(j);
+    u.end = u.begin + k.first + k.slope * j;
+    u.tiles = unit_tiles<ROWS, TILE>(a, u.lq, u.lk, (int)j);
     return u;
 }
-
-// Workgroups that share the line, and where the w-th begins.
-__device__ __forceinline__ int64_t line_groups(const CachedArgs& a, int64_t length) { return min((int64_t)a.groups, max((int64_t)1, length / a.least)); }
-__device__ __forceinline__ int64_t line_cut(int64_t length, int64_t groups, int64_t w) { return length * w / groups; }
-// The workgroup that holds a place.
-__device__ __forceinline__ int64_t line_group(int64_t length, int64_t groups, int64_t at) { return ((at + 1) * groups - 1) / length; }
 
 // One workgroup's piece of a unit: tiles [t0, t1) of it, and its place in the workspace (-1: it has all of the unit).
 struct CachedPiece {
     int t0, t1, slot;
 };
-__device__ __forceinline__ CachedPiece cut_unit(const CachedUnit& u, int64_t from, int64_t to, int w) {
-    const int64_t lo = max(from, u.begin) - u.begin, hi = min(to, u.end) - u.begin, weight = u.end - u.begin;
-    CachedPiece p;
-    p.t0 = (int)(u.tiles * lo / weight);
-    p.t1 = (int)(u.tiles * hi / weight);
-    p.slot = lo == 0 && hi == weight ? -1 : 2 * w + (lo == 0);
-    return p;
+__device__ __forceinline__ CachedPiece cut_unit(const CachedUnit& u, uint32_t from, uint32_t to, int w) {
+    const uint32_t lo = max(from, u.begin) - u.begin, hi = min(to, u.end) - u.begin, weight = u.end - u.begin;
+    // (a place of the line is one tile, whichever workgroup asks: the products are the same and grow with it)
+    const float each = (float)u.tiles / (float)weight;
+    auto tile = [&](uint32_t x) { return (uint32_t)u.tiles == weight ? (int)x : x == weight ? u.tiles : min((int)((float)x * each), u.tiles); };
+    return CachedPiece{tile(lo), tile(hi), lo == 0 && hi == weight ? -1 : 2 * w + (lo == 0)};
 }
-// What the join has to know of a workgroup's last unit (one thread).
-__device__ __forceinline__ void tell_join(const CachedArgs& a, const CachedUnit& u, int64_t to, int64_t length, int64_t groups, int w, bool begins) {
+// What the join has to know of a workgroup's last unit.
+template <class Args>
+__device__ __forceinline__ void tell_join(const Args& a, const CachedUnit& u, const Line& line, uint32_t to, int w, bool begins) {
     JoinItem j{};
-    if (begins && u.end > to) j = JoinItem{u.lq * a.share - u.first_row, u.first_row, u.row0, u.head, (int)line_group(length, groups, u.end - 1), {}};
-    a.join[w] = j;
+    if (begins && u.end > to) j = JoinItem{u.lq * a.share - u.first_row, u.first_row, u.row0, u.head, line.group(u.end - 1), {}};
+    if (threadIdx.x == 0) a.join[w] = j;
 }
 
 // Four bytes of codes as eight 16-bit values.
@@ -201,6 +224,13 @@ __device__ __forceinline__ f32x4_t mfma16(const u32x4_t& a, const u32x4_t& b, co
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// The largest of a value over the four lanes 16 apart.
+__device__ __forceinline__ float max_over_groups(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const float2 h = both_halves(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+    return fmaxf(h.x, h.y);
 }
 
 // Byte offset of a 16-byte piece of V in a staged tile: as v_piece, and the piece's lowest bit xored with the key's, so
@@ -230,44 +260,49 @@ __device__ __forceinline__ float value16(uint32_t b) { return BF16 ? bf16_bits_t
 // ---- few rows ------------------------------------------------------------------------------------------------------
 // NB: blocks of 32 channels a head; MX4: 4-bit pages; RT: tiles of 16 rows.
 template <bool BF16, int NB, bool MX4, int RT>
-__global__ __launch_bounds__(CF_NW * 64) void k_cached_few(CachedArgs a) {
+__global__ __launch_bounds__(CF_NW * 64, 2) void k_cached_few(CachedArgs) {
+#ifdef __HIP_DEVICE_COMPILE__
     constexpr int DP = NB * 32, ROWS = RT * 16, DB = NB * 2;
     constexpr int VP = MX4 ? NB : NB * 4;                        // 16-byte pieces of a key's V in the page
-    constexpr int VL = (CF_KEYS * VP + 63) / 64;                 // loads of them a lane
+    constexpr int VL = (16 * VP + 63) / 64;                      // loads of them a lane, for 16 keys
     constexpr int V_BYTES = CF_KEYS * DP * 2, O_BYTES = ROWS * DP * 4;
     __shared__ __attribute__((aligned(16))) char sBuf[CF_NW][V_BYTES > O_BYTES ? V_BYTES : O_BYTES];
     __shared__ float2 sStat[CF_NW][ROWS];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
     char* sV = sBuf[wave];
-    const KvArgs& kv = a.cache;
-    const int64_t length = line_length<ROWS, CF_KEYS>(a), groups = line_groups(a, length);
-    if (length == 0 || (int)blockIdx.x >= groups) {
-        if (threadIdx.x == 0) a.join[blockIdx.x].rows = 0;
+    const Line line = make_line<ROWS, CF_KEYS>(*reread_args());
+    const uint32_t to = line.cut(blockIdx.x + 1);
+    if (line.cut(blockIdx.x) >= to) {
+        if (threadIdx.x == 0) reread_args()->join[blockIdx.x].rows = 0;
         return;
     }
-    const int64_t to = line_cut(length, groups, blockIdx.x + 1);
-    const int page_mask = (1 << kv.page_bits) - 1;
     constexpr float LAG = BF16 ? 8.f : 4.f, LIFT = BF16 ? 0.f : 11.f;
 
-    for (int64_t from = line_cut(length, groups, blockIdx.x); from < to;) {
-        const CachedUnit u = find_unit<ROWS, CF_KEYS>(a, from);
+    for (uint32_t from = line.cut(blockIdx.x); from < to;) {
+        const auto& a = *reread_args();
+        const CachedUnit u = find_unit<ROWS, CF_KEYS>(a, line, from);
         const CachedPiece piece = cut_unit(u, from, to, blockIdx.x);
-        if (threadIdx.x == 0 && u.end >= to) tell_join(a, u, to, length, groups, blockIdx.x, from <= u.begin);
+        if (u.end >= to) tell_join(a, u, line, to, blockIdx.x, from <= u.begin);
         from = u.end;
         const int rows = u.lq * a.share;
+        const FastDiv by_share{a.by_share.mul, a.by_share.shift};
+        // (what the loop needs)
+        const int page_bits = a.cache.page_bits, page_mask = (1 << page_bits) - 1, pool = a.cache.pages, d = a.cache.d, lk = u.lk;
+        const int64_t page_bytes = a.cache.page_bytes;
+        const float scale2 = a.scale2;
         // rows past the sample's last are copies of it that are not stored
         int limit[RT];
         u32x4_t qf[RT][NB];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            const int r = min(u.first_row + rt * 16 + r16, rows - 1), qi = r / a.by_share, hq = u.head * a.share + r - qi * a.share;
+            const int r = min(u.first_row + rt * 16 + r16, rows - 1), qi = r / by_share, hq = u.head * a.share + r - qi * a.share;
             limit[rt] = cached_limit(a.causal, u.lq, u.lk, qi);
             const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (int64_t)(u.row0 + qi) * a.q_row + hq * a.q_head;
             // chunk c = NB g + i of eight channels
 #pragma unroll
-            for (int i = 0; i < NB; ++i) qf[rt][i] = (NB * g + i) * 8 < kv.d ? *reinterpret_cast<const u32x4_t*>(qp + (NB * g + i) * 8) : u32x4_t{0, 0, 0, 0};
+            for (int i = 0; i < NB; ++i) qf[rt][i] = (NB * g + i) * 8 < d ? *reinterpret_cast<const u32x4_t*>(qp + (NB * g + i) * 8) : u32x4_t{0, 0, 0, 0};
         }
-        const int all_see = cached_limit(a.causal, u.lq, u.lk, u.first_row / a.by_share);      // (the first row sees least)
+        const int all_see = cached_limit(a.causal, u.lq, u.lk, u.first_row / by_share);      // (the first row sees least)
         f32x4_t o[RT][DB];
         float m[RT], l[RT];
         bool seen[RT];
@@ -277,83 +312,99 @@ __global__ __launch_bounds__(CF_NW * 64) void k_cached_few(CachedArgs a) {
 #pragma unroll
             for (int db = 0; db < DB; ++db) o[rt][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         }
-        // What a tile's keys are loaded into: K's chunks as they are read, V's pieces.
+        // What a tile's two runs of 16 keys are loaded into: K's chunks as they are read, V's pieces.
         struct Raw {
-            u32x4_t k[2][MX4 ? 1 : NB], v[VL];
-            uint32_t kp[2][MX4 && NB == 3 ? 2 : 1], vp[MX4 ? VL : 1];
-            bool held[2];
+            u32x4_t k[2][MX4 ? 1 : NB], v[2][VL];
+            uint32_t kp[2][MX4 && NB == 3 ? 2 : 1], vp[2];
+        } w;
+        // Their pages (-1: none), by scalar loads.
+        const auto table = (const __attribute__((address_space(4))) int32_t*)(a.cache.table + (int64_t)u.sample * a.cache.max_pages);
+        struct Pages {
+            int p[2];
         };
-        auto load = [&](int tile, Raw& w) __attribute__((always_inline)) {
-            const uint8_t* head[2];
-            int slot[2];
+        auto pages_of = [&](int tile) __attribute__((always_inline)) {
+            Pages pages;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
-                const int key = tile * CF_KEYS + kb * 16;
-                head[kb] = key < u.lk ? kv_head(kv, u.sample, key, u.head) : nullptr;
-                w.held[kb] = head[kb] != nullptr;
-                slot[kb] = key & page_mask;
-                const int at = slot[kb] + r16;
-                if constexpr (MX4) {
-                    u32x4_t c{0, 0, 0, 0};
-                    w.kp[kb][0] = 0;
-                    if constexpr (NB == 3) w.kp[kb][1] = 0;
-                    if (head[kb]) {
-                        const uint8_t *p = head[kb] + kv_codes_at(kv, 0, at) + 4 * NB * g, *pw = head[kb] + kv_powers_at(kv, 0, at);
-                        if constexpr (NB == 4) c = *reinterpret_cast<const u32x4_t*>(p);
-                        else
+                const int key = __builtin_amdgcn_readfirstlane(tile * CF_KEYS + kb * 16);
+                pages.p[kb] = key < lk && tile < piece.t1 ? table[key >> page_bits] : -1;
+            }
+            return pages;
+        };
+        auto held = [&](const Pages& pages, int kb) __attribute__((always_inline)) { return (unsigned)pages.p[kb] < (unsigned)pool; };
+        // Within a head's bytes of a page: a lane's first byte of K and of V, and of their powers, at a run's slot 0.
+        const uint8_t* const head = a.cache.data + u.head * a.cache.head_bytes;
+        const int row_bytes = MX4 ? 16 * NB : d * 2;
+        const int k_at = r16 * row_bytes + (MX4 ? 4 * NB : 16 * NB) * g, v_key = lane / VP, v_piece_of = lane % VP;
+        const int v_at = v_key * row_bytes + v_piece_of * 16 + (row_bytes << page_bits);
+        const int kp_at = (2 * row_bytes << page_bits) + r16 * NB + NB * g / 4, vp_at = ((2 * row_bytes + NB) << page_bits) + lane;
+        auto load = [&](int tile, const Pages& pages) __attribute__((always_inline)) {
 #pragma unroll
-                            for (int i = 0; i < NB; ++i) c[i] = *reinterpret_cast<const uint32_t*>(p + 4 * i);
-                        w.kp[kb][0] = pw[NB * g / 4];
-                        if constexpr (NB == 3) w.kp[kb][1] = pw[(NB * g + 2) / 4];
+            for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+                for (int i = 0; i < (MX4 ? 1 : NB); ++i) w.k[kb][i] = u32x4_t{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < VL; ++i) w.v[kb][i] = u32x4_t{0, 0, 0, 0};
+                w.kp[kb][0] = w.vp[kb] = 0;
+                if constexpr (MX4 && NB == 3) w.kp[kb][1] = 0;
+                if (!held(pages, kb)) continue;
+                const int key = tile * CF_KEYS + kb * 16, slot = key & page_mask;
+                const uint8_t* const at = head + pages.p[kb] * page_bytes + slot * row_bytes;
+                const int left = lk - key;        // (keys past the sample's last: V zeros, whatever the page holds)
+                if constexpr (MX4) {
+                    if constexpr (NB == 4) w.k[kb][0] = *reinterpret_cast<const u32x4_t*>(at + k_at);
+                    else
+#pragma unroll
+                        for (int i = 0; i < NB; ++i) w.k[kb][0][i] = *reinterpret_cast<const uint32_t*>(at + k_at + 4 * i);
+                    const uint8_t* const power = at - slot * (row_bytes - NB);
+                    w.kp[kb][0] = power[kp_at];
+                    if constexpr (NB == 3) w.kp[kb][1] = power[kp_at + (NB * g + 2) / 4 - NB * g / 4];
+                    if (lane < 16 * VP && v_key < left) {
+                        w.v[kb][0] = *reinterpret_cast<const u32x4_t*>(at + v_at);
+                        w.vp[kb] = power[vp_at];
                     }
-                    w.k[kb][0] = c;
                 } else {
 #pragma unroll
-                    for (int i = 0; i < NB; ++i) {
-                        w.k[kb][i] = u32x4_t{0, 0, 0, 0};
-                        if (head[kb] && (NB * g + i) * 8 < kv.d)
-                            w.k[kb][i] = *reinterpret_cast<const u32x4_t*>(head[kb] + ((int64_t)at * kv.d + (NB * g + i) * 8) * 2);
-                    }
-                }
-            }
+                    for (int i = 0; i < NB; ++i)
+                        if ((NB * g + i) * 8 < d) w.k[kb][i] = *reinterpret_cast<const u32x4_t*>(at + k_at + 16 * i);
 #pragma unroll
-            for (int i = 0; i < VL; ++i) {
-                const int idx = i * 64 + lane, key = idx / VP, p = idx % VP;
-                const uint8_t* from_head = key < 16 ? head[0] : head[1];
-                const int at = (key < 16 ? slot[0] : slot[1]) + (key & 15);
-                w.v[i] = u32x4_t{0, 0, 0, 0};
-                if constexpr (MX4) w.vp[i] = 0;
-                // (keys past the sample's last: zeros, whatever the page holds)
-                if (key < CF_KEYS && from_head && tile * CF_KEYS + key < u.lk && (MX4 || p * 8 < kv.d)) {
-                    if constexpr (MX4) {
-                        w.v[i] = *reinterpret_cast<const u32x4_t*>(from_head + kv_codes_at(kv, 1, at) + p * 16);
-                        w.vp[i] = from_head[kv_powers_at(kv, 1, at) + p];
-                    } else {
-                        w.v[i] = *reinterpret_cast<const u32x4_t*>(from_head + ((int64_t)((1 << kv.page_bits) + at) * kv.d + p * 8) * 2);
+                    for (int i = 0; i < VL; ++i) {
+                        const int idx = i * 64 + lane, in = idx / VP, p = idx % VP;
+                        if (in < 16 && in < left && p * 8 < d)
+                            w.v[kb][i] = *reinterpret_cast<const u32x4_t*>(at + (row_bytes << page_bits) + in * row_bytes + p * 16);
                     }
                 }
             }
         };
-        auto attend = [&](int tile, const Raw& w) __attribute__((always_inline)) {
+        // The tile whose keys have been loaded; the next one's loads go out once they have been used.
+        auto attend = [&](int tile, const Pages& pages, const Pages& next) __attribute__((always_inline)) {
             const int base = tile * CF_KEYS;
-            // V to LDS, as 16-bit values
+            const bool held0 = held(pages, 0), held1 = held(pages, 1);
+            // V to LDS, as 16-bit values. (Places that differ in a few bits are formed where they are used: kept from tile to
+            // tile they would take the registers of two more waves.)
             bool odd = false;
 #pragma unroll
-            for (int i = 0; i < VL; ++i) {
-                const int idx = i * 64 + lane, key = idx / VP, p = idx % VP;
-                if (CF_KEYS * VP % 64 && key >= CF_KEYS) continue;
+            for (int kb = 0; kb < 2; ++kb) {
                 if constexpr (MX4) {
-                    const float s = mx_scale(w.vp[i]);
-                    odd |= w.vp[i] == 255;
+                    if (16 * VP < 64 && lane >= 16 * VP) continue;
+                    const float s = mx_scale(w.vp[kb]);
+                    odd |= w.vp[kb] == 255;
+                    int to = cv_piece<DP>(v_key, v_piece_of * 4);
+                    asm volatile("" : "+v"(to));
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const u32x4_t x = widen4<BF16>(w.v[i][j], s);
+                        const u32x4_t x = widen4<BF16>(w.v[kb][0][j], s);
                         if constexpr (!BF16) odd |= any_nonfinite<BF16>(x);
-                        *reinterpret_cast<u32x4_t*>(sV + cv_piece<DP>(key, p * 4 + j)) = x;
+                        *reinterpret_cast<u32x4_t*>(sV + kb * 16 * DP * 2 + (to ^ (j * 16))) = x;
                     }
                 } else {
-                    odd |= any_nonfinite<BF16>(w.v[i]);
-                    *reinterpret_cast<u32x4_t*>(sV + cv_piece<DP>(key, p)) = w.v[i];
+#pragma unroll
+                    for (int i = 0; i < VL; ++i) {
+                        const int idx = i * 64 + lane, in = idx / VP, p = idx % VP;
+                        if (16 * VP % 64 && in >= 16) continue;
+                        odd |= any_nonfinite<BF16>(w.v[kb][i]);
+                        *reinterpret_cast<u32x4_t*>(sV + kb * 16 * DP * 2 + cv_piece<DP>(in, p)) = w.v[kb][i];
+                    }
                 }
             }
             // scores: s[rt][kb][i] is key 16 kb + 4 g + i
@@ -371,7 +422,8 @@ __global__ __launch_bounds__(CF_NW * 64) void k_cached_few(CachedArgs a) {
                     for (int rt = 0; rt < RT; ++rt) s[rt][kb] = mfma16<BF16>(k, qf[rt][i], s[rt][kb]);
                 }
             }
-            const bool whole = base + CF_KEYS <= all_see && w.held[0] && w.held[1];
+            if (tile + CF_NW < piece.t1) load(tile + CF_NW, next);
+            const bool whole = base + CF_KEYS <= all_see && held0 && held1;
             u32x4_t pf[RT];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
@@ -382,18 +434,17 @@ __global__ __launch_bounds__(CF_NW * 64) void k_cached_few(CachedArgs a) {
                     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const bool sees = w.held[kb] && base + kb * 16 + 4 * g + i < limit[rt];
+                            const bool sees = (kb ? held1 : held0) && base + kb * 16 + 4 * g + i < limit[rt];
                             seen[rt] |= sees;
                             s[rt][kb][i] = sees ? s[rt][kb][i] : -INFINITY;
                         }
                 }
                 float mt = fmaxf(fmaxf(fmaxf(s[rt][0][0], s[rt][0][1]), fmaxf(s[rt][0][2], s[rt][0][3])),
                                  fmaxf(fmaxf(s[rt][1][0], s[rt][1][1]), fmaxf(s[rt][1][2], s[rt][1][3])));
-                mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-                mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+                mt = max_over_groups(mt);
                 // (the maximum moves where a row's has grown by a factor of 2^LAG alone; p has room for that)
-                if (__any((mt - m[rt]) * a.scale2 > LAG)) {
-                    const float mn = fmaxf(m[rt], mt), corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[rt] - mn) * a.scale2);
+                if (__any((mt - m[rt]) * scale2 > LAG)) {
+                    const float mn = fmaxf(m[rt], mt), corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[rt] - mn) * scale2);
                     m[rt] = mn;
                     l[rt] *= corr;
 #pragma unroll
@@ -406,7 +457,7 @@ __global__ __launch_bounds__(CF_NW * 64) void k_cached_few(CachedArgs a) {
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[rt][kb][i] = __builtin_amdgcn_exp2f(fmaf(s[rt][kb][i] - top, a.scale2, LIFT));
+                    for (int i = 0; i < 4; ++i) s[rt][kb][i] = __builtin_amdgcn_exp2f(fmaf(s[rt][kb][i] - top, scale2, LIFT));
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         pf[rt][2 * kb + i] = pack2<BF16>(s[rt][kb][2 * i], s[rt][kb][2 * i + 1]);
@@ -419,21 +470,35 @@ __global__ __launch_bounds__(CF_NW * 64) void k_cached_few(CachedArgs a) {
             __builtin_amdgcn_wave_barrier();
             // A probability of zero must not meet an Inf or a NaN of a key that its row does not see.
             odd = !whole && __any(odd);
+            int from_v = cv_piece<DP>(4 * g + ((lane >> 2) & 3), (lane >> 1) & 1) + (lane & 1) * 8;
+            asm volatile("" : "+v"(from_v));
+            auto values = [&](int db) __attribute__((always_inline)) {
+                const char* const at = sV + (NB == 3 ? from_v + db * 32 : from_v ^ (db * 32));      // (rows of 96 are not swizzled so far)
+                const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)at);
+                const s16x4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(at + 16 * DP * 2));
+                const uint2 ux = __builtin_bit_cast(uint2, x), uy = __builtin_bit_cast(uint2, y);
+                return u32x4_t{ux.x, ux.y, uy.x, uy.y};
+            };
+            if (__builtin_expect(!odd, 1)) {
+#pragma unroll
+                for (int db = 0; db < DB; ++db) {
+                    const u32x4_t v = values(db);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) o[rt][db] = mfma16<BF16>(v, pf[rt], o[rt][db]);
+                }
+                return;
+            }
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
-                const int key = 4 * g + ((lane >> 2) & 3), p = db * 2 + ((lane >> 1) & 1), sub = (lane & 1) * 8;
-                const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(sV + cv_piece<DP>(key, p) + sub));
-                const s16x4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(sV + cv_piece<DP>(key + 16, p) + sub));
-                const uint2 ux = __builtin_bit_cast(uint2, x), uy = __builtin_bit_cast(uint2, y);
-                u32x4_t v{ux.x, ux.y, uy.x, uy.y};
-                if (odd) v = finite_only<BF16>(v);
+                const u32x4_t v = finite_only<BF16>(values(db));
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) o[rt][db] = mfma16<BF16>(v, pf[rt], o[rt][db]);
+                __builtin_amdgcn_sched_barrier(0);      // (one operand at a time: registers)
             }
-            if (odd) {      // the values left out, key by key, for the rows that see them
+            // the values left out, key by key, for the rows that see them
+            {
                 for (int key = 0; key < CF_KEYS; ++key) {
-                    const bool held = key < 16 ? w.held[0] : w.held[1];
-                    if (!held) continue;
+                    if (!(key < 16 ? held0 : held1)) continue;
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) {
                         float p = 0.f;
@@ -444,13 +509,16 @@ __global__ __launch_bounds__(CF_NW * 64) void k_cached_few(CachedArgs a) {
                         }
                         p = __shfl(p, (key & 12) * 4 + r16, 64);
                         const bool sees = base + key < limit[rt];
+                        int at = 4 * g;
+                        asm volatile("" : "+v"(at));
 #pragma unroll
                         for (int db = 0; db < DB; ++db)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
-                                const int e = db * 16 + 4 * g + i;
+                                const int e = db * 16 + at + i;
                                 const uint32_t b = *reinterpret_cast<const uint16_t*>(sV + cv_piece<DP>(key, e >> 3) + (e & 7) * 2);
                                 if (sees && nonfinite16<BF16>(b)) o[rt][db][i] += p * value16<BF16>(b);
+                                __builtin_amdgcn_sched_barrier(0);
                             }
                     }
                 }
@@ -458,15 +526,17 @@ __global__ __launch_bounds__(CF_NW * 64) void k_cached_few(CachedArgs a) {
         };
         int tile = piece.t0 + wave;
         if (tile < piece.t1) {
-            Raw next;
-            load(tile, next);
+            Pages now = pages_of(tile), next = pages_of(tile + CF_NW);
+            load(tile, now);
             for (; tile < piece.t1; tile += CF_NW) {
-                const Raw now = next;
-                if (tile + CF_NW < piece.t1) load(tile + CF_NW, next);
-                attend(tile, now);
+                const Pages after = pages_of(tile + 2 * CF_NW);
+                attend(tile, now, next);
+                now = next;
+                next = after;
             }
         }
         // the waves' rows joined
+        const auto& b = *reread_args();
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             l[rt] += __shfl_xor(l[rt], 16, 64);
@@ -482,7 +552,7 @@ __global__ __launch_bounds__(CF_NW * 64) void k_cached_few(CachedArgs a) {
         __syncthreads();
         for (int item = threadIdx.x; item < ROWS * (DP / 4); item += CF_NW * 64) {
             const int row = item / (DP / 4), e = item % (DP / 4) * 4, r = u.first_row + row;
-            if (r >= rows || e >= kv.d) continue;
+            if (r >= rows || e >= b.cache.d) continue;
             float top = -INFINITY;
 #pragma unroll
             for (int w = 0; w < CF_NW; ++w) top = fmaxf(top, sStat[w][row].y == -1.f ? -INFINITY : sStat[w][row].x);
@@ -494,7 +564,7 @@ __global__ __launch_bounds__(CF_NW * 64) void k_cached_few(CachedArgs a) {
                 const float2 st = sStat[w][row];
                 if (st.y == -1.f) continue;
                 any = true;
-                const float c = st.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st.x - top) * a.scale2);
+                const float c = st.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st.x - top) * b.scale2);
                 sum += c * st.y;
                 const f32x4_t x = *reinterpret_cast<const f32x4_t*>(sBuf[w] + (row * DP + (e ^ ((row & 7) * 4))) * 4);
 #pragma unroll
@@ -502,17 +572,18 @@ __global__ __launch_bounds__(CF_NW * 64) void k_cached_few(CachedArgs a) {
             }
             if (piece.slot >= 0) {
                 const int64_t at = (int64_t)piece.slot * ROWS + row;
-                if (e == 0) a.stat[at] = float2{top, any ? sum : -1.f};
-                *reinterpret_cast<f32x4_t*>(a.part + at * kv.d + e) = acc;
+                if (e == 0) b.stat[at] = float2{top, any ? sum : -1.f};
+                *reinterpret_cast<f32x4_t*>(b.part + at * b.cache.d + e) = acc;
             } else {
                 const float inv = any ? 1.f / sum : 0.f;
-                const int qi = r / a.by_share, hq = u.head * a.share + r - qi * a.share;
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + (int64_t)(u.row0 + qi) * a.o_row + hq * a.o_head + e) =
+                const int qi = r / FastDiv{b.by_share.mul, b.by_share.shift}, hq = u.head * b.share + r - qi * b.share;
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(b.o) + (int64_t)(u.row0 + qi) * b.o_row + hq * b.o_head + e) =
                     uint2{pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv)};
             }
         }
         __syncthreads();
     }
+#endif
 }
 
 // ---- many rows -----------------------------------------------------------------------------------------------------
@@ -524,20 +595,20 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 ? 2 : 1) void k_cached_many(CachedA
     __shared__ __attribute__((aligned(16))) char sK0[TILE], sK1[TILE], sV0[TILE], sV1[TILE];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
     const KvArgs& kv = a.cache;
-    const int64_t length = line_length<CM_ROWS, CM_KEYS>(a), groups = line_groups(a, length);
-    if (length == 0 || (int)blockIdx.x >= groups) {
+    const Line line = make_line<CM_ROWS, CM_KEYS>(a);
+    const uint32_t to = line.cut(blockIdx.x + 1);
+    if (line.cut(blockIdx.x) >= to) {
         if (threadIdx.x == 0) a.join[blockIdx.x].rows = 0;
         return;
     }
-    const int64_t to = line_cut(length, groups, blockIdx.x + 1);
     const int page_mask = (1 << kv.page_bits) - 1;
     constexpr float LAG = BF16 ? 8.f : 4.f, LIFT = BF16 ? 0.f : 11.f, FAR = 1024.f;
     const float scale2 = a.scale2;
 
-    for (int64_t from = line_cut(length, groups, blockIdx.x); from < to;) {
-        const CachedUnit u = find_unit<CM_ROWS, CM_KEYS>(a, from);
+    for (uint32_t from = line.cut(blockIdx.x); from < to;) {
+        const CachedUnit u = find_unit<CM_ROWS, CM_KEYS>(a, line, from);
         const CachedPiece piece = cut_unit(u, from, to, blockIdx.x);
-        if (threadIdx.x == 0 && u.end >= to) tell_join(a, u, to, length, groups, blockIdx.x, from <= u.begin);
+        if (u.end >= to) tell_join(a, u, line, to, blockIdx.x, from <= u.begin);
         from = u.end;
         const int rows = u.lq * a.share;
         // rows past the sample's last are copies of it that are not stored
@@ -959,20 +1030,23 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // How a call is cut: the rows of a unit, the workgroups. Few rows are those that fit a unit of 32 in the mean (the host
 // does not know the lengths).
 struct CachedCut {
-    int rows, groups, least;
+    int rows, least, shift;
+    int64_t units;         // at most
     bool many_pieces;      // of a unit
 };
-CachedCut cached_cut(int64_t nq, int samples, int hkv, int share) {
+CachedCut cached_cut(int64_t nq, int samples, int hkv, int share, int64_t keys) {
     CachedCut c;
     const int64_t each = ceil_div(nq, samples) * share;
     c.rows = each <= 16 ? 16 : each <= 32 ? 32 : CM_ROWS;
-    c.groups = 512;      // two a CU
-    c.least = c.rows == CM_ROWS ? 4 : CF_NW;
-    c.many_pieces = c.groups > 32 * ceil_div(nq * share, c.rows) * hkv;
+    c.units = (ceil_div(nq * share, c.rows) + (samples > 1 ? samples : 0)) * hkv;
+    c.shift = 0;      // the line is shorter than 2^30
+    while (c.shift < 30 && c.units * ((ceil_div(keys, c.rows == CM_ROWS ? CM_KEYS : CF_KEYS) >> c.shift) + 1) >= 1ll << 30) ++c.shift;
+    c.least = std::max(1, (c.rows == CM_ROWS ? 4 : CF_NW) >> c.shift);
+    c.many_pieces = kGroups > 32 * ceil_div(nq * share, c.rows) * hkv;
     return c;
 }
 size_t cached_workspace(const CachedCut& c, int d) {
-    return (size_t)c.groups * (2 * c.rows * (d * sizeof(float) + sizeof(float2)) + sizeof(JoinItem));
+    return (size_t)kGroups * (2 * c.rows * (d * sizeof(float) + sizeof(float2)) + sizeof(JoinItem));
 }
 
 }  // namespace
@@ -982,7 +1056,7 @@ using namespace tsp;
 
 extern "C" size_t tsp_attention_cached_workspace_bytes(int64_t nq, int samples, int hq, const tsp_kv_cache* cache, int max_pages) {
     if (!cache || !kv_valid(*cache) || nq <= 0 || nq >= (1ll << 31) || samples <= 0 || hq <= 0 || hq % cache->heads || max_pages <= 0) return 0;
-    return cached_workspace(cached_cut(nq, samples, cache->heads, hq / cache->heads), cache->d);
+    return cached_workspace(cached_cut(nq, samples, cache->heads, hq / cache->heads, (int64_t)max_pages * cache->page), cache->d);
 }
 
 extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, int hq, const tsp_kv_cache* cache, const int32_t* d_offsets,
@@ -1012,21 +1086,22 @@ extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, i
                 "tsp_attention_cached: out must not alias q or the cache");
     const int share = hq / c.heads;
     TSP_REQUIRE(nq * share < (1ll << 31) - 1024, TSP_ERR_INVALID, "tsp_attention_cached: too many rows");
-    const CachedCut cut = cached_cut(nq, samples, c.heads, share);
+    const CachedCut cut = cached_cut(nq, samples, c.heads, share, (int64_t)max_pages * c.page);
+    TSP_REQUIRE(cut.units < 1ll << 29, TSP_ERR_INVALID, "tsp_attention_cached: too many rows and heads");
     const size_t need = cached_workspace(cut, c.d);
     TSP_REQUIRE(d_workspace, TSP_ERR_INVALID, "tsp_attention_cached: null workspace");
     TSP_REQUIRE(workspace_bytes >= need, TSP_ERR_WORKSPACE, "tsp_attention_cached: workspace of %zu bytes, needs %zu", workspace_bytes, need);
     TSP_REQUIRE(reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0, TSP_ERR_INVALID, "tsp_attention_cached: workspace not 16-byte aligned");
     float* part = static_cast<float*>(d_workspace);
-    float2* stat = reinterpret_cast<float2*>(part + (size_t)cut.groups * 2 * cut.rows * c.d);
+    float2* stat = reinterpret_cast<float2*>(part + (size_t)kGroups * 2 * cut.rows * c.d);
     const CachedArgs a{q->data, out->data, q->row_stride, q->head_stride, out->row_stride, out->head_stride, kv_args(c, d_table, max_pages, d_lengths),
-                       d_offsets, nq, samples, share, causal ? 1 : 0, cut.groups, cut.least, fast_div((uint32_t)share), scale * kLog2e, part, stat,
-                       reinterpret_cast<JoinItem*>(stat + (size_t)cut.groups * 2 * cut.rows)};
+                       d_offsets, nq, samples, share, causal ? 1 : 0, cut.least, cut.shift, fast_div((uint32_t)share), scale * kLog2e, part, stat,
+                       reinterpret_cast<JoinItem*>(stat + (size_t)kGroups * 2 * cut.rows)};
     hipStream_t s = as_stream(stream);
     auto go = [&](auto bf, auto nb, auto mx) {
         constexpr bool BF16 = decltype(bf)::value, MX4 = decltype(mx)::value;
         constexpr int NB = decltype(nb)::value;
-        const dim3 grid((unsigned)cut.groups);
+        const dim3 grid(kGroups);
         if (cut.rows == 16) hipLaunchKernelGGL((k_cached_few<BF16, NB, MX4, 1>), grid, dim3(CF_NW * 64), 0, s, a);
         else if (cut.rows == 32) hipLaunchKernelGGL((k_cached_few<BF16, NB, MX4, 2>), grid, dim3(CF_NW * 64), 0, s, a);
         else hipLaunchKernelGGL((k_cached_many<BF16, NB, MX4>), grid, dim3(CM_NW * 64), 0, s, a);
@@ -1040,7 +1115,7 @@ extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, i
     auto join = [&](auto bf, auto rows) {
         constexpr bool BF16 = decltype(bf)::value;
         constexpr int ROWS = decltype(rows)::value;
-        const unsigned cuts = (unsigned)cut.groups - 1;
+        const unsigned cuts = kGroups - 1;      // (a unit is not cut at the line's end)
         if (cut.many_pieces) hipLaunchKernelGGL((k_cached_join<BF16, ROWS, 16>), dim3(cuts, ROWS), dim3(256), 0, s, a);
         else hipLaunchKernelGGL((k_cached_join<BF16, ROWS, 4>), dim3(cuts, ROWS / 4), dim3(256), 0, s, a);
     };
