@@ -15,7 +15,7 @@
 // a lane holds scores of one row and P is the second product's operand where it stands. Statistics and accumulators are
 // fp32; P is rounded to the heads' type, as the packed attention's (attention.hip) is, and formed as there.
 //
-// Two kernels. Few rows (k_cached_few): waves of their own, each with every eighth tile of 32 keys: K goes from memory to its
+// Two kernels. Few rows (k_cached_few): waves of their own, each with every fourth tile of 32 keys: K goes from memory to its
 // operand, V through a piece of LDS that is the wave's alone, where it is turned. Many rows (k_cached_many): four waves of 32
 // rows share a tile of 64 keys, widened into LDS by all of them.
 #include <algorithm>
@@ -29,7 +29,7 @@
 namespace tsp {
 namespace {
 
-constexpr int CF_KEYS = 32, CF_NW = 8;                               // few rows: keys of a tile, waves
+constexpr int CF_KEYS = 32, CF_NW = 4;                               // few rows: keys of a tile, waves
 constexpr int CM_KEYS = 64, CM_NW = 4, CM_ROWS = CM_NW * 32;         // many
 
 struct CachedArgs {
@@ -40,15 +40,13 @@ struct CachedArgs {
     const int32_t* q_off;
     int64_t nq;                                // below 2^31, nq * share too
     int samples, share, causal;
-    int least, shift;                          // tiles that a workgroup has at least; weights are in 2^shift of them
-    FastDiv by_share;
+    int groups, least, shift;                  // workgroups at most, tiles that one has at least; weights are in 2^shift of them
+    FastDiv by_share, by_groups;
     float scale2;                              // scale * log2(e)
     float* part;                               // [2 * groups][row][d] sums of p v, and
-    float2* stat;                              // [2 * kGroups][row] maximum and sum of p (-1: no key seen), and
-    struct JoinItem* join;                     // [kGroups] the unit that is cut at the workgroup's end and began in it
+    float2* stat;                              // [2 * groups][row] maximum and sum of p (-1: no key seen), and
+    struct JoinItem* join;                     // [groups] the unit that is cut at the workgroup's end and began in it
 };
-
-constexpr int kGroups = 512;      // workgroups, two a CU
 
 // rows left in the unit from its first (0: none), the first, the sample's first row, the key head, the last workgroup.
 struct JoinItem {
@@ -99,13 +97,14 @@ struct Line {
     __device__ __forceinline__ uint32_t cut(int group) const { return min(per * (uint32_t)group, length); }
     __device__ __forceinline__ int group(uint32_t at) const { return (int)(at / per); }
 };
+// The sum over a lane and those before it (moves along a row of 16 lanes, then rows' last lanes to the rows after them).
 __device__ __forceinline__ uint32_t scan64(uint32_t v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t x = __shfl_up(v, o, 64);
-        if (lane >= o) v += x;
-    }
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);      // row_shr 1
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);      // 2
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);      // 4
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);      // 8
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);      // row_bcast 15, to rows 1 and 3
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);      // row_bcast 31, to rows 2 and 3
     return v;
 }
 template <int ROWS, int TILE, class Args>
@@ -122,7 +121,8 @@ __device__ __forceinline__ Line make_line(const Args& a) {
             l.length = __builtin_amdgcn_readlane(l.end, 63);
         }
     }
-    l.per = max((uint32_t)a.least, (l.length + kGroups - 1) / kGroups);
+    l.length = __builtin_amdgcn_readfirstlane(l.length);
+    l.per = max(a.least, (int)(l.length + a.groups - 1) / FastDiv{a.by_groups.mul, a.by_groups.shift});
     return l;
 }
 
@@ -137,7 +137,8 @@ struct CachedUnit {
 template <int ROWS, int TILE, class Args>
 __device__ __forceinline__ CachedUnit find_unit(const Args& a, const Line& line, uint32_t at) {
     CachedUnit u{0, 0, 0, 0, 0, 0, 0, 0, 0};
-    SampleWork k = line.w;
+    auto first = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
+    SampleWork k{(int)first(line.w.row0), (int)first(line.w.lq), (int)first(line.w.lk), (int)first(line.w.count), first(line.w.first), first(line.w.slope)};
     uint32_t base = 0;
     if (a.samples > 1) {
         SampleWork w = line.w;
@@ -162,7 +163,7 @@ __device__ __forceinline__ CachedUnit find_unit(const Args& a, const Line& line,
     }
     u.row0 = k.row0, u.lq = k.lq, u.lk = k.lk;
     const uint32_t per_head = k.before(k.count), in = at - base;
-    const uint32_t head = in / per_head, x = in - head * per_head;
+    const uint32_t head = first(in / per_head), x = in - head * per_head;
     u.head = (int)head;
     uint32_t j = 0;
     if (k.count > 1) {
@@ -175,12 +176,12 @@ __device__ __forceinline__ CachedUnit find_unit(const Args& a, const Line& line,
             while (j > 0 && k.before(j) > x) --j;
             while (j + 1 < (uint32_t)k.count && k.before(j + 1) <= x) ++j;
         }
-        j = __builtin_amdgcn_readfirstlane(j);
+        j = first(j);
     }
     u.first_row = (int)j * ROWS;
     u.begin = base + head * per_head + k.before(j);
     u.end = u.begin + k.first + k.slope * j;
-    u.tiles = unit_tiles<ROWS, TILE>(a, u.lq, u.lk, (int)j);
+    u.tiles = (int)first(unit_tiles<ROWS, TILE>(a, u.lq, u.lk, (int)j));
     return u;
 }
 
@@ -193,7 +194,7 @@ __device__ __forceinline__ CachedPiece cut_unit(const CachedUnit& u, uint32_t fr
     // (a place of the line is one tile, whichever workgroup asks: the products are the same and grow with it)
     const float each = (float)u.tiles / (float)weight;
     auto tile = [&](uint32_t x) { return (uint32_t)u.tiles == weight ? (int)x : x == weight ? u.tiles : min((int)((float)x * each), u.tiles); };
-    return CachedPiece{tile(lo), tile(hi), lo == 0 && hi == weight ? -1 : 2 * w + (lo == 0)};
+    return CachedPiece{__builtin_amdgcn_readfirstlane(tile(lo)), __builtin_amdgcn_readfirstlane(tile(hi)), lo == 0 && hi == weight ? -1 : 2 * w + (lo == 0)};
 }
 // What the join has to know of a workgroup's last unit.
 template <class Args>
@@ -407,6 +408,7 @@ __global__ __launch_bounds__(CF_NW * 64, 2) void k_cached_few(CachedArgs) {
                     }
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);      // (here and below: the registers of two more waves a SIMD)
             // scores: s[rt][kb][i] is key 16 kb + 4 g + i
             f32x4_t s[RT][2];
 #pragma unroll
@@ -421,6 +423,7 @@ __global__ __launch_bounds__(CF_NW * 64, 2) void k_cached_few(CachedArgs) {
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) s[rt][kb] = mfma16<BF16>(k, qf[rt][i], s[rt][kb]);
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
             if (tile + CF_NW < piece.t1) load(tile + CF_NW, next);
             const bool whole = base + CF_KEYS <= all_see && held0 && held1;
@@ -434,7 +437,7 @@ __global__ __launch_bounds__(CF_NW * 64, 2) void k_cached_few(CachedArgs) {
                     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const bool sees = (kb ? held1 : held0) && base + kb * 16 + 4 * g + i < limit[rt];
+                            const bool sees = (kb ? held1 : held0) && kb * 16 + i < limit[rt] - base - 4 * g;
                             seen[rt] |= sees;
                             s[rt][kb][i] = sees ? s[rt][kb][i] : -INFINITY;
                         }
@@ -485,6 +488,7 @@ __global__ __launch_bounds__(CF_NW * 64, 2) void k_cached_few(CachedArgs) {
                     const u32x4_t v = values(db);
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) o[rt][db] = mfma16<BF16>(v, pf[rt], o[rt][db]);
+                    if (db % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                 }
                 return;
             }
@@ -537,6 +541,9 @@ __global__ __launch_bounds__(CF_NW * 64, 2) void k_cached_few(CachedArgs) {
         }
         // the waves' rows joined
         const auto& b = *reread_args();
+        int tid = threadIdx.x;      // (as above: places of its own)
+        asm volatile("" : "+v"(tid));
+        const int row16 = tid & 15, group = tid >> 4 & 3;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             l[rt] += __shfl_xor(l[rt], 16, 64);
@@ -544,13 +551,13 @@ __global__ __launch_bounds__(CF_NW * 64, 2) void k_cached_few(CachedArgs) {
             int any = seen[rt];
             any |= __shfl_xor(any, 16, 64);
             any |= __shfl_xor(any, 32, 64);
-            if (g == 0) sStat[wave][rt * 16 + r16] = float2{m[rt], any ? l[rt] : -1.f};
+            if (group == 0) sStat[wave][rt * 16 + row16] = float2{m[rt], any ? l[rt] : -1.f};
 #pragma unroll
             for (int db = 0; db < DB; ++db)
-                *reinterpret_cast<f32x4_t*>(sV + ((rt * 16 + r16) * DP + ((db * 16 + 4 * g) ^ ((r16 & 7) * 4))) * 4) = o[rt][db];
+                *reinterpret_cast<f32x4_t*>(sV + ((rt * 16 + row16) * DP + ((db * 16 + 4 * group) ^ ((row16 & 7) * 4))) * 4) = o[rt][db];
         }
         __syncthreads();
-        for (int item = threadIdx.x; item < ROWS * (DP / 4); item += CF_NW * 64) {
+        for (int item = tid; item < ROWS * (DP / 4); item += CF_NW * 64) {
             const int row = item / (DP / 4), e = item % (DP / 4) * 4, r = u.first_row + row;
             if (r >= rows || e >= b.cache.d) continue;
             float top = -INFINITY;
@@ -946,18 +953,18 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 ? 2 : 1) void k_cached_many(CachedA
 }
 
 // ---- the pieces of units that were cut, joined -----------------------------------------------------------------------
-// sum_s w_s (p v)_s / sum_s w_s (sum p)_s, w_s = exp(max_s - max), in an order that the pieces' number alone sets. G groups of 16
-// lanes a row, eight channels a lane: 4 (a wave), or 16 where units have many pieces.
+// sum_s w_s (p v)_s / sum_s w_s (sum p)_s, w_s = exp(max_s - max), in an order that the pieces' number alone sets. A workgroup
+// takes 16 / G rows of a unit at a time, G groups of 16 lanes a row, eight channels a lane: one, 4 (a wave), or 16 where units
+// have many pieces. Which units were cut only the device knows: every workgroup counts them (a launch of a workgroup for each
+// place where one can be takes 10 to 30 us, nearly all of which leave at once).
+constexpr int CJ_EACH = 3, CJ_MAX = CJ_EACH * 256;      // workgroups of the first launch, at most
 template <bool BF16, int ROWS, int G>
-__global__ __launch_bounds__(256) void k_cached_join(CachedArgs a) {
-    constexpr int ITEMS = 16 / G, BATCH = 8;
-    __shared__ float sAcc[G == 16 ? 16 : 1][KV_MAX_D], sMax[4], sSum[4];
-    const JoinItem j = a.join[blockIdx.x];
+__device__ __forceinline__ void join_rows(const CachedArgs& a, int g0, int first, float (*sAcc)[KV_MAX_D], float* sMax, float* sSum) {
+    constexpr int BATCH = 8;
     const int group = threadIdx.x >> 4, g = group % G, e = (threadIdx.x & 15) * 8, mine = threadIdx.x % (G * 16);
-    const int row = blockIdx.y * ITEMS + group / G;
-    if ((int)(blockIdx.y * ITEMS) >= j.rows) return;
-    const bool live = row < j.rows;
-    const int g0 = blockIdx.x, pieces = j.last - g0 + 1;
+    const JoinItem j = a.join[g0];
+    const int row = first + group / G, pieces = j.last - g0 + 1;
+    const bool live = row < min(j.rows, ROWS);
     auto at = [&](int i) { return (int64_t)(2 * (g0 + i) + (i == 0)) * ROWS + (live ? row : 0); };
     float top = -INFINITY;
     for (int i = mine; i < pieces; i += G * 16) {
@@ -965,7 +972,7 @@ __global__ __launch_bounds__(256) void k_cached_join(CachedArgs a) {
         if (st.y != -1.f) top = fmaxf(top, st.x);
     }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    for (int o = G == 1 ? 8 : 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
     if constexpr (G == 16) {
         if ((threadIdx.x & 63) == 0) sMax[threadIdx.x >> 6] = top;
         __syncthreads();
@@ -996,8 +1003,10 @@ __global__ __launch_bounds__(256) void k_cached_join(CachedArgs a) {
     }
     // over the groups
     int seen = any;
-    sum += __shfl_xor(sum, 16, 64), seen |= __shfl_xor(seen, 16, 64);
-    sum += __shfl_xor(sum, 32, 64), seen |= __shfl_xor(seen, 32, 64);
+    if constexpr (G > 1) {
+        sum += __shfl_xor(sum, 16, 64), seen |= __shfl_xor(seen, 16, 64);
+        sum += __shfl_xor(sum, 32, 64), seen |= __shfl_xor(seen, 32, 64);
+    }
     if constexpr (G == 16) {
         if ((threadIdx.x & 63) == 0) sSum[threadIdx.x >> 6] = sum;
 #pragma unroll
@@ -1010,7 +1019,7 @@ __global__ __launch_bounds__(256) void k_cached_join(CachedArgs a) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) acc[k] += sAcc[o][e + k];
         }
-    } else {
+    } else if constexpr (G == 4) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             acc[k] += __shfl_xor(acc[k], 16, 64);
@@ -1025,14 +1034,55 @@ __global__ __launch_bounds__(256) void k_cached_join(CachedArgs a) {
     store8<BF16 ? TSP_BF16 : TSP_F16>(a.o, (int64_t)(j.row0 + qi) * a.o_row + hq * a.o_head + e, acc);
 }
 
+template <bool BF16, int ROWS, int G>
+__global__ __launch_bounds__(256) void k_cached_join(CachedArgs a) {
+    constexpr int ITEMS = 16 / G;
+    __shared__ float sAcc[G == 16 ? 16 : 1][KV_MAX_D], sMax[4], sSum[4];
+    __shared__ int sCount[CJ_EACH * 4], sFound[2];
+    const int wave = threadIdx.x >> 6;
+    int count[CJ_EACH], end[CJ_EACH];
+#pragma unroll
+    for (int i = 0; i < CJ_EACH; ++i) {
+        const int w = i * 256 + threadIdx.x;
+        count[i] = w < a.groups ? (min(a.join[w].rows, ROWS) + ITEMS - 1) / ITEMS : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < CJ_EACH; ++i) {
+        end[i] = (int)scan64((uint32_t)count[i]);
+        if ((threadIdx.x & 63) == 63) sCount[i * 4 + wave] = end[i];
+    }
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int i = 0; i < CJ_EACH * 4; ++i) {
+        const int c = sCount[i];
+#pragma unroll
+        for (int k = 0; k < CJ_EACH; ++k)
+            if (i < k * 4 + wave) end[k] += c;
+        total += c;
+    }
+    for (int item = blockIdx.x; item < total; item += gridDim.x) {
+#pragma unroll
+        for (int i = 0; i < CJ_EACH; ++i)
+            if (item < end[i] && item >= end[i] - count[i]) sFound[0] = i * 256 + threadIdx.x, sFound[1] = item - (end[i] - count[i]);
+        __syncthreads();
+        const int g0 = sFound[0], first = sFound[1] * ITEMS;
+        join_rows<BF16, ROWS, G>(a, g0, first, sAcc, sMax, sSum);
+        __syncthreads();
+    }
+}
+
+static_assert(CJ_MAX >= 768, "the join counts every workgroup");
+
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // How a call is cut: the rows of a unit, the workgroups. Few rows are those that fit a unit of 32 in the mean (the host
 // does not know the lengths).
 struct CachedCut {
-    int rows, least, shift;
-    int64_t units;         // at most
-    bool many_pieces;      // of a unit
+    int rows, groups, least, shift;
+    int64_t units;      // at most
+    int join;           // groups of lanes a row in the join
+    unsigned joins;     // its workgroups
 };
 CachedCut cached_cut(int64_t nq, int samples, int hkv, int share, int64_t keys) {
     CachedCut c;
@@ -1040,13 +1090,18 @@ CachedCut cached_cut(int64_t nq, int samples, int hkv, int share, int64_t keys) 
     c.rows = each <= 16 ? 16 : each <= 32 ? 32 : CM_ROWS;
     c.units = (ceil_div(nq * share, c.rows) + (samples > 1 ? samples : 0)) * hkv;
     c.shift = 0;      // the line is shorter than 2^30
-    while (c.shift < 30 && c.units * ((ceil_div(keys, c.rows == CM_ROWS ? CM_KEYS : CF_KEYS) >> c.shift) + 1) >= 1ll << 30) ++c.shift;
-    c.least = std::max(1, (c.rows == CM_ROWS ? 4 : CF_NW) >> c.shift);
-    c.many_pieces = kGroups > 32 * ceil_div(nq * share, c.rows) * hkv;
+    const int64_t tiles = ceil_div(keys, c.rows == CM_ROWS ? CM_KEYS : CF_KEYS);
+    while (c.shift < 30 && c.units * ((tiles >> c.shift) + 1) >= 1ll << 30) ++c.shift;
+    c.least = std::max(1, (c.rows == CM_ROWS ? 4 : 2 * CF_NW) >> c.shift);
+    // two or three a CU, as registers and LDS allow, where the line can be that long
+    c.groups = (int)std::min<int64_t>(c.rows == 16 ? 768 : 512, ceil_div(c.units * ((tiles >> c.shift) + 1), c.least));
+    const int64_t cut = std::min<int64_t>(c.units, c.groups), pieces = c.groups / std::max<int64_t>(1, ceil_div(nq * share, c.rows) * hkv);
+    c.join = pieces > 32 ? 16 : pieces > 2 ? 4 : 1;
+    c.joins = (unsigned)std::min<int64_t>(cut * ceil_div(std::min<int64_t>(each, c.rows), 16 / c.join), 2048);
     return c;
 }
 size_t cached_workspace(const CachedCut& c, int d) {
-    return (size_t)kGroups * (2 * c.rows * (d * sizeof(float) + sizeof(float2)) + sizeof(JoinItem));
+    return (size_t)c.groups * (2 * c.rows * (d * sizeof(float) + sizeof(float2)) + sizeof(JoinItem));
 }
 
 }  // namespace
@@ -1093,15 +1148,16 @@ extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, i
     TSP_REQUIRE(workspace_bytes >= need, TSP_ERR_WORKSPACE, "tsp_attention_cached: workspace of %zu bytes, needs %zu", workspace_bytes, need);
     TSP_REQUIRE(reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0, TSP_ERR_INVALID, "tsp_attention_cached: workspace not 16-byte aligned");
     float* part = static_cast<float*>(d_workspace);
-    float2* stat = reinterpret_cast<float2*>(part + (size_t)kGroups * 2 * cut.rows * c.d);
+    float2* stat = reinterpret_cast<float2*>(part + (size_t)cut.groups * 2 * cut.rows * c.d);
     const CachedArgs a{q->data, out->data, q->row_stride, q->head_stride, out->row_stride, out->head_stride, kv_args(c, d_table, max_pages, d_lengths),
-                       d_offsets, nq, samples, share, causal ? 1 : 0, cut.least, cut.shift, fast_div((uint32_t)share), scale * kLog2e, part, stat,
-                       reinterpret_cast<JoinItem*>(stat + (size_t)kGroups * 2 * cut.rows)};
+                       d_offsets, nq, samples, share, causal ? 1 : 0, cut.groups, cut.least, cut.shift, fast_div((uint32_t)share),
+                       fast_div((uint32_t)cut.groups), scale * kLog2e, part, stat,
+                       reinterpret_cast<JoinItem*>(stat + (size_t)cut.groups * 2 * cut.rows)};
     hipStream_t s = as_stream(stream);
     auto go = [&](auto bf, auto nb, auto mx) {
         constexpr bool BF16 = decltype(bf)::value, MX4 = decltype(mx)::value;
         constexpr int NB = decltype(nb)::value;
-        const dim3 grid(kGroups);
+        const dim3 grid((unsigned)cut.groups);
         if (cut.rows == 16) hipLaunchKernelGGL((k_cached_few<BF16, NB, MX4, 1>), grid, dim3(CF_NW * 64), 0, s, a);
         else if (cut.rows == 32) hipLaunchKernelGGL((k_cached_few<BF16, NB, MX4, 2>), grid, dim3(CF_NW * 64), 0, s, a);
         else hipLaunchKernelGGL((k_cached_many<BF16, NB, MX4>), grid, dim3(CM_NW * 64), 0, s, a);
@@ -1115,9 +1171,11 @@ extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, i
     auto join = [&](auto bf, auto rows) {
         constexpr bool BF16 = decltype(bf)::value;
         constexpr int ROWS = decltype(rows)::value;
-        const unsigned cuts = kGroups - 1;      // (a unit is not cut at the line's end)
-        if (cut.many_pieces) hipLaunchKernelGGL((k_cached_join<BF16, ROWS, 16>), dim3(cuts, ROWS), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((k_cached_join<BF16, ROWS, 4>), dim3(cuts, ROWS / 4), dim3(256), 0, s, a);
+        if (cut.groups == 1) return;
+        const dim3 grid(cut.joins), block(256);
+        if (cut.join == 16) hipLaunchKernelGGL((k_cached_join<BF16, ROWS, 16>), grid, block, 0, s, a);
+        else if (cut.join == 4) hipLaunchKernelGGL((k_cached_join<BF16, ROWS, 4>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((k_cached_join<BF16, ROWS, 1>), grid, block, 0, s, a);
     };
     auto by_type = [&](auto bf) {
         if (c.format == TSP_KV_MX4) by_width(bf, std::true_type{});
