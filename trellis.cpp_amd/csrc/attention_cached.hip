@@ -40,7 +40,7 @@ struct CachedArgs {
     const int32_t* q_off;
     int64_t nq;                                // below 2^31, nq * share too
     int samples, share, causal;
-    int groups, least, shift;                  // workgroups at most, tiles that one has at least; weights are in 2^shift of them
+    int groups, least, finer, coarser;         // workgroups at most, what one has at least; weights are tiles << finer >> coarser
     FastDiv by_share, by_groups;
     float scale2;                              // scale * log2(e)
     float* part;                               // [2 * groups][row][d] sums of p v, and
@@ -84,8 +84,9 @@ __device__ __forceinline__ SampleWork sample_work(const Args& a, int s) {
     w.lk = (int)min((int64_t)max(a.cache.lengths[s], 0), (int64_t)a.cache.max_pages << a.cache.page_bits);
     w.count = (int)((unsigned)(w.lq * a.share + ROWS - 1) / (unsigned)ROWS);
     if (w.count == 0) return w;
-    w.first = max(1, unit_tiles<ROWS, TILE>(a, w.lq, w.lk, 0) >> a.shift);
-    if (w.count > 1) w.slope = (uint32_t)max(0, (unit_tiles<ROWS, TILE>(a, w.lq, w.lk, w.count - 1) >> a.shift) - (int)w.first) / (uint32_t)(w.count - 1);
+    auto weight = [&](int j) { return max(1, (unit_tiles<ROWS, TILE>(a, w.lq, w.lk, j) << a.finer) >> a.coarser); };
+    w.first = weight(0);
+    if (w.count > 1) w.slope = (uint32_t)max(0, weight(w.count - 1) - (int)w.first) / (uint32_t)(w.count - 1);
     return w;
 }
 
@@ -595,85 +596,111 @@ __global__ __launch_bounds__(CF_NW * 64, 2) void k_cached_few(CachedArgs) {
 
 // ---- many rows -----------------------------------------------------------------------------------------------------
 template <bool BF16, int NB, bool MX4>
-__global__ __launch_bounds__(CM_NW * 64, MX4 ? 2 : 1) void k_cached_many(CachedArgs a) {
+__global__ __launch_bounds__(CM_NW * 64, MX4 || NB < 3 ? 2 : 1) void k_cached_many(CachedArgs) {
+#ifdef __HIP_DEVICE_COMPILE__
     constexpr int DP = NB * 32, KS = DP / 16, DB = NB, TILE = CM_KEYS * DP * 2, NT = CM_NW * 64;
     constexpr int PIECES = MX4 ? NB : NB * 4;                              // 16-byte pieces of a key in the page
-    constexpr int LOADS = (CM_KEYS * PIECES + NT - 1) / NT;                // of them a thread, of K and of V
+    constexpr int LOADS = (16 * PIECES + 63) / 64;                         // of them a lane, of K and of V: 16 keys a wave
+    static_assert(CM_KEYS == 16 * CM_NW, "a wave loads 16 of a tile's keys");
     __shared__ __attribute__((aligned(16))) char sK0[TILE], sK1[TILE], sV0[TILE], sV1[TILE];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
-    const KvArgs& kv = a.cache;
-    const Line line = make_line<CM_ROWS, CM_KEYS>(a);
-    const uint32_t to = line.cut(blockIdx.x + 1);
-    if (line.cut(blockIdx.x) >= to) {
-        if (threadIdx.x == 0) a.join[blockIdx.x].rows = 0;
+    uint32_t from, to;
+    {
+        const Line line = make_line<CM_ROWS, CM_KEYS>(*reread_args());
+        from = line.cut(blockIdx.x), to = line.cut(blockIdx.x + 1);
+    }
+    if (from >= to) {
+        if (threadIdx.x == 0) reread_args()->join[blockIdx.x].rows = 0;
         return;
     }
-    const int page_mask = (1 << kv.page_bits) - 1;
     constexpr float LAG = BF16 ? 8.f : 4.f, LIFT = BF16 ? 0.f : 11.f, FAR = 1024.f;
-    const float scale2 = a.scale2;
 
-    for (uint32_t from = line.cut(blockIdx.x); from < to;) {
+    while (from < to) {
+        const auto& a = *reread_args();
+        const Line line = make_line<CM_ROWS, CM_KEYS>(a);      // (made anew: kept it would take seven registers of the loop's)
         const CachedUnit u = find_unit<CM_ROWS, CM_KEYS>(a, line, from);
         const CachedPiece piece = cut_unit(u, from, to, blockIdx.x);
         if (u.end >= to) tell_join(a, u, line, to, blockIdx.x, from <= u.begin);
         from = u.end;
-        const int rows = u.lq * a.share;
-        // rows past the sample's last are copies of it that are not stored
-        auto query = [&](int r) __attribute__((always_inline)) { return min(r, rows - 1) / a.by_share; };
-        auto limit = [&](int r) __attribute__((always_inline)) { return cached_limit(a.causal, u.lq, u.lk, query(r)); };
-        const int r = u.first_row + wave * 32 + r32, lim = limit(r), wave_end = limit(u.first_row + wave * 32 + 31);
+        const int rows = u.lq * a.share, lk = u.lk, causal = a.causal;
+        const FastDiv by_share{a.by_share.mul, a.by_share.shift};
         const int t0 = piece.t0, t1 = piece.t1;
+        // (what the loop needs)
+        const int page_bits = a.cache.page_bits, page_mask = (1 << page_bits) - 1, pool = a.cache.pages, d = a.cache.d;
+        const int64_t page_bytes = a.cache.page_bytes;
+        const float scale2 = a.scale2;
+        // rows past the sample's last are copies of it that are not stored
+        auto query = [&](int r) __attribute__((always_inline)) { return min(r, rows - 1) / by_share; };
+        auto limit = [&](int r) __attribute__((always_inline)) { return cached_limit(causal, u.lq, lk, query(r)); };
+        const int lim = limit(u.first_row + wave * 32 + r32), wave_end = limit(u.first_row + wave * 32 + 31);
         // Q^T operand: d = 16 ks + 8 h .. + 7 of the lane's row
         u32x4_t qf[KS];
         {
-            const int qi = query(r), hq = u.head * a.share + min(r, rows - 1) - qi * a.share;
+            const int r = min(u.first_row + wave * 32 + r32, rows - 1), qi = r / by_share, hq = u.head * a.share + r - qi * a.share;
             const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (int64_t)(u.row0 + qi) * a.q_row + hq * a.q_head;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
-                qf[ks] = ks * 16 + h * 8 < kv.d ? *reinterpret_cast<const u32x4_t*>(qp + ks * 16 + h * 8) : u32x4_t{0, 0, 0, 0};
+                qf[ks] = ks * 16 + h * 8 < d ? *reinterpret_cast<const u32x4_t*>(qp + ks * 16 + h * 8) : u32x4_t{0, 0, 0, 0};
         }
         // Whether all of the piece's pages are the pool's (else every tile is looked at key by key).
+        const int32_t* const pages = a.cache.table + (int64_t)u.sample * a.cache.max_pages;
         bool sound = true;
-        const int32_t* pages = kv.table + (int64_t)u.sample * kv.max_pages;
-        const int end_key = min(t1 * CM_KEYS, u.lk);
-        for (int p = ((t0 * CM_KEYS) >> kv.page_bits) + threadIdx.x; (int64_t)p << kv.page_bits < end_key; p += NT) sound &= (unsigned)pages[p] < (unsigned)kv.pages;
+        const int end_key = min(t1 * CM_KEYS, lk);
+        for (int p = ((t0 * CM_KEYS) >> page_bits) + threadIdx.x; (int64_t)p << page_bits < end_key; p += NT) sound &= (unsigned)pages[p] < (unsigned)pool;
         sound = __syncthreads_and(sound);
 
-        // A thread's pieces of a tile: 16 bytes at keys idx / PIECES. Keys past the sample's last, and those of no page, are zeros.
+        // A wave's 16 keys of a tile: their page (-1: none) by a scalar load, a lane's pieces of them. Keys past the sample's last,
+        // and those of no page, are zeros.
         struct Raw {
             u32x4_t x[LOADS];
-            uint32_t p[MX4 ? LOADS : 1];
+            uint32_t p;
         };
-        auto load = [&](int tile, int side, Raw& w) __attribute__((always_inline)) {
+        const auto table = (const __attribute__((address_space(4))) int32_t*)pages;
+        const uint8_t* const head = a.cache.data + u.head * a.cache.head_bytes;
+        const int row_bytes = MX4 ? 16 * NB : d * 2;
+        const int in = lane / PIECES, at_piece = lane % PIECES;
+        auto page_of = [&](int tile) __attribute__((always_inline)) {
+            const int key = __builtin_amdgcn_readfirstlane(tile * CM_KEYS + wave * 16);
+            return key < lk && tile < t1 ? table[key >> page_bits] : -1;
+        };
+        auto load = [&](int tile, int page, int side, Raw& w) __attribute__((always_inline)) {
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const int idx = i * NT + threadIdx.x, in = idx / PIECES, p = idx % PIECES, key = tile * CM_KEYS + in;
-                w.x[i] = u32x4_t{0, 0, 0, 0};
-                if constexpr (MX4) w.p[i] = 0;
-                if (in >= CM_KEYS || key >= u.lk || tile >= t1 || (!MX4 && p * 8 >= kv.d)) continue;
-                const int page = pages[key >> kv.page_bits], slot = key & page_mask;
-                if ((unsigned)page >= (unsigned)kv.pages) continue;
-                const uint8_t* head = kv.data + page * kv.page_bytes + u.head * kv.head_bytes;
-                if constexpr (MX4) {
-                    w.x[i] = *reinterpret_cast<const u32x4_t*>(head + kv_codes_at(kv, side, slot) + p * 16);
-                    w.p[i] = head[kv_powers_at(kv, side, slot) + p];
-                } else {
-                    w.x[i] = *reinterpret_cast<const u32x4_t*>(head + ((int64_t)((side << kv.page_bits) + slot) * kv.d + p * 8) * 2);
+            for (int i = 0; i < LOADS; ++i) w.x[i] = u32x4_t{0, 0, 0, 0};
+            w.p = 0;
+            if ((unsigned)page >= (unsigned)pool) return;
+            const int key = tile * CM_KEYS + wave * 16, slot = key & page_mask, left = lk - key;
+            const uint8_t* const at = head + page * page_bytes + ((side << page_bits) + slot) * row_bytes;
+            if constexpr (MX4) {
+                const uint8_t* const power = head + page * page_bytes + (2 * row_bytes << page_bits) + ((side << page_bits) + slot) * NB;
+                if (lane < 16 * NB && in < left) {
+                    w.x[0] = *reinterpret_cast<const u32x4_t*>(at + lane * 16);
+                    w.p = power[lane];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) {
+                    const int idx = i * 64 + lane, k = idx / PIECES, p = idx % PIECES;
+                    if (k < 16 && k < left && p * 8 < d) w.x[i] = *reinterpret_cast<const u32x4_t*>(at + k * row_bytes + p * 16);
                 }
             }
         };
+        // Into LDS, as 16-bit values. (Places that differ in a few bits are formed where they are used: registers.)
         auto put = [&](const Raw& w, int side, char* s) __attribute__((always_inline)) {
+            s += wave * 16 * DP * 2;
+            if constexpr (MX4) {
+                int to = side ? cv_piece<DP>(in, at_piece * 4) : k_piece<DP>(in, at_piece * 4);
+                asm volatile("" : "+v"(to));
+                const float scale = mx_scale(w.p);
+                if (NB == 4 || lane < 16 * NB) {
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const int idx = i * NT + threadIdx.x, key = idx / PIECES, p = idx % PIECES;
-                if (CM_KEYS * PIECES % NT && key >= CM_KEYS) continue;
-                if constexpr (MX4) {
-                    const float scale = mx_scale(w.p[i]);
+                    for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4_t*>(s + (to ^ (j * 16))) = widen4<BF16>(w.x[0][j], scale);
+                }
+            } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        *reinterpret_cast<u32x4_t*>(s + (side ? cv_piece<DP>(key, p * 4 + j) : k_piece<DP>(key, p * 4 + j))) = widen4<BF16>(w.x[i][j], scale);
-                } else {
-                    *reinterpret_cast<u32x4_t*>(s + (side ? cv_piece<DP>(key, p) : k_piece<DP>(key, p))) = w.x[i];
+                for (int i = 0; i < LOADS; ++i) {
+                    const int idx = i * 64 + lane, k = idx / PIECES, p = idx % PIECES;
+                    if (16 * PIECES % 64 && k >= 16) continue;
+                    *reinterpret_cast<u32x4_t*>(s + (side ? cv_piece<DP>(k, p) : k_piece<DP>(k, p))) = w.x[i];
                 }
             }
         };
@@ -684,8 +711,12 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 ? 2 : 1) void k_cached_many(CachedA
         bool far = false, seen = false;
 
         // scores: s[kb][i] is key kb * 32 + 8 (i / 4) + 4 h + i % 4 of the tile
+        // (operand places: of the first product, and what the others differ by)
+        int k_from = k_piece<DP>(r32, h), v_from = cv_piece<DP>(4 * h + ((lane >> 2) & 3), ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1)) + (lane & 1) * 8;
+        auto fresh = [&]() __attribute__((always_inline)) { asm volatile("" : "+v"(k_from), "+v"(v_from)); };
         auto k_operand = [&](const char* sK, int t) __attribute__((always_inline)) {
-            return *reinterpret_cast<const u32x4_t*>(sK + k_piece<DP>((t & 1) * 32 + r32, (t >> 1) * 2 + h));
+            const int q = t >> 1, at = DP == 96 ? (k_from ^ ((q & 1) * 32)) + (q >> 1) * 64 : k_from ^ (q * 32);
+            return *reinterpret_cast<const u32x4_t*>(sK + at + (t & 1) * 32 * DP * 2);
         };
         auto scores = [&](const char* sK, f32x16_t (&s)[2]) __attribute__((always_inline)) {
 #pragma unroll
@@ -741,9 +772,9 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 ? 2 : 1) void k_cached_many(CachedA
         };
         // V^T operand, as v_operand with this kernel's places
         auto values = [&](const char* sV, int ks, int db) __attribute__((always_inline)) {
-            const int key = ks * 16 + 4 * h + ((lane >> 2) & 3), p = db * 4 + ((lane >> 4) & 1) * 2 + ((lane >> 1) & 1), sub = (lane & 1) * 8;
-            const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(sV + cv_piece<DP>(key, p) + sub));
-            const s16x4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(sV + cv_piece<DP>(key + 8, p) + sub));
+            const char* const at = sV + (DP == 96 ? v_from + db * 64 : v_from ^ (db * 64)) + ks * 16 * DP * 2;
+            const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)at);
+            const s16x4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(at + 8 * DP * 2));
             const uint2 ux = __builtin_bit_cast(uint2, x), uy = __builtin_bit_cast(uint2, y);
             return u32x4_t{ux.x, ux.y, uy.x, uy.y};
         };
@@ -751,13 +782,14 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 ? 2 : 1) void k_cached_many(CachedA
         auto attend_masked = [&](int base, const char* sK, const char* sV) __attribute__((always_inline)) {
             f32x16_t s[2];
             u32x4_t pf[4];
+            fresh();
             scores(sK, s);
             int held = 15;      // a bit for 16 keys
             if (!sound) {
                 held = 0;
                 for (int k = 0; k < 4; ++k) {
                     const int key = base + k * 16;
-                    if (key < u.lk && (unsigned)pages[key >> kv.page_bits] < (unsigned)kv.pages) held |= 1 << k;
+                    if (key < lk && (unsigned)pages[key >> page_bits] < (unsigned)pool) held |= 1 << k;
                 }
             }
             const int left = lim - base - 4 * h;
@@ -775,7 +807,7 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 ? 2 : 1) void k_cached_many(CachedA
             // A probability of zero must not meet an Inf or a NaN of a key that its row does not see. Zero times V
             // shows whether there is one.
             bool odd = false;
-            if (a.causal) {
+            if (causal) {
                 f32x16_t z = f32x16_t{};
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks)
@@ -793,6 +825,7 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 ? 2 : 1) void k_cached_many(CachedA
                     u32x4_t vf = values(sV, ks, db);
                     if (odd) vf = finite_only<BF16>(vf);
                     o[db] = mfma32<BF16>(vf, pf[ks], o[db]);
+                    __builtin_amdgcn_sched_barrier(0);      // (one operand at a time: registers)
                 }
             if (odd) {      // the values left out, key by key, for the rows that see them
                 for (int key = 0; key < CM_KEYS; ++key) {
@@ -805,13 +838,16 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 ? 2 : 1) void k_cached_many(CachedA
                     const float2 ph = both_halves(p);
                     p = key & 4 ? ph.y : ph.x;
                     const bool sees = base + key < lim;      // (a key of no page is zeros)
+                    int from_e = 4 * h;
+                    asm volatile("" : "+v"(from_e));
 #pragma unroll
                     for (int db = 0; db < DB; ++db)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const int e = db * 32 + 8 * (i / 4) + 4 * h + i % 4;
+                            const int e = db * 32 + 8 * (i / 4) + from_e + i % 4;
                             const uint32_t b = *reinterpret_cast<const uint16_t*>(sV + cv_piece<DP>(key, e >> 3) + (e & 7) * 2);
                             if (sees && nonfinite16<BF16>(b)) o[db][i] += p * value16<BF16>(b);
+                            __builtin_amdgcn_sched_barrier(0);
                         }
                 }
             }
@@ -822,16 +858,23 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 ? 2 : 1) void k_cached_many(CachedA
         const int all_see = sound ? limit(u.first_row) / CM_KEYS : 0;      // tiles that every row sees whole
         const int whole = min(t1, all_see);
         Raw wk, wv;
+        int page2 = -1, page3 = -1;      // of the tile after next, whose V is loaded next, and of the one after that, for K
+        auto on = [&](int tile) __attribute__((always_inline)) {      // the next loads, and the page of the K after them
+            load(tile + 3, page3, 0, wk);
+            load(tile + 2, page2, 1, wv);
+            page2 = page3;
+            page3 = page_of(tile + 4);
+        };
         auto step = [&](int tile, char* k_this, const char* k_next, const char* v_this, char* v_next, f32x16_t (&s)[2],
                         f32x16_t (&sn)[2]) __attribute__((always_inline)) {
-            constexpr int AHEAD = 4, NK = 2 * KS, NV = 4 * DB;
+            constexpr int AHEAD = NB == 4 ? 3 : 4, NK = 2 * KS, NV = 4 * DB;      // (four at width 128: registers spilled)
             u32x4_t pf[4], ring[AHEAD];
             float sum = 0.f;
             __syncthreads();
             put(wk, 0, k_this);
             put(wv, 1, v_next);
-            load(tile + 3, 0, wk);
-            load(tile + 2, 1, wv);
+            on(tile);
+            fresh();
 #pragma unroll
             for (int t = 0; t < AHEAD; ++t) ring[t] = k_operand(k_next, t);
 #pragma unroll
@@ -852,8 +895,8 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 ? 2 : 1) void k_cached_many(CachedA
             float mt = sn[0][0];
 #pragma unroll
             for (int t = 0; t < NV; ++t) {
-                o[t % DB] = mfma32<BF16>(ring[t % AHEAD], pf[t / DB], o[t % DB]);
-                if (t + AHEAD < NV) ring[t % AHEAD] = values(v_this, (t + AHEAD) / DB, (t + AHEAD) % DB);
+                o[t % DB] = mfma32<BF16>(ring[(NK + t) % AHEAD], pf[t / DB], o[t % DB]);
+                if (t + AHEAD < NV) ring[(NK + t) % AHEAD] = values(v_this, (t + AHEAD) / DB, (t + AHEAD) % DB);
 #pragma unroll
                 for (int i = t * 32 / NV; i < (t + 1) * 32 / NV; ++i) mt = fmaxf(mt, sn[i / 16][i % 16]);
                 __builtin_amdgcn_sched_barrier(0);
@@ -863,15 +906,18 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 ? 2 : 1) void k_cached_many(CachedA
         };
         // on the way: K of the first two tiles and V of the first in LDS, K of the third and V of the second in registers
         if (t0 < t1) {
-            load(t0, 0, wk);
-            load(t0, 1, wv);
+            const int page0 = page_of(t0), page1 = page_of(t0 + 1);
+            load(t0, page0, 0, wk);
+            load(t0, page0, 1, wv);
             __syncthreads();        // (the last piece's rows have left LDS)
             put(wk, 0, sK0);
             put(wv, 1, sV0);
-            load(t0 + 1, 0, wk);
+            load(t0 + 1, page1, 0, wk);
             put(wk, 0, sK1);
-            load(t0 + 2, 0, wk);
-            load(t0 + 1, 1, wv);
+            page2 = page_of(t0 + 2);
+            load(t0 + 2, page2, 0, wk);
+            load(t0 + 1, page1, 1, wv);
+            page3 = page_of(t0 + 3);
         }
         int tile = t0;
         bool second = false;
@@ -889,8 +935,7 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 ? 2 : 1) void k_cached_many(CachedA
             __syncthreads();
             put(wk, 0, sK0);
             put(wv, 1, sV1);
-            load(tile + 3, 0, wk);
-            load(tile + 2, 1, wv);
+            on(tile);
             u32x4_t pf[4];
             exponents(s0, pf);
 #pragma unroll
@@ -907,10 +952,11 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 ? 2 : 1) void k_cached_many(CachedA
             __syncthreads();
             put(wk, 0, second ? sK1 : sK0);
             put(wv, 1, second ? sV0 : sV1);
-            load(tile + 3, 0, wk);
-            load(tile + 2, 1, wv);
+            on(tile);
         }
 
+        const auto& b = *reread_args();
+        const int r = u.first_row + wave * 32 + r32;
         const float2 lh = both_halves(l);
         const float sum = lh.x + lh.y;
         const uint64_t some = __ballot(seen);
@@ -918,14 +964,14 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 ? 2 : 1) void k_cached_many(CachedA
         if (piece.slot >= 0) {
             if (r < rows) {
                 const int64_t item = (int64_t)piece.slot * CM_ROWS + (r - u.first_row);
-                if (h == 0) a.stat[item] = float2{m, any ? sum : -1.f};
-                float* op = a.part + item * kv.d;
+                if (h == 0) b.stat[item] = float2{m, any ? sum : -1.f};
+                float* op = b.part + item * d;
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
                         const int e = db * 32 + 8 * g + 4 * h;
-                        if (any && e < kv.d) *reinterpret_cast<f32x4_t*>(op + e) = f32x4_t{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+                        if (any && e < d) *reinterpret_cast<f32x4_t*>(op + e) = f32x4_t{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
                     }
             }
             continue;
@@ -945,11 +991,12 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 ? 2 : 1) void k_cached_many(CachedA
         for (int i = 0; i < P / 2; ++i) {
             const int row = (i * 64 + lane) / P, p = (i * 64 + lane) % P, rr = u.first_row + wave * 32 + row;
             const u32x4_t x = *reinterpret_cast<const u32x4_t*>(sO + k_piece<DP>(row, p));
-            if (rr >= rows || p * 8 >= kv.d) continue;
-            const int qr = rr / a.by_share, hr = u.head * a.share + rr - qr * a.share;
-            *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(a.o) + (int64_t)(u.row0 + qr) * a.o_row + hr * a.o_head + p * 8) = x;
+            if (rr >= rows || p * 8 >= d) continue;
+            const int qr = rr / by_share, hr = u.head * b.share + rr - qr * b.share;
+            *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(b.o) + (int64_t)(u.row0 + qr) * b.o_row + hr * b.o_head + p * 8) = x;
         }
     }
+#endif
 }
 
 // ---- the pieces of units that were cut, joined -----------------------------------------------------------------------
@@ -1079,7 +1126,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // How a call is cut: the rows of a unit, the workgroups. Few rows are those that fit a unit of 32 in the mean (the host
 // does not know the lengths).
 struct CachedCut {
-    int rows, groups, least, shift;
+    int rows, groups, least, finer, coarser;
     int64_t units;      // at most
     int join;           // groups of lanes a row in the join
     unsigned joins;     // its workgroups
@@ -1089,12 +1136,17 @@ CachedCut cached_cut(int64_t nq, int samples, int hkv, int share, int64_t keys) 
     const int64_t each = ceil_div(nq, samples) * share;
     c.rows = each <= 16 ? 16 : each <= 32 ? 32 : CM_ROWS;
     c.units = (ceil_div(nq * share, c.rows) + (samples > 1 ? samples : 0)) * hkv;
-    c.shift = 0;      // the line is shorter than 2^30
+    // The line is shorter than 2^30. Weights of many rows' units are in 64ths of a tile where that allows it: a causal
+    // prompt's grow by less than a tile from one to the next (8,000 rows to themselves: 678 us in whole tiles).
     const int64_t tiles = ceil_div(keys, c.rows == CM_ROWS ? CM_KEYS : CF_KEYS);
-    while (c.shift < 30 && c.units * ((tiles >> c.shift) + 1) >= 1ll << 30) ++c.shift;
-    c.least = std::max(1, (c.rows == CM_ROWS ? 4 : 2 * CF_NW) >> c.shift);
+    c.finer = c.rows == CM_ROWS ? 6 : 0;
+    c.coarser = 0;
+    auto longest = [&]() { return c.units * (((tiles << c.finer) >> c.coarser) + 1); };
+    while (c.finer > 0 && (longest() >= 1ll << 30 || tiles << c.finer >= 1ll << 30)) --c.finer;
+    while (c.coarser < 30 && longest() >= 1ll << 30) ++c.coarser;
+    c.least = std::max(1, ((c.rows == CM_ROWS ? 4 : 2 * CF_NW) << c.finer) >> c.coarser);
     // two or three a CU, as registers and LDS allow, where the line can be that long
-    c.groups = (int)std::min<int64_t>(c.rows == 16 ? 768 : 512, ceil_div(c.units * ((tiles >> c.shift) + 1), c.least));
+    c.groups = (int)std::min<int64_t>(c.rows == 16 ? 768 : 512, ceil_div(longest(), c.least));
     const int64_t cut = std::min<int64_t>(c.units, c.groups), pieces = c.groups / std::max<int64_t>(1, ceil_div(nq * share, c.rows) * hkv);
     c.join = pieces > 32 ? 16 : pieces > 2 ? 4 : 1;
     c.joins = (unsigned)std::min<int64_t>(cut * ceil_div(std::min<int64_t>(each, c.rows), 16 / c.join), 2048);
@@ -1150,7 +1202,7 @@ extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, i
     float* part = static_cast<float*>(d_workspace);
     float2* stat = reinterpret_cast<float2*>(part + (size_t)cut.groups * 2 * cut.rows * c.d);
     const CachedArgs a{q->data, out->data, q->row_stride, q->head_stride, out->row_stride, out->head_stride, kv_args(c, d_table, max_pages, d_lengths),
-                       d_offsets, nq, samples, share, causal ? 1 : 0, cut.groups, cut.least, cut.shift, fast_div((uint32_t)share),
+                       d_offsets, nq, samples, share, causal ? 1 : 0, cut.groups, cut.least, cut.finer, cut.coarser, fast_div((uint32_t)share),
                        fast_div((uint32_t)cut.groups), scale * kLog2e, part, stat,
                        reinterpret_cast<JoinItem*>(stat + (size_t)cut.groups * 2 * cut.rows)};
     hipStream_t s = as_stream(stream);
