@@ -596,11 +596,9 @@ __global__ __launch_bounds__(CF_NW * 64, 2) void k_cached_few(CachedArgs) {
 
 // ---- many rows -----------------------------------------------------------------------------------------------------
 template <bool BF16, int NB, bool MX4>
-__global__ __launch_bounds__(CM_NW * 64, MX4 || NB < 3 ? 2 : 1) void k_cached_many(CachedArgs) {
+__global__ __launch_bounds__(CM_NW * 64, 2) void k_cached_many(CachedArgs) {
 #ifdef __HIP_DEVICE_COMPILE__
     constexpr int DP = NB * 32, KS = DP / 16, DB = NB, TILE = CM_KEYS * DP * 2, NT = CM_NW * 64;
-    constexpr int PIECES = MX4 ? NB : NB * 4;                              // 16-byte pieces of a key in the page
-    constexpr int LOADS = (16 * PIECES + 63) / 64;                         // of them a lane, of K and of V: 16 keys a wave
     static_assert(CM_KEYS == 16 * CM_NW, "a wave loads 16 of a tile's keys");
     __shared__ __attribute__((aligned(16))) char sK0[TILE], sK1[TILE], sV0[TILE], sV1[TILE];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
@@ -651,57 +649,52 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 || NB < 3 ? 2 : 1) void k_cached_ma
 
         // A wave's 16 keys of a tile: their page (-1: none) by a scalar load, a lane's pieces of them. Keys past the sample's last,
         // and those of no page, are zeros.
+        // 4-bit codes wait in registers, a tile more ahead than 16-bit values, which go straight into LDS (16 bytes a lane, each
+        // from the piece that belongs in its place; what is out of the buffer's range reads as zeros).
         struct Raw {
-            u32x4_t x[LOADS];
+            u32x4_t x;
             uint32_t p;
         };
         const auto table = (const __attribute__((address_space(4))) int32_t*)pages;
         const uint8_t* const head = a.cache.data + u.head * a.cache.head_bytes;
         const int row_bytes = MX4 ? 16 * NB : d * 2;
-        const int in = lane / PIECES, at_piece = lane % PIECES;
+        const int in = lane / NB, at_piece = lane % NB;
         auto page_of = [&](int tile) __attribute__((always_inline)) {
             const int key = __builtin_amdgcn_readfirstlane(tile * CM_KEYS + wave * 16);
             return key < lk && tile < t1 ? table[key >> page_bits] : -1;
         };
         auto load = [&](int tile, int page, int side, Raw& w) __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < LOADS; ++i) w.x[i] = u32x4_t{0, 0, 0, 0};
+            w.x = u32x4_t{0, 0, 0, 0};
             w.p = 0;
             if ((unsigned)page >= (unsigned)pool) return;
-            const int key = tile * CM_KEYS + wave * 16, slot = key & page_mask, left = lk - key;
-            const uint8_t* const at = head + page * page_bytes + ((side << page_bits) + slot) * row_bytes;
-            if constexpr (MX4) {
-                const uint8_t* const power = head + page * page_bytes + (2 * row_bytes << page_bits) + ((side << page_bits) + slot) * NB;
-                if (lane < 16 * NB && in < left) {
-                    w.x[0] = *reinterpret_cast<const u32x4_t*>(at + lane * 16);
-                    w.p = power[lane];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < LOADS; ++i) {
-                    const int idx = i * 64 + lane, k = idx / PIECES, p = idx % PIECES;
-                    if (k < 16 && k < left && p * 8 < d) w.x[i] = *reinterpret_cast<const u32x4_t*>(at + k * row_bytes + p * 16);
-                }
+            const int key = tile * CM_KEYS + wave * 16, slot = key & page_mask;
+            if (lane < 16 * NB && in < lk - key) {
+                w.x = *reinterpret_cast<const u32x4_t*>(head + page * page_bytes + ((side << page_bits) + slot) * (16 * NB) + lane * 16);
+                w.p = head[page * page_bytes + (32 * NB << page_bits) + ((side << page_bits) + slot) * NB + lane];
             }
         };
         // Into LDS, as 16-bit values. (Places that differ in a few bits are formed where they are used: registers.)
         auto put = [&](const Raw& w, int side, char* s) __attribute__((always_inline)) {
-            s += wave * 16 * DP * 2;
-            if constexpr (MX4) {
-                int to = side ? cv_piece<DP>(in, at_piece * 4) : k_piece<DP>(in, at_piece * 4);
-                asm volatile("" : "+v"(to));
-                const float scale = mx_scale(w.p);
-                if (NB == 4 || lane < 16 * NB) {
+            int to = side ? cv_piece<DP>(in, at_piece * 4) : k_piece<DP>(in, at_piece * 4);
+            asm volatile("" : "+v"(to));
+            const float scale = mx_scale(w.p);
+            if (NB == 4 || lane < 16 * NB) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4_t*>(s + (to ^ (j * 16))) = widen4<BF16>(w.x[0][j], scale);
-                }
-            } else {
+                for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4_t*>(s + wave * 16 * DP * 2 + (to ^ (j * 16))) = widen4<BF16>(w.x[j], scale);
+            }
+        };
+        auto stage = [&](int tile, int page, int side, char* s) __attribute__((always_inline)) {
+            constexpr int P = DP / 8, NOWHERE = 1 << 30;
+            const int key = tile * CM_KEYS + wave * 16, slot = key & page_mask, left = (unsigned)page < (unsigned)pool ? min(16, lk - key) : 0;
+            const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(head + (left ? page : 0) * page_bytes + ((side << page_bits) + slot) * row_bytes), (short)0,
+                                                                left * row_bytes, 0x00027000);
+            int from_lane = lane;
+            asm volatile("" : "+v"(from_lane));
 #pragma unroll
-                for (int i = 0; i < LOADS; ++i) {
-                    const int idx = i * 64 + lane, k = idx / PIECES, p = idx % PIECES;
-                    if (16 * PIECES % 64 && k >= 16) continue;
-                    *reinterpret_cast<u32x4_t*>(s + (side ? cv_piece<DP>(k, p) : k_piece<DP>(k, p))) = w.x[i];
-                }
+            for (int i = 0; i < NB; ++i) {
+                const int at = i * 64 + from_lane, k = at / P, p = (side ? cv_piece<DP>(k, at % P) : k_piece<DP>(k, at % P)) / 16 % P;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(s + wave * 16 * DP * 2 + i * 1024), 16,
+                                                         p * 8 < d ? k * row_bytes + p * 16 : NOWHERE, 0, 0, 0);
             }
         };
         f32x16_t o[DB];
@@ -825,7 +818,7 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 || NB < 3 ? 2 : 1) void k_cached_ma
                     u32x4_t vf = values(sV, ks, db);
                     if (odd) vf = finite_only<BF16>(vf);
                     o[db] = mfma32<BF16>(vf, pf[ks], o[db]);
-                    __builtin_amdgcn_sched_barrier(0);      // (one operand at a time: registers)
+                    if (db % 2 == 1 || DB == 1) __builtin_amdgcn_sched_barrier(0);      // (two operands at a time: registers)
                 }
             if (odd) {      // the values left out, key by key, for the rows that see them
                 for (int key = 0; key < CM_KEYS; ++key) {
@@ -858,22 +851,35 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 || NB < 3 ? 2 : 1) void k_cached_ma
         const int all_see = sound ? limit(u.first_row) / CM_KEYS : 0;      // tiles that every row sees whole
         const int whole = min(t1, all_see);
         Raw wk, wv;
-        int page2 = -1, page3 = -1;      // of the tile after next, whose V is loaded next, and of the one after that, for K
-        auto on = [&](int tile) __attribute__((always_inline)) {      // the next loads, and the page of the K after them
-            load(tile + 3, page3, 0, wk);
-            load(tile + 2, page2, 1, wv);
-            page2 = page3;
-            page3 = page_of(tile + 4);
+        int page1 = -1, page2 = -1, page3 = -1;      // of the tiles after the present one
+        // Every wave's part of what has been on its way is in LDS, and none reads any more what was read before.
+        auto landed = [&]() __attribute__((always_inline)) {
+            if constexpr (!MX4) wait_loads();
+            __syncthreads();
+        };
+        // K of the tile after next and V of the next into LDS; then the loads after them
+        auto bring = [&](int tile, char* k_to, char* v_to) __attribute__((always_inline)) {
+            if constexpr (MX4) {
+                put(wk, 0, k_to);
+                put(wv, 1, v_to);
+                load(tile + 3, page3, 0, wk);
+                load(tile + 2, page2, 1, wv);
+                page2 = page3;
+                page3 = page_of(tile + 4);
+            } else {
+                stage(tile + 2, page2, 0, k_to);
+                stage(tile + 1, page1, 1, v_to);
+                page1 = page2;
+                page2 = page_of(tile + 3);
+            }
         };
         auto step = [&](int tile, char* k_this, const char* k_next, const char* v_this, char* v_next, f32x16_t (&s)[2],
                         f32x16_t (&sn)[2]) __attribute__((always_inline)) {
             constexpr int AHEAD = NB == 4 ? 3 : 4, NK = 2 * KS, NV = 4 * DB;      // (four at width 128: registers spilled)
             u32x4_t pf[4], ring[AHEAD];
             float sum = 0.f;
-            __syncthreads();
-            put(wk, 0, k_this);
-            put(wv, 1, v_next);
-            on(tile);
+            landed();
+            bring(tile, k_this, v_next);
             fresh();
 #pragma unroll
             for (int t = 0; t < AHEAD; ++t) ring[t] = k_operand(k_next, t);
@@ -904,27 +910,35 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 || NB < 3 ? 2 : 1) void k_cached_ma
             raise(mt);
             near_top(sn);
         };
-        // on the way: K of the first two tiles and V of the first in LDS, K of the third and V of the second in registers
+        // on the way: K of the first two tiles and V of the first in LDS, and of 4 bits K of the third and V of the second in registers
         if (t0 < t1) {
-            const int page0 = page_of(t0), page1 = page_of(t0 + 1);
-            load(t0, page0, 0, wk);
-            load(t0, page0, 1, wv);
-            __syncthreads();        // (the last piece's rows have left LDS)
-            put(wk, 0, sK0);
-            put(wv, 1, sV0);
-            load(t0 + 1, page1, 0, wk);
-            put(wk, 0, sK1);
+            const int page0 = page_of(t0);
+            page1 = page_of(t0 + 1);
             page2 = page_of(t0 + 2);
-            load(t0 + 2, page2, 0, wk);
-            load(t0 + 1, page1, 1, wv);
-            page3 = page_of(t0 + 3);
+            if constexpr (MX4) {
+                load(t0, page0, 0, wk);
+                load(t0, page0, 1, wv);
+                __syncthreads();        // (the last piece's rows have left LDS)
+                put(wk, 0, sK0);
+                put(wv, 1, sV0);
+                load(t0 + 1, page1, 0, wk);
+                put(wk, 0, sK1);
+                load(t0 + 2, page2, 0, wk);
+                load(t0 + 1, page1, 1, wv);
+                page3 = page_of(t0 + 3);
+            } else {
+                __syncthreads();
+                stage(t0, page0, 0, sK0);
+                stage(t0, page0, 1, sV0);
+                stage(t0 + 1, page1, 0, sK1);
+            }
         }
         int tile = t0;
         bool second = false;
         if (tile < whole) {
             seen = true;
             f32x16_t s0[2], s1[2];
-            __syncthreads();
+            landed();
             scores(sK0, s0);
             raise(top_of(s0));
             near_top(s0);
@@ -932,10 +946,8 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 || NB < 3 ? 2 : 1) void k_cached_ma
                 step(tile, sK0, sK1, sV0, sV1, s0, s1);
                 step(tile + 1, sK1, sK0, sV1, sV0, s1, s0);
             }
-            __syncthreads();
-            put(wk, 0, sK0);
-            put(wv, 1, sV1);
-            on(tile);
+            landed();
+            bring(tile, sK0, sV1);
             u32x4_t pf[4];
             exponents(s0, pf);
 #pragma unroll
@@ -947,13 +959,12 @@ __global__ __launch_bounds__(CM_NW * 64, MX4 || NB < 3 ? 2 : 1) void k_cached_ma
         }
         // the others, a whole one among them at times
         for (; tile < t1; ++tile, second = !second) {
-            __syncthreads();
+            landed();
             if (tile * CM_KEYS < wave_end) attend_masked(tile * CM_KEYS, second ? sK1 : sK0, second ? sV1 : sV0);
             __syncthreads();
-            put(wk, 0, second ? sK1 : sK0);
-            put(wv, 1, second ? sV0 : sV1);
-            on(tile);
+            bring(tile, second ? sK1 : sK0, second ? sV0 : sV1);
         }
+        if constexpr (!MX4) wait_loads();      // (none is on its way to LDS that the next piece uses)
 
         const auto& b = *reread_args();
         const int r = u.first_row + wave * 32 + r32;
@@ -1131,10 +1142,10 @@ struct CachedCut {
     int join;           // groups of lanes a row in the join
     unsigned joins;     // its workgroups
 };
-CachedCut cached_cut(int64_t nq, int samples, int hkv, int share, int64_t keys) {
+CachedCut cached_cut(int64_t nq, int samples, int hkv, int share, int64_t keys, bool mx4) {
     CachedCut c;
     const int64_t each = ceil_div(nq, samples) * share;
-    c.rows = each <= 16 ? 16 : each <= 32 ? 32 : CM_ROWS;
+    c.rows = each <= 16 ? 16 : each <= 32 && mx4 ? 32 : CM_ROWS;      // (two tiles of rows beside 16-bit keys would spill registers)
     c.units = (ceil_div(nq * share, c.rows) + (samples > 1 ? samples : 0)) * hkv;
     // The line is shorter than 2^30. Weights of many rows' units are in 64ths of a tile where that allows it: a causal
     // prompt's grow by less than a tile from one to the next (8,000 rows to themselves: 678 us in whole tiles).
@@ -1163,7 +1174,7 @@ using namespace tsp;
 
 extern "C" size_t tsp_attention_cached_workspace_bytes(int64_t nq, int samples, int hq, const tsp_kv_cache* cache, int max_pages) {
     if (!cache || !kv_valid(*cache) || nq <= 0 || nq >= (1ll << 31) || samples <= 0 || hq <= 0 || hq % cache->heads || max_pages <= 0) return 0;
-    return cached_workspace(cached_cut(nq, samples, cache->heads, hq / cache->heads, (int64_t)max_pages * cache->page), cache->d);
+    return cached_workspace(cached_cut(nq, samples, cache->heads, hq / cache->heads, (int64_t)max_pages * cache->page, cache->format == TSP_KV_MX4), cache->d);
 }
 
 extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, int hq, const tsp_kv_cache* cache, const int32_t* d_offsets,
@@ -1193,7 +1204,7 @@ extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, i
                 "tsp_attention_cached: out must not alias q or the cache");
     const int share = hq / c.heads;
     TSP_REQUIRE(nq * share < (1ll << 31) - 1024, TSP_ERR_INVALID, "tsp_attention_cached: too many rows");
-    const CachedCut cut = cached_cut(nq, samples, c.heads, share, (int64_t)max_pages * c.page);
+    const CachedCut cut = cached_cut(nq, samples, c.heads, share, (int64_t)max_pages * c.page, c.format == TSP_KV_MX4);
     TSP_REQUIRE(cut.units < 1ll << 29, TSP_ERR_INVALID, "tsp_attention_cached: too many rows and heads");
     const size_t need = cached_workspace(cut, c.d);
     TSP_REQUIRE(d_workspace, TSP_ERR_INVALID, "tsp_attention_cached: null workspace");
@@ -1211,7 +1222,7 @@ extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, i
         constexpr int NB = decltype(nb)::value;
         const dim3 grid((unsigned)cut.groups);
         if (cut.rows == 16) hipLaunchKernelGGL((k_cached_few<BF16, NB, MX4, 1>), grid, dim3(CF_NW * 64), 0, s, a);
-        else if (cut.rows == 32) hipLaunchKernelGGL((k_cached_few<BF16, NB, MX4, 2>), grid, dim3(CF_NW * 64), 0, s, a);
+        else if (MX4 && cut.rows == 32) hipLaunchKernelGGL((k_cached_few<BF16, NB, true, 2>), grid, dim3(CF_NW * 64), 0, s, a);
         else hipLaunchKernelGGL((k_cached_many<BF16, NB, MX4>), grid, dim3(CM_NW * 64), 0, s, a);
     };
     auto by_width = [&](auto bf, auto mx) {

@@ -151,7 +151,6 @@ __global__ __launch_bounds__(KV_NT) void k_kv_append(AppendArgs a) {
         int sample, row0, rows;
         if (!row_sample<L>(a.offsets, a.samples, (int)a.n, row, sample, row0, rows)) continue;
         KT cs[4], sn[4];
-        float fc[4], fs[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             cs[i] = 1, sn[i] = 0;
@@ -161,20 +160,12 @@ __global__ __launch_bounds__(KV_NT) void k_kv_append(AppendArgs a) {
                 if constexpr (HELD == TSP_KV_MX4) sincospi(f, &sn[i], &cs[i]);
                 else sincospif(f, &sn[i], &cs[i]);
             }
-            fc[i] = (float)cs[i], fs[i] = (float)sn[i];
-        }
-        for (int h = part; h < a.hq; h += a.parts) {
-            float u[4] = {}, v[4] = {};
-            if (live) load_pairs<XDT, HALVES>(a.q, row * a.q_row + h * a.q_head, unit, a.d, u, v);
-            turn<L, float>(u, v, a.q_gamma ? a.q_gamma + h * a.d : nullptr, HALVES, unit, a.d, live, a.eps, axis, fc, fs);
-            if (live) store_pairs<XDT, HALVES>(a.q_out, row * a.o_row + h * a.o_head, unit, a.d, u, v);
         }
         const int64_t key = (int64_t)a.cache.lengths[sample] - rows + (row - row0);
-        if (key < 0 || key >= (int64_t)a.cache.max_pages << a.cache.page_bits) continue;
         const int slot = (int)key & ((1 << a.cache.page_bits) - 1);
-        uint8_t* page = kv_head(a.cache, sample, key, 0);
-        if (!page) continue;
-        for (int h = part; h < a.cache.heads; h += a.parts) {
+        uint8_t* page = key >= 0 && key < (int64_t)a.cache.max_pages << a.cache.page_bits ? kv_head(a.cache, sample, key, 0) : nullptr;
+        // (keys first: their 64-bit angles are not kept for the queries)
+        for (int h = part; page && h < a.cache.heads; h += a.parts) {
             uint8_t* to = page + h * a.cache.head_bytes;
             float u[4] = {}, v[4] = {}, x[8] = {};
             if (live) {
@@ -219,6 +210,26 @@ __global__ __launch_bounds__(KV_NT) void k_kv_append(AppendArgs a) {
             } else if (live) {
                 store_pairs<HELD, HALVES>(to, (int64_t)slot * a.d, unit, a.d, u, v);
                 store8<HELD>(to, ((1ll << a.cache.page_bits) + slot) * a.d + 8 * unit, x);
+            }
+        }
+        float fc[4], fs[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fc[i] = (float)cs[i], fs[i] = (float)sn[i];
+        // (heads' loads go out BATCH at a time)
+        constexpr int BATCH = 4;
+        for (int h0 = part; h0 < a.hq; h0 += BATCH * a.parts) {
+            float u[BATCH][4] = {}, v[BATCH][4] = {};
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                const int h = h0 + b * a.parts;
+                if (live && h < a.hq) load_pairs<XDT, HALVES>(a.q, row * a.q_row + h * a.q_head, unit, a.d, u[b], v[b]);
+            }
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                const int h = h0 + b * a.parts;
+                if (h >= a.hq) break;
+                turn<L, float>(u[b], v[b], a.q_gamma ? a.q_gamma + h * a.d : nullptr, HALVES, unit, a.d, live, a.eps, axis, fc, fs);
+                if (live) store_pairs<XDT, HALVES>(a.q_out, row * a.o_row + h * a.o_head, unit, a.d, u[b], v[b]);
             }
         }
     }
