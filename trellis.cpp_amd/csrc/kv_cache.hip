@@ -29,7 +29,7 @@ struct AppendArgs {
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;     // strides in elements
     const float *q_gamma, *k_gamma;
     const int32_t *offsets, *pos;
-    int64_t n;
+    int64_t n, first;                // rows, the launch's first
     int samples, hq, d, axes, parts;
     double eps;
     double turns[KV_MAX_PAIRS];      // theta^(-j / P) / (2 pi) of each pair
@@ -144,93 +144,94 @@ __global__ __launch_bounds__(KV_NT) void k_kv_append(AppendArgs a) {
         axis[i] = live ? a.axis[4 * unit + i] : -1;
         turns[i] = axis[i] < 0 ? 0. : a.turns[4 * unit + i];
     }
-    const unsigned items = (unsigned)(a.n * a.parts);       // (below 2^31)
-    // (whole groups of lanes leave together)
-    for (unsigned item = (blockIdx.x * KV_NT + threadIdx.x) / L; item < items; item += gridDim.x * (KV_NT / L)) {
-        const int row = (int)(item / (unsigned)a.parts), part = (int)(item - (unsigned)row * a.parts);
-        int sample, row0, rows;
-        if (!row_sample<L>(a.offsets, a.samples, (int)a.n, row, sample, row0, rows)) continue;
-        KT cs[4], sn[4];
+    // (whole groups of lanes leave together. No loop: the sine's constants would be kept in registers for all of it)
+    const unsigned item = (blockIdx.x * KV_NT + threadIdx.x) / L;
+    const int64_t at = a.first + item / (unsigned)a.parts;
+    if (at >= a.n) return;
+    const int row = (int)at, part = (int)(item % (unsigned)a.parts);
+    int sample, row0, rows;
+    if (!row_sample<L>(a.offsets, a.samples, (int)a.n, row, sample, row0, rows)) return;
+    KT cs[4], sn[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            cs[i] = 1, sn[i] = 0;
-            if (axis[i] >= 0) {
-                const double t = (double)a.pos[(int64_t)row * a.axes + axis[i]] * turns[i];
-                const KT f = 2 * (KT)(t - rint(t));
-                if constexpr (HELD == TSP_KV_MX4) sincospi(f, &sn[i], &cs[i]);
-                else sincospif(f, &sn[i], &cs[i]);
-            }
+    for (int i = 0; i < 4; ++i) {
+        cs[i] = 1, sn[i] = 0;
+        if (axis[i] >= 0) {
+            const double t = (double)a.pos[(int64_t)row * a.axes + axis[i]] * turns[i];
+            const KT f = 2 * (KT)(t - rint(t));
+            if constexpr (HELD == TSP_KV_MX4) sincospi(f, &sn[i], &cs[i]);
+            else sincospif(f, &sn[i], &cs[i]);
         }
-        const int64_t key = (int64_t)a.cache.lengths[sample] - rows + (row - row0);
-        const int slot = (int)key & ((1 << a.cache.page_bits) - 1);
-        uint8_t* page = key >= 0 && key < (int64_t)a.cache.max_pages << a.cache.page_bits ? kv_head(a.cache, sample, key, 0) : nullptr;
-        // (keys first: their 64-bit angles are not kept for the queries)
-        for (int h = part; page && h < a.cache.heads; h += a.parts) {
-            uint8_t* to = page + h * a.cache.head_bytes;
-            float u[4] = {}, v[4] = {}, x[8] = {};
-            if (live) {
-                load_pairs<XDT, HALVES>(a.k, row * a.k_row + h * a.k_head, unit, a.d, u, v);
-                load8<XDT>(a.v, row * a.v_row + h * a.v_head + 8 * unit, x);
-            }
-            KT ku[4], kv[4];
+        if constexpr (HELD == TSP_KV_MX4) __builtin_amdgcn_sched_barrier(0);      // (one after the other: registers)
+    }
+    const int64_t key = (int64_t)a.cache.lengths[sample] - rows + (row - row0);
+    const int slot = (int)key & ((1 << a.cache.page_bits) - 1);
+    uint8_t* page = key >= 0 && key < (int64_t)a.cache.max_pages << a.cache.page_bits ? kv_head(a.cache, sample, key, 0) : nullptr;
+    // (keys first: their 64-bit angles are not kept for the queries)
+    for (int h = part; page && h < a.cache.heads; h += a.parts) {
+        uint8_t* to = page + h * a.cache.head_bytes;
+        float u[4] = {}, v[4] = {}, x[8] = {};
+        if (live) {
+            load_pairs<XDT, HALVES>(a.k, row * a.k_row + h * a.k_head, unit, a.d, u, v);
+            load8<XDT>(a.v, row * a.v_row + h * a.v_head + 8 * unit, x);
+        }
+        KT ku[4], kv[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ku[i] = u[i], kv[i] = v[i];
-            turn<L, KT>(ku, kv, a.k_gamma ? a.k_gamma + h * a.d : nullptr, HALVES, unit, a.d, live, a.eps, axis, cs, sn);
+        for (int i = 0; i < 4; ++i) ku[i] = u[i], kv[i] = v[i];
+        turn<L, KT>(ku, kv, a.k_gamma ? a.k_gamma + h * a.d : nullptr, HALVES, unit, a.d, live, a.eps, axis, cs, sn);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) u[i] = to_odd(ku[i]), v[i] = to_odd(kv[i]);
-            if constexpr (HELD == TSP_KV_MX4) {
-                float y[8];
-                if constexpr (HALVES) {
-                    // The lane's eight channels are two runs of four, which stand in the first half of some lane
-                    // or the second of another.
+        for (int i = 0; i < 4; ++i) u[i] = to_odd(ku[i]), v[i] = to_odd(kv[i]);
+        if constexpr (HELD == TSP_KV_MX4) {
+            float y[8];
+            if constexpr (HALVES) {
+                // The lane's eight channels are two runs of four, which stand in the first half of some lane
+                // or the second of another.
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const int run = 2 * unit + r, half = a.d / 8;
-                        const bool second = run >= half;
-                        const int from = second ? run - half : run;
+                for (int r = 0; r < 2; ++r) {
+                    const int run = 2 * unit + r, half = a.d / 8;
+                    const bool second = run >= half;
+                    const int from = second ? run - half : run;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float p = __shfl(u[i], from, L), q = __shfl(v[i], from, L);
-                            y[4 * r + i] = !live ? 0.f : second ? q : p;
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) y[2 * i] = u[i], y[2 * i + 1] = v[i];
-                }
-                const uint32_t kp = mx_power_of<MX_E2M1>(y), vp = mx_power_of<MX_E2M1>(x);
-                if (unit < 4 * a.cache.blocks) {        // (channels past d among them: zeros)
-                    *reinterpret_cast<uint32_t*>(to + kv_codes_at(a.cache, 0, slot) + unit * 4) = mx_codes4(y, kp);
-                    *reinterpret_cast<uint32_t*>(to + kv_codes_at(a.cache, 1, slot) + unit * 4) = mx_codes4(x, vp);
-                    if ((unit & 3) == 0) {
-                        to[kv_powers_at(a.cache, 0, slot) + unit / 4] = (uint8_t)kp;
-                        to[kv_powers_at(a.cache, 1, slot) + unit / 4] = (uint8_t)vp;
+                    for (int i = 0; i < 4; ++i) {
+                        const float p = __shfl(u[i], from, L), q = __shfl(v[i], from, L);
+                        y[4 * r + i] = !live ? 0.f : second ? q : p;
                     }
                 }
-            } else if (live) {
-                store_pairs<HELD, HALVES>(to, (int64_t)slot * a.d, unit, a.d, u, v);
-                store8<HELD>(to, ((1ll << a.cache.page_bits) + slot) * a.d + 8 * unit, x);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[2 * i] = u[i], y[2 * i + 1] = v[i];
             }
+            const uint32_t kp = mx_power_of<MX_E2M1>(y), vp = mx_power_of<MX_E2M1>(x);
+            if (unit < 4 * a.cache.blocks) {        // (channels past d among them: zeros)
+                *reinterpret_cast<uint32_t*>(to + kv_codes_at(a.cache, 0, slot) + unit * 4) = mx_codes4(y, kp);
+                *reinterpret_cast<uint32_t*>(to + kv_codes_at(a.cache, 1, slot) + unit * 4) = mx_codes4(x, vp);
+                if ((unit & 3) == 0) {
+                    to[kv_powers_at(a.cache, 0, slot) + unit / 4] = (uint8_t)kp;
+                    to[kv_powers_at(a.cache, 1, slot) + unit / 4] = (uint8_t)vp;
+                }
+            }
+        } else if (live) {
+            store_pairs<HELD, HALVES>(to, (int64_t)slot * a.d, unit, a.d, u, v);
+            store8<HELD>(to, ((1ll << a.cache.page_bits) + slot) * a.d + 8 * unit, x);
         }
-        float fc[4], fs[4];
+    }
+    float fc[4], fs[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) fc[i] = (float)cs[i], fs[i] = (float)sn[i];
-        // (heads' loads go out BATCH at a time)
-        constexpr int BATCH = 4;
-        for (int h0 = part; h0 < a.hq; h0 += BATCH * a.parts) {
-            float u[BATCH][4] = {}, v[BATCH][4] = {};
+    for (int i = 0; i < 4; ++i) fc[i] = (float)cs[i], fs[i] = (float)sn[i];
+    // (heads' loads go out BATCH at a time)
+    constexpr int BATCH = 4;
+    for (int h0 = part; h0 < a.hq; h0 += BATCH * a.parts) {
+        float u[BATCH][4] = {}, v[BATCH][4] = {};
 #pragma unroll
-            for (int b = 0; b < BATCH; ++b) {
-                const int h = h0 + b * a.parts;
-                if (live && h < a.hq) load_pairs<XDT, HALVES>(a.q, row * a.q_row + h * a.q_head, unit, a.d, u[b], v[b]);
-            }
+        for (int b = 0; b < BATCH; ++b) {
+            const int h = h0 + b * a.parts;
+            if (live && h < a.hq) load_pairs<XDT, HALVES>(a.q, row * a.q_row + h * a.q_head, unit, a.d, u[b], v[b]);
+        }
 #pragma unroll
-            for (int b = 0; b < BATCH; ++b) {
-                const int h = h0 + b * a.parts;
-                if (h >= a.hq) break;
-                turn<L, float>(u[b], v[b], a.q_gamma ? a.q_gamma + h * a.d : nullptr, HALVES, unit, a.d, live, a.eps, axis, fc, fs);
-                if (live) store_pairs<XDT, HALVES>(a.q_out, row * a.o_row + h * a.o_head, unit, a.d, u[b], v[b]);
-            }
+        for (int b = 0; b < BATCH; ++b) {
+            const int h = h0 + b * a.parts;
+            if (h >= a.hq) break;
+            turn<L, float>(u[b], v[b], a.q_gamma ? a.q_gamma + h * a.d : nullptr, HALVES, unit, a.d, live, a.eps, axis, fc, fs);
+            if (live) store_pairs<XDT, HALVES>(a.q_out, row * a.o_row + h * a.o_head, unit, a.d, u[b], v[b]);
         }
     }
 }
@@ -376,17 +377,20 @@ extern "C" int tsp_kv_append(const tsp_kv_cache* cache, const tsp_heads* k, cons
     // A row is shared by as many groups as it takes to give the device some 2048 workgroups, at most one a head.
     const int lanes = c.d <= 64 ? 8 : 16, groups = KV_NT / lanes;
     a.parts = (int)std::min<int64_t>(std::max(hq, c.heads), std::max<int64_t>(1, 2048ll * groups / n));
-    const int64_t blocks = std::min<int64_t>(ceil_div(n * a.parts, groups), 8192);
+    constexpr int64_t kRows = 1 << 26;       // of a launch
     dt_switch(dtype, [&](auto xd) {
         held_switch(c.format, [&](auto held) {
             constexpr int XD = decltype(xd)::value, HELD = decltype(held)::value;
-            const dim3 grid((unsigned)blocks), block(KV_NT);
+            const dim3 block(KV_NT);
             hipStream_t s = as_stream(stream);
             const bool halves = flags & TSP_ROPE_HALVES;
-            if (lanes == 8 && halves) hipLaunchKernelGGL((k_kv_append<XD, HELD, 8, true>), grid, block, 0, s, a);
-            else if (lanes == 8) hipLaunchKernelGGL((k_kv_append<XD, HELD, 8, false>), grid, block, 0, s, a);
-            else if (halves) hipLaunchKernelGGL((k_kv_append<XD, HELD, 16, true>), grid, block, 0, s, a);
-            else hipLaunchKernelGGL((k_kv_append<XD, HELD, 16, false>), grid, block, 0, s, a);
+            for (a.first = 0; a.first < n; a.first += kRows) {
+                const dim3 grid((unsigned)ceil_div(std::min(n - a.first, kRows) * a.parts, groups));
+                if (lanes == 8 && halves) hipLaunchKernelGGL((k_kv_append<XD, HELD, 8, true>), grid, block, 0, s, a);
+                else if (lanes == 8) hipLaunchKernelGGL((k_kv_append<XD, HELD, 8, false>), grid, block, 0, s, a);
+                else if (halves) hipLaunchKernelGGL((k_kv_append<XD, HELD, 16, true>), grid, block, 0, s, a);
+                else hipLaunchKernelGGL((k_kv_append<XD, HELD, 16, false>), grid, block, 0, s, a);
+            }
         });
     });
     TSP_CHECK_LAUNCH();
