@@ -167,51 +167,63 @@ __global__ __launch_bounds__(KV_NT) void k_kv_append(AppendArgs a) {
     const int slot = (int)key & ((1 << a.cache.page_bits) - 1);
     uint8_t* page = key >= 0 && key < (int64_t)a.cache.max_pages << a.cache.page_bits ? kv_head(a.cache, sample, key, 0) : nullptr;
     // (keys first: their 64-bit angles are not kept for the queries)
-    for (int h = part; page && h < a.cache.heads; h += a.parts) {
-        uint8_t* to = page + h * a.cache.head_bytes;
-        float u[4] = {}, v[4] = {}, x[8] = {};
-        if (live) {
-            load_pairs<XDT, HALVES>(a.k, row * a.k_row + h * a.k_head, unit, a.d, u, v);
-            load8<XDT>(a.v, row * a.v_row + h * a.v_head + 8 * unit, x);
+    // In 16 bits two heads' loads go out at a time; in 4 their registers would cost more than that gains (12,345 rows: 38 us, and
+    // 46 so).
+    constexpr int KB = HELD == TSP_KV_MX4 ? 1 : 2;
+    for (int h0 = part; page && h0 < a.cache.heads; h0 += KB * a.parts) {
+        float kus[KB][4] = {}, kvs[KB][4] = {}, xs[KB][8] = {};
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            const int h = h0 + b * a.parts;
+            if (!live || h >= a.cache.heads) continue;
+            load_pairs<XDT, HALVES>(a.k, row * a.k_row + h * a.k_head, unit, a.d, kus[b], kvs[b]);
+            load8<XDT>(a.v, row * a.v_row + h * a.v_head + 8 * unit, xs[b]);
         }
-        KT ku[4], kv[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ku[i] = u[i], kv[i] = v[i];
-        turn<L, KT>(ku, kv, a.k_gamma ? a.k_gamma + h * a.d : nullptr, HALVES, unit, a.d, live, a.eps, axis, cs, sn);
+        for (int b = 0; b < KB; ++b) {
+            const int h = h0 + b * a.parts;
+            if (h >= a.cache.heads) break;
+            uint8_t* to = page + h * a.cache.head_bytes;
+            float (&u)[4] = kus[b], (&v)[4] = kvs[b], (&x)[8] = xs[b];
+            KT ku[4], kv[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = to_odd(ku[i]), v[i] = to_odd(kv[i]);
-        if constexpr (HELD == TSP_KV_MX4) {
-            float y[8];
-            if constexpr (HALVES) {
-                // The lane's eight channels are two runs of four, which stand in the first half of some lane
-                // or the second of another.
+            for (int i = 0; i < 4; ++i) ku[i] = u[i], kv[i] = v[i];
+            turn<L, KT>(ku, kv, a.k_gamma ? a.k_gamma + h * a.d : nullptr, HALVES, unit, a.d, live, a.eps, axis, cs, sn);
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const int run = 2 * unit + r, half = a.d / 8;
-                    const bool second = run >= half;
-                    const int from = second ? run - half : run;
+            for (int i = 0; i < 4; ++i) u[i] = to_odd(ku[i]), v[i] = to_odd(kv[i]);
+            if constexpr (HELD == TSP_KV_MX4) {
+                float y[8];
+                if constexpr (HALVES) {
+                    // The lane's eight channels are two runs of four, which stand in the first half of some lane
+                    // or the second of another.
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p = __shfl(u[i], from, L), q = __shfl(v[i], from, L);
-                        y[4 * r + i] = !live ? 0.f : second ? q : p;
+                    for (int r = 0; r < 2; ++r) {
+                        const int run = 2 * unit + r, half = a.d / 8;
+                        const bool second = run >= half;
+                        const int from = second ? run - half : run;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float p = __shfl(u[i], from, L), q = __shfl(v[i], from, L);
+                            y[4 * r + i] = !live ? 0.f : second ? q : p;
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[2 * i] = u[i], y[2 * i + 1] = v[i];
+                }
+                const uint32_t kp = mx_power_of<MX_E2M1>(y), vp = mx_power_of<MX_E2M1>(x);
+                if (unit < 4 * a.cache.blocks) {        // (channels past d among them: zeros)
+                    *reinterpret_cast<uint32_t*>(to + kv_codes_at(a.cache, 0, slot) + unit * 4) = mx_codes4(y, kp);
+                    *reinterpret_cast<uint32_t*>(to + kv_codes_at(a.cache, 1, slot) + unit * 4) = mx_codes4(x, vp);
+                    if ((unit & 3) == 0) {
+                        to[kv_powers_at(a.cache, 0, slot) + unit / 4] = (uint8_t)kp;
+                        to[kv_powers_at(a.cache, 1, slot) + unit / 4] = (uint8_t)vp;
                     }
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) y[2 * i] = u[i], y[2 * i + 1] = v[i];
+            } else if (live) {
+                store_pairs<HELD, HALVES>(to, (int64_t)slot * a.d, unit, a.d, u, v);
+                store8<HELD>(to, ((1ll << a.cache.page_bits) + slot) * a.d + 8 * unit, x);
             }
-            const uint32_t kp = mx_power_of<MX_E2M1>(y), vp = mx_power_of<MX_E2M1>(x);
-            if (unit < 4 * a.cache.blocks) {        // (channels past d among them: zeros)
-                *reinterpret_cast<uint32_t*>(to + kv_codes_at(a.cache, 0, slot) + unit * 4) = mx_codes4(y, kp);
-                *reinterpret_cast<uint32_t*>(to + kv_codes_at(a.cache, 1, slot) + unit * 4) = mx_codes4(x, vp);
-                if ((unit & 3) == 0) {
-                    to[kv_powers_at(a.cache, 0, slot) + unit / 4] = (uint8_t)kp;
-                    to[kv_powers_at(a.cache, 1, slot) + unit / 4] = (uint8_t)vp;
-                }
-            }
-        } else if (live) {
-            store_pairs<HELD, HALVES>(to, (int64_t)slot * a.d, unit, a.d, u, v);
-            store8<HELD>(to, ((1ll << a.cache.page_bits) + slot) * a.d + 8 * unit, x);
         }
     }
     float fc[4], fs[4];
