@@ -332,6 +332,22 @@ def test_append_places(gpu_lib):
         torch.cuda.synchronize()
 
 
+def test_append_far_positions(gpu_lib):
+    """Positions up to 2^28: the codes are still those of 64-bit angles, to the angles' own 2^-24."""
+    import torch
+    n = 400
+    cache = gpu_lib.kv_cache(25, 16, 1, 128)
+    table = torch.arange(25, dtype=torch.int32, device="cuda").view(1, 25)
+    k = gen(1)(n, 1, 128)
+    pos = (torch.arange(n, device="cuda", dtype=torch.int32) * 671_088)[:, None].contiguous()
+    gpu_lib.kv_append(cache, k, k, table, ints([n]), pos=pos)
+    y, _ = ref.rope(k, pos, [64], 10000.0, True, None, 1e-6)
+    kd = sr.keys_of(cache, table, [n], 0)[0]
+    # between the codes of values that much smaller and larger
+    lo, hi = (sr.mx4_values(y * (1 + e)) for e in (-(2.0 ** -20), 2.0 ** -20))
+    assert bool(((kd == lo) | (kd == hi) | ((kd - y).abs() <= (sr.mx4_values(y) - y).abs() + 2.0 ** -18 * y.abs().amax())).all())
+
+
 def test_append_values(gpu_lib):
     """Blocks with Inf or NaN, of zeros, and of halfway values."""
     import torch
@@ -416,6 +432,50 @@ def test_attention_cached_behind_the_mask(gpu_lib, held, key, rows, hq):
         out = gpu_lib.attention_cached(q, cache, table, ints(lengths), offsets=ints(b), causal=causal)
         o, slack = sr.attention_cached(q, cache, table, lengths, b, causal, 0.125)
         ref.check(out, o, torch.nan_to_num(slack), "behind the mask")
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attention_cached_many_samples(gpu_lib, rows):
+    """More samples than a wave has lanes, some empty, in both kernels."""
+    import torch
+    lengths = [(i * 53) % 190 for i in range(150)]
+    cache, table = make_cache(gpu_lib, lengths, 32, 2, 64, "mx4", 3)
+    new = [0 if i % 11 == 3 else rows for i in range(150)]
+    b = ref.offsets_of(new)
+    q = gen(5)(sum(new), 4, 64).bfloat16()
+    out = gpu_lib.attention_cached(q, cache, table, ints(lengths), offsets=ints(b))
+    o, slack = sr.attention_cached(q, cache, table, lengths, b, True, 0.125)
+    ref.check(out, o, slack, "many samples")
+
+
+@pytest.mark.parametrize("rows", [1, 5, 70])
+def test_attention_cached_wide_table(gpu_lib, rows):
+    """A table for a billion keys a sample of which few are there: work is counted in coarser steps; the same bits or, where
+    the cuts lie elsewhere, within what the cuts allow."""
+    import torch
+    lengths = [500, 3000]
+    cache, table = make_cache(gpu_lib, lengths, 256, 32, 32, "mx4", 3)
+    wide = torch.full((2, 1 << 22), -1, dtype=torch.int32, device="cuda")
+    wide[:, : table.shape[1]] = table
+    q = gen(5)(2 * rows, 32, 32).bfloat16()
+    b = [0, rows, 2 * rows]
+    out = gpu_lib.attention_cached(q, cache, wide, ints(lengths), offsets=ints(b))
+    o, slack = sr.attention_cached(q, cache, table, lengths, b, True, 32 ** -0.5)
+    ref.check(out, o, slack, "wide table")
+    k, _ = gpu_lib.kv_gather(cache, wide, ints(lengths), offsets=ints(b), n=2 * rows)
+    assert torch.equal(k, gpu_lib.kv_gather(cache, table, ints(lengths), offsets=ints(b), n=2 * rows)[0])
+
+
+@pytest.mark.parametrize("held", ["mx4", "bf16"])
+def test_attention_cached_skewed(gpu_lib, held):
+    """One sample with nearly all keys, or nearly all rows, among many."""
+    for new, lengths in (([1] * 9, [3, 4, 20_000, 1, 0, 9, 70, 2, 5]), ([1, 1, 300, 1], [50, 2, 400, 900]), ([1] * 40 + [100], [30] * 41)):
+        cache, table = make_cache(gpu_lib, lengths, 64, 2, 128, held, 3)
+        b = ref.offsets_of(new)
+        q = gen(5)(sum(new), 8, 128).bfloat16()
+        out = gpu_lib.attention_cached(q, cache, table, ints(lengths), offsets=ints(b))
+        o, slack = sr.attention_cached(q, cache, table, lengths, b, True, 128 ** -0.5)
+        ref.check(out, o, slack, f"skewed {len(new)}")
 
 
 def test_attention_cached_rows(gpu_lib):
@@ -568,6 +628,21 @@ def test_two_calls_at_once(gpu_lib):
     torch.cuda.synchronize()
     for o in outs:
         assert torch.equal(o, want)
+
+
+def test_rows_past_32_bits(gpu_lib):
+    """Norms and linears of more than 4 GiB: the last rows as by themselves."""
+    import torch
+    n, c = 2_200_003, 1024
+    x = torch.zeros((n, c), dtype=torch.bfloat16, device="cuda")
+    x[-300:] = gen(1)(300, c).bfloat16()
+    tail = x[-300:].clone()
+    assert torch.equal(gpu_lib.rms_norm(x)[-300:], gpu_lib.rms_norm(tail))
+    m, t = gpu_lib.mx_quantize(x), gpu_lib.mx_quantize(tail)
+    assert same(m.codes[-300:], t.codes) and same(m.powers[-300:], t.powers)
+    w = gpu_lib.mx_quantize(gen(2)(1000, c) / 32)
+    y = gpu_lib.linear_mx(m, w)
+    assert y.numel() > 1 << 31 and torch.equal(y[-300:], gpu_lib.linear_mx(t, w))
 
 
 def test_cache_past_32_bits(gpu_lib):

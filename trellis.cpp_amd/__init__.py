@@ -1263,9 +1263,14 @@ class KVCache:
             raise ValueError(f"no cache of pages of {page} tokens (16, 32, 64, 128 or 256), {heads} heads of {d} (a multiple of 8 up to 128)")
         if data.dtype != torch.uint8 or data.dim() != 2 or data.shape[1] != size or not data.is_contiguous() or data.data_ptr() % 16:
             raise ValueError(f"data must be a contiguous uint8 [pages, {size}], 16-byte aligned")
-        self.data, self.page, self.heads, self.d, self.dtype = data, page, heads, d, dtype
+        self._data, self.page, self.heads, self.d, self.dtype = data, page, heads, d, dtype
         self.pages = data.shape[0]
         self.arg = KvCacheArg(data.data_ptr(), self.pages, page, heads, d, self.format)
+
+    @property
+    def data(self):
+        """The pages (one tensor for the cache's life: calls hold its address)."""
+        return self._data
 
 
 def kv_cache(pages: int, page: int, heads: int, d: int, dtype="mx4", device="cuda") -> KVCache:
