@@ -1011,13 +1011,23 @@ __global__ __launch_bounds__(CM_NW * 64, 2) void k_cached_many(CachedArgs) {
 }
 
 // ---- the pieces of units that were cut, joined -----------------------------------------------------------------------
-// sum_s w_s (p v)_s / sum_s w_s (sum p)_s, w_s = exp(max_s - max), in an order that the pieces' number alone sets. A workgroup
-// takes 16 / G rows of a unit at a time, G groups of 16 lanes a row, eight channels a lane: one, 4 (a wave), or 16 where units
-// have many pieces. Which units were cut only the device knows: every workgroup counts them (a launch of a workgroup for each
-// place where one can be takes 10 to 30 us, nearly all of which leave at once).
+// sum_s w_s (p v)_s / sum_s w_s (sum p)_s, w_s = exp(max_s - max), in an order that the pieces' number alone sets. Which units
+// were cut only the device knows: every workgroup counts them, and takes its share of their rows (a launch of a workgroup
+// for each place where one can be takes 10 to 30 us, nearly all of which leave at once).
 constexpr int CJ_EACH = 3, CJ_MAX = CJ_EACH * 256;      // workgroups of the first launch, at most
+
+template <bool BF16>
+__device__ __forceinline__ void join_out(const CachedArgs& a, const JoinItem& j, int row, int e, bool seen, float sum, float (&acc)[8]) {
+    const float inv = 1.f / sum;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[k] = seen ? acc[k] * inv : 0.f;
+    const int r = j.first_row + row, qi = r / a.by_share, hq = j.head * a.share + r - qi * a.share;
+    store8<BF16 ? TSP_BF16 : TSP_F16>(a.o, (int64_t)(j.row0 + qi) * a.o_row + hq * a.o_head + e, acc);
+}
+
+// Few pieces a unit: 16 / G rows at a time, G groups of 16 lanes a row (1, or 4: a wave), eight channels a lane.
 template <bool BF16, int ROWS, int G>
-__device__ __forceinline__ void join_rows(const CachedArgs& a, int g0, int first, float (*sAcc)[KV_MAX_D], float* sMax, float* sSum) {
+__device__ __forceinline__ void join_rows(const CachedArgs& a, int g0, int first) {
     constexpr int BATCH = 8;
     const int group = threadIdx.x >> 4, g = group % G, e = (threadIdx.x & 15) * 8, mine = threadIdx.x % (G * 16);
     const JoinItem j = a.join[g0];
@@ -1031,11 +1041,6 @@ __device__ __forceinline__ void join_rows(const CachedArgs& a, int g0, int first
     }
 #pragma unroll
     for (int o = G == 1 ? 8 : 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    if constexpr (G == 16) {
-        if ((threadIdx.x & 63) == 0) sMax[threadIdx.x >> 6] = top;
-        __syncthreads();
-        top = fmaxf(fmaxf(sMax[0], sMax[1]), fmaxf(sMax[2], sMax[3]));
-    }
     float sum = 0.f, acc[8] = {};
     bool any = false;
     for (int i0 = g; i0 < pieces; i0 += BATCH * G) {
@@ -1059,50 +1064,99 @@ __device__ __forceinline__ void join_rows(const CachedArgs& a, int g0, int first
             for (int k = 0; k < 8; ++k) acc[k] += c[b] * x[b][k];
         }
     }
-    // over the groups
     int seen = any;
-    if constexpr (G > 1) {
+    if constexpr (G == 4) {
         sum += __shfl_xor(sum, 16, 64), seen |= __shfl_xor(seen, 16, 64);
         sum += __shfl_xor(sum, 32, 64), seen |= __shfl_xor(seen, 32, 64);
-    }
-    if constexpr (G == 16) {
-        if ((threadIdx.x & 63) == 0) sSum[threadIdx.x >> 6] = sum;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) sAcc[g][e + k] = acc[k];
-        seen = __syncthreads_or(seen);
-        sum = (sSum[0] + sSum[1]) + (sSum[2] + sSum[3]);
-        if (g == 0) {
-#pragma unroll
-            for (int o = 1; o < 16; ++o)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) acc[k] += sAcc[o][e + k];
-        }
-    } else if constexpr (G == 4) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             acc[k] += __shfl_xor(acc[k], 16, 64);
             acc[k] += __shfl_xor(acc[k], 32, 64);
         }
     }
-    if (!live || g != 0 || e >= a.cache.d) return;
-    const float inv = 1.f / sum;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) acc[k] = seen ? acc[k] * inv : 0.f;
-    const int r = j.first_row + row, qi = r / a.by_share, hq = j.head * a.share + r - qi * a.share;
-    store8<BF16 ? TSP_BF16 : TSP_F16>(a.o, (int64_t)(j.row0 + qi) * a.o_row + hq * a.o_head + e, acc);
+    if (live && g == 0 && e < a.cache.d) join_out<BF16>(a, j, row, e, seen, sum, acc);
 }
 
+// Many pieces a unit: 32 channels of a row at a time, 64 groups of four lanes.
+struct JoinShared {
+    float weight[CJ_MAX], acc[4][32], top[4], sum[4];
+};
+template <bool BF16, int ROWS>
+__device__ __forceinline__ void join_many(const CachedArgs& a, int g0, int row, int part, JoinShared& s) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, e = part * 32 + (lane & 3) * 8;
+    const JoinItem j = a.join[g0];
+    const int pieces = j.last - g0 + 1;
+    auto at = [&](int i) { return (int64_t)(2 * (g0 + i) + (i == 0)) * ROWS + row; };
+    float2 st[CJ_EACH];
+    float top = -INFINITY, sum = 0.f;
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < CJ_EACH; ++i) {
+        const int p = i * 256 + threadIdx.x;
+        st[i] = p < pieces ? a.stat[at(p)] : float2{-INFINITY, -1.f};
+        if (st[i].y != -1.f) top = fmaxf(top, st[i].x), any = true;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    if (lane == 0) s.top[wave] = top;
+    const bool seen = __syncthreads_or(any);
+    top = fmaxf(fmaxf(s.top[0], s.top[1]), fmaxf(s.top[2], s.top[3]));
+#pragma unroll
+    for (int i = 0; i < CJ_EACH; ++i) {
+        const int p = i * 256 + threadIdx.x;
+        if (p >= pieces) break;
+        const float c = st[i].y == -1.f ? -1.f : st[i].x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st[i].x - top) * a.scale2);
+        s.weight[p] = c;
+        if (c != -1.f) sum += c * st[i].y;
+    }
+    sum = group_sum<64>(sum);
+    if (lane == 0) s.sum[wave] = sum;
+    __syncthreads();
+    sum = (s.sum[0] + s.sum[1]) + (s.sum[2] + s.sum[3]);
+    float acc[8] = {};
+    if (e < a.cache.d) {
+        constexpr int BATCH = 4;
+        for (int i0 = threadIdx.x >> 2; i0 < pieces; i0 += BATCH * 64) {
+            float c[BATCH], x[BATCH][8];
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                const int i = i0 + b * 64;
+                c[b] = i < pieces ? s.weight[i] : -1.f;
+                if (c[b] != -1.f) load8<TSP_F32>(a.part, at(i) * a.cache.d + e, x[b]);
+            }
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                if (c[b] == -1.f) continue;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) acc[k] += c[b] * x[b][k];
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+#pragma unroll
+        for (int o = 4; o < 64; o <<= 1) acc[k] += __shfl_xor(acc[k], o, 64);
+        if (lane < 4) s.acc[wave][lane * 8 + k] = acc[k];
+    }
+    __syncthreads();
+    if (threadIdx.x < 4 && e < a.cache.d) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] = (s.acc[0][lane * 8 + k] + s.acc[1][lane * 8 + k]) + (s.acc[2][lane * 8 + k] + s.acc[3][lane * 8 + k]);
+        join_out<BF16>(a, j, row, e, seen, sum, acc);
+    }
+}
+
+// G: 1 or 4 groups of lanes a row, 64 of join_many.
 template <bool BF16, int ROWS, int G>
 __global__ __launch_bounds__(256) void k_cached_join(CachedArgs a) {
-    constexpr int ITEMS = 16 / G;
-    __shared__ float sAcc[G == 16 ? 16 : 1][KV_MAX_D], sMax[4], sSum[4];
+    __shared__ JoinShared s;
     __shared__ int sCount[CJ_EACH * 4], sFound[2];
-    const int wave = threadIdx.x >> 6;
+    const int wave = threadIdx.x >> 6, blocks = a.cache.blocks;
     int count[CJ_EACH], end[CJ_EACH];
 #pragma unroll
     for (int i = 0; i < CJ_EACH; ++i) {
-        const int w = i * 256 + threadIdx.x;
-        count[i] = w < a.groups ? (min(a.join[w].rows, ROWS) + ITEMS - 1) / ITEMS : 0;
+        const int w = i * 256 + threadIdx.x, rows = w < a.groups ? min(a.join[w].rows, ROWS) : 0;
+        count[i] = G == 64 ? rows * blocks : (rows + 16 / G - 1) / (16 / G);
     }
 #pragma unroll
     for (int i = 0; i < CJ_EACH; ++i) {
@@ -1124,8 +1178,9 @@ __global__ __launch_bounds__(256) void k_cached_join(CachedArgs a) {
         for (int i = 0; i < CJ_EACH; ++i)
             if (item < end[i] && item >= end[i] - count[i]) sFound[0] = i * 256 + threadIdx.x, sFound[1] = item - (end[i] - count[i]);
         __syncthreads();
-        const int g0 = sFound[0], first = sFound[1] * ITEMS;
-        join_rows<BF16, ROWS, G>(a, g0, first, sAcc, sMax, sSum);
+        const int g0 = sFound[0], x = sFound[1];
+        if constexpr (G == 64) join_many<BF16, ROWS>(a, g0, x / blocks, x % blocks, s);
+        else join_rows<BF16, ROWS, G>(a, g0, x * (16 / G));
         __syncthreads();
     }
 }
@@ -1142,7 +1197,7 @@ struct CachedCut {
     int join;           // groups of lanes a row in the join
     unsigned joins;     // its workgroups
 };
-CachedCut cached_cut(int64_t nq, int samples, int hkv, int share, int64_t keys, bool mx4) {
+CachedCut cached_cut(int64_t nq, int samples, int hkv, int share, int64_t keys, int d, bool mx4) {
     CachedCut c;
     const int64_t each = ceil_div(nq, samples) * share;
     c.rows = each <= 16 ? 16 : each <= 32 && mx4 ? 32 : CM_ROWS;      // (two tiles of rows beside 16-bit keys would spill registers)
@@ -1159,8 +1214,11 @@ CachedCut cached_cut(int64_t nq, int samples, int hkv, int share, int64_t keys, 
     // two or three a CU, as registers and LDS allow, where the line can be that long
     c.groups = (int)std::min<int64_t>(c.rows == 16 ? 768 : 512, ceil_div(longest(), c.least));
     const int64_t cut = std::min<int64_t>(c.units, c.groups), pieces = c.groups / std::max<int64_t>(1, ceil_div(nq * share, c.rows) * hkv);
-    c.join = pieces > 32 ? 16 : pieces > 2 ? 4 : 1;
-    c.joins = (unsigned)std::min<int64_t>(cut * ceil_div(std::min<int64_t>(each, c.rows), 16 / c.join), 2048);
+    const int64_t rows = std::min<int64_t>(each, c.rows);
+    // (64 where its workgroups are few: 1 row on 200,000 keys 33 us by waves, 26 so; 256 rows of 4 heads on 20,000 44 and 57)
+    const int64_t wide = cut * rows * ((d + 31) / 32);
+    c.join = pieces > 32 && wide <= 1024 ? 64 : pieces > 2 ? 4 : 1;
+    c.joins = (unsigned)std::min<int64_t>(c.join == 64 ? wide : cut * ceil_div(rows, 16 / c.join), 2048);
     return c;
 }
 size_t cached_workspace(const CachedCut& c, int d) {
@@ -1174,7 +1232,8 @@ using namespace tsp;
 
 extern "C" size_t tsp_attention_cached_workspace_bytes(int64_t nq, int samples, int hq, const tsp_kv_cache* cache, int max_pages) {
     if (!cache || !kv_valid(*cache) || nq <= 0 || nq >= (1ll << 31) || samples <= 0 || hq <= 0 || hq % cache->heads || max_pages <= 0) return 0;
-    return cached_workspace(cached_cut(nq, samples, cache->heads, hq / cache->heads, (int64_t)max_pages * cache->page, cache->format == TSP_KV_MX4), cache->d);
+    return cached_workspace(cached_cut(nq, samples, cache->heads, hq / cache->heads, (int64_t)max_pages * cache->page, cache->d,
+                                       cache->format == TSP_KV_MX4), cache->d);
 }
 
 extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, int hq, const tsp_kv_cache* cache, const int32_t* d_offsets,
@@ -1204,7 +1263,7 @@ extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, i
                 "tsp_attention_cached: out must not alias q or the cache");
     const int share = hq / c.heads;
     TSP_REQUIRE(nq * share < (1ll << 31) - 1024, TSP_ERR_INVALID, "tsp_attention_cached: too many rows");
-    const CachedCut cut = cached_cut(nq, samples, c.heads, share, (int64_t)max_pages * c.page, c.format == TSP_KV_MX4);
+    const CachedCut cut = cached_cut(nq, samples, c.heads, share, (int64_t)max_pages * c.page, c.d, c.format == TSP_KV_MX4);
     TSP_REQUIRE(cut.units < 1ll << 29, TSP_ERR_INVALID, "tsp_attention_cached: too many rows and heads");
     const size_t need = cached_workspace(cut, c.d);
     TSP_REQUIRE(d_workspace, TSP_ERR_INVALID, "tsp_attention_cached: null workspace");
@@ -1236,7 +1295,7 @@ extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, i
         constexpr int ROWS = decltype(rows)::value;
         if (cut.groups == 1) return;
         const dim3 grid(cut.joins), block(256);
-        if (cut.join == 16) hipLaunchKernelGGL((k_cached_join<BF16, ROWS, 16>), grid, block, 0, s, a);
+        if (cut.join == 64) hipLaunchKernelGGL((k_cached_join<BF16, ROWS, 64>), grid, block, 0, s, a);
         else if (cut.join == 4) hipLaunchKernelGGL((k_cached_join<BF16, ROWS, 4>), grid, block, 0, s, a);
         else hipLaunchKernelGGL((k_cached_join<BF16, ROWS, 1>), grid, block, 0, s, a);
     };
