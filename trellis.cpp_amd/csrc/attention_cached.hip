@@ -1213,11 +1213,11 @@ CachedCut cached_cut(int64_t nq, int samples, int hkv, int share, int64_t keys, 
     c.least = std::max(1, ((c.rows == CM_ROWS ? 4 : 2 * CF_NW) << c.finer) >> c.coarser);
     // two or three a CU, as registers and LDS allow, where the line can be that long
     c.groups = (int)std::min<int64_t>(c.rows == 16 ? 768 : 512, ceil_div(longest(), c.least));
-    const int64_t cut = std::min<int64_t>(c.units, c.groups), pieces = c.groups / std::max<int64_t>(1, ceil_div(nq * share, c.rows) * hkv);
+    const int64_t cut = std::min<int64_t>(c.units, c.groups), pieces = c.groups / (std::max<int64_t>(ceil_div(nq * share, c.rows), std::min<int64_t>(samples, nq)) * hkv);
     const int64_t rows = std::min<int64_t>(each, c.rows);
     // (64 where its workgroups are few: 1 row on 200,000 keys 33 us by waves, 26 so; 256 rows of 4 heads on 20,000 44 and 57)
     const int64_t wide = cut * rows * ((d + 31) / 32);
-    c.join = pieces > 32 && wide <= 1024 ? 64 : pieces > 2 ? 4 : 1;
+    c.join = pieces > 32 && wide <= 2048 ? 64 : pieces > 2 ? 4 : 1;
     c.joins = (unsigned)std::min<int64_t>(c.join == 64 ? wide : cut * ceil_div(rows, 16 / c.join), 2048);
     return c;
 }
