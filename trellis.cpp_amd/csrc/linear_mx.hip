@@ -396,15 +396,18 @@ __global__ __launch_bounds__(LF_NW * 64) void k_linear_mx_few(LinearArgs a) {
 
 // The tile with the least time of its rounds. A step of 128 channels takes a workgroup so many us where the device is full
 // (8,192 rows and outputs of 8,192 channels) and where it has a CU to itself (1,000 rows, 4,096 -> 1,024); a tile's first loads
-// and its rows' way out some more. (35,001 rows, 4,096 -> 1,024, fp32 out: 323 us by tiles of 256 x 256, 299 by 128 x 128;
-// 1,024 -> 4,096 in bf16: 190 and 205; 1,000 rows, 4,096 -> 1,024 in bf16: 53, 33, 22 and 18 by the four.)
+// and its rows' way out some more. (us by tiles of 256 x 256, 256 x 128 with two steps on their way, 128 x 128: 8,192 rows and
+// outputs of 8,192 channels, bf16 600, 552, 640, fp32 out 870, 915, 940; 35,001 rows, 4,096 -> 1,024, fp32 out 330, 287, 298;
+// 1,024 -> 4,096 in bf16 191, 230, 208. 1,000 rows, 4,096 -> 1,024 in bf16: 53, 33, 22 and 18 by 256 x 256, 128 x 128, 128 x 64
+// and 64 x 64.)
 int linear_shape(int64_t n, int ci, int co, bool exact) {
     struct Shape { int x, w, slots; double full, alone, full_exact, alone_exact, rest; };
-    static const Shape shapes[4] = {{256, 256, 256, 2.08, 1.4, 3.4, 2.7, 6.}, {128, 128, 512, 1.2, 0.8, 1.84, 1.4, 3.},
-                                    {128, 64, 512, 0.98, 0.55, 1.17, 0.72, 2.5}, {64, 64, 512, 0.7, 0.4, 0.83, 0.7, 2.}};
+    static const Shape shapes[5] = {{256, 256, 256, 2.08, 1.4, 3.4, 2.7, 6.}, {128, 128, 512, 1.2, 0.8, 1.84, 1.4, 3.},
+                                    {128, 64, 512, 0.98, 0.55, 1.17, 0.72, 2.5}, {64, 64, 512, 0.7, 0.4, 0.83, 0.7, 2.},
+                                    {256, 128, 256, 1., 0.85, 1.71, 1.35, 5.}};
     int best = 0;
     double least = 1e30;
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 5; ++i) {
         const Shape& s = shapes[i];
         const int64_t tiles = ceil_div(n, s.x) * ceil_div(co, s.w), rest = tiles % s.slots, steps = ceil_div(ci, LM_K);
         const double full = steps * (exact ? s.full_exact : s.full) + s.rest, alone = steps * (exact ? s.alone_exact : s.alone) + s.rest;
@@ -487,7 +490,7 @@ extern "C" int tsp_linear_mx(const void* d_x, const uint8_t* d_x_powers, int64_t
             constexpr bool EXACT = decltype(exact)::value;
             const dim3 grid((unsigned)ceil_div(tiles, 8) * 8), block(WX * WW * 64);
             if (ci % LM_K == 0) hipLaunchKernelGGL((k_linear_mx<TX, TW, WX, WW, ST, EXACT, false>), grid, block, 0, s, a);
-            else hipLaunchKernelGGL((k_linear_mx<TX, TW, WX, WW, ST, EXACT, true>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((k_linear_mx<TX, TW, WX, WW, TX + TW == 384 ? 2 : ST, EXACT, true>), grid, block, 0, s, a);     // (its powers' places would not fit)
         });
         return TSP_OK;
     };
@@ -496,6 +499,7 @@ extern "C" int tsp_linear_mx(const void* d_x, const uint8_t* d_x_powers, int64_t
     if (shape == 0) rc = go(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{});
     else if (shape == 1) rc = go(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
     else if (shape == 2) rc = go(integral_constant<int, 128>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 3>{});
+    else if (shape == 4) rc = go(integral_constant<int, 256>{}, integral_constant<int, 128>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{}, integral_constant<int, 3>{});
     else rc = go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
     if (rc != TSP_OK) return rc;
     TSP_CHECK_LAUNCH();
