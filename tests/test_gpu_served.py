@@ -157,7 +157,7 @@ def test_rms_norm_places(gpu_lib):
 
 # ---- linear -------------------------------------------------------------------------------------
 LINEAR_CASES = [(1, 32, 1), (1, 1024, 64), (5, 96, 27), (3, 160, 100), (16, 128, 16), (17, 512, 333), (64, 2048, 72), (65, 256, 1000), (128, 1056, 130),
-                (200, 32, 7), (257, 640, 260), (1000, 1024, 1000), (515, 4096, 520), (2606, 768, 256)]
+                (200, 32, 7), (257, 640, 260), (1000, 1024, 1000), (515, 4096, 520), (2606, 768, 256), (3001, 2048, 2500), (3001, 2080, 2500)]
 
 
 @pytest.mark.parametrize("n,ci,co", LINEAR_CASES)
@@ -432,6 +432,38 @@ def test_attention_cached_behind_the_mask(gpu_lib, held, key, rows, hq):
         out = gpu_lib.attention_cached(q, cache, table, ints(lengths), offsets=ints(b), causal=causal)
         o, slack = sr.attention_cached(q, cache, table, lengths, b, causal, 0.125)
         ref.check(out, o, torch.nan_to_num(slack), "behind the mask")
+
+
+@pytest.mark.parametrize("key", ["bf16", "f16"])
+@pytest.mark.parametrize("rows", [4, 12, 150])
+def test_attention_cached_largest_values(gpu_lib, rows, key):
+    """A value at the end of the heads' range, whose code and power are past it, has no effect on the rows that do not see its key."""
+    import torch
+    cache = gpu_lib.kv_cache(20, 16, 1, 64)
+    n = 200
+    table = torch.arange(20, dtype=torch.int32, device="cuda").view(1, 20)
+    k, v = gen(1)(n, 1, 64).to(dtype(key)), gen(2)(n, 1, 64).to(dtype(key))
+    gpu_lib.kv_append(cache, k, v, table, ints([n]))
+    q = gen(3)(rows, 2, 64).to(dtype(key))
+    want = gpu_lib.attention_cached(q, cache, table, ints([n]))
+    v[n - 1, 0, 7] = torch.finfo(dtype(key)).max
+    gpu_lib.kv_append(cache, k, v, table, ints([n]))
+    got = gpu_lib.attention_cached(q, cache, table, ints([n]))
+    assert torch.equal(got[:-1], want[:-1])
+    assert bool(torch.isinf(got[-1, :, 7]).all())      # (the code nearest to it stands for 2^128, or 2^16)
+
+
+def test_attention_cached_falling_offsets(gpu_lib):
+    """Offsets that fall give no sample any rows, however many their samples would have together."""
+    import torch
+    cache, table = make_cache(gpu_lib, [64], 16, 2, 64, "mx4", 8)
+    for n in (12, 5000):
+        q = gen(4)(n, 4, 64).bfloat16()
+        for samples in (3, 64, 301):
+            out = torch.full_like(q, 7.0)
+            gpu_lib.attention_cached(q, cache, table.expand(samples, -1).contiguous(), ints([64] * samples),
+                                     offsets=ints([(i % 2) * n for i in range(samples + 1)]), out=out)
+            assert bool((out == 7).all())
 
 
 @pytest.mark.parametrize("rows", [1, 40])

@@ -116,11 +116,15 @@ __device__ __forceinline__ Line make_line(const Args& a) {
         l.w = sample_work<ROWS, TILE>(a, 0);
         l.length = l.end = __builtin_amdgcn_readfirstlane(l.w.before(l.w.count) * a.cache.heads);
     } else {
+        bool falls = false;
         for (int s0 = 0; s0 < a.samples; s0 += 64) {
-            l.w = sample_work<ROWS, TILE>(a, s0 + (threadIdx.x & 63));
+            const int s = s0 + (threadIdx.x & 63);
+            l.w = sample_work<ROWS, TILE>(a, s);
             l.end = l.length + scan64(l.w.before(l.w.count) * a.cache.heads);
             l.length = __builtin_amdgcn_readlane(l.end, 63);
+            if (s < a.samples) falls |= a.q_off[s] > a.q_off[s + 1];
         }
+        if (__any(falls)) l.length = 0;      // (samples would overlap, and the line could be of any length: no row is anyone's)
     }
     l.length = __builtin_amdgcn_readfirstlane(l.length);
     l.per = max(a.least, (int)(l.length + a.groups - 1) / FastDiv{a.by_groups.mul, a.by_groups.shift});
@@ -390,13 +394,12 @@ __global__ __launch_bounds__(CF_NW * 64, 2) void k_cached_few(CachedArgs) {
                 if constexpr (MX4) {
                     if (16 * VP < 64 && lane >= 16 * VP) continue;
                     const float s = mx_scale(w.vp[kb]);
-                    odd |= w.vp[kb] == 255;
+                    odd |= w.vp[kb] >= (BF16 ? 253 : 141);      // (NaN, and powers with which the largest codes are past the range)
                     int to = cv_piece<DP>(v_key, v_piece_of * 4);
                     asm volatile("" : "+v"(to));
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const u32x4_t x = widen4<BF16>(w.v[kb][0][j], s);
-                        if constexpr (!BF16) odd |= any_nonfinite<BF16>(x);
                         *reinterpret_cast<u32x4_t*>(sV + kb * 16 * DP * 2 + (to ^ (j * 16))) = x;
                     }
                 } else {

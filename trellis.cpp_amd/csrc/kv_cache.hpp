@@ -25,12 +25,6 @@ struct KvArgs {
     int page_bits, heads, d, blocks;     // page = 1 << page_bits tokens
 };
 
-// Keys of sample s that its pages can hold.
-__device__ __forceinline__ int kv_length(const KvArgs& a, int s) {
-    const int64_t most = (int64_t)a.max_pages << a.page_bits;
-    return (int)min((int64_t)max(a.lengths[s], 0), most);
-}
-
 // The bytes of key head `head` in the page that holds key j of sample s (0 <= j < max_pages * page), or NULL where
 // the table names none of the pool's.
 __device__ __forceinline__ uint8_t* kv_head(const KvArgs& a, int s, int64_t j, int head) {
