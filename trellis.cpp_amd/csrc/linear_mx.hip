@@ -396,23 +396,28 @@ __global__ __launch_bounds__(LF_NW * 64) void k_linear_mx_few(LinearArgs a) {
 
 // The tile with the least time of its rounds. A step of 128 channels takes a workgroup so many us where the device is full
 // (8,192 rows and outputs of 8,192 channels) and where it has a CU to itself (1,000 rows, 4,096 -> 1,024); a tile's first loads
-// and its rows' way out some more. (us by tiles of 256 x 256, 256 x 128 with two steps on their way, 128 x 128: 8,192 rows and
-// outputs of 8,192 channels, bf16 600, 552, 640, fp32 out 870, 915, 940; 35,001 rows, 4,096 -> 1,024, fp32 out 330, 287, 298;
-// 1,024 -> 4,096 in bf16 191, 230, 208. 1,000 rows, 4,096 -> 1,024 in bf16: 53, 33, 22 and 18 by 256 x 256, 128 x 128, 128 x 64
-// and 64 x 64.)
-int linear_shape(int64_t n, int ci, int co, bool exact) {
-    struct Shape { int x, w, slots; double full, alone, full_exact, alone_exact, rest; };
-    static const Shape shapes[5] = {{256, 256, 256, 2.08, 1.4, 3.4, 2.7, 6.}, {128, 128, 512, 1.2, 0.8, 1.84, 1.4, 3.},
-                                    {128, 64, 512, 0.98, 0.55, 1.17, 0.72, 2.5}, {64, 64, 512, 0.7, 0.4, 0.83, 0.7, 2.},
-                                    {256, 128, 256, 1., 0.85, 1.71, 1.35, 5.}};
+// and its rows' way out some more, three times that where a residual is read. us by tiles of 256 x 256, 192 x 256 (fp32 out alone),
+// 128 x 128, 128 x 64 and 64 x 64, bf16 out / fp32 out with a residual: 35,001 rows, 4,096 -> 1,024: 220, -, 259, 296, 354 / 398,
+// 340, 351, 401, 454; 1,024 -> 4,096: 187, -, 219, 265, 374 / 500, 503, 436, 489, 651; 12,345 rows, 1,024 -> 1,024: 22, -, 26, 30,
+// 38 / 48, -, 43, 46, 54; 1,000 rows, 4,096 -> 1,024: 56, -, 36, 20, 16 / 113, -, 45, 27, 20; 8,192 rows, 8,192 -> 8,192: 539, -,
+// 806, 1,040, 1,291 / 975, 1,115, 1,095, 1,324, 1,592. (More waves a tile than its products need hide the loads of what lies in
+// memory: 128 x 128 by eight takes 351 where four take 363. 256 x 128 with two steps on their way: no faster than the best.)
+int linear_shape(int64_t n, int ci, int co, bool exact, bool residual) {
+    struct Times { double full, alone, rest; };
+    struct Shape { int x, w, slots; Times by[2]; };
+    static const Shape shapes[5] = {{256, 256, 256, {{2.05, 1.56, 6.}, {3.4, 2.7, 10.}}}, {192, 256, 256, {{}, {2.6, 2.2, 9.}}},
+                                    {128, 128, 512, {{1.4, 1., 3.}, {1.95, 1.3, 3.2}}}, {128, 64, 512, {{0.95, 0.55, 2.5}, {1.23, 0.74, 2.}}},
+                                    {64, 64, 512, {{0.55, 0.42, 2.}, {0.74, 0.55, 1.5}}}};
     int best = 0;
     double least = 1e30;
     for (int i = 0; i < 5; ++i) {
+        if (i == 1 && !exact) continue;
         const Shape& s = shapes[i];
-        const int64_t tiles = ceil_div(n, s.x) * ceil_div(co, s.w), rest = tiles % s.slots, steps = ceil_div(ci, LM_K);
-        const double full = steps * (exact ? s.full_exact : s.full) + s.rest, alone = steps * (exact ? s.alone_exact : s.alone) + s.rest;
+        const Times& t = s.by[exact];
+        const int64_t tiles = ceil_div(n, s.x) * ceil_div(co, s.w), last = tiles % s.slots, steps = ceil_div(ci, LM_K);
+        const double out = t.rest * (residual ? 3. : 1.), full = steps * t.full + out, alone = steps * t.alone + out;
         // (a round of at most a workgroup a CU is as long as one alone; one of nearly 256 large ones is not)
-        const double time = (double)(tiles / s.slots) * full + (rest == 0 ? 0. : rest <= (s.slots == 256 ? 128 : 256) ? alone : full);
+        const double time = (double)(tiles / s.slots) * full + (last == 0 ? 0. : last <= (s.slots == 256 ? 128 : 256) ? alone : full);
         if (time < least) least = time, best = i;
     }
     return best;
@@ -460,10 +465,12 @@ extern "C" int tsp_linear_mx(const void* d_x, const uint8_t* d_x_powers, int64_t
         else go(std::false_type{});
     };
     // Few rows by the other kernel, with two tiles of outputs a workgroup where there are many: us, by it (one tile, two) and by
-    // tiles, in bf16 / fp32. 5 rows, 1,024 -> 4,096: 3.6 (3.8) and 5.4 / 3.9 (4.8) and 8.2. 32 rows, 4,096 -> 1,024: 10.1 (12.8)
-    // and 12.1 / 10.6 (13.0) and 22.8; 48: 12.9 and 12.1 / 13.3 and 22.9. 32 rows, 8,192 -> 8,192: 36 (24.9) and 27.3 / 37 (25.9)
-    // and 47; 4,096 -> 16,384: 37 (25) and 16.9 / 39 (27) and 27; 5 rows of it 17.8 (17.5) and 16.8 / 21.3 (19.9) and 26.4.
-    if (n <= 16 || (co <= 8192 && n <= (out_dtype == TSP_F32 ? 64 : 32))) {
+    // tiles, in bf16 / fp32. 5 rows, 1,024 -> 4,096: 3.9 (4.1) and 4.9 / 4.2 (5.0) and 6.1; 4,096 -> 5,000: 10.1 (9.1) and 9.8 / 11.0
+    // (10.2) and 15.3, -> 8,192: 10.3 (9.3) and 13.1 / 11.0 (10.2) and 16.0, -> 16,384: 18.1 (17.7) and 14.8 / 22.0 (20.3) and 17.6.
+    // 32 rows, 1,024 -> 1,024: 4.4 (5.2) and 5.2 / 5.4 (5.9) and 6.8; 4,096 -> 1,024: 10.3 (13.1) and 9.9 / 10.8 (13.3) and 15.3,
+    // -> 8,192: 19.9 (14.0) and 13.5 / 21.0 (14.3) and 16.6. 64 rows, 1,024 -> 1,024: 6.0 (6.8) and 5.0 / 6.5 (7.6) and 6.4.
+    const bool wide = co > 4096;
+    if (co <= 8192 && n <= (out_dtype == TSP_F32 ? (wide ? 32 : 48) : wide ? 16 : 32)) {
         by_form([&](auto exact) {
             constexpr bool EXACT = decltype(exact)::value;
             auto few = [&](auto rt, auto wt) {
@@ -473,34 +480,45 @@ extern "C" int tsp_linear_mx(const void* d_x, const uint8_t* d_x_powers, int64_t
             auto by_rows = [&](auto wt) {
                 if (n <= 16) few(integral_constant<int, 1>{}, wt);
                 else if (n <= 32) few(integral_constant<int, 2>{}, wt);
-                else few(integral_constant<int, 4>{}, wt);
+                else if constexpr (EXACT && decltype(wt)::value == 1) few(integral_constant<int, 4>{}, wt);
             };
-            if (co >= 8192) by_rows(integral_constant<int, 2>{});
+            if (wide) by_rows(integral_constant<int, 2>{});
             else by_rows(integral_constant<int, 1>{});
         });
         TSP_CHECK_LAUNCH();
         return TSP_OK;
     }
-    auto go = [&](auto tx, auto tw, auto wx, auto ww, auto stages) -> int {
+    auto go = [&](auto tx, auto tw, auto wx, auto ww, auto stages, auto exact, auto any) -> int {
         constexpr int TX = decltype(tx)::value, TW = decltype(tw)::value, WX = decltype(wx)::value, WW = decltype(ww)::value, ST = decltype(stages)::value;
         const int64_t tiles = ceil_div(n, TX) * ceil_div(co, TW);
         TSP_REQUIRE(tiles * WX * WW * 64 < (1ll << 31), TSP_ERR_INVALID, "tsp_linear_mx: too many rows and outputs");
         a.tiles = (int)tiles;
-        by_form([&](auto exact) {
-            constexpr bool EXACT = decltype(exact)::value;
-            const dim3 grid((unsigned)ceil_div(tiles, 8) * 8), block(WX * WW * 64);
-            if (ci % LM_K == 0) hipLaunchKernelGGL((k_linear_mx<TX, TW, WX, WW, ST, EXACT, false>), grid, block, 0, s, a);
-            else hipLaunchKernelGGL((k_linear_mx<TX, TW, WX, WW, TX + TW == 384 ? 2 : ST, EXACT, true>), grid, block, 0, s, a);     // (its powers' places would not fit)
-        });
+        hipLaunchKernelGGL((k_linear_mx<TX, TW, WX, WW, ST, decltype(exact)::value, decltype(any)::value>), dim3((unsigned)ceil_div(tiles, 8) * 8),
+                           dim3(WX * WW * 64), 0, s, a);
         return TSP_OK;
     };
-    const int shape = linear_shape(n, ci, co, out_dtype == TSP_F32);
-    int rc;
-    if (shape == 0) rc = go(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{});
-    else if (shape == 1) rc = go(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
-    else if (shape == 2) rc = go(integral_constant<int, 128>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 3>{});
-    else if (shape == 4) rc = go(integral_constant<int, 256>{}, integral_constant<int, 128>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{}, integral_constant<int, 3>{});
-    else rc = go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
+    const int shape = linear_shape(n, ci, co, out_dtype == TSP_F32, d_residual != nullptr);
+    int rc = TSP_OK;
+    by_form([&](auto exact) {
+        auto by_steps = [&](auto any) {
+            // (16 waves of 64 x 64 where 16-bit outputs' products are short; eight of 128 x 64 for fp32's, or channels that are
+            // no whole steps, whose powers would take more LDS by 16: 8,192^3 in bf16 539 and 619 us, in fp32 960 and 880)
+            constexpr int WX = decltype(exact)::value || decltype(any)::value ? 2 : 4;
+            const integral_constant<int, 64> c64;
+            const integral_constant<int, 128> c128;
+            const integral_constant<int, 256> c256;
+            const integral_constant<int, 2> c2;
+            const integral_constant<int, 3> c3;
+            const integral_constant<int, 4> c4;
+            if (shape == 0) rc = go(c256, c256, integral_constant<int, WX>{}, c4, c2, exact, any);
+            else if (shape == 2) rc = go(c128, c128, c2, c4, c2, exact, any);
+            else if (shape == 3) rc = go(c128, c64, c4, c2, c3, exact, any);
+            else if (shape == 4) rc = go(c64, c64, c2, c2, c4, exact, any);
+            else if constexpr (decltype(exact)::value) rc = go(integral_constant<int, 192>{}, c256, c2, c4, c2, exact, any);
+        };
+        if (ci % LM_K == 0) by_steps(std::false_type{});
+        else by_steps(std::true_type{});
+    });
     if (rc != TSP_OK) return rc;
     TSP_CHECK_LAUNCH();
     return TSP_OK;
