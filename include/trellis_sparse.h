@@ -543,7 +543,8 @@ int tsp_mx_quantize(const void* d_x, int x_dtype, int64_t n, int c, void* d_code
  * aligned; ci a multiple of 32); act 1 is y * sigmoid(y); bias f32 [co] and residual f32 [n][co] or NULL, out any dtype.
  * out may be the residual where it is f32, and must not overlap the inputs otherwise. With 16-bit outputs products are
  * added at the matrix cores' 8-bit precision (off by some 1.5e-5 of the result in the 2-norm, a small part of the
- * output's rounding); with f32 outputs in fp32, at half the rate. The result does not depend on what the workspace,
+ * output's rounding); with f32 outputs in fp32, at half the rate, and there codes times their power have to fit bf16: values
+ * below 2^-126 lose bits and powers above 246 may overflow. The result does not depend on what the workspace,
  * 16-byte aligned, of tsp_linear_mx_workspace_bytes bytes held (0, and NULL will do, where it needs none). */
 size_t tsp_linear_mx_workspace_bytes(int64_t n, int ci, int co);
 int tsp_linear_mx(const void* d_x, const uint8_t* d_x_powers, int64_t n, int ci, const void* d_w, const uint8_t* d_w_powers,
@@ -587,9 +588,11 @@ int tsp_kv_gather(const tsp_kv_cache* cache, int64_t n, const int32_t* d_offsets
 
 /* Softmax attention of q's rows to their samples' cached keys, as tsp_attention computes it: of sample s with m rows,
  * row i sees all of its d_lengths[s] keys, or with causal != 0 those with j <= i + (d_lengths[s] - m). A row that sees
- * no key gets zeros; a key that a row does not see has no effect on it, whatever it holds. q and out f16 or bf16, of the cache's
- * dtype where that holds 16 bits; hq a multiple of the cache's heads; scale > 0; with f16 heads a 4-bit cache's values have
- * to fit f16. nq * hq / heads and max_pages * page below 2^31 - 2^16. The line of all work is cut evenly over the device
+ * no key gets zeros; a key that a row does not see has no effect on it, whatever it holds. Offsets that fall give
+ * no sample any rows. q and out f16 or bf16, of the cache's dtype where that holds 16 bits; hq a multiple of the
+ * cache's heads; scale > 0; with f16 heads a 4-bit cache's values have to fit f16. Sums of p v are fp32, with p up to 2^8 in
+ * bf16: values near fp32's end may overflow before the division. nq * hq / heads and max_pages * page below
+ * 2^31 - 2^16. The line of all work is cut evenly over the device
  * whatever the samples' lengths, and joined in the workspace, 16-byte aligned, of
  * tsp_attention_cached_workspace_bytes bytes; the result does not depend on what that held, nor on the order in
  * which workgroups run. out must not overlap the inputs. */

@@ -18,6 +18,16 @@
 // Two kernels. Few rows (k_cached_few): waves of their own, each with every fourth tile of 32 keys: K goes from memory to its
 // operand, V through a piece of LDS that is the wave's alone, where it is turned. Many rows (k_cached_many): four waves of 32
 // rows share a tile of 64 keys, widened into LDS by all of them.
+//
+// What bounds them, in bf16, heads of 128, 4 bits. One row of 16 heads on 2, 40,009 keys: 16.5 us, of which the first kernel is 11 (768
+// workgroups: the latency of lengths, table and first tile, one after the other) and the join 6; 200,000 keys 26. 16
+// samples' tokens, 16 heads on 4, 400,009 keys: 54 us, 47 of them at 4.6 TB/s of cache read, where widening keeps the vector units
+// 40 % busy; in 16 bits 179 (4.6 TB/s). 5,003 rows on 35,001 keys, two samples: 826 us, 974 TFLOP/s; the matrix cores are
+// 43 % busy at 2.0 GHz, the vector units, which widen, form exponents and round, 45 %. A causal prompt of 8,000 rows 415; 20,000
+// rows of 16 heads of 64 on 1,029 keys 184.
+// Tried and taken back: eight waves a workgroup of many rows (tiles wait for the slowest wave), four waves a SIMD in either kernel
+// (registers spilled: a kernel with any scratch starts some 7 us later), one LDS array for both buffers (every
+// load waited for), a launch of the join for each place where a cut can be (10 to 30 us).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
