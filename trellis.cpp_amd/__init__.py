@@ -897,13 +897,13 @@ def _launch(device, stream, call, *args):
 
 def _same_device(device, *named):
     """named: name, tensor, name, tensor, ..."""
-    if device.type != "cuda":
+    index = device.index      # (None: not a GPU's)
+    if index is None or device.type != "cuda":
         raise ValueError("tensors must live on the GPU")
-    index = device.index
-    for i in range(1, len(named), 2):
-        t = named[i]
+    for t in named[1::2]:
         if t is not None and t.get_device() != index:
-            raise ValueError(f"{named[i - 1]} must live on {device}, got {t.device}")
+            name = next(n for n, u in zip(named[::2], named[1::2]) if u is t)
+            raise ValueError(f"{name} must live on {device}, got {t.device}")
 
 
 def _p(t) -> int:
@@ -1126,14 +1126,15 @@ def _check_mx(m, n, c, device, name: str):
     """n and c may be None: any. -> (n, c)"""
     torch = _torch()
     codes, powers = m
-    if codes.dtype != torch.float8_e4m3fn or powers.dtype not in (torch.float8_e8m0fnu, torch.uint8) or codes.dim() != 2 or powers.dim() != 2:
+    shape, blocks = codes.shape, powers.shape
+    if codes.dtype != torch.float8_e4m3fn or (powers.dtype != torch.float8_e8m0fnu and powers.dtype != torch.uint8) or len(shape) != 2:
         raise ValueError(f"{name} must be Mx(codes float8_e4m3fn [N, C], powers float8_e8m0fnu [N, C / 32])")
-    rows, ch = codes.shape
-    if (n is not None and rows != n) or (c is not None and ch != c) or ch % 32 or tuple(powers.shape) != (rows, ch // 32):
-        raise ValueError(f"{name} has codes {list(codes.shape)} and powers {list(powers.shape)}, expected {[n, c]} and one for 32 channels")
-    if not codes.is_contiguous() or not powers.is_contiguous():
+    rows, ch = shape
+    if ch % 32 or blocks != (rows, ch // 32) or (n is not None and rows != n) or (c is not None and ch != c):
+        raise ValueError(f"{name} has codes {list(shape)} and powers {list(blocks)}, expected {[n, c]} and one for 32 channels")
+    if not (codes.is_contiguous() and powers.is_contiguous()):
         raise ValueError(f"{name} must be contiguous")
-    _same_device(device, f"{name}'s codes", codes, f"{name}'s powers", powers)
+    _same_device(device, name, codes, name, powers)
     return rows, ch
 
 
@@ -1281,16 +1282,17 @@ def kv_cache(pages: int, page: int, heads: int, d: int, dtype="mx4", device="cud
     return KVCache(torch.zeros((pages, size), dtype=torch.uint8, device=device), page, heads, d, dtype)
 
 
-def _cache_places(cache, table, lengths, offsets, n: int, dev):
-    """Checks of a cache's table, lengths and rows' offsets -> (offsets, samples)."""
-    torch = _torch()
+def _cache_places(cache, table, lengths, offsets, dev):
+    """Checks of a cache's table, lengths and rows' offsets -> (offsets, samples, the table's columns)."""
+    int32 = _torch().int32
     offsets, samples = _offsets(offsets, "offsets")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != samples or table.shape[1] < 1 or not table.is_contiguous():
+    shape = table.shape
+    if table.dtype != int32 or len(shape) != 2 or shape[0] != samples or not shape[1] or not table.is_contiguous():
         raise ValueError(f"table must be a contiguous int32 [{samples}, max_pages]")
-    if lengths.dtype != torch.int32 or lengths.dim() != 1 or lengths.shape[0] != samples or not lengths.is_contiguous():
+    if lengths.dtype != int32 or lengths.shape != (samples,) or not lengths.is_contiguous():
         raise ValueError(f"lengths must be a contiguous int32 [{samples}]")
-    _same_device(dev, "cache", cache.data, "table", table, "lengths", lengths, "offsets", offsets)
-    return offsets, samples
+    _same_device(dev, "cache", cache._data, "table", table, "lengths", lengths, "offsets", offsets)
+    return offsets, samples, shape[1]
 
 
 def kv_append(cache: KVCache, k, v, table, lengths, offsets=None, q=None, pos=None, pairs=None, theta: float = 10000.0,
@@ -1314,7 +1316,7 @@ def kv_append(cache: KVCache, k, v, table, lengths, offsets=None, q=None, pos=No
     if q is not None and (q.dim() != 3 or q.shape[0] != n or q.shape[2] != d):
         raise ValueError(f"q must be [{n}, Hq, {d}]")
     hq = 0 if q is None else q.shape[1]
-    offsets, samples = _cache_places(cache, table, lengths, offsets, n, dev)
+    offsets, samples, columns = _cache_places(cache, table, lengths, offsets, dev)
     axes = 0
     if pos is not None:
         if pos.dtype != torch.int32 or pos.dim() != 2 or pos.shape[0] != n or not 1 <= pos.shape[1] <= 4:
@@ -1338,9 +1340,9 @@ def kv_append(cache: KVCache, k, v, table, lengths, offsets=None, q=None, pos=No
             qo, qoh = (q_out, given) if q_out is not None else _fitted(torch.empty((n, hq, d), dtype=q.dtype, device=dev), n, hq, d)
         pc = None if pos is None else pos.contiguous()
         gq, gk = _aligned(q_gamma), _aligned(k_gamma)
-        keep(k, v, q, kc, vc, qc, qo, pos, pc, q_gamma, k_gamma, gq, gk, table, lengths, offsets, cache.data)
+        keep(k, v, q, kc, vc, qc, qo, pos, pc, q_gamma, k_gamma, gq, gk, table, lengths, offsets, cache._data)
         _check("tsp_kv_append",
-               lib().tsp_kv_append(cache.arg, kh, vh, code, n, _p(offsets), samples, _p(table), table.shape[1], _p(lengths), qh, hq,
+               lib().tsp_kv_append(cache.arg, kh, vh, code, n, _p(offsets), samples, _p(table), columns, _p(lengths), qh, hq,
                                    _p(pc), axes, (ctypes.c_int * axes)(*pairs) if axes else None, theta, 0 if interleaved else 1,
                                    _p(gq), _p(gk), eps, qoh, s))
         return qo
@@ -1358,7 +1360,7 @@ def kv_gather(cache: KVCache, table, lengths, offsets=None, n=None, out_dtype=No
             n = o.shape[0]
     if n is None:
         raise ValueError("the number of rows: k_out, v_out or n")
-    offsets, samples = _cache_places(cache, table, lengths, offsets, n, dev)
+    offsets, samples, columns = _cache_places(cache, table, lengths, offsets, dev)
     odt = out_dtype or (k_out.dtype if k_out is not None else v_out.dtype if v_out is not None
                         else torch.bfloat16 if cache.dtype == "mx4" else cache.dtype)
     h, d = cache.heads, cache.d
@@ -1369,8 +1371,8 @@ def kv_gather(cache: KVCache, table, lengths, offsets=None, n=None, out_dtype=No
     def call(s, keep):
         ko, kh = (k_out, kg) if k_out is not None else _fitted(torch.empty((n, h, d), dtype=odt, device=dev), n, h, d)
         vo, vh = (v_out, vg) if v_out is not None else _fitted(torch.empty((n, h, d), dtype=odt, device=dev), n, h, d)
-        keep(ko, vo, table, lengths, offsets, cache.data)
-        _check("tsp_kv_gather", lib().tsp_kv_gather(cache.arg, n, _p(offsets), samples, _p(table), table.shape[1], _p(lengths), kh, vh, code, s))
+        keep(ko, vo, table, lengths, offsets, cache._data)
+        _check("tsp_kv_gather", lib().tsp_kv_gather(cache.arg, n, _p(offsets), samples, _p(table), columns, _p(lengths), kh, vh, code, s))
         return ko, vo
     return _launch(dev, stream, call)
 
@@ -1395,7 +1397,7 @@ def attention_cached(q, cache: KVCache, table, lengths, offsets=None, causal: bo
     dev = q.device
     if q.dtype not in (torch.float16, torch.bfloat16) or (cache.dtype != "mx4" and cache.dtype != q.dtype):
         raise ValueError(f"q must be float16 or bfloat16, and a 16-bit cache's dtype; got {q.dtype} on {cache.dtype}")
-    offsets, samples = _cache_places(cache, table, lengths, offsets, nq, dev)
+    offsets, samples, columns = _cache_places(cache, table, lengths, offsets, dev)
     _same_device(dev, "workspace", workspace)
     given = None if out is None else _heads_out(out, nq, hq, d, q.dtype, dev, "out")
     if workspace is not None:
@@ -1407,11 +1409,11 @@ def attention_cached(q, cache: KVCache, table, lengths, offsets=None, causal: bo
         o, oh = (out, given) if out is not None else _fitted(torch.empty((nq, hq, d), dtype=q.dtype, device=dev), nq, hq, d)
         ws = workspace
         if ws is None:
-            need = lib().tsp_attention_cached_workspace_bytes(nq, samples, hq, cache.arg, table.shape[1])
+            need = lib().tsp_attention_cached_workspace_bytes(nq, samples, hq, cache.arg, columns)
             ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-        keep(q, qc, o, ws, table, lengths, offsets, cache.data)
+        keep(q, qc, o, ws, table, lengths, offsets, cache._data)
         _check("tsp_attention_cached",
-               lib().tsp_attention_cached(qh, code, nq, hq, cache.arg, _p(offsets), samples, _p(table), table.shape[1], _p(lengths),
+               lib().tsp_attention_cached(qh, code, nq, hq, cache.arg, _p(offsets), samples, _p(table), columns, _p(lengths),
                                           d ** -0.5 if scale is None else scale, 1 if causal else 0, oh, _p(ws), ws.numel(), s))
         return o
     return _launch(dev, stream, call)
