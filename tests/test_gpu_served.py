@@ -158,7 +158,8 @@ def test_rms_norm_places(gpu_lib):
 # ---- linear -------------------------------------------------------------------------------------
 LINEAR_CASES = [(1, 32, 1), (1, 1024, 64), (5, 96, 27), (3, 160, 100), (16, 128, 16), (17, 512, 333), (64, 2048, 72), (65, 256, 1000), (128, 1056, 130),
                 (200, 32, 7), (257, 640, 260), (1000, 1024, 1000), (515, 4096, 520), (2606, 768, 256), (3001, 2048, 2500), (3001, 2080, 2500), (20000, 480, 1000), (9, 96, 8200), (29, 544, 5000), (45, 1024, 300), (9, 1024, 5000),
-                (1500, 1024, 1500), (1500, 1056, 1500), (12001, 1024, 1001), (12001, 1056, 1001), (13001, 1024, 1000), (13001, 1056, 1000)]
+                (1500, 1024, 1500), (1500, 1056, 1500), (12001, 1024, 1001), (12001, 1056, 1001), (13001, 1024, 1000), (13001, 1056, 1000),
+                (12001, 1024, 1004), (13001, 4096, 1000)]
 
 
 @pytest.mark.parametrize("n,ci,co", LINEAR_CASES)

@@ -11,7 +11,7 @@
 //
 // Large products are bound by the matrix cores at the clock that the chip's power leaves, and by how tiles reach them:
 // 8,192^3 takes 471 us in bf16 (2,330 TFLOP/s; the library's 8-bit product 419) and 862 in fp32 (1,280; its bf16 product
-// 782). 35,001 x 4,096 -> 1,024 in fp32 with a residual takes 337 us, the matrix cores 37 % busy at 2.1 GHz: half of a wave's
+// 782). 35,001 x 4,096 -> 1,024 in fp32 with a residual takes 319 us, the matrix cores 39 % busy at 2.1 GHz: half of a wave's
 // time goes into waiting for loads (tiles of 256 x 256 in cache, no residual: 323 us, 268 without the loop's loads, 229 without
 // its LDS reads), and x, W, residual and outputs, 435 MB, pass the memory-side cache. Few rows are bound by the latency of W:
 // 5 rows, 1,024 -> 4,096, 3.6 us.
@@ -82,14 +82,20 @@ __device__ __forceinline__ void finish1(const LinearArgs& a, int64_t row, int o,
     if (a.out_dtype == TSP_F32) static_cast<float*>(a.out)[at] = y;
     else static_cast<uint16_t*>(a.out)[at] = a.out_dtype == TSP_BF16 ? f32_to_bf16_bits(y) : f32_to_f16_bits(y);
 }
-// EACH pieces of four consecutive outputs of a row, which begin on a boundary of their size (co is a multiple of four).
+// EACH pieces of four consecutive outputs of a row, which begin on a boundary of their size (co is a multiple of four): the residual's
+// (zeros without one), and the outputs, the residual added.
 template <int EACH>
-__device__ __forceinline__ void finish4(const LinearArgs& a, int64_t row, int o, f32x4_t (&y)[EACH]) {
+__device__ __forceinline__ void residual4(const LinearArgs& a, int64_t row, int o, f32x4_t (&r)[EACH]) {
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+        r[k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        if (a.residual && row < a.n && o + 4 * k < a.co) r[k] = *reinterpret_cast<const f32x4_t*>(a.residual + row * a.co + o + 4 * k);
+    }
+}
+template <int EACH>
+__device__ __forceinline__ void finish4(const LinearArgs& a, int64_t row, int o, const f32x4_t (&y)[EACH]) {
     if (o >= a.co) return;
     const int64_t at = row * a.co + o;
-#pragma unroll
-    for (int k = 0; k < EACH; ++k)
-        if (a.residual && o + 4 * k < a.co) y[k] += *reinterpret_cast<const f32x4_t*>(a.residual + at + 4 * k);
     if (a.out_dtype == TSP_F32) {
 #pragma unroll
         for (int k = 0; k < EACH; ++k)
@@ -265,6 +271,17 @@ __global__ __launch_bounds__(WX * WW * 64) void k_linear_mx(LinearArgs a) {
     constexpr int PIECES = RW * 4;
     static_assert(NW * 16 * PIECES * 16 <= ROWS * LM_K && (PIECES == 16 || PIECES == 8), "the waves' parts fit a buffer");
     char* s = reinterpret_cast<char*>(sC0) + wave * (16 * PIECES * 16);
+    // (two pieces of four outputs a lane where they leave in 16 bits, one in 32, whose residual's are read 16 rows
+    // ahead: 35,001 x 4,096 -> 1,024 337 us, 319 so. In 16 bits that took 4 % where there is none)
+    constexpr int EACH = EXACT ? 1 : 2, LANES = PIECES / EACH, TURNS = 16 * LANES / 64;
+    f32x4_t ahead[EXACT ? 2 : 1][TURNS][EACH];
+    auto fetch = [&](int j, f32x4_t (&r)[TURNS][EACH]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < TURNS; ++q)
+            residual4<EACH>(a, x0 + wx + j * 16 + (q * 64 + lane) / LANES, w0 + ww + (q * 64 + lane) % LANES * EACH * 4, r[q]);
+    };
+    const bool adds = a.residual && a.vec;
+    if (EXACT && adds) fetch(0, ahead[0]);
     f32x4_t bias[RW];
 #pragma unroll
     for (int i = 0; i < RW; ++i)
@@ -275,6 +292,8 @@ __global__ __launch_bounds__(WX * WW * 64) void k_linear_mx(LinearArgs a) {
         }
 #pragma unroll
     for (int j = 0; j < RX; ++j) {
+        if constexpr (EXACT)
+            if (adds && j + 1 < RX) fetch(j + 1, ahead[(j + 1) % 2]);
 #pragma unroll
         for (int i = 0; i < RW; ++i) {
             f32x4_t y = acc[i][j] + bias[i];
@@ -290,20 +309,18 @@ __global__ __launch_bounds__(WX * WW * 64) void k_linear_mx(LinearArgs a) {
                 if (row0 + r < a.n && w0 + ww + e < a.co) finish1(a, row0 + r, w0 + ww + e, y);
             }
         } else {
-            // two pieces of four outputs a lane where they leave in 16 bits, one in 32
-            auto leave = [&](auto each) __attribute__((always_inline)) {
-                constexpr int EACH = decltype(each)::value, LANES = PIECES / EACH;
+            if (!EXACT && adds) fetch(j, ahead[0]);
 #pragma unroll
-                for (int q = 0; q < 16 * LANES / 64; ++q) {
-                    const int r = (q * 64 + lane) / LANES, p = (q * 64 + lane) % LANES * EACH;
-                    f32x4_t y[EACH];
+            for (int q = 0; q < TURNS; ++q) {
+                const int r = (q * 64 + lane) / LANES, p = (q * 64 + lane) % LANES * EACH;
+                f32x4_t y[EACH];
 #pragma unroll
-                    for (int k = 0; k < EACH; ++k) y[k] = *reinterpret_cast<const f32x4_t*>(s + (r * PIECES + ((p + k) ^ (r & (PIECES - 1)))) * 16);
-                    if (row0 + r < a.n) finish4<EACH>(a, row0 + r, w0 + ww + p * 4, y);
+                for (int k = 0; k < EACH; ++k) {
+                    y[k] = *reinterpret_cast<const f32x4_t*>(s + (r * PIECES + ((p + k) ^ (r & (PIECES - 1)))) * 16);
+                    if (adds) y[k] += ahead[EXACT ? j % 2 : 0][q][k];
                 }
-            };
-            if constexpr (EXACT) leave(std::integral_constant<int, 1>{});
-            else leave(std::integral_constant<int, 2>{});
+                if (row0 + r < a.n) finish4<EACH>(a, row0 + r, w0 + ww + p * 4, y);
+            }
         }
         asm volatile("" ::: "memory");
     }
@@ -394,7 +411,9 @@ __global__ __launch_bounds__(LF_NW * 64) void k_linear_mx_few(LinearArgs a) {
         if (a.bias && o + e < a.co) y[e] += a.bias[o + e];
     if (a.act) y = silu4(y);
     if (a.vec) {
-        f32x4_t one[1] = {y};
+        f32x4_t one[1];
+        residual4<1>(a, row, o, one);
+        one[0] += y;
         finish4<1>(a, row, o, one);
     } else {
 #pragma unroll
@@ -405,12 +424,12 @@ __global__ __launch_bounds__(LF_NW * 64) void k_linear_mx_few(LinearArgs a) {
 
 // The tile with the least time of its rounds. A step of 128 channels takes a workgroup so many us where the device is full
 // (8,192 rows and outputs of 8,192 channels) and where it has a CU to itself (1,000 rows, 4,096 -> 1,024); a tile's first loads
-// and its rows' way out some more, three times that where a residual is read. us by tiles of 256 x 256, 192 x 256 (fp32 out alone),
-// 128 x 128, 128 x 64 and 64 x 64, bf16 out / fp32 out with a residual: 35,001 rows, 4,096 -> 1,024: 220, -, 259, 296, 354 / 398,
-// 340, 351, 401, 454; 1,024 -> 4,096: 187, -, 219, 265, 374 / 500, 503, 436, 489, 651; 12,345 rows, 1,024 -> 1,024: 22, -, 26, 30,
-// 38 / 48, -, 43, 46, 54; 1,000 rows, 4,096 -> 1,024: 56, -, 36, 20, 16 / 113, -, 45, 27, 20; 8,192 rows, 8,192 -> 8,192: 539, -,
-// 806, 1,040, 1,291 / 975, 1,115, 1,095, 1,324, 1,592. (More waves a tile than its products need hide the loads of what lies in
-// memory: 128 x 128 by eight takes 351 where four take 363. 256 x 128 with two steps on their way: no faster than the best.)
+// and its rows' way out some more, twice that where a residual is read. us by tiles of 256 x 256, 192 x 256 (fp32 out alone),
+// 128 x 128 and 128 x 64, bf16 out / fp32 out with a residual: 35,001 rows, 4,096 -> 1,024: 220, -, 259, 295 / 390, 327, 336, 390;
+// 1,024 -> 4,096: 187, -, 221, 270 / 445, 413, 408, 470; 12,345 rows, 1,024 -> 1,024: 22, -, 25, 30 / 55, 70, 48, 48; 8,192 rows,
+// 8,192 -> 8,192: 539, -, 806, 1,040 / 960, 1,071, 1,049, 1,322; and with 64 x 64 as the last, 1,000 rows, 4,096 -> 1,024: 56, -, 36,
+// 20, 16 / 113, -, 45, 27, 20. (More waves a tile than its products need hide the loads of what lies in memory: 128 x 128 by
+// eight takes 351 where four take 363. 256 x 128 with two steps on their way: no faster than the best.)
 int linear_shape(int64_t n, int ci, int co, bool exact, bool residual) {
     struct Times { double full, alone, rest; };
     struct Shape { int x, w, slots; Times by[2]; };
@@ -424,7 +443,7 @@ int linear_shape(int64_t n, int ci, int co, bool exact, bool residual) {
         const Shape& s = shapes[i];
         const Times& t = s.by[exact];
         const int64_t tiles = ceil_div(n, s.x) * ceil_div(co, s.w), last = tiles % s.slots, steps = ceil_div(ci, LM_K);
-        const double out = t.rest * (residual ? 3. : 1.), full = steps * t.full + out, alone = steps * t.alone + out;
+        const double out = t.rest * (residual ? 2. : 1.), full = steps * t.full + out, alone = steps * t.alone + out;
         // (a round of at most a workgroup a CU is as long as one alone; one of nearly 256 large ones is not)
         const double time = (double)(tiles / s.slots) * full + (last == 0 ? 0. : last <= (s.slots == 256 ? 128 : 256) ? alone : full);
         if (time < least) least = time, best = i;
