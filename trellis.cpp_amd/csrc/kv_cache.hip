@@ -393,7 +393,8 @@ extern "C" int tsp_kv_append(const tsp_kv_cache* cache, const tsp_heads* k, cons
             a.axis[p] = (int8_t)ax;
             a.turns[p] = std::pow(theta, -(double)j / pairs[ax]) / (2 * M_PI);
         }
-    // A row is shared by as many groups as it takes to give the device some 2048 workgroups, at most one a head.
+    // A row is shared by as many groups as it takes to give the device some 2048 workgroups, at most one a head. (12,345 rows into 4
+    // bits: 40 us with 1024, 37 so, 47 with 4096; into 16: 36, 31 and 35.)
     const int lanes = c.d <= 64 ? 8 : 16, groups = KV_NT / lanes;
     a.parts = (int)std::min<int64_t>(std::max(hq, c.heads), std::max<int64_t>(1, 2048ll * groups / n));
     constexpr int64_t kRows = 1 << 26;       // of a launch
