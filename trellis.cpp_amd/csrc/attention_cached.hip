@@ -1047,34 +1047,36 @@ __device__ __forceinline__ void join_rows(const CachedArgs& a, int g0, int first
     const int row = first + group / G, pieces = j.last - g0 + 1;
     const bool live = row < min(j.rows, ROWS);
     auto at = [&](int i) { return (int64_t)(2 * (g0 + i) + (i == 0)) * ROWS + (live ? row : 0); };
+    float2 st[BATCH];
+    float x[BATCH][8];
+    auto load = [&](int i0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+            const int i = i0 + b * G;
+            st[b] = i < pieces ? a.stat[at(i)] : float2{-INFINITY, -1.f};
+            if (i < pieces && e < a.cache.d) load8<TSP_F32>(a.part, at(i) * a.cache.d + e, x[b]);
+        }
+    };
+    load(g);      // (on their way while the largest maximum is found)
     float top = -INFINITY;
     for (int i = mine; i < pieces; i += G * 16) {
-        const float2 st = a.stat[at(i)];
-        if (st.y != -1.f) top = fmaxf(top, st.x);
+        const float2 one = a.stat[at(i)];
+        if (one.y != -1.f) top = fmaxf(top, one.x);
     }
 #pragma unroll
     for (int o = G == 1 ? 8 : 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
     float sum = 0.f, acc[8] = {};
     bool any = false;
     for (int i0 = g; i0 < pieces; i0 += BATCH * G) {
-        float c[BATCH], x[BATCH][8];
+        if (i0 >= BATCH * G) load(i0);
 #pragma unroll
         for (int b = 0; b < BATCH; ++b) {
-            const int i = i0 + b * G;
-            c[b] = -1.f;
-            if (i >= pieces) continue;
-            const float2 st = a.stat[at(i)];
-            if (e < a.cache.d) load8<TSP_F32>(a.part, at(i) * a.cache.d + e, x[b]);
-            if (st.y == -1.f) continue;
+            if (st[b].y == -1.f) continue;
             any = true;
-            c[b] = st.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st.x - top) * a.scale2);
-            sum += c[b] * st.y;
-        }
+            const float c = st[b].x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st[b].x - top) * a.scale2);
+            sum += c * st[b].y;
 #pragma unroll
-        for (int b = 0; b < BATCH; ++b) {
-            if (c[b] == -1.f) continue;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) acc[k] += c[b] * x[b][k];
+            for (int k = 0; k < 8; ++k) acc[k] += c * x[b][k];
         }
     }
     int seen = any;
@@ -1100,7 +1102,15 @@ __device__ __forceinline__ void join_many(const CachedArgs& a, int g0, int row, 
     const JoinItem j = a.join[g0];
     const int pieces = j.last - g0 + 1;
     auto at = [&](int i) { return (int64_t)(2 * (g0 + i) + (i == 0)) * ROWS + row; };
+    constexpr int BATCH = 4;
     float2 st[CJ_EACH];
+    float x[BATCH][8];
+    auto load = [&](int i0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b)
+            if (i0 + b * 64 < pieces && e < a.cache.d) load8<TSP_F32>(a.part, at(i0 + b * 64) * a.cache.d + e, x[b]);
+    };
+    load(threadIdx.x >> 2);      // (on their way while the weights are formed)
     float top = -INFINITY, sum = 0.f;
     bool any = false;
 #pragma unroll
@@ -1128,20 +1138,14 @@ __device__ __forceinline__ void join_many(const CachedArgs& a, int g0, int row, 
     sum = (s.sum[0] + s.sum[1]) + (s.sum[2] + s.sum[3]);
     float acc[8] = {};
     if (e < a.cache.d) {
-        constexpr int BATCH = 4;
         for (int i0 = threadIdx.x >> 2; i0 < pieces; i0 += BATCH * 64) {
-            float c[BATCH], x[BATCH][8];
+            if (i0 >= BATCH * 64) load(i0);
 #pragma unroll
             for (int b = 0; b < BATCH; ++b) {
-                const int i = i0 + b * 64;
-                c[b] = i < pieces ? s.weight[i] : -1.f;
-                if (c[b] != -1.f) load8<TSP_F32>(a.part, at(i) * a.cache.d + e, x[b]);
-            }
+                const float c = i0 + b * 64 < pieces ? s.weight[i0 + b * 64] : -1.f;
+                if (c == -1.f) continue;
 #pragma unroll
-            for (int b = 0; b < BATCH; ++b) {
-                if (c[b] == -1.f) continue;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) acc[k] += c[b] * x[b][k];
+                for (int k = 0; k < 8; ++k) acc[k] += c * x[b][k];
             }
         }
     }
