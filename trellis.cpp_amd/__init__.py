@@ -1122,9 +1122,8 @@ def mx_empty(n: int, c: int, device="cuda") -> Mx:
               torch.empty((n, c // 32), dtype=torch.float8_e8m0fnu, device=device))
 
 
-def _check_mx(m, n, c, device, name: str):
+def _check_mx(torch, m, n, c, name: str):
     """n and c may be None: any. -> (n, c)"""
-    torch = _torch()
     codes, powers = m
     shape, blocks = codes.shape, powers.shape
     if codes.dtype != torch.float8_e4m3fn or (powers.dtype != torch.float8_e8m0fnu and powers.dtype != torch.uint8) or len(shape) != 2:
@@ -1134,7 +1133,6 @@ def _check_mx(m, n, c, device, name: str):
         raise ValueError(f"{name} has codes {list(shape)} and powers {list(blocks)}, expected {[n, c]} and one for 32 channels")
     if not (codes.is_contiguous() and powers.is_contiguous()):
         raise ValueError(f"{name} must be contiguous")
-    _same_device(device, name, codes, name, powers)
     return rows, ch
 
 
@@ -1157,6 +1155,7 @@ def rms_norm(x, gamma=None, eps: float = 1e-6, residual=None, residual_out=None,
             raise ValueError("residual_out needs a residual")
         _check_out(residual_out, n, c, residual.dtype, dev)
     _same_device(dev, "gamma", gamma, "residual", residual)
+    xd, rd = dtype_code(x.dtype), 0 if residual is None else dtype_code(residual.dtype)
     mx = isinstance(out, tuple) if out is not None else out_dtype == torch.float8_e4m3fn
     if mx:
         if out_dtype not in (None, torch.float8_e4m3fn):
@@ -1164,10 +1163,10 @@ def rms_norm(x, gamma=None, eps: float = 1e-6, residual=None, residual_out=None,
         if c % 32:
             raise ValueError(f"rows in 8 bits need a multiple of 32 channels, got {c}")
         if out is not None:
-            _check_mx(out, n, c, dev, "out")
+            _check_mx(torch, out, n, c, "out")
+            _same_device(dev, "out", out[0], "out", out[1])
     elif out is not None:
         _check_out(out, n, c, out_dtype or out.dtype, dev)
-    xd, rd = dtype_code(x.dtype), 0 if residual is None else dtype_code(residual.dtype)
     odt = None if mx else (out.dtype if out is not None else out_dtype or x.dtype)
     od = TSP_MX8 if mx else dtype_code(odt)
 
@@ -1196,7 +1195,8 @@ def mx_quantize(x, out=None, stream=None) -> Mx:
     _same_device(dev)
     xd = dtype_code(x.dtype)
     if out is not None:
-        _check_mx(out, n, c, dev, "out")
+        _check_mx(_torch(), out, n, c, "out")
+        _same_device(dev, "out", out[0], "out", out[1])
 
     def call(s, keep):
         xc = _aligned(x.contiguous())
@@ -1218,16 +1218,17 @@ def linear_mx(x, weight, bias=None, act: str = "none", residual=None, out_dtype=
     the rate). out may be given, and be a float32 residual itself; workspace (linear_mx_workspace) may be given to
     reuse it."""
     torch = _torch()
-    dev = x[0].device
-    n, ci = _check_mx(x, None, None, dev, "x")
-    co, _ = _check_mx(weight, None, ci, dev, "weight")
+    n, ci = _check_mx(torch, x, None, None, "x")
+    co, _ = _check_mx(torch, weight, None, ci, "weight")
+    (xc, xp), (wc, wp) = x, weight
+    dev = xc.device
     if bias is not None and (bias.dtype != torch.float32 or bias.numel() != co or not bias.is_contiguous()):
         raise ValueError(f"bias must be a contiguous float32 vector of {co}")
-    if residual is not None and (residual.dtype != torch.float32 or tuple(residual.shape) != (n, co)):
+    if residual is not None and (residual.dtype != torch.float32 or residual.shape != (n, co)):
         raise ValueError(f"residual must be float32 {[n, co]}")
     if out is not None:
         _check_out(out, n, co, out_dtype or out.dtype, dev)
-    _same_device(dev, "bias", bias, "residual", residual, "workspace", workspace)
+    _same_device(dev, "x's powers", xp, "weight's codes", wc, "weight's powers", wp, "bias", bias, "residual", residual, "workspace", workspace)
     if workspace is not None:
         _check_workspace(workspace)
     odt = out.dtype if out is not None else out_dtype or torch.bfloat16
@@ -1240,11 +1241,11 @@ def linear_mx(x, weight, bias=None, act: str = "none", residual=None, out_dtype=
         if ws is None:
             need = lib().tsp_linear_mx_workspace_bytes(n, ci, co)
             ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        xc, xp, wc, wp = _aligned(x[0]), _aligned(x[1]), _aligned(weight[0]), _aligned(weight[1])
-        keep(*x, *weight, xc, xp, wc, wp, bias, residual, rc, o, ws)
+        xa, pa, wa, qa = _aligned(xc), _aligned(xp), _aligned(wc), _aligned(wp)
+        keep(xc, xp, wc, wp, xa, pa, wa, qa, bias, residual, rc, o, ws)
         _check("tsp_linear_mx",
-               lib().tsp_linear_mx(_p(xc), _p(xp), n, ci, _p(wc), _p(wp), _p(bias), co, ac, _p(rc), _p(o), od, _p(ws),
-                                   0 if ws is None else ws.numel(), s))
+               lib().tsp_linear_mx(xa.data_ptr(), pa.data_ptr(), n, ci, wa.data_ptr(), qa.data_ptr(), _p(bias), co, ac, _p(rc),
+                                   o.data_ptr(), od, _p(ws), 0 if ws is None else ws.numel(), s))
         return o
     return _launch(dev, stream, call)
 
