@@ -1283,8 +1283,9 @@ def kv_cache(pages: int, page: int, heads: int, d: int, dtype="mx4", device="cud
     return KVCache(torch.zeros((pages, size), dtype=torch.uint8, device=device), page, heads, d, dtype)
 
 
-def _cache_places(cache, table, lengths, offsets, dev):
-    """Checks of a cache's table, lengths and rows' offsets -> (offsets, samples, the table's columns)."""
+def _cache_places(cache, table, lengths, offsets, dev, *named):
+    """Checks of a cache's table, lengths and rows' offsets, and of the device of theirs and the tensors named
+    -> (offsets, samples, the table's columns)."""
     int32 = _torch().int32
     offsets, samples = _offsets(offsets, "offsets")
     shape = table.shape
@@ -1292,7 +1293,7 @@ def _cache_places(cache, table, lengths, offsets, dev):
         raise ValueError(f"table must be a contiguous int32 [{samples}, max_pages]")
     if lengths.dtype != int32 or lengths.shape != (samples,) or not lengths.is_contiguous():
         raise ValueError(f"lengths must be a contiguous int32 [{samples}]")
-    _same_device(dev, "cache", cache._data, "table", table, "lengths", lengths, "offsets", offsets)
+    _same_device(dev, "cache", cache._data, "table", table, "lengths", lengths, "offsets", offsets, *named)
     return offsets, samples, shape[1]
 
 
@@ -1317,7 +1318,8 @@ def kv_append(cache: KVCache, k, v, table, lengths, offsets=None, q=None, pos=No
     if q is not None and (q.dim() != 3 or q.shape[0] != n or q.shape[2] != d):
         raise ValueError(f"q must be [{n}, Hq, {d}]")
     hq = 0 if q is None else q.shape[1]
-    offsets, samples, columns = _cache_places(cache, table, lengths, offsets, dev)
+    offsets, samples, columns = _cache_places(cache, table, lengths, offsets, dev, "q", q, "v", v, "pos", pos, "q_gamma", q_gamma,
+                                              "k_gamma", k_gamma)
     axes = 0
     if pos is not None:
         if pos.dtype != torch.int32 or pos.dim() != 2 or pos.shape[0] != n or not 1 <= pos.shape[1] <= 4:
@@ -1329,7 +1331,6 @@ def kv_append(cache: KVCache, k, v, table, lengths, offsets=None, q=None, pos=No
     for name, g, h in (("q_gamma", q_gamma, hq), ("k_gamma", k_gamma, hkv)):
         if g is not None and (g.dtype != torch.float32 or g.shape != (h, d) or not g.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous float32 {[h, d]}")
-    _same_device(dev, "q", q, "v", v, "pos", pos, "q_gamma", q_gamma, "k_gamma", k_gamma)
     given = None if q_out is None else _heads_out(q_out, n, hq, d, k.dtype, dev, "q_out")
     code = dtype_code(k.dtype)
 
@@ -1398,8 +1399,7 @@ def attention_cached(q, cache: KVCache, table, lengths, offsets=None, causal: bo
     dev = q.device
     if q.dtype not in (torch.float16, torch.bfloat16) or (cache.dtype != "mx4" and cache.dtype != q.dtype):
         raise ValueError(f"q must be float16 or bfloat16, and a 16-bit cache's dtype; got {q.dtype} on {cache.dtype}")
-    offsets, samples, columns = _cache_places(cache, table, lengths, offsets, dev)
-    _same_device(dev, "workspace", workspace)
+    offsets, samples, columns = _cache_places(cache, table, lengths, offsets, dev, "workspace", workspace)
     given = None if out is None else _heads_out(out, nq, hq, d, q.dtype, dev, "out")
     if workspace is not None:
         _check_workspace(workspace)
