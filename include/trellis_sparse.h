@@ -530,8 +530,8 @@ enum { TSP_MX8 = 3 };
  * both may be NULL, and residual_out alone; gamma f32 [c] or NULL. out_dtype TSP_MX8: codes to out, [n][c / 32] power
  * bytes to d_powers (c a multiple of 32); else d_powers is not used. out and residual_out may be x or residual where
  * the dtypes agree and must not overlap them or each other otherwise. c up to 2^20; rows of up to 8,192 channels
- * in whole 16-byte pieces (c a multiple of 8, tensors and gamma 16-byte aligned) are read once, piece by piece, others twice,
- * value by value. */
+ * in whole 16-byte pieces (c a multiple of 8, tensors and gamma 16-byte aligned) and others of up to 4,096 are read once, longer
+ * ones twice, value by value. */
 int tsp_rms_norm(const void* d_x, int x_dtype, int64_t n, int c, const void* d_residual, int residual_dtype,
                  const float* d_gamma, float eps, void* d_out, int out_dtype, uint8_t* d_powers, void* d_residual_out,
                  void* stream);

@@ -68,7 +68,8 @@ def test_mx_quantize(gpu_lib, n, c, key):
 
 # ---- RMS norm -----------------------------------------------------------------------------------
 RMS_CASES = [(1, 1), (1, 8), (3, 7), (5, 32), (1, 1024), (9, 100), (33, 512), (70, 520), (17, 2048), (6, 2056), (5, 4096),
-             (3, 8192), (2, 8224), (2, 20_000), (9001, 96), (8300, 1000)]
+             (3, 8192), (2, 8224), (2, 20_000), (9001, 96), (8300, 1000), (9, 500), (8193, 516),
+             (5, 1028), (4099, 1500), (3, 4092), (8195, 501), (7, 999), (4097, 1027), (2, 4095), (3, 4100), (2, 5001)]
 
 
 @pytest.mark.parametrize("n,c", RMS_CASES)
@@ -122,6 +123,17 @@ def test_rms_norm_mx(gpu_lib, n, c, xk, rk):
         out, ro = out
         ref.check(ro, h, h.abs() * 2.0 ** -24, "residual")
     check_mx(out, y, "8 bits")
+
+
+@pytest.mark.parametrize("n,c", [(3, 96), (9, 544), (8300, 1024), (5, 2080), (2, 4096), (2, 4128)])
+def test_rms_norm_mx_off_a_boundary(gpu_lib, n, c):
+    """Rows off a 16-byte boundary, value by value, into 8 bits."""
+    import torch
+    randn = gen(n + c)
+    x = torch.empty(n * c + 1, dtype=torch.bfloat16, device="cuda")[1:].view(n, c).copy_(randn(n, c) * 2)
+    gamma = 1 + 0.3 * randn(c)
+    out = gpu_lib.rms_norm(x, gamma, out_dtype=dtype("mx8"))
+    check_mx(out, sr.rms_norm(x, None, gamma, 1e-6)[0], "8 bits")
 
 
 def test_rms_norm_places(gpu_lib):

@@ -7,8 +7,8 @@
 // with part of it in the memory-side cache; 60,013 of 2,048 in bf16 187 us, 5.3 TB/s; the vector units are 15 % busy, and
 // 5 rows take 2.6 us. A wave holds a row of up to 2,048 channels in registers, eight consecutive
 // ones a lane and piece, four waves one of up to 8,192; gamma stays in registers while the wave goes over its
-// rows. Four neighbouring lanes hold a block of 32, so that its largest value is two lane moves. Other rows (not of
-// whole 16-byte pieces, or longer) are read twice, value by value, by a workgroup each.
+// rows. Four neighbouring lanes hold a block of 32, so that its largest value is two lane moves. Rows of no whole
+// pieces are held in smaller ones up to 4,096 channels; longer ones are read twice, value by value, by a workgroup each.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -32,83 +32,7 @@ struct RmsArgs {
     float eps, inv_c;
 };
 
-template <int DT>
-__device__ __forceinline__ void store_if(void* p, int64_t i, const float (&v)[8]) {
-    if constexpr (DT != RN_NONE) store8<DT>(p, i, v);
-}
-
-// A row by NW waves (1: four rows a workgroup), CHUNKS pieces of 8 channels a lane.
-template <int XDT, int RDT, int NW, int CHUNKS>
-__global__ __launch_bounds__(RN_NT) void k_rms_norm(RmsArgs a) {
-    __shared__ float sum_of[2][4];
-    const int lane = threadIdx.x % (NW * 64), wave = threadIdx.x / 64, pieces = a.c / 8;
-    float gamma[CHUNKS][8];
-#pragma unroll
-    for (int k = 0; k < CHUNKS; ++k) {
-        const int piece = k * NW * 64 + lane;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) gamma[k][e] = 1.f;
-        if (a.gamma && piece < pieces) load8<TSP_F32>(a.gamma, piece * 8, gamma[k]);
-    }
-    int turn = 0;
-    // (with NW = 4 the whole workgroup has one row, and leaves together)
-    for (int64_t row = NW == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x; row < a.n; row += (int64_t)gridDim.x * (NW == 1 ? 4 : 1), turn ^= 1) {
-        const int64_t base = row * a.c;
-        float h[CHUNKS][8], q = 0.f;
-#pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) {
-            const int piece = k * NW * 64 + lane;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[k][e] = 0.f;
-            if (piece < pieces) {
-                load8<XDT>(a.x, base + piece * 8, h[k]);
-                if constexpr (RDT != RN_NONE) {
-                    float r[8];
-                    load8<RDT>(a.residual, base + piece * 8, r);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) h[k][e] += r[e];
-                }
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) q += h[k][e] * h[k][e];
-        }
-        q = group_sum<64>(q);
-        if constexpr (NW > 1) {     // (two places taken in turn: one barrier a row)
-            if ((threadIdx.x & 63) == 0) sum_of[turn][wave] = q;
-            __syncthreads();
-            q = (sum_of[turn][0] + sum_of[turn][1]) + (sum_of[turn][2] + sum_of[turn][3]);
-        }
-        const float scale = __builtin_amdgcn_rsqf(fmaf(q, a.inv_c, a.eps));
-#pragma unroll
-        for (int k = 0; k < CHUNKS; ++k) {
-            const int piece = k * NW * 64 + lane;
-            if (piece >= pieces) break;      // (whole quads of lanes, where blocks of 32 are asked for)
-            const int64_t at = base + piece * 8;
-            if constexpr (RDT != RN_NONE) {
-                if (a.residual_out) store_if<RDT>(a.residual_out, at, h[k]);
-            }
-            float y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = h[k][e] * scale * gamma[k][e];
-            if (a.out_dtype == TSP_MX8) {
-                const uint32_t power = mx_power_of<MX_E4M3>(y);
-                *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.out) + at) = mx_codes8(y, power);
-                if ((lane & 3) == 0) a.powers[at / MX_BLOCK] = (uint8_t)power;
-            } else if (a.out_dtype == TSP_BF16) {
-                store8<TSP_BF16>(a.out, at, y);
-            } else if (a.out_dtype == TSP_F16) {
-                store8<TSP_F16>(a.out, at, y);
-            } else {
-                store8<TSP_F32>(a.out, at, y);
-            }
-        }
-    }
-}
-
-// Any row, value by value; a block of 32 channels is 32 neighbouring threads'.
+// One value; a block of 32 channels is 32 neighbouring threads'.
 __device__ __forceinline__ float load1(const void* p, int dt, int64_t i) {
     return dt == TSP_F32 ? static_cast<const float*>(p)[i]
            : dt == TSP_BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(p)[i]) : f16_bits_to_f32(static_cast<const uint16_t*>(p)[i]);
@@ -127,6 +51,115 @@ __device__ __forceinline__ void store_mx8(void* codes, uint8_t* powers, int64_t 
     static_cast<uint8_t*>(codes)[i] = (uint8_t)__builtin_bit_cast(uint32_t, c);
     if ((threadIdx.x & 31) == 0) powers[i / MX_BLOCK] = (uint8_t)power;
 }
+// A piece of V channels, 8, 4 or 1.
+template <int DT, int V>
+__device__ __forceinline__ void load_piece(const void* p, int64_t i, float (&v)[V]) {
+    if constexpr (V == 8) {
+        load8<DT>(p, i, v);
+    } else if constexpr (V == 1) {
+        v[0] = load1(p, DT, i);
+    } else if constexpr (DT == TSP_F32) {
+        const f32x4_t a = *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(p) + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = a[k];
+    } else {
+        const uint2 a = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+        auto f = [](uint32_t w) { return DT == TSP_BF16 ? bf16_bits_to_f32((uint16_t)w) : f16_bits_to_f32((uint16_t)w); };
+        v[0] = f(a.x), v[1] = f(a.x >> 16), v[2] = f(a.y), v[3] = f(a.y >> 16);
+    }
+}
+template <int DT, int V>
+__device__ __forceinline__ void store_piece(void* p, int64_t i, const float (&v)[V]) {
+    if constexpr (V == 8) {
+        store8<DT>(p, i, v);
+    } else if constexpr (V == 1) {
+        store1(p, DT, i, v[0]);
+    } else if constexpr (DT == TSP_F32) {
+        *reinterpret_cast<f32x4_t*>(static_cast<float*>(p) + i) = f32x4_t{v[0], v[1], v[2], v[3]};
+    } else {
+        auto two = [](float a, float b) {
+            return DT == TSP_BF16 ? f32x2_to_bf16x2_bits(a, b) : f32_to_f16_bits(a) | ((uint32_t)f32_to_f16_bits(b) << 16);
+        };
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) = uint2{two(v[0], v[1]), two(v[2], v[3])};
+    }
+}
+
+// A row by NW waves (1: four rows a workgroup), CHUNKS pieces of V channels a lane. (Pieces of 4 for rows of no
+// whole 8, single values for others and tensors that are not aligned.)
+template <int XDT, int RDT, int NW, int CHUNKS, int V>
+__global__ __launch_bounds__(RN_NT) void k_rms_norm(RmsArgs a) {
+    __shared__ float sum_of[2][4];
+    const int lane = threadIdx.x % (NW * 64), wave = threadIdx.x / 64, pieces = a.c / V;
+    float gamma[CHUNKS][V];
+#pragma unroll
+    for (int k = 0; k < CHUNKS; ++k) {
+        const int piece = k * NW * 64 + lane;
+#pragma unroll
+        for (int e = 0; e < V; ++e) gamma[k][e] = 1.f;
+        if (a.gamma && piece < pieces) load_piece<TSP_F32, V>(a.gamma, piece * V, gamma[k]);
+    }
+    int turn = 0;
+    // (with NW = 4 the whole workgroup has one row, and leaves together)
+    for (int64_t row = NW == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x; row < a.n; row += (int64_t)gridDim.x * (NW == 1 ? 4 : 1), turn ^= 1) {
+        const int64_t base = row * a.c;
+        float h[CHUNKS][V], q = 0.f;
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+            const int piece = k * NW * 64 + lane;
+#pragma unroll
+            for (int e = 0; e < V; ++e) h[k][e] = 0.f;
+            if (piece < pieces) {
+                load_piece<XDT, V>(a.x, base + piece * V, h[k]);
+                if constexpr (RDT != RN_NONE) {
+                    float r[V];
+                    load_piece<RDT, V>(a.residual, base + piece * V, r);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) h[k][e] += r[e];
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) q += h[k][e] * h[k][e];
+        }
+        q = group_sum<64>(q);
+        if constexpr (NW > 1) {     // (two places taken in turn: one barrier a row)
+            if ((threadIdx.x & 63) == 0) sum_of[turn][wave] = q;
+            __syncthreads();
+            q = (sum_of[turn][0] + sum_of[turn][1]) + (sum_of[turn][2] + sum_of[turn][3]);
+        }
+        const float scale = __builtin_amdgcn_rsqf(fmaf(q, a.inv_c, a.eps));
+#pragma unroll
+        for (int k = 0; k < CHUNKS; ++k) {
+            const int piece = k * NW * 64 + lane;
+            if (piece >= pieces) break;      // (whole blocks' lanes, where blocks of 32 are asked for)
+            const int64_t at = base + piece * V;
+            if constexpr (RDT != RN_NONE) {
+                if (a.residual_out) store_piece<RDT, V>(a.residual_out, at, h[k]);
+            }
+            float y[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) y[e] = h[k][e] * scale * gamma[k][e];
+            if (V != 4 && a.out_dtype == TSP_MX8) {
+                if constexpr (V == 1) store_mx8(a.out, a.powers, at, y[0]);
+                if constexpr (V == 8) {
+                    const uint32_t power = mx_power_of<MX_E4M3>(y);
+                    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.out) + at) = mx_codes8(y, power);
+                    if ((lane & 3) == 0) a.powers[at / MX_BLOCK] = (uint8_t)power;
+                }
+            } else if (a.out_dtype == TSP_BF16) {
+                store_piece<TSP_BF16, V>(a.out, at, y);
+            } else if (a.out_dtype == TSP_F16) {
+                store_piece<TSP_F16, V>(a.out, at, y);
+            } else {
+                store_piece<TSP_F32, V>(a.out, at, y);
+            }
+        }
+    }
+}
+
+// Any row, twice, value by value.
 __global__ __launch_bounds__(RN_NT) void k_rms_norm_any(RmsArgs a, int x_dtype, int residual_dtype) {
     __shared__ float sum_of[RN_NT / 64];
     for (int64_t row = blockIdx.x; row < a.n; row += gridDim.x) {
@@ -214,7 +247,10 @@ extern "C" int tsp_rms_norm(const void* d_x, int x_dtype, int64_t n, int c, cons
     auto off16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; };
     hipStream_t s = as_stream(stream);
     const dim3 block(RN_NT);
-    if (c % 8 || c > 8192 || off16(d_x) || off16(d_residual) || off16(d_gamma) || off16(d_out) || off16(d_residual_out)) {
+    const bool aligned = !(off16(d_x) || off16(d_residual) || off16(d_gamma) || off16(d_out) || off16(d_residual_out));
+    // (35,001 rows of 500 in bf16 with a residual: 23 us in pieces of four, 28 value by value, 86 twice)
+    const int v = aligned && c % 8 == 0 ? (c <= 8192 ? 8 : 0) : c > 4096 ? 0 : aligned && c % 4 == 0 ? 4 : 1;
+    if (v == 0) {
         hipLaunchKernelGGL(k_rms_norm_any, dim3((unsigned)std::min<int64_t>(n, 16384)), block, 0, s, a, x_dtype, residual_dtype);
         TSP_CHECK_LAUNCH();
         return TSP_OK;
@@ -223,11 +259,19 @@ extern "C" int tsp_rms_norm(const void* d_x, int x_dtype, int64_t n, int c, cons
         auto go = [&](auto rd) {
             constexpr int XD = decltype(xd)::value, RD = decltype(rd)::value;
             const dim3 by_wave((unsigned)std::min<int64_t>(ceil_div(n, 4), 2048)), by_group((unsigned)std::min<int64_t>(n, 4096));
-            if (c <= 512) hipLaunchKernelGGL((k_rms_norm<XD, RD, 1, 1>), by_wave, block, 0, s, a);
-            else if (c <= 1024) hipLaunchKernelGGL((k_rms_norm<XD, RD, 1, 2>), by_wave, block, 0, s, a);
-            else if (c <= 2048) hipLaunchKernelGGL((k_rms_norm<XD, RD, 1, 4>), by_wave, block, 0, s, a);
-            else if (c <= 4096) hipLaunchKernelGGL((k_rms_norm<XD, RD, 4, 2>), by_group, block, 0, s, a);
-            else hipLaunchKernelGGL((k_rms_norm<XD, RD, 4, 4>), by_group, block, 0, s, a);
+            if (v == 1) {
+                if (c <= 512) hipLaunchKernelGGL((k_rms_norm<XD, RD, 1, 8, 1>), by_wave, block, 0, s, a);
+                else if (c <= 1024) hipLaunchKernelGGL((k_rms_norm<XD, RD, 1, 16, 1>), by_wave, block, 0, s, a);
+                else hipLaunchKernelGGL((k_rms_norm<XD, RD, 4, 16, 1>), by_group, block, 0, s, a);
+            } else if (v == 4) {
+                if (c <= 512) hipLaunchKernelGGL((k_rms_norm<XD, RD, 1, 2, 4>), by_wave, block, 0, s, a);
+                else if (c <= 1024) hipLaunchKernelGGL((k_rms_norm<XD, RD, 1, 4, 4>), by_wave, block, 0, s, a);
+                else hipLaunchKernelGGL((k_rms_norm<XD, RD, 4, 4, 4>), by_group, block, 0, s, a);
+            } else if (c <= 512) hipLaunchKernelGGL((k_rms_norm<XD, RD, 1, 1, 8>), by_wave, block, 0, s, a);
+            else if (c <= 1024) hipLaunchKernelGGL((k_rms_norm<XD, RD, 1, 2, 8>), by_wave, block, 0, s, a);
+            else if (c <= 2048) hipLaunchKernelGGL((k_rms_norm<XD, RD, 1, 4, 8>), by_wave, block, 0, s, a);
+            else if (c <= 4096) hipLaunchKernelGGL((k_rms_norm<XD, RD, 4, 2, 8>), by_group, block, 0, s, a);
+            else hipLaunchKernelGGL((k_rms_norm<XD, RD, 4, 4, 8>), by_group, block, 0, s, a);
         };
         if (d_residual) dt_switch(residual_dtype, go);
         else go(std::integral_constant<int, RN_NONE>{});
