@@ -58,9 +58,9 @@ struct CachedArgs {
     struct JoinItem* join;                     // [groups] the unit that is cut at the workgroup's end and began in it
 };
 
-// rows left in the unit from its first (0: none), the first, the sample's first row, the key head, the last workgroup.
+// The unit's rows (0: there is none) and above them 256 times its last workgroup, its first row, the sample's, the key head.
 struct JoinItem {
-    int rows, first_row, row0, head, last, pad[3];
+    int cut, first_row, row0, head;
 };
 
 #ifdef __HIP_DEVICE_COMPILE__       // (the host pass knows neither the register constraint nor the argument segment)
@@ -215,10 +215,10 @@ __device__ __forceinline__ CachedPiece cut_unit(const CachedUnit& u, uint32_t fr
     return CachedPiece{__builtin_amdgcn_readfirstlane(tile(lo)), __builtin_amdgcn_readfirstlane(tile(hi)), lo == 0 && hi == weight ? -1 : 2 * w + (lo == 0)};
 }
 // What the join has to know of a workgroup's last unit.
-template <class Args>
+template <int ROWS, class Args>
 __device__ __forceinline__ void tell_join(const Args& a, const CachedUnit& u, const Line& line, uint32_t to, int w, bool begins) {
     JoinItem j{};
-    if (begins && u.end > to) j = JoinItem{u.lq * a.share - u.first_row, u.first_row, u.row0, u.head, line.group(u.end - 1), {}};
+    if (begins && u.end > to) j = JoinItem{min(u.lq * a.share - u.first_row, ROWS) | line.group(u.end - 1) << 8, u.first_row, u.row0, u.head};
     if (threadIdx.x == 0) a.join[w] = j;
 }
 
@@ -292,7 +292,7 @@ __global__ __launch_bounds__(CF_NW * 64, 2) void k_cached_few(CachedArgs) {
     const Line line = make_line<ROWS, CF_KEYS>(*reread_args());
     const uint32_t to = line.cut(blockIdx.x + 1);
     if (line.cut(blockIdx.x) >= to) {
-        if (threadIdx.x == 0) reread_args()->join[blockIdx.x].rows = 0;
+        if (threadIdx.x == 0) reread_args()->join[blockIdx.x].cut = 0;
         return;
     }
     constexpr float LAG = BF16 ? 8.f : 4.f, LIFT = BF16 ? 0.f : 11.f;
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(CF_NW * 64, 2) void k_cached_few(CachedArgs) {
         const auto& a = *reread_args();
         const CachedUnit u = find_unit<ROWS, CF_KEYS>(a, line, from);
         const CachedPiece piece = cut_unit(u, from, to, blockIdx.x);
-        if (u.end >= to) tell_join(a, u, line, to, blockIdx.x, from <= u.begin);
+        if (u.end >= to) tell_join<ROWS>(a, u, line, to, blockIdx.x, from <= u.begin);
         from = u.end;
         const int rows = u.lq * a.share;
         const FastDiv by_share{a.by_share.mul, a.by_share.shift};
@@ -624,7 +624,7 @@ __global__ __launch_bounds__(CM_NW * 64, 2) void k_cached_many(CachedArgs) {
         from = line.cut(blockIdx.x), to = line.cut(blockIdx.x + 1);
     }
     if (from >= to) {
-        if (threadIdx.x == 0) reread_args()->join[blockIdx.x].rows = 0;
+        if (threadIdx.x == 0) reread_args()->join[blockIdx.x].cut = 0;
         return;
     }
     constexpr float LAG = BF16 ? 8.f : 4.f, LIFT = BF16 ? 0.f : 11.f, FAR = 1024.f;
@@ -634,7 +634,7 @@ __global__ __launch_bounds__(CM_NW * 64, 2) void k_cached_many(CachedArgs) {
         const Line line = make_line<CM_ROWS, CM_KEYS>(a);      // (made anew: kept it would take seven registers of the loop's)
         const CachedUnit u = find_unit<CM_ROWS, CM_KEYS>(a, line, from);
         const CachedPiece piece = cut_unit(u, from, to, blockIdx.x);
-        if (u.end >= to) tell_join(a, u, line, to, blockIdx.x, from <= u.begin);
+        if (u.end >= to) tell_join<CM_ROWS>(a, u, line, to, blockIdx.x, from <= u.begin);
         from = u.end;
         const int rows = u.lq * a.share, lk = u.lk, causal = a.causal;
         const FastDiv by_share{a.by_share.mul, a.by_share.shift};
@@ -1043,12 +1043,12 @@ __device__ __forceinline__ void join_out(const CachedArgs& a, const JoinItem& j,
 
 // Few pieces a unit: 16 / G rows at a time, G groups of 16 lanes a row (1, or 4: a wave), eight channels a lane.
 template <bool BF16, int ROWS, int G>
-__device__ __forceinline__ void join_rows(const CachedArgs& a, int g0, int first) {
+__device__ __forceinline__ void join_rows(const CachedArgs& a, int g0, int cut, int first) {
     constexpr int BATCH = 8;
     const int group = threadIdx.x >> 4, g = group % G, e = (threadIdx.x & 15) * 8, mine = threadIdx.x % (G * 16);
     const JoinItem j = a.join[g0];
-    const int row = first + group / G, pieces = j.last - g0 + 1;
-    const bool live = row < min(j.rows, ROWS);
+    const int row = first + group / G, pieces = (cut >> 8) - g0 + 1;
+    const bool live = row < (cut & 255);
     auto at = [&](int i) { return (int64_t)(2 * (g0 + i) + (i == 0)) * ROWS + (live ? row : 0); };
     float2 st[BATCH];
     float x[BATCH][8];
@@ -1100,10 +1100,10 @@ struct JoinShared {
     float weight[CJ_MAX], acc[4][32], top[4], sum[4];
 };
 template <bool BF16, int ROWS>
-__device__ __forceinline__ void join_many(const CachedArgs& a, int g0, int row, int part, JoinShared& s) {
+__device__ __forceinline__ void join_many(const CachedArgs& a, int g0, int cut, int row, int part, JoinShared& s) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, e = part * 32 + (lane & 3) * 8;
     const JoinItem j = a.join[g0];
-    const int pieces = j.last - g0 + 1;
+    const int pieces = (cut >> 8) - g0 + 1;
     auto at = [&](int i) { return (int64_t)(2 * (g0 + i) + (i == 0)) * ROWS + row; };
     constexpr int BATCH = 4;
     float2 st[CJ_EACH];
@@ -1170,12 +1170,14 @@ __device__ __forceinline__ void join_many(const CachedArgs& a, int g0, int row, 
 template <bool BF16, int ROWS, int G>
 __global__ __launch_bounds__(256) void k_cached_join(CachedArgs a) {
     __shared__ JoinShared s;
-    __shared__ int sCount[CJ_EACH * 4], sFound[2];
+    __shared__ int sCount[CJ_EACH * 4], sFound[3];
     const int wave = threadIdx.x >> 6, blocks = a.cache.blocks;
-    int count[CJ_EACH], end[CJ_EACH];
+    int cut[CJ_EACH], count[CJ_EACH], end[CJ_EACH];
 #pragma unroll
     for (int i = 0; i < CJ_EACH; ++i) {
-        const int w = i * 256 + threadIdx.x, rows = w < a.groups ? min(a.join[w].rows, ROWS) : 0;
+        const int w = i * 256 + threadIdx.x;
+        cut[i] = w < a.groups ? a.join[w].cut : 0;
+        const int rows = cut[i] & 255;
         count[i] = G == 64 ? rows * blocks : (rows + 16 / G - 1) / (16 / G);
     }
 #pragma unroll
@@ -1196,16 +1198,16 @@ __global__ __launch_bounds__(256) void k_cached_join(CachedArgs a) {
     for (int item = blockIdx.x; item < total; item += gridDim.x) {
 #pragma unroll
         for (int i = 0; i < CJ_EACH; ++i)
-            if (item < end[i] && item >= end[i] - count[i]) sFound[0] = i * 256 + threadIdx.x, sFound[1] = item - (end[i] - count[i]);
+            if (item < end[i] && item >= end[i] - count[i]) sFound[0] = i * 256 + threadIdx.x, sFound[1] = item - (end[i] - count[i]), sFound[2] = cut[i];
         __syncthreads();
         const int g0 = sFound[0], x = sFound[1];
-        if constexpr (G == 64) join_many<BF16, ROWS>(a, g0, x / blocks, x % blocks, s);
-        else join_rows<BF16, ROWS, G>(a, g0, x * (16 / G));
+        if constexpr (G == 64) join_many<BF16, ROWS>(a, g0, sFound[2], x / blocks, x % blocks, s);
+        else join_rows<BF16, ROWS, G>(a, g0, sFound[2], x * (16 / G));
         __syncthreads();
     }
 }
 
-static_assert(CJ_MAX >= 768, "the join counts every workgroup");
+static_assert(CJ_MAX >= 768 && CM_ROWS < 256, "the join counts every workgroup, and its items hold a unit's rows");
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
