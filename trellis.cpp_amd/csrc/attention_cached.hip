@@ -19,9 +19,9 @@
 // operand, V through a piece of LDS that is the wave's alone, where it is turned. Many rows (k_cached_many): four waves of 32
 // rows share a tile of 64 keys, widened into LDS by all of them.
 //
-// What bounds them, in bf16, heads of 128, 4 bits. One row of 16 heads on 2, 40,009 keys: 15.2 us, latency: the lengths, the table, the
-// first tile and the next four one after the other on 500 workgroups, then the join's counts, maxima and pieces; 300 keys 9,
-// 200,000 25. 16 samples' tokens, 16 heads on 4, 400,009 keys: 52 us, 47 of them at 4.6 TB/s of cache read, where widening keeps the
+// What bounds them, in bf16, heads of 128, 4 bits. One row of 16 heads on 2, 40,009 keys: 14.6 us, latency: the lengths, the table, the
+// first tile and the next four one after the other on 500 workgroups, then the join's counts and pieces; 300 keys 9,
+// 200,000 25. 16 samples' tokens, 16 heads on 4, 400,009 keys: 51 us, 47 of them at 4.6 TB/s of cache read, where widening keeps the
 // vector units 40 % busy; in 16 bits 178 (4.6 TB/s). 5,003 rows on 35,001 keys, two samples: 800 us, 1,006 TFLOP/s; the matrix
 // cores are 42 % busy at 2.0 GHz, the vector units, which widen, form exponents and round, 45 %. A causal prompt of 8,000 rows
 // 410; 20,000 rows of 16 heads of 64 on 1,029 keys 181.
@@ -138,7 +138,7 @@ __device__ __forceinline__ Line make_line(const Args& a) {
     }
     l.length = __builtin_amdgcn_readfirstlane(l.length);
     // (two workgroups a CU until each has `least`: eight tiles of few rows, four of many. us with that many in each from the start,
-    // and so: 1 row on 300 keys 13.1 and 8.9, on 40,009 16 and 15.2; 8 rows on 4,000 24 and 15.4; a prompt of 300 rows 34 and 24)
+    // and so: 1 row on 300 keys 13.1 and 8.9, on 40,009 15.7 and 15.2; 8 rows on 4,000 24 and 15.4; a prompt of 300 rows 34 and 24)
     const int least = max(min(a.least, (int)((l.length + 511) / 512)), max((1 << a.finer) >> a.coarser, 1));
     l.per = max(least, (int)(l.length + a.groups - 1) / FastDiv{a.by_groups.mul, a.by_groups.shift});
     return l;
@@ -1237,7 +1237,7 @@ CachedCut cached_cut(int64_t nq, int samples, int hkv, int share, int64_t keys, 
     c.groups = longest() <= c.least ? 1 : (int)std::min<int64_t>(c.rows == 16 ? 768 : 512, ceil_div(longest() << c.coarser, 1ll << c.finer));
     const int64_t cut = std::min<int64_t>(c.units, c.groups), pieces = c.groups / (std::max<int64_t>(ceil_div(nq * share, c.rows), std::min<int64_t>(samples, nq)) * hkv);
     const int64_t rows = std::min<int64_t>(each, c.rows);
-    // (64 where its workgroups are few: 1 row on 200,000 keys 40 us by waves, 25 so; 256 rows of 4 heads on 20,000 46 and 55)
+    // (64 where its workgroups are few: 1 row on 200,000 keys 40 us by waves, 25 so; 256 rows of 4 heads on 20,000 45 and 55)
     const int64_t wide = cut * rows * ((d + 31) / 32);
     c.join = pieces > 32 && wide <= 2048 ? 64 : pieces > 2 ? 4 : 1;
     c.joins = (unsigned)std::min<int64_t>(c.join == 64 ? wide : cut * ceil_div(rows, 16 / c.join), 2048);
