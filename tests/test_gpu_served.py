@@ -524,6 +524,21 @@ def test_attention_cached_skewed(gpu_lib, held):
         ref.check(out, o, slack, f"skewed {len(new)}")
 
 
+@pytest.mark.parametrize("new,lengths", [([1], [9000]), ([1, 1, 1], [300, 0, 4000]), ([5], [2000]), ([40, 3], [20, 3000]), ([200, 90], [3000, 60])])
+@pytest.mark.parametrize("held", ["mx4", "bf16"])
+def test_attention_cached_workspace(gpu_lib, new, lengths, held):
+    """What the workspace held has no effect; rows that see no key among the cut ones."""
+    import torch
+    cache, table = make_cache(gpu_lib, lengths, 32, 2, 96, held, 4)
+    b = ints(ref.offsets_of(new))
+    q = gen(6)(sum(new), 8, 96).bfloat16()
+    ws = gpu_lib.attention_cached_workspace(sum(new), len(new), 8, cache, table.shape[1])
+    outs = [gpu_lib.attention_cached(q, cache, table, ints(lengths), offsets=b, workspace=ws.fill_(v)) for v in (0, 255, 127, 1)]
+    o, slack = sr.attention_cached(q, cache, table, lengths, ref.offsets_of(new), True, 96 ** -0.5)
+    ref.check(outs[0], o, slack, "workspace")
+    assert all(same(outs[0], x) for x in outs[1:])
+
+
 def test_attention_cached_rows(gpu_lib):
     """Rows of no sample left as they were; lengths past the table and below zero; samples on the same pages; empty caches."""
     import torch
