@@ -595,7 +595,8 @@ int tsp_kv_gather(const tsp_kv_cache* cache, int64_t n, const int32_t* d_offsets
  * 2^31 - 2^16. The line of all work is cut evenly over the device
  * whatever the samples' lengths, and joined in the workspace, 16-byte aligned, of
  * tsp_attention_cached_workspace_bytes bytes; the result does not depend on what that held, nor on the order in
- * which workgroups run. out must not overlap the inputs. */
+ * which workgroups run. Neither out nor the workspace may overlap another tensor of the call (views that interleave in one
+ * buffer may). */
 size_t tsp_attention_cached_workspace_bytes(int64_t nq, int samples, int hq, const tsp_kv_cache* cache, int max_pages);
 int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, int hq, const tsp_kv_cache* cache,
                          const int32_t* d_offsets, int samples, const int32_t* d_table, int max_pages,

@@ -1,0 +1,22 @@
+"""GPU tests of the served block's calls on views that interleave in one buffer: they share no value, and are taken."""
+from __future__ import annotations
+
+import pytest
+
+from test_gpu_served import gen, ints, make_cache
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+def test_attention_cached_between_q(gpu_lib, rows):
+    """out's heads beside q's in each row, and between q's."""
+    import torch
+    cache, table = make_cache(gpu_lib, [rows + 50], 16, 2, 64, "mx4", 1)
+    q = gen(rows)(rows, 4, 64).bfloat16()
+    want = gpu_lib.attention_cached(q, cache, table, ints([rows + 50]))
+    for q_at, o_at in ((slice(0, 4), slice(4, 8)), (slice(0, 8, 2), slice(1, 8, 2))):
+        both = torch.full((rows, 8, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+        both[:, q_at] = q
+        gpu_lib.attention_cached(both[:, q_at], cache, table, ints([rows + 50]), out=both[:, o_at])
+        assert torch.equal(both[:, o_at], want) and torch.equal(both[:, q_at], q)

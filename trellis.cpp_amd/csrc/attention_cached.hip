@@ -35,6 +35,7 @@
 #include "attention_internal.hpp"
 #include "kv_cache.hpp"
 #include "mx.hpp"
+#include "overlap.hpp"
 
 namespace tsp {
 namespace {
@@ -1280,9 +1281,13 @@ extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, i
     TSP_REQUIRE(heads_aligned(*q) && heads_aligned(*out) && reinterpret_cast<uintptr_t>(c.data) % 16 == 0, TSP_ERR_INVALID,
                 "tsp_attention_cached: data must be 16-byte aligned, strides multiples of 8 (a row's up to 2^20)");
     TSP_REQUIRE(heads_apart(*out, nq, hq, c.d), TSP_ERR_INVALID, "tsp_attention_cached: the output's heads overlap");
-    const size_t span = (size_t)((nq - 1) * out->row_stride + (hq - 1) * out->head_stride + c.d) * 2;
-    TSP_REQUIRE(out->data != q->data && !overlap(c.data, (size_t)(kv_head_bytes(c) * c.heads) * c.pages, out->data, span), TSP_ERR_INVALID,
-                "tsp_attention_cached: out must not alias q or the cache");
+    // (an out that lies over q at an offset, for instance, would be written by one workgroup before another has read it)
+    const Runs o_runs = runs_of(*out, nq, hq, c.d, 2), q_runs = runs_of(*q, nq, hq, c.d, 2);
+    const Runs read[4] = {runs_of(c.data, kv_head_bytes(c) * c.heads * c.pages), runs_of(d_table, 4ll * samples * max_pages),
+                          runs_of(d_lengths, 4ll * samples), runs_of(d_offsets, 4ll * (samples + 1ll))};
+    bool alias = meet(o_runs, q_runs);
+    for (const Runs& r : read) alias |= meet(o_runs, r);
+    TSP_REQUIRE(!alias, TSP_ERR_INVALID, "tsp_attention_cached: out must not alias q, the cache, table, lengths or offsets");
     const int share = hq / c.heads;
     TSP_REQUIRE(nq * share < (1ll << 31) - 1024, TSP_ERR_INVALID, "tsp_attention_cached: too many rows");
     const CachedCut cut = cached_cut(nq, samples, c.heads, share, (int64_t)max_pages * c.page, c.d, c.format == TSP_KV_MX4);
@@ -1291,6 +1296,10 @@ extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, i
     TSP_REQUIRE(d_workspace, TSP_ERR_INVALID, "tsp_attention_cached: null workspace");
     TSP_REQUIRE(workspace_bytes >= need, TSP_ERR_WORKSPACE, "tsp_attention_cached: workspace of %zu bytes, needs %zu", workspace_bytes, need);
     TSP_REQUIRE(reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0, TSP_ERR_INVALID, "tsp_attention_cached: workspace not 16-byte aligned");
+    const Runs ws_runs = runs_of(d_workspace, (int64_t)need);
+    alias = meet(ws_runs, o_runs) || meet(ws_runs, q_runs);
+    for (const Runs& r : read) alias |= meet(ws_runs, r);
+    TSP_REQUIRE(!alias, TSP_ERR_INVALID, "tsp_attention_cached: the workspace overlaps another tensor of the call");
     float* part = static_cast<float*>(d_workspace);
     float2* stat = reinterpret_cast<float2*>(part + (size_t)cut.groups * 2 * cut.rows * c.d);
     const CachedArgs a{q->data, out->data, q->row_stride, q->head_stride, out->row_stride, out->head_stride, kv_args(c, d_table, max_pages, d_lengths),

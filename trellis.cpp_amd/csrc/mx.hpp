@@ -10,6 +10,7 @@
 #include <cstdint>
 
 #include "common.hpp"
+#include "overlap.hpp"
 
 namespace tsp {
 
@@ -102,12 +103,6 @@ __device__ __forceinline__ void store8(void* p, int64_t i, const float (&v)[8]) 
                                   : f32_to_f16_bits(v[2 * k]) | ((uint32_t)f32_to_f16_bits(v[2 * k + 1]) << 16);
         *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(p) + i) = a;
     }
-}
-
-// Whether [a, a + an) and [b, b + bn) share a byte.
-inline bool overlap(const void* a, size_t an, const void* b, size_t bn) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return a && b && an && bn && x < y + bn && y < x + an;
 }
 
 }  // namespace tsp
