@@ -581,7 +581,8 @@ int tsp_kv_append(const tsp_kv_cache* cache, const tsp_heads* k, const tsp_heads
                   const float* d_q_gamma, const float* d_k_gamma, double eps, const tsp_heads* q_out, void* stream);
 
 /* Keys and values out of the cache, packed: of sample s with m rows of the outputs, row i is key d_lengths[s] - m + i
- * (zeros where the cache does not hold it). Outputs [n][heads][d] of any dtype. */
+ * (zeros where the cache does not hold it). Outputs [n][heads][d] of one dtype, any; they must not overlap each other or
+ * another tensor of the call (views that interleave in one buffer may). */
 int tsp_kv_gather(const tsp_kv_cache* cache, int64_t n, const int32_t* d_offsets, int samples, const int32_t* d_table,
                   int max_pages, const int32_t* d_lengths, const tsp_heads* k_out, const tsp_heads* v_out, int out_dtype,
                   void* stream);

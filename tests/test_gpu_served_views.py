@@ -20,3 +20,16 @@ def test_attention_cached_between_q(gpu_lib, rows):
         both[:, q_at] = q
         gpu_lib.attention_cached(both[:, q_at], cache, table, ints([rows + 50]), out=both[:, o_at])
         assert torch.equal(both[:, o_at], want) and torch.equal(both[:, q_at], q)
+
+
+@pytest.mark.parametrize("held", ["mx4", "bf16"])
+def test_gather_into_one_buffer(gpu_lib, held):
+    """Keys and values beside each other in a row, head by head in turn, and one after the other."""
+    import torch
+    cache, table = make_cache(gpu_lib, [90], 16, 2, 64, held, 2)
+    k, v = gpu_lib.kv_gather(cache, table, ints([90]), n=90)
+    row = torch.zeros((90, 4, 64), dtype=torch.bfloat16, device="cuda")
+    after = torch.zeros((180, 2, 64), dtype=torch.bfloat16, device="cuda")
+    for ko, vo in ((row[:, :2], row[:, 2:]), (row[:, ::2], row[:, 1::2]), (after[:90], after[90:]), (after[::2], after[1::2])):
+        gpu_lib.kv_gather(cache, table, ints([90]), k_out=ko, v_out=vo)
+        assert torch.equal(ko, k) and torch.equal(vo, v)

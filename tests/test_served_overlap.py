@@ -56,3 +56,17 @@ def test_attention_cached(pkg, name, kw):
     rc = L.tsp_attention_cached(ctypes.byref(q), 2, 100, 8, ctypes.byref(c), vp(kw.get("off", at(5))), 2, vp(kw.get("table", at(6))), 7,
                                 vp(kw.get("lengths", at(7))), 0.125, 1, ctypes.byref(o), vp(ws), need, NULL)
     assert rc == 1 and ("alias" in err(pkg) or "workspace overlaps" in err(pkg)), (name, rc)
+
+
+@pytest.mark.parametrize("name,kw", [
+    ("values a row into keys", dict(v=at(1, 1024))), ("a head", dict(v=at(1, 128))), ("keys into values", dict(k=at(2, 51200))),
+    ("wider rows", dict(v=at(1, 1024), v_row=1024)), ("the table", dict(table=at(1, 2048))), ("lengths", dict(lengths=at(2))),
+    ("offsets", dict(off=at(2, 102396))), ("the cache", dict(k=at(9, 4096))),
+])
+def test_kv_gather(pkg, name, kw):
+    L = pkg.lib()
+    k, v = pkg.Heads(kw.get("k", at(1)), 512, 64), pkg.Heads(kw.get("v", at(2)), kw.get("v_row", 512), 64)
+    c = cache_arg(pkg)
+    rc = L.tsp_kv_gather(ctypes.byref(c), 100, vp(kw.get("off", at(5))), 2, vp(kw.get("table", at(6))), 7, vp(kw.get("lengths", at(7))),
+                         ctypes.byref(k), ctypes.byref(v), 2, NULL)
+    assert rc == 1 and "overlap" in err(pkg), (name, rc)

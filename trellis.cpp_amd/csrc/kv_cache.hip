@@ -21,6 +21,7 @@
 #include "common.hpp"
 #include "kv_cache.hpp"
 #include "mx.hpp"
+#include "overlap.hpp"
 #include "packed.hpp"
 
 namespace tsp {
@@ -434,12 +435,14 @@ extern "C" int tsp_kv_gather(const tsp_kv_cache* cache, int64_t n, const int32_t
                 "tsp_kv_gather: null pointer");
     TSP_REQUIRE(heads_aligned(*k_out) && heads_aligned(*v_out) && reinterpret_cast<uintptr_t>(c.data) % 16 == 0, TSP_ERR_INVALID,
                 "tsp_kv_gather: data must be 16-byte aligned, strides multiples of 8 (a row's up to 2^20)");
-    TSP_REQUIRE(heads_apart(*k_out, n, c.heads, c.d) && heads_apart(*v_out, n, c.heads, c.d) && k_out->data != v_out->data, TSP_ERR_INVALID,
+    TSP_REQUIRE(heads_apart(*k_out, n, c.heads, c.d) && heads_apart(*v_out, n, c.heads, c.d), TSP_ERR_INVALID,
                 "tsp_kv_gather: the outputs' heads overlap");
-    const size_t cache_bytes = (size_t)(kv_head_bytes(c) * c.heads) * c.pages;
-    TSP_REQUIRE(!overlap(c.data, cache_bytes, k_out->data, heads_span(*k_out, n, c.heads, c.d, out_dtype)) &&
-                    !overlap(c.data, cache_bytes, v_out->data, heads_span(*v_out, n, c.heads, c.d, out_dtype)),
-                TSP_ERR_INVALID, "tsp_kv_gather: an output overlaps the cache");
+    const Runs out[2] = {runs_of(*k_out, n, c.heads, c.d, dtype_size(out_dtype)), runs_of(*v_out, n, c.heads, c.d, dtype_size(out_dtype))};
+    const Runs read[4] = {runs_of(c.data, kv_head_bytes(c) * c.heads * c.pages), runs_of(d_table, 4ll * samples * max_pages),
+                          runs_of(d_lengths, 4ll * samples), runs_of(d_offsets, 4ll * (samples + 1ll))};
+    bool over = meet(out[0], out[1]);
+    for (const Runs& r : read) over |= meet(out[0], r) || meet(out[1], r);
+    TSP_REQUIRE(!over, TSP_ERR_INVALID, "tsp_kv_gather: the outputs overlap each other, the cache, table, lengths or offsets");
     const GatherArgs a{kv_args(c, d_table, max_pages, d_lengths), k_out->data, v_out->data, k_out->row_stride, k_out->head_stride,
                        v_out->row_stride, v_out->head_stride, d_offsets, n, samples};
     const int lanes = c.d <= 64 ? 8 : 16;
