@@ -574,7 +574,8 @@ size_t tsp_kv_page_bytes(int page, int heads, int d, int format);
  * tsp_rope_axes; so is q [n][hq][d] (NULL and 0 without), which goes to q_out. axes 0: no turning, d_pos and pairs
  * not used. Keys for 4 bits are turned in 64 bits, so that each code is that of the exact value; their values
  * have to fit fp32. One dtype for q, k, v and q_out; strides and alignment as for tsp_rope_axes; q_out may be q with
- * the same strides. Two rows of a call must not go to one place in the cache. */
+ * the same strides; otherwise neither q_out nor the cache may overlap another tensor of the call (views that interleave
+ * in one buffer may). Two rows of a call must not go to one place in the cache. */
 int tsp_kv_append(const tsp_kv_cache* cache, const tsp_heads* k, const tsp_heads* v, int dtype, int64_t n,
                   const int32_t* d_offsets, int samples, const int32_t* d_table, int max_pages, const int32_t* d_lengths,
                   const tsp_heads* q, int hq, const int32_t* d_pos, int axes, const int* pairs, double theta, int flags,

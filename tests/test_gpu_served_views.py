@@ -33,3 +33,21 @@ def test_gather_into_one_buffer(gpu_lib, held):
     for ko, vo in ((row[:, :2], row[:, 2:]), (row[:, ::2], row[:, 1::2]), (after[:90], after[90:]), (after[::2], after[1::2])):
         gpu_lib.kv_gather(cache, table, ints([90]), k_out=ko, v_out=vo)
         assert torch.equal(ko, k) and torch.equal(vo, v)
+
+
+@pytest.mark.parametrize("held", ["mx4", "bf16"])
+@pytest.mark.parametrize("rows", [3, 700])
+def test_append_out_of_one_buffer(gpu_lib, held, rows):
+    """q, k, v and q_out beside each other in a row, or q_out's heads between q's."""
+    import torch
+    cache, table = make_cache(gpu_lib, [rows], 16, 2, 64, held, 3, fill=False)
+    q, k, v = gen(1)(rows, 4, 64).bfloat16(), gen(2)(rows, 2, 64).bfloat16(), gen(3)(rows, 2, 64).bfloat16()
+    pos = torch.arange(rows, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    want = gpu_lib.kv_append(cache, k, v, table, ints([rows]), q=q, pos=pos)
+    pages = cache.data.clone()
+    for q_at, o_at in ((slice(0, 4), slice(4, 8)), (slice(0, 8, 2), slice(1, 8, 2))):
+        one = torch.full((rows, 12, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+        one[:, q_at], one[:, 8:10], one[:, 10:] = q, k, v
+        cache.data.zero_()
+        gpu_lib.kv_append(cache, one[:, 8:10], one[:, 10:], table, ints([rows]), q=one[:, q_at], pos=pos, q_out=one[:, o_at])
+        assert torch.equal(one[:, o_at], want) and torch.equal(one[:, q_at], q) and torch.equal(cache.data, pages)

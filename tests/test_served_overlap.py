@@ -70,3 +70,23 @@ def test_kv_gather(pkg, name, kw):
     rc = L.tsp_kv_gather(ctypes.byref(c), 100, vp(kw.get("off", at(5))), 2, vp(kw.get("table", at(6))), 7, vp(kw.get("lengths", at(7))),
                          ctypes.byref(k), ctypes.byref(v), 2, NULL)
     assert rc == 1 and "overlap" in err(pkg), (name, rc)
+
+
+@pytest.mark.parametrize("name,kw", [
+    ("q_out a row into k", dict(qo=at(2, 1024))), ("q_out a head into v", dict(qo=at(3, 128))), ("k a row into q_out", dict(k=at(4, 1024))),
+    ("q_out a row into q", dict(qo=at(1, 1024))), ("q_out a head into q", dict(qo=at(1, 128))), ("q's rows with gaps", dict(qo=at(1, 128), qo_row=1024)),
+    ("the table", dict(table=at(4, 2048))), ("lengths", dict(lengths=at(4))), ("offsets", dict(off=at(4, 102396))), ("positions", dict(pos=at(4, 64))),
+    ("q's factors", dict(gq=at(4, 16))), ("k's factors", dict(gk=at(4, 16))), ("the cache", dict(qo=at(9, 4096))),
+    ("the cache over k", dict(k=at(9, 4096))), ("... v", dict(v=at(9, 4096))), ("... q", dict(q=at(9, 4096), qo=at(9, 4096))),
+    ("... the table", dict(table=at(9, 64))), ("... lengths", dict(lengths=at(9))), ("... offsets", dict(off=at(9))), ("... positions", dict(pos=at(9))),
+    ("... k's factors", dict(gk=at(9))), ("... q's factors", dict(gq=at(9))),
+])
+def test_kv_append(pkg, name, kw):
+    L = pkg.lib()
+    q, k, v = (pkg.Heads(kw.get(x, at(i + 1)), 512, 64) for i, x in enumerate("qkv"))
+    qo = pkg.Heads(kw.get("qo", at(4)), kw.get("qo_row", 512), 64)
+    c = cache_arg(pkg)
+    rc = L.tsp_kv_append(ctypes.byref(c), ctypes.byref(k), ctypes.byref(v), 2, 100, vp(kw.get("off", at(5))), 2, vp(kw.get("table", at(6))), 7,
+                         vp(kw.get("lengths", at(7))), ctypes.byref(q), 8, vp(kw.get("pos", at(8))), 3, (ctypes.c_int * 3)(10, 10, 10), 1e4, 0,
+                         vp(kw.get("gq", at(10))), vp(kw.get("gk", at(11))), 1e-6, ctypes.byref(qo), NULL)
+    assert rc == 1 and ("overlap no other tensor" in err(pkg) or "the cache overlaps" in err(pkg)), (name, rc, err(pkg))

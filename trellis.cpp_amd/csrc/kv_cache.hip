@@ -316,11 +316,6 @@ void held_switch(int format, F&& f) {
     }
 }
 
-// Bytes from a tensor of heads' first to its last.
-size_t heads_span(const tsp_heads& t, int64_t n, int heads, int d, int dtype) {
-    return n <= 0 ? 0 : (size_t)((n - 1) * t.row_stride + (heads - 1) * t.head_stride + d) * dtype_size(dtype);
-}
-
 }  // namespace
 }  // namespace tsp
 
@@ -363,18 +358,22 @@ extern "C" int tsp_kv_append(const tsp_kv_cache* cache, const tsp_heads* k, cons
                     reinterpret_cast<uintptr_t>(c.data) % 16 == 0 && reinterpret_cast<uintptr_t>(d_q_gamma) % 16 == 0 &&
                     reinterpret_cast<uintptr_t>(d_k_gamma) % 16 == 0,
                 TSP_ERR_INVALID, "tsp_kv_append: data must be 16-byte aligned, strides multiples of 8 (a row's up to 2^20)");
-    const size_t cache_bytes = (size_t)(kv_head_bytes(c) * c.heads) * c.pages;
-    TSP_REQUIRE(!overlap(c.data, cache_bytes, k->data, heads_span(*k, n, c.heads, c.d, dtype)) &&
-                    !overlap(c.data, cache_bytes, v->data, heads_span(*v, n, c.heads, c.d, dtype)),
-                TSP_ERR_INVALID, "tsp_kv_append: the cache overlaps k or v");
+    const size_t size = dtype_size(dtype);
+    const Runs held = runs_of(c.data, kv_head_bytes(c) * c.heads * c.pages), none = runs_of(nullptr, 0);
+    const Runs q_runs = hq ? runs_of(*q, n, hq, c.d, size) : none, o_runs = hq ? runs_of(*q_out, n, hq, c.d, size) : none;
+    const Runs read[8] = {runs_of(*k, n, c.heads, c.d, size), runs_of(*v, n, c.heads, c.d, size), runs_of(d_table, 4ll * samples * max_pages),
+                          runs_of(d_lengths, 4ll * samples), runs_of(d_offsets, 4ll * (samples + 1ll)), runs_of(axes ? d_pos : nullptr, 4ll * n * axes),
+                          runs_of(d_q_gamma, 4ll * hq * c.d), runs_of(d_k_gamma, 4ll * c.heads * c.d)};
+    bool over = meet(held, q_runs);
+    for (const Runs& r : read) over |= meet(held, r);
+    TSP_REQUIRE(!over, TSP_ERR_INVALID, "tsp_kv_append: the cache overlaps another tensor of the call");
     if (hq) {
-        const size_t out = heads_span(*q_out, n, hq, c.d, dtype);
         const bool same = q->data == q_out->data && (n <= 1 || q->row_stride == q_out->row_stride) && (hq <= 1 || q->head_stride == q_out->head_stride);
         TSP_REQUIRE(heads_apart(*q_out, n, hq, c.d), TSP_ERR_INVALID, "tsp_kv_append: the output's heads overlap");
-        // (views of one buffer interleave: only equal first bytes are known to be the same values)
-        TSP_REQUIRE((q->data != q_out->data || same) && q_out->data != k->data && q_out->data != v->data && !overlap(c.data, cache_bytes, q_out->data, out) &&
-                        !overlap(c.data, cache_bytes, q->data, heads_span(*q, n, hq, c.d, dtype)),
-                    TSP_ERR_INVALID, "tsp_kv_append: q_out may be q, with the same strides, and no other tensor of the call");
+        // (a row may be shared by groups of lanes: one's q_out over what another has yet to read would be a race)
+        over = meet(o_runs, held) || (!same && meet(o_runs, q_runs));
+        for (const Runs& r : read) over |= meet(o_runs, r);
+        TSP_REQUIRE(!over, TSP_ERR_INVALID, "tsp_kv_append: q_out may be q, with the same strides, and must overlap no other tensor of the call");
     }
     AppendArgs a{};
     a.cache = kv_args(c, d_table, max_pages, d_lengths);
