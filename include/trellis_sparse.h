@@ -544,8 +544,8 @@ int tsp_mx_quantize(const void* d_x, int x_dtype, int64_t n, int c, void* d_code
  * out may be the residual where it is f32, and must not overlap the inputs otherwise. With 16-bit outputs products are
  * added at the matrix cores' 8-bit precision (off by some 1.5e-5 of the result in the 2-norm, a small part of the
  * output's rounding); with f32 outputs in fp32, at half the rate, and there codes times their power have to fit bf16: values
- * below 2^-126 lose bits and powers above 246 may overflow. The result does not depend on what the workspace,
- * 16-byte aligned, of tsp_linear_mx_workspace_bytes bytes held (0, and NULL will do, where it needs none). */
+ * below 2^-126 lose bits and powers above 246 may overflow. No workspace is needed:
+ * tsp_linear_mx_workspace_bytes gives 0 for all sizes, and d_workspace is not used. */
 size_t tsp_linear_mx_workspace_bytes(int64_t n, int ci, int co);
 int tsp_linear_mx(const void* d_x, const uint8_t* d_x_powers, int64_t n, int ci, const void* d_w, const uint8_t* d_w_powers,
                   const float* d_bias, int co, int act, const float* d_residual, void* d_out, int out_dtype,

@@ -1208,15 +1208,15 @@ def mx_quantize(x, out=None, stream=None) -> Mx:
 
 
 def linear_mx_workspace(n: int, ci: int, co: int, device="cuda"):
-    """The uint8 workspace linear_mx needs for these sizes."""
+    """A workspace for linear_mx, which needs none: 16 bytes whatever the sizes."""
     return _torch().empty(max(lib().tsp_linear_mx_workspace_bytes(n, ci, co), 16), dtype=_torch().uint8, device=device)
 
 
 def linear_mx(x, weight, bias=None, act: str = "none", residual=None, out_dtype=None, out=None, workspace=None, stream=None):
     """act(x W^T + bias) + residual on operands in 8 bits: x Mx of [N, Ci], weight Mx of [Co, Ci], bias float32 [Co],
     residual float32 [N, Co] -> [N, Co] in out_dtype (bfloat16 by default; float32 is added in fp32 throughout, at half
-    the rate). out may be given, and be a float32 residual itself; workspace (linear_mx_workspace) may be given to
-    reuse it."""
+    the rate). out may be given, and be a float32 residual itself. workspace is taken as the other calls take theirs; none is
+    needed."""
     torch = _torch()
     n, ci = _check_mx(torch, x, None, None, "x")
     co, _ = _check_mx(torch, weight, None, ci, "weight")
@@ -1237,15 +1237,11 @@ def linear_mx(x, weight, bias=None, act: str = "none", residual=None, out_dtype=
     def call(s, keep):
         rc = None if residual is None else residual.contiguous()
         o = out if out is not None else torch.empty((n, co), dtype=odt, device=dev)
-        ws = workspace
-        if ws is None:
-            need = lib().tsp_linear_mx_workspace_bytes(n, ci, co)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         xa, pa, wa, qa = _aligned(xc), _aligned(xp), _aligned(wc), _aligned(wp)
-        keep(xc, xp, wc, wp, xa, pa, wa, qa, bias, residual, rc, o, ws)
+        keep(xc, xp, wc, wp, xa, pa, wa, qa, bias, residual, rc, o, workspace)
         _check("tsp_linear_mx",
                lib().tsp_linear_mx(xa.data_ptr(), pa.data_ptr(), n, ci, wa.data_ptr(), qa.data_ptr(), _p(bias), co, ac, _p(rc),
-                                   o.data_ptr(), od, _p(ws), 0 if ws is None else ws.numel(), s))
+                                   o.data_ptr(), od, _p(workspace), 0 if workspace is None else workspace.numel(), s))
         return o
     return _launch(dev, stream, call)
 

@@ -465,6 +465,7 @@ extern "C" int tsp_linear_mx(const void* d_x, const uint8_t* d_x_powers, int64_t
                              const float* d_bias, int co, int act, const float* d_residual, void* d_out, int out_dtype, void* d_workspace,
                              size_t workspace_bytes, void* stream) {
     clear_error();
+    (void)d_workspace, (void)workspace_bytes;      // (none is needed)
     TSP_REQUIRE(n >= 0 && n < (1ll << 31) && ci > 0 && ci <= (1 << 20) && co > 0 && co <= (1 << 24), TSP_ERR_INVALID,
                 "tsp_linear_mx: n=%lld ci=%d co=%d out of range", (long long)n, ci, co);
     TSP_REQUIRE(dtype_valid(out_dtype) && (act == 0 || act == 1), TSP_ERR_INVALID, "tsp_linear_mx: bad dtype or act");
@@ -474,9 +475,6 @@ extern "C" int tsp_linear_mx(const void* d_x, const uint8_t* d_x_powers, int64_t
     TSP_REQUIRE(reinterpret_cast<uintptr_t>(d_x) % 16 == 0 && reinterpret_cast<uintptr_t>(d_w) % 16 == 0 &&
                     reinterpret_cast<uintptr_t>(d_x_powers) % 4 == 0 && reinterpret_cast<uintptr_t>(d_w_powers) % 4 == 0,
                 TSP_ERR_INVALID, "tsp_linear_mx: codes must be 16-byte aligned, powers 4-byte aligned");
-    const size_t need = tsp_linear_mx_workspace_bytes(n, ci, co);
-    TSP_REQUIRE(need == 0 || d_workspace, TSP_ERR_INVALID, "tsp_linear_mx: null workspace");
-    TSP_REQUIRE(workspace_bytes >= need, TSP_ERR_WORKSPACE, "tsp_linear_mx: workspace of %zu bytes, needs %zu", workspace_bytes, need);
     const size_t out_bytes = (size_t)n * co * dtype_size(out_dtype), blocks = ci / MX_BLOCK;
     TSP_REQUIRE(!overlap(d_out, out_bytes, d_x, (size_t)n * ci) && !overlap(d_out, out_bytes, d_w, (size_t)co * ci) &&
                     !overlap(d_out, out_bytes, d_x_powers, n * blocks) && !overlap(d_out, out_bytes, d_w_powers, co * blocks) &&
@@ -507,8 +505,10 @@ extern "C" int tsp_linear_mx(const void* d_x, const uint8_t* d_x_powers, int64_t
             };
             auto by_rows = [&](auto wt) {
                 if (n <= 16) few(integral_constant<int, 1>{}, wt);
-                else if (n <= 32) few(integral_constant<int, 2>{}, wt);
-                else if constexpr (EXACT && decltype(wt)::value == 1) few(integral_constant<int, 4>{}, wt);
+                else if constexpr (EXACT || decltype(wt)::value == 1) {
+                    if (n <= 32) few(integral_constant<int, 2>{}, wt);
+                    else if constexpr (EXACT && decltype(wt)::value == 1) few(integral_constant<int, 4>{}, wt);
+                }
             };
             if (wide) by_rows(integral_constant<int, 2>{});
             else by_rows(integral_constant<int, 1>{});
