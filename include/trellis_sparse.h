@@ -526,7 +526,8 @@ int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_heads* v, in
 enum { TSP_MX8 = 3 };
 
 /* h = x + residual, out[i][c] = h[i][c] / sqrt(mean_c(h[i]^2) + eps) * gamma[c], residual_out = h, in fp32 (the norm is
- * of the sum before residual_out rounds it; h^2 summed has to fit fp32). residual and residual_out share a dtype;
+ * of the sum before residual_out rounds it; h^2 summed has to fit fp32, and with eps 0 squares below its normal range, of
+ * |h| below some 1e-19, lose bits). residual and residual_out share a dtype;
  * both may be NULL, and residual_out alone; gamma f32 [c] or NULL. out_dtype TSP_MX8: codes to out, [n][c / 32] power
  * bytes to d_powers (c a multiple of 32); else d_powers is not used. out and residual_out may be x or residual where
  * the dtypes agree and must not overlap them or each other otherwise. c up to 2^20; rows of up to 8,192 channels

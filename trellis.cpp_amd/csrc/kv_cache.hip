@@ -96,8 +96,6 @@ __device__ __forceinline__ double sum_of(double v) {
     for (int o = 1; o < L; o <<= 1) v += __shfl_xor(v, o, 64);
     return v;
 }
-__device__ __forceinline__ float inverse_root(float v) { return __builtin_amdgcn_rsqf(v); }
-__device__ __forceinline__ double inverse_root(double v) { return 1.0 / sqrt(v); }
 
 // v for a rounding to fewer bits that must be v's own: cut to 32 bits, the last of them 1 where that left any out.
 __device__ __forceinline__ float to_odd(float v) { return v; }

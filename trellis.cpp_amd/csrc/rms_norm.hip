@@ -129,7 +129,7 @@ __global__ __launch_bounds__(RN_NT) void k_rms_norm(RmsArgs a) {
             __syncthreads();
             q = (sum_of[turn][0] + sum_of[turn][1]) + (sum_of[turn][2] + sum_of[turn][3]);
         }
-        const float scale = __builtin_amdgcn_rsqf(fmaf(q, a.inv_c, a.eps));
+        const float scale = inverse_root(fmaf(q, a.inv_c, a.eps));
 #pragma unroll
         for (int k = 0; k < CHUNKS; ++k) {
             const int piece = k * NW * 64 + lane;
@@ -175,7 +175,7 @@ __global__ __launch_bounds__(RN_NT) void k_rms_norm_any(RmsArgs a, int x_dtype, 
         __syncthreads();
         q = (sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3]);
         __syncthreads();
-        const float scale = __builtin_amdgcn_rsqf(fmaf(q, a.inv_c, a.eps));
+        const float scale = inverse_root(fmaf(q, a.inv_c, a.eps));
         for (int i = threadIdx.x; i < a.c; i += RN_NT) {
             float h = load1(a.x, x_dtype, base + i);
             if (a.residual) h += load1(a.residual, residual_dtype, base + i);

@@ -152,7 +152,7 @@ __global__ __launch_bounds__(RP_NT, 4) void k_rope(RopeArgs a) {
                         pairs_of<TSP_F32, HALVES>(g, gu, gv);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) q += u[i] * u[i] + v[i] * v[i];
-                        const float scale = __builtin_amdgcn_rsqf(fmaf(group_sum<L>(q), a.inv_d, a.eps));
+                        const float scale = inverse_root(fmaf(group_sum<L>(q), a.inv_d, a.eps));
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             u[i] *= scale * gu[i];
