@@ -51,3 +51,16 @@ def test_append_out_of_one_buffer(gpu_lib, held, rows):
         cache.data.zero_()
         gpu_lib.kv_append(cache, one[:, 8:10], one[:, 10:], table, ints([rows]), q=one[:, q_at], pos=pos, q_out=one[:, o_at])
         assert torch.equal(one[:, o_at], want) and torch.equal(one[:, q_at], q) and torch.equal(cache.data, pages)
+
+
+@pytest.mark.parametrize("rows", [3, 700])
+def test_attention_between_q(gpu_lib, rows):
+    """The packed attention: q, k, v and out beside each other in a row, and out's heads between q's."""
+    import torch
+    q, k, v = gen(1)(rows, 4, 64).bfloat16(), gen(2)(rows, 2, 64).bfloat16(), gen(3)(rows, 2, 64).bfloat16()
+    want = gpu_lib.attention(q, k, v, causal=True)
+    for q_at, o_at in ((slice(0, 4), slice(4, 8)), (slice(0, 8, 2), slice(1, 8, 2))):
+        one = torch.full((rows, 12, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+        one[:, q_at], one[:, 8:10], one[:, 10:] = q, k, v
+        gpu_lib.attention(one[:, q_at], one[:, 8:10], one[:, 10:], causal=True, out=one[:, o_at])
+        assert torch.equal(one[:, o_at], want) and torch.equal(one[:, q_at], q)

@@ -38,6 +38,7 @@
 #include <cmath>
 
 #include "attention_internal.hpp"
+#include "overlap.hpp"
 
 namespace tsp {
 namespace {
@@ -685,6 +686,14 @@ extern "C" int tsp_attention(const tsp_heads* q, const tsp_heads* k, const tsp_h
     TSP_REQUIRE(need == 0 || d_workspace, TSP_ERR_INVALID, "tsp_attention: null workspace");
     TSP_REQUIRE(workspace_bytes >= need, TSP_ERR_WORKSPACE, "tsp_attention: workspace of %zu bytes, needs %zu", workspace_bytes, need);
     TSP_REQUIRE(need == 0 || reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0, TSP_ERR_INVALID, "tsp_attention: workspace not 16-byte aligned");
+    const size_t size = dtype_size(dtype);
+    const Runs o_runs = runs_of(*out, nq, hq, d, size), ws_runs = runs_of(d_workspace, (int64_t)need);
+    const Runs read[5] = {runs_of(*q, nq, hq, d, size), runs_of(kk, nk, hkv, d, size), runs_of(vv, nk, hkv, d, size),
+                          runs_of(d_q_offsets, 4ll * (samples + 1ll)), runs_of(d_k_offsets, 4ll * (samples + 1ll))};
+    bool alias = false, over = meet(ws_runs, o_runs);
+    for (const Runs& r : read) alias |= meet(o_runs, r), over |= meet(ws_runs, r);
+    TSP_REQUIRE(!alias, TSP_ERR_INVALID, "tsp_attention: out must not alias q, k, v or the offsets");
+    TSP_REQUIRE(!over, TSP_ERR_INVALID, "tsp_attention: the workspace overlaps another tensor of the call");
     float* part = need ? static_cast<float*>(d_workspace) : nullptr;
     float2* stat = need ? reinterpret_cast<float2*>(part + (blocks - c.whole) * c.nw * 32 * d) : nullptr;
     // workgroups of a unit's join, by the mean rows of a unit
