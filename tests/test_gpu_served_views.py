@@ -64,3 +64,17 @@ def test_attention_between_q(gpu_lib, rows):
         one[:, q_at], one[:, 8:10], one[:, 10:] = q, k, v
         gpu_lib.attention(one[:, q_at], one[:, 8:10], one[:, 10:], causal=True, out=one[:, o_at])
         assert torch.equal(one[:, o_at], want) and torch.equal(one[:, q_at], q)
+
+
+@pytest.mark.parametrize("rows", [3, 700])
+def test_rope_between_q(gpu_lib, rows):
+    """Rotary positions: q, k and the outputs beside each other in a row, in place, and an output's heads between q's."""
+    import torch
+    q, k = gen(1)(rows, 4, 64).bfloat16(), gen(2)(rows, 2, 64).bfloat16()
+    pos = torch.arange(rows, dtype=torch.int32, device="cuda")[:, None].contiguous()
+    wq, wk = gpu_lib.rope_axes(q, pos, k=k)
+    for q_at, o_at in ((slice(0, 4), slice(4, 8)), (slice(0, 8, 2), slice(1, 8, 2)), (slice(0, 4), slice(0, 4))):
+        one = torch.full((rows, 12, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+        one[:, q_at], one[:, 8:10] = q, k
+        gpu_lib.rope_axes(one[:, q_at], pos, k=one[:, 8:10], q_out=one[:, o_at], k_out=one[:, 10:])
+        assert torch.equal(one[:, o_at], wq) and torch.equal(one[:, 10:], wk) and torch.equal(one[:, 8:10], k)

@@ -38,3 +38,19 @@ def test_attention(pkg, name, kw):
     rc = L.tsp_attention(ctypes.byref(q), ctypes.byref(k), ctypes.byref(v), 2, n, nk, 8, 8, 64, vp(kw.get("qoff", at(5))), vp(kw.get("koff", at(6))),
                          samples, 0.125, 0, ctypes.byref(o), vp(kw.get("ws", at(7))), need, NULL)
     assert rc == 1 and ("out must not alias" in err(pkg) or "workspace overlaps" in err(pkg)), (name, rc, err(pkg))
+
+
+@pytest.mark.parametrize("name,kw", [
+    ("q_out a row into k", dict(qo=at(2, 1024))), ("q_out a row into q", dict(qo=at(1, 1024))), ("q_out a head into q", dict(qo=at(1, 128))),
+    ("q_out over q with gaps", dict(qo=at(1, 128), qo_row=1024)), ("k_out a head into q", dict(ko=at(1, 128))), ("k_out into k", dict(ko=at(2, 2048))),
+    ("k_out into q_out", dict(ko=at(4, 1024))), ("q_out over positions", dict(pos=at(4, 64))), ("k_out over positions", dict(pos=at(5, 64))),
+    ("q's factors", dict(gq=at(4, 16))), ("k's factors", dict(gk=at(5, 16))), ("k's factors in q_out", dict(gk=at(4, 16))),
+    ("wider values over q", dict(qo=at(1, 102272), odt=0)),
+])
+def test_rope(pkg, name, kw):
+    L = pkg.lib()
+    q, k, ko = pkg.Heads(at(1), 512, 64), pkg.Heads(at(2), 512, 64), pkg.Heads(kw.get("ko", at(5)), 512, 64)
+    qo = pkg.Heads(kw.get("qo", at(4)), kw.get("qo_row", 512), 64)
+    rc = L.tsp_rope_axes(ctypes.byref(q), 8, ctypes.byref(k), 8, 2, 100, 64, vp(kw.get("pos", at(6))), 3, (ctypes.c_int * 3)(10, 10, 10), 1e4, 0,
+                         vp(kw.get("gq", at(7))), vp(kw.get("gk", at(8))), 1e-6, ctypes.byref(qo), ctypes.byref(ko), kw.get("odt", 2), NULL)
+    assert rc == 1 and "an output overlaps" in err(pkg), (name, rc, err(pkg))

@@ -13,6 +13,7 @@
 #include <cmath>
 
 #include "common.hpp"
+#include "overlap.hpp"
 #include "packed.hpp"
 
 namespace tsp {
@@ -227,6 +228,14 @@ extern "C" int tsp_rope_axes(const tsp_heads* q, int hq, const tsp_heads* k, int
     TSP_REQUIRE(!other(*q, *q_out, hq) && (hk == 0 || (!other(*k, *k_out, hk) && q->data != k_out->data && k->data != q_out->data &&
                                                        q_out->data != k_out->data)),
                 TSP_ERR_INVALID, "tsp_rope_axes: an output may be its own input, with one dtype and the same strides, and no other");
+    const Runs none = runs_of(nullptr, 0);
+    auto runs = [&](const tsp_heads* t, int heads, int dt) { return heads ? runs_of(*t, n, heads, d, dtype_size(dt)) : none; };
+    const Runs out[2] = {runs(q_out, hq, out_dtype), runs(k_out, hk, out_dtype)}, in[2] = {runs(q, hq, dtype), runs(k, hk, dtype)};
+    const Runs read[3] = {runs_of(d_pos, 4ll * n * axes), runs_of(d_q_gamma, 4ll * hq * d), runs_of(d_k_gamma, 4ll * hk * d)};
+    bool over = meet(out[0], out[1]) || meet(out[0], in[1]) || meet(out[1], in[0]) || (q_out->data != q->data && meet(out[0], in[0])) ||
+                (hk && k_out->data != k->data && meet(out[1], in[1]));
+    for (const Runs& r : read) over |= meet(out[0], r) || meet(out[1], r);
+    TSP_REQUIRE(!over, TSP_ERR_INVALID, "tsp_rope_axes: an output overlaps another tensor of the call (it may be its own input)");
     RopeArgs a{};
     auto side = [](const tsp_heads& x, const tsp_heads& y, const float* g, int heads) {
         return RopeSide{x.data, y.data, x.row_stride, x.head_stride, y.row_stride, y.head_stride, g, heads};
