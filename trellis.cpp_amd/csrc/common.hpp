@@ -113,14 +113,6 @@ constexpr int kTaps = 27;
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// 1 / sqrt(v) of a norm. (The fp32 instruction takes values below the normal range for zero.)
-__device__ __forceinline__ float inverse_root(float v) {
-    const bool small = v < 0x1p-126f;
-    const float r = __builtin_amdgcn_rsqf(small ? v * 0x1p64f : v);
-    return small ? r * 0x1p32f : r;
-}
-__device__ __forceinline__ double inverse_root(double v) { return 1.0 / sqrt(v); }
-
 // Sum over aligned groups of L lanes (16 <= L <= 64); every lane of a group ends with the same
 // value. Within a 16-lane DPP row the moves are lane ^ 1, lane ^ 2, 7 - lane within each 8 and
 // 15 - lane, each pairing lanes whose partial sums cover disjoint lanes; across rows, shuffles.

@@ -19,6 +19,7 @@
 #include <type_traits>
 
 #include "common.hpp"
+#include "inverse_root.hpp"
 #include "kv_cache.hpp"
 #include "mx.hpp"
 #include "overlap.hpp"

@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "common.hpp"
+#include "inverse_root.hpp"
 #include "mx.hpp"
 
 namespace tsp {

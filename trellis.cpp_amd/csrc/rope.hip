@@ -13,6 +13,7 @@
 #include <cmath>
 
 #include "common.hpp"
+#include "inverse_root.hpp"
 #include "overlap.hpp"
 #include "packed.hpp"
 
