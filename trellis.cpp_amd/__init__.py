@@ -1297,7 +1297,8 @@ def kv_append(cache: KVCache, k, v, table, lengths, offsets=None, q=None, pos=No
               interleaved: bool = True, q_gamma=None, k_gamma=None, eps: float = 1e-6, q_out=None, stream=None):
     """New keys and values k, v [N, Hkv, D] of packed samples into the cache, turned to their positions on the way. Of sample
     s with m rows (offsets int32 [samples + 1]; None: one sample), row i becomes key lengths[s] - m + i (lengths int32
-    [samples]: the samples' keys after the call), in page table[s, key // page] of the int32 table [samples, max_pages].
+    [samples]: the samples' keys after the call, counted from as they are), in page table[s, key // page] of the int32 table
+    [samples, max_pages].
     pos int32 [N, axes], pairs, theta, interleaved and the gammas are rope_axes'; pos None: no turning. q [N, Hq, D] is
     normalised and turned in the same launch -> q's result (None without q); rows that are no sample's are left as
     they were in q_out, and in none. Keys whose place is not one of the cache's are not written; two rows must not have
@@ -1386,8 +1387,9 @@ def attention_cached(q, cache: KVCache, table, lengths, offsets=None, causal: bo
     """Softmax attention of q [Nq, Hq, D] (float16 or bfloat16; a 16-bit cache's dtype) to its samples' cached keys ->
     [Nq, Hq, D]. Of sample s with m rows (offsets int32 [samples + 1]; None: one sample), row i sees all lengths[s] keys, or
     with causal those with j <= i + (lengths[s] - m): after kv_append with the same lengths, its own key and those before. A
-    row that sees none gets zeros; rows of out outside every sample are left as they were. Hq is a multiple of the
-    cache's heads, scale defaults to D ** -0.5; workspace (attention_cached_workspace) may be given to reuse it."""
+    row that sees none gets zeros; rows of out outside every sample are left as they were. Lengths are cut to what the table
+    reaches. Hq is a multiple of the cache's heads, scale defaults to D ** -0.5; workspace (attention_cached_workspace) may be
+    given to reuse it. A prompt beside many single tokens is better a call of its own."""
     torch = _torch()
     if q.dim() != 3 or q.shape[2] != cache.d or q.shape[1] % cache.heads:
         raise ValueError(f"q must be [Nq, Hq, {cache.d}] with Hq a multiple of {cache.heads}, got {list(q.shape)}")

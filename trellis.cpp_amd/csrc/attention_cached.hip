@@ -21,10 +21,13 @@
 //
 // What bounds them, in bf16, heads of 128, 4 bits. One row of 16 heads on 2, 40,009 keys: 14.6 us, latency: the lengths, the table, the
 // first tile and the next four one after the other on 500 workgroups, then the join's counts and pieces; 300 keys 9,
-// 200,000 25. 16 samples' tokens, 16 heads on 4, 400,009 keys: 51 us, 47 of them at 4.6 TB/s of cache read, where widening keeps the
-// vector units 40 % busy; in 16 bits 178 (4.6 TB/s). 5,003 rows on 35,001 keys, two samples: 800 us, 1,006 TFLOP/s; the matrix
-// cores are 42 % busy at 2.0 GHz, the vector units, which widen, form exponents and round, 45 %. A causal prompt of 8,000 rows
-// 410; 20,000 rows of 16 heads of 64 on 1,029 keys 181.
+// 200,000 25. 16 samples' tokens, 16 heads on 4, 400,009 keys: 50 us, 46 of them at 4.6 TB/s of cache read, where widening keeps the
+// vector units 40 % busy; in 16 bits 174-178 (4.7 TB/s). 64 samples' tokens of 512 keys, 16 heads on 8: 29; the line's parts are
+// shorter than a unit there, so that nearly all are cut and joined. 5,003 rows on 35,001 keys, two samples: 807-838 us by the box,
+// 960-1,000 TFLOP/s; the matrix cores are 42 % busy at 2.0 GHz, the vector units, which widen, form exponents and round, 45 %. In 16
+// bits 945-960: a tile has one step to land. A causal prompt of 8,000 rows takes 411, 20,000 rows of 16 heads of 64 on 1,029
+// keys 182: 8.0 us for 64 keys (3.7 of products; the exponents of short products) and some 46 whatever the keys, in which units start (the
+// line, Q, a look at the pages, the first tiles) and end with nothing beside them. The packed attention takes 111 for the same.
 // Tried and taken back: eight waves a workgroup of many rows (tiles wait for the slowest wave), four waves a SIMD in either kernel
 // (registers spilled: a kernel with any scratch starts some 7 us later), one LDS array for both buffers (every
 // load waited for), a launch of the join for each place where a cut can be (10 to 30 us).
@@ -1213,7 +1216,9 @@ static_assert(CJ_MAX >= 768 && CM_ROWS < 256, "the join counts every workgroup, 
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // How a call is cut: the rows of a unit, the workgroups. Few rows are those that fit a unit of 32 in the mean (the host
-// does not know the lengths).
+// does not know the lengths). A batch of single tokens and a prompt is cut as its mean asks, and one of the two suffers: 255 tokens on
+// 1,000 keys each with 2,000 rows on 2,000 keys, 8 heads on 8 of 128, take 1,578 us together (the prompt by 16 rows a unit) and 80 and 52
+// as two calls; 16 heads on 4, 205 (the tokens by 128 rows a unit), 47 and 64; 63 tokens on 4,000, 2,000 rows on 20,000: 394, 37 and 337.
 struct CachedCut {
     int rows, groups, least, finer, coarser;
     int64_t units;      // at most

@@ -9,8 +9,8 @@
 // Bound by memory: one read and one write. 60,013 rows, 16 + 16 heads of 64 in f16 on three axes, take 156 us (738 MB, 4.7 TB/s,
 // a large copy's rate); into 4 bits 155, where the 64-bit angles and turns weigh as much. 12,345 rows, 16 + 4 heads of 128 in
 // bf16 with norms, into 4 bits take 38 us (134 MB moved, 3.5 TB/s; the vector units are 55 % busy) and
-// 30.5 into 16; their gather 10 (37 MB). 16 rows take 7.4 us, the latency of offsets, length, table and sine one
-// after the other, and their gather 3.7.
+// 30.5 into 16; their gather 10 (37 MB). 16 rows take 6 us in a graph's replay (7.4 in a trace), the latency of offsets,
+// length, table and sine one after the other, and their gather 2.9 (3.7).
 // A group of lanes takes a row, so that its angles, place and page are formed once for all heads; where rows are few, heads
 // are dealt to as many groups as fill the device. A loop over rows kept the sine's constants in registers for all of it
 // (12,345 rows 46 us, 38 without).

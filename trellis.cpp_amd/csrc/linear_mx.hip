@@ -9,12 +9,14 @@
 //
 // The roles are turned: W is the first operand, so that a lane holds four consecutive outputs of one row.
 //
-// Large products are bound by the matrix cores at the clock that the chip's power leaves, and by how tiles reach them:
-// 8,192^3 takes 471 us in bf16 (2,330 TFLOP/s; the library's 8-bit product 419) and 862 in fp32 (1,280; its bf16 product
-// 782). 35,001 x 4,096 -> 1,024 in fp32 with a residual takes 319 us, the matrix cores 39 % busy at 2.1 GHz: half of a wave's
-// time goes into waiting for loads (tiles of 256 x 256 in cache, no residual: 323 us, 268 without the loop's loads, 229 without
-// its LDS reads), and x, W, residual and outputs, 435 MB, pass the memory-side cache. Few rows are bound by the latency of W:
-// 5 rows, 1,024 -> 4,096, 3.6 us.
+// Figures here and below are of a captured graph's replays on one set of inputs. Large products are bound by the matrix cores at
+// the clock that the chip's power leaves, and by how tiles reach them: 8,192^3 takes 467-471 us in bf16 (2,340 TFLOP/s; the
+// library's 8-bit product 388-419) and 855-862 in fp32 (1,290; its bf16 product 763-782). 35,001 x 4,096 -> 1,024 in fp32 with
+// a residual takes 304 us (321 with input sets that take turns), the matrix cores 39 % busy at 2.1 GHz: half of a wave's time
+// goes into waiting for loads (tiles of 256 x 256 in cache, no residual: 323 us, 268 without the loop's loads, 229 without its
+// LDS reads), and a tile's rows leave at the memory's rate with nothing beside them, since a CU holds one such workgroup. Few rows
+// are bound by the latency of W: 5 rows, 1,024 -> 4,096, 4.0 us. No product is split along its channels: what has few tiles leaves
+// the device part empty (64 rows, 4,096 -> 1,024: 10 us on 16 workgroups; 2,606 x 8,192 -> 27: 19 on 41).
 // Tried and taken back: widening a step's codes while the products of the one before run (fp32; no faster, 40 registers more);
 // loads through registers to LDS (442 us where direct ones into buffers of their own took 295).
 #include <algorithm>
@@ -424,12 +426,14 @@ __global__ __launch_bounds__(LF_NW * 64) void k_linear_mx_few(LinearArgs a) {
 
 // The tile with the least time of its rounds. A step of 128 channels takes a workgroup so many us where the device is full
 // (8,192 rows and outputs of 8,192 channels) and where it has a CU to itself (1,000 rows, 4,096 -> 1,024); a tile's first loads
-// and its rows' way out some more, twice that where a residual is read. us by tiles of 256 x 256, 192 x 256 (fp32 out alone),
-// 128 x 128 and 128 x 64, bf16 out / fp32 out with a residual: 35,001 rows, 4,096 -> 1,024: 220, -, 259, 295 / 390, 327, 336, 390;
-// 1,024 -> 4,096: 187, -, 221, 270 / 445, 413, 408, 470; 12,345 rows, 1,024 -> 1,024: 22, -, 25, 30 / 55, 70, 48, 48; 8,192 rows,
-// 8,192 -> 8,192: 539, -, 806, 1,040 / 960, 1,071, 1,049, 1,322; and with 64 x 64 as the last, 1,000 rows, 4,096 -> 1,024: 56, -, 36,
-// 20, 16 / 113, -, 45, 27, 20. (More waves a tile than its products need hide the loads of what lies in memory: 128 x 128 by
-// eight takes 351 where four take 363. 256 x 128 with two steps on their way: no faster than the best.)
+// and its rows' way out some more, twice that where a residual is read. (The numbers were fitted while bf16's 256 x 256 tile had
+// eight waves, and with input sets that took turns: they say 549 us for 8,192^3 in bf16. For all of what follows they still name
+// the fastest tile.) us by tiles of 256 x 256, 192 x 256 (fp32 out alone), 128 x 128, 128 x 64 and 64 x 64, bf16 out / fp32 out with a
+// residual: 35,001 rows, 4,096 -> 1,024: 185, -, 204, 264, 311 / 368, 304, 323, 377, 430; 1,024 -> 4,096: 172, -, 205, 247, 363 /
+// 427, 406, 403, 451, 540; 12,345 rows, 1,024 -> 1,024: 21, -, 24, 28, 35 / 45, 62, 43, 44, 49; 8,192 rows, 8,192 -> 8,192, no
+// residual: 467, -, 654, 893, 1,157 / 857, 953, 992, 1,240, 1,358; 1,000 rows, 4,096 -> 1,024: 47, -, 36, 20, 12 / 98, 84, 45, 25, 18.
+// (More waves a tile than its products need hide the loads of what lies in memory: 128 x 128 by eight takes 351 where four take
+// 363. 256 x 128 with two steps on their way: no faster than the best.)
 int linear_shape(int64_t n, int ci, int co, bool exact, bool residual) {
     struct Times { double full, alone, rest; };
     struct Shape { int x, w, slots; Times by[2]; };
@@ -530,7 +534,7 @@ extern "C" int tsp_linear_mx(const void* d_x, const uint8_t* d_x_powers, int64_t
     by_form([&](auto exact) {
         auto by_steps = [&](auto any) {
             // (16 waves of 64 x 64 where 16-bit outputs' products are short; eight of 128 x 64 for fp32's, or channels that are
-            // no whole steps, whose powers would take more LDS by 16: 8,192^3 in bf16 539 and 619 us, in fp32 960 and 880)
+            // no whole steps, whose powers would take more LDS by 16: 8,192^3 in bf16 467 and 512 us, in fp32 1,092 and 857)
             constexpr int WX = decltype(exact)::value || decltype(any)::value ? 2 : 4;
             const integral_constant<int, 64> c64;
             const integral_constant<int, 128> c128;

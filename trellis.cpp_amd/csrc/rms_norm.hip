@@ -8,7 +8,10 @@
 // 5 rows take 2.6 us. A wave holds a row of up to 2,048 channels in registers, eight consecutive
 // ones a lane and piece, four waves one of up to 8,192; gamma stays in registers while the wave goes over its
 // rows. Four neighbouring lanes hold a block of 32, so that its largest value is two lane moves. Rows of no whole
-// pieces are held in smaller ones up to 4,096 channels; longer ones are read twice, value by value, by a workgroup each.
+// pieces are held in smaller ones up to 4,096 channels; longer ones, and whole pieces past 8,192 channels, are read twice, value by
+// value, by a workgroup each: 8,000 rows of 8,192 in bf16 with a residual take 98 us (5.3 TB/s), of 12,288 565 and of 16,384 760 (1.4).
+// tsp_mx_quantize: 35,001 rows of 1,024 bf16 17 us and 12,345 of 2,048 12.5 (6.2-6.4 TB/s, in part from the cache), of 35,001 x 4,096
+// 79 (5.5).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
