@@ -1215,21 +1215,26 @@ static_assert(CJ_MAX >= 768 && CM_ROWS < 256, "the join counts every workgroup, 
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// What a call may have: heads; keys a sample; (query, head of the group) pairs; units (cached_cut's numbers fit 64 bits up to it).
+constexpr int kMostHeads = 4096;
+constexpr int64_t kKeysEnd = (1ll << 31) - (1ll << 16), kRowsEnd = (1ll << 31) - 1024, kUnitsEnd = 1ll << 29;
+
 // How a call is cut: the rows of a unit, the workgroups. Few rows are those that fit a unit of 32 in the mean (the host
 // does not know the lengths). A batch of single tokens and a prompt is cut as its mean asks, and one of the two suffers: 255 tokens on
 // 1,000 keys each with 2,000 rows on 2,000 keys, 8 heads on 8 of 128, take 1,578 us together (the prompt by 16 rows a unit) and 80 and 52
 // as two calls; 16 heads on 4, 205 (the tokens by 128 rows a unit), 47 and 64; 63 tokens on 4,000, 2,000 rows on 20,000: 394, 37 and 337.
 struct CachedCut {
     int rows, groups, least, finer, coarser;
-    int64_t units;      // at most
+    int64_t units;      // at most (kUnitsEnd and more: nothing else is known)
     int join;           // groups of lanes a row in the join
     unsigned joins;     // its workgroups
 };
 CachedCut cached_cut(int64_t nq, int samples, int hkv, int share, int64_t keys, int d, bool mx4) {
-    CachedCut c;
+    CachedCut c{};
     const int64_t each = ceil_div(nq, samples) * share;
     c.rows = each <= 16 ? 16 : each <= 32 && mx4 ? 32 : CM_ROWS;      // (two tiles of rows beside 16-bit keys would spill registers)
     c.units = (ceil_div(nq * share, c.rows) + (samples > 1 ? samples : 0)) * hkv;
+    if (c.units >= kUnitsEnd) return c;
     // The line is shorter than 2^30. Weights of many rows' units are in 64ths of a tile where that allows it: a causal
     // prompt's grow by less than a tile from one to the next (8,000 rows to themselves: 678 us in whole tiles).
     const int64_t tiles = ceil_div(keys, c.rows == CM_ROWS ? CM_KEYS : CF_KEYS);
@@ -1259,7 +1264,9 @@ size_t cached_workspace(const CachedCut& c, int d) {
 using namespace tsp;
 
 extern "C" size_t tsp_attention_cached_workspace_bytes(int64_t nq, int samples, int hq, const tsp_kv_cache* cache, int max_pages) {
-    if (!cache || !kv_valid(*cache) || nq <= 0 || nq >= (1ll << 31) || samples <= 0 || hq <= 0 || hq % cache->heads || max_pages <= 0) return 0;
+    if (!cache || !kv_valid(*cache) || nq <= 0 || nq >= (1ll << 31) || samples <= 0 || hq <= 0 || hq > kMostHeads || hq % cache->heads ||
+        max_pages <= 0 || (int64_t)max_pages * cache->page >= kKeysEnd || nq * (hq / cache->heads) >= kRowsEnd)
+        return 0;
     return cached_workspace(cached_cut(nq, samples, cache->heads, hq / cache->heads, (int64_t)max_pages * cache->page, cache->d,
                                        cache->format == TSP_KV_MX4), cache->d);
 }
@@ -1276,9 +1283,9 @@ extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, i
                 "tsp_attention_cached: heads must be f16 or bf16");
     TSP_REQUIRE(c.format == TSP_KV_MX4 || c.format == dtype, TSP_ERR_UNSUPPORTED, "tsp_attention_cached: a 16-bit cache has the heads' dtype");
     TSP_REQUIRE(nq >= 0 && nq < (1ll << 31), TSP_ERR_INVALID, "tsp_attention_cached: nq=%lld out of range", (long long)nq);
-    TSP_REQUIRE(hq > 0 && hq % c.heads == 0 && hq <= 4096, TSP_ERR_INVALID, "tsp_attention_cached: %d heads on %d", hq, c.heads);
+    TSP_REQUIRE(hq > 0 && hq % c.heads == 0 && hq <= kMostHeads, TSP_ERR_INVALID, "tsp_attention_cached: %d heads on %d", hq, c.heads);
     TSP_REQUIRE(samples > 0 && (samples == 1 || d_offsets), TSP_ERR_INVALID, "tsp_attention_cached: samples=%d (without offsets: 1)", samples);
-    TSP_REQUIRE(max_pages > 0 && (int64_t)max_pages * c.page < (1ll << 31) - (1ll << 16), TSP_ERR_INVALID, "tsp_attention_cached: max_pages=%d", max_pages);
+    TSP_REQUIRE(max_pages > 0 && (int64_t)max_pages * c.page < kKeysEnd, TSP_ERR_INVALID, "tsp_attention_cached: max_pages=%d", max_pages);
     TSP_REQUIRE(std::isfinite(scale * kLog2e) && scale > 0.f, TSP_ERR_INVALID, "tsp_attention_cached: scale=%g", scale);
     if (nq == 0) return TSP_OK;
     TSP_REQUIRE(q && out && q->data && out->data && d_table && d_lengths && (c.data || c.pages == 0), TSP_ERR_INVALID,
@@ -1294,9 +1301,9 @@ extern "C" int tsp_attention_cached(const tsp_heads* q, int dtype, int64_t nq, i
     for (const Runs& r : read) alias |= meet(o_runs, r);
     TSP_REQUIRE(!alias, TSP_ERR_INVALID, "tsp_attention_cached: out must not alias q, the cache, table, lengths or offsets");
     const int share = hq / c.heads;
-    TSP_REQUIRE(nq * share < (1ll << 31) - 1024, TSP_ERR_INVALID, "tsp_attention_cached: too many rows");
+    TSP_REQUIRE(nq * share < kRowsEnd, TSP_ERR_INVALID, "tsp_attention_cached: too many rows");
     const CachedCut cut = cached_cut(nq, samples, c.heads, share, (int64_t)max_pages * c.page, c.d, c.format == TSP_KV_MX4);
-    TSP_REQUIRE(cut.units < 1ll << 29, TSP_ERR_INVALID, "tsp_attention_cached: too many rows and heads");
+    TSP_REQUIRE(cut.units < kUnitsEnd, TSP_ERR_INVALID, "tsp_attention_cached: too many rows and heads");
     const size_t need = cached_workspace(cut, c.d);
     TSP_REQUIRE(d_workspace, TSP_ERR_INVALID, "tsp_attention_cached: null workspace");
     TSP_REQUIRE(workspace_bytes >= need, TSP_ERR_WORKSPACE, "tsp_attention_cached: workspace of %zu bytes, needs %zu", workspace_bytes, need);
