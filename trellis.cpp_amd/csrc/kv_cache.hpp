@@ -60,7 +60,7 @@ __device__ __forceinline__ bool row_sample(const int32_t* offsets, int samples, 
     if (offsets) {
         const int lane = threadIdx.x % L, shift = (threadIdx.x & 63) / L * L;
         for (int span = samples; span > 0;) {       // the last sample that begins at row or before it
-            const int step = (span + L - 1) / L, i = lane * step;
+            const int step = (span - 1) / L + 1, i = lane * step;
             const bool before = i < span && offsets[s + i] <= row;
             const uint64_t mask = L == 64 ? ~0ull : (1ull << (L & 63)) - 1;
             const int c = __popcll((__ballot(before) >> shift) & mask);
